@@ -750,6 +750,52 @@ hd_status o1_denoise_step_cfg_sp(const hd_forward_binding *bw, o1_sp_ctx *ctx, o
  * (1 GPU: both branches; 2: CFG pair; 4: pair x SP2; 8: pair x SP4). */
 int o1_parallel_layout(int world, int rank, int *image, int *branch, int *sp_rank, int *sp_size);
 
+/* ------------------------------------------------ rows after a prompt: cached keys and values, added
+ * No counterpart in the reference, which computes every row of a sequence in every forward.  A prompt's text rows are
+ * causal, so their keys and values stay what they are when rows are added: these entry points keep them in a paged cache and
+ * run a decoder block for one new row of each of many sequences.
+ *
+ * A cache: k and v [pages][kv_heads][page_size][128], 16-byte aligned, page_size a multiple of 16.  O1_KV_BF16 stores rows as they are;
+ * O1_KV_FP8 (e4m3) and O1_KV_INT8 as codes of a byte with one fp32 scale for each token and head, k_scale and v_scale
+ * [pages][kv_heads][page_size] (16-byte aligned): scale = max|x| / 448 or / 127, code = x / scale to the nearest, ties to even.  A row with an Inf
+ * or NaN gets a NaN scale and reads as NaN.  A token's slot is page * page_size + its place in the page.
+ * A slot or page outside the cache, or a length outside its table, found on the device: that row is left out and the
+ * device error word gets 70 or 71 (o1_device_error). */
+enum { O1_KV_BF16 = 0, O1_KV_FP8 = 1, O1_KV_INT8 = 2 };
+typedef struct {
+    void *k, *v;
+    float *k_scale, *v_scale;      /* NULL with O1_KV_BF16 */
+    int type, pages, page_size, kv_heads, head_dim /* 128 */;
+} o1_kv_cache;
+/* Rows of keys and values, k / v [rows, ldk / ldv] bf16 with kv head h at columns [128h, 128h+128), into slots[r] (slots
+ * that are all different; a negative slot: the row is left out), quantised on the way. */
+hd_status o1_kv_write(const o1_kv_cache *cache, const void *k, int64_t ldk, const void *v, int64_t ldv,
+                      const int64_t *slots, int rows);
+/* The rows back as bf16(code * scale); zeros for a negative slot. */
+hd_status o1_kv_read(const o1_kv_cache *cache, void *k, int64_t ldk, void *v, int64_t ldv, const int64_t *slots, int rows);
+/* Attention of one new row of each sequence over its lens[b] cached rows: token t of sequence b is in page pages[b * ldp + t /
+ * page_size] (int32, width columns; entries behind a sequence's last page are not read).  q / out [batch, ldq / ldo] bf16, heads of 128
+ * columns, heads a multiple of kv_heads (query head j reads kv head j / (heads / kv_heads)); lse (may be NULL) [batch, heads] fp32:
+ * log of the sum of exponentials, to join the result with that of other keys.  lens[b] == 0: out row 0, lse -inf.
+ * k_new / v_new (both or neither): each sequence's row at position lens[b] - 1, stored into the cache (as by o1_kv_write) and
+ * attended to by the same call.  workspace: o1_kv_attention_workspace_bytes(heads) bytes, 16-byte aligned, zero-filled once before its first use and
+ * left to these calls from then on; calls that may overlap on the GPU each need their own.  The result is the same
+ * bits from call to call. */
+int64_t o1_kv_attention_workspace_bytes(int heads);
+hd_status o1_kv_attention(const o1_kv_cache *cache, const void *q, int64_t ldq, const void *k_new, int64_t ldk,
+                          const void *v_new, int64_t ldv, const int32_t *pages, int64_t ldp, int width, const int32_t *lens,
+                          void *out, int64_t ldo, float *lse, int batch, int heads, float scale, void *workspace,
+                          int64_t workspace_bytes);
+/* The end of one branch and the beginning of the next as one pass over the residual stream:
+ *   y = x + alpha * gate * u,  u = branch, or rmsnorm(branch) * post_w where post_w is given
+ *   h = rmsnorm(y) * pre_w, and * (1 + scale) + shift where they are given
+ * all in fp32, y and h rounded once (h is of the unrounded y).  x, branch, y, h: [rows, ld*] bf16; y may be x or branch; h may be NULL
+ * (pre_w is then not read).  gate (NULL: 1), scale and shift (both or neither): [groups, cols] bf16, row r takes vector
+ * r / (rows / groups), groups a divisor of rows. */
+hd_status o1_residual_norm(const void *x, int64_t ldx, const void *branch, int64_t ldb, const void *post_w, const void *gate,
+                           float alpha, const void *pre_w, const void *scale, const void *shift, int groups, void *y,
+                           int64_t ldy, void *h, int64_t ldh, int rows, int cols, float eps);
+
 #ifdef __cplusplus
 }
 #endif

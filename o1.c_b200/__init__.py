@@ -101,6 +101,12 @@ class WeightStore(C.Structure):
                 ("gemm", c_void_p), ("arena_ptr", c_void_p), ("arena_bytes", c_int64), ("upload_stream", c_void_p)]
 
 
+class KvCacheC(C.Structure):
+    """o1_kv_cache (include/o1_b200.h)."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p)] + [
+        (n, c_int) for n in ("type", "pages", "page_size", "kv_heads", "head_dim")]
+
+
 VISION_DEPTH, VISION_HIDDEN, VISION_HEADS, VISION_HEAD_DIM, VISION_FF = 27, 1152, 16, 72, 4304
 VISION_OUT, VISION_PATCH_DIM, VISION_NUM_POS = 4096, 1536, 2304
 # hd_vision_binding (src/model/vision.h:76-109) is 351 consecutive tensor pointers: patch_proj w, b, pos_embed,
@@ -279,6 +285,14 @@ _sig("o1_denoise_step_cfg_host", c_int, C.POINTER(ForwardBinding), C.POINTER(For
      _P, c_int, _P, c_int, _P, _P, c_int, c_float, c_float, c_float, _P, _P, _P, _P, c_int, c_int,
      c_int, c_int, c_int, c_int)
 
+_sig("o1_kv_write", c_int, C.POINTER(KvCacheC), _P, c_int64, _P, c_int64, _P, c_int)
+_sig("o1_kv_read", c_int, C.POINTER(KvCacheC), _P, c_int64, _P, c_int64, _P, c_int)
+_sig("o1_kv_attention_workspace_bytes", c_int64, c_int)
+_sig("o1_kv_attention", c_int, C.POINTER(KvCacheC), _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, c_int, _P, _P,
+     c_int64, _P, c_int, c_int, c_float, _P, c_int64)
+_sig("o1_residual_norm", c_int, _P, c_int64, _P, c_int64, _P, _P, c_float, _P, _P, _P, c_int, _P, c_int64, _P, c_int64,
+     c_int, c_int, c_float)
+
 EPI_STORE, EPI_BIAS, EPI_RESID, EPI_SWIGLU, EPI_LORA, EPI_BIAS_GELU, EPI_BIAS_RESID, EPI_GATE_RESID = 0, 1, 2, 3, 4, 7, 8, 9
 
 
@@ -322,3 +336,4 @@ def use_torch_stream():
 from .model import (  # noqa: E402
     Weights, GgufWeights, Engine, seq_t2i, seq_ref, dev_sigmas, write_gguf, gguf_tensor_name, weight_seed, SLOT_NAMES, GLOBAL_NAMES, tensor_shape,
 )
+from .kvcache import KvCache, residual_norm  # noqa: E402

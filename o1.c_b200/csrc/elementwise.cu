@@ -148,6 +148,180 @@ bool rmsnorm_mod(const void* x, const void* w, const void* scale, const void* sh
     return true;
 }
 
+// ------------------------------------------------------- residual add between two norms
+// y = x + alpha * gate * u with u = branch or rms(branch) * post; h = rms(y) * pre, then * (1 + scale) + shift.  One pass:
+// a row stays in registers (ITEMS x 8 values to a thread) from its load to both stores, so HBM sees x and branch
+// once and y and h once, 8 bytes a value.  Everything between is fp32 and y and h are rounded once; h is made from the unrounded
+// y, which the separate add and norm cannot do.
+struct ResidualNorm {
+    const uint16_t *x, *branch, *post, *gate, *pre, *scale, *shift;
+    uint16_t *y, *h;
+    int64_t ldx, ldb, ldy, ldh;
+    int rows, cols, per_group;
+    float alpha, eps;
+};
+template <int THREADS>
+__device__ __forceinline__ float block_sum(float v, float* red) {
+    v = warp_sum(v);
+    if (THREADS == 32) return v;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i) s += red[i];
+    return s;
+}
+// 1 / sqrt(mean of squares + eps) of a row, `squares(f)` a thread's part of the sum of its values times f.  Squares of values
+// above 2^57 or so do not fit fp32: such a row (and one with a NaN, to which it makes no difference) is summed again at 2^-80.
+template <int THREADS, class F>
+__device__ __forceinline__ float row_rms_inv(F squares, int cols, float eps, float (*red)[THREADS / 32]) {
+    const float sum = block_sum<THREADS>(squares(1.0f), red[0]);
+    if (sum < INFINITY) return rsqrtf(sum / (float)cols + eps);
+    return rsqrtf(block_sum<THREADS>(squares(8.271806125530277e-25f), red[1]) / (float)cols) * 8.271806125530277e-25f;
+}
+template <int THREADS, int ITEMS, bool POST>
+__global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS)
+residual_norm_vec_kernel(const ResidualNorm a) {
+    grid_dep_launch();
+    grid_dep_wait();
+    __shared__ float red[4][THREADS / 32];
+    const int tid = THREADS == 32 ? threadIdx.x & 31 : threadIdx.x;
+    const int row = THREADS == 32 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+    if (THREADS == 32 && row >= a.rows) return;
+    const int nvec = a.cols >> 3;
+    const size_t vec = (size_t)(row / a.per_group) * nvec;
+    const uint4* x = reinterpret_cast<const uint4*>(a.x + row * a.ldx);
+    const uint4* b = reinterpret_cast<const uint4*>(a.branch + row * a.ldb);
+    uint4 xv[ITEMS], bv[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const int idx = tid + i * THREADS;
+        if (idx < nvec) { xv[i] = x[idx]; bv[i] = b[idx]; }
+    }
+    float inv = 1.f;
+    if (POST) {
+        inv = row_rms_inv<THREADS>([&](float s) {
+            float sq = 0.f;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                if (tid + i * THREADS < nvec) {
+                    float f[8];
+                    unpack8(bv[i], f);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) sq += (f[j] * s) * (f[j] * s);
+                }
+            }
+            return sq;
+        }, a.cols, a.eps, red);
+    }
+    float y[ITEMS][8];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const int idx = tid + i * THREADS;
+        if (idx < nvec) {
+            float f[8], u[8], w[8];
+            unpack8(xv[i], f);
+            unpack8(bv[i], u);
+            if (POST) {
+                unpack8(reinterpret_cast<const uint4*>(a.post)[idx], w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) u[j] = u[j] * inv * w[j];
+            }
+            if (a.gate) {
+                unpack8(reinterpret_cast<const uint4*>(a.gate)[vec + idx], w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) u[j] *= w[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[i][j] = f[j] + a.alpha * u[j];
+            reinterpret_cast<uint4*>(a.y + row * a.ldy)[idx] = pack8(y[i]);
+        }
+    }
+    if (!a.h) return;
+    inv = row_rms_inv<THREADS>([&](float s) {
+        float sq = 0.f;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            if (tid + i * THREADS < nvec) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sq += (y[i][j] * s) * (y[i][j] * s);
+            }
+        }
+        return sq;
+    }, a.cols, a.eps, red + 2);
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const int idx = tid + i * THREADS;
+        if (idx < nvec) {
+            float w[8];
+            unpack8(reinterpret_cast<const uint4*>(a.pre)[idx], w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[i][j] = y[i][j] * inv * w[j];
+            if (a.scale) {
+                float sh[8];
+                unpack8(reinterpret_cast<const uint4*>(a.scale)[vec + idx], w);
+                unpack8(reinterpret_cast<const uint4*>(a.shift)[vec + idx], sh);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[i][j] = y[i][j] * (1.0f + w[j]) + sh[j];
+            }
+            reinterpret_cast<uint4*>(a.h + row * a.ldh)[idx] = pack8(y[i]);
+        }
+    }
+}
+// Any width, pitch and alignment: the row is read again in each step (from L1 and L2).
+__global__ void __launch_bounds__(256) residual_norm_any_kernel(const ResidualNorm a) {
+    grid_dep_launch();
+    grid_dep_wait();
+    __shared__ float red[4][8];
+    const int row = blockIdx.x;
+    const size_t vec = (size_t)(row / a.per_group) * a.cols;
+    const uint16_t *x = a.x + row * a.ldx, *b = a.branch + row * a.ldb;
+    float post = 1.f;
+    if (a.post) {
+        post = row_rms_inv<256>([&](float s) {
+            float sq = 0.f;
+            for (int i = threadIdx.x; i < a.cols; i += 256) { const float f = bf16_to_f32(b[i]) * s; sq += f * f; }
+            return sq;
+        }, a.cols, a.eps, red);
+    }
+    auto value = [&](int i) {
+        float u = bf16_to_f32(b[i]);
+        if (a.post) u = u * post * bf16_to_f32(a.post[i]);
+        if (a.gate) u *= bf16_to_f32(a.gate[vec + i]);
+        return bf16_to_f32(x[i]) + a.alpha * u;
+    };
+    float pre = 1.f;
+    if (a.h) {
+        pre = row_rms_inv<256>([&](float s) {
+            float sq = 0.f;
+            for (int i = threadIdx.x; i < a.cols; i += 256) { const float f = value(i) * s; sq += f * f; }
+            return sq;
+        }, a.cols, a.eps, red + 2);
+    }
+    for (int i = threadIdx.x; i < a.cols; i += 256) {
+        const float f = value(i);
+        if (a.h) {
+            float g = f * pre * bf16_to_f32(a.pre[i]);
+            if (a.scale) g = g * (1.0f + bf16_to_f32(a.scale[vec + i])) + bf16_to_f32(a.shift[vec + i]);
+            a.h[row * a.ldh + i] = f32_to_bf16(g);
+        }
+        a.y[row * a.ldy + i] = f32_to_bf16(f);
+    }
+}
+bool residual_norm(const void* x, int64_t ldx, const void* branch, int64_t ldb, const void* post, const void* gate, float alpha, const void* pre,
+                   const void* scale, const void* shift, int groups, void* y, int64_t ldy, void* h, int64_t ldh, int rows, int cols, float eps,
+                   cudaStream_t st) {
+    const ResidualNorm a = {(const uint16_t*)x, (const uint16_t*)branch, (const uint16_t*)post, (const uint16_t*)gate, (const uint16_t*)pre,
+                            (const uint16_t*)scale, (const uint16_t*)shift, (uint16_t*)y, (uint16_t*)h, ldx, ldb, ldy, ldh, rows, cols, rows / groups, alpha, eps};
+    const uintptr_t all = (uintptr_t)x | (uintptr_t)branch | (uintptr_t)post | (uintptr_t)gate | (uintptr_t)pre | (uintptr_t)scale | (uintptr_t)shift |
+                          (uintptr_t)y | (uintptr_t)h;
+    const bool vec = (all & 15) == 0 && ((ldx | ldb | ldy | (h ? ldh : 0) | cols) & 7) == 0 && cols <= 8192;
+    if (!vec) return launch_ok(launch_chained(residual_norm_any_kernel, dim3(rows), dim3(256), 0, st, 1, rows, a), "residual_norm");
+    auto kern = post ? (cols <= 1024 ? residual_norm_vec_kernel<32, 4, true> : cols <= 4096 ? residual_norm_vec_kernel<128, 4, true> : residual_norm_vec_kernel<256, 4, true>)
+                     : (cols <= 1024 ? residual_norm_vec_kernel<32, 4, false> : cols <= 4096 ? residual_norm_vec_kernel<128, 4, false> : residual_norm_vec_kernel<256, 4, false>);
+    return launch_ok(launch_chained(kern, dim3(cols <= 1024 ? (rows + 3) / 4 : rows), dim3(cols > 4096 ? 256 : 128), 0, st, 1, rows, a), "residual_norm");
+}
+
 // ------------------------------------------------------------------ materialising attention (small / odd shapes)
 // The path of o1.c's hd_attention_eager (src/cuda/attn.cu:22-174) for what the flash kernel does not cover: a head
 // dimension other than 128 or an additive mask that is not prefix-causal.  One block per (head, query row): scores

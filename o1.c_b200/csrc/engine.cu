@@ -978,6 +978,21 @@ int o1_qk_norm_rope(void* x, int ld, int S, int heads, const void* w, const floa
     count();
     return 0;
 }
+hd_status o1_residual_norm(const void* x, int64_t ldx, const void* branch, int64_t ldb, const void* post_w, const void* gate, float alpha,
+                           const void* pre_w, const void* scale, const void* shift, int groups, void* y, int64_t ldy, void* h, int64_t ldh,
+                           int rows, int cols, float eps) {
+    if (rows < 0 || cols <= 0 || groups <= 0 || rows % groups) {
+        set_error("residual_norm: rows %d, cols %d, groups %d (a divisor of rows)", rows, cols, groups);
+        return HD_ERR_UNSUPPORTED;
+    }
+    if (rows == 0) return HD_OK;
+    if (!x || !branch || !y || (h && !pre_w) || (!scale != !shift)) { set_error("residual_norm: null argument"); return HD_ERR_MISSING; }
+    if (ldx < cols || ldb < cols || ldy < cols || (h && ldh < cols)) { set_error("residual_norm: a row pitch is below cols"); return HD_ERR_UNSUPPORTED; }
+    if (!residual_norm(x, ldx, branch, ldb, post_w, gate, alpha, pre_w, scale, shift, groups, y, ldy, h, ldh, rows, cols, eps, g_stream))
+        return HD_ERR_RUNTIME;
+    count();
+    return HD_OK;
+}
 int o1_sched_cfg_flow_step(const void* z, const void* xc, const void* xu, float sigma, float sigma_next,
                            float g, void* z_next, size_t n) {
     if (!sched_cfg_flow_step(z, xc, xu, sigma, sigma_next, g, z_next, n, g_stream)) return 1;

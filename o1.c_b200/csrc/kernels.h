@@ -117,6 +117,10 @@ bool attention_materialised(const void* q, const void* k, const void* v, const v
 bool rmsnorm(const void* x, const void* w, void* y, int rows, int cols, float eps, cudaStream_t st);
 bool rmsnorm_mod(const void* x, const void* w, const void* scale, const void* shift, void* y, int rows, int cols,
                  float eps, cudaStream_t st);
+// y = x + alpha * gate * (branch or rms(branch) * post), h = rms(y) * pre [* (1 + scale) + shift]; see o1_residual_norm
+bool residual_norm(const void* x, int64_t ldx, const void* branch, int64_t ldb, const void* post, const void* gate, float alpha, const void* pre,
+                   const void* scale, const void* shift, int groups, void* y, int64_t ldy, void* h, int64_t ldh, int rows, int cols, float eps,
+                   cudaStream_t st);
 bool silu(const void* x, void* y, size_t n, cudaStream_t st);
 bool swiglu(const void* gate, const void* up, void* y, size_t n, cudaStream_t st);
 bool residual_add(const void* x, const void* a, void* y, size_t n, cudaStream_t st);
