@@ -759,8 +759,8 @@ int o1_parallel_layout(int world, int rank, int *image, int *branch, int *sp_ran
  * O1_KV_FP8 (e4m3) and O1_KV_INT8 as codes of a byte with one fp32 scale for each token and head, k_scale and v_scale
  * [pages][kv_heads][page_size] (16-byte aligned): scale = max|x| / 448 or / 127, code = x / scale to the nearest, ties to even.  A row with an Inf
  * or NaN gets a NaN scale and reads as NaN.  A token's slot is page * page_size + its place in the page.
- * A slot or page outside the cache, or a length outside its table, found on the device: that row is left out and the
- * device error word gets 70 or 71 (o1_device_error). */
+ * A slot or page outside the cache, or a length outside its table, found on the device: nothing outside the cache is read or
+ * written, that row's or sequence's result means nothing, and the device error word gets 70 or 71 (o1_device_error). */
 enum { O1_KV_BF16 = 0, O1_KV_FP8 = 1, O1_KV_INT8 = 2 };
 typedef struct {
     void *k, *v;
