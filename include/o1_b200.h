@@ -778,10 +778,10 @@ hd_status o1_kv_read(const o1_kv_cache *cache, void *k, int64_t ldk, void *v, in
  * columns, heads a multiple of kv_heads (query head j reads kv head j / (heads / kv_heads)); lse (may be NULL) [batch, heads] fp32:
  * log of the sum of exponentials, to join the result with that of other keys.  lens[b] == 0: out row 0, lse -inf.
  * k_new / v_new (both or neither): each sequence's row at position lens[b] - 1, stored into the cache (as by o1_kv_write) and
- * attended to by the same call.  workspace: o1_kv_attention_workspace_bytes(heads) bytes, 16-byte aligned, zero-filled once before its first use and
+ * attended to by the same call.  workspace: o1_kv_attention_workspace_bytes(heads, kv_heads) bytes, 16-byte aligned, zero-filled once before its first use and
  * left to these calls from then on; calls that may overlap on the GPU each need their own.  The result is the same
  * bits from call to call. */
-int64_t o1_kv_attention_workspace_bytes(int heads);
+int64_t o1_kv_attention_workspace_bytes(int heads, int kv_heads);
 hd_status o1_kv_attention(const o1_kv_cache *cache, const void *q, int64_t ldq, const void *k_new, int64_t ldk,
                           const void *v_new, int64_t ldv, const int32_t *pages, int64_t ldp, int width, const int32_t *lens,
                           void *out, int64_t ldo, float *lse, int batch, int heads, float scale, void *workspace,

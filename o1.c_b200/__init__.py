@@ -287,7 +287,7 @@ _sig("o1_denoise_step_cfg_host", c_int, C.POINTER(ForwardBinding), C.POINTER(For
 
 _sig("o1_kv_write", c_int, C.POINTER(KvCacheC), _P, c_int64, _P, c_int64, _P, c_int)
 _sig("o1_kv_read", c_int, C.POINTER(KvCacheC), _P, c_int64, _P, c_int64, _P, c_int)
-_sig("o1_kv_attention_workspace_bytes", c_int64, c_int)
+_sig("o1_kv_attention_workspace_bytes", c_int64, c_int, c_int)
 _sig("o1_kv_attention", c_int, C.POINTER(KvCacheC), _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, c_int, _P, _P,
      c_int64, _P, c_int, c_int, c_float, _P, c_int64)
 _sig("o1_residual_norm", c_int, _P, c_int64, _P, c_int64, _P, _P, c_float, _P, _P, _P, c_int, _P, c_int64, _P, c_int64,

@@ -12,12 +12,7 @@
 
 #include <math.h>
 
-#include <algorithm>
-
 namespace o1 {
-
-using std::max;
-using std::min;
 
 enum { KV_BF16 = O1_KV_BF16, KV_FP8 = O1_KV_FP8, KV_INT8 = O1_KV_INT8 };
 static constexpr int KV_D = 128;
@@ -187,24 +182,30 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
 // HBM bound: every cached value is read once and used by the G = heads / kv_heads queries that share it, 2 G multiply-adds for its one or two bytes,
 // so all that counts is that enough bytes are on their way at all times, on all SMs, whatever the lengths are.
 //
-//  * The work is one stream of chunks (16 tokens, 32 of a quantised cache: 8 KB of keys and values) over sequences, kv heads and length, and every
-//    block takes an equal, contiguous part of it.  Lengths are only on the device: each block sums them up itself.
-//  * A warp takes every KV_WARPS-th chunk of its block's part through a ring of its own (cp.async, KV_STAGES chunks), so its loads run ahead over the ends of
-//    sequences; no barrier but those at such an end.
+//  * The work is one stream of chunks (16 tokens, 32 of a quantised cache: 8 KB of keys and values) over sequences, kv heads and length.  A block is one SM's; its
+//    consumer warps form teams of four, and every team takes an equal, contiguous part of the stream.  How long that is follows from the lengths, which only the
+//    device knows: each block sums them up.
+//  * A fifth warp of each team does its loading: lane w walks the chunks of consumer warp w (every fourth one of the team's part), looks their pages up a round ahead,
+//    and one thread asks for them by TMA, into a ring that each consumer warp has of its own.  So loads run ahead over the ends of sequences, and a consumer
+//    does nothing but arithmetic: with loads of its own (cp.async) a chunk of codes was 920 instructions, of which an SM issued 2.3 a clock.
 //  * Products on the tensor cores (mma.sync: at most 16 rows of queries, tcgen05's tiles have 64 at least).  Scores: A = queries (rows = heads), B = keys.
 //    Their accumulators are, packed in pairs, the B operand of the second product, A = values transposed (rows = columns of a head).  The operands' k and row
-//    indices are permuted so that a thread's part of a key or value row is 16 contiguous bytes; the ring's 16-byte pieces are swizzled to be read without
-//    bank conflicts.
-//  * One pass with a running maximum and sum (in base 2) for each warp; warps join in shared memory, blocks that share a (sequence, kv head) over the
-//    workspace: the last one to finish adds all parts in their order, so the result does not depend on who that is.
+//    indices are permuted so that a thread's part of a key or value row is 16 contiguous bytes, and so that the eight threads which a step of a shared-memory
+//    load serves meet eight different sets of banks in TMA's 128-byte swizzle.
+//  * One pass with a running maximum and sum (in base 2) for each warp.  A team's warps join in shared memory.  Where teams share a (sequence, kv head), each
+//    leaves its maximum, sum and weighted sum, and the last team to come adds them up (of many: the last of each group, then the last group), always in the
+//    order of the teams: the result does not depend on which came when.
 //  * Rounding: scores and sums in fp32.  Probabilities (times v's scale) enter the second product as two parts of bf16, value and rest, 16 bits of significand; codes
 //    of a byte are exact in f16 and bf16.  Keys' codes go through f16, which takes fewer instructions, with queries scaled to f16 by a power of two for each head;
 //    values' codes through bf16, whose range a probability needs.  The result is rounded once.
-static constexpr int KV_WARPS = 4, KV_STAGES = 3;
 static constexpr int KV_STAGE_BYTES = 8192;            // keys and values of a chunk
-static constexpr int KV_BLOCKS_MAX = 320;
-static constexpr int KV_SEQS = 512;                    // sequences of a launch
-static constexpr int KV_PART = 16 * (KV_D + 2);        // floats of a block's part: up to 16 heads, each with its maximum and sum
+static constexpr int KV_SEQS = 256;                    // sequences of a launch
+static constexpr int KV_TEAM = 4;                      // warps
+static constexpr int KV_TEAMS_MAX = 160 * 3;           // what the workspace has room for
+static constexpr int KV_FLAT = 48;                     // so many teams' parts are joined at once, more in groups
+static constexpr int KV_JOIN_BYTES = 8192;             // of a team
+static constexpr int ERR_KV_WAIT = 72;                 // a wait of the attention kernel ran out
+static constexpr float KV_LIFT = 20.0f;                // probabilities are relative to 2^-20 of the largest: those that fp32 has no value for are 2^-146 and less of it
 
 struct KvAttn {
     KvView c;
@@ -213,9 +214,10 @@ struct KvAttn {
     const int32_t *pages, *lens;
     uint16_t* out;
     float* lse;
-    float* parts;          // [KV_BLOCKS_MAX][2][KV_PART]
-    unsigned* arrived;     // [KV_BLOCKS_MAX]
-    int batch, heads, group, chunks_of_heads, width, flags;    // flags: 1 = queries in 16-byte pieces, 2 = results, 4 = new rows
+    unsigned* arrived;     // [2][team][2] teams that have come, of a group whose first part that is; groups that have come
+    float2* stats;         // [team][2][heads of an item] maximum and sum of a team's first and last part of an item
+    float* parts;          // [team][2][heads of an item][128] weighted sum
+    int batch, heads, group, chunks_of_heads, per_item, width, flags;    // flags: 1 = queries in 16-byte pieces, 2 = results, 4 = new rows; 8 = a box of the maps is a whole chunk's rows
     float scale;
     int* err;
 };
@@ -240,7 +242,7 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 }
 __device__ __forceinline__ float exp2_fast(float x) {
     float r;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));      // (results below 2^-126 too: a probability may multiply a large value)
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 // Two values as bf16, and what is left of them as another two.
@@ -281,254 +283,355 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
         asm("add.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0xE480E480u));
     }
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ float lds_f32(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+    return v;
 }
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
     return v;
 }
-// Swizzle of a row's 16-byte pieces: the eight threads that one step of a shared-memory load serves read two rows 2m, 2m+1 (keys) or four rows 2t (values)
-// of the ring, and this puts their pieces into eight different sets of banks.
-__device__ __forceinline__ int kv_swizzle(int row) { return (row & 2) | ((((row >> 2) ^ row) & 1) << 2); }
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void team_sync(int team) { asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(KV_TEAM * 32) : "memory"); }
+// Of eight: 0 2 4 6 1 3 5 7's inverse.  Rows kv_perm(2m) and kv_perm(2m + 1) lie four apart, as the swizzle wants them.
+__device__ __forceinline__ int kv_perm(int i) { return (i >> 1) | (i & 1) << 2; }
 
 template <int TYPE, int HG>
 struct KvKernel {
     static constexpr int KEYS = TYPE == KV_BF16 ? 16 : 32, ROWB = TYPE == KV_BF16 ? 256 : 128, TILES = KEYS / 8;
-    static constexpr int STAGE = KV_STAGE_BYTES + (TYPE == KV_BF16 ? 0 : 2 * KEYS * 4);
-    static constexpr int RING = KV_WARPS * KV_STAGES * STAGE;
-    static constexpr int JOIN = KV_WARPS * 8 * 64 * 4;
-    static constexpr int SMEM = RING + JOIN;
+    static constexpr int TEAMS = HG == 1 ? 3 : 2, WARPS = KV_TEAM * TEAMS, STAGES = HG == 1 ? 2 : 3, THREADS = (WARPS + TEAMS) * 32;      // (as registers and shared memory allow)
+    // shared memory: the rings, their scales, the teams' join buffers, then Shared
+    static constexpr int SCALES = WARPS * STAGES * KV_STAGE_BYTES, JOIN = SCALES + (TYPE == KV_BF16 ? 0 : WARPS * STAGES * 256), SHARED = JOIN + TEAMS * KV_JOIN_BYTES;
+    struct Segment { int b, item, first, begin, end, n; };        // first: the item's first chunk; begin ... end - 1: the team's
+    struct Shared {
+        uint64_t full[WARPS][STAGES], empty[WARPS][STAGES];
+        Segment seg[TEAMS][2], part[TEAMS][2];
+        int prefix[KV_SEQS + 1], len[KV_SEQS], scan[WARPS + TEAMS], parts[TEAMS], last[TEAMS];
+        float m[TEAMS][KV_TEAM][8 * HG], l[TEAMS][KV_TEAM][8 * HG];
+    };
+    static constexpr int SMEM = SHARED + (int)sizeof(Shared);
 };
 
-// Position in the stream: flat index f = (sum of the chunks before sequence b) * items + item * (chunks of b) + chunk.
+// Position in the stream: chunk c of n of item `item` of sequence b.  Items are (kv head, up to 16 of its query heads) pairs.
 struct KvWalk {
-    int b, base, n;
-    __device__ __forceinline__ void load(const int* prefix, int items) { base = prefix[b] * items; n = prefix[b + 1] - prefix[b]; }
-    __device__ __forceinline__ void seek(int f, const int* prefix, int items) {
-        while (f - base >= n * items) { ++b; load(prefix, items); }
+    int b, item, c, n;
+    // the chunk f
+    __device__ __forceinline__ void seek(int f, const int* prefix, int batch, int items) {
+        int lo = 0, hi = batch - 1;       // the last sequence that begins at or before f; it is no empty one: the next one begins behind it
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (prefix[mid] * items <= f) lo = mid; else hi = mid - 1;
+        }
+        b = lo;
+        n = prefix[lo + 1] - prefix[lo];
+        item = (f - prefix[lo] * items) / n;
+        c = f - prefix[lo] * items - item * n;
+    }
+    __device__ __forceinline__ void step(int by, const int* prefix, int items) {       // not past the stream's end
+        c += by;
+        while (c >= n) {
+            c -= n;
+            if (++item < items) continue;
+            item = 0;
+            do { ++b; n = prefix[b + 1] - prefix[b]; } while (n == 0);
+        }
     }
 };
 
+// Sums of v over the block's threads before this one, and over all.  (One barrier before, one behind: `part` is free again.)
+template <int WARPS>
+__device__ __forceinline__ int block_scan(int v, int& all, int* part) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int sum = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += x;
+    }
+    if (lane == 31) part[warp] = sum;
+    __syncthreads();
+    int before = sum - v;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+        before += w < warp ? part[w] : 0;
+        all += part[w];
+    }
+    __syncthreads();
+    return before;
+}
+
+__device__ __forceinline__ void store_row4(uint16_t* dst, const float4& v, float f, bool vec) {
+    const uint2 r = make_uint2(pack_bf16x2(v.x * f, v.y * f), pack_bf16x2(v.z * f, v.w * f));
+    if (vec) { *reinterpret_cast<uint2*>(dst) = r; return; }
+    dst[0] = (uint16_t)r.x; dst[1] = (uint16_t)(r.x >> 16); dst[2] = (uint16_t)r.y; dst[3] = (uint16_t)(r.y >> 16);
+}
+
+// Sums of `count` parts, the first one `first`, the others in slot 0 of every `stride`-th team behind it, a head to a warp: into the result, or
+// (to_out false) into the first one's place.
+__device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, int count, int b, int head0, int heads, bool to_out) {
+    const int lane = threadIdx.x & 31;
+    auto place = [&](int i) { return (int64_t)(i == 0 ? first : (first & ~1) + 2 * stride * i) * a.per_item; };
+    for (int head = (threadIdx.x >> 5) & (KV_TEAM - 1); head < heads; head += KV_TEAM) {
+        float top = -INFINITY;
+        for (int i = lane; i < count; i += 32) top = fmaxf(top, __ldcg(&a.stats[place(i) + head]).x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+        float4 r = make_float4(0, 0, 0, 0);
+        for (int i0 = 0; i0 < count; i0 += 16) {
+            float4 x[16];
+            float2 s = make_float2(-INFINITY, 0.f);
+            if (lane < 16 && i0 + lane < count) s = __ldcg(&a.stats[place(i0 + lane) + head]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (i0 + i < count) x[i] = __ldcg(reinterpret_cast<const float4*>(a.parts + (place(i0 + i) + head) * KV_D) + lane);
+            const float w = exp2_fast(s.x - ref);
+            sum += s.y * w;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float f = __shfl_sync(0xffffffffu, w, i);
+                if (i0 + i < count) { r.x += x[i].x * f; r.y += x[i].y * f; r.z += x[i].z * f; r.w += x[i].w * f; }
+            }
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        sum = __shfl_sync(0xffffffffu, sum, 0);
+        if (to_out) {
+            store_row4(a.out + b * a.ldo + (head0 + head) * KV_D + lane * 4, r, 1.0f / sum, a.flags & 2);
+            if (a.lse && lane == 0) a.lse[(int64_t)b * a.heads + head0 + head] = (top - KV_LIFT + log2f(sum)) * 0.6931471805599453f;
+        } else {
+            reinterpret_cast<float4*>(a.parts + (place(0) + head) * KV_D)[lane] = r;
+            if (lane == 0) a.stats[place(0) + head] = make_float2(top, sum);
+        }
+    }
+}
+
 template <int TYPE, int HG>
-__global__ void __launch_bounds__(KV_WARPS * 32, 2)
-kv_attention_kernel(const KvAttn a) {
+__global__ void __launch_bounds__(KvKernel<TYPE, HG>::THREADS, 1)
+kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ KvAttn a) {
     using K = KvKernel<TYPE, HG>;
-    constexpr int KEYS = K::KEYS, ROWB = K::ROWB, TILES = K::TILES;
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int prefix[KV_SEQS + 1];
-    __shared__ float s_m[KV_WARPS][16], s_l[KV_WARPS][16];
-    __shared__ int s_sum[KV_WARPS];
-    __shared__ bool s_last;
-    const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, tid = threadIdx.x;
+    constexpr int KEYS = K::KEYS, TILES = K::TILES, WARPS = K::WARPS, STAGES = K::STAGES;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    auto& sh = *reinterpret_cast<typename K::Shared*>(smem + K::SHARED);
+    const int warp = warp_index(), lane = threadIdx.x & 31, tid = threadIdx.x;
+    if (tid < WARPS * STAGES) {
+        mbar_init(&sh.full[0][0] + tid, 1);
+        mbar_init(&sh.empty[0][0] + tid, 1);
+        fence_mbar_init();
+    }
+    if (tid < K::TEAMS) sh.parts[tid] = 0;
     grid_dep_launch();
     grid_dep_wait();
 
     // ---- the lengths, as numbers of chunks, summed up
-    const int ps = a.c.page_size, shift = a.c.page_shift;
+    const int ps = a.c.page_size, shift = a.c.page_shift, items = a.c.heads * a.chunks_of_heads;
+    int total;
     {
-        const int per = (a.batch + KV_WARPS * 32 - 1) / (KV_WARPS * 32);
-        int mine = 0;
-        for (int i = 0; i < per; ++i) {
-            const int b = tid * per + i;
-            int n = b < a.batch ? a.lens[b] : 0;
-            if (n < 0 || n > (int64_t)a.width * ps) { atomicExch(a.err, ERR_KV_LENGTH); n = 0; }
-            n = (n + KEYS - 1) / KEYS;
-            if (b < a.batch) prefix[b + 1] = mine + n;
-            mine += n;
-        }
-        int sum = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += v;
-        }
-        if (lane == 31) s_sum[warp] = sum;
-        if (tid == 0) prefix[0] = 0;
-        __syncthreads();
-        int before = sum - mine;
-#pragma unroll
-        for (int w = 0; w < KV_WARPS; ++w) before += w < warp ? s_sum[w] : 0;
-        for (int i = 0; i < per; ++i)
-            if (tid * per + i < a.batch) prefix[tid * per + i + 1] += before;
+        static_assert(KV_SEQS <= K::THREADS, "a sequence to a thread");
+        int len = tid < a.batch ? a.lens[tid] : 0;
+        if (len < 0 || len > (int64_t)a.width * ps) { atomicExch(a.err, ERR_KV_LENGTH); len = 0; }
+        const int before = block_scan<WARPS + K::TEAMS>((len + KEYS - 1) / KEYS, total, sh.scan);
+        if (tid < a.batch) { sh.prefix[tid] = before; sh.len[tid] = len; }
+        if (tid == 0) sh.prefix[a.batch] = total;
+        total *= items;
         __syncthreads();
     }
-    // ---- sequences without rows
-    for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
-        if (prefix[b + 1] != prefix[b]) continue;
-        for (int i = tid; i < a.heads * KV_D; i += KV_WARPS * 32) a.out[b * a.ldo + i] = 0;
-        if (a.lse) for (int i = tid; i < a.heads; i += KV_WARPS * 32) a.lse[(int64_t)b * a.heads + i] = -INFINITY;
-    }
+    // ---- a team's part of the stream
+    const int teams = min((int)gridDim.x * K::TEAMS, (total + KV_TEAM - 1) / KV_TEAM);
+    auto begin_of = [&](int id) { return (int)((int64_t)total * id / teams); };
 
-    const int items = a.c.heads * a.chunks_of_heads;
-    const int total = prefix[a.batch] * items;
-    const int blocks = min((int)gridDim.x, (total + KV_WARPS - 1) / KV_WARPS);
-    if ((int)blockIdx.x >= blocks) return;
-    const int c0 = (int)((int64_t)total * blockIdx.x / blocks), c1 = (int)((int64_t)total * (blockIdx.x + 1) / blocks);
-
-    KvWalk ld, cur;
-    {
-        int lo = 0, hi = a.batch - 1;       // the last sequence that begins at or before c0 and has chunks
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (prefix[mid] * items <= c0) lo = mid; else hi = mid - 1;
-        }
-        cur.b = lo;
-        cur.load(prefix, items);
-        cur.seek(c0, prefix, items);
-        ld = cur;
-    }
-    const uint32_t ring = smem_u32(smem) + warp * KV_STAGES * K::STAGE;
-    float* join = reinterpret_cast<float*>(smem + K::RING);
-
-    // ---- the load side: what the next chunk is, its pages asked for one chunk ahead
-    int lf = c0 + warp, l_off[2], l_page[2], l_head = 0, l_slot = 0;
-    bool l_two = false;
-    auto look = [&]() {
-        if (lf >= c1) return;
-        ld.seek(lf, prefix, items);
-        const int rel = lf - ld.base, item = rel / ld.n, tok = (rel - item * ld.n) * KEYS;
-        l_head = item / a.chunks_of_heads;
-        const int32_t* row = a.pages + ld.b * a.ldp;
-        const int p0 = shift >= 0 ? tok >> shift : tok / ps;
-        l_off[0] = tok - p0 * ps;
-        l_page[0] = row[p0];
-        if (KEYS == 32) {
-            l_two = tok + 16 < a.lens[ld.b];
-            const int p1 = shift >= 0 ? (tok + 16) >> shift : (tok + 16) / ps;
-            l_off[1] = tok + 16 - p1 * ps;
-            l_page[1] = l_two ? row[p1] : 0;
-        }
-    };
-    auto issue = [&]() {
-        if (lf < c1) {
-            const uint32_t dst = ring + l_slot * K::STAGE;
+    if (warp >= WARPS) {
+        // ---- the team's loading warp
+        const int team = warp - WARPS, id = team * gridDim.x + blockIdx.x;
+        if (id >= teams) return;
+        const int c1 = lane < KV_TEAM ? begin_of(id + 1) : 0;
+        int f = lane < KV_TEAM ? begin_of(id) + lane : 0, place[2] = {-1, -1};
+        KvWalk at = {};
+        auto look = [&]() {        // the chunk's rows of the cache, 16 at a time; -1: none
+            const int tok = at.c * KEYS, len = sh.len[at.b], head = a.chunks_of_heads == 1 ? at.item : at.item / a.chunks_of_heads;
 #pragma unroll
             for (int h = 0; h < KEYS / 16; ++h) {
-                if (h == 1 && !l_two) break;
-                int page = l_page[h];
-                if ((unsigned)page >= (unsigned)a.c.pages) { if (lane == 0) atomicExch(a.err, ERR_KV_PLACE); page = 0; }
-                const int64_t at = ((int64_t)page * a.c.heads + l_head) * ps + l_off[h];
-                constexpr int LANES = ROWB / 16, ROWS = 32 / LANES;      // lanes of a row, rows of a step
+                const int token = tok + 16 * h, p = shift >= 0 ? token >> shift : token / ps;
+                place[h] = -1;
+                if (token >= len) continue;
+                const int page = a.pages[at.b * a.ldp + p];
+                place[h] = 0;
+                if ((unsigned)page >= (unsigned)a.c.pages) atomicExch(a.err, ERR_KV_PLACE);
+                else place[h] = (page * a.c.heads + head) * ps + token - p * ps;
+            }
+        };
+        if (f < c1) { at.seek(f, sh.prefix, a.batch, items); look(); }
+        bool ok = true;
+        for (int round = 0; ok; ++round) {
+            unsigned left = __ballot_sync(0xffffffffu, f < c1);
+            if (!left) break;
+            const int now[2] = {place[0], place[1]}, slot = round % STAGES;
+            f += KV_TEAM;
+            if (f < c1) { at.step(KV_TEAM, sh.prefix, items); look(); }
+            for (; left && ok; left &= left - 1) {
+                const int mate = __ffs(left) - 1, w = team * KV_TEAM + mate, r0 = __shfl_sync(0xffffffffu, now[0], mate), r1 = KEYS == 32 ? __shfl_sync(0xffffffffu, now[1], mate) : -1;
+                uint64_t* const full = &sh.full[w][slot];
+                if (elect_one()) {
+                    ok = mbar_wait(&sh.empty[w][slot], ((round / STAGES) & 1) ^ 1);
+                    if (!ok) atomicExch(a.err, ERR_KV_WAIT);
+                    else {
+                        uint8_t* const dst = smem + (w * STAGES + slot) * KV_STAGE_BYTES;
+                        const uint32_t scales = smem_u32(smem) + K::SCALES + (w * STAGES + slot) * 256;
+                        if (TYPE == KV_BF16) {
+                            mbar_expect_tx(full, 8192);
+                            tma_load_2d(dst, &k_map, full, 0, r0);
+                            tma_load_2d(dst + 2048, &k_map, full, 64, r0);
+                            tma_load_2d(dst + 4096, &v_map, full, 0, r0);
+                            tma_load_2d(dst + 6144, &v_map, full, 64, r0);
+                        } else if (a.flags & 8) {
+                            mbar_expect_tx(full, 8192 + 256);
+                            tma_load_2d(dst, &k_map, full, 0, r0);
+                            tma_load_2d(dst + 4096, &v_map, full, 0, r0);
+                            bulk_load(scales, a.c.ks + r0, 128, full);
+                            bulk_load(scales + 128, a.c.vs + r0, 128, full);
+                        } else {
+                            mbar_expect_tx(full, r1 >= 0 ? 8192 + 256 : 4096 + 128);
 #pragma unroll
-                for (int i = 0; i < 16 / ROWS; ++i) {
-                    const int r = h * 16 + i * ROWS + lane / LANES, piece = lane % LANES;
-                    const uint32_t to = r * ROWB + ((piece ^ kv_swizzle(r)) << 4);
-                    const int64_t from = at * ROWB + i * 512 + lane * 16;
-                    cp_async16(dst + to, a.c.k + from);
-                    cp_async16(dst + 4096 + to, a.c.v + from);
+                            for (int h = 0; h < 2; ++h) {
+                                const int r = h ? r1 : r0;
+                                if (r < 0) break;
+                                tma_load_2d(dst + h * 2048, &k_map, full, 0, r);
+                                tma_load_2d(dst + 4096 + h * 2048, &v_map, full, 0, r);
+                                bulk_load(scales + h * 64, a.c.ks + r, 64, full);
+                                bulk_load(scales + 128 + h * 64, a.c.vs + r, 64, full);
+                            }
+                        }
+                    }
                 }
-                if (TYPE != KV_BF16 && lane < 8)
-                    cp_async16(dst + 8192 + (lane & 4) * 32 + h * 64 + (lane & 3) * 16, (lane < 4 ? a.c.ks : a.c.vs) + at + (lane & 3) * 4);
+                ok = __all_sync(0xffffffffu, ok);
             }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        l_slot = l_slot + 1 == KV_STAGES ? 0 : l_slot + 1;
-        lf += KV_WARPS;
-        look();
+        return;
+    }
+
+    const int team = warp / KV_TEAM, mate = warp % KV_TEAM, g = lane >> 2, t = lane & 3, gp = kv_perm(g), id = team * gridDim.x + blockIdx.x;
+    // ---- sequences without rows
+    for (int b = id; b < a.batch; b += gridDim.x * K::TEAMS) {
+        if (sh.len[b] > 0) continue;
+        for (int i = mate * 32 + lane; i < a.heads * KV_D; i += KV_TEAM * 32) a.out[b * a.ldo + i] = 0;
+        if (a.lse) for (int i = mate * 32 + lane; i < a.heads; i += KV_TEAM * 32) a.lse[(int64_t)b * a.heads + i] = -INFINITY;
+    }
+    if (id >= teams) return;
+    const int c0 = begin_of(id), c1 = begin_of(id + 1);
+
+    auto head_of = [&](int item) {         // the first query head of an item
+        const int kvh = a.chunks_of_heads == 1 ? item : item / a.chunks_of_heads;
+        return kvh * a.group + (item - kvh * a.chunks_of_heads) * (8 * HG);
     };
-    look();
-    for (int i = 0; i < KV_STAGES; ++i) issue();
-
-    // ---- segments: what the block has of one (sequence, kv head, up to 16 query heads)
-    int f = c0 + warp, slot = 0;
-    for (int seg = c0; seg < c1;) {
-        cur.seek(seg, prefix, items);
-        const int item = (seg - cur.base) / cur.n, first = cur.base + item * cur.n, end = min(c1, first + cur.n);
-        const int kvh = item / a.chunks_of_heads, head0 = kvh * a.group + (item - kvh * a.chunks_of_heads) * (8 * HG);
-        const int heads = min(8 * HG, (kvh + 1) * a.group - head0), b = cur.b, len = a.lens[b];
-
-        // queries: rows g (and g + 8) of the A operand; the 16-byte pieces 4i + t of a key row are this thread's
-        uint32_t qa[HG][16];
-        float z_scale[HG];
+    auto heads_of = [&](int item) { return a.chunks_of_heads == 1 ? a.group : min(8 * HG, a.group - item % a.chunks_of_heads * (8 * HG)); };
+    // queries: rows g (and g + 8) of the A operand; the 16-byte pieces 4i + t of a key row are this thread's
+    uint32_t qa[HG][16];
+    auto ask_queries = [&](int b, int item) {
+        const int head0 = head_of(item), heads = heads_of(item);
 #pragma unroll
         for (int h = 0; h < HG; ++h) {
             const bool on = g + 8 * h < heads;
             const uint16_t* src = a.q + b * a.ldq + (head0 + g + 8 * h) * KV_D;
-            uint4 v[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int at = TYPE == KV_BF16 ? (4 * i + t) * 8 : (4 * (i >> 1) + t) * 16 + (i & 1) * 8;
-                v[i] = !on ? make_uint4(0, 0, 0, 0) : (a.flags & 1) ? load8<true>(src + at) : load8<false>(src + at);
+                const uint4 v = !on ? make_uint4(0, 0, 0, 0) : (a.flags & 1) ? load8<true>(src + at) : load8<false>(src + at);
+                qa[h][4 * i] = v.x; qa[h][4 * i + 1] = v.y; qa[h][4 * i + 2] = v.z; qa[h][4 * i + 3] = v.w;
             }
-            z_scale[h] = a.scale * 1.4426950408889634f;
-            if (TYPE == KV_BF16) {
+        }
+    };
+    // segments: what the team has of one item; the first warp writes the next one down while all work on this one
+    auto describe = [&](int f, typename K::Segment& to) {
+        KvWalk at;
+        at.seek(f, sh.prefix, a.batch, items);
+        if (lane == 0) to = {at.b, at.item, f - at.c, f, min(c1, f - at.c + at.n), at.n};
+    };
+    if (mate == 0) describe(c0, sh.seg[team][0]);
+    team_sync(team);
+    ask_queries(sh.seg[team][0].b, sh.seg[team][0].item);
+    float* const buf = reinterpret_cast<float*>(smem + K::JOIN + team * KV_JOIN_BYTES);
+    int f = c0 + mate, slot = 0, parity = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (int k = 0;; ++k) {
+        const typename K::Segment seg = sh.seg[team][k & 1];
+        if (mate == 0 && seg.end < c1) describe(seg.end, sh.seg[team][(k + 1) & 1]);
+        float z_scale[HG], acc[HG][8][4], m[HG], l[HG];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { qa[h][4 * i] = v[i].x; qa[h][4 * i + 1] = v[i].y; qa[h][4 * i + 2] = v[i].z; qa[h][4 * i + 3] = v[i].w; }
-            } else {
+        for (int h = 0; h < HG; ++h) {
+            z_scale[h] = a.scale * 1.4426950408889634f;
+            if (TYPE != KV_BF16) {
                 uint32_t top = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) top = max(top, max(w[j] & 0x7FFFu, (w[j] >> 16) & 0x7FFFu));
-                }
+                for (int i = 0; i < 16; ++i) top = max(top, max(qa[h][i] & 0x7FFFu, (qa[h][i] >> 16) & 0x7FFFu));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const uint32_t e = min(max(top >> 7, 1u), 253u);         // the largest one's exponent
                 const float down = __uint_as_float((254u - e) << 23);
                 z_scale[h] *= __uint_as_float(e << 23);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) qa[h][4 * i + j] = pack_f16x2(bf16lo(w[j]) * down, bf16hi(w[j]) * down);
-                }
+                for (int i = 0; i < 16; ++i) qa[h][i] = pack_f16x2(bf16lo(qa[h][i]) * down, bf16hi(qa[h][i]) * down);
             }
-        }
-        float acc[HG][8][4], m[HG], l[HG];
-#pragma unroll
-        for (int h = 0; h < HG; ++h) {
             m[h] = -INFINITY;
             l[h] = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) acc[h][j][0] = acc[h][j][1] = acc[h][j][2] = acc[h][j][3] = 0.f;
         }
 
-        for (; f < end; f += KV_WARPS) {
-            const int valid = len - (f - first) * KEYS;        // rows of the chunk that the sequence has, >= 1
-            const uint32_t st = ring + slot * K::STAGE;
-            uint4 fresh = make_uint4(0, 0, 0, 0);
+        int valid = sh.len[seg.b] - (f - seg.first) * KEYS;       // rows that the sequence has from the warp's chunk on
+#pragma unroll 1
+        for (; f < seg.end; f += KV_TEAM, valid -= KV_TEAM * KEYS) {
+            const uint32_t st = smem_u32(smem) + (warp * STAGES + slot) * KV_STAGE_BYTES, scales = smem_u32(smem) + K::SCALES + (warp * STAGES + slot) * 256;
             const bool append = a.kn && valid <= KEYS;
+            uint4 fresh = make_uint4(0, 0, 0, 0);
+            int page = -1, last = 0, kvh = 0;
             if (append) {
-                const uint16_t* src = (lane < 16 ? a.kn + b * a.ldk : a.vn + b * a.ldv) + kvh * KV_D + (lane & 15) * 8;
+                kvh = a.chunks_of_heads == 1 ? seg.item : seg.item / a.chunks_of_heads;
+                last = sh.len[seg.b] - 1;
+                const uint16_t* src = (lane < 16 ? a.kn + seg.b * a.ldk : a.vn + seg.b * a.ldv) + kvh * KV_D + (lane & 15) * 8;
                 fresh = (a.flags & 4) ? load8<true>(src) : load8<false>(src);
+                page = a.pages[seg.b * a.ldp + (shift >= 0 ? last >> shift : last / ps)];
             }
-            asm volatile("cp.async.wait_group %0;" ::"n"(KV_STAGES - 1) : "memory");
+            if (ok && !mbar_wait(&sh.full[warp][slot], parity)) { ok = false; atomicExch(a.err, ERR_KV_WAIT); }
             __syncwarp();
             if (append) {     // the sequence's last row is the new one: into the ring, and into the cache
-                const int r = valid - 1, tok = len - 1, pi = tok / ps;
-                const int page = a.pages[b * a.ldp + pi];
-                const bool store = item == kvh * a.chunks_of_heads && (unsigned)page < (unsigned)a.c.pages;
-                const int64_t at = ((int64_t)page * a.c.heads + kvh) * ps + tok - pi * ps;
-                const uint32_t dst = st + (lane < 16 ? 0 : 4096) + r * ROWB;
+                const int r = valid - 1, part = lane & 15;
+                const bool store = (a.chunks_of_heads == 1 || seg.item % a.chunks_of_heads == 0) && (unsigned)page < (unsigned)a.c.pages;
+                const int64_t at = ((int64_t)page * a.c.heads + kvh) * ps + (shift >= 0 ? last & (ps - 1) : last % ps);
+                const uint32_t dst = st + (lane < 16 ? 0 : 4096) + r * 128;
                 uint8_t* const base = lane < 16 ? a.c.k : a.c.v;
                 if (TYPE == KV_BF16) {
-                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (((lane & 15) ^ kv_swizzle(r)) << 4)), "r"(fresh.x), "r"(fresh.y), "r"(fresh.z), "r"(fresh.w) : "memory");
-                    if (store) reinterpret_cast<uint4*>(base)[at * 16 + (lane & 15)] = fresh;
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (part >> 3) * 2048 + (((part & 7) ^ (r & 7)) << 4)), "r"(fresh.x), "r"(fresh.y), "r"(fresh.z), "r"(fresh.w) : "memory");
+                    if (store) reinterpret_cast<uint4*>(base)[at * 16 + part] = fresh;
                 } else {
                     float sc;
                     const uint2 codes = quantise8(fresh, TYPE, sc);
-                    asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(dst + ((((lane & 15) >> 1) ^ kv_swizzle(r)) << 4) + (lane & 1) * 8), "r"(codes.x), "r"(codes.y) : "memory");
-                    if ((lane & 15) == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(st + 8192 + (lane >> 4) * 128 + r * 4), "f"(sc) : "memory");
+                    asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(dst + (((part >> 1) ^ (r & 7)) << 4) + (part & 1) * 8), "r"(codes.x), "r"(codes.y) : "memory");
+                    if (part == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(scales + (lane >> 4) * 128 + r * 4), "f"(sc) : "memory");
                     if (store) {
-                        reinterpret_cast<uint2*>(base)[at * 16 + (lane & 15)] = codes;
-                        if ((lane & 15) == 0) (lane < 16 ? a.c.ks : a.c.vs)[at] = sc;
+                        reinterpret_cast<uint2*>(base)[at * 16 + part] = codes;
+                        if (part == 0) (lane < 16 ? a.c.ks : a.c.vs)[at] = sc;
                     }
                 }
+                fence_proxy_async_smem();
                 __syncwarp();
             }
 
-            // scores of 8 keys a tile
+            // scores of 8 keys a tile; a tile's column n is its key kv_perm(n), so keys t and t + 4 are this thread's
             float s[TILES][4];
 #pragma unroll
             for (int n = 0; n < TILES; ++n) {
                 s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-                const uint32_t row = st + (n * 8 + g) * ROWB;
+                const uint32_t row = st + n * 1024 + gp * 128;
 #pragma unroll
-                for (int i = 0; i < ROWB / 64; ++i) {
-                    const uint4 k = lds128(row + (((4 * i + t) ^ kv_swizzle(g)) << 4));
+                for (int i = 0; i < (TYPE == KV_BF16 ? 4 : 2); ++i) {
+                    const uint4 k = lds128(row + (i >> 1) * 2048 + (((4 * (i & 1) + t) ^ gp) << 4));
                     const uint32_t w[4] = {k.x, k.y, k.z, k.w};
                     if (TYPE == KV_BF16) {
 #pragma unroll
@@ -544,22 +647,34 @@ kv_attention_kernel(const KvAttn a) {
                     }
                 }
             }
-            // this thread's keys: 8n + 2t and the next
             float vs[TILES][2];
             if (TYPE != KV_BF16) {
 #pragma unroll
                 for (int n = 0; n < TILES; ++n) {
-                    float2 ks, v2;
-                    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(ks.x), "=f"(ks.y) : "r"(st + 8192 + (8 * n + 2 * t) * 4));
-                    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v2.x), "=f"(v2.y) : "r"(st + 8192 + 128 + (8 * n + 2 * t) * 4));
-                    s[n][0] *= ks.x; s[n][1] *= ks.y;
-                    if (HG == 2) { s[n][2] *= ks.x; s[n][3] *= ks.y; }
-                    vs[n][0] = 8 * n + 2 * t < valid ? v2.x : 0.f;
-                    vs[n][1] = 8 * n + 2 * t + 1 < valid ? v2.y : 0.f;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float ks = lds_f32(scales + (8 * n + 4 * j + t) * 4);
+                        vs[n][j] = lds_f32(scales + 128 + (8 * n + 4 * j + t) * 4);
+#pragma unroll
+                        for (int h = 0; h < HG; ++h) s[n][2 * h + j] *= ks;
+                    }
+                }
+            }
+            if (valid < KEYS) {        // what the memory behind a sequence holds, NaN too, takes no part
+#pragma unroll
+                for (int n = 0; n < TILES; ++n) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        if (8 * n + 4 * j + t < valid) continue;
+                        vs[n][j] = 0.f;
+#pragma unroll
+                        for (int h = 0; h < HG; ++h) s[n][2 * h + j] = -INFINITY;
+                    }
                 }
             }
             // running maximum and sum; a tile's accumulators become the probabilities
             float alpha[HG];
+            bool moved = false;
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
                 float top = -INFINITY;
@@ -567,16 +682,15 @@ kv_attention_kernel(const KvAttn a) {
                 for (int n = 0; n < TILES; ++n) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float z = s[n][2 * h + j] * z_scale[h];
-                        if (8 * n + 2 * t + j >= valid) z = -INFINITY;
-                        s[n][2 * h + j] = z;
-                        top = fmaxf(top, z);
+                        s[n][2 * h + j] *= z_scale[h];
+                        top = fmaxf(top, s[n][2 * h + j]);
                     }
                 }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float m_new = fmaxf(m[h], top), ref = m_new == -INFINITY ? 0.f : m_new;
-                alpha[h] = exp2_fast(m[h] - ref);
+                const float m_new = fmaxf(m[h], top), ref = (m_new == -INFINITY ? 0.f : m_new) - KV_LIFT;
+                alpha[h] = exp2_fast(m[h] - KV_LIFT - ref);
+                moved = moved || alpha[h] != 1.f;
                 m[h] = m_new;
                 float sum = 0.f;
 #pragma unroll
@@ -590,9 +704,6 @@ kv_attention_kernel(const KvAttn a) {
                     for (int n = 0; n < TILES; ++n) { s[n][2 * h] *= vs[n][0]; s[n][2 * h + 1] *= vs[n][1]; }
                 }
             }
-            bool moved = false;
-#pragma unroll
-            for (int h = 0; h < HG; ++h) moved = moved || alpha[h] != 1.f;
             if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
                 for (int h = 0; h < HG; ++h) {
@@ -601,7 +712,7 @@ kv_attention_kernel(const KvAttn a) {
                     for (int j = 0; j < 8; ++j) { acc[h][j][0] *= a0; acc[h][j][1] *= a1; acc[h][j][2] *= a0; acc[h][j][3] *= a1; }
                 }
             }
-            // out^T += V^T P^T, 16 keys a step
+            // out^T += V^T P^T, 16 keys a step: this thread's rows are keys t, t + 4, t + 8, t + 12
 #pragma unroll
             for (int u = 0; u < KEYS / 16; ++u) {
                 uint32_t p_hi[HG][2], p_lo[HG][2];
@@ -610,23 +721,27 @@ kv_attention_kernel(const KvAttn a) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) two_parts(s[2 * u + j][2 * h], s[2 * u + j][2 * h + 1], p_hi[h][j], p_lo[h][j]);
                 }
-                const uint32_t base = st + 4096 + u * 16 * ROWB;
-                // rows of this thread: 2t, 2t+1, 2t+8, 2t+9 of the 16; masked rows as zeros, whatever the memory behind a sequence holds
-                uint4 v[4][ROWB / 128];
+                constexpr int PIECES = TYPE == KV_BF16 ? 2 : 1;
+                uint4 v[4][PIECES];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int key = 2 * t + (r & 1) + (r >> 1) * 8;
 #pragma unroll
-                    for (int i = 0; i < ROWB / 128; ++i) {
-                        v[r][i] = lds128(base + key * ROWB + ((g ^ kv_swizzle(key)) << 4) + 128 * i);
-                        if (valid < KEYS && u * 16 + key >= valid) v[r][i] = make_uint4(0, 0, 0, 0);
+                    for (int i = 0; i < PIECES; ++i)
+                        v[r][i] = lds128(st + 4096 + (u + i) * 2048 + (t + 4 * r) * 128 + ((gp ^ (t + 4 * (r & 1))) << 4));
+                }
+                if (valid < KEYS) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        if (u * 16 + t + 4 * r < valid) continue;
+#pragma unroll
+                        for (int i = 0; i < PIECES; ++i) v[r][i] = make_uint4(0, 0, 0, 0);
                     }
                 }
-                uint32_t pair[2][16];      // [rows 2t, 2t+1 | 2t+8, 2t+9][16 columns: bf16 8g + j and 64 + 8g + j, codes 16g + j]
+                uint32_t pair[2][16];      // [keys t, t + 4 | t + 8, t + 12][16 columns: bf16 8 gp + j and 64 + 8 gp + j, codes 16 gp + j]
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
 #pragma unroll
-                    for (int i = 0; i < ROWB / 128; ++i) {
+                    for (int i = 0; i < PIECES; ++i) {
                         const uint32_t x[4] = {v[2 * r][i].x, v[2 * r][i].y, v[2 * r][i].z, v[2 * r][i].w};
                         const uint32_t y[4] = {v[2 * r + 1][i].x, v[2 * r + 1][i].y, v[2 * r + 1][i].z, v[2 * r + 1][i].w};
 #pragma unroll
@@ -653,116 +768,112 @@ kv_attention_kernel(const KvAttn a) {
                 }
             }
             __syncwarp();
-            issue();
-            slot = slot + 1 == KV_STAGES ? 0 : slot + 1;
+            if (lane == 0) mbar_arrive(&sh.empty[warp][slot]);
+            if (++slot == STAGES) { slot = 0; parity ^= 1; }
         }
 
-        // ---- the warps' parts together
+        // ---- the warps' parts together, 32 columns at a time or as many as fit the team's buffer
+        const int head0 = head_of(seg.item), heads = heads_of(seg.item), log_q = heads <= 4 ? 2 : heads <= 8 ? 1 : 0, quarters = 1 << log_q;
+        team_sync(team);
+        if (seg.end < c1) ask_queries(sh.seg[team][(k + 1) & 1].b, sh.seg[team][(k + 1) & 1].item);
 #pragma unroll
         for (int h = 0; h < HG; ++h) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-            if (t == 0) { s_m[warp][8 * h + g] = m[h]; s_l[warp][8 * h + g] = l[h]; }
+            if (t == 0) { sh.m[team][mate][8 * h + g] = m[h]; sh.l[team][mate][8 * h + g] = l[h]; }
         }
-        __syncthreads();
-        const bool whole = seg == first && end == first + cur.n;
-        float* part = a.parts + ((size_t)blockIdx.x * 2 + (seg == c0 ? 0 : 1)) * KV_PART;
+        const bool whole = seg.begin == seg.first && seg.end == seg.first + seg.n;
+        const int64_t mine = (int64_t)(2 * id + (seg.begin == c0 ? 0 : 1)) * a.per_item;
+        if (!whole && mate == 0 && lane == 0) sh.part[team][sh.parts[team]++] = seg;
 #pragma unroll
-        for (int h = 0; h < HG; ++h) {
-            float fac[2];
+        for (int q = 0; q < 4; ++q) {
+            const int at_q = q & (quarters - 1);
+            if (q > 0 && at_q == 0) team_sync(team);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < KV_WARPS; ++w) top = fmaxf(top, s_m[w][8 * h + 2 * t + j]);
-                fac[j] = exp2_fast(s_m[warp][8 * h + 2 * t + j] - (top == -INFINITY ? 0.f : top));
-            }
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                if (h + half > 0) __syncthreads();
+            for (int h = 0; h < HG; ++h) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    float* to = join + (warp * 8 + 2 * t + j) * 64 + 8 * g;
-#pragma unroll
-                    for (int i = 0; i < 8; i += 4)
-                        *reinterpret_cast<float4*>(to + i) = make_float4(acc[h][i][2 * half + j] * fac[j], acc[h][i + 1][2 * half + j] * fac[j],
-                                                                         acc[h][i + 2][2 * half + j] * fac[j], acc[h][i + 3][2 * half + j] * fac[j]);
-                }
-                __syncthreads();
-                for (int i = tid; i < 8 * 16; i += KV_WARPS * 32) {       // four columns of a head each
-                    const int head = 8 * h + (i >> 4), at = (i & 15) * 4;
-                    if (head >= heads) continue;
-                    float top = -INFINITY, sum = 0.f;
-                    float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll
-                    for (int w = 0; w < KV_WARPS; ++w) top = fmaxf(top, s_m[w][head]);
-#pragma unroll
-                    for (int w = 0; w < KV_WARPS; ++w) {
-                        const float4 x = *reinterpret_cast<const float4*>(join + (w * 8 + (i >> 4)) * 64 + at);
-                        o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
-                        sum += s_l[w][head] * exp2_fast(s_m[w][head] - (top == -INFINITY ? 0.f : top));
-                    }
-                    // columns of the join buffer: bf16 64 half + at; codes 16 (at / 8) + 8 half + at % 8
-                    const int col = TYPE == KV_BF16 ? 64 * half + at : 16 * (at >> 3) + 8 * half + (at & 7);
-                    if (whole) {
-                        const float inv = 1.0f / sum;
-                        uint16_t* dst = a.out + b * a.ldo + (head0 + head) * KV_D + col;
-                        const uint2 r = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-                        if (a.flags & 2) *reinterpret_cast<uint2*>(dst) = r;
-                        else { dst[0] = (uint16_t)r.x; dst[1] = (uint16_t)(r.x >> 16); dst[2] = (uint16_t)r.y; dst[3] = (uint16_t)(r.y >> 16); }
-                        if (a.lse && at == 0 && half == 0) a.lse[(int64_t)b * a.heads + head0 + head] = (top + log2f(sum)) * 0.6931471805599453f;
-                    } else {
-                        *reinterpret_cast<float4*>(part + head * KV_D + col) = o;
-                        if (at == 0 && half == 0) { part[16 * KV_D + head] = top; part[16 * KV_D + 16 + head] = sum; }
-                    }
+                    const int head = 8 * h + 2 * t + j, c = 2 * (q >> 1) + j, four = (q & 1) * 4;
+                    if (head < heads)
+                        *reinterpret_cast<float4*>(buf + ((mate * heads + head) * quarters + at_q) * 32 + 4 * g) =
+                            make_float4(acc[h][four][c], acc[h][four + 1][c], acc[h][four + 2][c], acc[h][four + 3][c]);
                 }
             }
+            if (at_q + 1 < quarters) continue;
+            team_sync(team);
+            const int i = mate * 32 + lane, at = i & 7, qq = (i >> 3) & (quarters - 1), head = i >> (3 + log_q);
+            if (head >= heads) continue;
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < KV_TEAM; ++w) top = fmaxf(top, sh.m[team][w][head]);
+            float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int w = 0; w < KV_TEAM; ++w) {
+                const float e = exp2_fast(sh.m[team][w][head] - (top == -INFINITY ? 0.f : top));
+                const float4 x = *reinterpret_cast<const float4*>(buf + ((w * heads + head) * quarters + qq) * 32 + 4 * at);
+                o.x += x.x * e; o.y += x.y * e; o.z += x.z * e; o.w += x.w * e;
+                sum += sh.l[team][w][head] * e;
+            }
+            // thread g's accumulators are columns 64 half + 8 gp + tile of bf16, 16 gp + 8 half + tile of codes
+            const int quarter = q - quarters + 1 + qq, half = quarter >> 1, col = (TYPE == KV_BF16 ? 64 * half + 8 * kv_perm(at) : 8 * half + 16 * kv_perm(at)) + (quarter & 1) * 4;
+            const bool one = at == 0 && quarter == 0;
+            if (whole) {
+                store_row4(a.out + seg.b * a.ldo + (head0 + head) * KV_D + col, o, 1.0f / sum, a.flags & 2);
+                if (a.lse && one) a.lse[(int64_t)seg.b * a.heads + head0 + head] = (top - KV_LIFT + log2f(sum)) * 0.6931471805599453f;
+            } else {
+                *reinterpret_cast<float4*>(a.parts + (mine + head) * KV_D + col) = o;
+                if (one) a.stats[mine + head] = make_float2(top, sum);
+            }
         }
-
-        // ---- blocks that share the item: the last one joins all parts, in their order
-        if (!whole) {
-            const int from = (int)((((int64_t)first + 1) * blocks - 1) / total), to = (int)(((int64_t)(first + cur.n) * blocks - 1) / total);
+        if (seg.end == c1) break;
+    }
+    // ---- items that the team shares with others
+    team_sync(team);
+    auto come = [&](unsigned* counter, int wanted) {      // whether this team is the last one to come
+        if (mate == 0 && lane == 0) {
             __threadfence();
-            __syncthreads();
-            if (tid == 0) s_last = atomicAdd(a.arrived + from, 1u) == (unsigned)(to - from);
-            __syncthreads();
-            if (s_last) {
-                __threadfence();
-                if (tid == 0) a.arrived[from] = 0;
-                const bool late = first != (int)((int64_t)total * from / blocks);       // the item begins inside the first block's part
-                for (int head = warp; head < heads; head += KV_WARPS) {
-                    float top = -INFINITY, sum = 0.f;
-                    float4 o = make_float4(0, 0, 0, 0);
-                    for (int p = from; p <= to; ++p) top = fmaxf(top, __ldcg(a.parts + ((size_t)p * 2 + (p == from && late)) * KV_PART + 16 * KV_D + head));
-                    const float ref = top == -INFINITY ? 0.f : top;
-                    for (int p = from; p <= to; ++p) {
-                        const float* src = a.parts + ((size_t)p * 2 + (p == from && late)) * KV_PART;
-                        const float w = exp2_fast(__ldcg(src + 16 * KV_D + head) - ref);
-                        const float4 x = __ldcg(reinterpret_cast<const float4*>(src + head * KV_D) + lane);
-                        o.x += x.x * w; o.y += x.y * w; o.z += x.z * w; o.w += x.w * w;
-                        sum += __ldcg(src + 16 * KV_D + 16 + head) * w;
-                    }
-                    const float inv = 1.0f / sum;
-                    uint16_t* dst = a.out + b * a.ldo + (head0 + head) * KV_D + lane * 4;
-                    const uint2 r = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-                    if (a.flags & 2) *reinterpret_cast<uint2*>(dst) = r;
-                    else { dst[0] = (uint16_t)r.x; dst[1] = (uint16_t)(r.x >> 16); dst[2] = (uint16_t)r.y; dst[3] = (uint16_t)(r.y >> 16); }
-                    if (a.lse && lane == 0) a.lse[(int64_t)b * a.heads + head0 + head] = (top + log2f(sum)) * 0.6931471805599453f;
-                }
-            }
+            const bool last = atomicAdd(counter, 1u) == (unsigned)(wanted - 1);
+            __threadfence();
+            if (last) *counter = 0;
+            sh.last[team] = last;
         }
-        __syncthreads();        // s_m, s_l and the join buffer are free again
-        seg = end;
+        team_sync(team);
+        const bool last = sh.last[team];
+        team_sync(team);
+        return last;
+    };
+#pragma unroll 1
+    for (int i = 0; i < sh.parts[team]; ++i) {
+        const typename K::Segment seg = sh.part[team][i];
+        // teams from ... to share the item, in groups of `fan`; the first one's part is in slot `late`
+        const int from = (int)((((int64_t)seg.first + 1) * teams - 1) / total), to = (int)(((int64_t)(seg.first + seg.n) * teams - 1) / total);
+        const int late = seg.first != begin_of(from), count = to - from + 1;
+        const int fan = count <= KV_FLAT ? count : (int)ceilf(sqrtf((float)count)), groups = (count + fan - 1) / fan;
+        const int mine = (id - from) / fan, first = 2 * (from + mine * fan) + (mine == 0 ? late : 0), here = min(fan, count - mine * fan);
+        bool last = come(a.arrived + first, here), done = false;
+        int j_first = first, j_stride = 1, j_count = here;
+#pragma unroll 1
+        while (last && !done) {
+            done = groups == 1 || j_stride > 1;
+            kv_join(a, j_first, j_stride, j_count, seg.b, head_of(seg.item), heads_of(seg.item), done);
+            if (done) break;
+            team_sync(team);
+            last = come(a.arrived + 2 * KV_TEAMS_MAX + 2 * from + late, groups);
+            j_first = 2 * from + late;
+            j_stride = fan;
+            j_count = groups;
+        }
     }
 }
 
 template <int TYPE, int HG>
-static cudaError_t launch_attention(const KvAttn& a, int64_t chunks, cudaStream_t st) {
+static cudaError_t launch_attention(const CUtensorMap& k_map, const CUtensorMap& v_map, const KvAttn& a, int64_t chunks, cudaStream_t st) {
     static std::atomic<uint64_t> done{0};
     using K = KvKernel<TYPE, HG>;
+    static_assert(K::SMEM <= 232448, "more than an SM's block can have");
     if (!func_attr_once(done, (const void*)kv_attention_kernel<TYPE, HG>, K::SMEM, "kv_attention")) return cudaErrorInvalidValue;
-    const int64_t most = min((int64_t)2 * sm_count(), (int64_t)KV_BLOCKS_MAX), want = (chunks + KV_WARPS - 1) / KV_WARPS;
-    return launch_chained(kv_attention_kernel<TYPE, HG>, dim3((unsigned)max((int64_t)1, min(most, want))), dim3(KV_WARPS * 32), K::SMEM, st, 1, 1, a);
+    const int blocks = (int)min((int64_t)min(sm_count(), KV_TEAMS_MAX / K::TEAMS), (chunks + KV_TEAM - 1) / KV_TEAM);
+    return launch_chained(kv_attention_kernel<TYPE, HG>, dim3((unsigned)max(1, blocks)), dim3(K::THREADS), K::SMEM, st, 1, 1, k_map, v_map, a);
 }
 
 static bool aligned16(const void* p, int64_t ld) { return (((uintptr_t)p) & 15) == 0 && (ld & 7) == 0; }
@@ -832,9 +943,10 @@ hd_status o1_kv_read(const o1_kv_cache* cache, void* k, int64_t ldk, void* v, in
     return HD_OK;
 }
 
-int64_t o1_kv_attention_workspace_bytes(int heads) {
-    (void)heads;      // a block's part has room for the 16 heads that it takes at a time
-    return (int64_t)KV_BLOCKS_MAX * (2 * KV_PART * sizeof(float) + sizeof(unsigned));
+// Two counters and, for every head of an item, 128 values, a maximum and a sum, for each team's two parts.
+int64_t o1_kv_attention_workspace_bytes(int heads, int kv_heads) {
+    if (heads <= 0 || kv_heads <= 0 || heads % kv_heads) return -1;
+    return (int64_t)KV_TEAMS_MAX * 2 * (2 * 4 + min(heads / kv_heads, 16) * (KV_D + 2) * 4);
 }
 
 hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, const void* k_new, int64_t ldk, const void* v_new, int64_t ldv,
@@ -852,15 +964,29 @@ hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, 
     const int64_t qrow = (int64_t)heads * KV_D, krow = (int64_t)c.heads * KV_D;
     if (ldq < qrow || ldo < qrow || ldp < width || (k_new && (ldk < krow || ldv < krow))) { set_error("kv_attention: a row pitch is below the row"); return HD_ERR_UNSUPPORTED; }
     if (!(scale > 0.f) || scale > 3.0e38f) { set_error("kv_attention: scale %g", scale); return HD_ERR_UNSUPPORTED; }
-    if (workspace_bytes < o1_kv_attention_workspace_bytes(heads) || (((uintptr_t)workspace) & 15)) { set_error("kv_attention: workspace too small or unaligned"); return HD_ERR_OOM; }
+    if (workspace_bytes < o1_kv_attention_workspace_bytes(heads, c.heads) || (((uintptr_t)workspace) & 15)) { set_error("kv_attention: workspace too small or unaligned"); return HD_ERR_OOM; }
     const int group = heads / c.heads, hg = group <= 8 ? 1 : 2, of_heads = (group + 8 * hg - 1) / (8 * hg), keys = cache->type == O1_KV_BF16 ? 16 : 32;
     // the stream's index is an int: fewer sequences a launch where the table allows for more
     const int64_t each = ((int64_t)width * c.page_size + keys - 1) / keys * c.heads * of_heads;
-    if ((int64_t)width * c.page_size > INT32_MAX - 64 || each > (1 << 30)) { set_error("kv_attention: a table of %d pages of %d is too long for %d heads", width, c.page_size, heads); return HD_ERR_UNSUPPORTED; }
+    if ((int64_t)width * c.page_size > INT32_MAX - 64 || each > (1 << 30) || (int64_t)c.pages * c.heads * c.page_size > INT32_MAX) { set_error("kv_attention: a table of %d pages of %d tokens for %d heads, or a cache of %d pages, is too large", width, c.page_size, heads, c.pages); return HD_ERR_UNSUPPORTED; }
     const int step = (int)min((int64_t)KV_SEQS, each > 0 ? max((int64_t)1, (int64_t)(1 << 30) / each) : (int64_t)KV_SEQS);
-    KvAttn a = {c, nullptr, nullptr, nullptr, ldq, ldk, ldv, ldp, ldo, nullptr, nullptr, nullptr, nullptr, (float*)workspace,
-                (unsigned*)((float*)workspace + (size_t)KV_BLOCKS_MAX * 2 * KV_PART), 0, heads, group, of_heads, width, 0, scale, device_error_word()};
+    const int per_item = min(group, 8 * hg);
+    KvAttn a = {};
+    a.c = c;
+    a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldp = ldp; a.ldo = ldo;
+    a.arrived = (unsigned*)workspace;
+    a.parts = (float*)(a.arrived + 4 * KV_TEAMS_MAX);
+    a.stats = (float2*)(a.parts + (int64_t)2 * KV_TEAMS_MAX * per_item * KV_D);
+    a.heads = heads; a.group = group; a.chunks_of_heads = of_heads; a.per_item = per_item; a.width = width;
+    a.scale = scale;
+    a.err = device_error_word();
     a.flags = (aligned16(q, ldq) ? 1 : 0) | (aligned16(out, ldo) ? 2 : 0) | (aligned16(k_new, ldk) && aligned16(v_new, ldv) ? 4 : 0);
+    // maps of the rows, 128 bytes (64 columns of bf16, all codes) x 16, or 32 where a chunk of codes never crosses a page
+    const bool wide = keys == 32 && c.page_size % 32 == 0;
+    if (wide) a.flags |= 8;
+    const uint64_t rows_all = (uint64_t)c.pages * c.heads * c.page_size, cols = cache->type == O1_KV_BF16 ? 128 : 64;
+    CUtensorMap k_map, v_map;
+    if (!make_tmap_bf16(&k_map, c.k, rows_all, cols, cols, wide ? 32 : 16) || !make_tmap_bf16(&v_map, c.v, rows_all, cols, cols, wide ? 32 : 16)) return HD_ERR_RUNTIME;
     for (int b = 0; b < batch; b += step) {
         a.batch = min(step, batch - b);
         a.q = (const uint16_t*)q + b * ldq;
@@ -872,9 +998,9 @@ hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, 
         a.lse = lse ? lse + (int64_t)b * heads : nullptr;
         const int64_t chunks = each * a.batch;
         cudaError_t e;
-        if (cache->type == O1_KV_BF16) e = hg == 1 ? launch_attention<KV_BF16, 1>(a, chunks, current_stream()) : launch_attention<KV_BF16, 2>(a, chunks, current_stream());
-        else if (cache->type == O1_KV_FP8) e = hg == 1 ? launch_attention<KV_FP8, 1>(a, chunks, current_stream()) : launch_attention<KV_FP8, 2>(a, chunks, current_stream());
-        else e = hg == 1 ? launch_attention<KV_INT8, 1>(a, chunks, current_stream()) : launch_attention<KV_INT8, 2>(a, chunks, current_stream());
+        if (cache->type == O1_KV_BF16) e = hg == 1 ? launch_attention<KV_BF16, 1>(k_map, v_map, a, chunks, current_stream()) : launch_attention<KV_BF16, 2>(k_map, v_map, a, chunks, current_stream());
+        else if (cache->type == O1_KV_FP8) e = hg == 1 ? launch_attention<KV_FP8, 1>(k_map, v_map, a, chunks, current_stream()) : launch_attention<KV_FP8, 2>(k_map, v_map, a, chunks, current_stream());
+        else e = hg == 1 ? launch_attention<KV_INT8, 1>(k_map, v_map, a, chunks, current_stream()) : launch_attention<KV_INT8, 2>(k_map, v_map, a, chunks, current_stream());
         if (!launch_ok(e, "kv_attention")) return HD_ERR_RUNTIME;
         o1_launch_count_add(1);
     }

@@ -109,7 +109,9 @@ class KvCache:
         key = (lib.o1_get_stream(), heads)
         w = self._work.get(key)
         if w is None:
-            w = self._work[key] = torch.zeros(lib.o1_kv_attention_workspace_bytes(heads), dtype=torch.uint8, device=self.device)
+            need = lib.o1_kv_attention_workspace_bytes(heads, self.kv_heads)
+            _need(need >= 0, f"KvCache.attend: heads {heads} (a multiple of kv_heads {self.kv_heads})")
+            w = self._work[key] = torch.zeros(need, dtype=torch.uint8, device=self.device)
         return w
 
     def attend(self, q, pages, lens, k=None, v=None, out=None, lse=None, scale=None):

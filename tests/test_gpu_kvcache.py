@@ -476,7 +476,7 @@ def test_entry_points_refuse_before_they_touch_the_gpu(pkg):
     assert write(rows=0) == 0 and lib.o1_kv_read(C.byref(K(**good)), one, 256, one, 256, one, 0) == 0
     assert lib.o1_kv_read(C.byref(K(**{**good, "v": None})), one, 256, one, 256, one, 1) == 6
     assert lib.o1_kv_read(C.byref(K(**{**good, "k": 4104})), one, 256, one, 256, one, 1) == 9
-    need = lib.o1_kv_attention_workspace_bytes(4)
+    need = lib.o1_kv_attention_workspace_bytes(4, 2)
 
     def attend(q=one, ldq=512, kn=None, ldk=256, vn=None, ldv=256, pages=one, ldp=3, width=3, lens=one, out=one, ldo=512, batch=1, heads=4, scale=0.1,
                ws=one, nb=need, **change):
