@@ -202,7 +202,12 @@ static constexpr int KV_STAGE_BYTES = 8192;            // keys and values of a c
 static constexpr int KV_SEQS = 256;                    // sequences of a launch
 static constexpr int KV_TEAM = 4;                      // warps
 static constexpr int KV_TEAMS_MAX = 160 * 3;           // what the workspace has room for
-static constexpr int KV_FLAT = 48;                     // so many teams' parts are joined at once, more in groups
+#ifndef KVOV
+#define KVOV 4
+#define KVFL 32
+#endif
+static constexpr int KV_FLAT = KVFL;                   // so many teams' parts are joined at once, more in groups
+static constexpr int KV_ITEM_COST = KVOV;              // what an item costs a team beside its chunks, in chunks
 static constexpr int KV_JOIN_BYTES = 8192;             // of a team
 static constexpr int ERR_KV_WAIT = 72;                 // a wait of the attention kernel ran out
 static constexpr float KV_LIFT = 20.0f;                // probabilities are relative to 2^-20 of the largest: those that fp32 has no value for are 2^-146 and less of it
@@ -310,7 +315,8 @@ struct KvKernel {
     struct Shared {
         uint64_t full[WARPS][STAGES], empty[WARPS][STAGES];
         Segment seg[TEAMS][2], part[TEAMS][2];
-        int prefix[KV_SEQS + 1], len[KV_SEQS], scan[WARPS + TEAMS], parts[TEAMS], last[TEAMS];
+        int prefix[KV_SEQS + 1], cost[KV_SEQS], len[KV_SEQS], parts[TEAMS], last[TEAMS];      // chunks and costs before a sequence
+        int2 scan[WARPS + TEAMS];
         float m[TEAMS][KV_TEAM][8 * HG], l[TEAMS][KV_TEAM][8 * HG];
     };
     static constexpr int SMEM = SHARED + (int)sizeof(Shared);
@@ -342,26 +348,27 @@ struct KvWalk {
     }
 };
 
-// Sums of v over the block's threads before this one, and over all.  (One barrier before, one behind: `part` is free again.)
+// Sums of v over the block's threads before this one, and over all, of both components.
 template <int WARPS>
-__device__ __forceinline__ int block_scan(int v, int& all, int* part) {
+__device__ __forceinline__ int2 block_scan(int2 v, int2& all, int2* part) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int sum = v;
+    int2 sum = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += x;
+        const int x = __shfl_up_sync(0xffffffffu, sum.x, o), y = __shfl_up_sync(0xffffffffu, sum.y, o);
+        if (lane >= o) { sum.x += x; sum.y += y; }
     }
     if (lane == 31) part[warp] = sum;
     __syncthreads();
-    int before = sum - v;
-    all = 0;
+    int2 before = make_int2(sum.x - v.x, sum.y - v.y);
+    all = make_int2(0, 0);
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-        before += w < warp ? part[w] : 0;
-        all += part[w];
+        const int2 p = part[w];
+        if (w < warp) { before.x += p.x; before.y += p.y; }
+        all.x += p.x;
+        all.y += p.y;
     }
-    __syncthreads();
     return before;
 }
 
@@ -377,22 +384,23 @@ __device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, 
     const int lane = threadIdx.x & 31;
     auto place = [&](int i) { return (int64_t)(i == 0 ? first : (first & ~1) + 2 * stride * i) * a.per_item; };
     for (int head = (threadIdx.x >> 5) & (KV_TEAM - 1); head < heads; head += KV_TEAM) {
-        float top = -INFINITY;
-        for (int i = lane; i < count; i += 32) top = fmaxf(top, __ldcg(&a.stats[place(i) + head]).x);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float ref = top == -INFINITY ? 0.f : top;
-        float sum = 0.f;
+        float top = -INFINITY, sum = 0.f;
         float4 r = make_float4(0, 0, 0, 0);
-        for (int i0 = 0; i0 < count; i0 += 16) {
+#pragma unroll 1
+        for (int i0 = 0; i0 < count; i0 += 16) {      // all that 16 parts need is asked for at once
             float4 x[16];
             float2 s = make_float2(-INFINITY, 0.f);
             if (lane < 16 && i0 + lane < count) s = __ldcg(&a.stats[place(i0 + lane) + head]);
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 if (i0 + i < count) x[i] = __ldcg(reinterpret_cast<const float4*>(a.parts + (place(i0 + i) + head) * KV_D) + lane);
-            const float w = exp2_fast(s.x - ref);
-            sum += s.y * w;
+            float here = s.x;
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, o));
+            const float m = fmaxf(top, __shfl_sync(0xffffffffu, here, 0)), ref = m == -INFINITY ? 0.f : m, old = exp2_fast(top - ref), w = exp2_fast(s.x - ref);
+            top = m;
+            sum = sum * old + s.y * w;
+            r.x *= old; r.y *= old; r.z *= old; r.w *= old;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float f = __shfl_sync(0xffffffffu, w, i);
@@ -431,20 +439,35 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 
     // ---- the lengths, as numbers of chunks, summed up
     const int ps = a.c.page_size, shift = a.c.page_shift, items = a.c.heads * a.chunks_of_heads;
-    int total;
+    int total, cost;
     {
         static_assert(KV_SEQS <= K::THREADS, "a sequence to a thread");
         int len = tid < a.batch ? a.lens[tid] : 0;
         if (len < 0 || len > (int64_t)a.width * ps) { atomicExch(a.err, ERR_KV_LENGTH); len = 0; }
-        const int before = block_scan<WARPS + K::TEAMS>((len + KEYS - 1) / KEYS, total, sh.scan);
-        if (tid < a.batch) { sh.prefix[tid] = before; sh.len[tid] = len; }
-        if (tid == 0) sh.prefix[a.batch] = total;
-        total *= items;
+        const int n = (len + KEYS - 1) / KEYS;
+        int2 all;
+        const int2 before = block_scan<WARPS + K::TEAMS>(make_int2(n, n > 0 ? n + KV_ITEM_COST : 0), all, sh.scan);
+        if (tid < a.batch) { sh.prefix[tid] = before.x; sh.cost[tid] = before.y; sh.len[tid] = len; }
+        if (tid == 0) sh.prefix[a.batch] = all.x;
+        total = all.x * items;
+        cost = all.y * items;
         __syncthreads();
     }
-    // ---- a team's part of the stream
-    const int teams = min((int)gridDim.x * K::TEAMS, (total + KV_TEAM - 1) / KV_TEAM);
-    auto begin_of = [&](int id) { return (int)((int64_t)total * id / teams); };
+    // ---- a team's part of the stream: equal costs, where each item costs some chunks more than it has; ends inside an item that is not worth a join are moved
+    const int teams = min((int)gridDim.x * K::TEAMS, (total + KV_TEAM - 1) / KV_TEAM), share = teams > 0 ? total / teams : 0, keep = share <= 8 ? 24 : max(8, share >> 2);
+    auto begin_of = [&](int id) {
+        if (id >= teams) return total;
+        const int at = (int)((int64_t)cost * id / teams);
+        int lo = 0, hi = a.batch - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (sh.cost[mid] * items <= at) lo = mid; else hi = mid - 1;
+        }
+        const int n = sh.prefix[lo + 1] - sh.prefix[lo], rel = at - sh.cost[lo] * items, item = rel / (n + KV_ITEM_COST);
+        int c = min(rel - item * (n + KV_ITEM_COST), n);
+        if (n <= keep) c = 2 * c < n ? 0 : n;
+        return sh.prefix[lo] * items + item * n + c;
+    };
 
     if (warp >= WARPS) {
         // ---- the team's loading warp
@@ -522,8 +545,8 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         for (int i = mate * 32 + lane; i < a.heads * KV_D; i += KV_TEAM * 32) a.out[b * a.ldo + i] = 0;
         if (a.lse) for (int i = mate * 32 + lane; i < a.heads; i += KV_TEAM * 32) a.lse[(int64_t)b * a.heads + i] = -INFINITY;
     }
-    if (id >= teams) return;
     const int c0 = begin_of(id), c1 = begin_of(id + 1);
+    if (c0 >= c1) return;
 
     auto head_of = [&](int item) {         // the first query head of an item
         const int kvh = a.chunks_of_heads == 1 ? item : item / a.chunks_of_heads;
@@ -846,7 +869,8 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     for (int i = 0; i < sh.parts[team]; ++i) {
         const typename K::Segment seg = sh.part[team][i];
         // teams from ... to share the item, in groups of `fan`; the first one's part is in slot `late`
-        const int from = (int)((((int64_t)seg.first + 1) * teams - 1) / total), to = (int)(((int64_t)(seg.first + seg.n) * teams - 1) / total);
+        const int64_t at = (int64_t)sh.cost[seg.b] * items + (int64_t)seg.item * (seg.n + KV_ITEM_COST);
+        const int from = (int)(((at + 1) * teams - 1) / cost), to = (int)(((at + seg.n) * teams - 1) / cost);
         const int late = seg.first != begin_of(from), count = to - from + 1;
         const int fan = count <= KV_FLAT ? count : (int)ceilf(sqrtf((float)count)), groups = (count + fan - 1) / fan;
         const int mine = (id - from) / fan, first = 2 * (from + mine * fan) + (mine == 0 ? late : 0), here = min(fan, count - mine * fan);
