@@ -179,7 +179,7 @@ __device__ __forceinline__ float row_rms_inv(F squares, int cols, float eps, flo
     if (sum < INFINITY) return rsqrtf(sum / (float)cols + eps);
     return rsqrtf(block_sum<THREADS>(squares(8.271806125530277e-25f), red[1]) / (float)cols) * 8.271806125530277e-25f;
 }
-template <int THREADS, int ITEMS, bool POST>
+template <int THREADS, int ITEMS, bool POST, bool EARLY>
 __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS)
 residual_norm_vec_kernel(const ResidualNorm a) {
     grid_dep_launch();
@@ -192,11 +192,23 @@ residual_norm_vec_kernel(const ResidualNorm a) {
     const size_t vec = (size_t)(row / a.per_group) * nvec;
     const uint4* x = reinterpret_cast<const uint4*>(a.x + row * a.ldx);
     const uint4* b = reinterpret_cast<const uint4*>(a.branch + row * a.ldb);
-    uint4 xv[ITEMS], bv[ITEMS];
+    const uint4 *post = reinterpret_cast<const uint4*>(a.post), *gate = a.gate ? reinterpret_cast<const uint4*>(a.gate) + vec : nullptr;
+    const uint4 *pre = reinterpret_cast<const uint4*>(a.pre), *scale = a.scale ? reinterpret_cast<const uint4*>(a.scale) + vec : nullptr,
+                *shift = reinterpret_cast<const uint4*>(a.shift) + vec;
+    uint4 xv[ITEMS], bv[ITEMS], wv[EARLY ? ITEMS : 1], gv[EARLY ? ITEMS : 1], pv[EARLY ? ITEMS : 1], cv[EARLY ? ITEMS : 1], sv[EARLY ? ITEMS : 1];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         const int idx = tid + i * THREADS;
-        if (idx < nvec) { xv[i] = x[idx]; bv[i] = b[idx]; }
+        if (idx < nvec) {
+            xv[i] = x[idx];
+            bv[i] = b[idx];
+            if (EARLY) {
+                if (POST) wv[i] = post[idx];
+                if (gate) gv[i] = gate[idx];
+                if (a.h) pv[i] = pre[idx];
+                if (scale) { cv[i] = scale[idx]; sv[i] = shift[idx]; }
+            }
+        }
     }
     float inv = 1.f;
     if (POST) {
@@ -223,12 +235,12 @@ residual_norm_vec_kernel(const ResidualNorm a) {
             unpack8(xv[i], f);
             unpack8(bv[i], u);
             if (POST) {
-                unpack8(reinterpret_cast<const uint4*>(a.post)[idx], w);
+                unpack8(EARLY ? wv[EARLY ? i : 0] : post[idx], w);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) u[j] = u[j] * inv * w[j];
             }
-            if (a.gate) {
-                unpack8(reinterpret_cast<const uint4*>(a.gate)[vec + idx], w);
+            if (gate) {
+                unpack8(EARLY ? gv[EARLY ? i : 0] : gate[idx], w);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) u[j] *= w[j];
             }
@@ -254,13 +266,13 @@ residual_norm_vec_kernel(const ResidualNorm a) {
         const int idx = tid + i * THREADS;
         if (idx < nvec) {
             float w[8];
-            unpack8(reinterpret_cast<const uint4*>(a.pre)[idx], w);
+            unpack8(EARLY ? pv[EARLY ? i : 0] : pre[idx], w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[i][j] = y[i][j] * inv * w[j];
-            if (a.scale) {
+            if (scale) {
                 float sh[8];
-                unpack8(reinterpret_cast<const uint4*>(a.scale)[vec + idx], w);
-                unpack8(reinterpret_cast<const uint4*>(a.shift)[vec + idx], sh);
+                unpack8(EARLY ? cv[EARLY ? i : 0] : scale[idx], w);
+                unpack8(EARLY ? sv[EARLY ? i : 0] : shift[idx], sh);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) y[i][j] = y[i][j] * (1.0f + w[j]) + sh[j];
             }
@@ -308,6 +320,7 @@ __global__ void __launch_bounds__(256) residual_norm_any_kernel(const ResidualNo
         a.y[row * a.ldy + i] = f32_to_bf16(f);
     }
 }
+static constexpr int RESIDUAL_EARLY_ROWS = 1200;
 bool residual_norm(const void* x, int64_t ldx, const void* branch, int64_t ldb, const void* post, const void* gate, float alpha, const void* pre,
                    const void* scale, const void* shift, int groups, void* y, int64_t ldy, void* h, int64_t ldh, int rows, int cols, float eps,
                    cudaStream_t st) {
@@ -315,11 +328,18 @@ bool residual_norm(const void* x, int64_t ldx, const void* branch, int64_t ldb, 
                             (const uint16_t*)scale, (const uint16_t*)shift, (uint16_t*)y, (uint16_t*)h, ldx, ldb, ldy, ldh, rows, cols, rows / groups, alpha, eps};
     const uintptr_t all = (uintptr_t)x | (uintptr_t)branch | (uintptr_t)post | (uintptr_t)gate | (uintptr_t)pre | (uintptr_t)scale | (uintptr_t)shift |
                           (uintptr_t)y | (uintptr_t)h;
-    const bool vec = (all & 15) == 0 && ((ldx | ldb | ldy | (h ? ldh : 0) | cols) & 7) == 0 && cols <= 8192;
+    const bool vec = (all & 15) == 0 && ((ldx | ldb | ldy | (h ? ldh : 0) | cols) & 7) == 0 && cols <= 16384;
     if (!vec) return launch_ok(launch_chained(residual_norm_any_kernel, dim3(rows), dim3(256), 0, st, 1, rows, a), "residual_norm");
-    auto kern = post ? (cols <= 1024 ? residual_norm_vec_kernel<32, 4, true> : cols <= 4096 ? residual_norm_vec_kernel<128, 4, true> : residual_norm_vec_kernel<256, 4, true>)
-                     : (cols <= 1024 ? residual_norm_vec_kernel<32, 4, false> : cols <= 4096 ? residual_norm_vec_kernel<128, 4, false> : residual_norm_vec_kernel<256, 4, false>);
-    return launch_ok(launch_chained(kern, dim3(cols <= 1024 ? (rows + 3) / 4 : rows), dim3(cols > 4096 ? 256 : 128), 0, st, 1, rows, a), "residual_norm");
+    // EARLY where the rows fit the GPU at once: what a row needs is asked for together
+    const bool early = rows <= RESIDUAL_EARLY_ROWS;
+#define O1_RN(T, I) (post ? (early ? residual_norm_vec_kernel<T, I, true, true> : residual_norm_vec_kernel<T, I, true, false>) \
+                          : (early ? residual_norm_vec_kernel<T, I, false, true> : residual_norm_vec_kernel<T, I, false, false>))
+    auto kern = cols <= 256 ? O1_RN(32, 1) : cols <= 1024 ? O1_RN(32, 4) : cols <= 1280 ? O1_RN(32, 5) : cols <= 2048 ? O1_RN(64, 4) : cols <= 4096 ? O1_RN(128, 4)
+                : cols <= 8192 ? O1_RN(256, 4) : O1_RN(512, 4);
+#undef O1_RN
+    const bool warps = cols <= 1280;
+    const int threads = warps || cols <= 4096 ? (warps || cols > 2048 ? 128 : 64) : cols <= 8192 ? 256 : 512;
+    return launch_ok(launch_chained(kern, dim3(warps ? (rows + 3) / 4 : rows), dim3(threads), 0, st, 1, rows, a), "residual_norm");
 }
 
 // ------------------------------------------------------------------ materialising attention (small / odd shapes)

@@ -106,76 +106,89 @@ __device__ __forceinline__ void store8(uint16_t* p, const uint4& v) {
     for (int i = 0; i < 4; ++i) { p[2 * i] = (uint16_t)w[i]; p[2 * i + 1] = (uint16_t)(w[i] >> 16); }
 }
 
-// Slot of a new row of sequence b: its last one, by the page table.  -1: nothing to write.
-__device__ __forceinline__ int64_t last_slot(const int32_t* pages, int64_t ldp, int width, const int32_t* lens, int b, const KvView& c, int* err) {
-    const int n = lens[b];
-    if (n == 0) return -1;
-    if (n < 0 || n > (int64_t)width * c.page_size) { atomicExch(err, ERR_KV_LENGTH); return -1; }
-    const int page = pages[b * ldp + (n - 1) / c.page_size];
-    if ((unsigned)page >= (unsigned)c.pages) { atomicExch(err, ERR_KV_PLACE); return -1; }
-    return (int64_t)page * c.page_size + (n - 1) % c.page_size;
-}
-
-// Row r's place in a [pages][heads][page_size] array, -1: none.
-__device__ __forceinline__ int64_t place(int64_t slot, int head, const KvView& c, int* err) {
+// A slot's row of head 0 in a [pages][heads][page_size] array, -1: none.  (The other heads' lie page_size apart.)
+__device__ __forceinline__ int64_t place(int64_t slot, const KvView& c, int* err) {
     if (slot < 0) return -1;
     if (slot >= (int64_t)c.pages * c.page_size) { atomicExch(err, ERR_KV_PLACE); return -1; }
-    const int64_t page = slot / c.page_size;
-    return (page * c.heads + head) * c.page_size + slot - page * c.page_size;
+    const int64_t page = c.page_shift >= 0 ? slot >> c.page_shift : slot / c.page_size;
+    return page * c.heads * c.page_size + slot - page * c.page_size;
 }
 
-// One row of 128 of one of the tensors to 16 lanes.  HBM bound for many rows: 2 bytes in, 1 (or 2) and the scale out a value.
+// A row to a warp: its keys to the lower 16 lanes, its values to the others, eight columns to a lane, KV_ROW_HEADS heads at a time.  HBM bound for many rows: 2 bytes
+// in, 1 (or 2) and the scale out a value.  What a row's heads need is asked for together, beside its slot, so that a warp has 4 KB on its way;
+// with a head to a half warp (and a 64-bit division in each) 16640 rows of 8 heads took 34 us, written, and 35, read.
+static constexpr int KV_ROW_HEADS = 8;
 template <bool VEC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
 kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk, const uint16_t* __restrict__ v, int64_t ldv,
-                const int64_t* __restrict__ slots, const int32_t* __restrict__ pages, int64_t ldp, int width,
-                const int32_t* __restrict__ lens, int rows, int* err) {
+                const int64_t* __restrict__ slots, int rows, int* err) {
     grid_dep_launch();
     grid_dep_wait();
-    const int64_t unit = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (row >= rows) return;
     const int lane = threadIdx.x & 15;
-    const int64_t row = unit / (2 * c.heads);
-    const int part = (int)(unit - row * 2 * c.heads), head = part >> 1;
-    const bool is_v = part & 1, on = row < rows;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    int64_t at = -1;
-    if (on) {
-        x = load8<VEC>((is_v ? v + row * ldv : k + row * ldk) + head * KV_D + lane * 8);
-        at = place(slots ? slots[row] : last_slot(pages, ldp, width, lens, (int)row, c, err), head, c, err);
-    }
-    uint8_t* base = is_v ? c.v : c.k;
-    if (type == KV_BF16) {
-        if (at >= 0) reinterpret_cast<uint4*>(base)[at * 16 + lane] = x;
-        return;
-    }
-    float scale;
-    const uint2 codes = quantise8(x, type, scale);
-    if (at >= 0) {
-        reinterpret_cast<uint2*>(base)[at * 16 + lane] = codes;
-        if (lane == 0) (is_v ? c.vs : c.ks)[at] = scale;
+    const bool is_v = threadIdx.x & 16;
+    const uint16_t* src = (is_v ? v + row * ldv : k + row * ldk) + lane * 8;
+    uint8_t* const base = is_v ? c.v : c.k;
+    float* const scales = is_v ? c.vs : c.ks;
+    const int64_t slot = slots[row];
+    for (int h0 = 0; h0 < c.heads; h0 += KV_ROW_HEADS) {
+        uint4 x[KV_ROW_HEADS];
+#pragma unroll
+        for (int i = 0; i < KV_ROW_HEADS; ++i)
+            if (h0 + i < c.heads) x[i] = load8<VEC>(src + (h0 + i) * KV_D);
+        const int64_t first = place(slot, c, err);
+        if (first < 0) return;
+#pragma unroll
+        for (int i = 0; i < KV_ROW_HEADS; ++i) {
+            if (h0 + i >= c.heads) break;
+            const int64_t at = first + (int64_t)(h0 + i) * c.page_size;
+            if (type == KV_BF16) {
+                reinterpret_cast<uint4*>(base)[at * 16 + lane] = x[i];
+                continue;
+            }
+            float scale;
+            reinterpret_cast<uint2*>(base)[at * 16 + lane] = quantise8(x[i], type, scale);
+            if (lane == 0) scales[at] = scale;
+        }
     }
 }
 
 template <bool VEC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
 kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16_t* __restrict__ v, int64_t ldv,
                const int64_t* __restrict__ slots, int rows, int* err) {
     grid_dep_launch();
     grid_dep_wait();
-    const int64_t unit = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const int lane = threadIdx.x & 15;
-    const int64_t row = unit / (2 * c.heads);
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     if (row >= rows) return;
-    const int part = (int)(unit - row * 2 * c.heads), head = part >> 1;
-    const bool is_v = part & 1;
-    const int64_t at = place(slots[row], head, c, err);
-    const uint8_t* base = is_v ? c.v : c.k;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (at >= 0) {
-        if (type == KV_BF16) x = reinterpret_cast<const uint4*>(base)[at * 16 + lane];
-        else x = dequantise8(reinterpret_cast<const uint2*>(base)[at * 16 + lane], type, (is_v ? c.vs : c.ks)[at]);
+    const int lane = threadIdx.x & 15;
+    const bool is_v = threadIdx.x & 16;
+    uint16_t* dst = (is_v ? v + row * ldv : k + row * ldk) + lane * 8;
+    const uint8_t* const base = is_v ? c.v : c.k;
+    const float* const scales = is_v ? c.vs : c.ks;
+    const int64_t first = place(slots[row], c, err);
+    for (int h0 = 0; h0 < c.heads; h0 += KV_ROW_HEADS) {
+        uint4 x[KV_ROW_HEADS];
+        float scale[KV_ROW_HEADS];
+#pragma unroll
+        for (int i = 0; i < KV_ROW_HEADS; ++i) {
+            x[i] = make_uint4(0, 0, 0, 0);
+            scale[i] = 0.f;
+            if (h0 + i >= c.heads || first < 0) continue;
+            const int64_t at = first + (int64_t)(h0 + i) * c.page_size;
+            if (type == KV_BF16) { x[i] = reinterpret_cast<const uint4*>(base)[at * 16 + lane]; continue; }
+            const uint2 codes = reinterpret_cast<const uint2*>(base)[at * 16 + lane];
+            x[i].x = codes.x;
+            x[i].y = codes.y;
+            scale[i] = scales[at];
+        }
+#pragma unroll
+        for (int i = 0; i < KV_ROW_HEADS; ++i) {
+            if (h0 + i >= c.heads) break;
+            store8<VEC>(dst + (h0 + i) * KV_D, type == KV_BF16 ? x[i] : dequantise8(make_uint2(x[i].x, x[i].y), type, scale[i]));
+        }
     }
-    store8<VEC>((is_v ? v + row * ldv : k + row * ldk) + head * KV_D + lane * 8, x);
 }
 
 // ------------------------------------------------------------------ attention of a new row
@@ -940,10 +953,9 @@ hd_status o1_kv_write(const o1_kv_cache* cache, const void* k, int64_t ldk, cons
     if (!k || !v || !slots) { set_error("kv_write: null argument"); return HD_ERR_MISSING; }
     const int64_t row = (int64_t)c.heads * KV_D;
     if (ldk < row || ldv < row) { set_error("kv_write: row pitch below %lld", (long long)row); return HD_ERR_UNSUPPORTED; }
-    const int64_t units = (int64_t)rows * c.heads * 2;
     auto kern = aligned16(k, ldk) && aligned16(v, ldv) ? kv_write_kernel<true> : kv_write_kernel<false>;
-    if (!launch_ok(launch_chained(kern, dim3((unsigned)((units + 15) / 16)), dim3(256), 0, current_stream(), 1, rows, c, cache->type, (const uint16_t*)k, ldk,
-                                  (const uint16_t*)v, ldv, slots, (const int32_t*)nullptr, (int64_t)0, 0, (const int32_t*)nullptr, rows, device_error_word()), "kv_write"))
+    if (!launch_ok(launch_chained(kern, dim3((unsigned)(((int64_t)rows + 3) / 4)), dim3(128), 0, current_stream(), 1, rows, c, cache->type, (const uint16_t*)k, ldk,
+                                  (const uint16_t*)v, ldv, slots, rows, device_error_word()), "kv_write"))
         return HD_ERR_RUNTIME;
     o1_launch_count_add(1);
     return HD_OK;
@@ -958,9 +970,8 @@ hd_status o1_kv_read(const o1_kv_cache* cache, void* k, int64_t ldk, void* v, in
     if (!k || !v || !slots) { set_error("kv_read: null argument"); return HD_ERR_MISSING; }
     const int64_t row = (int64_t)c.heads * KV_D;
     if (ldk < row || ldv < row) { set_error("kv_read: row pitch below %lld", (long long)row); return HD_ERR_UNSUPPORTED; }
-    const int64_t units = (int64_t)rows * c.heads * 2;
     auto kern = aligned16(k, ldk) && aligned16(v, ldv) ? kv_read_kernel<true> : kv_read_kernel<false>;
-    if (!launch_ok(launch_chained(kern, dim3((unsigned)((units + 15) / 16)), dim3(256), 0, current_stream(), 1, rows, c, cache->type, (uint16_t*)k, ldk,
+    if (!launch_ok(launch_chained(kern, dim3((unsigned)(((int64_t)rows + 3) / 4)), dim3(128), 0, current_stream(), 1, rows, c, cache->type, (uint16_t*)k, ldk,
                                   (uint16_t*)v, ldv, slots, rows, device_error_word()), "kv_read"))
         return HD_ERR_RUNTIME;
     o1_launch_count_add(1);
