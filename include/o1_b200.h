@@ -795,6 +795,19 @@ hd_status o1_kv_attention(const o1_kv_cache *cache, const void *q, int64_t ldq, 
 hd_status o1_residual_norm(const void *x, int64_t ldx, const void *branch, int64_t ldb, const void *post_w, const void *gate,
                            float alpha, const void *pre_w, const void *scale, const void *shift, int groups, void *y,
                            int64_t ldy, void *h, int64_t ldh, int rows, int cols, float eps);
+/* The decoder blocks on cached rows: caches [n_layers] (one of each block, with the same pages and page_size, so that one page table serves
+ * all), ids int64 on the device, pos_f32 [3, rows] as hd_forward's, out [rows, hidden] bf16: the rows behind the final norm.
+ * o1_prompt_rows: all rows of one sequence, causal, their keys and values into slots[r] of each cache.  o1_decode_step: one new row of each of `batch` sequences, which
+ * becomes row lens[b] - 1 of sequence b.  scratch: o1_decode_scratch_bytes(rows, ...) bytes, its first o1_kv_attention_workspace_bytes zero-filled once (zero all
+ * of it); one for each stream.  The residual stream's norms are of its unrounded sums (o1_residual_norm), so the rows agree with hd_decoder_block's within rounding, and a row
+ * does not depend on which other rows a step has. */
+int64_t o1_decode_scratch_bytes(int64_t rows, int heads, int kv_heads, int hidden, int ff_hidden, int head_dim);
+hd_status o1_prompt_rows(const hd_forward_binding *bw, const o1_kv_cache *caches, const int64_t *ids, const float *pos_f32,
+                         const int64_t *slots, void *scratch, int64_t scratch_bytes, void *out, int rows, int heads,
+                         int kv_heads, int hidden, int ff_hidden, int head_dim, int vocab);
+hd_status o1_decode_step(const hd_forward_binding *bw, const o1_kv_cache *caches, const int64_t *ids, const float *pos_f32,
+                         const int32_t *pages, int64_t ldp, int width, const int32_t *lens, void *scratch, int64_t scratch_bytes,
+                         void *out, int batch, int heads, int kv_heads, int hidden, int ff_hidden, int head_dim, int vocab);
 
 #ifdef __cplusplus
 }

@@ -293,6 +293,12 @@ _sig("o1_kv_attention", c_int, C.POINTER(KvCacheC), _P, c_int64, _P, c_int64, _P
 _sig("o1_residual_norm", c_int, _P, c_int64, _P, c_int64, _P, _P, c_float, _P, _P, _P, c_int, _P, c_int64, _P, c_int64,
      c_int, c_int, c_float)
 
+_sig("o1_decode_scratch_bytes", c_int64, c_int64, c_int, c_int, c_int, c_int, c_int)
+_sig("o1_prompt_rows", c_int, C.POINTER(ForwardBinding), C.POINTER(KvCacheC), _P, _P, _P, _P, c_int64, _P, c_int, c_int, c_int,
+     c_int, c_int, c_int, c_int)
+_sig("o1_decode_step", c_int, C.POINTER(ForwardBinding), C.POINTER(KvCacheC), _P, _P, _P, c_int64, c_int, _P, _P, c_int64, _P,
+     c_int, c_int, c_int, c_int, c_int, c_int, c_int)
+
 EPI_STORE, EPI_BIAS, EPI_RESID, EPI_SWIGLU, EPI_LORA, EPI_BIAS_GELU, EPI_BIAS_RESID, EPI_GATE_RESID = 0, 1, 2, 3, 4, 7, 8, 9
 
 
@@ -336,4 +342,4 @@ def use_torch_stream():
 from .model import (  # noqa: E402
     Weights, GgufWeights, Engine, seq_t2i, seq_ref, dev_sigmas, write_gguf, gguf_tensor_name, weight_seed, SLOT_NAMES, GLOBAL_NAMES, tensor_shape,
 )
-from .kvcache import KvCache, residual_norm  # noqa: E402
+from .kvcache import KvCache, Decoder, residual_norm  # noqa: E402

@@ -41,9 +41,12 @@ __device__ __forceinline__ uint32_t f32_to_e4m3x2(float lo, float hi) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// To the nearest integers, ties to even, in bytes: the sum with 1.5 * 2^23 has them in its low bits.  (Conversions to and from integers go through a pipe of a
+// quarter of the rate.)
 __device__ __forceinline__ uint32_t int8x4(float a, float b, float c, float d) {
-    const int i = __float2int_rn(a), j = __float2int_rn(b), k = __float2int_rn(c), l = __float2int_rn(d);
-    return __byte_perm(__byte_perm(i, j, 0x0040), __byte_perm(k, l, 0x0040), 0x5410);
+    constexpr float M = 12582912.0f;
+    auto bits = [](float x) { return __float_as_uint(__fadd_rn(x, M)); };      // (x, a product, is rounded by itself)
+    return __byte_perm(__byte_perm(bits(a), bits(b), 0x0040), __byte_perm(bits(c), bits(d), 0x0040), 0x5410);
 }
 
 // Quantising a row of 128, eight values to each of 16 lanes.  The scale is the row's largest magnitude over the
@@ -78,7 +81,8 @@ __device__ __forceinline__ uint4 dequantise8(const uint2& c, int type, float sca
     const uint32_t w[2] = {c.x, c.y};
     if (type == KV_INT8) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3))) * scale;
+        for (int i = 0; i < 8; ++i)      // (c ^ 0x80) + 2^23 as bits
+            f[i] = (__uint_as_float(__byte_perm(w[i >> 2] ^ 0x80808080u, 0x4B000000u, 0x7540 + (i & 3))) - 8388736.0f) * scale;
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -114,34 +118,34 @@ __device__ __forceinline__ int64_t place(int64_t slot, const KvView& c, int* err
     return page * c.heads * c.page_size + slot - page * c.page_size;
 }
 
-// A row to a warp: its keys to the lower 16 lanes, its values to the others, eight columns to a lane, KV_ROW_HEADS heads at a time.  HBM bound for many rows: 2 bytes
+// A row (few rows: `each` of its heads) to a warp: its keys to the lower 16 lanes, its values to the others, eight columns to a lane, KV_ROW_HEADS heads at a time.  HBM bound for many rows: 2 bytes
 // in, 1 (or 2) and the scale out a value.  What a row's heads need is asked for together, beside its slot, so that a warp has 4 KB on its way;
 // with a head to a half warp (and a 64-bit division in each) 16640 rows of 8 heads took 34 us, written, and 35, read.
-static constexpr int KV_ROW_HEADS = 8;
+static constexpr int KV_ROW_HEADS = 8, KV_FEW_ROWS = 2400;
 template <bool VEC>
 __global__ void __launch_bounds__(128)
 kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk, const uint16_t* __restrict__ v, int64_t ldv,
-                const int64_t* __restrict__ slots, int rows, int* err) {
+                const int64_t* __restrict__ slots, int rows, int each, int* err) {
     grid_dep_launch();
     grid_dep_wait();
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     if (row >= rows) return;
-    const int lane = threadIdx.x & 15;
+    const int lane = threadIdx.x & 15, from = blockIdx.y * each, heads = min(c.heads, from + each);
     const bool is_v = threadIdx.x & 16;
     const uint16_t* src = (is_v ? v + row * ldv : k + row * ldk) + lane * 8;
     uint8_t* const base = is_v ? c.v : c.k;
     float* const scales = is_v ? c.vs : c.ks;
     const int64_t slot = slots[row];
-    for (int h0 = 0; h0 < c.heads; h0 += KV_ROW_HEADS) {
+    for (int h0 = from; h0 < heads; h0 += KV_ROW_HEADS) {
         uint4 x[KV_ROW_HEADS];
 #pragma unroll
         for (int i = 0; i < KV_ROW_HEADS; ++i)
-            if (h0 + i < c.heads) x[i] = load8<VEC>(src + (h0 + i) * KV_D);
+            if (h0 + i < heads) x[i] = load8<VEC>(src + (h0 + i) * KV_D);
         const int64_t first = place(slot, c, err);
         if (first < 0) return;
 #pragma unroll
         for (int i = 0; i < KV_ROW_HEADS; ++i) {
-            if (h0 + i >= c.heads) break;
+            if (h0 + i >= heads) break;
             const int64_t at = first + (int64_t)(h0 + i) * c.page_size;
             if (type == KV_BF16) {
                 reinterpret_cast<uint4*>(base)[at * 16 + lane] = x[i];
@@ -157,25 +161,25 @@ kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk,
 template <bool VEC>
 __global__ void __launch_bounds__(128)
 kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16_t* __restrict__ v, int64_t ldv,
-               const int64_t* __restrict__ slots, int rows, int* err) {
+               const int64_t* __restrict__ slots, int rows, int each, int* err) {
     grid_dep_launch();
     grid_dep_wait();
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     if (row >= rows) return;
-    const int lane = threadIdx.x & 15;
+    const int lane = threadIdx.x & 15, from = blockIdx.y * each, heads = min(c.heads, from + each);
     const bool is_v = threadIdx.x & 16;
     uint16_t* dst = (is_v ? v + row * ldv : k + row * ldk) + lane * 8;
     const uint8_t* const base = is_v ? c.v : c.k;
     const float* const scales = is_v ? c.vs : c.ks;
     const int64_t first = place(slots[row], c, err);
-    for (int h0 = 0; h0 < c.heads; h0 += KV_ROW_HEADS) {
+    for (int h0 = from; h0 < heads; h0 += KV_ROW_HEADS) {
         uint4 x[KV_ROW_HEADS];
         float scale[KV_ROW_HEADS];
 #pragma unroll
         for (int i = 0; i < KV_ROW_HEADS; ++i) {
             x[i] = make_uint4(0, 0, 0, 0);
             scale[i] = 0.f;
-            if (h0 + i >= c.heads || first < 0) continue;
+            if (h0 + i >= heads || first < 0) continue;
             const int64_t at = first + (int64_t)(h0 + i) * c.page_size;
             if (type == KV_BF16) { x[i] = reinterpret_cast<const uint4*>(base)[at * 16 + lane]; continue; }
             const uint2 codes = reinterpret_cast<const uint2*>(base)[at * 16 + lane];
@@ -185,7 +189,7 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
         }
 #pragma unroll
         for (int i = 0; i < KV_ROW_HEADS; ++i) {
-            if (h0 + i >= c.heads) break;
+            if (h0 + i >= heads) break;
             store8<VEC>(dst + (h0 + i) * KV_D, type == KV_BF16 ? x[i] : dequantise8(make_uint2(x[i].x, x[i].y), type, scale[i]));
         }
     }
@@ -953,9 +957,10 @@ hd_status o1_kv_write(const o1_kv_cache* cache, const void* k, int64_t ldk, cons
     if (!k || !v || !slots) { set_error("kv_write: null argument"); return HD_ERR_MISSING; }
     const int64_t row = (int64_t)c.heads * KV_D;
     if (ldk < row || ldv < row) { set_error("kv_write: row pitch below %lld", (long long)row); return HD_ERR_UNSUPPORTED; }
+    const int each = rows < KV_FEW_ROWS ? 2 : KV_ROW_HEADS;
     auto kern = aligned16(k, ldk) && aligned16(v, ldv) ? kv_write_kernel<true> : kv_write_kernel<false>;
-    if (!launch_ok(launch_chained(kern, dim3((unsigned)(((int64_t)rows + 3) / 4)), dim3(128), 0, current_stream(), 1, rows, c, cache->type, (const uint16_t*)k, ldk,
-                                  (const uint16_t*)v, ldv, slots, rows, device_error_word()), "kv_write"))
+    if (!launch_ok(launch_chained(kern, dim3((unsigned)(((int64_t)rows + 3) / 4), (unsigned)((c.heads + each - 1) / each)), dim3(128), 0, current_stream(), 1, rows, c, cache->type, (const uint16_t*)k, ldk,
+                                  (const uint16_t*)v, ldv, slots, rows, each, device_error_word()), "kv_write"))
         return HD_ERR_RUNTIME;
     o1_launch_count_add(1);
     return HD_OK;
@@ -970,9 +975,10 @@ hd_status o1_kv_read(const o1_kv_cache* cache, void* k, int64_t ldk, void* v, in
     if (!k || !v || !slots) { set_error("kv_read: null argument"); return HD_ERR_MISSING; }
     const int64_t row = (int64_t)c.heads * KV_D;
     if (ldk < row || ldv < row) { set_error("kv_read: row pitch below %lld", (long long)row); return HD_ERR_UNSUPPORTED; }
+    const int each = rows < KV_FEW_ROWS ? 2 : KV_ROW_HEADS;
     auto kern = aligned16(k, ldk) && aligned16(v, ldv) ? kv_read_kernel<true> : kv_read_kernel<false>;
-    if (!launch_ok(launch_chained(kern, dim3((unsigned)(((int64_t)rows + 3) / 4)), dim3(128), 0, current_stream(), 1, rows, c, cache->type, (uint16_t*)k, ldk,
-                                  (uint16_t*)v, ldv, slots, rows, device_error_word()), "kv_read"))
+    if (!launch_ok(launch_chained(kern, dim3((unsigned)(((int64_t)rows + 3) / 4), (unsigned)((c.heads + each - 1) / each)), dim3(128), 0, current_stream(), 1, rows, c, cache->type, (uint16_t*)k, ldk,
+                                  (uint16_t*)v, ldv, slots, rows, each, device_error_word()), "kv_read"))
         return HD_ERR_RUNTIME;
     o1_launch_count_add(1);
     return HD_OK;

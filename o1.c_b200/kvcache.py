@@ -1,5 +1,5 @@
-"""Rows after a prompt: a paged cache of keys and values, the attention of new rows over it, and the residual add between
-two norms -- o1_kv_write, o1_kv_read, o1_kv_attention and o1_residual_norm on torch tensors.
+"""Rows after a prompt: a paged cache of keys and values, the attention of new rows over it, the residual add between
+two norms -- o1_kv_write, o1_kv_read, o1_kv_attention and o1_residual_norm on torch tensors -- and a Decoder that continues prompts with them.
 
 Like every entry point they enqueue on the library's current stream (use_torch_stream()) and return at once.  Arguments that
 do not fit raise O1Error; a slot, page or length that does not fit is found on the device (lib.o1_device_error() gives 70 or 71).
@@ -8,7 +8,7 @@ import ctypes as C
 
 import torch
 
-from . import HEAD_DIM, KV_HEADS, KvCacheC, O1Error, check, lib
+from . import HEAD_DIM, KV_HEADS, KvCacheC, O1Error, check, lib, ptr
 
 KINDS = {"bf16": (0, torch.bfloat16), "fp8": (1, torch.float8_e4m3fn), "int8": (2, torch.int8)}
 _BY_DTYPE = {d: n for n, d in KINDS.values()}
@@ -245,3 +245,103 @@ def _each_group(t, cols, groups):
         return t
     _need(t.numel() == cols, "residual_norm: gate, scale and shift differ in groups")
     return t.reshape(1, cols).expand(groups, cols).contiguous()
+
+
+class Decoder:
+    """Continues prompts through the decoder blocks, a row of every sequence at a time, over cached keys and values.
+
+    weights: Weights (or GgufWeights).  max_seqs sequences of at most max_tokens rows each; kind: how keys and values are kept (KvCache).
+    prompt() and step() return rows behind the final norm, [rows, hidden] bf16, and enqueue on the library's current stream."""
+
+    def __init__(self, weights, max_seqs, max_tokens, kind="bf16", page_size=64):
+        d = weights.dims
+        self.w, self.device = weights, weights.device
+        self.dims = (d["heads"], d["kv_heads"], d["hidden"], d["ff"], d["head_dim"], d["vocab"])
+        self.max_seqs, self.max_tokens, self.page_size = max_seqs, max_tokens, page_size
+        self.width = -(-max_tokens // page_size)
+        layers = weights.binding.n_layers
+        self.caches = [KvCache(max_seqs * self.width, page_size, kind, d["kv_heads"], self.device) for _ in range(layers)]
+        self._c = (KvCacheC * layers)(*[c.c for c in self.caches])
+        self._free = list(range(max_seqs * self.width - 1, -1, -1))
+        self._pages, self._len, self._table = {}, {}, {}
+        self._next = 0
+        self._scratch = {}
+
+    def _room(self, rows):
+        """Scratch for so many rows on the current stream."""
+        key = _stream()
+        s = self._scratch.get(key)
+        need = lib.o1_decode_scratch_bytes(rows, *self.dims[:5])
+        if s is None or s.numel() < need:
+            s = self._scratch[key] = torch.zeros(need, dtype=torch.uint8, device=self.device)
+        return s
+
+    def _grow(self, seq, tokens):
+        """Room for so many rows of the sequence; its pages' table on the GPU."""
+        pages = self._pages[seq]
+        if tokens > self.max_tokens:
+            raise O1Error(f"Decoder: a sequence of {tokens} rows (max_tokens is {self.max_tokens})")
+        while len(pages) * self.page_size < tokens:
+            pages.append(self._free.pop())
+            self._table[seq] = None
+        if self._table[seq] is None:
+            row = torch.zeros(self.width, dtype=torch.int32)
+            row[:len(pages)] = torch.tensor(pages, dtype=torch.int32)
+            self._table[seq] = row.to(self.device)
+
+    def prompt(self, ids):
+        """A new sequence of rows ids [n] (int64): (its name, hidden rows [n, hidden])."""
+        n = ids.numel()
+        if ids.dtype is not I64 or ids.dim() != 1 or n == 0 or not ids.is_cuda:
+            raise O1Error("Decoder.prompt: ids int64 [n] on the GPU wanted, n > 0")
+        if len(self._pages) == self.max_seqs:
+            raise O1Error(f"Decoder.prompt: {self.max_seqs} sequences are open")
+        seq = self._next
+        self._pages[seq], self._len[seq], self._table[seq] = [], 0, None
+        try:
+            self._grow(seq, n)
+        except O1Error:
+            self.close(seq)
+            raise
+        self._next += 1
+        self._len[seq] = n
+        t = torch.arange(n, device=self.device)
+        slots = self._table[seq].long()[t // self.page_size] * self.page_size + t % self.page_size
+        pos = t.float().expand(3, n).contiguous()
+        out = torch.empty(n, self.dims[2], dtype=BF16, device=self.device)
+        s = self._room(n)
+        check(lib.o1_prompt_rows(C.byref(self.w.binding), self._c, ptr(ids.contiguous()), ptr(pos), ptr(slots), ptr(s), s.numel(), ptr(out), n, *self.dims),
+              "o1_prompt_rows")
+        return seq, out
+
+    def step(self, seqs, ids):
+        """One new row of each sequence in seqs (all different), ids [len(seqs)] (int64): hidden rows [len(seqs), hidden]."""
+        n = len(seqs)
+        if ids.dtype is not I64 or ids.dim() != 1 or ids.numel() != n or not ids.is_cuda or len(set(seqs)) != n:
+            raise O1Error("Decoder.step: ids int64, one for each of different sequences, on the GPU wanted")
+        for s in seqs:
+            if s not in self._pages:
+                raise O1Error(f"Decoder.step: no sequence {s}")
+            self._grow(s, self._len[s] + 1)
+        for s in seqs:
+            self._len[s] += 1
+        lens = torch.tensor([self._len[s] for s in seqs], dtype=I32).to(self.device)
+        pages = torch.stack([self._table[s] for s in seqs]) if n else torch.zeros(0, self.width, dtype=I32, device=self.device)
+        pos = (lens - 1).float().expand(3, n).contiguous()
+        out = torch.empty(n, self.dims[2], dtype=BF16, device=self.device)
+        s = self._room(n)
+        check(lib.o1_decode_step(C.byref(self.w.binding), self._c, ptr(ids.contiguous()), ptr(pos), ptr(pages), self.width, self.width, ptr(lens), ptr(s), s.numel(),
+                                 ptr(out), n, *self.dims), "o1_decode_step")
+        return out
+
+    def rows(self, seq, layer):
+        """(keys, values) [rows, kv_heads, 128] bf16 that a layer keeps of a sequence, as KvCache.read gives them."""
+        if seq not in self._pages:
+            raise O1Error(f"Decoder.rows: no sequence {seq}")
+        t = torch.arange(self._len[seq], device=self.device)
+        return self.caches[layer].read(self._table[seq].long()[t // self.page_size] * self.page_size + t % self.page_size)
+
+    def close(self, seq):
+        """Gives a sequence's pages back.  (Calls on other streams that still read them are the caller's to wait for.)"""
+        self._free.extend(reversed(self._pages.pop(seq)))
+        del self._len[seq], self._table[seq]

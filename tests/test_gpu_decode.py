@@ -1,0 +1,179 @@
+"""Prompts and the rows after them over cached keys and values: Decoder (o1_prompt_rows, o1_decode_step) against the whole sequence, computed in 64 bits
+between the points where the decoder stores bf16 (as the oracle does), within the framework's tolerance of a block for each block (cosine >= 0.999,
+relative L2 <= 1e-2; single roundings that fall the other way make the rest of a chain differ, so blocks add)."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from test_gpu_kvcache import quantised, value
+
+gpu = pytest.mark.gpu
+DIMS = dict(hidden=512, heads=4, kv_heads=2, head_dim=128, ff=1024, vocab=1000)
+SECTION = [24, 20, 20]
+
+
+@pytest.fixture(scope="module")
+def models(pkg):
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    pkg.use_torch_stream()
+    return {n: pkg.Weights(n_layers=n, seed=5, weight_set="B", device="cuda:0", std=0.05, **DIMS) for n in (1, 3)}
+
+
+@pytest.fixture
+def weights(models):
+    return models[3]
+
+
+def r(x):
+    return x.to(torch.bfloat16).double()
+
+
+def reference(w, ids, prompt, kind):
+    """Rows behind the final norm of a text sequence, and each layer's keys and values as they are kept.  Rows from `prompt` on attend to those."""
+    d = w.dims
+
+    def t(layer, name):
+        return w.tensor(layer, name).cpu().double()
+
+    def norm(a, v):
+        return r(a / torch.sqrt((a * a).mean(-1, keepdim=True) + 1e-6) * v)
+
+    n = ids.numel()
+    half = d["head_dim"] // 2
+    freq = 5000000.0 ** (-torch.arange(half, dtype=torch.float64) * 2 / d["head_dim"])
+    ang = torch.arange(n, dtype=torch.float64)[:, None] * freq      # text rows have the same position on all three axes
+    cos, sin = (torch.cat([f(ang), f(ang)], 1)[:, None, :] for f in (torch.cos, torch.sin))
+
+    def rope(x):
+        turned = torch.cat([-x[..., half:], x[..., :half]], -1)
+        return r(r(x * cos) + r(turned * sin))
+
+    x = t(-1, "embed_tokens")[ids.cpu()]
+    mask = torch.full((n, n), -math.inf, dtype=torch.float64).triu(1)
+    kept = []
+    h = norm(x, t(0, "input_ln"))
+    for layer in range(w.n_layers):
+        q, k, v = (r(h @ t(layer, name).T).view(n, -1, d["head_dim"]) for name in ("q_proj", "k_proj", "v_proj"))
+        q, k = rope(norm(q, t(layer, "q_norm"))), rope(norm(k, t(layer, "k_norm")))
+        kept.append(tuple(value(*quantised(x_.to(torch.bfloat16), kind)) for x_ in (k, v)))
+        g = d["heads"] // d["kv_heads"]
+        parts = []
+        for rows, (k_, v_) in ((slice(0, prompt), (k, v)), (slice(prompt, n), kept[-1])):
+            z = torch.einsum("qhd,khd->hqk", q[rows], k_.repeat_interleave(g, 1)) / math.sqrt(d["head_dim"]) + mask[rows]
+            parts.append(torch.einsum("hqk,khd->qhd", torch.softmax(z, -1), v_.repeat_interleave(g, 1)).reshape(-1, g * d["kv_heads"] * d["head_dim"]))
+        a = r(torch.cat(parts))
+        y = x + r(a @ t(layer, "o_proj").T)
+        x, h = r(y), norm(y, t(layer, "post_ln"))
+        gate, up = r(h @ t(layer, "gate_proj").T), r(h @ t(layer, "up_proj").T)
+        y = x + r(r(r(gate * torch.sigmoid(gate)) * up) @ t(layer, "down_proj").T)
+        x, h = r(y), norm(y, t(layer + 1, "input_ln") if layer + 1 < w.n_layers else t(-1, "fnorm_w"))
+    return h, kept
+
+
+def near(got, want, tol):
+    got, want = got.cpu().double(), want.double()
+    rel = (got - want).norm() / want.norm()
+    cos = (got * want).sum() / (got.norm() * want.norm())
+    assert cos >= 0.999 and rel <= tol, f"cosine {cos:.6f}, relative L2 {rel:.3g}"
+
+
+def ids_of(n, seed):
+    return torch.randint(0, DIMS["vocab"], (n,), generator=torch.Generator().manual_seed(seed))
+
+
+@gpu
+@pytest.mark.parametrize("layers", [1, 3])
+@pytest.mark.parametrize("kind,tol", [("bf16", 1e-2), ("fp8", 5e-2), ("int8", 1e-2)])
+@pytest.mark.parametrize("lens,page", [([1], 16), ([5, 40, 130], 64), ([16, 17, 15, 64, 1, 2, 3, 33, 200], 16)])
+def test_prompts_and_the_rows_after_them(pkg, dev, models, layers, kind, tol, lens, page):
+    """Every step's rows beside the whole sequence's.  (A key that differs in its last bit can take another code, and e4m3's lie 2^-3 apart: its bound is wider.)"""
+    steps, weights = 5, models[layers]
+    seqs = [ids_of(n + steps, 10 * n + i) for i, n in enumerate(lens)]
+    dec = pkg.Decoder(weights, len(lens), max(lens) + steps, kind, page)
+    wants = [reference(weights, s, n, kind) for s, n in zip(seqs, lens)]
+    names = []
+    for s, n, want in zip(seqs, lens, wants):
+        name, rows = dec.prompt(s[:n].to(dev))
+        near(rows, want[0][:n], 1e-2 * layers)
+        names.append(name)
+    for i in range(steps):
+        new = torch.tensor([int(s[n + i]) for s, n in zip(seqs, lens)]).to(dev)
+        rows = dec.step(names, new)
+        near(rows, torch.stack([want[0][n + i] for n, want in zip(lens, wants)]), tol * layers)
+    for name, want in zip(names, wants):
+        for layer in range(layers):
+            k, v = dec.rows(name, layer)
+            near(k, want[1][layer][0], tol * (layer + 1))
+            near(v, want[1][layer][1], tol * (layer + 1))
+
+
+@gpu
+def test_a_row_does_not_depend_on_the_others(pkg, dev, weights):
+    """A sequence alone and among others: the same bits; pages of a closed sequence are used again."""
+    prompts = [ids_of(n, n) for n in (20, 300, 7, 64)]
+    a, b = pkg.Decoder(weights, 4, 320, "int8", 32), pkg.Decoder(weights, 1, 320, "int8", 32)
+    names = [a.prompt(p.to(dev))[0] for p in prompts]
+    a.close(names[1])
+    again, _ = a.prompt(prompts[1].to(dev))
+    names[1] = again
+    alone, _ = b.prompt(prompts[2].to(dev))
+    for i in range(4):
+        new = ids_of(4, 50 + i).to(dev)
+        together = a.step(names, new)
+        assert torch.equal(together[2:3], b.step([alone], new[2:3]))
+    assert torch.equal(a.rows(names[2], 1)[0], b.rows(alone, 1)[0])
+
+
+@gpu
+def test_arguments_that_do_not_fit(pkg, dev, weights):
+    dec = pkg.Decoder(weights, 2, 32, "bf16", 16)
+    E = pkg.O1Error
+    for bad in (torch.zeros(3, dtype=torch.int32, device=dev), torch.zeros(0, dtype=torch.int64, device=dev), torch.zeros(3, dtype=torch.int64), torch.zeros(1, 3, dtype=torch.int64, device=dev)):
+        with pytest.raises(E, match="Decoder.prompt"):
+            dec.prompt(bad)
+    with pytest.raises(E, match="max_tokens"):
+        dec.prompt(ids_of(33, 1).to(dev))
+    a, _ = dec.prompt(ids_of(32, 1).to(dev))
+    b, _ = dec.prompt(ids_of(3, 1).to(dev))
+    with pytest.raises(E, match="2 sequences are open"):
+        dec.prompt(ids_of(3, 1).to(dev))
+    with pytest.raises(E, match="max_tokens"):
+        dec.step([a], ids_of(1, 1).to(dev))
+    with pytest.raises(E, match="different"):
+        dec.step([b, b], ids_of(2, 1).to(dev))
+    with pytest.raises(E, match="no sequence"):
+        dec.step([77], ids_of(1, 1).to(dev))
+    assert dec.step([], torch.zeros(0, dtype=torch.int64, device=dev)).shape == (0, DIMS["hidden"])
+    dec.close(a)
+    dec.prompt(ids_of(32, 2).to(dev))
+
+
+def test_entry_points_refuse_before_they_touch_the_gpu(pkg):
+    lib = pkg.lib
+    one = C.c_void_p(4096)
+    blocks = (pkg.BlockBinding * 1)()
+    bw = pkg.ForwardBinding(embed_tokens=4096, fnorm_w=4096, n_layers=1, blocks=C.cast(blocks, C.POINTER(pkg.BlockBinding)))
+    cache = (pkg.KvCacheC * 1)(pkg.KvCacheC(4096, 4096, None, None, 0, 4, 16, 2, 128))
+    need = lib.o1_decode_scratch_bytes(3, 4, 2, 512, 1024, 128)
+    assert need > 0 and lib.o1_decode_scratch_bytes(3, 4, 3, 512, 1024, 128) == -1
+    # up to eight rows take the same room, beyond that it grows with the rows
+    assert lib.o1_decode_scratch_bytes(8, 4, 2, 512, 1024, 128) == need < lib.o1_decode_scratch_bytes(9, 4, 2, 512, 1024, 128)
+
+    def step(bw_=bw, caches=cache, ids=one, pos=one, pages=one, lens=one, ws=one, nb=need, out=one, batch=3, heads=4, kv=2, hidden=512, ff=1024, hd=128):
+        return lib.o1_decode_step(C.byref(bw_), caches, ids, pos, pages, 4, 4, lens, ws, nb, out, batch, heads, kv, hidden, ff, hd, 1000)
+
+    def prompt(ids=one, pos=one, slots=one, ws=one, nb=need, out=one, rows=3, hidden=512):
+        return lib.o1_prompt_rows(C.byref(bw), cache, ids, pos, slots, ws, nb, out, rows, 4, 2, hidden, 1024, 128, 1000)
+
+    for want, args in ((6, dict(caches=None)), (6, dict(ids=None)), (6, dict(pos=None)), (6, dict(pages=None)), (6, dict(lens=None)), (6, dict(ws=None)), (6, dict(out=None)),
+                       (6, dict(bw_=pkg.ForwardBinding())), (7, dict(nb=need - 1)), (9, dict(batch=-1)), (9, dict(heads=3)), (9, dict(hidden=500)), (9, dict(ff=100)), (9, dict(hd=64)),
+                       (5, dict(heads=4, kv=1))):
+        assert step(**args) == want, args
+        assert b"decode" in lib.hd_last_error(), args
+    for want, args in ((6, dict(ids=None)), (6, dict(slots=None)), (6, dict(out=None)), (7, dict(nb=5)), (9, dict(rows=-1)), (9, dict(hidden=511))):
+        assert prompt(**args) == want, args
+    assert step(batch=0) == 0 and prompt(rows=0) == 0
+    lib.hd_cuda_clear_error()
