@@ -1,4 +1,5 @@
-"""Builds libo1b200.so (the CUDA kernels + C ABI) in-tree with nvcc for sm_100a.
+"""Builds libo1b200.so (the CUDA kernels + C ABI) in-tree with nvcc for sm_100a, and _binding.so (the Python calls
+whose host time counts, on torch tensors) with g++.
 
 Run as a script or call build(); nothing is JIT-compiled at import time, so
 the built library travels with the source tree.
@@ -16,6 +17,18 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
 ]
+
+
+BINDING, BINDING_SRC = os.path.join(HERE, "_binding.so"), os.path.join(CSRC, "binding.cpp")
+
+
+def _binding_command():
+    import sysconfig
+    import torch
+    root = os.path.dirname(torch.__file__)
+    return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+            + [f"-I{d}" for d in (sysconfig.get_paths()["include"], os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"))]
+            + [BINDING_SRC, "-o", BINDING, f"-L{os.path.join(root, 'lib')}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"])
 
 
 def _nvcc():
@@ -47,6 +60,8 @@ def build(verbose=False, force=False):
         if force or _stale(o, [s] + headers):
             cmd = [nvcc] + NVCC_FLAGS + extra + (["-Xptxas", "-v"] if verbose else []) + ["-c", s, "-o", o]
             procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    if force or _stale(BINDING, [BINDING_SRC, headers[-1]]):
+        procs.append(("binding.cpp", subprocess.Popen(_binding_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     failed = False
     for src, p in procs:
         out, _ = p.communicate()

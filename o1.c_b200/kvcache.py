@@ -6,32 +6,27 @@ do not fit raise O1Error; a slot, page or length that does not fit is found on t
 """
 import ctypes as C
 
+import os
+
 import torch
 
-from . import HEAD_DIM, KV_HEADS, KvCacheC, O1Error, check, lib, ptr
+_BINDING = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_binding.so")
+if not os.path.exists(_BINDING):
+    raise ImportError(f"{_BINDING} is missing: build it with `python o1.c_b200/build.py`. There is no fallback path.")
+
+from . import _binding  # noqa: E402
+from . import HEAD_DIM, KV_HEADS, KvCacheC, O1Error, check, lib, ptr  # noqa: E402
 
 KINDS = {"bf16": (0, torch.bfloat16), "fp8": (1, torch.float8_e4m3fn), "int8": (2, torch.int8)}
 _BY_DTYPE = {d: n for n, d in KINDS.values()}
 BF16, I32, I64, F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
-SCALE = HEAD_DIM ** -0.5
-_write, _read, _attend, _norm, _stream = lib.o1_kv_write, lib.o1_kv_read, lib.o1_kv_attention, lib.o1_residual_norm, lib.o1_get_stream
+_stream = lib.o1_get_stream
+_binding.setup(*(C.cast(f, C.c_void_p).value for f in (lib.o1_kv_write, lib.o1_kv_read, lib.o1_kv_attention, lib.o1_residual_norm, lib.o1_get_stream)), O1Error, check)
 
 
 def _need(ok, what):
     if not ok:
         raise O1Error(what)
-
-
-def _rows(t, heads, what):
-    """Rows and row pitch of bf16 rows [n, heads, 128] whose heads lie side by side.  (Short on purpose: for a few rows a call is bound by its checks.)"""
-    shape = t.shape
-    if t.dtype is not BF16 or len(shape) != 3 or shape[1] != heads or shape[2] != HEAD_DIM:
-        raise O1Error(f"{what}: bf16 [rows, {heads}, {HEAD_DIM}] wanted, got {t.dtype} {tuple(shape)}")
-    ld, hs, cs = t.stride()
-    if cs != 1 or (hs != HEAD_DIM and heads > 1) or not t.is_cuda:
-        raise O1Error(f"{what}: a CUDA tensor with a row's heads side by side wanted, got strides {t.stride()}")
-    n = shape[0]
-    return n, (ld if n > 1 else heads * HEAD_DIM)
 
 
 class KvCache:
@@ -73,51 +68,23 @@ class KvCache:
         self.device = k.device
         p = [t.data_ptr() for t in tensors] + ([] if kind else [None, None])
         self.c = KvCacheC(*p, kind, self.pages, self.page_size, self.kv_heads, HEAD_DIM)
-        self._ref = C.byref(self.c)
+        self._h = _binding.handle(C.addressof(self.c), self.kv_heads, k.get_device())
         self._work = {}
-
-    def _slots(self, slots, what):
-        shape = slots.shape
-        if slots.dtype is not I64 or len(shape) != 1 or not slots.is_contiguous() or slots.device != self.device:
-            raise O1Error(f"{what}: slots int64 [rows], contiguous, on the cache's GPU wanted")
-        return shape[0]
 
     def write(self, k, v, slots):
         """Rows k, v [n, kv_heads, 128] bf16 into slots [n] (int64, all different; negative: left out), quantised on the way."""
-        n = self._slots(slots, "KvCache.write")
-        nk, ldk = _rows(k, self.kv_heads, "KvCache.write: k")
-        nv, ldv = _rows(v, self.kv_heads, "KvCache.write: v")
-        if nk != n or nv != n:
-            raise O1Error("KvCache.write: k, v and slots differ in rows")
-        rc = _write(self._ref, k.data_ptr(), ldk, v.data_ptr(), ldv, slots.data_ptr(), n)
-        if rc:
-            check(rc, "o1_kv_write")
+        _binding.write(self._h, k, v, slots)
 
-    def read(self, slots, out=None):
+    def read(self, slots, out=(None, None)):
         """(k, v) [n, kv_heads, 128] bf16 of slots [n]; zeros where a slot is negative.  out: a pair of tensors to fill, rows of any pitch."""
-        n = self._slots(slots, "KvCache.read")
-        if out is None:
-            k = torch.empty(n, self.kv_heads, HEAD_DIM, dtype=BF16, device=self.device)
-            v = torch.empty_like(k)
-            ldk = ldv = self.kv_heads * HEAD_DIM
-        else:
-            k, v = out
-            nk, ldk = _rows(k, self.kv_heads, "KvCache.read: k")
-            nv, ldv = _rows(v, self.kv_heads, "KvCache.read: v")
-            if nk != n or nv != n:
-                raise O1Error("KvCache.read: out and slots differ in rows")
-        rc = _read(self._ref, k.data_ptr(), ldk, v.data_ptr(), ldv, slots.data_ptr(), n)
-        if rc:
-            check(rc, "o1_kv_read")
-        return k, v
+        return _binding.read(self._h, slots, *out)
 
     def _workspace(self, heads):
         """Scratch of attend(), its address and bytes: one for each stream the calls run on, as calls that overlap must not share it."""
         need = lib.o1_kv_attention_workspace_bytes(heads, self.kv_heads)
         _need(need >= 0, f"KvCache.attend: heads {heads} (a multiple of kv_heads {self.kv_heads})")
-        t = torch.zeros(need, dtype=torch.uint8, device=self.device)
-        w = self._work[_stream(), heads] = (t.data_ptr(), need, t)
-        return w
+        t = self._work[_stream(), heads] = torch.zeros(need, dtype=torch.uint8, device=self.device)
+        return t.data_ptr(), need
 
     def attend(self, q, pages, lens, k=None, v=None, out=None, lse=None, scale=None):
         """Attention of one new row per sequence, q [batch, heads, 128] bf16, over its first lens[b] cached rows.
@@ -126,51 +93,7 @@ class KvCache:
         k, v [batch, kv_heads, 128]: each sequence's row at position lens[b] - 1, stored into the cache and attended to.
         Returns out [batch, heads, 128] bf16, with lse=True (or a tensor [batch, heads] fp32) a pair (out, log-sum-exp).  An empty sequence
         gives zeros and -inf.  scale: 1 / sqrt(128)."""
-        shape = q.shape
-        if len(shape) != 3:
-            raise O1Error("KvCache.attend: q [batch, heads, 128] wanted")
-        heads = shape[1]
-        n, ldq = _rows(q, heads, "KvCache.attend: q")
-        shape = pages.shape
-        if pages.dtype is not I32 or len(shape) != 2 or shape[0] != n or pages.device != self.device:
-            raise O1Error("KvCache.attend: pages int32 [batch, width] on the cache's GPU wanted")
-        width = shape[1]
-        ldp, cs = pages.stride()
-        if cs != 1 and width > 1:
-            raise O1Error("KvCache.attend: the pages of a sequence must lie side by side")
-        shape = lens.shape
-        if lens.dtype is not I32 or len(shape) != 1 or shape[0] != n or not lens.is_contiguous() or lens.device != self.device:
-            raise O1Error("KvCache.attend: lens int32 [batch] on the cache's GPU wanted")
-        pk = pv = pl = None
-        ldk = ldv = 0
-        if k is not None and v is not None:
-            nk, ldk = _rows(k, self.kv_heads, "KvCache.attend: k")
-            nv, ldv = _rows(v, self.kv_heads, "KvCache.attend: v")
-            if nk != n or nv != n:
-                raise O1Error("KvCache.attend: k, v and q differ in rows")
-            pk, pv = k.data_ptr(), v.data_ptr()
-        elif k is not None or v is not None:
-            raise O1Error("KvCache.attend: k and v [batch, kv_heads, 128], both or neither")
-        if out is None:
-            out = torch.empty_like(q)
-            ldo = out.stride()[0] if n > 1 else heads * HEAD_DIM
-        else:
-            no, ldo = _rows(out, heads, "KvCache.attend: out")
-            if no != n:
-                raise O1Error("KvCache.attend: out and q differ in rows")
-        if lse is True:
-            lse = torch.empty(n, heads, dtype=F32, device=self.device)
-            pl = lse.data_ptr()
-        elif lse is not None and lse is not False:
-            if lse.dtype is not F32 or tuple(lse.shape) != (n, heads) or not lse.is_contiguous() or not lse.is_cuda:
-                raise O1Error("KvCache.attend: lse fp32 [batch, heads] wanted")
-            pl = lse.data_ptr()
-        w = self._work.get((_stream(), heads)) or self._workspace(heads)
-        rc = _attend(self._ref, q.data_ptr(), ldq, pk, ldk, pv, ldv, pages.data_ptr(), ldp if n > 1 else width, width, lens.data_ptr(),
-                     out.data_ptr(), ldo, pl, n, heads, SCALE if scale is None else scale, w[0], w[1])
-        if rc:
-            check(rc, "o1_kv_attention")
-        return out if pl is None else (out, lse)
+        return _binding.attend(self._h, self, q, pages, lens, k, v, out, lse, scale)
 
 
 def residual_norm(x, branch, pre_w, post_w=None, gate=None, scale=None, shift=None, alpha=1.0, eps=1e-6, y=None, h=None):
@@ -178,73 +101,7 @@ def residual_norm(x, branch, pre_w, post_w=None, gate=None, scale=None, shift=No
 
     x, branch [rows, cols] bf16 with rows of any pitch; the weights [cols]; gate, scale, shift [cols] or [groups, cols], a vector for each
     rows / groups rows.  pre_w None: no norm behind the sum, h is None.  y, h: tensors to fill (y may be x or branch)."""
-    shape = x.shape
-    if x.dtype is not BF16 or branch.dtype is not BF16 or len(shape) != 2 or branch.shape != shape or not x.is_cuda or not branch.is_cuda:
-        raise O1Error("residual_norm: x and branch bf16 [rows, cols] on the GPU wanted")
-    rows, cols = shape
-    p_post = p_pre = p_gate = p_scale = p_shift = p_h = None
-    groups, ldh = 1, 0
-    if post_w is not None:
-        _vector(post_w, cols, 1, "post_w")
-        p_post = post_w.data_ptr()
-    if gate is not None:
-        groups = _vector(gate, cols, 2, "gate")
-    if scale is not None:
-        g = _vector(scale, cols, 2, "scale")
-        groups = g if groups == 1 else groups
-        _need(shift is not None, "residual_norm: scale without shift")
-    if shift is not None:
-        g = _vector(shift, cols, 2, "shift")
-        groups = g if groups == 1 else groups
-    if groups > 1:
-        gate, scale, shift = (_each_group(t, cols, groups) for t in (gate, scale, shift))
-    if gate is not None:
-        p_gate = gate.data_ptr()
-    if scale is not None:
-        p_scale = scale.data_ptr()
-    if shift is not None:
-        p_shift = shift.data_ptr()
-    if y is None:
-        y = torch.empty_like(x)
-    elif y.dtype is not BF16 or y.shape != shape or not y.is_cuda:
-        raise O1Error("residual_norm: y bf16 [rows, cols] wanted")
-    if pre_w is not None:
-        _vector(pre_w, cols, 1, "pre_w")
-        p_pre = pre_w.data_ptr()
-        if h is None:
-            h = torch.empty_like(x)
-        elif h.dtype is not BF16 or h.shape != shape or not h.is_cuda:
-            raise O1Error("residual_norm: h bf16 [rows, cols] wanted")
-        ldh, ch = h.stride()
-        p_h = h.data_ptr()
-    elif h is not None:
-        raise O1Error("residual_norm: h without pre_w")
-    else:
-        ch = 1
-    (ldx, cx), (ldb, cb), (ldy, cy) = x.stride(), branch.stride(), y.stride()
-    if not cx == cb == cy == ch == 1 and cols > 1:
-        raise O1Error("residual_norm: the values of a row must lie side by side")
-    if rows == 1 or cols == 1:
-        ldx, ldb, ldy, ldh = (max(ld, cols) for ld in (ldx, ldb, ldy, ldh))
-    rc = _norm(x.data_ptr(), ldx, branch.data_ptr(), ldb, p_post, p_gate, alpha, p_pre, p_scale, p_shift, groups, y.data_ptr(), ldy, p_h, ldh, rows, cols, eps)
-    if rc:
-        check(rc, "o1_residual_norm")
-    return y, h
-
-
-def _vector(t, cols, dims, name):
-    """The number of vectors [cols] in t."""
-    shape = t.shape
-    if t.dtype is not BF16 or not 0 < len(shape) <= dims or shape[-1] != cols or not t.is_contiguous() or not t.is_cuda or shape[0] == 0:
-        raise O1Error(f"residual_norm: {name} bf16 [{'groups, ' if dims > 1 else ''}{cols}] wanted")
-    return shape[0] if len(shape) == 2 else 1
-
-
-def _each_group(t, cols, groups):
-    if t is None or t.numel() == groups * cols:
-        return t
-    _need(t.numel() == cols, "residual_norm: gate, scale and shift differ in groups")
-    return t.reshape(1, cols).expand(groups, cols).contiguous()
+    return _binding.residual_norm(x, branch, pre_w, post_w, gate, scale, shift, alpha, eps, y, h)
 
 
 class Decoder:
