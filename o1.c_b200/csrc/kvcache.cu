@@ -328,11 +328,13 @@ struct KvKernel {
     static constexpr int TEAMS = HG == 1 ? 3 : 2, WARPS = KV_TEAM * TEAMS, STAGES = HG == 1 ? 2 : 3, THREADS = (WARPS + TEAMS) * 32;      // (as registers and shared memory allow)
     // shared memory: the rings, their scales, the teams' join buffers, then Shared
     static constexpr int SCALES = WARPS * STAGES * KV_STAGE_BYTES, JOIN = SCALES + (TYPE == KV_BF16 ? 0 : WARPS * STAGES * 256), SHARED = JOIN + TEAMS * KV_JOIN_BYTES;
+    struct Share { int first, here, fan, item, groups, head0, heads; };        // a part's group begins at part `first` and has `here`, its item at part `item`
     struct Segment { int b, item, first, begin, end, n; };        // first: the item's first chunk; begin ... end - 1: the team's
     struct Shared {
         uint64_t full[WARPS][STAGES], empty[WARPS][STAGES];
         Segment seg[TEAMS][2], part[TEAMS][2];
-        int prefix[KV_SEQS + 1], cost[KV_SEQS], len[KV_SEQS], parts[TEAMS], last[TEAMS];      // chunks and costs before a sequence
+        Share share[TEAMS][2];
+        int prefix[KV_SEQS + 1], cost[KV_SEQS], len[KV_SEQS], parts[TEAMS], last[TEAMS][2];      // chunks and costs before a sequence
         int2 scan[WARPS + TEAMS];
         float m[TEAMS][KV_TEAM][8 * HG], l[TEAMS][KV_TEAM][8 * HG];
     };
@@ -395,45 +397,54 @@ __device__ __forceinline__ void store_row4(uint16_t* dst, const float4& v, float
     dst[0] = (uint16_t)r.x; dst[1] = (uint16_t)(r.x >> 16); dst[2] = (uint16_t)r.y; dst[3] = (uint16_t)(r.y >> 16);
 }
 
-// Sums of `count` parts, the first one `first`, the others in slot 0 of every `stride`-th team behind it, a head to a warp: into the result, or
+// Whether this thread is the last of `wanted` to come, each with what its team has written before a barrier; the counter is then as it was.
+__device__ __forceinline__ bool all_came(unsigned* counter, int wanted) {
+    unsigned seen;
+    asm volatile("fence.acq_rel.gpu;" ::: "memory");
+    asm volatile("atom.relaxed.gpu.global.add.u32 %0, [%1], 1;" : "=r"(seen) : "l"(counter) : "memory");
+    if (seen != (unsigned)(wanted - 1)) return false;
+    asm volatile("fence.acq_rel.gpu;" ::: "memory");
+    *counter = 0;
+    return true;
+}
+
+// The sums of `count` parts of one head, by a warp: the first one `first`, the others in slot 0 of every `stride`-th team behind it.  Into the result, or
 // (to_out false) into the first one's place.
-__device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, int count, int b, int head0, int heads, bool to_out) {
+__device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, int count, int b, int head, int out_head, bool to_out) {
     const int lane = threadIdx.x & 31;
     auto place = [&](int i) { return (int64_t)(i == 0 ? first : (first & ~1) + 2 * stride * i) * a.per_item; };
-    for (int head = (threadIdx.x >> 5) & (KV_TEAM - 1); head < heads; head += KV_TEAM) {
-        float top = -INFINITY, sum = 0.f;
-        float4 r = make_float4(0, 0, 0, 0);
+    float top = -INFINITY, sum = 0.f;
+    float4 r = make_float4(0, 0, 0, 0);
 #pragma unroll 1
-        for (int i0 = 0; i0 < count; i0 += 16) {      // all that 16 parts need is asked for at once
-            float4 x[16];
-            float2 s = make_float2(-INFINITY, 0.f);
-            if (lane < 16 && i0 + lane < count) s = __ldcg(&a.stats[place(i0 + lane) + head]);
+    for (int i0 = 0; i0 < count; i0 += 16) {      // all that 16 parts need is asked for at once
+        float4 x[16];
+        float2 s = make_float2(-INFINITY, 0.f);
+        if (lane < 16 && i0 + lane < count) s = __ldcg(&a.stats[place(i0 + lane) + head]);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (i0 + i < count) x[i] = __ldcg(reinterpret_cast<const float4*>(a.parts + (place(i0 + i) + head) * KV_D) + lane);
-            float here = s.x;
+        for (int i = 0; i < 16; ++i)
+            if (i0 + i < count) x[i] = __ldcg(reinterpret_cast<const float4*>(a.parts + (place(i0 + i) + head) * KV_D) + lane);
+        float here = s.x;
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, o));
-            const float m = fmaxf(top, __shfl_sync(0xffffffffu, here, 0)), ref = m == -INFINITY ? 0.f : m, old = exp2_fast(top - ref), w = exp2_fast(s.x - ref);
-            top = m;
-            sum = sum * old + s.y * w;
-            r.x *= old; r.y *= old; r.z *= old; r.w *= old;
+        for (int o = 8; o > 0; o >>= 1) here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, o));
+        const float m = fmaxf(top, __shfl_sync(0xffffffffu, here, 0)), ref = m == -INFINITY ? 0.f : m, old = exp2_fast(top - ref), w = exp2_fast(s.x - ref);
+        top = m;
+        sum = sum * old + s.y * w;
+        r.x *= old; r.y *= old; r.z *= old; r.w *= old;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float f = __shfl_sync(0xffffffffu, w, i);
-                if (i0 + i < count) { r.x += x[i].x * f; r.y += x[i].y * f; r.z += x[i].z * f; r.w += x[i].w * f; }
-            }
+        for (int i = 0; i < 16; ++i) {
+            const float f = __shfl_sync(0xffffffffu, w, i);
+            if (i0 + i < count) { r.x += x[i].x * f; r.y += x[i].y * f; r.z += x[i].z * f; r.w += x[i].w * f; }
         }
+    }
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        sum = __shfl_sync(0xffffffffu, sum, 0);
-        if (to_out) {
-            store_row4(a.out + b * a.ldo + (head0 + head) * KV_D + lane * 4, r, 1.0f / sum, a.flags & 2);
-            if (a.lse && lane == 0) a.lse[(int64_t)b * a.heads + head0 + head] = (top - KV_LIFT + log2f(sum)) * 0.6931471805599453f;
-        } else {
-            reinterpret_cast<float4*>(a.parts + (place(0) + head) * KV_D)[lane] = r;
-            if (lane == 0) a.stats[place(0) + head] = make_float2(top, sum);
-        }
+    for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    sum = __shfl_sync(0xffffffffu, sum, 0);
+    if (to_out) {
+        store_row4(a.out + b * a.ldo + out_head * KV_D + lane * 4, r, 1.0f / sum, a.flags & 2);
+        if (a.lse && lane == 0) a.lse[(int64_t)b * a.heads + out_head] = (top - KV_LIFT + log2f(sum)) * 0.6931471805599453f;
+    } else {
+        reinterpret_cast<float4*>(a.parts + (place(0) + head) * KV_D)[lane] = r;
+        if (lane == 0) a.stats[place(0) + head] = make_float2(top, sum);
     }
 }
 
@@ -451,6 +462,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         fence_mbar_init();
     }
     if (tid < K::TEAMS) sh.parts[tid] = 0;
+    if (warp >= WARPS && elect_one()) { tma_prefetch_desc(&k_map); tma_prefetch_desc(&v_map); }
     grid_dep_launch();
     grid_dep_wait();
 
@@ -472,9 +484,11 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     }
     // ---- a team's part of the stream: equal costs, where each item costs some chunks more than it has; ends inside an item that is not worth a join are moved
     const int teams = min((int)gridDim.x * K::TEAMS, (total + KV_TEAM - 1) / KV_TEAM), share = teams > 0 ? total / teams : 0, keep = share <= 8 ? 24 : max(8, share >> 2);
+    const int each = teams > 0 ? cost / teams : 0, over = cost - each * teams;
+    auto cost_of = [&](int id) { return each * id + over * id / teams; };         // cost * id / teams, in 32 bits (over and id are below 480)
     auto begin_of = [&](int id) {
         if (id >= teams) return total;
-        const int at = (int)((int64_t)cost * id / teams);
+        const int at = cost_of(id);
         int lo = 0, hi = a.batch - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
@@ -485,13 +499,19 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         if (n <= keep) c = 2 * c < n ? 0 : n;
         return sh.prefix[lo] * items + item * n + c;
     };
+    auto part_of = [&](int id, int lane, int& c0, int& c1) {        // both ends at once
+        const int at = begin_of(id + (lane & 1));
+        c0 = __shfl_sync(0xffffffffu, at, 0);
+        c1 = __shfl_sync(0xffffffffu, at, 1);
+    };
 
     if (warp >= WARPS) {
         // ---- the team's loading warp
         const int team = warp - WARPS, id = team * gridDim.x + blockIdx.x;
-        if (id >= teams) return;
-        const int c1 = lane < KV_TEAM ? begin_of(id + 1) : 0;
-        int f = lane < KV_TEAM ? begin_of(id) + lane : 0, place[2] = {-1, -1};
+        int f, c1, place[2] = {-1, -1};
+        part_of(id, lane, f, c1);
+        f += lane;
+        if (lane >= KV_TEAM) c1 = 0;
         KvWalk at = {};
         auto look = [&]() {        // the chunk's rows of the cache, 16 at a time; -1: none
             const int tok = at.c * KEYS, len = sh.len[at.b], head = a.chunks_of_heads == 1 ? at.item : at.item / a.chunks_of_heads;
@@ -562,7 +582,8 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         for (int i = mate * 32 + lane; i < a.heads * KV_D; i += KV_TEAM * 32) a.out[b * a.ldo + i] = 0;
         if (a.lse) for (int i = mate * 32 + lane; i < a.heads; i += KV_TEAM * 32) a.lse[(int64_t)b * a.heads + i] = -INFINITY;
     }
-    const int c0 = begin_of(id), c1 = begin_of(id + 1);
+    int c0, c1;
+    part_of(id, lane, c0, c1);
     if (c0 >= c1) return;
 
     auto head_of = [&](int item) {         // the first query head of an item
@@ -721,14 +742,11 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 #pragma unroll
                 for (int n = 0; n < TILES; ++n) {
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        s[n][2 * h + j] *= z_scale[h];
-                        top = fmaxf(top, s[n][2 * h + j]);
-                    }
+                    for (int j = 0; j < 2; ++j) top = fmaxf(top, s[n][2 * h + j]);
                 }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float m_new = fmaxf(m[h], top), ref = (m_new == -INFINITY ? 0.f : m_new) - KV_LIFT;
+                const float m_new = fmaxf(m[h], top * z_scale[h]), ref = (m_new == -INFINITY ? 0.f : m_new) - KV_LIFT;
                 alpha[h] = exp2_fast(m[h] - KV_LIFT - ref);
                 moved = moved || alpha[h] != 1.f;
                 m[h] = m_new;
@@ -736,7 +754,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 #pragma unroll
                 for (int n = 0; n < TILES; ++n) {
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) { s[n][2 * h + j] = exp2_fast(s[n][2 * h + j] - ref); sum += s[n][2 * h + j]; }
+                    for (int j = 0; j < 2; ++j) { s[n][2 * h + j] = exp2_fast(__fmaf_rn(s[n][2 * h + j], z_scale[h], -ref)); sum += s[n][2 * h + j]; }
                 }
                 l[h] = l[h] * alpha[h] + sum;
                 if (TYPE != KV_BF16) {
@@ -867,43 +885,46 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         }
         if (seg.end == c1) break;
     }
-    // ---- items that the team shares with others
+    // ---- items that the team shares with others, the first and the last of its part: it is known for both at once whether all have come
     team_sync(team);
-    auto come = [&](unsigned* counter, int wanted) {      // whether this team is the last one to come
-        if (mate == 0 && lane == 0) {
-            __threadfence();
-            const bool last = atomicAdd(counter, 1u) == (unsigned)(wanted - 1);
-            __threadfence();
-            if (last) *counter = 0;
-            sh.last[team] = last;
-        }
-        team_sync(team);
-        const bool last = sh.last[team];
-        team_sync(team);
-        return last;
-    };
-#pragma unroll 1
-    for (int i = 0; i < sh.parts[team]; ++i) {
-        const typename K::Segment seg = sh.part[team][i];
+    const int parts = sh.parts[team];
+    if (parts == 0) return;
+    if (mate == 0 && lane < parts) {
         // teams from ... to share the item, in groups of `fan`; the first one's part is in slot `late`
-        const int64_t at = (int64_t)sh.cost[seg.b] * items + (int64_t)seg.item * (seg.n + KV_ITEM_COST);
-        const int from = (int)(((at + 1) * teams - 1) / cost), to = (int)(((at + seg.n) * teams - 1) / cost);
-        const int late = seg.first != begin_of(from), count = to - from + 1;
-        const int fan = count <= KV_FLAT ? count : (int)ceilf(sqrtf((float)count)), groups = (count + fan - 1) / fan;
-        const int mine = (id - from) / fan, first = 2 * (from + mine * fan) + (mine == 0 ? late : 0), here = min(fan, count - mine * fan);
-        bool last = come(a.arrived + first, here), done = false;
-        int j_first = first, j_stride = 1, j_count = here;
+        const typename K::Segment& seg = sh.part[team][lane];
+        const int at = sh.cost[seg.b] * items + seg.item * (seg.n + KV_ITEM_COST);
+        auto owner = [&](int v) {
+            int o = min(teams - 1, (int)((float)v * ((float)teams / (float)cost)));
+            while (cost_of(o) > v) --o;
+            while (o + 1 < teams && cost_of(o + 1) <= v) ++o;
+            return o;
+        };
+        const int from = owner(at), to = owner(at + seg.n - 1), late = seg.first != begin_of(from), count = to - from + 1;
+        const int fan = count <= KV_FLAT ? count : (int)ceilf(sqrtf((float)count)), mine = (id - from) / fan, first = 2 * (from + mine * fan) + (mine == 0 ? late : 0);
+        const int here = min(fan, count - mine * fan);
+        sh.share[team][lane] = {first, here, fan, 2 * from + late, (count + fan - 1) / fan, head_of(seg.item), heads_of(seg.item)};
+        sh.last[team][lane] = all_came(a.arrived + first, here);
+    }
+    team_sync(team);
 #pragma unroll 1
-        while (last && !done) {
-            done = groups == 1 || j_stride > 1;
-            kv_join(a, j_first, j_stride, j_count, seg.b, head_of(seg.item), heads_of(seg.item), done);
-            if (done) break;
-            team_sync(team);
-            last = come(a.arrived + 2 * KV_TEAMS_MAX + 2 * from + late, groups);
-            j_first = 2 * from + late;
-            j_stride = fan;
-            j_count = groups;
+    for (int level = 0; level < 2; ++level) {
+        int done = 0, again = 0;         // heads to join before this part's
+#pragma unroll 1
+        for (int i = 0; i < parts; ++i) {
+            if (!sh.last[team][i]) continue;
+            const typename K::Share s = sh.share[team][i];
+            again |= level == 0 && s.groups > 1;
+            for (int head = (mate - done) & (KV_TEAM - 1); head < s.heads; head += KV_TEAM)
+                kv_join(a, level ? s.item : s.first, level ? s.fan : 1, level ? s.groups : s.here, sh.part[team][i].b, head, s.head0 + head, level || s.groups == 1);
+            done += s.heads;
         }
+        if (!again) break;
+        team_sync(team);
+        if (mate == 0 && lane < parts && sh.last[team][lane]) {       // the groups of an item
+            const typename K::Share& s = sh.share[team][lane];
+            sh.last[team][lane] = s.groups > 1 && all_came(a.arrived + 2 * KV_TEAMS_MAX + s.item, s.groups);
+        }
+        team_sync(team);
     }
 }
 
