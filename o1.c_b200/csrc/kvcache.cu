@@ -219,12 +219,9 @@ static constexpr int KV_STAGE_BYTES = 8192;            // keys and values of a c
 static constexpr int KV_SEQS = 256;                    // sequences of a launch
 static constexpr int KV_TEAM = 4;                      // warps
 static constexpr int KV_TEAMS_MAX = 160 * 3;           // what the workspace has room for
-#ifndef KVOV
-#define KVOV 4
-#define KVFL 32
-#endif
-static constexpr int KV_FLAT = KVFL;                   // so many teams' parts are joined at once, more in groups
-static constexpr int KV_ITEM_COST = KVOV;              // what an item costs a team beside its chunks, in chunks
+static constexpr int KV_FLAT = 32, KV_FAN = 16;          // up to so many teams' parts are joined at once, more in groups of so many
+static constexpr int KV_ITEM_COST = 7;                 // what an item costs a team beside its chunks, in chunks
+static constexpr int KV_KEEP = 16;                     // items of so few chunks are not cut
 static constexpr int KV_JOIN_BYTES = 8192;             // of a team
 static constexpr int ERR_KV_WAIT = 72;                 // a wait of the attention kernel ran out
 static constexpr float KV_LIFT = 20.0f;                // probabilities are relative to 2^-20 of the largest: those that fp32 has no value for are 2^-146 and less of it
@@ -468,7 +465,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 
     // ---- the lengths, as numbers of chunks, summed up
     const int ps = a.c.page_size, shift = a.c.page_shift, items = a.c.heads * a.chunks_of_heads;
-    int total, cost;
+    int total, cost, all_chunks, sequences;
     {
         static_assert(KV_SEQS <= K::THREADS, "a sequence to a thread");
         int len = tid < a.batch ? a.lens[tid] : 0;
@@ -478,12 +475,15 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         const int2 before = block_scan<WARPS + K::TEAMS>(make_int2(n, n > 0 ? n + KV_ITEM_COST : 0), all, sh.scan);
         if (tid < a.batch) { sh.prefix[tid] = before.x; sh.cost[tid] = before.y; sh.len[tid] = len; }
         if (tid == 0) sh.prefix[a.batch] = all.x;
+        all_chunks = all.x;
+        sequences = (all.y - all.x) / KV_ITEM_COST;      // that are not empty
         total = all.x * items;
         cost = all.y * items;
         __syncthreads();
     }
     // ---- a team's part of the stream: equal costs, where each item costs some chunks more than it has; ends inside an item that is not worth a join are moved
-    const int teams = min((int)gridDim.x * K::TEAMS, (total + KV_TEAM - 1) / KV_TEAM), share = teams > 0 ? total / teams : 0, keep = share <= 8 ? 24 : max(8, share >> 2);
+    const int least = all_chunks > 32 * sequences ? 2 * KV_TEAM : KV_TEAM, teams = min((int)gridDim.x * K::TEAMS, (total + least - 1) / least);
+    const int share = teams > 0 ? total / teams : 0, keep = max(KV_KEEP, share >> 2);
     const int each = teams > 0 ? cost / teams : 0, over = cost - each * teams;
     auto cost_of = [&](int id) { return each * id + over * id / teams; };         // cost * id / teams, in 32 bits (over and id are below 480)
     auto begin_of = [&](int id) {
@@ -900,7 +900,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             return o;
         };
         const int from = owner(at), to = owner(at + seg.n - 1), late = seg.first != begin_of(from), count = to - from + 1;
-        const int fan = count <= KV_FLAT ? count : (int)ceilf(sqrtf((float)count)), mine = (id - from) / fan, first = 2 * (from + mine * fan) + (mine == 0 ? late : 0);
+        const int fan = count <= KV_FLAT ? count : KV_FAN, mine = (id - from) / fan, first = 2 * (from + mine * fan) + (mine == 0 ? late : 0);
         const int here = min(fan, count - mine * fan);
         sh.share[team][lane] = {first, here, fan, 2 * from + late, (count + fan - 1) / fan, head_of(seg.item), heads_of(seg.item)};
         sh.last[team][lane] = all_came(a.arrived + first, here);
