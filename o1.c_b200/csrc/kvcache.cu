@@ -220,9 +220,10 @@ static constexpr int KV_SEQS = 256;                    // sequences of a launch
 static constexpr int KV_TEAM = 4;                      // warps
 static constexpr int KV_TEAMS_MAX = 160 * 3;           // what the workspace has room for
 static constexpr int KV_FLAT = 32, KV_FAN = 16;          // up to so many teams' parts are joined at once, more in groups of so many
-static constexpr int KV_ITEM_COST = 7;                 // what an item costs a team beside its chunks, in chunks
+static constexpr int KV_ITEM_COST = 10;                // what an item costs a team beside its chunks, in chunks
 static constexpr int KV_KEEP = 16;                     // items of so few chunks are not cut
 static constexpr int KV_JOIN_BYTES = 8192;             // of a team
+static constexpr int KV_JOIN_STEP = 4;                 // parts that a join has under way
 static constexpr int ERR_KV_WAIT = 72;                 // a wait of the attention kernel ran out
 static constexpr float KV_LIFT = 20.0f;                // probabilities are relative to 2^-20 of the largest: those that fp32 has no value for are 2^-146 and less of it
 
@@ -325,13 +326,13 @@ struct KvKernel {
     static constexpr int TEAMS = HG == 1 ? 3 : 2, WARPS = KV_TEAM * TEAMS, STAGES = HG == 1 ? 2 : 3, THREADS = (WARPS + TEAMS) * 32;      // (as registers and shared memory allow)
     // shared memory: the rings, their scales, the teams' join buffers, then Shared
     static constexpr int SCALES = WARPS * STAGES * KV_STAGE_BYTES, JOIN = SCALES + (TYPE == KV_BF16 ? 0 : WARPS * STAGES * 256), SHARED = JOIN + TEAMS * KV_JOIN_BYTES;
-    struct Share { int first, here, fan, item, groups, head0, heads; };        // a part's group begins at part `first` and has `here`, its item at part `item`
+    struct Share { int first, here, fan, item, groups, b, head0, heads; };        // a part's group begins at part `first` and has `here` (0: no part), its item at part `item`
     struct Segment { int b, item, first, begin, end, n; };        // first: the item's first chunk; begin ... end - 1: the team's
     struct Shared {
         uint64_t full[WARPS][STAGES], empty[WARPS][STAGES];
-        Segment seg[TEAMS][2], part[TEAMS][2];
+        Segment seg[TEAMS][2];
         Share share[TEAMS][2];
-        int prefix[KV_SEQS + 1], cost[KV_SEQS], len[KV_SEQS], parts[TEAMS], last[TEAMS][2];      // chunks and costs before a sequence
+        int prefix[KV_SEQS + 1], cost[KV_SEQS], len[KV_SEQS], last[TEAMS][2];      // chunks and costs before a sequence
         int2 scan[WARPS + TEAMS];
         float m[TEAMS][KV_TEAM][8 * HG], l[TEAMS][KV_TEAM][8 * HG];
     };
@@ -405,43 +406,70 @@ __device__ __forceinline__ bool all_came(unsigned* counter, int wanted) {
     return true;
 }
 
-// The sums of `count` parts of one head, by a warp: the first one `first`, the others in slot 0 of every `stride`-th team behind it.  Into the result, or
-// (to_out false) into the first one's place.
-__device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, int count, int b, int head, int out_head, bool to_out) {
+// The sums of `count` parts of HEADS heads (head, head + KV_TEAM, ... below `heads`), by a warp: the first part is `first`, the others in slot 0 of every `stride`-th
+// team behind it.  Into the result, or (to_out false) into the first one's place.  A lane has a part's weights; the first parts' rows are under way while the
+// weights are, and all heads' at once.
+template <int HEADS>
+__device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, int count, int b, int head, int heads, int head0, bool to_out) {
+    static_assert(KV_FLAT <= 32 && KV_FAN <= 32 && (KV_TEAMS_MAX + KV_FAN - 1) / KV_FAN <= 32, "a part to a lane");
     const int lane = threadIdx.x & 31;
-    auto place = [&](int i) { return (int64_t)(i == 0 ? first : (first & ~1) + 2 * stride * i) * a.per_item; };
-    float top = -INFINITY, sum = 0.f;
-    float4 r = make_float4(0, 0, 0, 0);
+    const int64_t step = (int64_t)2 * stride * a.per_item, at0 = (int64_t)first * a.per_item + head, at1 = (int64_t)(first & ~1) * a.per_item + head;
+    float4* const mine = reinterpret_cast<float4*>(a.parts) + at0 * (KV_D / 4) + lane;
+    const float4* src = reinterpret_cast<const float4*>(a.parts) + at1 * (KV_D / 4) + lane;
+    float2 s[HEADS];
+    const float2* const stats = a.stats + (lane == 0 ? at0 : at1 + lane * step);
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+        s[h] = make_float2(-INFINITY, 0.f);
+        if (lane < count && head + h * KV_TEAM < heads) s[h] = __ldcg(stats + h * KV_TEAM);
+    }
+    float top[HEADS], sum[HEADS], w[HEADS];
+    float4 r[HEADS];
 #pragma unroll 1
-    for (int i0 = 0; i0 < count; i0 += 16) {      // all that 16 parts need is asked for at once
-        float4 x[16];
-        float2 s = make_float2(-INFINITY, 0.f);
-        if (lane < 16 && i0 + lane < count) s = __ldcg(&a.stats[place(i0 + lane) + head]);
+    for (int i0 = 0; i0 < count; i0 += KV_JOIN_STEP, src += KV_JOIN_STEP * step * (KV_D / 4)) {
+        float4 x[KV_JOIN_STEP][HEADS];
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (i0 + i < count) x[i] = __ldcg(reinterpret_cast<const float4*>(a.parts + (place(i0 + i) + head) * KV_D) + lane);
-        float here = s.x;
+        for (int i = 0; i < KV_JOIN_STEP; ++i) {
+            const float4* const from = i0 + i == 0 ? mine : src + i * step * (KV_D / 4);
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, o));
-        const float m = fmaxf(top, __shfl_sync(0xffffffffu, here, 0)), ref = m == -INFINITY ? 0.f : m, old = exp2_fast(top - ref), w = exp2_fast(s.x - ref);
-        top = m;
-        sum = sum * old + s.y * w;
-        r.x *= old; r.y *= old; r.z *= old; r.w *= old;
+            for (int h = 0; h < HEADS; ++h) {
+                x[i][h] = make_float4(0, 0, 0, 0);
+                if (i0 + i < count && head + h * KV_TEAM < heads) x[i][h] = __ldcg(from + h * (KV_TEAM * KV_D / 4));
+            }
+        }
+        if (i0 == 0) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float f = __shfl_sync(0xffffffffu, w, i);
-            if (i0 + i < count) { r.x += x[i].x * f; r.y += x[i].y * f; r.z += x[i].z * f; r.w += x[i].w * f; }
+            for (int h = 0; h < HEADS; ++h) {
+                r[h] = make_float4(0, 0, 0, 0);
+                top[h] = s[h].x;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], o));
+                w[h] = exp2_fast(s[h].x - (top[h] == -INFINITY ? 0.f : top[h]));
+                sum[h] = s[h].y * w[h];
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], o);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < KV_JOIN_STEP; ++i) {
+#pragma unroll
+            for (int h = 0; h < HEADS; ++h) {
+                const float f = __shfl_sync(0xffffffffu, w[h], i0 + i);
+                if (i0 + i < count) { r[h].x += x[i][h].x * f; r[h].y += x[i][h].y * f; r[h].z += x[i][h].z * f; r[h].w += x[i][h].w * f; }
+            }
         }
     }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    sum = __shfl_sync(0xffffffffu, sum, 0);
-    if (to_out) {
-        store_row4(a.out + b * a.ldo + out_head * KV_D + lane * 4, r, 1.0f / sum, a.flags & 2);
-        if (a.lse && lane == 0) a.lse[(int64_t)b * a.heads + out_head] = (top - KV_LIFT + log2f(sum)) * 0.6931471805599453f;
-    } else {
-        reinterpret_cast<float4*>(a.parts + (place(0) + head) * KV_D)[lane] = r;
-        if (lane == 0) a.stats[place(0) + head] = make_float2(top, sum);
+    for (int h = 0; h < HEADS; ++h) {
+        const int at = head + h * KV_TEAM;
+        if (at >= heads) break;
+        if (to_out) {
+            store_row4(a.out + b * a.ldo + (head0 + at) * KV_D + lane * 4, r[h], 1.0f / sum[h], a.flags & 2);
+            if (a.lse && lane == 0) a.lse[(int64_t)b * a.heads + head0 + at] = (top[h] - KV_LIFT + log2f(sum[h])) * 0.6931471805599453f;
+        } else {
+            mine[h * (KV_TEAM * KV_D / 4)] = r[h];
+            if (lane == 0) a.stats[at0 + h * KV_TEAM] = make_float2(top[h], sum[h]);
+        }
     }
 }
 
@@ -458,7 +486,6 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         mbar_init(&sh.empty[0][0] + tid, 1);
         fence_mbar_init();
     }
-    if (tid < K::TEAMS) sh.parts[tid] = 0;
     if (warp >= WARPS && elect_one()) { tma_prefetch_desc(&k_map); tma_prefetch_desc(&v_map); }
     grid_dep_launch();
     grid_dep_wait();
@@ -616,6 +643,27 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     if (mate == 0) describe(c0, sh.seg[team][0]);
     team_sync(team);
     ask_queries(sh.seg[team][0].b, sh.seg[team][0].item);
+    if (mate == KV_TEAM - 1 && lane < 2) {
+        // the items that the team's part begins and ends in, while the first rows are under way: teams from ... to share one, in groups of `fan`; the first
+        // one's part is in slot `late`
+        KvWalk w;
+        w.seek(lane ? c1 - 1 : c0, sh.prefix, a.batch, items);
+        const int f0 = (lane ? c1 - 1 : c0) - w.c;
+        typename K::Share& to = sh.share[team][lane];
+        if ((c0 <= f0 && f0 + w.n <= c1) || (lane && f0 <= c0)) to.here = 0;         // whole, or slot 0's
+        else {
+            const int at = sh.cost[w.b] * items + w.item * (w.n + KV_ITEM_COST);
+            auto owner = [&](int v) {
+                int o = min(teams - 1, (int)((float)v * ((float)teams / (float)cost)));
+                while (cost_of(o) > v) --o;
+                while (o + 1 < teams && cost_of(o + 1) <= v) ++o;
+                return o;
+            };
+            const int from = owner(at), last = owner(at + w.n - 1), late = f0 != begin_of(from), count = last - from + 1;
+            const int fan = count <= KV_FLAT ? count : KV_FAN, mine = (id - from) / fan, first = 2 * (from + mine * fan) + (mine == 0 ? late : 0);
+            to = {first, min(fan, count - mine * fan), fan, 2 * from + late, (count + fan - 1) / fan, w.b, head_of(w.item), heads_of(w.item)};
+        }
+    }
     float* const buf = reinterpret_cast<float*>(smem + K::JOIN + team * KV_JOIN_BYTES);
     int f = c0 + mate, slot = 0, parity = 0;
     bool ok = true;
@@ -795,33 +843,36 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                         for (int i = 0; i < PIECES; ++i) v[r][i] = make_uint4(0, 0, 0, 0);
                     }
                 }
-                uint32_t pair[2][16];      // [keys t, t + 4 | t + 8, t + 12][16 columns: bf16 8 gp + j and 64 + 8 gp + j, codes 16 gp + j]
+                // pairs of keys (t, t + 4), (t + 8, t + 12), of the columns that a word of each row holds: bf16 8 gp + 2 w, + 1 and 64 + those, codes 16 gp + 4 w ... + 3 and 8 + those
+                constexpr int EACH = TYPE == KV_BF16 ? 2 : 4;
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
+                for (int w = 0; w < 8 / EACH; ++w) {
+                    uint32_t pair[2][2][EACH];       // [keys][columns' half]
 #pragma unroll
-                    for (int i = 0; i < PIECES; ++i) {
-                        const uint32_t x[4] = {v[2 * r][i].x, v[2 * r][i].y, v[2 * r][i].z, v[2 * r][i].w};
-                        const uint32_t y[4] = {v[2 * r + 1][i].x, v[2 * r + 1][i].y, v[2 * r + 1][i].z, v[2 * r + 1][i].w};
+                    for (int r = 0; r < 2; ++r) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
+                        for (int half = 0; half < 2; ++half) {
+                            const uint4 x4 = v[2 * r][TYPE == KV_BF16 ? half : 0], y4 = v[2 * r + 1][TYPE == KV_BF16 ? half : 0];
+                            const int at = TYPE == KV_BF16 ? w : w + 2 * half;
+                            const uint32_t x = at == 0 ? x4.x : at == 1 ? x4.y : at == 2 ? x4.z : x4.w, y = at == 0 ? y4.x : at == 1 ? y4.y : at == 2 ? y4.z : y4.w;
                             if (TYPE == KV_BF16) {
-                                pair[r][8 * i + 2 * j] = __byte_perm(x[j], y[j], 0x5410);
-                                pair[r][8 * i + 2 * j + 1] = __byte_perm(x[j], y[j], 0x7632);
+                                pair[r][half][0] = __byte_perm(x, y, 0x5410);
+                                pair[r][half][1] = __byte_perm(x, y, 0x7632);
                             } else {
-                                pair[r][4 * j] = pair_to_bf16<TYPE, 0>(x[j], y[j]);
-                                pair[r][4 * j + 1] = pair_to_bf16<TYPE, 1>(x[j], y[j]);
-                                pair[r][4 * j + 2] = pair_to_bf16<TYPE, 2>(x[j], y[j]);
-                                pair[r][4 * j + 3] = pair_to_bf16<TYPE, 3>(x[j], y[j]);
+                                pair[r][half][0] = pair_to_bf16<TYPE, 0>(x, y);
+                                pair[r][half][1] = pair_to_bf16<TYPE, 1>(x, y);
+                                pair[r][half][EACH - 2] = pair_to_bf16<TYPE, 2>(x, y);
+                                pair[r][half][EACH - 1] = pair_to_bf16<TYPE, 3>(x, y);
                             }
                         }
                     }
-                }
 #pragma unroll
-                for (int h = 0; h < HG; ++h) {
+                    for (int h = 0; h < HG; ++h) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        mma_bf16(acc[h][j], pair[0][j], pair[0][8 + j], pair[1][j], pair[1][8 + j], p_hi[h][0], p_hi[h][1]);
-                        mma_bf16(acc[h][j], pair[0][j], pair[0][8 + j], pair[1][j], pair[1][8 + j], p_lo[h][0], p_lo[h][1]);
+                        for (int j = 0; j < EACH; ++j) {
+                            mma_bf16(acc[h][EACH * w + j], pair[0][0][j], pair[0][1][j], pair[1][0][j], pair[1][1][j], p_hi[h][0], p_hi[h][1]);
+                            mma_bf16(acc[h][EACH * w + j], pair[0][0][j], pair[0][1][j], pair[1][0][j], pair[1][1][j], p_lo[h][0], p_lo[h][1]);
+                        }
                     }
                 }
             }
@@ -842,7 +893,6 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         }
         const bool whole = seg.begin == seg.first && seg.end == seg.first + seg.n;
         const int64_t mine = (int64_t)(2 * id + (seg.begin == c0 ? 0 : 1)) * a.per_item;
-        if (!whole && mate == 0 && lane == 0) sh.part[team][sh.parts[team]++] = seg;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int at_q = q & (quarters - 1);
@@ -885,45 +935,28 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         }
         if (seg.end == c1) break;
     }
-    // ---- items that the team shares with others, the first and the last of its part: it is known for both at once whether all have come
+    // ---- items that the team shares with others: it is known for both at once whether all have come
     team_sync(team);
-    const int parts = sh.parts[team];
-    if (parts == 0) return;
-    if (mate == 0 && lane < parts) {
-        // teams from ... to share the item, in groups of `fan`; the first one's part is in slot `late`
-        const typename K::Segment& seg = sh.part[team][lane];
-        const int at = sh.cost[seg.b] * items + seg.item * (seg.n + KV_ITEM_COST);
-        auto owner = [&](int v) {
-            int o = min(teams - 1, (int)((float)v * ((float)teams / (float)cost)));
-            while (cost_of(o) > v) --o;
-            while (o + 1 < teams && cost_of(o + 1) <= v) ++o;
-            return o;
-        };
-        const int from = owner(at), to = owner(at + seg.n - 1), late = seg.first != begin_of(from), count = to - from + 1;
-        const int fan = count <= KV_FLAT ? count : KV_FAN, mine = (id - from) / fan, first = 2 * (from + mine * fan) + (mine == 0 ? late : 0);
-        const int here = min(fan, count - mine * fan);
-        sh.share[team][lane] = {first, here, fan, 2 * from + late, (count + fan - 1) / fan, head_of(seg.item), heads_of(seg.item)};
-        sh.last[team][lane] = all_came(a.arrived + first, here);
-    }
+    const typename K::Share (&shares)[2] = sh.share[team];
+    if (shares[0].here + shares[1].here == 0) return;
+    if (mate == 0 && lane < 2) sh.last[team][lane] = shares[lane].here > 0 && all_came(a.arrived + shares[lane].first, shares[lane].here);
     team_sync(team);
 #pragma unroll 1
     for (int level = 0; level < 2; ++level) {
         int done = 0, again = 0;         // heads to join before this part's
 #pragma unroll 1
-        for (int i = 0; i < parts; ++i) {
+        for (int i = 0; i < 2; ++i) {
             if (!sh.last[team][i]) continue;
-            const typename K::Share s = sh.share[team][i];
+            const typename K::Share s = shares[i];
             again |= level == 0 && s.groups > 1;
-            for (int head = (mate - done) & (KV_TEAM - 1); head < s.heads; head += KV_TEAM)
-                kv_join(a, level ? s.item : s.first, level ? s.fan : 1, level ? s.groups : s.here, sh.part[team][i].b, head, s.head0 + head, level || s.groups == 1);
+            for (int head = (mate - done) & (KV_TEAM - 1); head < s.heads; head += 2 * HG * KV_TEAM)
+                kv_join<2 * HG>(a, level ? s.item : s.first, level ? s.fan : 1, level ? s.groups : s.here, s.b, head, s.heads, s.head0, level || s.groups == 1);
             done += s.heads;
         }
         if (!again) break;
         team_sync(team);
-        if (mate == 0 && lane < parts && sh.last[team][lane]) {       // the groups of an item
-            const typename K::Share& s = sh.share[team][lane];
-            sh.last[team][lane] = s.groups > 1 && all_came(a.arrived + 2 * KV_TEAMS_MAX + s.item, s.groups);
-        }
+        if (mate == 0 && lane < 2 && sh.last[team][lane])       // the groups of an item
+            sh.last[team][lane] = shares[lane].groups > 1 && all_came(a.arrived + 2 * KV_TEAMS_MAX + shares[lane].item, shares[lane].groups);
         team_sync(team);
     }
 }
