@@ -153,6 +153,9 @@ bool rmsnorm_mod(const void* x, const void* w, const void* scale, const void* sh
 // a row stays in registers (ITEMS x 8 values to a thread) from its load to both stores, so HBM sees x and branch
 // once and y and h once, 8 bytes a value.  Everything between is fp32 and y and h are rounded once; h is made from the unrounded
 // y, which the separate add and norm cannot do.
+//
+// What bounds it: HBM with many rows (16640 x 4096: 84 us without the inner norm, 6.5 TB/s; 90 with it), the chain of a row's load, sums and stores with
+// few.  So many rows have to be under way, and what a step needs is asked for before the sum ahead of it where registers for that do not cost rows.
 struct ResidualNorm {
     const uint16_t *x, *branch, *post, *gate, *pre, *scale, *shift;
     uint16_t *y, *h;
@@ -160,12 +163,15 @@ struct ResidualNorm {
     int rows, cols, per_group;
     float alpha, eps;
 };
+// The sum over a row's threads: a warp's (THREADS 32), a block's of THREADS, or of any number (0).
 template <int THREADS>
-__device__ __forceinline__ float block_sum(float v, float* red) {
+__device__ __forceinline__ float row_sum(float v, float* red) {
     v = warp_sum(v);
     if (THREADS == 32) return v;
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
+    if (THREADS == 0) return warp_sum(lane < (int)blockDim.x >> 5 ? red[lane] : 0.f);
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < THREADS / 32; ++i) s += red[i];
@@ -174,20 +180,22 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 // 1 / sqrt(mean of squares + eps) of a row, `squares(f)` a thread's part of the sum of its values times f.  Squares of values
 // above 2^57 or so do not fit fp32: such a row (and one with a NaN, to which it makes no difference) is summed again at 2^-80.
 template <int THREADS, class F>
-__device__ __forceinline__ float row_rms_inv(F squares, int cols, float eps, float (*red)[THREADS / 32]) {
-    const float sum = block_sum<THREADS>(squares(1.0f), red[0]);
+__device__ __forceinline__ float row_rms_inv(F squares, int cols, float eps, float (*red)[32]) {
+    const float sum = row_sum<THREADS>(squares(1.0f), red[0]);
     if (sum < INFINITY) return rsqrtf(sum / (float)cols + eps);
-    return rsqrtf(block_sum<THREADS>(squares(8.271806125530277e-25f), red[1]) / (float)cols) * 8.271806125530277e-25f;
+    return rsqrtf(row_sum<THREADS>(squares(8.271806125530277e-25f), red[1]) / (float)cols) * 8.271806125530277e-25f;
 }
-template <int THREADS, int ITEMS, bool POST, bool EARLY>
-__global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS)
+// THREADS: 32 = a warp to a row, four rows to a block; 0 = a block of any size to a row.
+template <int THREADS, int ITEMS, bool POST, bool AHEAD>
+__global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS ? THREADS : 1024)
 residual_norm_vec_kernel(const ResidualNorm a) {
     grid_dep_launch();
     grid_dep_wait();
-    __shared__ float red[4][THREADS / 32];
-    const int tid = THREADS == 32 ? threadIdx.x & 31 : threadIdx.x;
-    const int row = THREADS == 32 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
-    if (THREADS == 32 && row >= a.rows) return;
+    __shared__ float red[4][32];
+    constexpr bool WARP = THREADS == 32;
+    const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, threads = THREADS ? THREADS : blockDim.x;
+    const int row = WARP ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+    if (WARP && row >= a.rows) return;
     const int nvec = a.cols >> 3;
     const size_t vec = (size_t)(row / a.per_group) * nvec;
     const uint4* x = reinterpret_cast<const uint4*>(a.x + row * a.ldx);
@@ -195,19 +203,22 @@ residual_norm_vec_kernel(const ResidualNorm a) {
     const uint4 *post = reinterpret_cast<const uint4*>(a.post), *gate = a.gate ? reinterpret_cast<const uint4*>(a.gate) + vec : nullptr;
     const uint4 *pre = reinterpret_cast<const uint4*>(a.pre), *scale = a.scale ? reinterpret_cast<const uint4*>(a.scale) + vec : nullptr,
                 *shift = reinterpret_cast<const uint4*>(a.shift) + vec;
-    uint4 xv[ITEMS], bv[ITEMS], wv[EARLY ? ITEMS : 1], gv[EARLY ? ITEMS : 1], pv[EARLY ? ITEMS : 1], cv[EARLY ? ITEMS : 1], sv[EARLY ? ITEMS : 1];
+    // AHEAD: the vectors that a step needs are asked for before the sum ahead of it, else where they are used
+    uint4 xv[ITEMS], bv[ITEMS], wv[AHEAD ? ITEMS : 1], gv[AHEAD ? ITEMS : 1];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        const int idx = tid + i * THREADS;
+        const int idx = tid + i * threads;
         if (idx < nvec) {
-            xv[i] = x[idx];
             bv[i] = b[idx];
-            if (EARLY) {
-                if (POST) wv[i] = post[idx];
-                if (gate) gv[i] = gate[idx];
-                if (a.h) pv[i] = pre[idx];
-                if (scale) { cv[i] = scale[idx]; sv[i] = shift[idx]; }
-            }
+            xv[i] = x[idx];
+        }
+    }
+#pragma unroll
+    for (int i = 0; AHEAD && i < ITEMS; ++i) {
+        const int idx = tid + i * threads;
+        if (idx < nvec) {
+            if (POST) wv[i] = post[idx];
+            if (gate) gv[i] = gate[idx];
         }
     }
     float inv = 1.f;
@@ -216,7 +227,7 @@ residual_norm_vec_kernel(const ResidualNorm a) {
             float sq = 0.f;
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
-                if (tid + i * THREADS < nvec) {
+                if (tid + i * threads < nvec) {
                     float f[8];
                     unpack8(bv[i], f);
 #pragma unroll
@@ -229,18 +240,18 @@ residual_norm_vec_kernel(const ResidualNorm a) {
     float y[ITEMS][8];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        const int idx = tid + i * THREADS;
+        const int idx = tid + i * threads;
         if (idx < nvec) {
             float f[8], u[8], w[8];
             unpack8(xv[i], f);
             unpack8(bv[i], u);
             if (POST) {
-                unpack8(EARLY ? wv[EARLY ? i : 0] : post[idx], w);
+                unpack8(AHEAD ? wv[AHEAD ? i : 0] : post[idx], w);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) u[j] = u[j] * inv * w[j];
             }
             if (gate) {
-                unpack8(EARLY ? gv[EARLY ? i : 0] : gate[idx], w);
+                unpack8(AHEAD ? gv[AHEAD ? i : 0] : gate[idx], w);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) u[j] *= w[j];
             }
@@ -250,11 +261,20 @@ residual_norm_vec_kernel(const ResidualNorm a) {
         }
     }
     if (!a.h) return;
+    uint4 pv[AHEAD ? ITEMS : 1], cv[AHEAD ? ITEMS : 1], sv[AHEAD ? ITEMS : 1];
+#pragma unroll
+    for (int i = 0; AHEAD && i < ITEMS; ++i) {
+        const int idx = tid + i * threads;
+        if (idx < nvec) {
+            pv[i] = pre[idx];
+            if (scale) { cv[i] = scale[idx]; sv[i] = shift[idx]; }
+        }
+    }
     inv = row_rms_inv<THREADS>([&](float s) {
         float sq = 0.f;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            if (tid + i * THREADS < nvec) {
+            if (tid + i * threads < nvec) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) sq += (y[i][j] * s) * (y[i][j] * s);
             }
@@ -263,16 +283,16 @@ residual_norm_vec_kernel(const ResidualNorm a) {
     }, a.cols, a.eps, red + 2);
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        const int idx = tid + i * THREADS;
+        const int idx = tid + i * threads;
         if (idx < nvec) {
             float w[8];
-            unpack8(EARLY ? pv[EARLY ? i : 0] : pre[idx], w);
+            unpack8(AHEAD ? pv[AHEAD ? i : 0] : pre[idx], w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[i][j] = y[i][j] * inv * w[j];
             if (scale) {
                 float sh[8];
-                unpack8(EARLY ? cv[EARLY ? i : 0] : scale[idx], w);
-                unpack8(EARLY ? sv[EARLY ? i : 0] : shift[idx], sh);
+                unpack8(AHEAD ? cv[AHEAD ? i : 0] : scale[idx], w);
+                unpack8(AHEAD ? sv[AHEAD ? i : 0] : shift[idx], sh);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) y[i][j] = y[i][j] * (1.0f + w[j]) + sh[j];
             }
@@ -280,11 +300,11 @@ residual_norm_vec_kernel(const ResidualNorm a) {
         }
     }
 }
-// Any width, pitch and alignment: the row is read again in each step (from L1 and L2).
+// Any width, pitch and alignment: the row is read again in each step (from L1 and L2).  4000 x 1801: 37 us, where the other kernel has 15 for 4000 x 1800.
 __global__ void __launch_bounds__(256) residual_norm_any_kernel(const ResidualNorm a) {
     grid_dep_launch();
     grid_dep_wait();
-    __shared__ float red[4][8];
+    __shared__ float red[4][32];
     const int row = blockIdx.x;
     const size_t vec = (size_t)(row / a.per_group) * a.cols;
     const uint16_t *x = a.x + row * a.ldx, *b = a.branch + row * a.ldb;
@@ -320,7 +340,6 @@ __global__ void __launch_bounds__(256) residual_norm_any_kernel(const ResidualNo
         a.y[row * a.ldy + i] = f32_to_bf16(f);
     }
 }
-static constexpr int RESIDUAL_EARLY_ROWS = 1200;
 bool residual_norm(const void* x, int64_t ldx, const void* branch, int64_t ldb, const void* post, const void* gate, float alpha, const void* pre,
                    const void* scale, const void* shift, int groups, void* y, int64_t ldy, void* h, int64_t ldh, int rows, int cols, float eps,
                    cudaStream_t st) {
@@ -330,15 +349,24 @@ bool residual_norm(const void* x, int64_t ldx, const void* branch, int64_t ldb, 
                           (uintptr_t)y | (uintptr_t)h;
     const bool vec = (all & 15) == 0 && ((ldx | ldb | ldy | (h ? ldh : 0) | cols) & 7) == 0 && cols <= 16384;
     if (!vec) return launch_ok(launch_chained(residual_norm_any_kernel, dim3(rows), dim3(256), 0, st, 1, rows, a), "residual_norm");
-    // EARLY where the rows fit the GPU at once: what a row needs is asked for together
-    const bool early = rows <= RESIDUAL_EARLY_ROWS;
-#define O1_RN(T, I) (post ? (early ? residual_norm_vec_kernel<T, I, true, true> : residual_norm_vec_kernel<T, I, true, false>) \
-                          : (early ? residual_norm_vec_kernel<T, I, false, true> : residual_norm_vec_kernel<T, I, false, false>))
-    auto kern = cols <= 256 ? O1_RN(32, 1) : cols <= 1024 ? O1_RN(32, 4) : cols <= 1280 ? O1_RN(32, 5) : cols <= 2048 ? O1_RN(64, 4) : cols <= 4096 ? O1_RN(128, 4)
-                : cols <= 8192 ? O1_RN(256, 4) : O1_RN(512, 4);
+    // Measured in us.  Rows up to 1280 wide by a warp each, vectors ahead (2000 x 1152 with both norms 4.2, at use 5.4; a block to a row, at use, 6.4).
+    // Wider ones, few of them: two pieces of 16 bytes to a thread, vectors ahead; many: fewer registers, so that more rows are under way - with the
+    // inner norm four pieces and a fixed number of threads.  Both norms, ahead / at use: 592 x 4096 4.4 / 6.2, 3000 x 4096 22 / 27, 3000 x 8192 44 / 45,
+    // 16640 x 4096 101 / 90, 592 x 12288 19 / 20, 2000 x 12288 56 / 44.  Without the inner norm: 592 x 4096 3.3 / 3.7, 1500 x 4096 10.5 / 9.1; at use
+    // with two pieces, and with four: 16640 x 4096 84 and 87, 2000 x 12288 40 and 32.
+    const bool warps = cols <= 1280, few = (int64_t)rows * cols <= (!post ? 4000000 : cols <= 8192 ? 20000000 : 8000000);
+    int threads = 128;
+    void (*kern)(const ResidualNorm);
+#define O1_RN(T, I, AHEAD) (post ? residual_norm_vec_kernel<T, I, true, AHEAD> : residual_norm_vec_kernel<T, I, false, AHEAD>)
+    if (warps) kern = cols <= 256 ? O1_RN(32, 1, true) : cols <= 512 ? O1_RN(32, 2, true) : cols <= 1024 ? O1_RN(32, 4, true) : O1_RN(32, 5, true);
+    else if (few || cols <= (post ? 2048 : 4096)) {
+        kern = post ? residual_norm_vec_kernel<0, 2, true, true> : few ? residual_norm_vec_kernel<0, 2, false, true> : residual_norm_vec_kernel<0, 2, false, false>;
+        threads = ((cols >> 3) + 63) / 64 * 32;
+    } else {
+        threads = cols <= 4096 ? 128 : cols <= 8192 ? 256 : 512;
+        kern = cols <= 4096 ? residual_norm_vec_kernel<128, 4, true, false> : cols <= 8192 ? O1_RN(256, 4, false) : O1_RN(512, 4, false);
+    }
 #undef O1_RN
-    const bool warps = cols <= 1280;
-    const int threads = warps || cols <= 4096 ? (warps || cols > 2048 ? 128 : 64) : cols <= 8192 ? 256 : 512;
     return launch_ok(launch_chained(kern, dim3(warps ? (rows + 3) / 4 : rows), dim3(threads), 0, st, 1, rows, a), "residual_norm");
 }
 
