@@ -154,7 +154,7 @@ bool rmsnorm_mod(const void* x, const void* w, const void* scale, const void* sh
 // once and y and h once, 8 bytes a value.  Everything between is fp32 and y and h are rounded once; h is made from the unrounded
 // y, which the separate add and norm cannot do.
 //
-// What bounds it: HBM with many rows (16640 x 4096: 84 us without the inner norm, 6.5 TB/s; 90 with it), the chain of a row's load, sums and stores with
+// What bounds it: HBM with many rows (16640 x 4096: 84 us without the inner norm, 6.5 TB/s; 88 with it), the chain of a row's load, sums and stores with
 // few.  So many rows have to be under way, and what a step needs is asked for before the sum ahead of it where registers for that do not cost rows.
 struct ResidualNorm {
     const uint16_t *x, *branch, *post, *gate, *pre, *scale, *shift;
@@ -185,9 +185,9 @@ __device__ __forceinline__ float row_rms_inv(F squares, int cols, float eps, flo
     if (sum < INFINITY) return rsqrtf(sum / (float)cols + eps);
     return rsqrtf(row_sum<THREADS>(squares(8.271806125530277e-25f), red[1]) / (float)cols) * 8.271806125530277e-25f;
 }
-// THREADS: 32 = a warp to a row, four rows to a block; 0 = a block of any size to a row.
+// THREADS: 32 = a warp to a row, four rows to a block; 0 = a block of any size to a row; else as many rows on an SM as 64 or 72 registers to a thread give.
 template <int THREADS, int ITEMS, bool POST, bool AHEAD>
-__global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS ? THREADS : 1024)
+__global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS ? THREADS : 1024, THREADS == 128 ? 7 : THREADS == 256 ? 4 : THREADS == 512 ? 2 : 1)
 residual_norm_vec_kernel(const ResidualNorm a) {
     grid_dep_launch();
     grid_dep_wait();
@@ -196,29 +196,27 @@ residual_norm_vec_kernel(const ResidualNorm a) {
     const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, threads = THREADS ? THREADS : blockDim.x;
     const int row = WARP ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
     if (WARP && row >= a.rows) return;
+    const uint16_t *x = a.x + row * a.ldx, *b = a.branch + row * a.ldb;
+    const size_t vec = (size_t)(row / a.per_group) * a.cols;
+    const uint16_t *post = a.post, *gate = a.gate ? a.gate + vec : nullptr, *pre = a.pre, *scale = a.scale ? a.scale + vec : nullptr, *shift = a.shift + vec;
     const int nvec = a.cols >> 3;
-    const size_t vec = (size_t)(row / a.per_group) * nvec;
-    const uint4* x = reinterpret_cast<const uint4*>(a.x + row * a.ldx);
-    const uint4* b = reinterpret_cast<const uint4*>(a.branch + row * a.ldb);
-    const uint4 *post = reinterpret_cast<const uint4*>(a.post), *gate = a.gate ? reinterpret_cast<const uint4*>(a.gate) + vec : nullptr;
-    const uint4 *pre = reinterpret_cast<const uint4*>(a.pre), *scale = a.scale ? reinterpret_cast<const uint4*>(a.scale) + vec : nullptr,
-                *shift = reinterpret_cast<const uint4*>(a.shift) + vec;
+    auto get = [](const uint16_t* p, int idx) { return reinterpret_cast<const uint4*>(p)[idx]; };
     // AHEAD: the vectors that a step needs are asked for before the sum ahead of it, else where they are used
     uint4 xv[ITEMS], bv[ITEMS], wv[AHEAD ? ITEMS : 1], gv[AHEAD ? ITEMS : 1];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         const int idx = tid + i * threads;
         if (idx < nvec) {
-            bv[i] = b[idx];
-            xv[i] = x[idx];
+            bv[i] = get(b, idx);
+            xv[i] = get(x, idx);
         }
     }
 #pragma unroll
     for (int i = 0; AHEAD && i < ITEMS; ++i) {
         const int idx = tid + i * threads;
         if (idx < nvec) {
-            if (POST) wv[i] = post[idx];
-            if (gate) gv[i] = gate[idx];
+            if (POST) wv[i] = get(post, idx);
+            if (gate) gv[i] = get(gate, idx);
         }
     }
     float inv = 1.f;
@@ -246,12 +244,12 @@ residual_norm_vec_kernel(const ResidualNorm a) {
             unpack8(xv[i], f);
             unpack8(bv[i], u);
             if (POST) {
-                unpack8(AHEAD ? wv[AHEAD ? i : 0] : post[idx], w);
+                unpack8(AHEAD ? wv[AHEAD ? i : 0] : get(post, idx), w);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) u[j] = u[j] * inv * w[j];
             }
             if (gate) {
-                unpack8(AHEAD ? gv[AHEAD ? i : 0] : gate[idx], w);
+                unpack8(AHEAD ? gv[AHEAD ? i : 0] : get(gate, idx), w);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) u[j] *= w[j];
             }
@@ -266,8 +264,8 @@ residual_norm_vec_kernel(const ResidualNorm a) {
     for (int i = 0; AHEAD && i < ITEMS; ++i) {
         const int idx = tid + i * threads;
         if (idx < nvec) {
-            pv[i] = pre[idx];
-            if (scale) { cv[i] = scale[idx]; sv[i] = shift[idx]; }
+            pv[i] = get(pre, idx);
+            if (scale) { cv[i] = get(scale, idx); sv[i] = get(shift, idx); }
         }
     }
     inv = row_rms_inv<THREADS>([&](float s) {
@@ -286,13 +284,13 @@ residual_norm_vec_kernel(const ResidualNorm a) {
         const int idx = tid + i * threads;
         if (idx < nvec) {
             float w[8];
-            unpack8(AHEAD ? pv[AHEAD ? i : 0] : pre[idx], w);
+            unpack8(AHEAD ? pv[AHEAD ? i : 0] : get(pre, idx), w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[i][j] = y[i][j] * inv * w[j];
             if (scale) {
                 float sh[8];
-                unpack8(AHEAD ? cv[AHEAD ? i : 0] : scale[idx], w);
-                unpack8(AHEAD ? sv[AHEAD ? i : 0] : shift[idx], sh);
+                unpack8(AHEAD ? cv[AHEAD ? i : 0] : get(scale, idx), w);
+                unpack8(AHEAD ? sv[AHEAD ? i : 0] : get(shift, idx), sh);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) y[i][j] = y[i][j] * (1.0f + w[j]) + sh[j];
             }
@@ -351,8 +349,8 @@ bool residual_norm(const void* x, int64_t ldx, const void* branch, int64_t ldb, 
     if (!vec) return launch_ok(launch_chained(residual_norm_any_kernel, dim3(rows), dim3(256), 0, st, 1, rows, a), "residual_norm");
     // Measured in us.  Rows up to 1280 wide by a warp each, vectors ahead (2000 x 1152 with both norms 4.2, at use 5.4; a block to a row, at use, 6.4).
     // Wider ones, few of them: two pieces of 16 bytes to a thread, vectors ahead; many: fewer registers, so that more rows are under way - with the
-    // inner norm four pieces and a fixed number of threads.  Both norms, ahead / at use: 592 x 4096 4.4 / 6.2, 3000 x 4096 22 / 27, 3000 x 8192 44 / 45,
-    // 16640 x 4096 101 / 90, 592 x 12288 19 / 20, 2000 x 12288 56 / 44.  Without the inner norm: 592 x 4096 3.3 / 3.7, 1500 x 4096 10.5 / 9.1; at use
+    // inner norm four pieces and a fixed number of threads.  Both norms, ahead / at use: 592 x 4096 4.4 / 6.2, 3000 x 4096 22 / 27, 3000 x 8192 44 / 43,
+    // 16640 x 4096 101 / 88, 592 x 12288 19 / 20, 2000 x 12288 56 / 44.  Without the inner norm: 592 x 4096 3.3 / 3.7, 1500 x 4096 10.5 / 9.1; at use
     // with two pieces, and with four: 16640 x 4096 84 and 87, 2000 x 12288 40 and 32.
     const bool warps = cols <= 1280, few = (int64_t)rows * cols <= (!post ? 4000000 : cols <= 8192 ? 20000000 : 8000000);
     int threads = 128;
