@@ -110,88 +110,94 @@ __device__ __forceinline__ void store8(uint16_t* p, const uint4& v) {
     for (int i = 0; i < 4; ++i) { p[2 * i] = (uint16_t)w[i]; p[2 * i + 1] = (uint16_t)(w[i] >> 16); }
 }
 
-// A slot's row of head 0 in a [pages][heads][page_size] array, -1: none.  (The other heads' lie page_size apart.)
-__device__ __forceinline__ int64_t place(int64_t slot, const KvView& c, int* err) {
+// A unit is a row's head; a warp has EACH of them, behind one another: keys in the lower 16 lanes, values in the others, eight columns to a lane.  HBM bound for
+// many rows: 2 bytes in, 1 (or 2) and the scale out a value.  A lane finds a unit's place and has its scale, and what the units need is asked for together: a warp
+// of eight has 4 KB on its way, one of two, for few rows, more warps.  us, written and read: 16640 rows of 8 heads of int8 22.8 + 18.7 (5.0 TB/s), 100000 rows of
+// one head 18.5 + 15; with a row to a warp, its heads together, 23.5 + 19.5 and 43 + 39; with a head to a half warp 34 + 35 for the former.  Two units or
+// eight to a warp: 2200 rows of 8 heads 4.5 + 4.2 and 6.8 + 4.6, 4111 rows 10 + 7.9 and 6.9 + 6.1.
+static constexpr int KV_EACH = 8, KV_EACH_OF_FEW = 2, KV_FEW_UNITS = 19200;
+// A unit's place in a [pages][heads][page_size] array, -1: none.
+__device__ __forceinline__ int64_t place(int64_t slot, int head, const KvView& c, int* err) {
     if (slot < 0) return -1;
     if (slot >= (int64_t)c.pages * c.page_size) { atomicExch(err, ERR_KV_PLACE); return -1; }
     const int64_t page = c.page_shift >= 0 ? slot >> c.page_shift : slot / c.page_size;
-    return page * c.heads * c.page_size + slot - page * c.page_size;
+    return (page * c.heads + head) * c.page_size + slot - page * c.page_size;
 }
-
-// A row (few rows: `each` of its heads) to a warp: its keys to the lower 16 lanes, its values to the others, eight columns to a lane, KV_ROW_HEADS heads at a time.  HBM bound for many rows: 2 bytes
-// in, 1 (or 2) and the scale out a value.  What a row's heads need is asked for together, beside its slot, so that a warp has 4 KB on its way;
-// with a head to a half warp (and a 64-bit division in each) 16640 rows of 8 heads took 34 us, written, and 35, read.
-static constexpr int KV_ROW_HEADS = 8, KV_FEW_ROWS = 2400;
-template <bool VEC>
-__global__ void __launch_bounds__(128)
+template <bool VEC, int EACH>
+__global__ void __launch_bounds__(128, EACH == 8 ? 9 : 12)
 kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk, const uint16_t* __restrict__ v, int64_t ldv,
-                const int64_t* __restrict__ slots, int rows, int each, int* err) {
+                const int64_t* __restrict__ slots, unsigned units, int* err) {
     grid_dep_launch();
     grid_dep_wait();
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= rows) return;
-    const int lane = threadIdx.x & 15, from = blockIdx.y * each, heads = min(c.heads, from + each);
+    const unsigned from = (blockIdx.x * 4 + (threadIdx.x >> 5)) * EACH;
+    if (from >= units) return;
+    const int lane = threadIdx.x & 15, count = min((unsigned)EACH, units - from);
     const bool is_v = threadIdx.x & 16;
-    const uint16_t* src = (is_v ? v + row * ldv : k + row * ldk) + lane * 8;
+    const unsigned row = from / (unsigned)c.heads, my_row = (from + lane) / (unsigned)c.heads;
+    const int64_t slot = lane < count ? slots[my_row] : -1, ld = is_v ? ldv : ldk;       // lane i's and 16 + i's: unit i's
+    int head = from - row * c.heads;
+    const uint16_t* src = (is_v ? v : k) + row * ld + lane * 8;
     uint8_t* const base = is_v ? c.v : c.k;
     float* const scales = is_v ? c.vs : c.ks;
-    const int64_t slot = slots[row];
-    for (int h0 = from; h0 < heads; h0 += KV_ROW_HEADS) {
-        uint4 x[KV_ROW_HEADS];
+    float scale = 0.f;
+    uint4 x[EACH];
 #pragma unroll
-        for (int i = 0; i < KV_ROW_HEADS; ++i)
-            if (h0 + i < heads) x[i] = load8<VEC>(src + (h0 + i) * KV_D);
-        const int64_t first = place(slot, c, err);
-        if (first < 0) return;
-#pragma unroll
-        for (int i = 0; i < KV_ROW_HEADS; ++i) {
-            if (h0 + i >= heads) break;
-            const int64_t at = first + (int64_t)(h0 + i) * c.page_size;
-            if (type == KV_BF16) {
-                reinterpret_cast<uint4*>(base)[at * 16 + lane] = x[i];
-                continue;
-            }
-            float scale;
-            reinterpret_cast<uint2*>(base)[at * 16 + lane] = quantise8(x[i], type, scale);
-            if (lane == 0) scales[at] = scale;
-        }
+    for (int i = 0; i < EACH; ++i) {
+        if (i < count) x[i] = load8<VEC>(src + head * KV_D);
+        if (++head == c.heads) { head = 0; src += ld; }
     }
+    const int64_t places = place(slot, from + lane - my_row * c.heads, c, err);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        if (i >= count) break;
+        const int64_t at = __shfl_sync(0xffffffffu, places, i, 16);
+        if (type == KV_BF16) {
+            if (at >= 0) reinterpret_cast<uint4*>(base)[at * 16 + lane] = x[i];
+            continue;
+        }
+        float s;
+        const uint2 codes = quantise8(x[i], type, s);
+        if (at >= 0) reinterpret_cast<uint2*>(base)[at * 16 + lane] = codes;
+        if (lane == i) scale = s;
+    }
+    if (type != KV_BF16 && places >= 0) scales[places] = scale;
 }
 
-template <bool VEC>
-__global__ void __launch_bounds__(128)
+template <bool VEC, int EACH>
+__global__ void __launch_bounds__(128, EACH == 8 ? 7 : 12)
 kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16_t* __restrict__ v, int64_t ldv,
-               const int64_t* __restrict__ slots, int rows, int each, int* err) {
+               const int64_t* __restrict__ slots, unsigned units, int* err) {
     grid_dep_launch();
     grid_dep_wait();
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= rows) return;
-    const int lane = threadIdx.x & 15, from = blockIdx.y * each, heads = min(c.heads, from + each);
+    const unsigned from = (blockIdx.x * 4 + (threadIdx.x >> 5)) * EACH;
+    if (from >= units) return;
+    const int lane = threadIdx.x & 15, count = min((unsigned)EACH, units - from);
     const bool is_v = threadIdx.x & 16;
-    uint16_t* dst = (is_v ? v + row * ldv : k + row * ldk) + lane * 8;
+    const unsigned row = from / (unsigned)c.heads, my_row = (from + lane) / (unsigned)c.heads;
+    const int64_t slot = lane < count ? slots[my_row] : -1, ld = is_v ? ldv : ldk;       // lane i's and 16 + i's: unit i's
+    int head = from - row * c.heads;
+    uint16_t* dst = (is_v ? v : k) + row * ld + lane * 8;
     const uint8_t* const base = is_v ? c.v : c.k;
     const float* const scales = is_v ? c.vs : c.ks;
-    const int64_t first = place(slots[row], c, err);
-    for (int h0 = from; h0 < heads; h0 += KV_ROW_HEADS) {
-        uint4 x[KV_ROW_HEADS];
-        float scale[KV_ROW_HEADS];
+    const int64_t places = place(slot, from + lane - my_row * c.heads, c, err);
+    const float scale = type != KV_BF16 && places >= 0 ? scales[places] : 0.f;
+    uint4 x[EACH];
 #pragma unroll
-        for (int i = 0; i < KV_ROW_HEADS; ++i) {
-            x[i] = make_uint4(0, 0, 0, 0);
-            scale[i] = 0.f;
-            if (h0 + i >= heads || first < 0) continue;
-            const int64_t at = first + (int64_t)(h0 + i) * c.page_size;
-            if (type == KV_BF16) { x[i] = reinterpret_cast<const uint4*>(base)[at * 16 + lane]; continue; }
-            const uint2 codes = reinterpret_cast<const uint2*>(base)[at * 16 + lane];
-            x[i].x = codes.x;
-            x[i].y = codes.y;
-            scale[i] = scales[at];
-        }
+    for (int i = 0; i < EACH; ++i) {
+        const int64_t at = __shfl_sync(0xffffffffu, places, i, 16);
+        x[i] = make_uint4(0, 0, 0, 0);
+        if (at < 0) continue;
+        if (type == KV_BF16) { x[i] = reinterpret_cast<const uint4*>(base)[at * 16 + lane]; continue; }
+        const uint2 codes = reinterpret_cast<const uint2*>(base)[at * 16 + lane];
+        x[i].x = codes.x;
+        x[i].y = codes.y;
+    }
 #pragma unroll
-        for (int i = 0; i < KV_ROW_HEADS; ++i) {
-            if (h0 + i >= heads) break;
-            store8<VEC>(dst + (h0 + i) * KV_D, type == KV_BF16 ? x[i] : dequantise8(make_uint2(x[i].x, x[i].y), type, scale[i]));
-        }
+    for (int i = 0; i < EACH; ++i) {
+        if (i >= count) break;
+        const float s = __shfl_sync(0xffffffffu, scale, i, 16);
+        store8<VEC>(dst + head * KV_D, type == KV_BF16 ? x[i] : dequantise8(make_uint2(x[i].x, x[i].y), type, s));
+        if (++head == c.heads) { head = 0; dst += ld; }
     }
 }
 
@@ -1011,12 +1017,19 @@ hd_status o1_kv_write(const o1_kv_cache* cache, const void* k, int64_t ldk, cons
     if (!k || !v || !slots) { set_error("kv_write: null argument"); return HD_ERR_MISSING; }
     const int64_t row = (int64_t)c.heads * KV_D;
     if (ldk < row || ldv < row) { set_error("kv_write: row pitch below %lld", (long long)row); return HD_ERR_UNSUPPORTED; }
-    const int each = rows < KV_FEW_ROWS ? 2 : KV_ROW_HEADS;
-    auto kern = aligned16(k, ldk) && aligned16(v, ldv) ? kv_write_kernel<true> : kv_write_kernel<false>;
-    if (!launch_ok(launch_chained(kern, dim3((unsigned)(((int64_t)rows + 3) / 4), (unsigned)((c.heads + each - 1) / each)), dim3(128), 0, current_stream(), 1, rows, c, cache->type, (const uint16_t*)k, ldk,
-                                  (const uint16_t*)v, ldv, slots, rows, each, device_error_word()), "kv_write"))
-        return HD_ERR_RUNTIME;
-    o1_launch_count_add(1);
+    const bool vec = aligned16(k, ldk) && aligned16(v, ldv);
+    const int most = INT32_MAX / c.heads;      // of a launch, which counts units in 32 bits
+    for (int first = 0; first < rows; first += most) {
+        const unsigned units = (unsigned)min(most, rows - first) * c.heads;
+        const bool few = units < KV_FEW_UNITS;
+        const unsigned block = 4 * (few ? KV_EACH_OF_FEW : KV_EACH);
+        auto kern = few ? (vec ? kv_write_kernel<true, KV_EACH_OF_FEW> : kv_write_kernel<false, KV_EACH_OF_FEW>) : vec ? kv_write_kernel<true, KV_EACH> : kv_write_kernel<false, KV_EACH>;
+        if (!launch_ok(launch_chained(kern, dim3((units + block - 1) / block), dim3(128), 0, current_stream(), 1, rows, c, cache->type, (const uint16_t*)k + first * ldk, ldk,
+                                      (const uint16_t*)v + first * ldv, ldv, slots + first, units, device_error_word()), "kv_write"))
+            return HD_ERR_RUNTIME;
+        o1_launch_count_add(1);
+        if (rows - first <= most) break;
+    }
     return HD_OK;
 }
 
@@ -1029,12 +1042,19 @@ hd_status o1_kv_read(const o1_kv_cache* cache, void* k, int64_t ldk, void* v, in
     if (!k || !v || !slots) { set_error("kv_read: null argument"); return HD_ERR_MISSING; }
     const int64_t row = (int64_t)c.heads * KV_D;
     if (ldk < row || ldv < row) { set_error("kv_read: row pitch below %lld", (long long)row); return HD_ERR_UNSUPPORTED; }
-    const int each = rows < KV_FEW_ROWS ? 2 : KV_ROW_HEADS;
-    auto kern = aligned16(k, ldk) && aligned16(v, ldv) ? kv_read_kernel<true> : kv_read_kernel<false>;
-    if (!launch_ok(launch_chained(kern, dim3((unsigned)(((int64_t)rows + 3) / 4), (unsigned)((c.heads + each - 1) / each)), dim3(128), 0, current_stream(), 1, rows, c, cache->type, (uint16_t*)k, ldk,
-                                  (uint16_t*)v, ldv, slots, rows, each, device_error_word()), "kv_read"))
-        return HD_ERR_RUNTIME;
-    o1_launch_count_add(1);
+    const bool vec = aligned16(k, ldk) && aligned16(v, ldv);
+    const int most = INT32_MAX / c.heads;      // of a launch, which counts units in 32 bits
+    for (int first = 0; first < rows; first += most) {
+        const unsigned units = (unsigned)min(most, rows - first) * c.heads;
+        const bool few = units < KV_FEW_UNITS;
+        const unsigned block = 4 * (few ? KV_EACH_OF_FEW : KV_EACH);
+        auto kern = few ? (vec ? kv_read_kernel<true, KV_EACH_OF_FEW> : kv_read_kernel<false, KV_EACH_OF_FEW>) : vec ? kv_read_kernel<true, KV_EACH> : kv_read_kernel<false, KV_EACH>;
+        if (!launch_ok(launch_chained(kern, dim3((units + block - 1) / block), dim3(128), 0, current_stream(), 1, rows, c, cache->type, (uint16_t*)k + first * ldk, ldk,
+                                      (uint16_t*)v + first * ldv, ldv, slots + first, units, device_error_word()), "kv_read"))
+            return HD_ERR_RUNTIME;
+        o1_launch_count_add(1);
+        if (rows - first <= most) break;
+    }
     return HD_OK;
 }
 
