@@ -54,27 +54,40 @@ __device__ __forceinline__ uint32_t int8x4(float a, float b, float c, float d) {
 // reciprocal, rounded to nearest even (as are scale and reciprocal, in fp32).  A maximum below 2^-100 counts as 2^-100: its reciprocal stays finite and a
 // row of zeros gets codes of zero.  A row with an Inf or NaN gets a NaN scale: it reads as NaN, as its bf16 form would
 // carry it into the attention, where int8 has no code for either.
-__device__ __forceinline__ uint2 quantise8(const uint4& x, int type, float& scale) {
-    uint32_t top = 0;
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        top = max(top, w[i] & 0x7FFFu);
-        top = max(top, (w[i] >> 16) & 0x7FFFu);
-    }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// Magnitudes of eight values as bits, the largest in each half of a word.
+__device__ __forceinline__ uint32_t magnitudes(const uint4& x) {
+    constexpr uint32_t M = 0x7FFF7FFFu;
+    return max_u16x2(max_u16x2(x.x & M, x.y & M), max_u16x2(x.z & M, x.w & M));
+}
+// Of a row's largest magnitude (either half of a word): scale and reciprocal, 0 where there are no codes.
+__device__ __forceinline__ float scale_of(uint32_t top, int type, float& inv) {
+    top = max(top & 0xFFFFu, top >> 16);
     const bool finite = top < 0x7F80u;
-    const float a = fmaxf(__uint_as_float(top << 16), 7.888609052210118e-31f);
-    const float q = type == KV_INT8 ? 127.0f : 448.0f;
-    scale = finite ? __fdiv_rn(a, q) : __uint_as_float(0x7FC00000u);
-    const float inv = finite ? __fdiv_rn(q, a) : 0.0f;
-    if (!finite) return make_uint2(0, 0);
+    const float a = fmaxf(__uint_as_float(top << 16), 7.888609052210118e-31f), q = type == KV_INT8 ? 127.0f : 448.0f;
+    inv = finite ? __fdiv_rn(q, a) : 0.0f;
+    return finite ? __fdiv_rn(a, q) : __uint_as_float(0x7FC00000u);
+}
+__device__ __forceinline__ uint2 codes_of(const uint4& x, int type, float inv) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
     float f[8];
+    if (inv == 0.0f) return make_uint2(0, 0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) { f[2 * i] = bf16lo(w[i]) * inv; f[2 * i + 1] = bf16hi(w[i]) * inv; }
     if (type == KV_INT8) return make_uint2(int8x4(f[0], f[1], f[2], f[3]), int8x4(f[4], f[5], f[6], f[7]));
     return make_uint2(f32_to_e4m3x2(f[0], f[1]) | (f32_to_e4m3x2(f[2], f[3]) << 16), f32_to_e4m3x2(f[4], f[5]) | (f32_to_e4m3x2(f[6], f[7]) << 16));
+}
+__device__ __forceinline__ uint2 quantise8(const uint4& x, int type, float& scale) {
+    uint32_t top = magnitudes(x);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max_u16x2(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float inv;
+    scale = scale_of(top, type, inv);
+    return codes_of(x, type, inv);
 }
 __device__ __forceinline__ uint4 dequantise8(const uint2& c, int type, float scale) {
     float f[8];
@@ -111,10 +124,11 @@ __device__ __forceinline__ void store8(uint16_t* p, const uint4& v) {
 }
 
 // A unit is a row's head; a warp has EACH of them, behind one another: keys in the lower 16 lanes, values in the others, eight columns to a lane.  HBM bound for
-// many rows: 2 bytes in, 1 (or 2) and the scale out a value.  A lane finds a unit's place and has its scale, and what the units need is asked for together: a warp
-// of eight has 4 KB on its way, one of two, for few rows, more warps.  us, written and read: 16640 rows of 8 heads of int8 22.8 + 18.7 (5.0 TB/s), 100000 rows of
-// one head 18.5 + 15; with a row to a warp, its heads together, 23.5 + 19.5 and 43 + 39; with a head to a half warp 34 + 35 for the former.  Two units or
-// eight to a warp: 2200 rows of 8 heads 4.5 + 4.2 and 6.8 + 4.6, 4111 rows 10 + 7.9 and 6.9 + 6.1.
+// many rows: 2 bytes in, 1 (or 2) and the scale out a value.  What the units need is asked for together (a warp of eight has 4 KB on its way), a lane has one
+// unit's place and scale, and the maxima are found for all units at once: with four exchanges for each and divisions in every lane the write's instructions
+// (135 a unit, against 80) took longer than its bytes, 22.8 us.  Written and read, us: 16640 rows of 8 heads of int8 18.9 + 18.7 (5.5 TB/s), 100000 rows of one head
+// 15.2 + 15.1; a row to a warp 23.5 + 19.5 and 43 + 39, a head to a half warp 34 + 35 for the former.  Few rows have more warps with two units: 1800 rows of
+// 8 heads 3.5 + 3.7, with eight 5.3 + 4.0; 2600 rows 4.5 + 4.7 and 4.3 + 4.3; 4111 rows 6.9 + 7.5 and 5.8 + 6.2.
 static constexpr int KV_EACH = 8, KV_EACH_OF_FEW = 2, KV_FEW_UNITS = 19200;
 // A unit's place in a [pages][heads][page_size] array, -1: none.
 __device__ __forceinline__ int64_t place(int64_t slot, int head, const KvView& c, int* err) {
@@ -133,34 +147,47 @@ kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk,
     if (from >= units) return;
     const int lane = threadIdx.x & 15, count = min((unsigned)EACH, units - from);
     const bool is_v = threadIdx.x & 16;
-    const unsigned row = from / (unsigned)c.heads, my_row = (from + lane) / (unsigned)c.heads;
-    const int64_t slot = lane < count ? slots[my_row] : -1, ld = is_v ? ldv : ldk;       // lane i's and 16 + i's: unit i's
+    const int mine = lane / (16 / EACH);       // the unit whose place and scale are this lane's
+    const unsigned row = from / (unsigned)c.heads, my_row = (from + mine) / (unsigned)c.heads;
+    const int64_t slot = mine < count ? slots[my_row] : -1, ld = is_v ? ldv : ldk;
     int head = from - row * c.heads;
     const uint16_t* src = (is_v ? v : k) + row * ld + lane * 8;
     uint8_t* const base = is_v ? c.v : c.k;
     float* const scales = is_v ? c.vs : c.ks;
-    float scale = 0.f;
     uint4 x[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
+        x[i] = make_uint4(0, 0, 0, 0);
         if (i < count) x[i] = load8<VEC>(src + head * KV_D);
         if (++head == c.heads) { head = 0; src += ld; }
     }
-    const int64_t places = place(slot, from + lane - my_row * c.heads, c, err);
+    const int64_t places = place(slot, from + mine - my_row * c.heads, c, err);
+    float inv = 0.f;
+    if (type != KV_BF16) {
+        // maxima: a step halves the lanes that a unit is spread over, and, until a lane has one, its units
+        uint32_t top[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) top[i] = magnitudes(x[i]);
+#pragma unroll
+        for (int o = 8, n = EACH / 2; o > 0; o >>= 1, n >>= 1) {
+            if (n == 0) top[0] = max_u16x2(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
+#pragma unroll
+            for (int i = 0; i < n; ++i) {
+                const uint32_t keep = lane & o ? top[n + i] : top[i], give = lane & o ? top[i] : top[n + i];
+                top[i] = max_u16x2(keep, __shfl_xor_sync(0xffffffffu, give, o));
+            }
+        }
+        const float scale = scale_of(top[0], type, inv);
+        if (places >= 0 && lane % (16 / EACH) == 0) scales[places] = scale;
+    }
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-        if (i >= count) break;
-        const int64_t at = __shfl_sync(0xffffffffu, places, i, 16);
-        if (type == KV_BF16) {
-            if (at >= 0) reinterpret_cast<uint4*>(base)[at * 16 + lane] = x[i];
-            continue;
-        }
-        float s;
-        const uint2 codes = quantise8(x[i], type, s);
-        if (at >= 0) reinterpret_cast<uint2*>(base)[at * 16 + lane] = codes;
-        if (lane == i) scale = s;
+        const int64_t at = __shfl_sync(0xffffffffu, places, i * (16 / EACH), 16);
+        const float f = __shfl_sync(0xffffffffu, inv, i * (16 / EACH), 16);
+        if (at < 0) continue;
+        if (type == KV_BF16) reinterpret_cast<uint4*>(base)[at * 16 + lane] = x[i];
+        else reinterpret_cast<uint2*>(base)[at * 16 + lane] = codes_of(x[i], type, f);
     }
-    if (type != KV_BF16 && places >= 0) scales[places] = scale;
 }
 
 template <bool VEC, int EACH>
@@ -173,18 +200,19 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
     if (from >= units) return;
     const int lane = threadIdx.x & 15, count = min((unsigned)EACH, units - from);
     const bool is_v = threadIdx.x & 16;
-    const unsigned row = from / (unsigned)c.heads, my_row = (from + lane) / (unsigned)c.heads;
-    const int64_t slot = lane < count ? slots[my_row] : -1, ld = is_v ? ldv : ldk;       // lane i's and 16 + i's: unit i's
+    const int mine = lane / (16 / EACH);       // the unit whose place and scale are this lane's
+    const unsigned row = from / (unsigned)c.heads, my_row = (from + mine) / (unsigned)c.heads;
+    const int64_t slot = mine < count ? slots[my_row] : -1, ld = is_v ? ldv : ldk;
     int head = from - row * c.heads;
     uint16_t* dst = (is_v ? v : k) + row * ld + lane * 8;
     const uint8_t* const base = is_v ? c.v : c.k;
     const float* const scales = is_v ? c.vs : c.ks;
-    const int64_t places = place(slot, from + lane - my_row * c.heads, c, err);
+    const int64_t places = place(slot, from + mine - my_row * c.heads, c, err);
     const float scale = type != KV_BF16 && places >= 0 ? scales[places] : 0.f;
     uint4 x[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-        const int64_t at = __shfl_sync(0xffffffffu, places, i, 16);
+        const int64_t at = __shfl_sync(0xffffffffu, places, i * (16 / EACH), 16);
         x[i] = make_uint4(0, 0, 0, 0);
         if (at < 0) continue;
         if (type == KV_BF16) { x[i] = reinterpret_cast<const uint4*>(base)[at * 16 + lane]; continue; }
@@ -195,7 +223,7 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
         if (i >= count) break;
-        const float s = __shfl_sync(0xffffffffu, scale, i, 16);
+        const float s = __shfl_sync(0xffffffffu, scale, i * (16 / EACH), 16);
         store8<VEC>(dst + head * KV_D, type == KV_BF16 ? x[i] : dequantise8(make_uint2(x[i].x, x[i].y), type, s));
         if (++head == c.heads) { head = 0; dst += ld; }
     }
