@@ -759,8 +759,10 @@ int o1_parallel_layout(int world, int rank, int *image, int *branch, int *sp_ran
  * O1_KV_FP8 (e4m3) and O1_KV_INT8 as codes of a byte with one fp32 scale for each token and head, k_scale and v_scale
  * [pages][kv_heads][page_size] (16-byte aligned): scale = max|x| / 448 or / 127, code = x / scale to the nearest, ties to even.  A row with an Inf
  * or NaN gets a NaN scale and reads as NaN.  A token's slot is page * page_size + its place in the page.
+ * Codes are those that o1_kv_write makes: in particular no e4m3 NaN (0x7F, 0xFF), whose row has its NaN in the scale.
  * A slot or page outside the cache, or a length outside its table, found on the device: nothing outside the cache is read or
- * written, that row's or sequence's result means nothing, and the device error word gets 70 or 71 (o1_device_error). */
+ * written, that row's or sequence's result means nothing, and the device error word gets 70 (slot or page) or 71 (length); 72 is a wait that ran
+ * out (o1_device_error). */
 enum { O1_KV_BF16 = 0, O1_KV_FP8 = 1, O1_KV_INT8 = 2 };
 typedef struct {
     void *k, *v;
@@ -780,7 +782,8 @@ hd_status o1_kv_read(const o1_kv_cache *cache, void *k, int64_t ldk, void *v, in
  * k_new / v_new (both or neither): each sequence's row at position lens[b] - 1, stored into the cache (as by o1_kv_write) and
  * attended to by the same call.  workspace: o1_kv_attention_workspace_bytes(heads, kv_heads) bytes, 16-byte aligned, zero-filled once before its first use and
  * left to these calls from then on; calls that may overlap on the GPU each need their own.  The result is the same
- * bits from call to call. */
+ * bits from call to call.  Values of v up to 2^90 in magnitude (the sums are 2^20 times larger and in fp32); at most 2^31 - 1 rows (pages *
+ * kv_heads * page_size) in the cache. */
 int64_t o1_kv_attention_workspace_bytes(int heads, int kv_heads);
 hd_status o1_kv_attention(const o1_kv_cache *cache, const void *q, int64_t ldq, const void *k_new, int64_t ldk,
                           const void *v_new, int64_t ldv, const int32_t *pages, int64_t ldp, int width, const int32_t *lens,

@@ -230,34 +230,46 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
 }
 
 // ------------------------------------------------------------------ attention of a new row
-// HBM bound: every cached value is read once and used by the G = heads / kv_heads queries that share it, 2 G multiply-adds for its one or two bytes,
-// so all that counts is that enough bytes are on their way at all times, on all SMs, whatever the lengths are.
+// out = sum_t p_t v_t / sum_t p_t, p_t = exp(scale q . k_t - max): one pass over the keys with a running maximum and sum (in base 2).  HBM bound: every cached
+// value is read once and used by the G = heads / kv_heads queries that share it, 2 G multiply-adds for its one or two bytes, so all that counts is that
+// enough bytes are on their way at all times, on all SMs, whatever the lengths are.  Measured: 582 MB of fp8 rows (96 sequences of 300 to 5400 tokens, 8 kv heads) in
+// 97 us, 6.0 TB/s, 92 % of a copy's rate; 211 MB of int8 (one sequence of 100003) in 46 us, 4.6 TB/s; 100 MB of bf16 (24 sequences of 1 to 2100) in 25 us.
+// With few bytes the chain of steps counts: 2.3 us until the first loads are asked for (lengths, their sums, parts, pages), 2 for them, 1.3 for the
+// warps' join, 3 for that of the teams: 85 tokens of one sequence take 5.8 us, 600 take 8.5.
 //
 //  * The work is one stream of chunks (16 tokens, 32 of a quantised cache: 8 KB of keys and values) over sequences, kv heads and length.  A block is one SM's; its
-//    consumer warps form teams of four, and every team takes an equal, contiguous part of the stream.  How long that is follows from the lengths, which only the
-//    device knows: each block sums them up.
+//    consumer warps form teams of four, and every team takes a contiguous part of the stream, of equal cost.  How long that is follows from the lengths, which only the
+//    device knows: each block sums them up.  (Parts of an equal number of chunks, whatever they hold, kept SMs busy for between 24 and 49 us with the 211 MB.)
 //  * A fifth warp of each team does its loading: lane w walks the chunks of consumer warp w (every fourth one of the team's part), looks their pages up a round ahead,
 //    and one thread asks for them by TMA, into a ring that each consumer warp has of its own.  So loads run ahead over the ends of sequences, and a consumer
-//    does nothing but arithmetic: with loads of its own (cp.async) a chunk of codes was 920 instructions, of which an SM issued 2.3 a clock.
+//    does nothing but arithmetic: with loads of its own (cp.async) a chunk of codes was 920 instructions, of which an SM issued 2.3 a clock.  One loading warp
+//    for an SM was not enough: 145 us where one for each team took 107.
 //  * Products on the tensor cores (mma.sync: at most 16 rows of queries, tcgen05's tiles have 64 at least).  Scores: A = queries (rows = heads), B = keys.
 //    Their accumulators are, packed in pairs, the B operand of the second product, A = values transposed (rows = columns of a head).  The operands' k and row
 //    indices are permuted so that a thread's part of a key or value row is 16 contiguous bytes, and so that the eight threads which a step of a shared-memory
-//    load serves meet eight different sets of banks in TMA's 128-byte swizzle.
-//  * One pass with a running maximum and sum (in base 2) for each warp.  A team's warps join in shared memory.  Where teams share a (sequence, kv head), each
-//    leaves its maximum, sum and weighted sum, and the last team to come adds them up (of many: the last of each group, then the last group), always in the
-//    order of the teams: the result does not depend on which came when.
+//    load serves meet eight different sets of banks in TMA's 128-byte swizzle.  The arithmetic alone takes 91 us for the 582 MB, the loads alone 101 (then).
+//  * A team's warps join in shared memory.  Where teams share an item - a (sequence, kv head, up to 16 of its query heads) - each leaves its maximum, sum and weighted
+//    sum, and the last team to come adds them up (of many: the last of each group, then the last group), always in the order of the teams: the result does not
+//    depend on which came when.  Which teams share an item is found while the first rows load, and a warp's heads are joined at once: a head after the
+//    other, 16 heads on one kv head took 45 us for 50000 bf16 rows, now 21.
 //  * Rounding: scores and sums in fp32.  Probabilities (times v's scale) enter the second product as two parts of bf16, value and rest, 16 bits of significand; codes
 //    of a byte are exact in f16 and bf16.  Keys' codes go through f16, which takes fewer instructions, with queries scaled to f16 by a power of two for each head;
 //    values' codes through bf16, whose range a probability needs.  The result is rounded once.
+// Times below: "batch" 24 sequences of 1 to 2100 rows of bf16, "shared" 32 sequences of 1000 to 3000, 16 query heads on one kv head; us.
 static constexpr int KV_STAGE_BYTES = 8192;            // keys and values of a chunk
 static constexpr int KV_SEQS = 256;                    // sequences of a launch
 static constexpr int KV_TEAM = 4;                      // warps
 static constexpr int KV_TEAMS_MAX = 160 * 3;           // what the workspace has room for
-static constexpr int KV_FLAT = 32, KV_FAN = 16;          // up to so many teams' parts are joined at once, more in groups of so many
-static constexpr int KV_ITEM_COST = 10;                // what an item costs a team beside its chunks, in chunks
-static constexpr int KV_KEEP = 16;                     // items of so few chunks are not cut
+// Up to so many teams' parts of an item are joined at once (a part to a lane), more in groups of so many: 100003 tokens, 55 parts to an item, in two steps 48.1 us, at once 50.8 (then).
+static constexpr int KV_FLAT = 32, KV_FAN = 16;
+// What an item costs a team beside its chunks (the warps' join, the next queries), in chunks: 4, 7, 10, 12: batch 26.1, 25.5, 24.9, 24.5, shared 22.5, 20.0, 18.1, 17.8,
+// 582 MB 97.4, 97.1, 96.9, 97.6.
+static constexpr int KV_ITEM_COST = 10;
+// Items of so few chunks, or of a quarter of a team's part (half: 582 MB 104), are not cut: 9 sequences of up to 1999 rows of fp8, 16 kv heads: 16 or 24 18, 48 26;
+// 60 of 100 to 900 rows of int8: 16 18.3, 24 19.8.
+static constexpr int KV_KEEP = 16;
 static constexpr int KV_JOIN_BYTES = 8192;             // of a team
-static constexpr int KV_JOIN_STEP = 4;                 // parts that a join has under way
+static constexpr int KV_JOIN_STEP = 4;                 // parts that a join has under way (of all a warp's heads; two take 1 us longer for 16 heads, eight spill registers)
 static constexpr int ERR_KV_WAIT = 72;                 // a wait of the attention kernel ran out
 static constexpr float KV_LIFT = 20.0f;                // probabilities are relative to 2^-20 of the largest: those that fp32 has no value for are 2^-146 and less of it
 
@@ -357,7 +369,8 @@ __device__ __forceinline__ int kv_perm(int i) { return (i >> 1) | (i & 1) << 2; 
 template <int TYPE, int HG>
 struct KvKernel {
     static constexpr int KEYS = TYPE == KV_BF16 ? 16 : 32, ROWB = TYPE == KV_BF16 ? 256 : 128, TILES = KEYS / 8;
-    static constexpr int TEAMS = HG == 1 ? 3 : 2, WARPS = KV_TEAM * TEAMS, STAGES = HG == 1 ? 2 : 3, THREADS = (WARPS + TEAMS) * 32;      // (as registers and shared memory allow)
+    static constexpr int TEAMS = HG == 1 ? 3 : 2, WARPS = KV_TEAM * TEAMS, STAGES = HG == 1 ? 2 : 3, THREADS = (WARPS + TEAMS) * 32;
+    // (HG == 1: 128 registers and 24 slots of 8 KB; HG == 2 holds twice the queries and sums: 168 registers, two teams, again 24 slots)
     // shared memory: the rings, their scales, the teams' join buffers, then Shared
     static constexpr int SCALES = WARPS * STAGES * KV_STAGE_BYTES, JOIN = SCALES + (TYPE == KV_BF16 ? 0 : WARPS * STAGES * 256), SHARED = JOIN + TEAMS * KV_JOIN_BYTES;
     struct Share { int first, here, fan, item, groups, b, head0, heads; };        // a part's group begins at part `first` and has `here` (0: no part), its item at part `item`
@@ -543,7 +556,9 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         __syncthreads();
     }
     // ---- a team's part of the stream: equal costs, where each item costs some chunks more than it has; ends inside an item that is not worth a join are moved
-    const int least = all_chunks > 32 * sequences ? 2 * KV_TEAM : KV_TEAM, teams = min((int)gridDim.x * K::TEAMS, (total + least - 1) / least);
+    // (A team has at least four chunks, one to a warp; eight where sequences are long, which halves the parts to join: one sequence of 2000 rows of bf16 10.3 us, with four
+    // 11.7; of 600 rows 9.1 and 8.5.)
+    const int least = all_chunks > 48 * sequences ? 2 * KV_TEAM : KV_TEAM, teams = min((int)gridDim.x * K::TEAMS, (total + least - 1) / least);
     const int share = teams > 0 ? total / teams : 0, keep = max(KV_KEEP, share >> 2);
     const int each = teams > 0 ? cost / teams : 0, over = cost - each * teams;
     auto cost_of = [&](int id) { return each * id + over * id / teams; };         // cost * id / teams, in 32 bits (over and id are below 480)
