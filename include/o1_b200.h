@@ -452,6 +452,8 @@ hd_status o1_decoder_block_adaln(const void *in_dev, const float *pos_dev, const
 /* Stream every later call enqueues on (a cudaStream_t; NULL = legacy default). */
 void o1_set_stream(void *stream);
 void *o1_get_stream(void);
+/* The capture that stream is in, by a number of its own; 0: none.  (What a captured call keeps for itself must not serve calls outside.) */
+uint64_t o1_capture_id(void);
 /* Kernels whose bounded waits ran out record a code in a device word;
  * this reads and clears it (synchronises the current stream). 0 = clean. */
 int o1_device_error(void);

@@ -19,13 +19,14 @@ decltype(&o1_kv_read) f_read;
 decltype(&o1_kv_attention) f_attend;
 decltype(&o1_residual_norm) f_norm;
 decltype(&o1_get_stream) f_stream;
+decltype(&o1_capture_id) f_capture;
 PyObject *O1Error, *check;
 
 struct Handle {
     const o1_kv_cache* cache;
     int64_t heads;
     int device;
-    struct Work { void* stream; int64_t heads; void* p; int64_t bytes; };
+    struct Work { void* stream; uint64_t capture; int64_t heads; void* p; int64_t bytes; };
     std::vector<Work> work;
 };
 
@@ -178,13 +179,14 @@ PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const double scale = a[9] == Py_None ? 0.08838834764831845 : PyFloat_AsDouble(a[9]);
     if (PyErr_Occurred()) return nullptr;
     void* const stream = f_stream();
+    const uint64_t capture = f_capture();
     const Handle::Work* work = nullptr;
     for (const auto& w : h->work)
-        if (w.stream == stream && w.heads == heads) work = &w;
+        if (w.stream == stream && w.capture == capture && w.heads == heads) work = &w;
     if (!work) {       // the cache object makes it, and keeps it
         PyObject* made = PyObject_CallMethod(a[1], "_workspace", "L", (long long)heads);
         if (!made) return nullptr;
-        Handle::Work w = {stream, heads, nullptr, 0};
+        Handle::Work w = {stream, capture, heads, nullptr, 0};
         unsigned long long p = 0;
         long long bytes = 0;
         const int got = PyArg_ParseTuple(made, "KL", &p, &bytes);
@@ -288,19 +290,20 @@ PyObject* py_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// setup(addresses of o1_kv_write, o1_kv_read, o1_kv_attention, o1_residual_norm, o1_get_stream; O1Error; check)
+// setup(addresses of o1_kv_write, o1_kv_read, o1_kv_attention, o1_residual_norm, o1_get_stream, o1_capture_id; O1Error; check)
 PyObject* py_setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    if (!arguments(n, 7)) return nullptr;
-    unsigned long long p[5];
-    for (int i = 0; i < 5; ++i) p[i] = PyLong_AsUnsignedLongLong(a[i]);
+    if (!arguments(n, 8)) return nullptr;
+    unsigned long long p[6];
+    for (int i = 0; i < 6; ++i) p[i] = PyLong_AsUnsignedLongLong(a[i]);
     if (PyErr_Occurred()) return nullptr;
     f_write = (decltype(f_write))p[0];
     f_read = (decltype(f_read))p[1];
     f_attend = (decltype(f_attend))p[2];
     f_norm = (decltype(f_norm))p[3];
     f_stream = (decltype(f_stream))p[4];
-    O1Error = Py_NewRef(a[5]);
-    check = Py_NewRef(a[6]);
+    f_capture = (decltype(f_capture))p[5];
+    O1Error = Py_NewRef(a[6]);
+    check = Py_NewRef(a[7]);
     Py_RETURN_NONE;
 }
 

@@ -134,6 +134,12 @@ const char* hd_lora_last_error(void) { return g_lora_err; }
 
 void o1_set_stream(void* stream) { g_stream = (cudaStream_t)stream; }
 void* o1_get_stream(void) { return (void*)g_stream; }
+uint64_t o1_capture_id(void) {
+    cudaStreamCaptureStatus status;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(g_stream, &status, &id) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
+    return status == cudaStreamCaptureStatusActive ? id : 0;
+}
 int o1_sm_count(void) { return sm_count(); }
 void o1_launch_count_add(int n) { count(n); }
 int64_t o1_launch_count(int reset) {

@@ -21,12 +21,19 @@ KINDS = {"bf16": (0, torch.bfloat16), "fp8": (1, torch.float8_e4m3fn), "int8": (
 _BY_DTYPE = {d: n for n, d in KINDS.values()}
 BF16, I32, I64, F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
 _stream = lib.o1_get_stream
-_binding.setup(*(C.cast(f, C.c_void_p).value for f in (lib.o1_kv_write, lib.o1_kv_read, lib.o1_kv_attention, lib.o1_residual_norm, lib.o1_get_stream)), O1Error, check)
+_binding.setup(*(C.cast(f, C.c_void_p).value for f in (lib.o1_kv_write, lib.o1_kv_read, lib.o1_kv_attention, lib.o1_residual_norm, lib.o1_get_stream, lib.o1_capture_id)),
+               O1Error, check)
 
 
 def _need(ok, what):
     if not ok:
         raise O1Error(what)
+
+
+def _zeros(n, device):
+    """n bytes of zeros, filled on the library's current stream."""
+    with torch.cuda.stream(torch.cuda.ExternalStream(_stream() or 0, device)):
+        return torch.zeros(n, dtype=torch.uint8, device=device)
 
 
 class KvCache:
@@ -80,10 +87,11 @@ class KvCache:
         return _binding.read(self._h, slots, *out)
 
     def _workspace(self, heads):
-        """Scratch of attend(), its address and bytes: one for each stream the calls run on, as calls that overlap must not share it."""
+        """Scratch of attend(), its address and bytes: one for each stream the calls run on and for each capture, as calls that overlap must not share it
+        (and a capture's is filled by its graph).  Kept as long as the cache."""
         need = lib.o1_kv_attention_workspace_bytes(heads, self.kv_heads)
         _need(need >= 0, f"KvCache.attend: heads {heads} (a multiple of kv_heads {self.kv_heads})")
-        t = self._work[_stream(), heads] = torch.zeros(need, dtype=torch.uint8, device=self.device)
+        t = self._work[_stream(), lib.o1_capture_id(), heads] = _zeros(need, self.device)
         return t.data_ptr(), need
 
     def attend(self, q, pages, lens, k=None, v=None, out=None, lse=None, scale=None):
@@ -130,7 +138,7 @@ class Decoder:
         s = self._scratch.get(key)
         need = lib.o1_decode_scratch_bytes(rows, *self.dims[:5])
         if s is None or s.numel() < need:
-            s = self._scratch[key] = torch.zeros(need, dtype=torch.uint8, device=self.device)
+            s = self._scratch[key] = _zeros(need, self.device)
         return s
 
     def _grow(self, seq, tokens):

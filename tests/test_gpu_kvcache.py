@@ -422,6 +422,44 @@ def test_other_streams_and_graphs(pkg, dev):
     assert torch.equal(out, c.cache.attend(q, c.dtable, torch.tensor([100, 0, 33], dtype=torch.int32, device=dev)))
 
 
+@gpu
+def test_captures_share_no_workspace(pkg, dev):
+    """The first call on a stream may be a captured one; graphs of one stream, replayed in any order or on other streams, and calls outside do not share scratch."""
+    c = Case(pkg, dev, "int8", [5000, 2000], 1, 32)
+    c.fill()
+    host = normal((2, 8, D), gen(3))
+    q = host.to(dev)
+    outs = [torch.zeros(2, 8, D, dtype=torch.bfloat16, device=dev) for _ in range(4)]
+    s, other = torch.cuda.Stream(), torch.cuda.Stream()
+    try:
+        graphs = []
+        for i in range(2):
+            torch.cuda.synchronize()
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[i], stream=s):
+                pkg.use_torch_stream()
+                assert pkg.lib.o1_capture_id() != 0
+                c.cache.attend(q, c.dtable, c.dlens, out=outs[i])
+                c.cache.attend(q, c.dtable, c.dlens, out=outs[i])
+        with torch.cuda.stream(s):
+            pkg.use_torch_stream()
+            assert pkg.lib.o1_capture_id() == 0
+            c.cache.attend(q, c.dtable, c.dlens, out=outs[2])
+        assert len(c.cache._work) == 3 and len({t.data_ptr() for t in c.cache._work.values()}) == 3
+        torch.cuda.synchronize()
+        for _ in range(5):
+            with torch.cuda.stream(s):
+                graphs[1].replay()
+            with torch.cuda.stream(other):
+                graphs[0].replay()
+        torch.cuda.synchronize()
+    finally:
+        pkg.use_torch_stream()
+    c.cache.attend(q, c.dtable, c.dlens, out=outs[3])
+    assert all(torch.equal(o, outs[3]) for o in outs)
+    c.check(host, outs[0])
+
+
 # ------------------------------------------------------------------ refusals
 @gpu
 def test_arguments_that_do_not_fit(pkg, dev):
