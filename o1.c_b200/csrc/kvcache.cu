@@ -667,14 +667,19 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         return kvh * a.group + (item - kvh * a.chunks_of_heads) * (8 * HG);
     };
     auto heads_of = [&](int item) { return a.chunks_of_heads == 1 ? a.group : min(8 * HG, a.group - item % a.chunks_of_heads * (8 * HG)); };
-    // queries: rows g (and g + 8) of the A operand; the 16-byte pieces 4i + t of a key row are this thread's
+    // queries: rows g (and g + 8) of the A operand; the 16-byte pieces 4i + t of a key row are this thread's.  Up to four heads are there twice: rows 4 to 7 of the
+    // probabilities are then the second parts of rows 0 to 3, and one product has both (582 MB of fp8 without a pause, at the 1620 MHz that 1000 W allow: 107 us, with two
+    // products 109.5; a chunk of bf16 has half as many products, and gains nothing)
+    const bool twice = HG == 1 && TYPE != KV_BF16 && a.group <= 4;
+    const bool second = twice && g >= 4;
     uint32_t qa[HG][16];
     auto ask_queries = [&](int b, int item) {
         const int head0 = head_of(item), heads = heads_of(item);
 #pragma unroll
         for (int h = 0; h < HG; ++h) {
-            const bool on = g + 8 * h < heads;
-            const uint16_t* src = a.q + b * a.ldq + (head0 + g + 8 * h) * KV_D;
+            const int row = twice ? g & 3 : g + 8 * h;
+            const bool on = row < heads;
+            const uint16_t* src = a.q + b * a.ldq + (head0 + row) * KV_D;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int at = TYPE == KV_BF16 ? (4 * i + t) * 8 : (4 * (i >> 1) + t) * 16 + (i & 1) * 8;
@@ -874,7 +879,10 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 #pragma unroll
                 for (int h = 0; h < HG; ++h) {
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) two_parts(s[2 * u + j][2 * h], s[2 * u + j][2 * h + 1], p_hi[h][j], p_lo[h][j]);
+                    for (int j = 0; j < 2; ++j) {
+                        two_parts(s[2 * u + j][2 * h], s[2 * u + j][2 * h + 1], p_hi[h][j], p_lo[h][j]);
+                        if (second) p_hi[h][j] = p_lo[h][j];
+                    }
                 }
                 constexpr int PIECES = TYPE == KV_BF16 ? 2 : 1;
                 uint4 v[4][PIECES];
@@ -920,7 +928,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 #pragma unroll
                         for (int j = 0; j < EACH; ++j) {
                             mma_bf16(acc[h][EACH * w + j], pair[0][0][j], pair[0][1][j], pair[1][0][j], pair[1][1][j], p_hi[h][0], p_hi[h][1]);
-                            mma_bf16(acc[h][EACH * w + j], pair[0][0][j], pair[0][1][j], pair[1][0][j], pair[1][1][j], p_lo[h][0], p_lo[h][1]);
+                            if (!twice) mma_bf16(acc[h][EACH * w + j], pair[0][0][j], pair[0][1][j], pair[1][0][j], pair[1][1][j], p_lo[h][0], p_lo[h][1]);
                         }
                     }
                 }
@@ -939,6 +947,13 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
             if (t == 0) { sh.m[team][mate][8 * h + g] = m[h]; sh.l[team][mate][8 * h + g] = l[h]; }
+        }
+        if (twice) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[0][j][c] += __shfl_xor_sync(0xffffffffu, acc[0][j][c], 2);
+            }
         }
         const bool whole = seg.begin == seg.first && seg.end == seg.first + seg.n;
         const int64_t mine = (int64_t)(2 * id + (seg.begin == c0 ? 0 : 1)) * a.per_item;
