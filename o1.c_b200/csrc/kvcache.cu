@@ -233,7 +233,7 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
 // out = sum_t p_t v_t / sum_t p_t, p_t = exp(scale q . k_t - max): one pass over the keys with a running maximum and sum (in base 2).  HBM bound: every cached
 // value is read once and used by the G = heads / kv_heads queries that share it, 2 G multiply-adds for its one or two bytes, so all that counts is that
 // enough bytes are on their way at all times, on all SMs, whatever the lengths are.  Measured: 582 MB of fp8 rows (96 sequences of 300 to 5400 tokens, 8 kv heads) in
-// 97 us, 6.0 TB/s, 92 % of a copy's rate; 211 MB of int8 (one sequence of 100003) in 46 us, 4.6 TB/s; 100 MB of bf16 (24 sequences of 1 to 2100) in 25 us.
+// 97 us, 6.0 TB/s, 92 % of a copy's rate (107 without a pause, when 1000 W allow 1620 MHz); 211 MB of int8 (one sequence of 100003) in 46 us, 4.6 TB/s; 100 MB of bf16 (24 sequences of 1 to 2100) in 25 us.
 // With few bytes the chain of steps counts: 2.3 us until the first loads are asked for (lengths, their sums, parts, pages), 2 for them, 1.3 for the
 // warps' join, 3 for that of the teams: 85 tokens of one sequence take 5.8 us, 600 take 8.5.
 //
