@@ -778,7 +778,7 @@ hd_status o1_kv_write(const o1_kv_cache *cache, const void *k, int64_t ldk, cons
 /* The rows back as bf16(code * scale); zeros for a negative slot. */
 hd_status o1_kv_read(const o1_kv_cache *cache, void *k, int64_t ldk, void *v, int64_t ldv, const int64_t *slots, int rows);
 /* Attention of one new row of each sequence over its lens[b] cached rows: token t of sequence b is in page pages[b * ldp + t /
- * page_size] (int32, width columns; entries behind a sequence's last page are not read).  q / out [batch, ldq / ldo] bf16, heads of 128
+ * page_size] (int32, width columns; entries behind a sequence's last page are not used).  q / out [batch, ldq / ldo] bf16, heads of 128
  * columns, heads a multiple of kv_heads (query head j reads kv head j / (heads / kv_heads)); lse (may be NULL) [batch, heads] fp32:
  * log of the sum of exponentials, to join the result with that of other keys.  lens[b] == 0: out row 0, lse -inf.
  * k_new / v_new (both or neither): each sequence's row at position lens[b] - 1, stored into the cache (as by o1_kv_write) and

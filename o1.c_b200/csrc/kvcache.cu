@@ -543,6 +543,13 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     {
         static_assert(KV_SEQS <= K::THREADS, "a sequence to a thread");
         int len = tid < a.batch ? a.lens[tid] : 0;
+        // a short page table into L1 meanwhile, a line to a thread (0.1 to 0.2 us of a call)
+        const int lines = (a.width + 31) >> 5;
+        if (tid < a.batch * lines) {
+            int entry;
+            const int b = tid / lines;
+            asm volatile("ld.global.ca.b32 %0, [%1];" : "=r"(entry) : "l"(a.pages + b * a.ldp + (tid - b * lines) * 32));
+        }
         if (len < 0 || len > (int64_t)a.width * ps) { atomicExch(a.err, ERR_KV_LENGTH); len = 0; }
         const int n = (len + KEYS - 1) / KEYS;
         int2 all;

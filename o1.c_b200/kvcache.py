@@ -97,7 +97,7 @@ class KvCache:
     def attend(self, q, pages, lens, k=None, v=None, out=None, lse=None, scale=None):
         """Attention of one new row per sequence, q [batch, heads, 128] bf16, over its first lens[b] cached rows.
 
-        pages [batch, width] int32: the pages of each sequence in order (entries behind its last page are not read); lens [batch] int32.
+        pages [batch, width] int32: the pages of each sequence in order (entries behind its last page are not used); lens [batch] int32.
         k, v [batch, kv_heads, 128]: each sequence's row at position lens[b] - 1, stored into the cache and attended to.
         Returns out [batch, heads, 128] bf16, with lse=True (or a tensor [batch, heads] fp32) a pair (out, log-sum-exp).  An empty sequence
         gives zeros and -inf.  scale: 1 / sqrt(128)."""
