@@ -565,7 +565,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     // ---- a team's part of the stream: equal costs, where each item costs some chunks more than it has; ends inside an item that is not worth a join are moved
     // (A team has at least four chunks, one to a warp; eight where sequences are long, which halves the parts to join: one sequence of 2000 rows of bf16 10.3 us, with four
     // 11.7; of 600 rows 9.1 and 8.5.)
-    const int least = all_chunks > 48 * sequences ? 2 * KV_TEAM : KV_TEAM, teams = min((int)gridDim.x * K::TEAMS, (total + least - 1) / least);
+    const int least = all_chunks > 48 * sequences ? 2 * KV_TEAM : KV_TEAM, teams = min((int)gridDim.x * K::TEAMS, max((total + least - 1) / least, sequences * items));
     const int share = teams > 0 ? total / teams : 0, keep = max(KV_KEEP, share >> 2);
     const int each = teams > 0 ? cost / teams : 0, over = cost - each * teams;
     auto cost_of = [&](int id) { return each * id + over * id / teams; };         // cost * id / teams, in 32 bits (over and id are below 480)
@@ -1033,12 +1033,12 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 }
 
 template <int TYPE, int HG>
-static cudaError_t launch_attention(const CUtensorMap& k_map, const CUtensorMap& v_map, const KvAttn& a, int64_t chunks, cudaStream_t st) {
+static cudaError_t launch_attention(const CUtensorMap& k_map, const CUtensorMap& v_map, const KvAttn& a, int64_t chunks, int64_t items, cudaStream_t st) {
     static std::atomic<uint64_t> done{0};
     using K = KvKernel<TYPE, HG>;
     static_assert(K::SMEM <= 232448, "more than an SM's block can have");
     if (!func_attr_once(done, (const void*)kv_attention_kernel<TYPE, HG>, K::SMEM, "kv_attention")) return cudaErrorInvalidValue;
-    const int blocks = (int)min((int64_t)min(sm_count(), KV_TEAMS_MAX / K::TEAMS), (chunks + KV_TEAM - 1) / KV_TEAM);
+    const int blocks = (int)min((int64_t)min(sm_count(), KV_TEAMS_MAX / K::TEAMS), max((chunks + KV_TEAM - 1) / KV_TEAM, items));
     return launch_chained(kv_attention_kernel<TYPE, HG>, dim3((unsigned)max(1, blocks)), dim3(K::THREADS), K::SMEM, st, 1, 1, k_map, v_map, a);
 }
 
@@ -1176,11 +1176,11 @@ hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, 
         a.lens = lens + b;
         a.out = (uint16_t*)out + b * ldo;
         a.lse = lse ? lse + (int64_t)b * heads : nullptr;
-        const int64_t chunks = each * a.batch;
+        const int64_t chunks = each * a.batch, items = (int64_t)c.heads * of_heads * a.batch;
         cudaError_t e;
-        if (cache->type == O1_KV_BF16) e = hg == 1 ? launch_attention<KV_BF16, 1>(k_map, v_map, a, chunks, current_stream()) : launch_attention<KV_BF16, 2>(k_map, v_map, a, chunks, current_stream());
-        else if (cache->type == O1_KV_FP8) e = hg == 1 ? launch_attention<KV_FP8, 1>(k_map, v_map, a, chunks, current_stream()) : launch_attention<KV_FP8, 2>(k_map, v_map, a, chunks, current_stream());
-        else e = hg == 1 ? launch_attention<KV_INT8, 1>(k_map, v_map, a, chunks, current_stream()) : launch_attention<KV_INT8, 2>(k_map, v_map, a, chunks, current_stream());
+        if (cache->type == O1_KV_BF16) e = hg == 1 ? launch_attention<KV_BF16, 1>(k_map, v_map, a, chunks, items, current_stream()) : launch_attention<KV_BF16, 2>(k_map, v_map, a, chunks, items, current_stream());
+        else if (cache->type == O1_KV_FP8) e = hg == 1 ? launch_attention<KV_FP8, 1>(k_map, v_map, a, chunks, items, current_stream()) : launch_attention<KV_FP8, 2>(k_map, v_map, a, chunks, items, current_stream());
+        else e = hg == 1 ? launch_attention<KV_INT8, 1>(k_map, v_map, a, chunks, items, current_stream()) : launch_attention<KV_INT8, 2>(k_map, v_map, a, chunks, items, current_stream());
         if (!launch_ok(e, "kv_attention")) return HD_ERR_RUNTIME;
         o1_launch_count_add(1);
     }
