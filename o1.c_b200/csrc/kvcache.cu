@@ -251,7 +251,8 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
 //  * A team's warps join in shared memory.  Where teams share an item - a (sequence, kv head, up to 16 of its query heads) - each leaves its maximum, sum and weighted
 //    sum, and the last team to come adds them up (of many: the last of each group, then the last group), always in the order of the teams: the result does not
 //    depend on which came when.  Which teams share an item is found while the first rows load, and a warp's heads are joined at once: a head after the
-//    other, 16 heads on one kv head took 45 us for 50000 bf16 rows, now 21.
+//    other, 16 heads on one kv head took 45 us for 50000 bf16 rows, now 21.  An item costs a team 3.8 us however short it is, so where the table is short and items
+//    are many, each goes to one warp, which needs no join (200 sequences of 30 rows of fp8, 8 kv heads: 20 us, now 7.7).
 //  * Rounding: scores and sums in fp32.  Probabilities (times v's scale) enter the second product as two parts of bf16, value and rest, 16 bits of significand; codes
 //    of a byte are exact in f16 and bf16.  Keys' codes go through f16, which takes fewer instructions, with queries scaled to f16 by a power of two for each head;
 //    values' codes through bf16, whose range a probability needs.  The result is rounded once.
@@ -268,6 +269,8 @@ static constexpr int KV_ITEM_COST = 10;
 // Items of so few chunks, or of a quarter of a team's part (half: 582 MB 104), are not cut: 9 sequences of up to 1999 rows of fp8, 16 kv heads: 16 or 24 18, 48 26;
 // 60 of 100 to 900 rows of int8: 16 18.3, 24 19.8.
 static constexpr int KV_KEEP = 16;
+static constexpr int KV_SOLO = 16;                     // chunks of an item that a warp can have for itself (no item of KV_KEEP chunks is cut)
+static_assert(KV_SOLO <= KV_KEEP, "an item of a warp is whole");
 static constexpr int KV_JOIN_BYTES = 8192;             // of a team
 static constexpr int KV_JOIN_STEP = 4;                 // parts that a join has under way (of all a warp's heads; two take 1 us longer for 16 heads, eight spill registers)
 static constexpr int ERR_KV_WAIT = 72;                 // a wait of the attention kernel ran out
@@ -520,7 +523,8 @@ __device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, 
     }
 }
 
-template <int TYPE, int HG>
+// solo: items of at most KV_SOLO chunks, each to one warp; "teams" are then warps.
+template <int TYPE, int HG, bool solo>
 __global__ void __launch_bounds__(KvKernel<TYPE, HG>::THREADS, 1)
 kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ KvAttn a) {
     using K = KvKernel<TYPE, HG>;
@@ -565,10 +569,11 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     // ---- a team's part of the stream: equal costs, where each item costs some chunks more than it has; ends inside an item that is not worth a join are moved
     // (A team has at least four chunks, one to a warp; eight where sequences are long, which halves the parts to join: one sequence of 2000 rows of bf16 10.3 us, with four
     // 11.7; of 600 rows 9.1 and 8.5.)
-    const int least = all_chunks > 48 * sequences ? 2 * KV_TEAM : KV_TEAM, teams = min((int)gridDim.x * K::TEAMS, max((total + least - 1) / least, sequences * items));
+    const int least = all_chunks > 48 * sequences ? 2 * KV_TEAM : KV_TEAM, most = gridDim.x * K::TEAMS, wanted = sequences * items;
+    const int teams = solo ? min(KV_TEAM * most, wanted) : min(most, max((total + least - 1) / least, wanted));       // (solo: warps)
     const int share = teams > 0 ? total / teams : 0, keep = max(KV_KEEP, share >> 2);
     const int each = teams > 0 ? cost / teams : 0, over = cost - each * teams;
-    auto cost_of = [&](int id) { return each * id + over * id / teams; };         // cost * id / teams, in 32 bits (over and id are below 480)
+    auto cost_of = [&](int id) { return each * id + over * id / teams; };         // cost * id / teams, in 32 bits (over and id are below 1921)
     auto begin_of = [&](int id) {
         if (id >= teams) return total;
         const int at = cost_of(id);
@@ -578,8 +583,9 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             if (sh.cost[mid] * items <= at) lo = mid; else hi = mid - 1;
         }
         const int n = sh.prefix[lo + 1] - sh.prefix[lo], rel = at - sh.cost[lo] * items, item = rel / (n + KV_ITEM_COST);
-        int c = min(rel - item * (n + KV_ITEM_COST), n);
-        if (n <= keep) c = 2 * c < n ? 0 : n;
+        int c = rel - item * (n + KV_ITEM_COST);
+        if (n <= keep) c = 2 * c < n + KV_ITEM_COST ? 0 : n;      // the nearer end
+        else c = min(c, n);
         return sh.prefix[lo] * items + item * n + c;
     };
     auto part_of = [&](int id, int lane, int& c0, int& c1) {        // both ends at once
@@ -591,9 +597,10 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     if (warp >= WARPS) {
         // ---- the team's loading warp
         const int team = warp - WARPS, id = team * gridDim.x + blockIdx.x;
-        int f, c1, place[2] = {-1, -1};
-        part_of(id, lane, f, c1);
-        f += lane;
+        // (solo: lane w has the part of warp w)
+        const int by = solo ? 1 : KV_TEAM, at_end = begin_of((solo ? (team * KV_TEAM + (lane >> 1 & 3)) * gridDim.x + blockIdx.x : id) + (lane & 1));
+        int f = __shfl_sync(0xffffffffu, at_end, solo ? lane * 2 & 7 : 0), c1 = __shfl_sync(0xffffffffu, at_end, solo ? (lane * 2 & 7) + 1 : 1), place[2] = {-1, -1};
+        if (!solo) f += lane;
         if (lane >= KV_TEAM) c1 = 0;
         KvWalk at = {};
         auto look = [&]() {        // the chunk's rows of the cache, 16 at a time; -1: none
@@ -615,8 +622,8 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             unsigned left = __ballot_sync(0xffffffffu, f < c1);
             if (!left) break;
             const int now[2] = {place[0], place[1]}, slot = round % STAGES;
-            f += KV_TEAM;
-            if (f < c1) { at.step(KV_TEAM, sh.prefix, items); look(); }
+            f += by;
+            if (f < c1) { at.step(by, sh.prefix, items); look(); }
             for (; left && ok; left &= left - 1) {
                 const int mate = __ffs(left) - 1, w = team * KV_TEAM + mate, r0 = __shfl_sync(0xffffffffu, now[0], mate), r1 = KEYS == 32 ? __shfl_sync(0xffffffffu, now[1], mate) : -1;
                 uint64_t* const full = &sh.full[w][slot];
@@ -666,7 +673,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         if (a.lse) for (int i = mate * 32 + lane; i < a.heads; i += KV_TEAM * 32) a.lse[(int64_t)b * a.heads + i] = -INFINITY;
     }
     int c0, c1;
-    part_of(id, lane, c0, c1);
+    part_of(solo ? (team * KV_TEAM + mate) * gridDim.x + blockIdx.x : id, lane, c0, c1);
     if (c0 >= c1) return;
 
     auto head_of = [&](int item) {         // the first query head of an item
@@ -695,16 +702,18 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             }
         }
     };
-    // segments: what the team has of one item; the first warp writes the next one down while all work on this one
+    // segments: what the team has of one item; the first warp writes the next one down while all work on this one (solo: each warp its own)
     auto describe = [&](int f, typename K::Segment& to) {
         KvWalk at;
         at.seek(f, sh.prefix, a.batch, items);
         if (lane == 0) to = {at.b, at.item, f - at.c, f, min(c1, f - at.c + at.n), at.n};
     };
-    if (mate == 0) describe(c0, sh.seg[team][0]);
-    team_sync(team);
-    ask_queries(sh.seg[team][0].b, sh.seg[team][0].item);
-    if (mate == KV_TEAM - 1 && lane < 2) {
+    typename K::Segment* const segs = solo ? reinterpret_cast<typename K::Segment*>(smem + K::JOIN) + 2 * warp : sh.seg[team];      // (solo: where no warps are joined)
+    auto together = [&]() { if (solo) __syncwarp(); else team_sync(team); };
+    if (solo || mate == 0) describe(c0, segs[0]);
+    together();
+    ask_queries(segs[0].b, segs[0].item);
+    if (!solo && mate == KV_TEAM - 1 && lane < 2) {
         // the items that the team's part begins and ends in, while the first rows are under way: teams from ... to share one, in groups of `fan`; the first
         // one's part is in slot `late`
         KvWalk w;
@@ -726,12 +735,13 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         }
     }
     float* const buf = reinterpret_cast<float*>(smem + K::JOIN + team * KV_JOIN_BYTES);
-    int f = c0 + mate, slot = 0, parity = 0;
+    const int by = solo ? 1 : KV_TEAM;
+    int f = solo ? c0 : c0 + mate, slot = 0, parity = 0;
     bool ok = true;
 #pragma unroll 1
     for (int k = 0;; ++k) {
-        const typename K::Segment seg = sh.seg[team][k & 1];
-        if (mate == 0 && seg.end < c1) describe(seg.end, sh.seg[team][(k + 1) & 1]);
+        const typename K::Segment seg = segs[k & 1];
+        if ((solo || mate == 0) && seg.end < c1) describe(seg.end, segs[(k + 1) & 1]);
         float z_scale[HG], acc[HG][8][4], m[HG], l[HG];
 #pragma unroll
         for (int h = 0; h < HG; ++h) {
@@ -756,7 +766,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 
         int valid = sh.len[seg.b] - (f - seg.first) * KEYS;       // rows that the sequence has from the warp's chunk on
 #pragma unroll 1
-        for (; f < seg.end; f += KV_TEAM, valid -= KV_TEAM * KEYS) {
+        for (; f < seg.end; f += by, valid -= by * KEYS) {
             const uint32_t st = smem_u32(smem) + (warp * STAGES + slot) * KV_STAGE_BYTES, scales = smem_u32(smem) + K::SCALES + (warp * STAGES + slot) * 256;
             const bool append = a.kn && valid <= KEYS;
             uint4 fresh = make_uint4(0, 0, 0, 0);
@@ -945,16 +955,9 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             if (++slot == STAGES) { slot = 0; parity ^= 1; }
         }
 
-        // ---- the warps' parts together, 32 columns at a time or as many as fit the team's buffer
-        const int head0 = head_of(seg.item), heads = heads_of(seg.item), log_q = heads <= 4 ? 2 : heads <= 8 ? 1 : 0, quarters = 1 << log_q;
-        team_sync(team);
-        if (seg.end < c1) ask_queries(sh.seg[team][(k + 1) & 1].b, sh.seg[team][(k + 1) & 1].item);
-#pragma unroll
-        for (int h = 0; h < HG; ++h) {
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-            if (t == 0) { sh.m[team][mate][8 * h + g] = m[h]; sh.l[team][mate][8 * h + g] = l[h]; }
-        }
+        const int head0 = head_of(seg.item), heads = heads_of(seg.item);
+        together();
+        if (seg.end < c1) ask_queries(segs[(k + 1) & 1].b, segs[(k + 1) & 1].item);
         if (twice) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -962,6 +965,37 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 for (int c = 0; c < 4; ++c) acc[0][j][c] += __shfl_xor_sync(0xffffffffu, acc[0][j][c], 2);
             }
         }
+#pragma unroll
+        for (int h = 0; h < HG; ++h) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        }
+        // a thread's accumulators, of heads 2t, 2t + 1 (and 8 + those): columns 64 half + 8 gp + tile of bf16, 16 gp + 8 half + tile of codes
+        auto column = [&](int quarter, int p) { return (TYPE == KV_BF16 ? 64 * (quarter >> 1) + 8 * p : 8 * (quarter >> 1) + 16 * p) + (quarter & 1) * 4; };
+        if (solo) {
+#pragma unroll
+            for (int h = 0; h < HG; ++h) {
+                if (a.lse && t == 0 && 8 * h + g < heads) a.lse[(int64_t)seg.b * a.heads + head0 + 8 * h + g] = (m[h] - KV_LIFT + log2f(l[h])) * 0.6931471805599453f;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int head = 8 * h + 2 * t + j;
+                    const float inv = 1.0f / __shfl_sync(0xffffffffu, l[h], 8 * t + 4 * j);
+                    if (head >= heads) continue;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int c = 2 * (q >> 1) + j, four = (q & 1) * 4;
+                        store_row4(a.out + seg.b * a.ldo + (head0 + head) * KV_D + column(q, gp), make_float4(acc[h][four][c], acc[h][four + 1][c], acc[h][four + 2][c], acc[h][four + 3][c]), inv, a.flags & 2);
+                    }
+                }
+            }
+            if (seg.end == c1) return;
+            continue;
+        }
+        // ---- the warps' parts together, 32 columns at a time or as many as fit the team's buffer
+        const int log_q = heads <= 4 ? 2 : heads <= 8 ? 1 : 0, quarters = 1 << log_q;
+#pragma unroll
+        for (int h = 0; h < HG; ++h)
+            if (t == 0) { sh.m[team][mate][8 * h + g] = m[h]; sh.l[team][mate][8 * h + g] = l[h]; }
         const bool whole = seg.begin == seg.first && seg.end == seg.first + seg.n;
         const int64_t mine = (int64_t)(2 * id + (seg.begin == c0 ? 0 : 1)) * a.per_item;
 #pragma unroll
@@ -993,8 +1027,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 o.x += x.x * e; o.y += x.y * e; o.z += x.z * e; o.w += x.w * e;
                 sum += sh.l[team][w][head] * e;
             }
-            // thread g's accumulators are columns 64 half + 8 gp + tile of bf16, 16 gp + 8 half + tile of codes
-            const int quarter = q - quarters + 1 + qq, half = quarter >> 1, col = (TYPE == KV_BF16 ? 64 * half + 8 * kv_perm(at) : 8 * half + 16 * kv_perm(at)) + (quarter & 1) * 4;
+            const int quarter = q - quarters + 1 + qq, col = column(quarter, kv_perm(at));
             const bool one = at == 0 && quarter == 0;
             if (whole) {
                 store_row4(a.out + seg.b * a.ldo + (head0 + head) * KV_D + col, o, 1.0f / sum, a.flags & 2);
@@ -1032,14 +1065,22 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     }
 }
 
-template <int TYPE, int HG>
-static cudaError_t launch_attention(const CUtensorMap& k_map, const CUtensorMap& v_map, const KvAttn& a, int64_t chunks, int64_t items, cudaStream_t st) {
+template <int TYPE, int HG, bool SOLO>
+static cudaError_t launch_attention(const CUtensorMap& k_map, const CUtensorMap& v_map, const KvAttn& a, int blocks, cudaStream_t st) {
     static std::atomic<uint64_t> done{0};
     using K = KvKernel<TYPE, HG>;
     static_assert(K::SMEM <= 232448, "more than an SM's block can have");
-    if (!func_attr_once(done, (const void*)kv_attention_kernel<TYPE, HG>, K::SMEM, "kv_attention")) return cudaErrorInvalidValue;
-    const int blocks = (int)min((int64_t)min(sm_count(), KV_TEAMS_MAX / K::TEAMS), max((chunks + KV_TEAM - 1) / KV_TEAM, items));
-    return launch_chained(kv_attention_kernel<TYPE, HG>, dim3((unsigned)max(1, blocks)), dim3(K::THREADS), K::SMEM, st, 1, 1, k_map, v_map, a);
+    if (!func_attr_once(done, (const void*)kv_attention_kernel<TYPE, HG, SOLO>, K::SMEM, "kv_attention")) return cudaErrorInvalidValue;
+    return launch_chained(kv_attention_kernel<TYPE, HG, SOLO>, dim3((unsigned)blocks), dim3(K::THREADS), K::SMEM, st, 1, 1, k_map, v_map, a);
+}
+template <int TYPE, int HG>
+static cudaError_t launch_attention(const CUtensorMap& k_map, const CUtensorMap& v_map, const KvAttn& a, int64_t item_chunks, int64_t items, cudaStream_t st) {
+    const int most = min(sm_count(), KV_TEAMS_MAX / KvKernel<TYPE, HG>::TEAMS), teams = most * KvKernel<TYPE, HG>::TEAMS;
+    // A table of few tokens for more items than teams: an item to a warp, where its chunks one after the other take less than a team's items with their joins.
+    // us, to warps and to teams: 200 sequences of 30 rows of fp8, 8 kv heads 7.7 and 20; 62 of 54 of bf16, 16 kv heads 9.7 and 12.7; 128 of up to 100 of bf16 11.6 and 13.3.
+    // (Chosen on the device instead, by the lengths, it cost all other calls 0.4 us: one kernel with both.)
+    if (items > teams && item_chunks <= KV_SOLO && item_chunks * teams <= KV_TEAM * items) return launch_attention<TYPE, HG, true>(k_map, v_map, a, most, st);
+    return launch_attention<TYPE, HG, false>(k_map, v_map, a, (int)max((int64_t)1, min((int64_t)most, max((item_chunks * items + KV_TEAM - 1) / KV_TEAM, items))), st);
 }
 
 static bool aligned16(const void* p, int64_t ld) { return (((uintptr_t)p) & 15) == 0 && (ld & 7) == 0; }
@@ -1147,7 +1188,7 @@ hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, 
     if (workspace_bytes < o1_kv_attention_workspace_bytes(heads, c.heads) || (((uintptr_t)workspace) & 15)) { set_error("kv_attention: workspace too small or unaligned"); return HD_ERR_OOM; }
     const int group = heads / c.heads, hg = group <= 8 ? 1 : 2, of_heads = (group + 8 * hg - 1) / (8 * hg), keys = cache->type == O1_KV_BF16 ? 16 : 32;
     // the stream's index is an int: fewer sequences a launch where the table allows for more
-    const int64_t each = ((int64_t)width * c.page_size + keys - 1) / keys * c.heads * of_heads;
+    const int64_t item_chunks = ((int64_t)width * c.page_size + keys - 1) / keys, each = item_chunks * c.heads * of_heads;
     if ((int64_t)width * c.page_size > INT32_MAX - 64 || each > (1 << 30) || (int64_t)c.pages * c.heads * c.page_size > INT32_MAX) { set_error("kv_attention: a table of %d pages of %d tokens for %d heads, or a cache of %d pages, is too large", width, c.page_size, heads, c.pages); return HD_ERR_UNSUPPORTED; }
     const int step = (int)min((int64_t)KV_SEQS, each > 0 ? max((int64_t)1, (int64_t)(1 << 30) / each) : (int64_t)KV_SEQS);
     const int per_item = min(group, 8 * hg);
@@ -1176,11 +1217,11 @@ hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, 
         a.lens = lens + b;
         a.out = (uint16_t*)out + b * ldo;
         a.lse = lse ? lse + (int64_t)b * heads : nullptr;
-        const int64_t chunks = each * a.batch, items = (int64_t)c.heads * of_heads * a.batch;
+        const int64_t items = (int64_t)c.heads * of_heads * a.batch;
         cudaError_t e;
-        if (cache->type == O1_KV_BF16) e = hg == 1 ? launch_attention<KV_BF16, 1>(k_map, v_map, a, chunks, items, current_stream()) : launch_attention<KV_BF16, 2>(k_map, v_map, a, chunks, items, current_stream());
-        else if (cache->type == O1_KV_FP8) e = hg == 1 ? launch_attention<KV_FP8, 1>(k_map, v_map, a, chunks, items, current_stream()) : launch_attention<KV_FP8, 2>(k_map, v_map, a, chunks, items, current_stream());
-        else e = hg == 1 ? launch_attention<KV_INT8, 1>(k_map, v_map, a, chunks, items, current_stream()) : launch_attention<KV_INT8, 2>(k_map, v_map, a, chunks, items, current_stream());
+        if (cache->type == O1_KV_BF16) e = hg == 1 ? launch_attention<KV_BF16, 1>(k_map, v_map, a, item_chunks, items, current_stream()) : launch_attention<KV_BF16, 2>(k_map, v_map, a, item_chunks, items, current_stream());
+        else if (cache->type == O1_KV_FP8) e = hg == 1 ? launch_attention<KV_FP8, 1>(k_map, v_map, a, item_chunks, items, current_stream()) : launch_attention<KV_FP8, 2>(k_map, v_map, a, item_chunks, items, current_stream());
+        else e = hg == 1 ? launch_attention<KV_INT8, 1>(k_map, v_map, a, item_chunks, items, current_stream()) : launch_attention<KV_INT8, 2>(k_map, v_map, a, item_chunks, items, current_stream());
         if (!launch_ok(e, "kv_attention")) return HD_ERR_RUNTIME;
         o1_launch_count_add(1);
     }

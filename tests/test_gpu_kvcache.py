@@ -279,6 +279,55 @@ def test_new_rows_appended_by_the_same_call(pkg, dev, kind, lens, kv_heads, grou
     b.check(q, out, lse, what=kind)
 
 
+MANY = [(300, 4, 4, 16, 90), (130, 8, 7, 32, 64), (230, 2, 16, 32, 33), (160, 3, 24, 16, 48), (470, 1, 1, 48, 48), (64, 16, 3, 16, 33), (600, 8, 2, 16, 200)]
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "int8"])
+@pytest.mark.parametrize("batch,kv_heads,group,page,most", MANY)
+def test_many_short_sequences(pkg, dev, kind, batch, kv_heads, group, page, most):
+    """More (sequence, kv head) pairs than the GPU has teams of warps, a short table: a pair to a warp, lengths from 0."""
+    lens = [(37 * b) % (most + 1) for b in range(batch)]
+    c = Case(pkg, dev, kind, lens, kv_heads, page, seed=batch)
+    c.fill()
+    q = normal((batch, kv_heads * group, D), gen(13), 1.5)
+    out, lse = c.cache.attend(q.to(dev), c.dtable, c.dlens, lse=True)
+    assert pkg.lib.o1_device_error() == 0
+    c.check(q, out, lse, what=kind)
+    again, lse2 = c.cache.attend(q.to(dev), c.dtable, c.dlens, lse=True)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+    # in a wide table the pairs go to teams
+    wide = torch.full((batch, 300), -1, dtype=torch.int32, device=dev)
+    wide[:, :c.dtable.size(1)] = c.dtable
+    out, lse = c.cache.attend(q.to(dev), wide, c.dlens, lse=True)
+    c.check(q, out, lse, what=kind)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "int8"])
+@pytest.mark.parametrize("batch,kv_heads,group,page,most", [(300, 4, 4, 16, 90), (230, 2, 16, 32, 33), (470, 1, 1, 48, 48)])
+def test_many_short_sequences_with_new_rows(pkg, dev, kind, batch, kv_heads, group, page, most):
+    test_new_rows_appended_by_the_same_call(pkg, dev, kind, [(37 * b) % (most + 1) for b in range(batch)], kv_heads, group, page)
+
+
+@gpu
+def test_many_short_sequences_with_wrong_tables(pkg, dev):
+    lens = [1 + b % 40 for b in range(260)]
+    c = Case(pkg, dev, "fp8", lens, 2, 16)
+    c.fill()
+    q = normal((260, 8, D), gen(1)).to(dev)
+    good = c.cache.attend(q, c.dtable, c.dlens)
+    assert pkg.lib.o1_device_error() == 0
+    t, ln = c.dtable.clone(), c.dlens.clone()
+    t[100, 0], t[7, 0] = c.cache.pages, -1
+    out = c.cache.attend(q, t, c.dlens)
+    rest = [b for b in range(260) if b not in (7, 100)]
+    assert pkg.lib.o1_device_error() == 70 and torch.equal(out[rest], good[rest])
+    ln[100], ln[7] = -1, 16 * c.table.shape[1] + 1
+    out = c.cache.attend(q, c.dtable, ln)
+    assert pkg.lib.o1_device_error() == 71 and torch.equal(out[rest], good[rest])
+
+
 @gpu
 @pytest.mark.parametrize("kind", ["bf16", "fp8", "int8"])
 def test_scores_of_any_size(pkg, dev, kind):
