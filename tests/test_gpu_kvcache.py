@@ -577,3 +577,18 @@ def test_entry_points_refuse_before_they_touch_the_gpu(pkg):
         assert b"kv_attention" in lib.hd_cuda_last_error(), args
     assert attend(batch=0) == 0
     lib.hd_cuda_clear_error()
+
+
+def test_tables_and_heads_beyond_32_bits_are_refused(pkg):
+    """The stream of chunks and its costs are counted in 32 bits; what does not fit is refused on the host, before anything is launched."""
+    K, lib, one = pkg.KvCacheC, pkg.lib, 4096
+
+    def attend(heads=4, width=3, pages=8, kv_heads=2):
+        c = K(one, one, None, None, 0, pages, 16, kv_heads, 128)
+        need = lib.o1_kv_attention_workspace_bytes(heads, kv_heads)
+        return lib.o1_kv_attention(C.byref(c), one, heads * 128, None, 0, None, 0, one, width, width, one, one, heads * 128, None, 1, heads, 0.1, one, need)
+
+    for args in (dict(heads=1 << 24), dict(heads=1 << 23), dict(width=1 << 27), dict(pages=1 << 27), dict(kv_heads=4096, heads=4096, width=1 << 20)):
+        assert attend(**args) == 9, args
+        assert b"too large" in lib.hd_cuda_last_error(), args
+    lib.hd_cuda_clear_error()
