@@ -189,7 +189,6 @@ __device__ __forceinline__ float row_rms_inv(F squares, int cols, float eps, flo
 template <int THREADS, int ITEMS, bool POST, bool AHEAD>
 __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS ? THREADS : 1024, THREADS == 128 ? 7 : THREADS == 256 ? 4 : THREADS == 512 ? 2 : 1)
 residual_norm_vec_kernel(const ResidualNorm a) {
-    grid_dep_launch();
     grid_dep_wait();
     __shared__ float red[4][32];
     constexpr bool WARP = THREADS == 32;
@@ -219,6 +218,8 @@ residual_norm_vec_kernel(const ResidualNorm a) {
             if (gate) gv[i] = get(gate, idx);
         }
     }
+    // (the next launch is let in late: blocks of it that are placed early leave these unevenly spread, 1024 x 1152 4.0 us, so 3.2)
+    if (WARP) grid_dep_launch();
     float inv = 1.f;
     if (POST) {
         inv = row_rms_inv<THREADS>([&](float s) {
@@ -258,6 +259,7 @@ residual_norm_vec_kernel(const ResidualNorm a) {
             reinterpret_cast<uint4*>(a.y + row * a.ldy)[idx] = pack8(y[i]);
         }
     }
+    if (!WARP) grid_dep_launch();
     if (!a.h) return;
     uint4 pv[AHEAD ? ITEMS : 1], cv[AHEAD ? ITEMS : 1], sv[AHEAD ? ITEMS : 1];
 #pragma unroll
@@ -346,7 +348,7 @@ bool residual_norm(const void* x, int64_t ldx, const void* branch, int64_t ldb, 
     const uintptr_t all = (uintptr_t)x | (uintptr_t)branch | (uintptr_t)post | (uintptr_t)gate | (uintptr_t)pre | (uintptr_t)scale | (uintptr_t)shift |
                           (uintptr_t)y | (uintptr_t)h;
     const bool vec = (all & 15) == 0 && ((ldx | ldb | ldy | (h ? ldh : 0) | cols) & 7) == 0 && cols <= 16384;
-    if (!vec) return launch_ok(launch_chained(residual_norm_any_kernel, dim3(rows), dim3(256), 0, st, 1, rows, a), "residual_norm");
+    if (!vec) return launch_ok(launch_chained(residual_norm_any_kernel, dim3(rows), dim3(256), 0, st, 1, 1, a), "residual_norm");
     // Measured in us.  Rows up to 1280 wide by a warp each, vectors ahead (2000 x 1152 with both norms 4.2, at use 5.4; a block to a row, at use, 6.4).
     // Wider ones, few of them: two pieces of 16 bytes to a thread, vectors ahead; many: fewer registers, so that more rows are under way - with the
     // inner norm four pieces and a fixed number of threads.  Both norms, ahead / at use: 592 x 4096 4.4 / 6.2, 3000 x 4096 22 / 27, 3000 x 8192 44 / 43,
@@ -365,7 +367,7 @@ bool residual_norm(const void* x, int64_t ldx, const void* branch, int64_t ldb, 
         kern = cols <= 4096 ? residual_norm_vec_kernel<128, 4, true, false> : cols <= 8192 ? O1_RN(256, 4, false) : O1_RN(512, 4, false);
     }
 #undef O1_RN
-    return launch_ok(launch_chained(kern, dim3(warps ? (rows + 3) / 4 : rows), dim3(threads), 0, st, 1, rows, a), "residual_norm");
+    return launch_ok(launch_chained(kern, dim3(warps ? (rows + 3) / 4 : rows), dim3(threads), 0, st, 1, 1, a), "residual_norm");
 }
 
 // ------------------------------------------------------------------ materialising attention (small / odd shapes)

@@ -129,6 +129,8 @@ __device__ __forceinline__ void store8(uint16_t* p, const uint4& v) {
 // (135 a unit, against 80) took longer than its bytes, 22.8 us.  Written and read, us: 16640 rows of 8 heads of int8 18.9 + 18.7 (5.5 TB/s), 100000 rows of one head
 // 15.2 + 15.1; a row to a warp 23.5 + 19.5 and 43 + 39, a head to a half warp 34 + 35 for the former.  Few rows have more warps with two units: 1800 rows of
 // 8 heads 3.5 + 3.7, with eight 5.3 + 4.0; 2600 rows 4.5 + 4.7 and 4.3 + 4.3; 4111 rows 6.9 + 7.5 and 5.8 + 6.2.
+// Launches overlap at any size (the next one is let in once the rows have been asked for: its blocks, placed earlier, leave these unevenly spread, 1000 rows 5.1 us, so
+// 4.1): written and read through a stream, 4111 rows 14.4 us without, 12.4 with; 16640 42.7 and 38.
 static constexpr int KV_EACH = 8, KV_EACH_OF_FEW = 2, KV_FEW_UNITS = 19200;
 // A unit's place in a [pages][heads][page_size] array, -1: none.
 __device__ __forceinline__ int64_t place(int64_t slot, int head, const KvView& c, int* err) {
@@ -141,7 +143,6 @@ template <bool VEC, int EACH>
 __global__ void __launch_bounds__(128, EACH == 8 ? 9 : 12)
 kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk, const uint16_t* __restrict__ v, int64_t ldv,
                 const int64_t* __restrict__ slots, unsigned units, int* err) {
-    grid_dep_launch();
     grid_dep_wait();
     const unsigned from = (blockIdx.x * 4 + (threadIdx.x >> 5)) * EACH;
     if (from >= units) return;
@@ -162,6 +163,7 @@ kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk,
         if (++head == c.heads) { head = 0; src += ld; }
     }
     const int64_t places = place(slot, from + mine - my_row * c.heads, c, err);
+    grid_dep_launch();
     float inv = 0.f;
     if (type != KV_BF16) {
         // maxima: a step halves the lanes that a unit is spread over, and, until a lane has one, its units
@@ -194,7 +196,6 @@ template <bool VEC, int EACH>
 __global__ void __launch_bounds__(128, EACH == 8 ? 7 : 12)
 kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16_t* __restrict__ v, int64_t ldv,
                const int64_t* __restrict__ slots, unsigned units, int* err) {
-    grid_dep_launch();
     grid_dep_wait();
     const unsigned from = (blockIdx.x * 4 + (threadIdx.x >> 5)) * EACH;
     if (from >= units) return;
@@ -220,6 +221,7 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
         x[i].x = codes.x;
         x[i].y = codes.y;
     }
+    grid_dep_launch();
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
         if (i >= count) break;
@@ -1130,7 +1132,7 @@ hd_status o1_kv_write(const o1_kv_cache* cache, const void* k, int64_t ldk, cons
         const bool few = units < KV_FEW_UNITS;
         const unsigned block = 4 * (few ? KV_EACH_OF_FEW : KV_EACH);
         auto kern = few ? (vec ? kv_write_kernel<true, KV_EACH_OF_FEW> : kv_write_kernel<false, KV_EACH_OF_FEW>) : vec ? kv_write_kernel<true, KV_EACH> : kv_write_kernel<false, KV_EACH>;
-        if (!launch_ok(launch_chained(kern, dim3((units + block - 1) / block), dim3(128), 0, current_stream(), 1, rows, c, cache->type, (const uint16_t*)k + first * ldk, ldk,
+        if (!launch_ok(launch_chained(kern, dim3((units + block - 1) / block), dim3(128), 0, current_stream(), 1, 1, c, cache->type, (const uint16_t*)k + first * ldk, ldk,
                                       (const uint16_t*)v + first * ldv, ldv, slots + first, units, device_error_word()), "kv_write"))
             return HD_ERR_RUNTIME;
         o1_launch_count_add(1);
@@ -1155,7 +1157,7 @@ hd_status o1_kv_read(const o1_kv_cache* cache, void* k, int64_t ldk, void* v, in
         const bool few = units < KV_FEW_UNITS;
         const unsigned block = 4 * (few ? KV_EACH_OF_FEW : KV_EACH);
         auto kern = few ? (vec ? kv_read_kernel<true, KV_EACH_OF_FEW> : kv_read_kernel<false, KV_EACH_OF_FEW>) : vec ? kv_read_kernel<true, KV_EACH> : kv_read_kernel<false, KV_EACH>;
-        if (!launch_ok(launch_chained(kern, dim3((units + block - 1) / block), dim3(128), 0, current_stream(), 1, rows, c, cache->type, (uint16_t*)k + first * ldk, ldk,
+        if (!launch_ok(launch_chained(kern, dim3((units + block - 1) / block), dim3(128), 0, current_stream(), 1, 1, c, cache->type, (uint16_t*)k + first * ldk, ldk,
                                       (uint16_t*)v + first * ldv, ldv, slots + first, units, device_error_word()), "kv_read"))
             return HD_ERR_RUNTIME;
         o1_launch_count_add(1);
