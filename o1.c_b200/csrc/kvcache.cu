@@ -126,7 +126,7 @@ __device__ __forceinline__ void store8(uint16_t* p, const uint4& v) {
 // A unit is a row's head; a warp has EACH of them, behind one another: keys in the lower 16 lanes, values in the others, eight columns to a lane.  HBM bound for
 // many rows: 2 bytes in, 1 (or 2) and the scale out a value.  What the units need is asked for together (a warp of eight has 4 KB on its way), a lane has one
 // unit's place and scale, and the maxima are found for all units at once: with four exchanges for each and divisions in every lane the write's instructions
-// (135 a unit, against 80) took longer than its bytes, 22.8 us.  Written and read, us: 16640 rows of 8 heads of int8 18.9 + 18.7 (5.5 TB/s), 100000 rows of one head
+// (135 a unit, now 100) took longer than its bytes, 22.8 us.  Written and read, us: 16640 rows of 8 heads of int8 18.9 + 18.7 (5.5 TB/s), 100000 rows of one head
 // 15.2 + 15.1; a row to a warp 23.5 + 19.5 and 43 + 39, a head to a half warp 34 + 35 for the former.  Few rows have more warps with two units: 1800 rows of
 // 8 heads 3.5 + 3.7, with eight 5.3 + 4.0; 2600 rows 4.5 + 4.7 and 4.3 + 4.3; 4111 rows 6.9 + 7.5 and 5.8 + 6.2.
 // Launches overlap at any size (the next one is let in once the rows have been asked for: its blocks, placed earlier, leave these unevenly spread, 1000 rows 5.1 us, so
