@@ -268,8 +268,9 @@ static constexpr int KV_FLAT = 32, KV_FAN = 16;
 // What an item costs a team beside its chunks (the warps' join, the next queries), in chunks: 4, 7, 10, 12: batch 26.1, 25.5, 24.9, 24.5, shared 22.5, 20.0, 18.1, 17.8,
 // 582 MB 97.4, 97.1, 96.9, 97.6.
 static constexpr int KV_ITEM_COST = 10;
-// Items of so few chunks, or of a quarter of a team's part (half: 582 MB 104), are not cut: 9 sequences of up to 1999 rows of fp8, 16 kv heads: 16 or 24 18, 48 26;
-// 60 of 100 to 900 rows of int8: 16 18.3, 24 19.8.
+// Items of so few chunks are not cut: 9 sequences of up to 1999 rows of fp8, 16 kv heads: 16 or 24 18, 48 26; 60 of 100 to 900 rows of int8: 16 18.3, 24 19.8.
+// Nor are those of a quarter of a team's part (half: 582 MB 104), and, where there are no more items than teams, of up to half more cost than a team has on average:
+// 51 sequences of 304 rows of bf16, 8 kv heads, 16.0, cut 20.6; 54 of 1000 of fp8 24.7 and 30.5; 55 of 100 to 700 of bf16 23.0 and 24.3.
 static constexpr int KV_KEEP = 16;
 static constexpr int KV_SOLO = 16;                     // chunks of an item that a warp can have for itself (no item of KV_KEEP chunks is cut)
 static_assert(KV_SOLO <= KV_KEEP, "an item of a warp is whole");
@@ -573,8 +574,8 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     // 11.7; of 600 rows 9.1 and 8.5.)
     const int least = all_chunks > 48 * sequences ? 2 * KV_TEAM : KV_TEAM, most = gridDim.x * K::TEAMS, wanted = sequences * items;
     const int teams = solo ? min(KV_TEAM * most, wanted) : min(most, max((total + least - 1) / least, wanted));       // (solo: warps)
-    const int share = teams > 0 ? total / teams : 0, keep = max(KV_KEEP, share >> 2);
-    const int each = teams > 0 ? cost / teams : 0, over = cost - each * teams;
+    const int share = teams > 0 ? total / teams : 0, each = teams > 0 ? cost / teams : 0, over = cost - each * teams;
+    const int keep = max(KV_KEEP, wanted <= most ? each + (each >> 1) - KV_ITEM_COST : share >> 2);
     auto cost_of = [&](int id) { return each * id + over * id / teams; };         // cost * id / teams, in 32 bits (over and id are below 1921)
     auto begin_of = [&](int id) {
         if (id >= teams) return total;
