@@ -454,8 +454,10 @@ void o1_set_stream(void *stream);
 void *o1_get_stream(void);
 /* The capture that stream is in, by a number of its own; 0: none.  (What a captured call keeps for itself must not serve calls outside.) */
 uint64_t o1_capture_id(void);
-/* Kernels whose bounded waits ran out record a code in a device word;
- * this reads and clears it (synchronises the current stream). 0 = clean. */
+/* Kernels whose bounded waits ran out record a code in a device word, and kernels
+ * after them store nothing until it is cleared; an entry of a caller's table that does
+ * not fit (o1_kv_*) is recorded in a word of its own, which stops nothing.  This reads
+ * a code and clears its word, a failed wait's first (synchronises the current stream). 0 = clean. */
 int o1_device_error(void);
 int o1_sm_count(void);
 /* Per-launch CUDA-event timing of the tensor-core kernels on their own stream (off by default;
@@ -763,8 +765,8 @@ int o1_parallel_layout(int world, int rank, int *image, int *branch, int *sp_ran
  * or NaN gets a NaN scale and reads as NaN.  A token's slot is page * page_size + its place in the page.
  * Codes are those that o1_kv_write makes: in particular no e4m3 NaN (0x7F, 0xFF), whose row has its NaN in the scale.
  * A slot or page outside the cache, or a length outside its table, found on the device: nothing outside the cache is read or
- * written, that row's or sequence's result means nothing, and the device error word gets 70 (slot or page) or 71 (length); 72 is a wait that ran
- * out (o1_device_error). */
+ * written, that row's or sequence's result means nothing (a wrong length: zeros, and no row is appended), other rows and sequences and every other call are
+ * as without it, and o1_device_error() gives 70 (slot or page) or 71 (length).  72 is a wait that ran out. */
 enum { O1_KV_BF16 = 0, O1_KV_FP8 = 1, O1_KV_INT8 = 2 };
 typedef struct {
     void *k, *v;

@@ -120,6 +120,7 @@ char* errbuf();             // 512 bytes
 void set_error(const char* fmt, ...);
 int* device_failed_word();  // one int of mapped host memory per device, beside the error word (see lora.cu), or NULL
 int* device_error_word();   // per-device int set by kernels whose bounded waits ran out
+int* device_table_word();   // per-device int beside it: what a kernel found wrong in a caller's table (slots, pages, lengths); it stops no other kernel
 int sm_count();
 
 #define O1_CUDA_OK(call, what)                                                     \

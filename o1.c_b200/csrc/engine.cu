@@ -55,7 +55,7 @@ static void set_model_error(const char* fmt, ...) {
 }
 
 struct DevState {
-    int* err_word = nullptr;   // [0] error word of the bounded waits, [1] result slot of the mask probe
+    int* err_word = nullptr;   // [0] error word of the bounded waits, [1] result slot of the mask probe, [2] table word
     int* failed = nullptr;     // host memory that the device writes: the code of a merge that failed
     int sms = 0;
 };
@@ -67,7 +67,7 @@ static DevState& dev_state() {
     std::lock_guard<std::mutex> lk(mu);
     DevState& s = states[dev];
     if (!s.err_word) {
-        if (cudaMalloc(&s.err_word, 2 * sizeof(int)) == cudaSuccess) cudaMemset(s.err_word, 0, 2 * sizeof(int));
+        if (cudaMalloc(&s.err_word, 3 * sizeof(int)) == cudaSuccess) cudaMemset(s.err_word, 0, 3 * sizeof(int));
         if (cudaHostAlloc(&s.failed, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) == cudaSuccess) *s.failed = 0;
         cudaDeviceGetAttribute(&s.sms, cudaDevAttrMultiProcessorCount, dev);
         if (s.sms <= 0) s.sms = 148;
@@ -75,6 +75,7 @@ static DevState& dev_state() {
     return s;
 }
 int* device_error_word() { return dev_state().err_word; }
+int* device_table_word() { return dev_state().err_word ? dev_state().err_word + 2 : nullptr; }
 int* device_failed_word() { return dev_state().failed; }
 int sm_count() { return dev_state().sms; }
 
@@ -172,15 +173,17 @@ int o1_profile_summary(int kind, double* total_ms, int64_t* launches, double* wo
 int o1_device_error(void) {
     int* w = device_error_word();
     if (!w) return -1;
-    int v = 0;
-    cudaError_t e = cudaMemcpyAsync(&v, w, sizeof(int), cudaMemcpyDeviceToHost, g_stream);
+    int v[3] = {0, 0, 0};
+    cudaError_t e = cudaMemcpyAsync(v, w, sizeof(v), cudaMemcpyDeviceToHost, g_stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(g_stream);
     if (e != cudaSuccess) { set_error("device_error: %s", cudaGetErrorString(e)); return -1; }
-    if (v != 0) {
+    if (v[0] != 0) {         // (a table's code beside it is the next call's)
         cudaMemsetAsync(w, 0, sizeof(int), g_stream);
         if (device_failed_word()) *(volatile int*)device_failed_word() = 0;
+        return v[0];
     }
-    return v;
+    if (v[2] != 0) cudaMemsetAsync(w + 2, 0, sizeof(int), g_stream);
+    return v[2];
 }
 
 // ================================================================ bf16 helpers

@@ -16,7 +16,7 @@ namespace o1 {
 
 enum { KV_BF16 = O1_KV_BF16, KV_FP8 = O1_KV_FP8, KV_INT8 = O1_KV_INT8 };
 static constexpr int KV_D = 128;
-// Codes of the device's error word: what a kernel found in a table on the device.  Nothing is read or written for such an entry.
+// Codes of the device's table word: what a kernel found in a table on the device.  Nothing is read or written for such an entry, and nothing else stops for it.
 static constexpr int ERR_KV_PLACE = 70;    // a slot or page outside the cache
 static constexpr int ERR_KV_LENGTH = 71;   // a length that is negative or does not fit its row of the page table
 
@@ -133,16 +133,16 @@ __device__ __forceinline__ void store8(uint16_t* p, const uint4& v) {
 // 4.1): written and read through a stream, 4111 rows 14.4 us without, 12.4 with; 16640 42.7 and 38.
 static constexpr int KV_EACH = 8, KV_EACH_OF_FEW = 2, KV_FEW_UNITS = 19200;
 // A unit's place in a [pages][heads][page_size] array, -1: none.
-__device__ __forceinline__ int64_t place(int64_t slot, int head, const KvView& c, int* err) {
+__device__ __forceinline__ int64_t place(int64_t slot, int head, const KvView& c, int* bad) {
     if (slot < 0) return -1;
-    if (slot >= (int64_t)c.pages * c.page_size) { atomicExch(err, ERR_KV_PLACE); return -1; }
+    if (slot >= (int64_t)c.pages * c.page_size) { atomicExch(bad, ERR_KV_PLACE); return -1; }
     const int64_t page = c.page_shift >= 0 ? slot >> c.page_shift : slot / c.page_size;
     return (page * c.heads + head) * c.page_size + slot - page * c.page_size;
 }
 template <bool VEC, int EACH>
 __global__ void __launch_bounds__(128, EACH == 8 ? 9 : 12)
 kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk, const uint16_t* __restrict__ v, int64_t ldv,
-                const int64_t* __restrict__ slots, unsigned units, int* err) {
+                const int64_t* __restrict__ slots, unsigned units, int* bad) {
     grid_dep_wait();
     const unsigned from = (blockIdx.x * 4 + (threadIdx.x >> 5)) * EACH;
     if (from >= units) return;
@@ -162,7 +162,7 @@ kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk,
         if (i < count) x[i] = load8<VEC>(src + head * KV_D);
         if (++head == c.heads) { head = 0; src += ld; }
     }
-    const int64_t places = place(slot, from + mine - my_row * c.heads, c, err);
+    const int64_t places = place(slot, from + mine - my_row * c.heads, c, bad);
     grid_dep_launch();
     float inv = 0.f;
     if (type != KV_BF16) {
@@ -195,7 +195,7 @@ kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk,
 template <bool VEC, int EACH>
 __global__ void __launch_bounds__(128, EACH == 8 ? 7 : 12)
 kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16_t* __restrict__ v, int64_t ldv,
-               const int64_t* __restrict__ slots, unsigned units, int* err) {
+               const int64_t* __restrict__ slots, unsigned units, int* bad) {
     grid_dep_wait();
     const unsigned from = (blockIdx.x * 4 + (threadIdx.x >> 5)) * EACH;
     if (from >= units) return;
@@ -208,7 +208,7 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
     uint16_t* dst = (is_v ? v : k) + row * ld + lane * 8;
     const uint8_t* const base = is_v ? c.v : c.k;
     const float* const scales = is_v ? c.vs : c.ks;
-    const int64_t places = place(slot, from + mine - my_row * c.heads, c, err);
+    const int64_t places = place(slot, from + mine - my_row * c.heads, c, bad);
     const float scale = type != KV_BF16 && places >= 0 ? scales[places] : 0.f;
     uint4 x[EACH];
 #pragma unroll
@@ -291,7 +291,7 @@ struct KvAttn {
     float* parts;          // [team][2][heads of an item][128] weighted sum
     int batch, heads, group, chunks_of_heads, per_item, width, flags;    // flags: 1 = queries in 16-byte pieces, 2 = results, 4 = new rows; 8 = a box of the maps is a whole chunk's rows
     float scale;
-    int* err;
+    int *err, *bad;        // the device's error and table words
 };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -557,7 +557,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             const int b = tid / lines;
             asm volatile("ld.global.ca.b32 %0, [%1];" : "=r"(entry) : "l"(a.pages + b * a.ldp + (tid - b * lines) * 32));
         }
-        if (len < 0 || len > (int64_t)a.width * ps) { atomicExch(a.err, ERR_KV_LENGTH); len = 0; }
+        if (len < 0 || len > (int64_t)a.width * ps) { atomicExch(a.bad, ERR_KV_LENGTH); len = 0; }
         const int n = (len + KEYS - 1) / KEYS;
         int2 all;
         const int2 before = block_scan<WARPS + K::TEAMS>(make_int2(n, n > 0 ? n + KV_ITEM_COST : 0), all, sh.scan);
@@ -615,7 +615,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 if (token >= len) continue;
                 const int page = a.pages[at.b * a.ldp + p];
                 place[h] = 0;
-                if ((unsigned)page >= (unsigned)a.c.pages) atomicExch(a.err, ERR_KV_PLACE);
+                if ((unsigned)page >= (unsigned)a.c.pages) atomicExch(a.bad, ERR_KV_PLACE);
                 else place[h] = (page * a.c.heads + head) * ps + token - p * ps;
             }
         };
@@ -1134,7 +1134,7 @@ hd_status o1_kv_write(const o1_kv_cache* cache, const void* k, int64_t ldk, cons
         const unsigned block = 4 * (few ? KV_EACH_OF_FEW : KV_EACH);
         auto kern = few ? (vec ? kv_write_kernel<true, KV_EACH_OF_FEW> : kv_write_kernel<false, KV_EACH_OF_FEW>) : vec ? kv_write_kernel<true, KV_EACH> : kv_write_kernel<false, KV_EACH>;
         if (!launch_ok(launch_chained(kern, dim3((units + block - 1) / block), dim3(128), 0, current_stream(), 1, 1, c, cache->type, (const uint16_t*)k + first * ldk, ldk,
-                                      (const uint16_t*)v + first * ldv, ldv, slots + first, units, device_error_word()), "kv_write"))
+                                      (const uint16_t*)v + first * ldv, ldv, slots + first, units, device_table_word()), "kv_write"))
             return HD_ERR_RUNTIME;
         o1_launch_count_add(1);
         if (rows - first <= most) break;
@@ -1159,7 +1159,7 @@ hd_status o1_kv_read(const o1_kv_cache* cache, void* k, int64_t ldk, void* v, in
         const unsigned block = 4 * (few ? KV_EACH_OF_FEW : KV_EACH);
         auto kern = few ? (vec ? kv_read_kernel<true, KV_EACH_OF_FEW> : kv_read_kernel<false, KV_EACH_OF_FEW>) : vec ? kv_read_kernel<true, KV_EACH> : kv_read_kernel<false, KV_EACH>;
         if (!launch_ok(launch_chained(kern, dim3((units + block - 1) / block), dim3(128), 0, current_stream(), 1, 1, c, cache->type, (uint16_t*)k + first * ldk, ldk,
-                                      (uint16_t*)v + first * ldv, ldv, slots + first, units, device_error_word()), "kv_read"))
+                                      (uint16_t*)v + first * ldv, ldv, slots + first, units, device_table_word()), "kv_read"))
             return HD_ERR_RUNTIME;
         o1_launch_count_add(1);
         if (rows - first <= most) break;
@@ -1204,6 +1204,7 @@ hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, 
     a.heads = heads; a.group = group; a.chunks_of_heads = of_heads; a.per_item = per_item; a.width = width;
     a.scale = scale;
     a.err = device_error_word();
+    a.bad = device_table_word();
     a.flags = (aligned16(q, ldq) ? 1 : 0) | (aligned16(out, ldo) ? 2 : 0) | (aligned16(k_new, ldk) && aligned16(v_new, ldv) ? 4 : 0);
     // maps of the rows, 128 bytes (64 columns of bf16, all codes) x 16, or 32 where a chunk of codes never crosses a page
     const bool wide = keys == 32 && c.page_size % 32 == 0;

@@ -177,3 +177,46 @@ def test_entry_points_refuse_before_they_touch_the_gpu(pkg):
         assert prompt(**args) == want, args
     assert step(batch=0) == 0 and prompt(rows=0) == 0
     lib.hd_cuda_clear_error()
+
+
+def raw_step(pkg, dec, names, ids, pages, lens):
+    """Decoder.step's call with tables of the test's own."""
+    n = len(names)
+    pos = (lens - 1).clamp(0, 10 ** 6).float().expand(3, n).contiguous()
+    out = torch.full((n, dec.dims[2]), 7.0, dtype=torch.bfloat16, device=dec.device)
+    s = dec._room(n)
+    pkg.check(pkg.lib.o1_decode_step(C.byref(dec.w.binding), dec._c, pkg.ptr(ids), pkg.ptr(pos), pkg.ptr(pages), pages.size(1), pages.size(1), pkg.ptr(lens),
+                                     pkg.ptr(s), s.numel(), pkg.ptr(out), n, *dec.dims), "o1_decode_step")
+    return out
+
+
+@gpu
+@pytest.mark.parametrize("what,code", [("page", 70), ("negative", 70), ("length", 71), ("long", 71)])
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+def test_a_wrong_entry_reaches_one_sequence_only(pkg, dev, weights, kind, what, code):
+    """A page or length of one sequence that does not fit: the others' rows, and what every layer keeps of them, are as without it."""
+    lens = [9, 5, 14]
+    dec = pkg.Decoder(weights, 3, 64, kind, 16)
+    names = [dec.prompt(ids_of(n, n).to(dev))[0] for n in lens]
+    before = [[t.clone() for t in (c.k.view(torch.uint8), c.v.view(torch.uint8))] for c in dec.caches]
+    ids = ids_of(3, 99).to(dev)
+    pages = torch.stack([dec._table[s] for s in names])
+    ln = torch.tensor([n + 1 for n in lens], dtype=torch.int32, device=dev)
+    want = raw_step(pkg, dec, names, ids, pages, ln)
+    after = [[t.clone() for t in (c.k.view(torch.uint8), c.v.view(torch.uint8))] for c in dec.caches]
+    for c, (k, v) in zip(dec.caches, before):
+        c.k.view(torch.uint8).copy_(k), c.v.view(torch.uint8).copy_(v)
+    bad_pages, bad_ln = pages.clone(), ln.clone()
+    if what == "page":
+        bad_pages[1, 0] = dec.caches[0].pages
+    elif what == "negative":
+        bad_pages[1, 0] = -3
+    else:
+        bad_ln[1] = -1 if what == "length" else 16 * pages.size(1) + 1
+    got = raw_step(pkg, dec, names, ids, bad_pages, bad_ln)
+    assert pkg.lib.o1_device_error() == code and pkg.lib.o1_device_error() == 0
+    assert torch.equal(got[[0, 2]], want[[0, 2]])
+    mine = {int(p) for p in pages[1]}
+    others = [p for p in range(dec.caches[0].pages) if p not in mine]
+    for c, (k, v) in zip(dec.caches, after):
+        assert torch.equal(c.k.view(torch.uint8)[others], k[others]) and torch.equal(c.v.view(torch.uint8)[others], v[others])

@@ -592,3 +592,17 @@ def test_tables_and_heads_beyond_32_bits_are_refused(pkg):
         assert attend(**args) == 9, args
         assert b"too large" in lib.hd_cuda_last_error(), args
     lib.hd_cuda_clear_error()
+
+
+@gpu
+def test_a_wrong_slot_stops_no_other_call(pkg, dev):
+    """A slot outside the cache is reported, and a product enqueued behind it is made all the same."""
+    cache = pkg.KvCache(2, 16, "int8", 2, dev)
+    x = normal((1, 2, D), gen(1)).to(dev)
+    a, w = normal((300, 256), gen(2)).to(dev), normal((512, 256), gen(3)).to(dev)
+    y = torch.full((300, 512), 777.0, dtype=torch.bfloat16, device=dev)
+    cache.write(x, x, torch.tensor([99], device=dev))
+    assert pkg.lib.o1_gemm(pkg.ptr(a), 256, pkg.ptr(w), None, pkg.ptr(y), 512, 300, 512, 256, 0, None, None, 0, 0.0, 0) == 0
+    torch.cuda.synchronize()
+    assert pkg.lib.o1_device_error() == 70 and pkg.lib.o1_device_error() == 0
+    assert (y != 777.0).float().mean() > 0.99
