@@ -142,7 +142,7 @@ __device__ __forceinline__ int64_t place(int64_t slot, int head, const KvView& c
 template <bool VEC, int EACH>
 __global__ void __launch_bounds__(128, EACH == 8 ? 9 : 12)
 kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk, const uint16_t* __restrict__ v, int64_t ldv,
-                const int64_t* __restrict__ slots, unsigned units, int* bad) {
+                const int64_t* __restrict__ slots, unsigned units, const int* err, int* bad) {
     grid_dep_wait();
     const unsigned from = (blockIdx.x * 4 + (threadIdx.x >> 5)) * EACH;
     if (from >= units) return;
@@ -151,6 +151,7 @@ kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk,
     const int mine = lane / (16 / EACH);       // the unit whose place and scale are this lane's
     const unsigned row = from / (unsigned)c.heads, my_row = (from + mine) / (unsigned)c.heads;
     const int64_t slot = mine < count ? slots[my_row] : -1, ld = is_v ? ldv : ldk;
+    const int failed = error_word(err);        // rows that a failed kernel should have made stay out of the cache
     int head = from - row * c.heads;
     const uint16_t* src = (is_v ? v : k) + row * ld + lane * 8;
     uint8_t* const base = is_v ? c.v : c.k;
@@ -162,7 +163,7 @@ kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk,
         if (i < count) x[i] = load8<VEC>(src + head * KV_D);
         if (++head == c.heads) { head = 0; src += ld; }
     }
-    const int64_t places = place(slot, from + mine - my_row * c.heads, c, bad);
+    const int64_t places = place(failed ? -1 : slot, from + mine - my_row * c.heads, c, bad);
     grid_dep_launch();
     float inv = 0.f;
     if (type != KV_BF16) {
@@ -386,6 +387,7 @@ struct KvKernel {
         Segment seg[TEAMS][2];
         Share share[TEAMS][2];
         int prefix[KV_SEQS + 1], cost[KV_SEQS], len[KV_SEQS], last[TEAMS][2];      // chunks and costs before a sequence
+        int rows[WARPS][STAGES][2];       // where the cache has a chunk's rows, 16 at a time, if new ones may go there, else negative
         int2 scan[WARPS + TEAMS];
         float m[TEAMS][KV_TEAM][8 * HG], l[TEAMS][KV_TEAM][8 * HG];
     };
@@ -606,7 +608,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         if (!solo) f += lane;
         if (lane >= KV_TEAM) c1 = 0;
         KvWalk at = {};
-        auto look = [&]() {        // the chunk's rows of the cache, 16 at a time; -1: none
+        auto look = [&]() {        // the chunk's rows of the cache, 16 at a time; -1: none, -2: a page outside the cache
             const int tok = at.c * KEYS, len = sh.len[at.b], head = a.chunks_of_heads == 1 ? at.item : at.item / a.chunks_of_heads;
 #pragma unroll
             for (int h = 0; h < KEYS / 16; ++h) {
@@ -614,11 +616,12 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 place[h] = -1;
                 if (token >= len) continue;
                 const int page = a.pages[at.b * a.ldp + p];
-                place[h] = 0;
+                place[h] = -2;
                 if ((unsigned)page >= (unsigned)a.c.pages) atomicExch(a.bad, ERR_KV_PLACE);
                 else place[h] = (page * a.c.heads + head) * ps + token - p * ps;
             }
         };
+        const int failed = a.kn ? error_word(a.err) : 0;       // a kernel before this one: no row goes into the cache
         if (f < c1) { at.seek(f, sh.prefix, a.batch, items); look(); }
         bool ok = true;
         for (int round = 0; ok; ++round) {
@@ -628,12 +631,14 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             f += by;
             if (f < c1) { at.step(by, sh.prefix, items); look(); }
             for (; left && ok; left &= left - 1) {
-                const int mate = __ffs(left) - 1, w = team * KV_TEAM + mate, r0 = __shfl_sync(0xffffffffu, now[0], mate), r1 = KEYS == 32 ? __shfl_sync(0xffffffffu, now[1], mate) : -1;
+                const int mate = __ffs(left) - 1, w = team * KV_TEAM + mate, p0 = __shfl_sync(0xffffffffu, now[0], mate), p1 = KEYS == 32 ? __shfl_sync(0xffffffffu, now[1], mate) : -1;
                 uint64_t* const full = &sh.full[w][slot];
                 if (elect_one()) {
                     ok = mbar_wait(&sh.empty[w][slot], ((round / STAGES) & 1) ^ 1);
                     if (!ok) atomicExch(a.err, ERR_KV_WAIT);
                     else {
+                        if (a.kn) { sh.rows[w][slot][0] = failed ? -1 : p0; sh.rows[w][slot][1] = failed ? -1 : p1; }
+                        const int r0 = max(p0, 0), r1 = p1 == -2 ? 0 : p1;       // (of a page outside, the cache's first rows are loaded)
                         uint8_t* const dst = smem + (w * STAGES + slot) * KV_STAGE_BYTES;
                         const uint32_t scales = smem_u32(smem) + K::SCALES + (w * STAGES + slot) * 256;
                         if (TYPE == KV_BF16) {
@@ -773,20 +778,17 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             const uint32_t st = smem_u32(smem) + (warp * STAGES + slot) * KV_STAGE_BYTES, scales = smem_u32(smem) + K::SCALES + (warp * STAGES + slot) * 256;
             const bool append = a.kn && valid <= KEYS;
             uint4 fresh = make_uint4(0, 0, 0, 0);
-            int page = -1, last = 0, kvh = 0;
             if (append) {
-                kvh = a.chunks_of_heads == 1 ? seg.item : seg.item / a.chunks_of_heads;
-                last = sh.len[seg.b] - 1;
+                const int kvh = a.chunks_of_heads == 1 ? seg.item : seg.item / a.chunks_of_heads;
                 const uint16_t* src = (lane < 16 ? a.kn + seg.b * a.ldk : a.vn + seg.b * a.ldv) + kvh * KV_D + (lane & 15) * 8;
                 fresh = (a.flags & 4) ? load8<true>(src) : load8<false>(src);
-                page = a.pages[seg.b * a.ldp + (shift >= 0 ? last >> shift : last / ps)];
             }
             if (ok && !mbar_wait(&sh.full[warp][slot], parity)) { ok = false; atomicExch(a.err, ERR_KV_WAIT); }
             __syncwarp();
             if (append) {     // the sequence's last row is the new one: into the ring, and into the cache
-                const int r = valid - 1, part = lane & 15;
-                const bool store = (a.chunks_of_heads == 1 || seg.item % a.chunks_of_heads == 0) && (unsigned)page < (unsigned)a.c.pages;
-                const int64_t at = ((int64_t)page * a.c.heads + kvh) * ps + (shift >= 0 ? last & (ps - 1) : last % ps);
+                const int r = valid - 1, part = lane & 15, row = ok ? sh.rows[warp][slot][r >> 4] : -1;
+                const bool store = (a.chunks_of_heads == 1 || seg.item % a.chunks_of_heads == 0) && row >= 0;
+                const int64_t at = (int64_t)row + (r & 15);
                 const uint32_t dst = st + (lane < 16 ? 0 : 4096) + r * 128;
                 uint8_t* const base = lane < 16 ? a.c.k : a.c.v;
                 if (TYPE == KV_BF16) {
@@ -1134,7 +1136,7 @@ hd_status o1_kv_write(const o1_kv_cache* cache, const void* k, int64_t ldk, cons
         const unsigned block = 4 * (few ? KV_EACH_OF_FEW : KV_EACH);
         auto kern = few ? (vec ? kv_write_kernel<true, KV_EACH_OF_FEW> : kv_write_kernel<false, KV_EACH_OF_FEW>) : vec ? kv_write_kernel<true, KV_EACH> : kv_write_kernel<false, KV_EACH>;
         if (!launch_ok(launch_chained(kern, dim3((units + block - 1) / block), dim3(128), 0, current_stream(), 1, 1, c, cache->type, (const uint16_t*)k + first * ldk, ldk,
-                                      (const uint16_t*)v + first * ldv, ldv, slots + first, units, device_table_word()), "kv_write"))
+                                      (const uint16_t*)v + first * ldv, ldv, slots + first, units, (const int*)device_error_word(), device_table_word()), "kv_write"))
             return HD_ERR_RUNTIME;
         o1_launch_count_add(1);
         if (rows - first <= most) break;

@@ -606,3 +606,50 @@ def test_a_wrong_slot_stops_no_other_call(pkg, dev):
     torch.cuda.synchronize()
     assert pkg.lib.o1_device_error() == 70 and pkg.lib.o1_device_error() == 0
     assert (y != 777.0).float().mean() > 0.99
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "int8"])
+@pytest.mark.parametrize("rows", [3, 3000])
+def test_nothing_is_written_after_a_failure(pkg, dev, kind, rows):
+    """A kernel before this one fails while the write waits for it: its rows may be stale and stay out of the cache."""
+    from latefail import late_failure
+    cache = pkg.KvCache(1 + rows // 32, 32, kind, 8, dev)
+    x = normal((rows, 8, D), gen(1)).to(dev)
+    slots = torch.arange(rows, device=dev)
+    cache.write(x, x, torch.full_like(slots, -1))
+    torch.cuda.synchronize()
+    late_failure(pkg, 98)
+    cache.write(x, x, slots)
+    torch.cuda.synchronize()
+    assert pkg.lib.o1_device_error() == 98
+    for t in (cache.k, cache.v):
+        assert (t.view(torch.uint8) == 0).all()
+    if kind != "bf16":
+        assert (cache.k_scale == 0).all() and (cache.v_scale == 0).all()
+    cache.write(x, x, slots)
+    assert (cache.k.view(torch.uint8) != 0).any()
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "int8"])
+@pytest.mark.parametrize("lens,heads", [([40, 700, 3], 4), ([20000], 8), ([1 + i % 20 for i in range(250)], 2)])
+def test_no_row_is_appended_after_a_failure(pkg, dev, kind, lens, heads):
+    """Whole items, shared ones and an item to a warp; the next call is as ever."""
+    from latefail import late_failure
+    c = Case(pkg, dev, kind, lens, 2, 32)
+    c.fill()
+    q = normal((len(lens), 2 * heads, D), gen(3)).to(dev)
+    new = normal((len(lens), 2, D), gen(4)).to(dev)
+    want, want_l = c.cache.attend(q, c.dtable, c.dlens, lse=True)
+    k, v = c.cache.k.view(torch.uint8).clone(), c.cache.v.view(torch.uint8).clone()
+    scales = [t.view(torch.int32).clone() for t in (c.cache.k_scale, c.cache.v_scale) if t is not None]
+    torch.cuda.synchronize()
+    late_failure(pkg, 98)
+    c.cache.attend(q, c.dtable, c.dlens, k=new, v=new)
+    torch.cuda.synchronize()
+    assert pkg.lib.o1_device_error() == 98
+    assert torch.equal(c.cache.k.view(torch.uint8), k) and torch.equal(c.cache.v.view(torch.uint8), v)
+    assert all(torch.equal(s, t.view(torch.int32)) for s, t in zip(scales, (c.cache.k_scale, c.cache.v_scale)))
+    again, again_l = c.cache.attend(q, c.dtable, c.dlens, lse=True)
+    assert torch.equal(again, want) and torch.equal(again_l, want_l)
