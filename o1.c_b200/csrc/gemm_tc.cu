@@ -1277,7 +1277,7 @@ gemm_pair_fit_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                 int mb, nb;
                 tile_coords(tile, num_m, g.num_n, group_m, mb, nb);
                 for (int kb = 0; kb < kblocks; ++kb) {
-                    if (!mbar_wait(&empty[stage], phase ^ 1)) { ok = false; atomicExch(g.err, 71); break; }
+                    if (!mbar_wait(&empty[stage], phase ^ 1)) { ok = false; atomicExch(g.err, 75); break; }
                     uint8_t* a_s = smem + stage * stage_bytes;
                     if (rank == 0) mbar_expect_tx(&full[stage], 2 * stage_bytes);      // both CTAs' halves
                     int a_c0 = kb * BK, a_c1 = (mb * 2 + (int)rank) * BM;
@@ -1299,11 +1299,11 @@ gemm_pair_fit_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
             uint32_t phase = 0, aphase = 0;
             bool ok = true;
             for (int tile = tile0; tile < num_tiles && ok; tile += tile_step) {
-                if (!mbar_wait(&tempty[as], aphase ^ 1)) { atomicExch(g.err, 72); break; }
+                if (!mbar_wait(&tempty[as], aphase ^ 1)) { atomicExch(g.err, 76); break; }
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + as * 256;
                 for (int kb = 0; kb < kblocks; ++kb) {
-                    if (!mbar_wait(&full[stage], phase)) { ok = false; atomicExch(g.err, 73); break; }
+                    if (!mbar_wait(&full[stage], phase)) { ok = false; atomicExch(g.err, 77); break; }
                     tc_fence_after();
                     const uint32_t a_addr = smem_u32(smem + stage * stage_bytes);
                     const uint64_t ad = umma_desc_sw128(a_addr, 16, 1024);
@@ -1335,7 +1335,7 @@ gemm_pair_fit_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                 uint2* bs = reinterpret_cast<uint2*>(stg + 32 * VQ_PITCH);
                 if (lane < 18) bs[lane] = *reinterpret_cast<const uint2*>(g.bias + col0 + lane * 4);
                 const bool got = __all_sync(0xffffffffu, mbar_wait(&tfull[as], aphase));
-                if (!got) { atomicExch(g.err, 74); break; }
+                if (!got) { atomicExch(g.err, 78); break; }
                 tc_fence_after();
                 vrope_head(g, t_row + half * 72, col0, bs, vcs, vsn, stg, row0, failed, lane);
                 __syncwarp();      // (the bias and the staged rows have been read)
@@ -1344,7 +1344,7 @@ gemm_pair_fit_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                 PlainEpilogue<EPI> plain;
                 plain.ahead(g, row0, col0, cols, half * 32, lane);
                 const bool got = __all_sync(0xffffffffu, mbar_wait(&tfull[as], aphase));
-                if (!got) { atomicExch(g.err, 74); break; }
+                if (!got) { atomicExch(g.err, 78); break; }
                 tc_fence_after();
                 plain.run(g, t_row, row0, col0, cols, half * 32, 64, stg, lane, failed);
             }

@@ -442,3 +442,21 @@ def test_a_pair_takes_tensor_memory_between_cluster_barriers():
         assert k.count("tmem_relinquish_pair(") == 1
         at = [k.index(c) for c in ("cluster_arrive()", "cluster_wait()", "tmem_alloc_pair(", "cluster_sync_all()", "tmem_relinquish_pair(", "grid_dep_launch()")]
         assert at == sorted(at), k[:200]
+
+
+def test_a_code_of_a_table_is_no_wait_s(pkg):
+    """o1_device_error() gives a failed wait's code or one of a wrong table entry; no number means both."""
+    import glob
+    csrc = os.path.join(os.path.dirname(os.path.abspath(pkg.__file__)), "csrc")
+    waits, tables = set(), set()
+    for path in glob.glob(os.path.join(csrc, "*.cu")):
+        text = open(path).read()
+        named = dict(re.findall(r"constexpr int (ERR_\w+) = (\d+);", text))
+        for word, code in re.findall(r"atomicExch\((?:\w+\.)?(\w+), (\w+)\)", text):
+            if code.isdigit() or code in named:
+                (tables if word == "bad" else waits).add((os.path.basename(path), int(named.get(code, code))))
+    codes = {c for _, c in tables}
+    assert codes == {70, 71} and waits
+    assert not codes & {c for _, c in waits}
+    kv = {c for f, c in waits if f == "kvcache.cu"}
+    assert kv == {72} and not kv & {c for f, c in waits if f != "kvcache.cu"}
