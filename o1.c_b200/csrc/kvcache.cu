@@ -257,7 +257,8 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
 //    other, 16 heads on one kv head took 45 us for 50000 bf16 rows, now 21.  An item costs a team 3.8 us however short it is, so where the table is short and items
 //    are many, each goes to one warp, which needs no join (200 sequences of 30 rows of fp8, 8 kv heads: 20 us, now 7.7).
 //  * Rounding: scores and sums in fp32.  Probabilities (times v's scale) enter the second product as two parts of bf16, value and rest, 16 bits of significand; codes
-//    of a byte are exact in f16 and bf16.  Keys' codes go through f16, which takes fewer instructions, with queries scaled to f16 by a power of two for each head;
+//    of a byte are exact in f16 and bf16.  Keys' codes go through f16, which takes fewer instructions, with queries scaled to f16's top by a power of two for each head (those
+//    below 2^-29 of its largest lose bits);
 //    values' codes through bf16, whose range a probability needs.  The result is rounded once.
 // Times below: "batch" 24 sequences of 1 to 2100 rows of bf16, "shared" 32 sequences of 1000 to 3000, 16 query heads on one kv head; us.
 static constexpr int KV_STAGE_BYTES = 8192;            // keys and values of a chunk
@@ -760,9 +761,11 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 for (int i = 0; i < 16; ++i) top = max(top, max(qa[h][i] & 0x7FFFu, (qa[h][i] >> 16) & 0x7FFFu));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const uint32_t e = min(max(top >> 7, 1u), 253u);         // the largest one's exponent
-                const float down = __uint_as_float((254u - e) << 23);
-                z_scale[h] *= __uint_as_float(e << 23);
+                // the largest one to between 2^15 and 2^16, the top of f16's range: values down to 2^-29 of it keep their eight bits, so that a large one
+                // whose keys are small costs the others nothing
+                const uint32_t e = min(max(top >> 7, 16u), 254u);         // the largest one's exponent
+                const float down = __uint_as_float((269u - e) << 23);
+                z_scale[h] *= __uint_as_float(e << 23);              // (the 2^15 goes with the keys' scales, which keeps scores as far from fp32's end as they were)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) qa[h][i] = pack_f16x2(bf16lo(qa[h][i]) * down, bf16hi(qa[h][i]) * down);
             }
@@ -838,7 +841,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 for (int n = 0; n < TILES; ++n) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const float ks = lds_f32(scales + (8 * n + 4 * j + t) * 4);
+                        const float ks = lds_f32(scales + (8 * n + 4 * j + t) * 4) * 3.0517578125e-05f;      // 2^-15
                         vs[n][j] = lds_f32(scales + 128 + (8 * n + 4 * j + t) * 4);
 #pragma unroll
                         for (int h = 0; h < HG; ++h) s[n][2 * h + j] *= ks;

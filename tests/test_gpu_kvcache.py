@@ -653,3 +653,19 @@ def test_no_row_is_appended_after_a_failure(pkg, dev, kind, lens, heads):
     assert all(torch.equal(s, t.view(torch.int32)) for s, t in zip(scales, (c.cache.k_scale, c.cache.v_scale)))
     again, again_l = c.cache.attend(q, c.dtable, c.dlens, lse=True)
     assert torch.equal(again, want) and torch.equal(again_l, want_l)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "int8"])
+@pytest.mark.parametrize("big", [14, 17, 20, 24])
+def test_queries_with_one_large_channel(pkg, dev, kind, big):
+    """A query's channel of 2^14 to 2^24 where the keys have zeros: the scores are of the others, and as exact as without it."""
+    lens = [100, 700]
+    c = Case(pkg, dev, kind, lens, 2, 32, std=1.0)
+    for x in c.k:
+        x[:, :, 0] = 0.0
+    c.fill()
+    q = normal((2, 8, D), gen(3), 2.0)
+    q[:, :, 0] = 2.0 ** big
+    out, lse = c.cache.attend(q.to(dev), c.dtable, c.dlens, lse=True)
+    c.check(q, out, lse, what=kind)
