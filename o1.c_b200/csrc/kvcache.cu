@@ -625,6 +625,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         const int failed = a.kn ? error_word(a.err) : 0;       // a kernel before this one: no row goes into the cache
         if (f < c1) { at.seek(f, sh.prefix, a.batch, items); look(); }
         bool ok = true;
+        int issued = 0;          // of the lane's warp
         for (int round = 0; ok; ++round) {
             unsigned left = __ballot_sync(0xffffffffu, f < c1);
             if (!left) break;
@@ -669,8 +670,12 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                     }
                 }
                 ok = __all_sync(0xffffffffu, ok);
+                if (lane == mate && ok) ++issued;
             }
         }
+        // Copies land before the block ends, also where a consumer has given up waiting for them: its shared memory is another block's then.
+        if (lane < KV_TEAM)
+            for (int r = max(0, issued - STAGES); r < issued; ++r) mbar_wait(&sh.full[team * KV_TEAM + lane][r % STAGES], (r / STAGES) & 1);
         return;
     }
 
