@@ -786,7 +786,7 @@ hd_status o1_kv_read(const o1_kv_cache *cache, void *k, int64_t ldk, void *v, in
  * k_new / v_new (both or neither): each sequence's row at position lens[b] - 1, stored into the cache (as by o1_kv_write) and
  * attended to by the same call.  workspace: o1_kv_attention_workspace_bytes(heads, kv_heads) bytes, 16-byte aligned, zero-filled once before its first use and
  * left to these calls from then on; calls that may overlap on the GPU each need their own.  The result is the same
- * bits from call to call.  Values of v up to 2^90 in magnitude (the sums are 2^20 times larger and in fp32); at most 2^31 - 1 rows (pages *
+ * bits from call to call with the same lengths and width; beside other sequences a sequence's differs by the order of its fp32 sums.  Values of v up to 2^90 in magnitude (the sums are 2^20 times larger and in fp32); at most 2^31 - 1 rows (pages *
  * kv_heads * page_size) in the cache. */
 int64_t o1_kv_attention_workspace_bytes(int heads, int kv_heads);
 hd_status o1_kv_attention(const o1_kv_cache *cache, const void *q, int64_t ldq, const void *k_new, int64_t ldk,
@@ -806,8 +806,9 @@ hd_status o1_residual_norm(const void *x, int64_t ldx, const void *branch, int64
  * all), ids int64 on the device, pos_f32 [3, rows] as hd_forward's, out [rows, hidden] bf16: the rows behind the final norm.
  * o1_prompt_rows: all rows of one sequence, causal, their keys and values into slots[r] of each cache.  o1_decode_step: one new row of each of `batch` sequences, which
  * becomes row lens[b] - 1 of sequence b.  scratch: o1_decode_scratch_bytes(rows, ...) bytes, its first o1_kv_attention_workspace_bytes zero-filled once (zero all
- * of it); one for each stream.  The residual stream's norms are of its unrounded sums (o1_residual_norm), so the rows agree with hd_decoder_block's within rounding, and a row
- * does not depend on which other rows a step has. */
+ * of it); one for each stream.  The residual stream's norms are of its unrounded sums (o1_residual_norm), so the rows agree with hd_decoder_block's within rounding.  A row is a
+ * function of its own sequence within rounding too: the same step gives the same bits, but how a sequence's cached rows are shared out, and with it the order of fp32
+ * sums, follows from the lengths of all sequences of the step. */
 int64_t o1_decode_scratch_bytes(int64_t rows, int heads, int kv_heads, int hidden, int ff_hidden, int head_dim);
 hd_status o1_prompt_rows(const hd_forward_binding *bw, const o1_kv_cache *caches, const int64_t *ids, const float *pos_f32,
                          const int64_t *slots, void *scratch, int64_t scratch_bytes, void *out, int rows, int heads,

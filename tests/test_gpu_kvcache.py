@@ -669,3 +669,20 @@ def test_queries_with_one_large_channel(pkg, dev, kind, big):
     q[:, :, 0] = 2.0 ** big
     out, lse = c.cache.attend(q.to(dev), c.dtable, c.dlens, lse=True)
     c.check(q, out, lse, what=kind)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "int8"])
+@pytest.mark.parametrize("lens", [[600, 17, 90, 2500, 33, 1, 300, 600], [600] * 32])
+def test_a_sequence_alone_and_among_others(pkg, dev, kind, lens):
+    """How rows are shared out follows from all lengths, so the bits may differ; alone and among others a sequence's result keeps its bound from 64 bits."""
+    c = Case(pkg, dev, kind, lens, 8, 32, seed=3)
+    c.fill()
+    q = normal((len(lens), 32, D), gen(3), 1.5)
+    out, lse = c.cache.attend(q.to(dev), c.dtable, c.dlens, lse=True)
+    c.check(q, out, lse, what="together")
+    every = c.lens, c.k, c.v
+    for b in range(min(len(lens), 8)):
+        out, lse = c.cache.attend(q[b:b + 1].to(dev), c.dtable[b:b + 1], c.dlens[b:b + 1], lse=True)
+        c.lens, c.k, c.v = every[0][b:b + 1], every[1][b:b + 1], every[2][b:b + 1]
+        c.check(q[b:b + 1], out, lse, what=f"sequence {b} alone")
