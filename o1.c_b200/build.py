@@ -27,8 +27,9 @@ def _binding_command():
     import torch
     root = os.path.dirname(torch.__file__)
     return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-            + [f"-I{d}" for d in (sysconfig.get_paths()["include"], os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"))]
-            + [BINDING_SRC, "-o", BINDING, f"-L{os.path.join(root, 'lib')}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10"])
+            + [f"-I{d}" for d in (sysconfig.get_paths()["include"], os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                                  os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include"))]
+            + [BINDING_SRC, "-o", BINDING, f"-L{os.path.join(root, 'lib')}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10_cuda", "-lc10"])
 
 
 def _nvcc():

@@ -3,6 +3,7 @@
 // The entry points come as addresses from the loaded library (setup); nothing of it is linked here, and the library knows nothing of torch.
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -44,6 +45,17 @@ bool status(hd_status rc, const char* what) {        // Python's check() takes t
     if (r) PyErr_Format(O1Error, "%s failed", what);
     return false;
 }
+
+// The library's current stream as torch's, where they differ: what torch allocates, copies and frees on a call's behalf is in the order of the call's kernels.
+struct OnLibrary {
+    c10::cuda::OptionalCUDAStreamGuard guard;
+    explicit OnLibrary(int device) {
+        const auto at = (c10::DeviceIndex)device;
+        const auto stream = (cudaStream_t)f_stream();
+        if (c10::cuda::getCurrentCUDAStream(at).stream() != stream)
+            guard.reset_stream(stream ? c10::cuda::getStreamFromExternal(stream, at) : c10::cuda::getDefaultCUDAStream(at));
+    }
+};
 
 // As torch.empty() makes it, without the dispatcher's steps (0.3 us of a call).
 at::Tensor empty_on(at::IntArrayRef size, at::ScalarType type, int device) {
@@ -118,6 +130,7 @@ PyObject* py_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!h || !slots) return nullptr;
     const int64_t rows = slots_of(*slots, h, who);
     if (rows < 0) return nullptr;
+    const OnLibrary on(h->device);
     at::Tensor out[2];
     int64_t ld[2] = {h->heads * D, h->heads * D};
     for (int i = 0; i < 2; ++i) {
@@ -162,6 +175,7 @@ PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
         pk = k->data_ptr();
         pv = v->data_ptr();
     }
+    const OnLibrary on(h->device);
     at::Tensor out, lse;
     if (a[7] == Py_None) {
         out = empty_on({batch, heads, D}, at::kBFloat16, h->device);
@@ -250,6 +264,7 @@ PyObject* py_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (each[i] > groups) groups = each[i];
     }
     if ((mod[1] == nullptr) != (mod[2] == nullptr)) return fail(who, "scale and shift, both or neither");
+    const OnLibrary on(device);
     at::Tensor spread[3];
     void* pm[3];
     for (int i = 0; i < 3; ++i) {

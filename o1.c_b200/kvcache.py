@@ -3,9 +3,11 @@ two norms -- o1_kv_write, o1_kv_read, o1_kv_attention and o1_residual_norm on to
 
 Like every entry point they enqueue on the library's current stream (use_torch_stream()) and return at once.  Arguments that
 do not fit raise O1Error; a slot, page or length that does not fit is found on the device (lib.o1_device_error() gives 70 or 71).
+Where torch's current stream is another one, what these calls make (caches, results, tables) is made, filled and freed in the order of the library's;
+ordering that, and their inputs, with torch's own work is the caller's.
 """
+import contextlib
 import ctypes as C
-
 import os
 
 import torch
@@ -30,9 +32,18 @@ def _need(ok, what):
         raise O1Error(what)
 
 
+def _on_library(device):
+    """The library's current stream as torch's, for what torch does on a call's behalf."""
+    s = _stream() or 0
+    if torch.device(device).type != "cuda" or torch.cuda.current_stream(device).cuda_stream == s:
+        return contextlib.nullcontext()
+    # (an ExternalStream of 0 would be a new stream, not the default one)
+    return torch.cuda.stream(torch.cuda.ExternalStream(s, device) if s else torch.cuda.default_stream(device))
+
+
 def _zeros(n, device):
     """n bytes of zeros, filled on the library's current stream."""
-    with torch.cuda.stream(torch.cuda.ExternalStream(_stream() or 0, device)):
+    with _on_library(device):
         return torch.zeros(n, dtype=torch.uint8, device=device)
 
 
@@ -46,9 +57,10 @@ class KvCache:
         _need(kind in KINDS, f"KvCache: kind {kind!r} (one of {', '.join(KINDS)})")
         shape = (pages, kv_heads, page_size, HEAD_DIM)
         dtype = KINDS[kind][1]
-        k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) if kind != "bf16" else
-                torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
-        ks, vs = (torch.zeros(shape[:3], device=device) if kind != "bf16" else None for _ in range(2))
+        with _on_library(device):
+            k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) if kind != "bf16" else
+                    torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
+            ks, vs = (torch.zeros(shape[:3], device=device) if kind != "bf16" else None for _ in range(2))
         self._set(k, v, ks, vs)
 
     @classmethod
@@ -152,7 +164,13 @@ class Decoder:
         if self._table[seq] is None:
             row = torch.zeros(self.width, dtype=torch.int32)
             row[:len(pages)] = torch.tensor(pages, dtype=torch.int32)
-            self._table[seq] = row.to(self.device)
+            with _on_library(self.device):
+                self._table[seq] = row.to(self.device)
+
+    def _slots(self, seq, n):
+        """Slots and numbers of a sequence's first n rows."""
+        t = torch.arange(n, device=self.device)
+        return self._table[seq].long()[t // self.page_size] * self.page_size + t % self.page_size, t
 
     def prompt(self, ids):
         """A new sequence of rows ids [n] (int64): (its name, hidden rows [n, hidden])."""
@@ -170,13 +188,13 @@ class Decoder:
             raise
         self._next += 1
         self._len[seq] = n
-        t = torch.arange(n, device=self.device)
-        slots = self._table[seq].long()[t // self.page_size] * self.page_size + t % self.page_size
-        pos = t.float().expand(3, n).contiguous()
-        out = torch.empty(n, self.dims[2], dtype=BF16, device=self.device)
-        s = self._room(n)
-        check(lib.o1_prompt_rows(C.byref(self.w.binding), self._c, ptr(ids.contiguous()), ptr(pos), ptr(slots), ptr(s), s.numel(), ptr(out), n, *self.dims),
-              "o1_prompt_rows")
+        with _on_library(self.device):
+            slots, t = self._slots(seq, n)
+            pos, ids = t.float().expand(3, n).contiguous(), ids.contiguous()
+            out = torch.empty(n, self.dims[2], dtype=BF16, device=self.device)
+            s = self._room(n)
+            check(lib.o1_prompt_rows(C.byref(self.w.binding), self._c, ptr(ids), ptr(pos), ptr(slots), ptr(s), s.numel(), ptr(out), n, *self.dims),
+                  "o1_prompt_rows")
         return seq, out
 
     def step(self, seqs, ids):
@@ -190,21 +208,22 @@ class Decoder:
             self._grow(s, self._len[s] + 1)
         for s in seqs:
             self._len[s] += 1
-        lens = torch.tensor([self._len[s] for s in seqs], dtype=I32).to(self.device)
-        pages = torch.stack([self._table[s] for s in seqs]) if n else torch.zeros(0, self.width, dtype=I32, device=self.device)
-        pos = (lens - 1).float().expand(3, n).contiguous()
-        out = torch.empty(n, self.dims[2], dtype=BF16, device=self.device)
-        s = self._room(n)
-        check(lib.o1_decode_step(C.byref(self.w.binding), self._c, ptr(ids.contiguous()), ptr(pos), ptr(pages), self.width, self.width, ptr(lens), ptr(s), s.numel(),
-                                 ptr(out), n, *self.dims), "o1_decode_step")
+        with _on_library(self.device):
+            lens = torch.tensor([self._len[s] for s in seqs], dtype=I32).to(self.device)
+            pages = torch.stack([self._table[s] for s in seqs]) if n else torch.zeros(0, self.width, dtype=I32, device=self.device)
+            pos, ids = (lens - 1).float().expand(3, n).contiguous(), ids.contiguous()
+            out = torch.empty(n, self.dims[2], dtype=BF16, device=self.device)
+            s = self._room(n)
+            check(lib.o1_decode_step(C.byref(self.w.binding), self._c, ptr(ids), ptr(pos), ptr(pages), self.width, self.width, ptr(lens), ptr(s), s.numel(),
+                                     ptr(out), n, *self.dims), "o1_decode_step")
         return out
 
     def rows(self, seq, layer):
         """(keys, values) [rows, kv_heads, 128] bf16 that a layer keeps of a sequence, as KvCache.read gives them."""
         if seq not in self._pages:
             raise O1Error(f"Decoder.rows: no sequence {seq}")
-        t = torch.arange(self._len[seq], device=self.device)
-        return self.caches[layer].read(self._table[seq].long()[t // self.page_size] * self.page_size + t % self.page_size)
+        with _on_library(self.device):
+            return self.caches[layer].read(self._slots(seq, self._len[seq])[0])
 
     def close(self, seq):
         """Gives a sequence's pages back.  (Calls on other streams that still read them are the caller's to wait for.)"""
