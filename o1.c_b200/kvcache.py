@@ -47,6 +47,12 @@ def _zeros(n, device):
         return torch.zeros(n, dtype=torch.uint8, device=device)
 
 
+def _to_gpu(values, device):
+    """A list of the host's as int32 on the GPU, copied on the library's current stream from pinned memory: the host does not wait for what is under way."""
+    with _on_library(device):
+        return torch.tensor(values, dtype=I32, pin_memory=True).to(device, non_blocking=True)
+
+
 class KvCache:
     """Keys and values of many sequences in pages of page_size tokens, [pages, kv_heads, page_size, 128].
 
@@ -128,7 +134,7 @@ class Decoder:
     """Continues prompts through the decoder blocks, a row of every sequence at a time, over cached keys and values.
 
     weights: Weights (or GgufWeights).  max_seqs sequences of at most max_tokens rows each; kind: how keys and values are kept (KvCache).
-    prompt() and step() return rows behind the final norm, [rows, hidden] bf16, and enqueue on the library's current stream."""
+    prompt() and step() return rows behind the final norm, [rows, hidden] bf16, enqueue on the library's current stream and return at once; they cannot be captured."""
 
     def __init__(self, weights, max_seqs, max_tokens, kind="bf16", page_size=64):
         d = weights.dims
@@ -162,10 +168,11 @@ class Decoder:
             pages.append(self._free.pop())
             self._table[seq] = None
         if self._table[seq] is None:
-            row = torch.zeros(self.width, dtype=torch.int32)
-            row[:len(pages)] = torch.tensor(pages, dtype=torch.int32)
-            with _on_library(self.device):
-                self._table[seq] = row.to(self.device)
+            self._table[seq] = _to_gpu(pages + [0] * (self.width - len(pages)), self.device)
+
+    def _not_captured(self, what):
+        if lib.o1_capture_id():
+            raise O1Error(f"Decoder.{what}: lengths and pages are the host's, which a graph would not see (capture o1_decode_step with tables on the GPU)")
 
     def _slots(self, seq, n):
         """Slots and numbers of a sequence's first n rows."""
@@ -179,6 +186,7 @@ class Decoder:
             raise O1Error("Decoder.prompt: ids int64 [n] on the GPU wanted, n > 0")
         if len(self._pages) == self.max_seqs:
             raise O1Error(f"Decoder.prompt: {self.max_seqs} sequences are open")
+        self._not_captured("prompt")
         seq = self._next
         self._pages[seq], self._len[seq], self._table[seq] = [], 0, None
         try:
@@ -202,6 +210,7 @@ class Decoder:
         n = len(seqs)
         if ids.dtype is not I64 or ids.dim() != 1 or ids.numel() != n or not ids.is_cuda or len(set(seqs)) != n:
             raise O1Error("Decoder.step: ids int64, one for each of different sequences, on the GPU wanted")
+        self._not_captured("step")
         for s in seqs:
             if s not in self._pages:
                 raise O1Error(f"Decoder.step: no sequence {s}")
@@ -209,7 +218,7 @@ class Decoder:
         for s in seqs:
             self._len[s] += 1
         with _on_library(self.device):
-            lens = torch.tensor([self._len[s] for s in seqs], dtype=I32).to(self.device)
+            lens = _to_gpu([self._len[s] for s in seqs], self.device)
             pages = torch.stack([self._table[s] for s in seqs]) if n else torch.zeros(0, self.width, dtype=I32, device=self.device)
             pos, ids = (lens - 1).float().expand(3, n).contiguous(), ids.contiguous()
             out = torch.empty(n, self.dims[2], dtype=BF16, device=self.device)

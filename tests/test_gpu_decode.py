@@ -220,3 +220,46 @@ def test_a_wrong_entry_reaches_one_sequence_only(pkg, dev, weights, kind, what, 
     others = [p for p in range(dec.caches[0].pages) if p not in mine]
     for c, (k, v) in zip(dec.caches, after):
         assert torch.equal(c.k.view(torch.uint8)[others], k[others]) and torch.equal(c.v.view(torch.uint8)[others], v[others])
+
+
+@gpu
+def test_a_step_does_not_wait(pkg, dev, weights):
+    """A prompt and a step return while the stream is still busy with what came before."""
+    dec = pkg.Decoder(weights, 2, 64, "int8", 16)
+    a, _ = dec.prompt(ids_of(20, 1).to(dev))
+    new, two = ids_of(1, 2).to(dev), ids_of(9, 3).to(dev)
+    dec.step([a], new)
+    b, _ = dec.prompt(two)
+    dec.close(b)
+    for call in (lambda: dec.step([a], new), lambda: dec.prompt(two)):
+        torch.cuda.synchronize()
+        torch.cuda._sleep(2000000000)
+        e = torch.cuda.Event()
+        e.record()
+        call()
+        assert not e.query()
+    torch.cuda.synchronize()
+
+
+@gpu
+def test_calls_in_a_capture_are_refused(pkg, dev, weights):
+    """A graph would keep the lengths and pages of its capture; nothing is changed, and what else is captured stays."""
+    dec = pkg.Decoder(weights, 2, 64, "bf16", 16)
+    a, _ = dec.prompt(ids_of(20, 1).to(dev))
+    new, x = ids_of(1, 2).to(dev), torch.zeros(4, device=dev)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph, stream=s):
+            pkg.use_torch_stream()
+            x += 1
+            with pytest.raises(pkg.O1Error, match="Decoder.step.*graph"):
+                dec.step([a], new)
+            with pytest.raises(pkg.O1Error, match="Decoder.prompt.*graph"):
+                dec.prompt(new)
+    finally:
+        pkg.use_torch_stream()
+    graph.replay()
+    assert (x == 1).all() and dec.rows(a, 0)[0].size(0) == 20
+    dec.step([a], new)
