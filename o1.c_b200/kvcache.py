@@ -188,21 +188,20 @@ class Decoder:
             raise O1Error(f"Decoder.prompt: {self.max_seqs} sequences are open")
         self._not_captured("prompt")
         seq = self._next
-        self._pages[seq], self._len[seq], self._table[seq] = [], 0, None
+        self._pages[seq], self._len[seq], self._table[seq] = [], n, None
         try:
             self._grow(seq, n)
-        except O1Error:
+            with _on_library(self.device):
+                slots, t = self._slots(seq, n)
+                pos, ids = t.float().expand(3, n).contiguous(), ids.contiguous()
+                out = torch.empty(n, self.dims[2], dtype=BF16, device=self.device)
+                s = self._room(n)
+                check(lib.o1_prompt_rows(C.byref(self.w.binding), self._c, ptr(ids), ptr(pos), ptr(slots), ptr(s), s.numel(), ptr(out), n, *self.dims),
+                      "o1_prompt_rows")
+        except BaseException:        # its name would reach nobody
             self.close(seq)
             raise
         self._next += 1
-        self._len[seq] = n
-        with _on_library(self.device):
-            slots, t = self._slots(seq, n)
-            pos, ids = t.float().expand(3, n).contiguous(), ids.contiguous()
-            out = torch.empty(n, self.dims[2], dtype=BF16, device=self.device)
-            s = self._room(n)
-            check(lib.o1_prompt_rows(C.byref(self.w.binding), self._c, ptr(ids), ptr(pos), ptr(slots), ptr(s), s.numel(), ptr(out), n, *self.dims),
-                  "o1_prompt_rows")
         return seq, out
 
     def step(self, seqs, ids):
@@ -215,16 +214,16 @@ class Decoder:
             if s not in self._pages:
                 raise O1Error(f"Decoder.step: no sequence {s}")
             self._grow(s, self._len[s] + 1)
-        for s in seqs:
-            self._len[s] += 1
         with _on_library(self.device):
-            lens = _to_gpu([self._len[s] for s in seqs], self.device)
+            lens = _to_gpu([self._len[s] + 1 for s in seqs], self.device)
             pages = torch.stack([self._table[s] for s in seqs]) if n else torch.zeros(0, self.width, dtype=I32, device=self.device)
             pos, ids = (lens - 1).float().expand(3, n).contiguous(), ids.contiguous()
             out = torch.empty(n, self.dims[2], dtype=BF16, device=self.device)
             s = self._room(n)
             check(lib.o1_decode_step(C.byref(self.w.binding), self._c, ptr(ids), ptr(pos), ptr(pages), self.width, self.width, ptr(lens), ptr(s), s.numel(),
                                      ptr(out), n, *self.dims), "o1_decode_step")
+        for name in seqs:            # (rows of a call that has failed are not counted: the next one writes them)
+            self._len[name] += 1
         return out
 
     def rows(self, seq, layer):

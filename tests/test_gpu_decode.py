@@ -263,3 +263,38 @@ def test_calls_in_a_capture_are_refused(pkg, dev, weights):
     graph.replay()
     assert (x == 1).all() and dec.rows(a, 0)[0].size(0) == 20
     dec.step([a], new)
+
+
+class Fails:
+    """The library with one entry point that fails."""
+
+    def __init__(self, lib, name):
+        self._lib, self._name = lib, name
+
+    def __getattr__(self, n):
+        return (lambda *a: 3) if n == self._name else getattr(self._lib, n)
+
+
+@gpu
+def test_failed_calls_change_nothing(pkg, dev, weights, monkeypatch):
+    """A failed prompt leaves no sequence open, a failed step counts no row."""
+    import sys
+    kv = sys.modules[pkg.Decoder.__module__]
+    dec, same = pkg.Decoder(weights, 2, 64, "bf16", 16), pkg.Decoder(weights, 2, 64, "bf16", 16)
+    a, _ = dec.prompt(ids_of(20, 1).to(dev))
+    b, _ = same.prompt(ids_of(20, 1).to(dev))
+    free = len(dec._free)
+    with monkeypatch.context() as m:
+        m.setattr(kv, "lib", Fails(kv.lib, "o1_prompt_rows"))
+        for _ in range(3):
+            with pytest.raises(pkg.O1Error, match="o1_prompt_rows"):
+                dec.prompt(ids_of(30, 2).to(dev))
+    assert len(dec._free) == free
+    c, _ = dec.prompt(ids_of(30, 2).to(dev))
+    with monkeypatch.context() as m:
+        m.setattr(kv, "lib", Fails(kv.lib, "o1_decode_step"))
+        with pytest.raises(pkg.O1Error, match="o1_decode_step"):
+            dec.step([a, c], ids_of(2, 3).to(dev))
+    new = ids_of(1, 4).to(dev)
+    assert torch.equal(dec.step([a], new), same.step([b], new))
+    assert dec.rows(a, 0)[0].size(0) == 21
