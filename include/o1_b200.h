@@ -454,6 +454,10 @@ void o1_set_stream(void *stream);
 void *o1_get_stream(void);
 /* The capture that stream is in, by a number of its own; 0: none.  (What a captured call keeps for itself must not serve calls outside.) */
 uint64_t o1_capture_id(void);
+/* Keeps an eye on that capture's graph (0: there is none, or it cannot be watched; else o1_capture_id()): o1_capture_gone(id) says once, with 1, that the graph and
+ * all that was made of it have been destroyed, so that what the capture kept for itself can go too. */
+uint64_t o1_capture_watch(void);
+int o1_capture_gone(uint64_t id);
 /* Kernels whose bounded waits ran out record a code in a device word, and kernels
  * after them store nothing until it is cleared; an entry of a caller's table that does
  * not fit (o1_kv_*) is recorded in a word of its own, which stops nothing.  This reads

@@ -246,6 +246,8 @@ _sig("hd_forward_binding_free", None, C.POINTER(ForwardBinding))
 _sig("o1_set_stream", None, _P)
 _sig("o1_get_stream", _P)
 _sig("o1_capture_id", C.c_uint64)
+_sig("o1_capture_watch", C.c_uint64)
+_sig("o1_capture_gone", c_int, C.c_uint64)
 _sig("o1_device_error", c_int)
 _sig("o1_sm_count", c_int)
 _sig("o1_profile_enable", None, c_int)

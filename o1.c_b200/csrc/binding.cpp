@@ -197,10 +197,10 @@ PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (PyErr_Occurred()) return nullptr;
     void* const stream = f_stream();
     const uint64_t capture = f_capture();
-    const Handle::Work* work = nullptr;
-    for (const auto& w : h->work)
-        if (w.stream == stream && w.capture == capture && w.heads == heads) work = &w;
-    if (!work) {       // the cache object makes it, and keeps it
+    Handle::Work* work = nullptr;
+    for (auto& w : h->work)
+        if (w.stream == stream && w.heads == heads) work = &w;
+    if (!work || work->capture != capture) {       // the cache object has it
         PyObject* made = PyObject_CallMethod(a[1], "_workspace", "L", (long long)heads);
         if (!made) return nullptr;
         Handle::Work w = {stream, capture, heads, nullptr, 0};
@@ -211,8 +211,11 @@ PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (!got) return nullptr;
         w.p = (void*)p;
         w.bytes = bytes;
-        h->work.push_back(w);
-        work = &h->work.back();
+        if (work) *work = w;       // (a stream is in one capture at a time)
+        else {
+            h->work.push_back(w);
+            work = &h->work.back();
+        }
     }
     if (!status(f_attend(h->cache, q->data_ptr(), ldq, pk, ldk, pv, ldv, (const int32_t*)pages->data_ptr(), ldp, (int)width, (const int32_t*)lens->data_ptr(), out.data_ptr(), ldo,
                          (float*)pl, (int)batch, (int)heads, (float)scale, work->p, work->bytes), "o1_kv_attention"))

@@ -24,6 +24,7 @@
 #include <atomic>
 #include <map>
 #include <mutex>
+#include <set>
 #include <vector>
 
 // ===================================================================== state
@@ -140,6 +141,39 @@ uint64_t o1_capture_id(void) {
     unsigned long long id = 0;
     if (cudaStreamGetCaptureInfo(g_stream, &status, &id) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
     return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+// Captures whose graphs are gone.  Filled by the runtime's callbacks, which may come from a thread of its own, also while the process ends: never destroyed.
+struct GoneCaptures {
+    std::mutex mu;
+    std::set<uint64_t> ids;
+};
+static GoneCaptures& gone_captures() {
+    static GoneCaptures* const g = new GoneCaptures;
+    return *g;
+}
+static void CUDART_CB capture_gone(void* id) {
+    std::lock_guard<std::mutex> lk(gone_captures().mu);
+    gone_captures().ids.insert((uint64_t)(uintptr_t)id);
+}
+uint64_t o1_capture_watch(void) {
+    cudaStreamCaptureStatus status;
+    unsigned long long id = 0;
+    cudaGraph_t graph = nullptr;
+    cudaUserObject_t object;
+    (void)gone_captures();
+    if (cudaStreamGetCaptureInfo_v2(g_stream, &status, &id, &graph, nullptr, nullptr) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
+    if (status != cudaStreamCaptureStatusActive || !graph) return 0;
+    if (cudaUserObjectCreate(&object, (void*)(uintptr_t)id, capture_gone, 1, cudaUserObjectNoDestructorSync) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
+    if (cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove) != cudaSuccess) {
+        (void)cudaGetLastError();
+        cudaUserObjectRelease(object, 1);
+        return 0;
+    }
+    return id;
+}
+int o1_capture_gone(uint64_t id) {
+    std::lock_guard<std::mutex> lk(gone_captures().mu);
+    return gone_captures().ids.erase(id) ? 1 : 0;
 }
 int o1_sm_count(void) { return sm_count(); }
 void o1_launch_count_add(int n) { count(n); }

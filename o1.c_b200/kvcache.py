@@ -53,6 +53,31 @@ def _to_gpu(values, device):
         return torch.tensor(values, dtype=I32, pin_memory=True).to(device, non_blocking=True)
 
 
+class _Workspace:
+    """Scratch of attend(), for all caches: one for each device, stream and capture, as calls that overlap must not share it (and a capture's is filled by its graph).
+    A stream's stays, a capture's goes when its graph has."""
+    made, watched = {}, {}
+
+    def __init__(self, device, nbytes):
+        self.scratch = _zeros(nbytes, device)
+        self.address = self.scratch.data_ptr()
+
+    def data_ptr(self):
+        return self.address
+
+    @classmethod
+    def get(cls, device, capture, nbytes):
+        key = (device, _stream(), capture, nbytes)
+        if key not in cls.made:
+            for gone in [c for c in cls.watched if lib.o1_capture_gone(c)]:
+                for k in cls.watched.pop(gone):
+                    cls.made.pop(k).scratch = None
+            cls.made[key] = cls(device, nbytes)
+            if capture and (capture in cls.watched or lib.o1_capture_watch()):
+                cls.watched.setdefault(capture, []).append(key)
+        return cls.made[key]
+
+
 class KvCache:
     """Keys and values of many sequences in pages of page_size tokens, [pages, kv_heads, page_size, 128].
 
@@ -105,12 +130,14 @@ class KvCache:
         return _binding.read(self._h, slots, *out)
 
     def _workspace(self, heads):
-        """Scratch of attend(), its address and bytes: one for each stream the calls run on and for each capture, as calls that overlap must not share it
-        (and a capture's is filled by its graph).  Kept as long as the cache."""
+        """Address and bytes of attend()'s scratch for the library's current stream."""
         need = lib.o1_kv_attention_workspace_bytes(heads, self.kv_heads)
         _need(need >= 0, f"KvCache.attend: heads {heads} (a multiple of kv_heads {self.kv_heads})")
-        t = self._work[_stream(), lib.o1_capture_id(), heads] = _zeros(need, self.device)
-        return t.data_ptr(), need
+        capture = lib.o1_capture_id()
+        w = _Workspace.get(self.device, capture, need)
+        self._work = {k: old for k, old in self._work.items() if old.scratch is not None}
+        self._work[_stream(), capture, heads] = w
+        return w.address, need
 
     def attend(self, q, pages, lens, k=None, v=None, out=None, lse=None, scale=None):
         """Attention of one new row per sequence, q [batch, heads, 128] bf16, over its first lens[b] cached rows.

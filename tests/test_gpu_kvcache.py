@@ -686,3 +686,51 @@ def test_a_sequence_alone_and_among_others(pkg, dev, kind, lens):
         out, lse = c.cache.attend(q[b:b + 1].to(dev), c.dtable[b:b + 1], c.dlens[b:b + 1], lse=True)
         c.lens, c.k, c.v = every[0][b:b + 1], every[1][b:b + 1], every[2][b:b + 1]
         c.check(q[b:b + 1], out, lse, what=f"sequence {b} alone")
+
+
+@gpu
+def test_caches_of_one_stream_share_a_workspace(pkg, dev):
+    """Calls on a stream follow one another: a model's caches, one of each layer, need one workspace."""
+    q, pages, lens = normal((2, 16, D), gen(1)).to(dev), torch.zeros(2, 1, dtype=torch.int32, device=dev), torch.ones(2, dtype=torch.int32, device=dev)
+    caches = [pkg.KvCache(2, 16, "int8", 1, dev) for _ in range(9)]
+    caches[0].attend(q, pages, lens)
+    torch.cuda.synchronize()
+    at = torch.cuda.memory_allocated()
+    for c in caches[1:]:
+        c.attend(q, pages, lens)
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() - at < 2 ** 20
+
+
+@gpu
+def test_workspaces_of_captures_go_with_their_graphs(pkg, dev):
+    """A process that captures again and again does not grow; a graph that lives keeps its own."""
+    import gc
+    c = Case(pkg, dev, "int8", [5000, 2000], 1, 32)
+    c.fill()
+    q = normal((2, 8, D), gen(3)).to(dev)
+    out = torch.empty_like(q)
+    s = torch.cuda.Stream()
+
+    def once():
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            pkg.use_torch_stream()
+            c.cache.attend(q, c.dtable, c.dlens, out=out)
+        g.replay()
+        torch.cuda.synchronize()
+        return g
+    try:
+        sizes, kept = [], once()
+        for _ in range(12):
+            once()
+            gc.collect()
+            sizes.append(torch.cuda.memory_allocated())
+        want = c.cache.attend(q, c.dtable, c.dlens)
+        kept.replay()
+        torch.cuda.synchronize()
+    finally:
+        pkg.use_torch_stream()
+    # (a destroyed graph is reported by a thread of the runtime's, so one or two may be there)
+    assert sizes[-1] - sizes[3] < 3 * pkg.lib.o1_kv_attention_workspace_bytes(8, 1), sizes
+    assert torch.equal(out, want)
