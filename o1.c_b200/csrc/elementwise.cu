@@ -178,16 +178,18 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
     return s;
 }
 // 1 / sqrt(mean of squares + eps) of a row, `squares(f)` a thread's part of the sum of its values times f.  Squares of values
-// above 2^57 or so do not fit fp32: such a row (and one with a NaN, to which it makes no difference) is summed again at 2^-80.
+// above 2^57 or so do not fit fp32, nor do those below 2^-63: a row of the former (and one with a NaN, to which it makes no difference) is summed again at 2^-80, and one
+// whose mean, eps included, is below 2^-100 at 2^80.
 template <int THREADS, class F>
 __device__ __forceinline__ float row_rms_inv(F squares, int cols, float eps, float (*red)[32]) {
-    const float sum = row_sum<THREADS>(squares(1.0f), red[0]);
-    if (sum < INFINITY) return rsqrtf(sum / (float)cols + eps);
-    return rsqrtf(row_sum<THREADS>(squares(8.271806125530277e-25f), red[1]) / (float)cols) * 8.271806125530277e-25f;
+    const float sum = row_sum<THREADS>(squares(1.0f), red[0]), mean = sum / (float)cols + eps;
+    if (mean > 7.888609052210118e-31f && mean < INFINITY) return rsqrtf(mean);
+    const float s = sum < 1.0f ? 1.2089258196146292e24f : 8.271806125530277e-25f;       // 2^80, 2^-80
+    return rsqrtf(row_sum<THREADS>(squares(s), red[1]) / (float)cols + eps * s * s) * s;
 }
-// THREADS: 32 = a warp to a row, four rows to a block; 0 = a block of any size to a row; else as many rows on an SM as 64 or 72 registers to a thread give.
+// THREADS: 32 = a warp to a row, four rows to a block; 0 = a block of any size to a row; else as many rows on an SM as 64 or 72 registers to a thread give (128 where a warp has a row: 4093 x 1152 7.9 us, with 129 9.2).
 template <int THREADS, int ITEMS, bool POST, bool AHEAD>
-__global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS ? THREADS : 1024, THREADS == 128 ? 7 : THREADS == 256 ? 4 : THREADS == 512 ? 2 : 1)
+__global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS ? THREADS : 1024, THREADS == 32 ? 4 : THREADS == 128 ? 7 : THREADS == 256 ? 4 : THREADS == 512 ? 2 : 1)
 residual_norm_vec_kernel(const ResidualNorm a) {
     grid_dep_wait();
     __shared__ float red[4][32];

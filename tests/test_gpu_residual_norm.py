@@ -141,3 +141,21 @@ def test_the_entry_point_refuses_before_it_touches_the_gpu(pkg):
         assert b"residual_norm" in pkg.lib.hd_cuda_last_error()
     assert call(rows=0) == 0
     pkg.lib.hd_cuda_clear_error()
+
+
+@gpu
+@pytest.mark.parametrize("cols", [1152, 4096, 1001])
+@pytest.mark.parametrize("eps", [0.0, 1e-37])
+def test_small_rows_and_eps(pkg, dev, cols, eps):
+    """Rows down to 2^-110 with little or no eps: their squares have no place in 32 bits."""
+    f = torch.tensor([1.0, 2.0 ** -40, 2.0 ** -66, 2.0 ** -75, 2.0 ** -110])[:, None]
+    x, b = (normal((5, cols), 1).float() * f).to(torch.bfloat16), (normal((5, cols), 2).float() * f).to(torch.bfloat16)
+    pre, post = normal((cols,), 3, 0.1), normal((cols,), 4, 0.1)
+    y, h = pkg.residual_norm(x.to(dev), b.to(dev), pre.to(dev), post_w=post.to(dev), eps=eps)
+    ry, rh, ty, th = reference(x, b, pre, post, None, None, None, 1.0, eps)
+    between(y, ry, ty + 1e-45, "y")
+    between(h, rh, th + 1e-45, "h")
+    y, h = pkg.residual_norm(x.to(dev), b.to(dev), pre.to(dev), eps=eps)
+    ry, rh, ty, th = reference(x, b, pre, None, None, None, None, 1.0, eps)
+    between(y, ry, ty + 1e-45, "y, no inner norm")
+    between(h, rh, th + 1e-45, "h, no inner norm")
