@@ -369,7 +369,7 @@ bool residual_norm(const void* x, int64_t ldx, const void* branch, int64_t ldb, 
         kern = cols <= 4096 ? residual_norm_vec_kernel<128, 4, true, false> : cols <= 8192 ? O1_RN(256, 4, false) : O1_RN(512, 4, false);
     }
 #undef O1_RN
-    return launch_ok(launch_chained(kern, dim3(warps ? (rows + 3) / 4 : rows), dim3(threads), 0, st, 1, 1, a), "residual_norm");
+    return launch_ok(launch_chained(kern, dim3(warps ? ((unsigned)rows + 3) / 4 : rows), dim3(threads), 0, st, 1, 1, a), "residual_norm");
 }
 
 // ------------------------------------------------------------------ materialising attention (small / odd shapes)

@@ -159,3 +159,13 @@ def test_small_rows_and_eps(pkg, dev, cols, eps):
     ry, rh, ty, th = reference(x, b, pre, None, None, None, None, 1.0, eps)
     between(y, ry, ty + 1e-45, "y, no inner norm")
     between(h, rh, th + 1e-45, "h, no inner norm")
+
+
+@gpu
+def test_the_most_rows(pkg, dev):
+    """As many rows as an int counts, four to a block (34 GB, in place)."""
+    rows = 2 ** 31 - 1
+    x = torch.zeros(rows, 8, dtype=torch.bfloat16, device=dev)
+    x[-1], x[0] = 1.0, 2.0
+    _, h = pkg.residual_norm(x, x, None, y=x)
+    assert (x[-1] == 2.0).all() and (x[0] == 4.0).all() and h is None
