@@ -165,6 +165,7 @@ PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     auto on_gpu = [&](const at::Tensor& t) { return t.is_cuda() && t.device().index() == h->device; };
     if (pages->scalar_type() != at::kInt || pages->dim() != 2 || pages->size(0) != batch || !on_gpu(*pages)) return fail(who, "pages int32 [batch, width] on the cache's GPU wanted");
     const int64_t width = pages->size(1), ldp = batch > 1 ? pages->stride(0) : width;
+    if (width > INT32_MAX) return fail(who, "a table of too many pages");
     if (width > 1 && pages->stride(1) != 1) return fail(who, "the pages of a sequence must lie side by side");
     if (lens->scalar_type() != at::kInt || lens->dim() != 1 || lens->size(0) != batch || !lens->is_contiguous() || !on_gpu(*lens)) return fail(who, "lens int32 [batch] on the cache's GPU wanted");
     if ((a[5] == Py_None) != (a[6] == Py_None)) return fail(who, "k and v [batch, kv_heads, 128], both or neither");

@@ -734,3 +734,13 @@ def test_workspaces_of_captures_go_with_their_graphs(pkg, dev):
     # (a destroyed graph is reported by a thread of the runtime's, so one or two may be there)
     assert sizes[-1] - sizes[3] < 3 * pkg.lib.o1_kv_attention_workspace_bytes(8, 1), sizes
     assert torch.equal(out, want)
+
+
+@gpu
+def test_a_table_wider_than_an_int_is_refused(pkg, dev):
+    """Its width was cut to 32 bits (17 GB, not touched)."""
+    c = pkg.KvCache(4, 16, "int8", 2, dev)
+    q, lens = normal((1, 4, D), gen(0)).to(dev), torch.ones(1, dtype=torch.int32, device=dev)
+    with pytest.raises(pkg.O1Error, match="pages"):
+        c.attend(q, torch.empty(1, 2 ** 32 + 1, dtype=torch.int32, device=dev), lens)
+    assert pkg.lib.o1_device_error() == 0
