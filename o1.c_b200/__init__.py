@@ -345,4 +345,11 @@ def use_torch_stream():
 from .model import (  # noqa: E402
     Weights, GgufWeights, Engine, seq_t2i, seq_ref, dev_sigmas, write_gguf, gguf_tensor_name, weight_seed, SLOT_NAMES, GLOBAL_NAMES, tensor_shape,
 )
-from .kvcache import KvCache, Decoder, residual_norm  # noqa: E402
+
+
+def __getattr__(name):
+    # (with their first use: they need _binding.so, the rest of the package does not)
+    if name in ("KvCache", "Decoder", "residual_norm"):
+        from . import kvcache
+        return globals().setdefault(name, getattr(kvcache, name))
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

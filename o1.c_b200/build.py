@@ -1,9 +1,10 @@
 """Builds libo1b200.so (the CUDA kernels + C ABI) in-tree with nvcc for sm_100a, and _binding.so (the Python calls
-whose host time counts, on torch tensors) with g++.
+whose host time counts, on torch tensors) with g++ where there is a torch with CUDA: the library itself needs none.
 
 Run as a script or call build(); nothing is JIT-compiled at import time, so
 the built library travels with the source tree.
 """
+import glob
 import os
 import shutil
 import subprocess
@@ -22,14 +23,23 @@ NVCC_FLAGS = [
 BINDING, BINDING_SRC = os.path.join(HERE, "_binding.so"), os.path.join(CSRC, "binding.cpp")
 
 
-def _binding_command():
+def _binding():
+    """(object file, which names the torch it is for; commands that compile and link) of the native module, or (None, why there is none)."""
     import sysconfig
-    import torch
+    try:
+        import torch
+    except ImportError:
+        return None, "there is no torch"
     root = os.path.dirname(torch.__file__)
-    return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-            + [f"-I{d}" for d in (sysconfig.get_paths()["include"], os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
-                                  os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include"))]
-            + [BINDING_SRC, "-o", BINDING, f"-L{os.path.join(root, 'lib')}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10_cuda", "-lc10"])
+    if not os.path.exists(os.path.join(root, "lib", "libtorch_cuda.so")):
+        return None, f"torch {torch.__version__} is without CUDA"
+    obj = os.path.join(CSRC, f"binding.{torch.__version__}.o")
+    compile_ = (["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+                + [f"-I{d}" for d in (sysconfig.get_paths()["include"], os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                                      os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include"))]
+                + ["-c", BINDING_SRC, "-o", obj])
+    link = ["g++", "-shared", obj, "-o", BINDING, f"-L{os.path.join(root, 'lib')}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10_cuda", "-lc10"]
+    return obj, (compile_, link)
 
 
 def _nvcc():
@@ -61,8 +71,13 @@ def build(verbose=False, force=False):
         if force or _stale(o, [s] + headers):
             cmd = [nvcc] + NVCC_FLAGS + extra + (["-Xptxas", "-v"] if verbose else []) + ["-c", s, "-o", o]
             procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
-    if force or _stale(BINDING, [BINDING_SRC, headers[-1]]):
-        procs.append(("binding.cpp", subprocess.Popen(_binding_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    binding, how = _binding()
+    if binding is None:
+        sys.stderr.write(f"{os.path.basename(BINDING)} is not built ({how}): KvCache, Decoder and residual_norm are not to be had from Python\n")
+    elif force or _stale(binding, [BINDING_SRC, headers[-1]]):
+        for old in glob.glob(os.path.join(CSRC, "binding.*.o")):       # of another torch
+            os.remove(old)
+        procs.append(("binding.cpp", subprocess.Popen(how[0], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     failed = False
     for src, p in procs:
         out, _ = p.communicate()
@@ -76,6 +91,8 @@ def build(verbose=False, force=False):
     if force or procs or _stale(LIB, objs):
         cmd = [nvcc, "-shared", "-o", LIB] + objs + ["-Xlinker", "-Bsymbolic", "-lcudart"]
         subprocess.run(cmd, check=True)
+    if binding is not None and (force or _stale(BINDING, [binding])):
+        subprocess.run(how[1], check=True)
     return LIB
 
 

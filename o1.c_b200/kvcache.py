@@ -17,6 +17,10 @@ if not os.path.exists(_BINDING):
     raise ImportError(f"{_BINDING} is missing: build it with `python o1.c_b200/build.py`. There is no fallback path.")
 
 from . import _binding  # noqa: E402
+
+if _binding.torch_version != torch.__version__.split("+")[0]:
+    raise ImportError(f"{_BINDING} is of torch {_binding.torch_version}, this is {torch.__version__}: build it with `python o1.c_b200/build.py`")
+
 from . import HEAD_DIM, KV_HEADS, KvCacheC, O1Error, check, lib, ptr  # noqa: E402
 
 KINDS = {"bf16": (0, torch.bfloat16), "fp8": (1, torch.float8_e4m3fn), "int8": (2, torch.int8)}
