@@ -5,6 +5,7 @@ this module only binds it with ctypes and supplies device memory, streams and
 process-group plumbing through PyTorch.  There is no CPU or PyTorch fallback:
 importing this module without the built library raises.
 """
+import contextlib
 import ctypes as C
 import os
 
@@ -340,6 +341,16 @@ def use_torch_stream():
     """Make the library enqueue on torch's current CUDA stream."""
     import torch
     lib.o1_set_stream(C.c_void_p(torch.cuda.current_stream().cuda_stream))
+
+
+def _on_library(device):
+    """The library's current stream as torch's, for what torch does on a call's behalf."""
+    import torch
+    s = lib.o1_get_stream() or 0
+    if torch.device(device).type != "cuda" or torch.cuda.current_stream(device).cuda_stream == s:
+        return contextlib.nullcontext()
+    # (an ExternalStream of 0 would be a new stream, not the default one)
+    return torch.cuda.stream(torch.cuda.ExternalStream(s, device) if s else torch.cuda.default_stream(device))
 
 
 from .model import (  # noqa: E402

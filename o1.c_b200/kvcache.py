@@ -6,7 +6,6 @@ do not fit raise O1Error; a slot, page or length that does not fit is found on t
 Where torch's current stream is another one, what these calls make (caches, results, tables) is made, filled and freed in the order of the library's;
 ordering that, and their inputs, with torch's own work is the caller's.
 """
-import contextlib
 import ctypes as C
 import os
 
@@ -21,7 +20,7 @@ from . import _binding  # noqa: E402
 if _binding.torch_version != torch.__version__.split("+")[0]:
     raise ImportError(f"{_BINDING} is of torch {_binding.torch_version}, this is {torch.__version__}: build it with `python o1.c_b200/build.py`")
 
-from . import HEAD_DIM, KV_HEADS, KvCacheC, O1Error, check, lib, ptr  # noqa: E402
+from . import HEAD_DIM, KV_HEADS, KvCacheC, O1Error, _on_library, check, lib, ptr  # noqa: E402
 
 KINDS = {"bf16": (0, torch.bfloat16), "fp8": (1, torch.float8_e4m3fn), "int8": (2, torch.int8)}
 _BY_DTYPE = {d: n for n, d in KINDS.values()}
@@ -34,15 +33,6 @@ _binding.setup(*(C.cast(f, C.c_void_p).value for f in (lib.o1_kv_write, lib.o1_k
 def _need(ok, what):
     if not ok:
         raise O1Error(what)
-
-
-def _on_library(device):
-    """The library's current stream as torch's, for what torch does on a call's behalf."""
-    s = _stream() or 0
-    if torch.device(device).type != "cuda" or torch.cuda.current_stream(device).cuda_stream == s:
-        return contextlib.nullcontext()
-    # (an ExternalStream of 0 would be a new stream, not the default one)
-    return torch.cuda.stream(torch.cuda.ExternalStream(s, device) if s else torch.cuda.default_stream(device))
 
 
 def _zeros(n, device):

@@ -12,7 +12,7 @@ import os
 import torch
 
 from . import (  # noqa: F401  (re-exported names)
-    lib, ptr, check, check_cuda_errbuf, BlockBinding, BlockInternals, ForwardBinding,
+    _on_library, lib, ptr, check, check_cuda_errbuf, BlockBinding, BlockInternals, ForwardBinding,
     ForwardWorkspace, ForwardDiagnostics, LoraEntry, HIDDEN, HEADS, KV_HEADS, HEAD_DIM, FF, PATCH_DIM,
     XE_MID, VOCAB, TMS_ID, N_LAYERS,
 )
@@ -219,13 +219,15 @@ class Engine:
     def block(self, x, pos, layer, internals=False, mod6=None):
         """hd_decoder_block on x [S, hidden] bf16; returns out (and the five internals).  With mod6
         ([6*hidden] bf16: shift/scale/gate for the attention and the MLP branch) the adaLN variant runs."""
-        out = torch.empty_like(x)
+        with _on_library(self.device):
+            out = torch.empty_like(x)
         scratch = self.ws_region("block_scratch", self.block_scratch_bytes)
         ints, bufs = None, {}
         if internals:
             ints = BlockInternals()
             for n in ("ln0", "attn_hidden", "attn_resid", "post_ln", "mlp_out"):
-                bufs[n] = torch.empty_like(x)
+                with _on_library(self.device):
+                    bufs[n] = torch.empty_like(x)
                 setattr(ints, n, bufs[n].data_ptr())
         bb = self.w.block_binding(layer)
         fn = lib.hd_decoder_block if mod6 is None else lib.o1_decoder_block_adaln
@@ -244,9 +246,10 @@ class Engine:
     def forward(self, ids, pos, vinputs, t, out=None, diag_names=(), visual=None):
         """hd_forward; t is the model timestep (1 - sigma). Returns x_pred [S, 3072] bf16.
         visual = (mask uint8 [S], image_embeds [V,H], (deepstack0, 1, 2)) device tensors, or None."""
-        if out is None:
-            out = torch.empty(self.S, PATCH_DIM, dtype=torch.bfloat16, device=self.device)
-        self.timestep.fill_(float(t))
+        with _on_library(self.device):
+            if out is None:
+                out = torch.empty(self.S, PATCH_DIM, dtype=torch.bfloat16, device=self.device)
+            self.timestep.fill_(float(t))
         diag, bufs = None, {}
         if diag_names:
             diag = ForwardDiagnostics()
@@ -255,7 +258,8 @@ class Engine:
                 rows = {"after_embedding": self.T, "after_timestep_conditioning": self.T,
                         "after_target_embedding": self.I}.get(n, self.S)
                 cols = PATCH_DIM if n == "after_final_head" else d["hidden"]
-                bufs[n] = torch.empty(rows, cols, dtype=torch.bfloat16, device=self.device)
+                with _on_library(self.device):
+                    bufs[n] = torch.empty(rows, cols, dtype=torch.bfloat16, device=self.device)
                 setattr(diag, n, bufs[n].data_ptr())
         d = self.w.dims
         vc = None
@@ -273,9 +277,10 @@ class Engine:
 
     def denoise_step_cfg(self, ids_c, ids_u, pos, z, sigma, sigma_next, guidance, z_next=None):
         """One CFG flow-match step on device-resident latents z [I, 3072] bf16."""
-        if z_next is None:
-            z_next = torch.empty_like(z)
-        self.timestep.fill_(1.0 - float(sigma))
+        with _on_library(self.device):
+            if z_next is None:
+                z_next = torch.empty_like(z)
+            self.timestep.fill_(1.0 - float(sigma))
         rc = lib.o1_denoise_step_cfg(C.byref(self.w.binding), C.byref(self.ws), ptr(ids_c), ptr(ids_u),
                                      self.T, ptr(pos), self.ar_len, ptr(z), self.I, ptr(self.timestep),
                                      float(sigma), float(sigma_next), float(guidance), ptr(self.xp),
@@ -286,7 +291,8 @@ class Engine:
     def denoise_step_cfg_ref(self, ids_c, ids_u, pos, vin, target_tokens, sigma, sigma_next, guidance, z_next):
         """CFG step of a reference / edit sequence: vin [I, 3072] = target latent rows then the static
         reference rows; only the first target_tokens rows are stepped into z_next."""
-        self.timestep.fill_(1.0 - float(sigma))
+        with _on_library(self.device):
+            self.timestep.fill_(1.0 - float(sigma))
         rc = lib.o1_denoise_step_cfg_ref(C.byref(self.w.binding), C.byref(self.ws), ptr(ids_c), ptr(ids_u), self.T,
                                          ptr(pos), self.ar_len, ptr(vin), self.I, target_tokens, None,
                                          ptr(self.timestep), float(sigma), float(sigma_next), float(guidance),
@@ -298,9 +304,10 @@ class Engine:
         """CFG step whose branches have their own sequences: cond / uncond = (ids [T_b], pos [3, T_b + I],
         ar_len) with T_b <= the text length this engine was sized for."""
         from . import CfgBranch
-        if z_next is None:
-            z_next = torch.empty_like(z)
-        self.timestep.fill_(1.0 - float(sigma))
+        with _on_library(self.device):
+            if z_next is None:
+                z_next = torch.empty_like(z)
+            self.timestep.fill_(1.0 - float(sigma))
         br = []
         for ids, pos, ar in (cond, uncond):
             assert ids.numel() <= self.T

@@ -10,7 +10,7 @@ import ctypes as C
 
 import torch
 
-from . import lib, ptr, check, BlockBinding, ForwardBinding, PATCH_DIM, TMS_ID
+from . import _on_library, lib, ptr, check, BlockBinding, ForwardBinding, PATCH_DIM, TMS_ID
 
 c_int, c_void_p = C.c_int, C.c_void_p
 
@@ -215,7 +215,8 @@ class EngineSP:
     # emulated ranks; `forward()` runs them back to back for a real rank
     def stages(self, ids, pos, vin_local, t, out_local):
         ws, w = C.byref(self.ws), self.w
-        self.timestep.fill_(float(t))
+        with _on_library(self.w.device):
+            self.timestep.fill_(float(t))
         if self.direct:
             yield from self._stages_direct(ids, pos, vin_local, out_local)
             return
@@ -269,7 +270,8 @@ class EngineSP:
         """The same forward driven by ONE library call (o1_sp_forward) instead of the stage-by-stage loop."""
         if out_local is None:
             out_local = torch.empty(self.rows, PATCH_DIM, dtype=torch.bfloat16, device=self.w.device)
-        self.timestep.fill_(float(t))
+        with _on_library(self.w.device):
+            self.timestep.fill_(float(t))
         c = self.ctx()
         c.epoch = max(c.epoch, self.epoch)          # one monotonic epoch sequence whichever path ran before
         check(lib.o1_sp_forward(C.byref(self.w.binding), C.byref(c), ptr(ids), ptr(pos), ptr(vin_local),

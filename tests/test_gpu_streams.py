@@ -111,3 +111,28 @@ def test_what_is_filled_for_the_default_stream(pkg, dev):
                 assert torch.cuda.current_stream().cuda_stream == s.cuda_stream
     finally:
         pkg.use_torch_stream()
+
+
+@gpu
+def test_an_engine_on_another_stream(pkg, dev):
+    """The timestep of a forward and of a guided step is set where they read it."""
+    T, I = 19, 48
+    w = pkg.Weights(n_layers=1, seed=3, device=dev)
+    eng = pkg.Engine(w, T, I)
+    pos, _ = pkg.seq_t2i(T, 6, 8)
+    pos, ids = pos.to(dev), ids_of(T, 1).to(dev)
+    ids[-1] = 151673      # the row of the timestep
+    z = normal((I, 3072), gen(1)).to(dev)
+
+    def run():
+        return eng.forward(ids, pos, z, 0.3), eng.denoise_step_cfg(ids, ids, pos, z, 0.7, 0.6, 2.0), \
+            eng.denoise_step_cfg_branches((ids, pos, T - 1), (ids, pos, T - 1), z, 0.5, 0.4, 2.0)
+    want = [t.clone() for t in run()]
+    assert not torch.equal(eng.forward(ids, pos, z, 0.9), want[0])
+    for i in range(3):
+        eng.forward(ids, pos, z, 0.9)
+        with Apart(pkg):
+            old = [torch.full_like(t, 9.0) for t in want for _ in range(4)]
+            del old
+            got = run()[i]
+        assert torch.equal(got, want[i])
