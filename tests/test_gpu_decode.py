@@ -298,3 +298,52 @@ def test_failed_calls_change_nothing(pkg, dev, weights, monkeypatch):
     new = ids_of(1, 4).to(dev)
     assert torch.equal(dec.step([a], new), same.step([b], new))
     assert dec.rows(a, 0)[0].size(0) == 21
+
+
+class Kept:
+    """Weights whose tensors are brought to the host, in 64 bits, once."""
+
+    def __init__(self, w):
+        self.w, self.dims, self.n_layers, self.got = w, w.dims, w.n_layers, {}
+
+    def tensor(self, layer, name):
+        if (layer, name) not in self.got:
+            self.got[layer, name] = self.w.tensor(layer, name).cpu().double()
+        return self.got[layer, name]
+
+
+@gpu
+@pytest.mark.parametrize("kind,tol", [("bf16", 1e-2), ("fp8", 5e-2), ("int8", 1e-2)])
+@pytest.mark.parametrize("size,count", [("small", 33), ("small", 140), ("full", 12)])
+def test_steps_of_many_rows(pkg, dev, models, kind, tol, size, count):
+    """More rows than the few that a step's products take as eight, and a block of the framework's own size: 32 / 8 heads, width 4096, 12288 in the middle."""
+    w = models[1] if size == "small" else pkg.Weights(n_layers=1, seed=6, weight_set="B", device="cuda:0")
+    kept, steps = Kept(w), 2
+    lens = [1 + (29 * i) % 71 for i in range(count)]
+    seqs = [ids_of(n + steps, 100 * n + i) for i, n in enumerate(lens)]
+    dec = pkg.Decoder(w, count, max(lens) + steps, kind, 16)
+    names = [dec.prompt(s[:n].to(dev))[0] for s, n in zip(seqs, lens)]
+    some = range(0, count, max(1, count // 12))
+    wants = {i: reference(kept, seqs[i], lens[i], kind)[0] for i in some}
+    for at in range(steps):
+        rows = dec.step(names, torch.tensor([int(s[n + at]) for s, n in zip(seqs, lens)]).to(dev))
+        near(rows[list(some)], torch.stack([wants[i][lens[i] + at] for i in some]), tol)
+    assert pkg.lib.o1_device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("layers", [1, 3])
+def test_steps_beside_the_prompt_pass(pkg, dev, models, layers):
+    """Rows that were steps, beside the same rows in one prompt pass: each is within the tolerance of the reference, so they are within twice that of one another."""
+    dec = pkg.Decoder(models[layers], 4, 400, "bf16", 32)
+    for n, steps in ((1, 6), (30, 5), (300, 9)):
+        ids = ids_of(n + steps, n).to(dev)
+        name, _ = dec.prompt(ids[:n])
+        got = torch.cat([dec.step([name], ids[n + i:n + i + 1]) for i in range(steps)])
+        whole, rows = dec.prompt(ids)
+        near(got, rows[n:].cpu(), 2e-2 * layers)
+        for layer in range(layers):
+            for a, b in zip(dec.rows(name, layer), dec.rows(whole, layer)):
+                near(a, b.cpu(), 2e-2 * (layer + 1))
+        dec.close(name)
+        dec.close(whole)

@@ -744,3 +744,58 @@ def test_a_table_wider_than_an_int_is_refused(pkg, dev):
     with pytest.raises(pkg.O1Error, match="pages"):
         c.attend(q, torch.empty(1, 2 ** 32 + 1, dtype=torch.int32, device=dev), lens)
     assert pkg.lib.o1_device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "int8"])
+@pytest.mark.parametrize("rows,heads,page,off,pad", [(19201, 1, 16, 0, 0), (6403, 3, 48, 0, 8), (2405, 8, 64, 0, 0), (2401, 8, 16, 1, 3), (1205, 16, 32, 8, 8), (19999, 1, 128, 3, 1)])
+def test_many_rows_written_and_read_back(pkg, dev, kind, rows, heads, page, off, pad):
+    """Eight heads of rows to a warp: a last warp that is not full, heads that do not divide eight, rows inside wider ones at any address, rows left out, rows of zeros,
+    with a NaN and of 2^120."""
+    g = torch.Generator(device=dev).manual_seed(rows)
+    pages = -(-rows // page) + 3
+    cache = pkg.KvCache(pages, page, kind, heads, dev)
+    pitch = 2 * heads * D + pad
+    wide = torch.empty(rows * pitch + off, dtype=torch.bfloat16, device=dev).normal_(0, 1, generator=g)
+    w = wide[off:].view(rows, pitch)
+    k, v = (w[:, i * heads * D:(i + 1) * heads * D].unflatten(1, (heads, D)) for i in (0, 1))
+    k[5], v[7], v[9] = 0.0, 2.0 ** 120, -0.0
+    k[11, heads - 1, 5], v[rows - 1, 0, 127] = math.nan, math.inf
+    slots = torch.randperm(pages * page, generator=g, device=dev)[:rows]
+    left_out = torch.zeros(rows, dtype=torch.bool, device=dev)
+    left_out[[3, 100, rows - 2]] = True
+    asked = torch.where(left_out, -1, slots)
+    cache.write(k, v, asked)
+    page_at, at = slots // page, slots % page
+    want = []
+    for x, store, scales in ((k, cache.k, cache.k_scale), (v, cache.v, cache.v_scale)):
+        codes, scale = (None if t is None else t.to(dev) for t in quantised(x.cpu(), kind))
+        held = store.view(torch.uint8 if kind != "bf16" else torch.int16)[page_at, :, at]
+        assert torch.equal(held[~left_out], codes.view(held.dtype)[~left_out])
+        assert (held[left_out] == 0).all()
+        if kind != "bf16":
+            s = scales[page_at, :, at]
+            assert torch.equal(torch.isnan(s)[~left_out], torch.isnan(scale)[~left_out]) and torch.equal(s.nan_to_num(0)[~left_out], scale.nan_to_num(0)[~left_out])
+            assert (s[left_out] == 0).all()
+        want.append(torch.where(left_out[:, None, None], 0.0, value(codes, scale).to(torch.bfloat16) if kind != "bf16" else x.clone()))
+    wide.fill_(7.0)
+    cache.read(asked, out=(k, v))
+    for name, y, x in (("k", k, want[0]), ("v", v, want[1])):
+        assert torch.equal(torch.isnan(y), torch.isnan(x)) and torch.equal(y.nan_to_num(7), x.nan_to_num(7)), name
+    assert (w[:, 2 * heads * D:] == 7.0).all() and (wide[:off] == 7.0).all()
+    assert pkg.lib.o1_device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("lens,kv_heads,group", [([0, 1, 17, 65, 300], 8, 4), ([4097], 2, 8), ([30011], 1, 8), ([700] * 40, 1, 16), ([33] * 300, 4, 3), ([9001, 1, 0, 12000, 3], 2, 24)])
+def test_probabilities_keep_sixteen_bits(pkg, dev, kind, lens, kv_heads, group):
+    """Codes are exact, and a probability times v's scale is multiplied as two parts of bf16: 2^-17 of itself over fp8 and int8 rows too, so the values that those
+    stand for have the bound of bf16 rows."""
+    c = Case(pkg, dev, kind, lens, kv_heads, 32, seed=len(lens))
+    c.fill()
+    q = normal((len(lens), kv_heads * group, D), gen(11), 1.5)
+    out, lse = c.cache.attend(q.to(dev), c.dtable, c.dlens, lse=True)
+    c.k, c.v = ([value(*quantised(x, kind)) for x in rows] for rows in (c.k, c.v))
+    c.kind = "bf16"
+    c.check(q, out, lse, what=kind)

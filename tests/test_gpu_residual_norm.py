@@ -169,3 +169,23 @@ def test_the_most_rows(pkg, dev):
     x[-1], x[0] = 1.0, 2.0
     _, h = pkg.residual_norm(x, x, None, y=x)
     assert (x[-1] == 2.0).all() and (x[0] == 4.0).all() and h is None
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols,post,groups", [(1100, 4096, 0, 1), (5003, 4096, 1, 1), (2600, 8192, 1, 2), (600, 8192, 0, 1), (701, 12288, 1, 1), (402, 12288, 0, 2), (1501, 2048, 1, 1),
+                                                   (2100, 2048, 0, 3), (10003, 2048, 1, 1), (9001, 1152, 1, 1), (970, 4096, 0, 1), (4800, 4096, 1, 1), (2400, 8192, 1, 1), (400, 8192, 0, 1),
+                                                   (640, 12288, 1, 2), (310, 12288, 0, 1)])
+def test_many_rows(pkg, dev, rows, cols, post, groups):
+    """Sizes beyond which a row has fewer registers and vectors are asked for where they are used, on both sides of each."""
+    g = torch.Generator(device=dev).manual_seed(1)
+    n = lambda *s: torch.empty(s, dtype=torch.bfloat16, device=dev).normal_(0, 1, generator=g)  # noqa: E731
+    x, b, pre, pw = n(rows, cols), n(rows, cols), n(cols), n(cols) if post else None
+    gate, scale, shift = n(groups, cols), n(groups, cols), n(groups, cols)
+    y, h = pkg.residual_norm(x, b, pre, post_w=pw, gate=gate, scale=scale, shift=shift, alpha=0.4)
+    ry, rh, ty, th = reference(x, b, pre, pw, gate, scale, shift, 0.4, 1e-6)
+    for got, ref, tol, name in ((y, ry, ty, "y"), (h, rh, th, "h")):
+        got = got.double()
+        ok = (got >= (ref - tol).to(torch.bfloat16).double()) & (got <= (ref + tol).to(torch.bfloat16).double())
+        assert ok.all(), name
+    y2, none = pkg.residual_norm(x, b, None, post_w=pw, gate=gate, alpha=0.4)
+    assert none is None and torch.equal(y, y2)
