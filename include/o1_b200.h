@@ -765,7 +765,7 @@ int o1_parallel_layout(int world, int rank, int *image, int *branch, int *sp_ran
  *
  * A cache: k and v [pages][kv_heads][page_size][128], 16-byte aligned, page_size a multiple of 16.  O1_KV_BF16 stores rows as they are;
  * O1_KV_FP8 (e4m3) and O1_KV_INT8 as codes of a byte with one fp32 scale for each token and head, k_scale and v_scale
- * [pages][kv_heads][page_size] (16-byte aligned): scale = max|x| / 448 or / 127, code = x / scale to the nearest, ties to even.  A row with an Inf
+ * [pages][kv_heads][page_size] (16-byte aligned): scale = max|x| / 448 or / 127, code = x * (448 or 127 / max|x|) to the nearest, ties to even, in fp32 (max|x| at least 2^-100).  A row with an Inf
  * or NaN gets a NaN scale and reads as NaN.  A token's slot is page * page_size + its place in the page.
  * Codes are those that o1_kv_write makes: in particular no e4m3 NaN (0x7F, 0xFF), whose row has its NaN in the scale.
  * A slot or page outside the cache, or a length outside its table, found on the device: nothing outside the cache is read or
@@ -788,7 +788,7 @@ hd_status o1_kv_read(const o1_kv_cache *cache, void *k, int64_t ldk, void *v, in
  * columns, heads a multiple of kv_heads (query head j reads kv head j / (heads / kv_heads)); lse (may be NULL) [batch, heads] fp32:
  * log of the sum of exponentials, to join the result with that of other keys.  lens[b] == 0: out row 0, lse -inf.
  * k_new / v_new (both or neither): each sequence's row at position lens[b] - 1, stored into the cache (as by o1_kv_write) and
- * attended to by the same call.  workspace: o1_kv_attention_workspace_bytes(heads, kv_heads) bytes, 16-byte aligned, zero-filled once before its first use and
+ * attended to by the same call; no other sequence of the call has that slot among its rows.  workspace: o1_kv_attention_workspace_bytes(heads, kv_heads) bytes, 16-byte aligned, zero-filled once before its first use and
  * left to these calls from then on; calls that may overlap on the GPU each need their own.  The result is the same
  * bits from call to call with the same lengths and width; beside other sequences a sequence's differs by the order of its fp32 sums.  Values of v up to 2^90 in magnitude (the sums are 2^20 times larger and in fp32); at most 2^31 - 1 rows (pages *
  * kv_heads * page_size) in the cache. */
@@ -809,8 +809,8 @@ hd_status o1_residual_norm(const void *x, int64_t ldx, const void *branch, int64
 /* The decoder blocks on cached rows: caches [n_layers] (one of each block, with the same pages and page_size, so that one page table serves
  * all), ids int64 on the device, pos_f32 [3, rows] as hd_forward's, out [rows, hidden] bf16: the rows behind the final norm.
  * o1_prompt_rows: all rows of one sequence, causal, their keys and values into slots[r] of each cache.  o1_decode_step: one new row of each of `batch` sequences, which
- * becomes row lens[b] - 1 of sequence b.  scratch: o1_decode_scratch_bytes(rows, ...) bytes, its first o1_kv_attention_workspace_bytes zero-filled once (zero all
- * of it); one for each stream.  The residual stream's norms are of its unrounded sums (o1_residual_norm), so the rows agree with hd_decoder_block's within rounding.  A row is a
+ * becomes row lens[b] - 1 of sequence b.  scratch: o1_decode_scratch_bytes(rows, ...) bytes, zero-filled once; one for each
+ * stream.  The residual stream's norms are of its unrounded sums (o1_residual_norm), so the rows agree with hd_decoder_block's within rounding.  A row is a
  * function of its own sequence within rounding too: the same step gives the same bits, but how a sequence's cached rows are shared out, and with it the order of fp32
  * sums, follows from the lengths of all sequences of the step. */
 int64_t o1_decode_scratch_bytes(int64_t rows, int heads, int kv_heads, int hidden, int ff_hidden, int head_dim);

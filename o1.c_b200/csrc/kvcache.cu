@@ -236,9 +236,10 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
 // out = sum_t p_t v_t / sum_t p_t, p_t = exp(scale q . k_t - max): one pass over the keys with a running maximum and sum (in base 2).  HBM bound: every cached
 // value is read once and used by the G = heads / kv_heads queries that share it, 2 G multiply-adds for its one or two bytes, so all that counts is that
 // enough bytes are on their way at all times, on all SMs, whatever the lengths are.  Measured: 582 MB of fp8 rows (96 sequences of 300 to 5400 tokens, 8 kv heads) in
-// 97 us, 6.0 TB/s, 92 % of a copy's rate (107 without a pause, when 1000 W allow 1620 MHz); 211 MB of int8 (one sequence of 100003) in 46 us, 4.6 TB/s; 100 MB of bf16 (24 sequences of 1 to 2100) in 25 us.
+// 98 us of the GPU, 5.9 TB/s, 91 % of a copy's rate (101 to 109 through the Python call; without a pause 1000 W allow 1620 MHz); 211 MB of int8 (one sequence of 100003) in
+// 45.5 us, 4.6 TB/s; 100 MB of bf16 (24 sequences of 1 to 2100) in 25.
 // With few bytes the chain of steps counts: 2.3 us until the first loads are asked for (lengths, their sums, parts, pages), 2 for them, 1.3 for the
-// warps' join, 3 for that of the teams: 85 tokens of one sequence take 5.8 us, 600 take 8.5.
+// warps' join, 3 for that of the teams: 85 tokens of one sequence take 6.0 us, 600 take 8.5.
 //
 //  * The work is one stream of chunks (16 tokens, 32 of a quantised cache: 8 KB of keys and values) over sequences, kv heads and length.  A block is one SM's; its
 //    consumer warps form teams of four, and every team takes a contiguous part of the stream, of equal cost.  How long that is follows from the lengths, which only the
@@ -258,8 +259,7 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
 //    are many, each goes to one warp, which needs no join (200 sequences of 30 rows of fp8, 8 kv heads: 20 us, now 7.7).
 //  * Rounding: scores and sums in fp32.  Probabilities (times v's scale) enter the second product as two parts of bf16, value and rest, 16 bits of significand; codes
 //    of a byte are exact in f16 and bf16.  Keys' codes go through f16, which takes fewer instructions, with queries scaled to f16's top by a power of two for each head (those
-//    below 2^-29 of its largest lose bits);
-//    values' codes through bf16, whose range a probability needs.  The result is rounded once.
+//    below 2^-29 of its largest lose bits); values' codes through bf16, whose range a probability needs.  The result is rounded once.
 // Times below: "batch" 24 sequences of 1 to 2100 rows of bf16, "shared" 32 sequences of 1000 to 3000, 16 query heads on one kv head; us.
 static constexpr int KV_STAGE_BYTES = 8192;            // keys and values of a chunk
 static constexpr int KV_SEQS = 256;                    // sequences of a launch
@@ -277,7 +277,7 @@ static constexpr int KV_KEEP = 16;
 static constexpr int KV_SOLO = 16;                     // chunks of an item that a warp can have for itself (no item of KV_KEEP chunks is cut)
 static_assert(KV_SOLO <= KV_KEEP, "an item of a warp is whole");
 static constexpr int KV_JOIN_BYTES = 8192;             // of a team
-static constexpr int KV_JOIN_STEP = 4;                 // parts that a join has under way (of all a warp's heads; two take 1 us longer for 16 heads, eight spill registers)
+static constexpr int KV_JOIN_STEP = 4;                 // parts that a join has under way (of all a warp's heads; two take 1 us longer for 16 heads; eight spill registers of all types, four of bf16 only)
 static constexpr int ERR_KV_WAIT = 72;                 // a wait of the attention kernel ran out
 static constexpr float KV_LIFT = 20.0f;                // probabilities are relative to 2^-20 of the largest: those that fp32 has no value for are 2^-146 and less of it
 
