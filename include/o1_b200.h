@@ -766,12 +766,15 @@ int o1_parallel_layout(int world, int rank, int *image, int *branch, int *sp_ran
  * A cache: k and v [pages][kv_heads][page_size][128], 16-byte aligned, page_size a multiple of 16.  O1_KV_BF16 stores rows as they are;
  * O1_KV_FP8 (e4m3) and O1_KV_INT8 as codes of a byte with one fp32 scale for each token and head, k_scale and v_scale
  * [pages][kv_heads][page_size] (16-byte aligned): scale = max|x| / 448 or / 127, code = x * (448 or 127 / max|x|) to the nearest, ties to even, in fp32 (max|x| at least 2^-100).  A row with an Inf
- * or NaN gets a NaN scale and reads as NaN.  A token's slot is page * page_size + its place in the page.
+ * or NaN gets a NaN scale and reads as NaN.  O1_KV_UINT4 stores codes of four bits, two to a byte with the first one in the low bits, so k and v are
+ * [pages][kv_heads][page_size][64] bytes, and k_scale and v_scale hold two bf16 values where the other kinds have one fp32, scale and least value: x ~ least + code * scale,
+ * least = min x, scale = bf16((max x - min x) / 15) (0 where the spread is below 2^-100), code = (x - least) * (1 / scale) to the nearest, ties to even, in fp32.  A row with an Inf
+ * or NaN, or a spread beyond fp32, gets NaN for both and reads as NaN.  A token's slot is page * page_size + its place in the page.
  * Codes are those that o1_kv_write makes: in particular no e4m3 NaN (0x7F, 0xFF), whose row has its NaN in the scale.
  * A slot or page outside the cache, or a length outside its table, found on the device: nothing outside the cache is read or
  * written, that row's or sequence's result means nothing (a wrong length: zeros, and no row is appended), other rows and sequences and every other call are
  * as without it, and o1_device_error() gives 70 (slot or page) or 71 (length).  72 is a wait that ran out. */
-enum { O1_KV_BF16 = 0, O1_KV_FP8 = 1, O1_KV_INT8 = 2 };
+enum { O1_KV_BF16 = 0, O1_KV_FP8 = 1, O1_KV_INT8 = 2, O1_KV_UINT4 = 4 };
 typedef struct {
     void *k, *v;
     float *k_scale, *v_scale;      /* NULL with O1_KV_BF16 */
@@ -781,7 +784,7 @@ typedef struct {
  * that are all different; a negative slot: the row is left out), quantised on the way. */
 hd_status o1_kv_write(const o1_kv_cache *cache, const void *k, int64_t ldk, const void *v, int64_t ldv,
                       const int64_t *slots, int rows);
-/* The rows back as bf16(code * scale); zeros for a negative slot. */
+/* The rows back as bf16(code * scale), or bf16(least + code * scale); zeros for a negative slot. */
 hd_status o1_kv_read(const o1_kv_cache *cache, void *k, int64_t ldk, void *v, int64_t ldv, const int64_t *slots, int rows);
 /* Attention of one new row of each sequence over its lens[b] cached rows: token t of sequence b is in page pages[b * ldp + t /
  * page_size] (int32, width columns; entries behind a sequence's last page are not used).  q / out [batch, ldq / ldo] bf16, heads of 128
@@ -797,6 +800,51 @@ hd_status o1_kv_attention(const o1_kv_cache *cache, const void *q, int64_t ldq, 
                           const void *v_new, int64_t ldv, const int32_t *pages, int64_t ldp, int width, const int32_t *lens,
                           void *out, int64_t ldo, float *lse, int batch, int heads, float scale, void *workspace,
                           int64_t workspace_bytes);
+/* Pages handed out on the device: the pages and rows of up to max_seqs (at most 8192) sequences and a list of free pages.  table [max_seqs][width]: a sequence's pages in
+ * order, -1 behind them; lens [max_seqs]: its rows; free_pages [pages]: a stack, its top at state[0] - 1; state [2]: the number of free pages, and a counter that belongs to
+ * these calls (0 between them).  All int32 on the device.  o1_kv_pages_reset makes every page free and every sequence empty.  Calls on the same pages follow one another (one
+ * stream, or ordered); like all entry points they can be captured, and a captured call serves what its arguments hold at each replay.
+ * o1_kv_pages_grow: counts[b] new rows for sequence seqs[b] (NULL: sequence b).  With the requests' rows behind one another, request b's from starts[b] to starts[b + 1] - 1 (starts
+ * [batch + 1]): row r gets slots[r] (for o1_kv_write) and positions[r], its number in the sequence.  slots and positions have room for `rows`; rows behind the last
+ * request get slot -1 and position 0.  lens[b]: the sequence's rows with the new ones; tables (NULL: not wanted) [batch][ldp]: its row of the table (lens and tables as
+ * o1_kv_attention takes them).  Requests are served in order: new pages come from the top of the stack.
+ * o1_kv_pages_shrink: sequence seqs[b] keeps its first keep[b] rows (0: it is closed); pages behind them are free again and come back in the order in which they went.
+ * A request that cannot be served changes nothing of its sequence, its rows get slot -1 and its lens[b] is 0; others are as without it, but for the places of their rows.
+ * o1_device_error() then gives 70 (no such sequence, or one that the call names twice: neither request is served), 71 (a negative count, more rows than width pages
+ * have, than `rows` has room for, or, to keep, than there are) or 73 (not enough free pages: all requests behind it that need pages are refused too). */
+typedef struct {
+    int32_t *table, *lens, *free_pages, *state;
+    int pages, page_size, max_seqs, width;
+} o1_kv_pages;
+hd_status o1_kv_pages_reset(const o1_kv_pages *pages);
+hd_status o1_kv_pages_grow(const o1_kv_pages *pages, const int32_t *seqs, const int32_t *counts, int batch, int64_t *slots,
+                           int32_t *positions, int rows, int32_t *starts, int32_t *lens, int32_t *tables, int64_t ldp);
+hd_status o1_kv_pages_shrink(const o1_kv_pages *pages, const int32_t *seqs, const int32_t *keep, int batch);
+/* Rotary positions of any rows: the first rot_dim values of each head are turned in pairs, (a, b) -> factor * (a cos - b sin, b cos + a sin) with the angle position *
+ * frequency, pairs (i, i + rot_dim / 2) or (2i, 2i + 1); the others stay.  In fp32, rounded once.  Frequencies are kept as turns a position, the fraction of
+ * a turn in 64 bits (turns [rot_dim / 2] on the device, 8-byte aligned), so angles are exact to position * 2^-65 turns plus fp32's rounding at any position.
+ * o1_rope_turns fills them on the host, theta^(-2i / rot_dim), and gives the factor: O1_ROPE_LINEAR divides all by `factor`; O1_ROPE_NTK takes theta * factor^(rot_dim /
+ * (rot_dim - 2)); O1_ROPE_YARN (the YaRN method) divides pairs that turn at most `slow` times within `original` positions, leaves those that turn `fast` times or more, with a
+ * linear ramp between, and multiplies results by 0.1 ln(factor) + 1; O1_ROPE_FACTORS divides pair i by factors[i].  attention > 0: the factor of results instead.
+ * o1_rotary: x [rows, ldx] with `heads` heads of head_dim side by side into y (which may be x), and x2 into y2 likewise in the same launch (heads2 0: not there; queries and
+ * keys as a rule); type O1_ROPE_BF16 or O1_ROPE_FP32; positions [rows] int32, or int64 where wide_positions, negative ones too.  inverse: turned back (also the gradient). */
+enum { O1_ROPE_HALF = 0, O1_ROPE_INTERLEAVED = 1 };
+enum { O1_ROPE_BF16 = 0, O1_ROPE_FP32 = 1 };
+enum { O1_ROPE_PLAIN = 0, O1_ROPE_LINEAR = 1, O1_ROPE_NTK = 2, O1_ROPE_YARN = 3, O1_ROPE_FACTORS = 4 };
+typedef struct {
+    int kind;
+    double factor, original, fast, slow, attention;
+    const double *factors;
+} o1_rope_scaling;
+typedef struct {
+    const uint64_t *turns;
+    float factor;
+    int head_dim, rot_dim, layout;
+} o1_rope;
+hd_status o1_rope_turns(double theta, int rot_dim, const o1_rope_scaling *scaling, uint64_t *turns_host, float *factor);
+hd_status o1_rotary(const o1_rope *rope, const void *positions, int wide_positions, const void *x, int64_t ldx, void *y,
+                    int64_t ldy, int heads, const void *x2, int64_t ldx2, void *y2, int64_t ldy2, int heads2, int rows, int type,
+                    int inverse);
 /* The end of one branch and the beginning of the next as one pass over the residual stream:
  *   y = x + alpha * gate * u,  u = branch, or rmsnorm(branch) * post_w where post_w is given
  *   h = rmsnorm(y) * pre_w, and * (1 + scale) + shift where they are given

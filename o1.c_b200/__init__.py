@@ -108,6 +108,21 @@ class KvCacheC(C.Structure):
         (n, c_int) for n in ("type", "pages", "page_size", "kv_heads", "head_dim")]
 
 
+class KvPagesC(C.Structure):
+    """o1_kv_pages (include/o1_b200.h)."""
+    _fields_ = [(n, c_void_p) for n in ("table", "lens", "free_pages", "state")] + [(n, c_int) for n in ("pages", "page_size", "max_seqs", "width")]
+
+
+class RopeScalingC(C.Structure):
+    """o1_rope_scaling (include/o1_b200.h)."""
+    _fields_ = [("kind", c_int)] + [(n, C.c_double) for n in ("factor", "original", "fast", "slow", "attention")] + [("factors", C.POINTER(C.c_double))]
+
+
+class RopeC(C.Structure):
+    """o1_rope (include/o1_b200.h)."""
+    _fields_ = [("turns", c_void_p), ("factor", c_float), ("head_dim", c_int), ("rot_dim", c_int), ("layout", c_int)]
+
+
 VISION_DEPTH, VISION_HIDDEN, VISION_HEADS, VISION_HEAD_DIM, VISION_FF = 27, 1152, 16, 72, 4304
 VISION_OUT, VISION_PATCH_DIM, VISION_NUM_POS = 4096, 1536, 2304
 # hd_vision_binding (src/model/vision.h:76-109) is 351 consecutive tensor pointers: patch_proj w, b, pos_embed,
@@ -297,6 +312,12 @@ _sig("o1_kv_attention", c_int, C.POINTER(KvCacheC), _P, c_int64, _P, c_int64, _P
 _sig("o1_residual_norm", c_int, _P, c_int64, _P, c_int64, _P, _P, c_float, _P, _P, _P, c_int, _P, c_int64, _P, c_int64,
      c_int, c_int, c_float)
 
+_sig("o1_kv_pages_reset", c_int, C.POINTER(KvPagesC))
+_sig("o1_kv_pages_grow", c_int, C.POINTER(KvPagesC), _P, _P, c_int, _P, _P, c_int, _P, _P, _P, c_int64)
+_sig("o1_kv_pages_shrink", c_int, C.POINTER(KvPagesC), _P, _P, c_int)
+_sig("o1_rope_turns", c_int, C.c_double, c_int, C.POINTER(RopeScalingC), C.POINTER(c_uint64), C.POINTER(c_float))
+_sig("o1_rotary", c_int, C.POINTER(RopeC), _P, c_int, _P, c_int64, _P, c_int64, c_int, _P, c_int64, _P, c_int64, c_int, c_int, c_int, c_int)
+
 _sig("o1_decode_scratch_bytes", c_int64, c_int64, c_int, c_int, c_int, c_int, c_int)
 _sig("o1_prompt_rows", c_int, C.POINTER(ForwardBinding), C.POINTER(KvCacheC), _P, _P, _P, _P, c_int64, _P, c_int, c_int, c_int,
      c_int, c_int, c_int, c_int)
@@ -360,7 +381,7 @@ from .model import (  # noqa: E402
 
 def __getattr__(name):
     # (with their first use: they need _binding.so, the rest of the package does not)
-    if name in ("KvCache", "Decoder", "residual_norm"):
+    if name in ("KvCache", "KvPages", "Rotary", "Decoder", "residual_norm"):
         from . import kvcache
         return globals().setdefault(name, getattr(kvcache, name))
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

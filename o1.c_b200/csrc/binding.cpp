@@ -1,4 +1,4 @@
-// The calls of KvCache and residual_norm from Python: checks of their tensors, results, and the C entry point, without an interpreter's steps between.
+// The calls of KvCache, KvPages, Rotary and residual_norm from Python: checks of their tensors, results, and the C entry point, without an interpreter's steps between.
 // For a few rows such a call is bound by the host: one new row of one sequence took 10.2 us through ctypes, of which the library and the launch are 3.9.
 // The entry points come as addresses from the loaded library (setup); nothing of it is linked here, and the library knows nothing of torch.
 #include <ATen/core/Tensor.h>
@@ -21,6 +21,9 @@ decltype(&o1_kv_attention) f_attend;
 decltype(&o1_residual_norm) f_norm;
 decltype(&o1_get_stream) f_stream;
 decltype(&o1_capture_id) f_capture;
+decltype(&o1_kv_pages_grow) f_grow;
+decltype(&o1_kv_pages_shrink) f_shrink;
+decltype(&o1_rotary) f_rotary;
 PyObject *O1Error, *check;
 
 struct Handle {
@@ -313,11 +316,127 @@ PyObject* py_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// setup(addresses of o1_kv_write, o1_kv_read, o1_kv_attention, o1_residual_norm, o1_get_stream, o1_capture_id; O1Error; check)
+// A contiguous int32 [n] (n < 0: any number); null on error.
+const at::Tensor* ints(PyObject* o, int64_t n, int device, const char* who, const char* name) {
+    const at::Tensor* t = tensor(o, who);
+    if (t && (t->scalar_type() != at::kInt || t->dim() != 1 || !t->is_contiguous() || !t->is_cuda() || t->device().index() != device || (n >= 0 && t->size(0) != n) ||
+              t->size(0) > INT32_MAX)) {
+        PyErr_Format(O1Error, "%s: %s int32 [requests], contiguous, on the pages' GPU wanted", who, name);
+        return nullptr;
+    }
+    return t;
+}
+
+// pages_grow(address of an o1_kv_pages, device index, its table, counts, rows, seqs or None) -> (slots, positions, starts, lens, pages)
+PyObject* py_grow(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    static const char* who = "KvPages.grow";
+    if (!arguments(n, 6)) return nullptr;
+    const auto* pages = (const o1_kv_pages*)PyLong_AsUnsignedLongLong(a[0]);
+    const int device = (int)PyLong_AsLong(a[1]);
+    const at::Tensor *table = tensor(a[2], who), *counts = table ? ints(a[3], -1, device, who, "counts") : nullptr;
+    if (!counts) return nullptr;
+    const int64_t rows = PyLong_AsLongLong(a[4]), batch = counts->size(0);
+    if (PyErr_Occurred()) return nullptr;
+    if (rows < 0 || rows > INT32_MAX) return fail(who, "rows between 0 and 2^31 - 1 wanted");
+    if (batch > pages->max_seqs) return fail(who, "more requests than sequences");
+    const at::Tensor* seqs = nullptr;
+    if (a[5] != Py_None && !(seqs = ints(a[5], batch, device, who, "seqs"))) return nullptr;
+    const OnLibrary on(device);
+    at::Tensor out[5] = {empty_on({rows}, at::kLong, device), empty_on({rows}, at::kInt, device), empty_on({batch + 1}, at::kInt, device), empty_on({batch}, at::kInt, device),
+                         seqs ? empty_on({batch, pages->width}, at::kInt, device) : table->narrow(0, 0, batch)};
+    if (!status(f_grow(pages, seqs ? (const int32_t*)seqs->data_ptr() : nullptr, (const int32_t*)counts->data_ptr(), (int)batch, (int64_t*)out[0].data_ptr(), (int32_t*)out[1].data_ptr(),
+                       (int)rows, (int32_t*)out[2].data_ptr(), (int32_t*)out[3].data_ptr(), seqs ? (int32_t*)out[4].data_ptr() : nullptr, pages->width), "o1_kv_pages_grow"))
+        return nullptr;
+    PyObject* all = PyTuple_New(5);
+    for (int i = 0; all && i < 5; ++i) {
+        PyObject* o = THPVariable_Wrap(out[i]);
+        if (!o) { Py_DECREF(all); return nullptr; }
+        PyTuple_SET_ITEM(all, i, o);
+    }
+    return all;
+    END_HANDLE_TH_ERRORS
+}
+
+// pages_shrink(address of an o1_kv_pages, device index, keep, seqs or None)
+PyObject* py_shrink(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    static const char* who = "KvPages.shrink";
+    if (!arguments(n, 4)) return nullptr;
+    const auto* pages = (const o1_kv_pages*)PyLong_AsUnsignedLongLong(a[0]);
+    const int device = (int)PyLong_AsLong(a[1]);
+    if (PyErr_Occurred()) return nullptr;
+    const at::Tensor *keep = ints(a[2], -1, device, who, "keep"), *seqs = nullptr;
+    if (!keep) return nullptr;
+    if (keep->size(0) > pages->max_seqs) return fail(who, "more requests than sequences");
+    if (a[3] != Py_None && !(seqs = ints(a[3], keep->size(0), device, who, "seqs"))) return nullptr;
+    if (!status(f_shrink(pages, seqs ? (const int32_t*)seqs->data_ptr() : nullptr, (const int32_t*)keep->data_ptr(), (int)keep->size(0)), "o1_kv_pages_shrink")) return nullptr;
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// rotary(address of an o1_rope, device index, positions, inverse, x, y or None[, x, y or None]) -> y or (y, y)
+PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    static const char* who = "Rotary";
+    if (n != 6 && n != 8) { PyErr_SetString(PyExc_TypeError, "wrong number of arguments"); return nullptr; }
+    const auto* rope = (const o1_rope*)PyLong_AsUnsignedLongLong(a[0]);
+    const int device = (int)PyLong_AsLong(a[1]), inverse = PyObject_IsTrue(a[3]), sides = n == 8 ? 2 : 1;
+    if (PyErr_Occurred()) return nullptr;
+    const at::Tensor* positions = tensor(a[2], who);
+    if (!positions) return nullptr;
+    const bool wide = positions->scalar_type() == at::kLong;
+    if ((!wide && positions->scalar_type() != at::kInt) || positions->dim() != 1 || !positions->is_contiguous() || !positions->is_cuda() || positions->device().index() != device ||
+        positions->size(0) > INT32_MAX)
+        return fail(who, "positions int32 or int64 [rows], contiguous, on the frequencies' GPU wanted");
+    const int64_t rows = positions->size(0), dim = rope->head_dim;
+    at::ScalarType type = at::kBFloat16;
+    auto rows_of = [&](const at::Tensor& t, int64_t heads, int64_t& ld) {
+        if (t.dim() != 3 || t.scalar_type() != type || !t.is_cuda() || t.device().index() != device || t.size(0) != rows || (heads >= 0 && t.size(1) != heads) || t.size(2) != dim) {
+            PyErr_Format(O1Error, "%s: rows [%lld, heads, %lld] bf16 or fp32, all of one type, on the frequencies' GPU wanted", who, (long long)rows, (long long)dim);
+            return false;
+        }
+        if ((t.stride(2) != 1 && dim > 1) || (t.stride(1) != dim && t.size(1) > 1)) { fail(who, "a row's heads must lie side by side"); return false; }
+        if (t.size(1) > 65536) { fail(who, "too many heads"); return false; }
+        ld = rows > 1 ? t.stride(0) : t.size(1) * dim;
+        return true;
+    };
+    const OnLibrary on(device);
+    at::Tensor out[2];
+    const at::Tensor* in[2] = {nullptr, nullptr};
+    int64_t ldx[2] = {0, 0}, ldy[2] = {0, 0};
+    for (int i = 0; i < sides; ++i) {
+        if (!(in[i] = tensor(a[4 + 2 * i], who))) return nullptr;
+        if (i == 0 && in[0]->scalar_type() == at::kFloat) type = at::kFloat;
+        if (!rows_of(*in[i], -1, ldx[i])) return nullptr;
+        const int64_t heads = in[i]->size(1);
+        if (a[5 + 2 * i] == Py_None) {
+            out[i] = empty_on({rows, heads, dim}, type, device);
+            ldy[i] = heads * dim;
+        } else {
+            const at::Tensor* t = tensor(a[5 + 2 * i], who);
+            if (!t || !rows_of(*t, heads, ldy[i])) return nullptr;
+            out[i] = *t;
+        }
+    }
+    if (!status(f_rotary(rope, positions->data_ptr(), wide, in[0]->data_ptr(), ldx[0], out[0].data_ptr(), ldy[0], (int)in[0]->size(1), sides == 2 ? in[1]->data_ptr() : nullptr, ldx[1],
+                         sides == 2 ? out[1].data_ptr() : nullptr, ldy[1], sides == 2 ? (int)in[1]->size(1) : 0, (int)rows, type == at::kFloat ? O1_ROPE_FP32 : O1_ROPE_BF16, inverse),
+                "o1_rotary"))
+        return nullptr;
+    PyObject* y = THPVariable_Wrap(out[0]);
+    if (sides == 1) return y;
+    PyObject *z = THPVariable_Wrap(out[1]), *both = y && z ? PyTuple_Pack(2, y, z) : nullptr;
+    Py_XDECREF(y);
+    Py_XDECREF(z);
+    return both;
+    END_HANDLE_TH_ERRORS
+}
+
+// setup(addresses of o1_kv_write, o1_kv_read, o1_kv_attention, o1_residual_norm, o1_get_stream, o1_capture_id, o1_kv_pages_grow, o1_kv_pages_shrink, o1_rotary; O1Error; check)
 PyObject* py_setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    if (!arguments(n, 8)) return nullptr;
-    unsigned long long p[6];
-    for (int i = 0; i < 6; ++i) p[i] = PyLong_AsUnsignedLongLong(a[i]);
+    if (!arguments(n, 11)) return nullptr;
+    unsigned long long p[9];
+    for (int i = 0; i < 9; ++i) p[i] = PyLong_AsUnsignedLongLong(a[i]);
     if (PyErr_Occurred()) return nullptr;
     f_write = (decltype(f_write))p[0];
     f_read = (decltype(f_read))p[1];
@@ -325,15 +444,18 @@ PyObject* py_setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
     f_norm = (decltype(f_norm))p[3];
     f_stream = (decltype(f_stream))p[4];
     f_capture = (decltype(f_capture))p[5];
-    O1Error = Py_NewRef(a[6]);
-    check = Py_NewRef(a[7]);
+    f_grow = (decltype(f_grow))p[6];
+    f_shrink = (decltype(f_shrink))p[7];
+    f_rotary = (decltype(f_rotary))p[8];
+    O1Error = Py_NewRef(a[9]);
+    check = Py_NewRef(a[10]);
     Py_RETURN_NONE;
 }
 
 #define FAST(name, f) {name, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST("setup", py_setup), FAST("handle", py_handle), FAST("write", py_write), FAST("read", py_read), FAST("attend", py_attend),
-                         FAST("residual_norm", py_norm), {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", "Calls of KvCache and residual_norm.", -1, methods, nullptr, nullptr, nullptr, nullptr};
+                         FAST("residual_norm", py_norm), FAST("pages_grow", py_grow), FAST("pages_shrink", py_shrink), FAST("rotary", py_rotary), {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", "Calls of KvCache, KvPages, Rotary and residual_norm.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
 

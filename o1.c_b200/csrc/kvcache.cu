@@ -2,7 +2,8 @@
 //
 // Layout: k and v each [pages][kv_heads][page_size][128], a head's rows of a page behind one another, so that what one
 // (sequence, kv head) pair reads of a page is contiguous.  Stored as bf16, or as fp8 (e4m3) or int8 codes with one fp32 scale for each token
-// and head in arrays [pages][kv_heads][page_size]: x ~ code * scale.  No counterpart in o1.c, which keeps no keys or values
+// and head in arrays [pages][kv_heads][page_size]: x ~ code * scale; or as codes of four bits, two to a byte (64 bytes a row), with a scale and a least value in bf16
+// in the same place: x ~ least + code * scale.  No counterpart in o1.c, which keeps no keys or values
 // from one forward to the next.
 #include "common.cuh"
 #include "kernels.h"
@@ -14,7 +15,7 @@
 
 namespace o1 {
 
-enum { KV_BF16 = O1_KV_BF16, KV_FP8 = O1_KV_FP8, KV_INT8 = O1_KV_INT8 };
+enum { KV_BF16 = O1_KV_BF16, KV_FP8 = O1_KV_FP8, KV_INT8 = O1_KV_INT8, KV_UINT4 = O1_KV_UINT4 };
 static constexpr int KV_D = 128;
 // Codes of the device's table word: what a kernel found in a table on the device.  Nothing is read or written for such an entry, and nothing else stops for it.
 static constexpr int ERR_KV_PLACE = 70;    // a slot or page outside the cache
@@ -107,6 +108,66 @@ __device__ __forceinline__ uint4 dequantise8(const uint2& c, int type, float sca
     return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
 }
 
+
+// Four bits: sixteen values from a row's least to its largest one, evenly spaced, so that rows to one side of zero lose nothing.  The distance is (largest - least) / 15
+// rounded to bf16 (code 15 is at most 0.03 of it from the largest value, no code is out of range); the least value is one of the row's and exact.  A spread below
+// 2^-100 counts as none: all values read as the least one.  Scale and least value share the four bytes that the other kinds' scale has.  A row with an Inf or NaN, or
+// whose spread is beyond fp32, gets NaN for both.
+__device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// Of eight values the largest (low half) and the least one's negative (high half).
+__device__ __forceinline__ uint32_t extremes(const uint4& x) {
+    constexpr uint32_t S = 0x80008000u;
+    const uint32_t hi = max_nan_bf16x2(max_nan_bf16x2(x.x, x.y), max_nan_bf16x2(x.z, x.w));
+    const uint32_t lo = max_nan_bf16x2(max_nan_bf16x2(x.x ^ S, x.y ^ S), max_nan_bf16x2(x.z ^ S, x.w ^ S));
+    return max_nan_bf16x2(__byte_perm(hi, lo, 0x5410), __byte_perm(hi, lo, 0x7632));
+}
+// Of a row's extremes the pair (scale, least) as it is kept, and the scale's reciprocal, 0 where there are no codes.
+__device__ __forceinline__ uint32_t scale4_of(uint32_t top, float& inv, float& least) {
+    const float spread = __fadd_rn(bf16lo(top), bf16hi(top));
+    least = 0.0f - bf16hi(top);
+    inv = 0.0f;
+    if (!(spread <= 3.4028234663852886e38f)) return 0x7FC07FC0u;
+    uint32_t scale = 0;
+    if (spread >= 7.888609052210118e-31f) {
+        scale = f32_to_bf16(__fmul_rn(spread, 1.0f / 15.0f));
+        inv = __fdiv_rn(1.0f, bf16_to_f32((uint16_t)scale));
+    }
+    return scale | (__float_as_uint(least) & 0xFFFF0000u);
+}
+// Eight codes, the first one in the lowest bits.
+__device__ __forceinline__ uint32_t codes4_of(const uint4& x, float inv, float least) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    float f[8];
+    if (inv == 0.0f) return 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[2 * i] = __fmul_rn(__fsub_rn(bf16lo(w[i]), least), inv); f[2 * i + 1] = __fmul_rn(__fsub_rn(bf16hi(w[i]), least), inv); }
+    return int8x4(f[0], f[2], f[4], f[6]) | int8x4(f[1], f[3], f[5], f[7]) << 4;
+}
+__device__ __forceinline__ uint32_t quantise8_4(const uint4& x, uint32_t& pair) {
+    uint32_t top = extremes(x);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max_nan_bf16x2(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float inv, least;
+    pair = scale4_of(top, inv, least);
+    return codes4_of(x, inv, least);
+}
+__device__ __forceinline__ void values4(uint32_t c, uint32_t pair, float (&f)[8]) {
+    const uint32_t half[2] = {c & 0x0F0F0F0Fu, (c >> 4) & 0x0F0F0F0Fu};
+    const float scale = bf16lo(pair), least = bf16hi(pair);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)      // 2^23 + c as bits
+        f[i] = __fmaf_rn(__uint_as_float(__byte_perm(half[i & 1], 0x4B000000u, 0x7540 + (i >> 1))) - 8388608.0f, scale, least);
+}
+__device__ __forceinline__ uint4 dequantise8_4(uint32_t c, uint32_t pair) {
+    float f[8];
+    values4(c, pair, f);
+    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+}
+
 template <bool VEC>
 __device__ __forceinline__ uint4 load8(const uint16_t* p) {
     if (VEC) return *reinterpret_cast<const uint4*>(p);
@@ -139,7 +200,7 @@ __device__ __forceinline__ int64_t place(int64_t slot, int head, const KvView& c
     const int64_t page = c.page_shift >= 0 ? slot >> c.page_shift : slot / c.page_size;
     return (page * c.heads + head) * c.page_size + slot - page * c.page_size;
 }
-template <bool VEC, int EACH>
+template <bool VEC, int EACH, bool FOUR>
 __global__ void __launch_bounds__(128, EACH == 8 ? 9 : 12)
 kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk, const uint16_t* __restrict__ v, int64_t ldv,
                 const int64_t* __restrict__ slots, unsigned units, const int* err, int* bad) {
@@ -165,8 +226,23 @@ kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk,
     }
     const int64_t places = place(failed ? -1 : slot, from + mine - my_row * c.heads, c, bad);
     grid_dep_launch();
-    float inv = 0.f;
-    if (type != KV_BF16) {
+    float inv = 0.f, least = 0.f;
+    if (FOUR) {          // as below, the largest and the least value together
+        uint32_t top[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) top[i] = extremes(x[i]);
+#pragma unroll
+        for (int o = 8, n = EACH / 2; o > 0; o >>= 1, n >>= 1) {
+            if (n == 0) top[0] = max_nan_bf16x2(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
+#pragma unroll
+            for (int i = 0; i < n; ++i) {
+                const uint32_t keep = lane & o ? top[n + i] : top[i], give = lane & o ? top[i] : top[n + i];
+                top[i] = max_nan_bf16x2(keep, __shfl_xor_sync(0xffffffffu, give, o));
+            }
+        }
+        const uint32_t pair = scale4_of(top[0], inv, least);
+        if (places >= 0 && lane % (16 / EACH) == 0) reinterpret_cast<uint32_t*>(scales)[places] = pair;
+    } else if (type != KV_BF16) {
         // maxima: a step halves the lanes that a unit is spread over, and, until a lane has one, its units
         uint32_t top[EACH];
 #pragma unroll
@@ -186,14 +262,15 @@ kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk,
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
         const int64_t at = __shfl_sync(0xffffffffu, places, i * (16 / EACH), 16);
-        const float f = __shfl_sync(0xffffffffu, inv, i * (16 / EACH), 16);
+        const float f = __shfl_sync(0xffffffffu, inv, i * (16 / EACH), 16), from_least = FOUR ? __shfl_sync(0xffffffffu, least, i * (16 / EACH), 16) : 0.f;
         if (at < 0) continue;
-        if (type == KV_BF16) reinterpret_cast<uint4*>(base)[at * 16 + lane] = x[i];
+        if (FOUR) reinterpret_cast<uint32_t*>(base)[at * 16 + lane] = codes4_of(x[i], f, from_least);
+        else if (type == KV_BF16) reinterpret_cast<uint4*>(base)[at * 16 + lane] = x[i];
         else reinterpret_cast<uint2*>(base)[at * 16 + lane] = codes_of(x[i], type, f);
     }
 }
 
-template <bool VEC, int EACH>
+template <bool VEC, int EACH, bool FOUR>
 __global__ void __launch_bounds__(128, EACH == 8 ? 7 : 12)
 kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16_t* __restrict__ v, int64_t ldv,
                const int64_t* __restrict__ slots, unsigned units, int* bad) {
@@ -217,6 +294,7 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
         const int64_t at = __shfl_sync(0xffffffffu, places, i * (16 / EACH), 16);
         x[i] = make_uint4(0, 0, 0, 0);
         if (at < 0) continue;
+        if (FOUR) { x[i].x = reinterpret_cast<const uint32_t*>(base)[at * 16 + lane]; continue; }
         if (type == KV_BF16) { x[i] = reinterpret_cast<const uint4*>(base)[at * 16 + lane]; continue; }
         const uint2 codes = reinterpret_cast<const uint2*>(base)[at * 16 + lane];
         x[i].x = codes.x;
@@ -227,7 +305,7 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
     for (int i = 0; i < EACH; ++i) {
         if (i >= count) break;
         const float s = __shfl_sync(0xffffffffu, scale, i * (16 / EACH), 16);
-        store8<VEC>(dst + head * KV_D, type == KV_BF16 ? x[i] : dequantise8(make_uint2(x[i].x, x[i].y), type, s));
+        store8<VEC>(dst + head * KV_D, FOUR ? dequantise8_4(x[i].x, __float_as_uint(s)) : type == KV_BF16 ? x[i] : dequantise8(make_uint2(x[i].x, x[i].y), type, s));
         if (++head == c.heads) { head = 0; dst += ld; }
     }
 }
@@ -1096,11 +1174,49 @@ static cudaError_t launch_attention(const CUtensorMap& k_map, const CUtensorMap&
     return launch_attention<TYPE, HG, false>(k_map, v_map, a, (int)max((int64_t)1, min((int64_t)most, max((item_chunks * items + KV_TEAM - 1) / KV_TEAM, items))), st);
 }
 
+// Over codes of four bits, a warp to a query head of a sequence, four columns to a lane.
+__global__ void kv_append4_kernel(const KvAttn a) {
+    const int b = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, len = a.lens[b];
+    if (head >= a.c.heads || len <= 0 || len > (int64_t)a.width * a.c.page_size || error_word(a.err)) return;
+    const int page = a.pages[b * a.ldp + (len - 1) / a.c.page_size];
+    if ((unsigned)page >= (unsigned)a.c.pages) return;
+    const int64_t at = ((int64_t)page * a.c.heads + head) * a.c.page_size + (len - 1) % a.c.page_size;
+    uint32_t pair;
+    const uint4 x = load8<false>((lane < 16 ? a.kn + b * a.ldk : a.vn + b * a.ldv) + head * KV_D + (lane & 15) * 8);
+    const uint32_t codes = quantise8_4(x, pair);
+    reinterpret_cast<uint32_t*>(lane < 16 ? a.c.k : a.c.v)[at * 16 + (lane & 15)] = codes;
+    if ((lane & 15) == 0) reinterpret_cast<uint32_t*>(lane < 16 ? a.c.ks : a.c.vs)[at] = pair;
+}
+__global__ void kv_attention4_kernel(const KvAttn a) {
+    const int b = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (head >= a.heads) return;
+    int len = a.lens[b];
+    if (len < 0 || len > (int64_t)a.width * a.c.page_size) { atomicExch(a.bad, ERR_KV_LENGTH); len = 0; }
+    float q[4], o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0.f;
+    for (int i = 0; i < 4; ++i) q[i] = bf16_to_f32(a.q[b * a.ldq + head * KV_D + 4 * lane + i]) * a.scale;
+    for (int t = 0; t < len; ++t) {
+        const int page = a.pages[b * a.ldp + t / a.c.page_size];
+        if ((unsigned)page >= (unsigned)a.c.pages) { atomicExch(a.bad, ERR_KV_PLACE); break; }
+        const int64_t at = ((int64_t)page * a.c.heads + head / a.group) * a.c.page_size + t % a.c.page_size;
+        const uint32_t kp = reinterpret_cast<const uint32_t*>(a.c.ks)[at], vp = reinterpret_cast<const uint32_t*>(a.c.vs)[at];
+        const uint32_t kc = reinterpret_cast<const uint16_t*>(a.c.k)[at * 32 + lane], vc = reinterpret_cast<const uint16_t*>(a.c.v)[at * 32 + lane];
+        float z = 0.f;
+        for (int i = 0; i < 4; ++i) z += q[i] * (bf16hi(kp) + (float)((kc >> (4 * i)) & 15) * bf16lo(kp));
+        for (int s = 16; s > 0; s >>= 1) z += __shfl_xor_sync(0xffffffffu, z, s);
+        const float top = fmaxf(m, z), alpha = m == -INFINITY ? 0.f : expf(m - top), p = expf(z - top);
+        l = l * alpha + p;
+        for (int i = 0; i < 4; ++i) o[i] = o[i] * alpha + p * (bf16hi(vp) + (float)((vc >> (4 * i)) & 15) * bf16lo(vp));
+        m = z != z ? z : top;
+    }
+    for (int i = 0; i < 4; ++i) a.out[b * a.ldo + head * KV_D + 4 * lane + i] = f32_to_bf16(l > 0.f || l != l ? o[i] / l : 0.f);
+    if (a.lse && lane == 0) a.lse[(int64_t)b * a.heads + head] = m + logf(l);
+}
+
 static bool aligned16(const void* p, int64_t ld) { return (((uintptr_t)p) & 15) == 0 && (ld & 7) == 0; }
 
 static hd_status kv_view(const o1_kv_cache* c, KvView* out, const char* what) {
     if (!c || !c->k || !c->v) { set_error("%s: null cache", what); return HD_ERR_MISSING; }
-    if (c->type != O1_KV_BF16 && c->type != O1_KV_FP8 && c->type != O1_KV_INT8) { set_error("%s: unknown cache type %d", what, c->type); return HD_ERR_UNSUPPORTED; }
+    if (c->type != O1_KV_BF16 && c->type != O1_KV_FP8 && c->type != O1_KV_INT8 && c->type != O1_KV_UINT4) { set_error("%s: unknown cache type %d", what, c->type); return HD_ERR_UNSUPPORTED; }
     if (c->head_dim != KV_D) { set_error("%s: head_dim %d (must be 128)", what, c->head_dim); return HD_ERR_UNSUPPORTED; }
     if (c->pages <= 0 || c->kv_heads <= 0 || c->page_size <= 0 || c->page_size % 16) {
         set_error("%s: pages %d, kv_heads %d, page_size %d (a multiple of 16)", what, c->pages, c->kv_heads, c->page_size);
@@ -1142,7 +1258,10 @@ hd_status o1_kv_write(const o1_kv_cache* cache, const void* k, int64_t ldk, cons
         const unsigned units = (unsigned)min(most, rows - first) * c.heads;
         const bool few = units < KV_FEW_UNITS;
         const unsigned block = 4 * (few ? KV_EACH_OF_FEW : KV_EACH);
-        auto kern = few ? (vec ? kv_write_kernel<true, KV_EACH_OF_FEW> : kv_write_kernel<false, KV_EACH_OF_FEW>) : vec ? kv_write_kernel<true, KV_EACH> : kv_write_kernel<false, KV_EACH>;
+        auto kern = cache->type == O1_KV_UINT4 ? (few ? (vec ? kv_write_kernel<true, KV_EACH_OF_FEW, true> : kv_write_kernel<false, KV_EACH_OF_FEW, true>)
+                                                        : (vec ? kv_write_kernel<true, KV_EACH, true> : kv_write_kernel<false, KV_EACH, true>))
+                    : few ? (vec ? kv_write_kernel<true, KV_EACH_OF_FEW, false> : kv_write_kernel<false, KV_EACH_OF_FEW, false>)
+                          : (vec ? kv_write_kernel<true, KV_EACH, false> : kv_write_kernel<false, KV_EACH, false>);
         if (!launch_ok(launch_chained(kern, dim3((units + block - 1) / block), dim3(128), 0, current_stream(), 1, 1, c, cache->type, (const uint16_t*)k + first * ldk, ldk,
                                       (const uint16_t*)v + first * ldv, ldv, slots + first, units, (const int*)device_error_word(), device_table_word()), "kv_write"))
             return HD_ERR_RUNTIME;
@@ -1167,7 +1286,10 @@ hd_status o1_kv_read(const o1_kv_cache* cache, void* k, int64_t ldk, void* v, in
         const unsigned units = (unsigned)min(most, rows - first) * c.heads;
         const bool few = units < KV_FEW_UNITS;
         const unsigned block = 4 * (few ? KV_EACH_OF_FEW : KV_EACH);
-        auto kern = few ? (vec ? kv_read_kernel<true, KV_EACH_OF_FEW> : kv_read_kernel<false, KV_EACH_OF_FEW>) : vec ? kv_read_kernel<true, KV_EACH> : kv_read_kernel<false, KV_EACH>;
+        auto kern = cache->type == O1_KV_UINT4 ? (few ? (vec ? kv_read_kernel<true, KV_EACH_OF_FEW, true> : kv_read_kernel<false, KV_EACH_OF_FEW, true>)
+                                                        : (vec ? kv_read_kernel<true, KV_EACH, true> : kv_read_kernel<false, KV_EACH, true>))
+                    : few ? (vec ? kv_read_kernel<true, KV_EACH_OF_FEW, false> : kv_read_kernel<false, KV_EACH_OF_FEW, false>)
+                          : (vec ? kv_read_kernel<true, KV_EACH, false> : kv_read_kernel<false, KV_EACH, false>);
         if (!launch_ok(launch_chained(kern, dim3((units + block - 1) / block), dim3(128), 0, current_stream(), 1, 1, c, cache->type, (uint16_t*)k + first * ldk, ldk,
                                       (uint16_t*)v + first * ldv, ldv, slots + first, units, device_table_word()), "kv_read"))
             return HD_ERR_RUNTIME;
@@ -1216,6 +1338,14 @@ hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, 
     a.err = device_error_word();
     a.bad = device_table_word();
     a.flags = (aligned16(q, ldq) ? 1 : 0) | (aligned16(out, ldo) ? 2 : 0) | (aligned16(k_new, ldk) && aligned16(v_new, ldv) ? 4 : 0);
+    if (cache->type == O1_KV_UINT4) {
+        a.batch = batch;
+        a.q = (const uint16_t*)q; a.kn = (const uint16_t*)k_new; a.vn = (const uint16_t*)v_new; a.pages = pages; a.lens = lens; a.out = (uint16_t*)out; a.lse = lse;
+        if (k_new) kv_append4_kernel<<<dim3(batch, (c.heads + 3) / 4), 128, 0, current_stream()>>>(a);
+        kv_attention4_kernel<<<dim3(batch, (heads + 3) / 4), 128, 0, current_stream()>>>(a);
+        o1_launch_count_add(k_new ? 2 : 1);
+        return launch_ok(cudaGetLastError(), "kv_attention") ? HD_OK : HD_ERR_RUNTIME;
+    }
     // maps of the rows, 128 bytes (64 columns of bf16, all codes) x 16, or 32 where a chunk of codes never crosses a page
     const bool wide = keys == 32 && c.page_size % 32 == 0;
     if (wide) a.flags |= 8;

@@ -1,13 +1,15 @@
-"""Rows after a prompt: a paged cache of keys and values, the attention of new rows over it, the residual add between
-two norms -- o1_kv_write, o1_kv_read, o1_kv_attention and o1_residual_norm on torch tensors -- and a Decoder that continues prompts with them.
+"""Rows after a prompt: a paged cache of keys and values, the attention of new rows over it, pages handed out on the GPU, rotary positions, the residual
+add between two norms -- o1_kv_write, o1_kv_read, o1_kv_attention, o1_kv_pages_grow, o1_kv_pages_shrink, o1_rotary and o1_residual_norm on torch tensors -- and a
+Decoder that continues prompts with them.
 
 Like every entry point they enqueue on the library's current stream (use_torch_stream()) and return at once.  Arguments that
-do not fit raise O1Error; a slot, page or length that does not fit is found on the device (lib.o1_device_error() gives 70 or 71).
+do not fit raise O1Error; a slot, page, sequence or length that does not fit is found on the device (lib.o1_device_error() gives 70, 71 or, with no pages left, 73).
 Where torch's current stream is another one, what these calls make (caches, results, tables) is made, filled and freed in the order of the library's;
 ordering that, and their inputs, with torch's own work is the caller's.
 """
 import ctypes as C
 import os
+from collections import namedtuple
 
 import torch
 
@@ -20,14 +22,14 @@ from . import _binding  # noqa: E402
 if _binding.torch_version != torch.__version__.split("+")[0]:
     raise ImportError(f"{_BINDING} is of torch {_binding.torch_version}, this is {torch.__version__}: build it with `python o1.c_b200/build.py`")
 
-from . import HEAD_DIM, KV_HEADS, KvCacheC, O1Error, _on_library, check, lib, ptr  # noqa: E402
+from . import HEAD_DIM, KV_HEADS, ROPE_THETA, KvCacheC, KvPagesC, O1Error, RopeC, RopeScalingC, _on_library, check, lib, ptr  # noqa: E402
 
-KINDS = {"bf16": (0, torch.bfloat16), "fp8": (1, torch.float8_e4m3fn), "int8": (2, torch.int8)}
+KINDS = {"bf16": (0, torch.bfloat16), "fp8": (1, torch.float8_e4m3fn), "int8": (2, torch.int8), "uint4": (4, torch.uint8)}
 _BY_DTYPE = {d: n for n, d in KINDS.values()}
 BF16, I32, I64, F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
 _stream = lib.o1_get_stream
-_binding.setup(*(C.cast(f, C.c_void_p).value for f in (lib.o1_kv_write, lib.o1_kv_read, lib.o1_kv_attention, lib.o1_residual_norm, lib.o1_get_stream, lib.o1_capture_id)),
-               O1Error, check)
+_binding.setup(*(C.cast(f, C.c_void_p).value for f in (lib.o1_kv_write, lib.o1_kv_read, lib.o1_kv_attention, lib.o1_residual_norm, lib.o1_get_stream, lib.o1_capture_id,
+                                                       lib.o1_kv_pages_grow, lib.o1_kv_pages_shrink, lib.o1_rotary)), O1Error, check)
 
 
 def _need(ok, what):
@@ -75,17 +77,19 @@ class _Workspace:
 class KvCache:
     """Keys and values of many sequences in pages of page_size tokens, [pages, kv_heads, page_size, 128].
 
-    kind: "bf16", or "fp8" / "int8" (a byte a value and one fp32 scale for each token and head).  A token's slot is
-    page * page_size + its place in the page; which pages a sequence has is the caller's table."""
+    kind: "bf16", or "fp8" / "int8" (a byte a value and one fp32 scale for each token and head), or "uint4" (two values to a byte, uint8 [pages, kv_heads, page_size,
+    64] with the first value in the low bits, and a bf16 pair (scale, least value) [pages, kv_heads, page_size, 2] for each token and head).  A token's slot is
+    page * page_size + its place in the page; which pages a sequence has is the caller's table (KvPages hands them out on the GPU)."""
 
     def __init__(self, pages, page_size=64, kind="bf16", kv_heads=KV_HEADS, device="cuda"):
         _need(kind in KINDS, f"KvCache: kind {kind!r} (one of {', '.join(KINDS)})")
-        shape = (pages, kv_heads, page_size, HEAD_DIM)
+        shape = (pages, kv_heads, page_size, HEAD_DIM // 2 if kind == "uint4" else HEAD_DIM)
         dtype = KINDS[kind][1]
         with _on_library(device):
             k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) if kind != "bf16" else
                     torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
-            ks, vs = (torch.zeros(shape[:3], device=device) if kind != "bf16" else None for _ in range(2))
+            ks, vs = (None if kind == "bf16" else torch.zeros(shape[:3] + (2,), dtype=BF16, device=device) if kind == "uint4" else
+                      torch.zeros(shape[:3], device=device) for _ in range(2))
         self._set(k, v, ks, vs)
 
     @classmethod
@@ -96,13 +100,17 @@ class KvCache:
         return self
 
     def _set(self, k, v, k_scale, v_scale):
-        _need(k.dtype in _BY_DTYPE and k.dim() == 4 and k.size(3) == HEAD_DIM, "KvCache: k [pages, kv_heads, page_size, 128] bf16, float8_e4m3fn or int8 wanted")
+        _need(k.dtype in _BY_DTYPE and k.dim() == 4 and k.size(3) == (HEAD_DIM // 2 if k.dtype is torch.uint8 else HEAD_DIM),
+              "KvCache: k [pages, kv_heads, page_size, 128] bf16, float8_e4m3fn or int8, or [pages, kv_heads, page_size, 64] uint8 wanted")
         _need(v.dtype == k.dtype and v.shape == k.shape, "KvCache: v differs from k in shape or type")
         kind = _BY_DTYPE[k.dtype]
         tensors = [k, v]
         if kind:
             for s in (k_scale, v_scale):
-                _need(s is not None and s.dtype is F32 and s.shape == k.shape[:3], "KvCache: scales [pages, kv_heads, page_size] fp32 wanted")
+                if k.dtype is torch.uint8:
+                    _need(s is not None and s.dtype is BF16 and s.shape == (*k.shape[:3], 2), "KvCache: scales [pages, kv_heads, page_size, 2] bf16 (scale, least value) wanted")
+                else:
+                    _need(s is not None and s.dtype is F32 and s.shape == k.shape[:3], "KvCache: scales [pages, kv_heads, page_size] fp32 wanted")
                 tensors.append(s)
         for t in tensors:
             _need(t.is_cuda and t.device == k.device and t.is_contiguous() and t.data_ptr() % 16 == 0, "KvCache: contiguous, 16-byte aligned tensors of one GPU wanted")
@@ -141,6 +149,100 @@ class KvCache:
         Returns out [batch, heads, 128] bf16, with lse=True (or a tensor [batch, heads] fp32) a pair (out, log-sum-exp).  An empty sequence
         gives zeros and -inf.  scale: 1 / sqrt(128)."""
         return _binding.attend(self._h, self, q, pages, lens, k, v, out, lse, scale)
+
+
+Grown = namedtuple("Grown", "slots positions starts lens pages")
+Grown.__doc__ = """What KvPages.grow gives: slots [rows] int64 and positions [rows] int32 of the new rows, starts [requests + 1] (where each request's rows begin), lens [requests]
+and pages [requests, width] as KvCache.attend takes them."""
+
+
+class KvPages:
+    """Which pages of a cache sequences have, handed out on the GPU: table [max_seqs, width] (a sequence's pages in order, -1 behind them), lens [max_seqs] (its rows),
+    free [pages] (a stack of free pages) and state [2] (how many are free; the calls' own), all int32.
+
+    Calls on the same pages follow one another.  They can be captured: a graph serves the counts and sequences that its tensors hold at each replay."""
+
+    def __init__(self, pages, page_size=64, max_seqs=64, width=64, device="cuda"):
+        _need(min(pages, max_seqs, width) > 0, "KvPages: pages, max_seqs and width must be positive")
+        with _on_library(device):
+            table, lens, free, state = (torch.empty(s, dtype=I32, device=device) for s in ((max_seqs, width), (max_seqs,), (pages,), (2,)))
+        self._set(table, lens, free, state, page_size)
+        self.reset()
+
+    @classmethod
+    def over(cls, table, lens, free, state, page_size):
+        """Pages in tensors that the caller has, as they stand."""
+        self = cls.__new__(cls)
+        self._set(table, lens, free, state, page_size)
+        return self
+
+    def _set(self, table, lens, free, state, page_size):
+        for name, t, dim in (("table", table, 2), ("lens", lens, 1), ("free", free, 1), ("state", state, 1)):
+            _need(t.dtype is I32 and t.dim() == dim and t.is_cuda and t.device == table.device and t.is_contiguous() and 0 < t.numel() and max(t.shape) < 2 ** 31,
+                  f"KvPages: {name} int32, of {dim} dimensions, contiguous, on one GPU wanted")
+        _need(lens.size(0) == table.size(0) <= 8192 and state.size(0) == 2, "KvPages: lens [max_seqs], at most 8192, and state [2] wanted")
+        _need(0 < page_size < 2 ** 31 and page_size % 16 == 0 and table.size(1) * page_size < 2 ** 31, "KvPages: page_size must be a multiple of 16, and a table's rows fewer than 2^31")
+        self.table, self.lens, self.free, self.state, self.page_size = table, lens, free, state, page_size
+        self.pages, self.max_seqs, self.width = free.size(0), *table.shape
+        self.device = table.device
+        self.c = KvPagesC(*(t.data_ptr() for t in (table, lens, free, state)), self.pages, page_size, self.max_seqs, self.width)
+        self._at, self._gpu = C.addressof(self.c), table.get_device()
+
+    def reset(self):
+        """Every page free, every sequence empty."""
+        check(lib.o1_kv_pages_reset(C.byref(self.c)), "o1_kv_pages_reset")
+
+    def grow(self, counts, rows, seqs=None):
+        """counts [requests] int32 new rows of sequences seqs [requests] int32 (all different; None: 0, 1, ...), with room for `rows` of them in all: Grown.
+
+        The requests' rows lie behind one another; rows behind the last one have slot -1.  A request that cannot be served (70: no such sequence, or named twice; 71: too many
+        rows; 73: no pages left) has slots of -1 and a length of 0.  pages is the table itself where seqs is None."""
+        return Grown._make(_binding.pages_grow(self._at, self._gpu, self.table, counts, rows, seqs))
+
+    def shrink(self, keep, seqs=None):
+        """Sequences seqs [requests] int32 (None: 0, 1, ...) keep their first keep [requests] int32 rows; the pages behind them are free again."""
+        _binding.pages_shrink(self._at, self._gpu, keep, seqs)
+
+
+class Rotary:
+    """Rotary positions: the first rot_dim values of each head turned in pairs, "half" (i, i + rot_dim / 2) or "interleaved" (2i, 2i + 1), by position *
+    theta^(-2i / rot_dim).  Angles are exact at any position (turns as 64-bit fractions).
+
+    scaling, for contexts longer than the model was made for: {"kind": "linear", "factor": f}, {"kind": "ntk", "factor": f}, {"kind": "yarn", "factor": f, "original":
+    rows, "fast": 32, "slow": 1}, or {"kind": "factors", "factors": [rot_dim / 2 divisors]}; with "attention": what results are multiplied by."""
+
+    def __init__(self, head_dim=HEAD_DIM, rot_dim=None, theta=ROPE_THETA, layout="half", scaling=None, device="cuda"):
+        rot_dim = head_dim if rot_dim is None else rot_dim
+        _need(0 < rot_dim <= head_dim <= 4096 and rot_dim % 2 == 0, f"Rotary: rot_dim {rot_dim} (even, at most head_dim {head_dim}, which is at most 4096)")
+        _need(layout in ("half", "interleaved"), f"Rotary: layout {layout!r} (half or interleaved)")
+        scaling = dict(scaling or {"kind": "none"})
+        kinds = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "factors": 4}
+        kind = scaling.pop("kind", None)
+        _need(kind in kinds, f"Rotary: scaling of kind {kind!r} (one of {', '.join(kinds)})")
+        unknown = set(scaling) - {"factor", "original", "fast", "slow", "attention", "factors"}
+        _need(not unknown, f"Rotary: scaling has no {', '.join(sorted(unknown))}")
+        factors = [float(f) for f in scaling.get("factors", ())]
+        _need(len(factors) == (rot_dim // 2 if kind == "factors" else 0), "Rotary: factors, one for each pair, belong to scaling of that kind")
+        c = RopeScalingC(kinds[kind], scaling.get("factor", 1.0), scaling.get("original", 0.0), scaling.get("fast", 32.0), scaling.get("slow", 1.0), scaling.get("attention", 0.0),
+                         (C.c_double * len(factors))(*factors) if factors else None)
+        turns, factor = (C.c_uint64 * (rot_dim // 2))(), C.c_float()
+        check(lib.o1_rope_turns(theta, rot_dim, C.byref(c), turns, C.byref(factor)), "o1_rope_turns")
+        signed = [t - 2 ** 64 if t >> 63 else t for t in turns]
+        with _on_library(device):
+            self.turns = torch.tensor(signed, dtype=I64).to(device)
+        self.factor, self.head_dim, self.rot_dim, self.layout = factor.value, head_dim, rot_dim, layout
+        self.c = RopeC(self.turns.data_ptr(), factor, head_dim, rot_dim, 0 if layout == "half" else 1)
+        self._at, self._gpu = C.addressof(self.c), self.turns.get_device()
+
+    def __call__(self, x, positions, inverse=False, out=None):
+        """Rows x [rows, heads, head_dim] bf16 or fp32 (rows of any pitch), or a pair of them (queries and keys), turned by positions [rows] int32 or int64.
+
+        inverse: turned back, which is also the gradient.  out: what to fill, like x (x itself: in place)."""
+        if isinstance(x, tuple):
+            _need(len(x) == 2 and (out is None or len(out) == 2), "Rotary: a tensor or a pair of them")
+            y = (None, None) if out is None else out
+            return _binding.rotary(self._at, self._gpu, positions, inverse, x[0], y[0], x[1], y[1])
+        return _binding.rotary(self._at, self._gpu, positions, inverse, x, out)
 
 
 def residual_norm(x, branch, pre_w, post_w=None, gate=None, scale=None, shift=None, alpha=1.0, eps=1e-6, y=None, h=None):

@@ -1,0 +1,371 @@
+"""Rows kept in four bits and the attention over them, against 64-bit arithmetic on the CPU: KvCache with kind "uint4".
+
+The tests of the other kinds (test_gpu_kvcache) run over these rows too, with this file's definition of what is kept and its bounds.  Bounds, from the arithmetic and
+not from a run, are as there (a score's error 2^-19 of the sum of its terms' magnitudes, a probability times v's scale 2^-17 of itself, the result rounded
+once), but a value is least + code * scale and both products are summed apart, so a value counts with |least| + code * scale in the place of its own magnitude."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+import test_gpu_kvcache as base
+from test_gpu_kvcache import D, between, gen, normal
+
+gpu = pytest.mark.gpu
+
+
+def kept(x):
+    """Packed codes and (scale, least) of bf16 rows by the definition, in fp32 with its roundings."""
+    x = x.float()
+    least, most = x.amin(-1) + 0.0, x.amax(-1)
+    spread = most - least
+    good = torch.isfinite(x).all(-1) & torch.isfinite(spread)
+    scale = torch.where(spread >= 2.0 ** -100, spread * torch.tensor(1.0 / 15.0), 0.0).to(torch.bfloat16).float()
+    inv = torch.where(good & (scale > 0), torch.ones(()) / scale, 0.0)
+    codes = torch.where(good[..., None] & (inv[..., None] > 0), (x - least[..., None]) * inv[..., None], 0.0).round()
+    assert codes.min() >= 0 and codes.max() <= 15
+    codes = codes.to(torch.uint8)
+    pair = torch.stack([torch.where(good, scale, math.nan), torch.where(good, least, math.nan)], -1).to(torch.bfloat16)
+    return codes[..., ::2] | codes[..., 1::2] << 4, pair
+
+
+def unpacked(codes):
+    return torch.stack([codes & 15, codes >> 4], -1).flatten(-2)
+
+
+def quantised(x, kind):
+    return kept(x) if kind == "uint4" else OTHERS[0](x, kind)
+
+
+def value(codes, scale):
+    if codes.dtype is not torch.uint8 or scale is None or scale.dtype is not torch.bfloat16:
+        return OTHERS[1](codes, scale)
+    return scale[..., 1:].double() + unpacked(codes).double() * scale[..., :1].double()
+
+
+def magnitude(codes, scale):
+    return scale[..., 1:].double().abs() + unpacked(codes).double() * scale[..., :1].double()
+
+
+OTHERS = base.quantised, base.value
+
+
+class Case4(base.Case):
+    def reference(self, q, scale=None):
+        B, H = q.shape[:2]
+        sc = D ** -0.5 if scale is None else scale
+        out, lse = torch.zeros(B, H, D, dtype=torch.float64), torch.full((B, H), -math.inf, dtype=torch.float64)
+        tol_o, tol_l = torch.zeros_like(out), torch.zeros_like(lse)
+        for b, n in enumerate(self.lens):
+            if n == 0:
+                continue
+            held = [kept(x[b]) for x in (self.k, self.v)]
+            (k, v), (ka, va) = ([f(*h).repeat_interleave(H // self.hk, 1) for h in held] for f in (value, magnitude))
+            qd = q[b].double()
+            z = torch.einsum("hd,thd->ht", qd, k) * sc
+            size = (torch.einsum("hd,thd->ht", qd.abs(), ka) * sc).amax(-1)
+            lse[b] = torch.logsumexp(z, -1)
+            p = torch.exp(z - lse[b][:, None])
+            out[b] = torch.einsum("ht,thd->hd", p, v)
+            rel = 2.0 * 2.0 ** -19 * size + 2.0 ** -17 + 2.0 ** -18
+            tol_o[b] = torch.einsum("ht,thd->hd", p, va) * rel[:, None] + 1e-30
+            tol_l[b] = 2.0 ** -19 * size + 2.0 ** -21 * (1 + lse[b].abs())
+        return out, lse, tol_o, tol_l
+
+
+@pytest.fixture(autouse=True)
+def four_bits(monkeypatch):
+    monkeypatch.setattr(base, "Case", Case4)
+    monkeypatch.setattr(base, "quantised", quantised)
+    monkeypatch.setattr(base, "value", value)
+
+
+def test_the_definition():
+    """Every value within half a scale (0.53 where code 15 is off by the scale's rounding), the least one exact, ties to even, codes in range."""
+    x = normal((500, D), gen(1), 3.0) + torch.randint(-3, 4, (500, 1), generator=gen(2)).bfloat16() * 8
+    x[0], x[1, 3:], x[2] = 0.0, 5.0, 1.0e30
+    x[3, :16] = torch.arange(16).bfloat16()
+    x[3, 16:] = 7.5                                # a tie: to 8
+    codes, pair = kept(x)
+    got, scale = value(codes, pair), pair[..., 0].double()
+    assert ((got - x.double()).abs() <= 0.53125 * scale[:, None]).all()
+    assert (got.amin(-1) == x.double().amin(-1)).all()
+    assert unpacked(codes)[3].tolist() == list(range(16)) + [8] * 112 and pair[3].tolist() == [1.0, 0.0]
+    assert (scale[[0, 2]] == 0).all()
+
+
+# ------------------------------------------------------------------ rows
+def check_rows(pkg, dev, cache, k, v, slots, left_out=None):
+    page, pages = cache.page_size, cache.pages
+    page_at, at = slots // page, slots % page
+    for x, y, store, scales in ((k, 0, cache.k, cache.k_scale), (v, 1, cache.v, cache.v_scale)):
+        codes, pair = (t.to(dev) for t in kept(x.cpu()))
+        held, s = store[page_at, :, at], scales[page_at, :, at]
+        if left_out is not None:
+            codes[left_out], pair[left_out] = 0, 0.0
+        assert torch.equal(held, codes)
+        assert torch.equal(torch.isnan(s), torch.isnan(pair)) and torch.equal(s.nan_to_num(0), pair.nan_to_num(0))
+        want = (pair[..., 1:].float() + unpacked(codes).float() * pair[..., :1].float()).to(torch.bfloat16)
+        got = cache.read(slots if left_out is None else torch.where(left_out, -1, slots))[y]
+        assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.nan_to_num(7), want.nan_to_num(7))
+    rest = torch.ones(pages * page, dtype=torch.bool, device=dev)
+    rest[slots] = False
+    for t in (cache.k, cache.v):
+        assert (t.permute(0, 2, 1, 3).reshape(pages * page, -1)[rest] == 0).all()
+    for t in (cache.k_scale, cache.v_scale):
+        assert (t.permute(0, 2, 1, 3).reshape(pages * page, -1)[rest] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("rows,heads,page", [(1, 1, 16), (1, 8, 64), (37, 8, 48), (515, 3, 16), (64, 16, 128), (19201, 1, 16), (2405, 8, 64), (6403, 3, 48)])
+def test_rows_written_and_read_back(pkg, dev, rows, heads, page):
+    g = gen(rows + heads)
+    pages = -(-rows // page) + 3
+    cache = pkg.KvCache(pages, page, "uint4", heads, dev)
+    k, v = normal((rows, heads, D), g, 2.0), normal((rows, heads, D), g) + 100.0
+    k[:, :, ::13] *= 50
+    if rows > 6:
+        k[0], v[1], k[2, 0], v[2], k[4], v[4] = 0.0, 2.0 ** -130, -0.0, -3.0, k[4] * 2.0 ** -101, v[4] * 2.0 ** -106
+        v[3] = 2.0 ** 120
+        k[3] = torch.linspace(-1.6e38, 1.6e38, D).bfloat16()
+        k[5, 0, 0], k[5, 0, 1] = 3.0e38, -3.0e38                 # a spread beyond fp32
+        k[1, 0, 5], v[2, heads - 1, 7], v[3, 0, 0], v[5, 0] = math.nan, math.inf, -math.inf, -math.inf
+    slots = torch.randperm(pages * page, generator=g)[:rows].to(dev)
+    cache.write(k.to(dev), v.to(dev), slots)
+    check_rows(pkg, dev, cache, k, v, slots)
+    assert pkg.lib.o1_device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("rows,heads,page,off,pad", [(2401, 8, 16, 1, 3), (1205, 16, 32, 8, 8), (19999, 1, 128, 3, 1), (30, 2, 16, 5, 7)])
+def test_rows_inside_wider_ones_and_rows_left_out(pkg, dev, rows, heads, page, off, pad):
+    g = torch.Generator(device=dev).manual_seed(rows)
+    pages = -(-rows // page) + 3
+    cache = pkg.KvCache(pages, page, "uint4", heads, dev)
+    pitch = 2 * heads * D + pad
+    wide = torch.empty(rows * pitch + off, dtype=torch.bfloat16, device=dev).normal_(0, 1, generator=g)
+    w = wide[off:].view(rows, pitch)
+    k, v = (w[:, i * heads * D:(i + 1) * heads * D].unflatten(1, (heads, D)) for i in (0, 1))
+    slots = torch.randperm(pages * page, generator=g, device=dev)[:rows]
+    left_out = torch.zeros(rows, dtype=torch.bool, device=dev)
+    left_out[[3, 10, rows - 2]] = True
+    cache.write(k, v, torch.where(left_out, -1, slots))
+    check_rows(pkg, dev, cache, k, v, slots, left_out)
+    want = cache.read(slots)
+    wide.fill_(7.0)
+    cache.read(slots, out=(k, v))
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+    assert (w[:, 2 * heads * D:] == 7.0).all() and (wide[:off] == 7.0).all()
+
+
+@gpu
+def test_negative_and_wrong_slots(pkg, dev):
+    cache = pkg.KvCache(2, 16, "uint4", 2, dev)
+    x = normal((4, 2, D), gen(1)).to(dev)
+    cache.write(x, x, torch.tensor([-1, 3, -5, 31], device=dev))
+    k, v = cache.read(torch.tensor([3, -2, 31, 0], device=dev))
+    assert pkg.lib.o1_device_error() == 0
+    assert (k[1] == 0).all() and (v[1] == 0).all() and (k[3] == 0).all() and (k[0] != 0).any()
+    before, scales = cache.k.clone(), cache.k_scale.clone()
+    cache.write(x, x, torch.tensor([32, -1, -1, 2 ** 40], device=dev))
+    assert pkg.lib.o1_device_error() == 70
+    assert torch.equal(before, cache.k) and torch.equal(scales, cache.k_scale)
+    k, _ = cache.read(torch.tensor([32], device=dev))
+    assert (k == 0).all() and pkg.lib.o1_device_error() == 70
+
+
+# ------------------------------------------------------------------ the other kinds' tests, over these rows
+@gpu
+@pytest.mark.parametrize("kv_heads,group,page", [(8, 4, 16), (1, 1, 16), (2, 8, 64), (3, 3, 48), (2, 7, 32), (1, 16, 128), (2, 12, 16), (1, 24, 64), (1, 33, 16), (16, 1, 32),
+                                                 (8, 4, 64), (4, 2, 96)])
+def test_attention_of_ragged_sequences(pkg, dev, kv_heads, group, page):
+    base.test_attention_of_ragged_sequences(pkg, dev, "uint4", kv_heads, group, page)
+
+
+@gpu
+@pytest.mark.parametrize("lens,kv_heads,group", [([1], 1, 1), ([1], 8, 4), ([85], 8, 4), ([4097], 8, 4), ([30011], 1, 8), ([30011], 2, 16), ([9001, 1, 0, 12000, 3], 2, 4),
+                                                 ([700] * 40, 1, 4), ([0, 0, 0], 2, 2), ([257] * 300, 1, 2), ([1] * 700 + [5000], 1, 1)])
+def test_attention_over_few_and_many_rows(pkg, dev, lens, kv_heads, group):
+    base.test_attention_over_few_and_many_rows(pkg, dev, "uint4", lens, kv_heads, group)
+
+
+@gpu
+@pytest.mark.parametrize("lens,kv_heads,group,page", [([1, 16, 17, 0, 33, 128, 2, 129], 8, 4, 16), ([1], 8, 4, 64), ([20000], 2, 4, 64), ([5, 700, 1300], 1, 24, 48),
+                                                      ([3] * 90, 4, 1, 16), ([64, 65, 63, 127, 128, 49], 2, 4, 32), ([64, 65, 63, 127, 128, 49], 2, 16, 128)])
+def test_new_rows_appended_by_the_same_call(pkg, dev, lens, kv_heads, group, page):
+    base.test_new_rows_appended_by_the_same_call(pkg, dev, "uint4", lens, kv_heads, group, page)
+
+
+@gpu
+@pytest.mark.parametrize("batch,kv_heads,group,page,most", base.MANY)
+def test_many_short_sequences(pkg, dev, batch, kv_heads, group, page, most):
+    base.test_many_short_sequences(pkg, dev, "uint4", batch, kv_heads, group, page, most)
+
+
+@gpu
+@pytest.mark.parametrize("batch,kv_heads,group,page,most", [(300, 4, 4, 16, 90), (230, 2, 16, 32, 33), (470, 1, 1, 48, 48)])
+def test_many_short_sequences_with_new_rows(pkg, dev, batch, kv_heads, group, page, most):
+    base.test_many_short_sequences_with_new_rows(pkg, dev, "uint4", batch, kv_heads, group, page, most)
+
+
+@gpu
+def test_scores_of_any_size(pkg, dev):
+    base.test_scores_of_any_size(pkg, dev, "uint4")
+
+
+@gpu
+def test_not_finite_rows_stay_where_they_are(pkg, dev):
+    base.test_not_finite_rows_stay_where_they_are(pkg, dev, "uint4")
+
+
+@gpu
+@pytest.mark.parametrize("rows", [3, 3000])
+def test_nothing_is_written_after_a_failure(pkg, dev, rows):
+    base.test_nothing_is_written_after_a_failure(pkg, dev, "uint4", rows)
+
+
+@gpu
+@pytest.mark.parametrize("lens,heads", [([40, 700, 3], 4), ([20000], 8), ([1 + i % 20 for i in range(250)], 2)])
+def test_no_row_is_appended_after_a_failure(pkg, dev, lens, heads):
+    base.test_no_row_is_appended_after_a_failure(pkg, dev, "uint4", lens, heads)
+
+
+@gpu
+@pytest.mark.parametrize("big", [14, 24])
+def test_queries_with_one_large_channel(pkg, dev, big):
+    base.test_queries_with_one_large_channel(pkg, dev, "uint4", big)
+
+
+@gpu
+@pytest.mark.parametrize("lens", [[600, 17, 90, 2500, 33, 1, 300, 600], [600] * 32])
+def test_a_sequence_alone_and_among_others(pkg, dev, lens):
+    base.test_a_sequence_alone_and_among_others(pkg, dev, "uint4", lens)
+
+
+# ------------------------------------------------------------------ what four bits add
+@gpu
+@pytest.mark.parametrize("group", [1, 4, 5, 8, 16])
+def test_values_of_very_different_sizes(pkg, dev, group):
+    """Values of 2^-90 to 2^90 from row to row: rows that count for nothing take no bits from those that count, whichever come first."""
+    lens = [700, 700, 65, 900]
+    c = Case4(pkg, dev, "uint4", lens, 2, 32, seed=5, std=6.0)
+    for b, n in enumerate(lens):
+        size = torch.linspace(-90, 90, n).flip(0) if b % 2 else torch.linspace(-90, 90, n)
+        c.v[b] = (c.v[b].double() * torch.exp2(size[:, None, None].double())).to(torch.bfloat16)
+    c.v[3][::2] = 0.0
+    c.fill()
+    q = normal((4, 2 * group, D), gen(3), 4.0)
+    out, lse = c.cache.attend(q.to(dev), c.dtable, c.dlens, lse=True)
+    c.check(q, out, lse)
+
+
+@gpu
+@pytest.mark.parametrize("group", [2, 8, 12])
+def test_rows_far_from_zero_and_constant_rows(pkg, dev, group):
+    """Values to one side of zero, rows of one value (no codes), rows of zeros."""
+    lens = [130, 1, 64, 300]
+    c = Case4(pkg, dev, "uint4", lens, 1, 16, seed=6)
+    c.v[0], c.k[0] = c.v[0] + 50.0, c.k[0] - 3.0
+    c.v[1][:], c.k[1][:] = -2.5, 0.75
+    c.v[2][:] = 0.0
+    c.v[3][::3], c.k[3][1::3] = 9.0, 0.0
+    c.fill()
+    q = normal((4, group, D), gen(3), 0.5)
+    out, lse = c.cache.attend(q.to(dev), c.dtable, c.dlens, lse=True)
+    c.check(q, out, lse)
+
+
+@gpu
+def test_offsets_past_32_bits(pkg, dev):
+    """A cache of more than 2^32 bytes of codes, with rows at its end."""
+    heads, page = 8, 128
+    pages = 2 ** 33 // (heads * page * D) + 40
+    cache = pkg.KvCache(pages, page, "uint4", heads, dev)
+    c = Case4(pkg, dev, "uint4", [300, 128], heads, page, width_extra=0)
+    c.cache = cache
+    c.table += pages - 10
+    c.table[c.table >= pages] = 0
+    c.dtable = c.table.to(dev)
+    c.fill()
+    k, _ = cache.read(c.slots(0).to(dev))
+    assert torch.equal(k.cpu().double(), value(*kept(c.k[0])).to(torch.bfloat16).double())
+    q = normal((2, 32, D), gen(3))
+    c.check(q, c.cache.attend(q.to(dev), c.dtable, c.dlens))
+
+
+@gpu
+def test_streams_graphs_and_wrong_tables(pkg, dev):
+    lens = [3000, 17, 900]
+    c = Case4(pkg, dev, "uint4", lens, 4, 32)
+    c.fill()
+    q = normal((3, 16, D), gen(3)).to(dev)
+    want = c.cache.attend(q, c.dtable, c.dlens)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    try:
+        for _ in range(6):
+            for s in streams:
+                with torch.cuda.stream(s):
+                    pkg.use_torch_stream()
+                    outs.append(c.cache.attend(q, c.dtable, c.dlens))
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
+        ln, out = c.dlens.clone(), torch.empty_like(want)
+        with torch.cuda.stream(streams[0]):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=streams[0]):
+                pkg.use_torch_stream()
+                c.cache.attend(q, c.dtable, ln, out=out)
+        ln.copy_(torch.tensor([100, 0, 33], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+    finally:
+        pkg.use_torch_stream()
+    assert torch.equal(out, c.cache.attend(q, c.dtable, ln))
+    for page in (c.cache.pages, -1, 2 ** 31 - 1, -2 ** 31):
+        t = c.dtable.clone()
+        t[0, 1] = page
+        got = c.cache.attend(q, t, c.dlens)
+        assert pkg.lib.o1_device_error() == 70 and torch.equal(got[1:], want[1:])
+    new, before = normal((3, 4, D), gen(2)).to(dev), c.cache.k.clone()
+    for n in (-1, 32 * c.table.shape[1] + 1, 2 ** 31 - 1, -2 ** 31):
+        bad = c.dlens.clone()
+        bad[0] = n
+        got = c.cache.attend(q, c.dtable, bad)
+        assert pkg.lib.o1_device_error() == 71 and torch.equal(got[1:], want[1:]) and (got[0] == 0).all()
+    bad = torch.tensor([-3, 2 ** 30, 0], dtype=torch.int32, device=dev)
+    c.cache.attend(q, c.dtable, bad, k=new, v=new)
+    assert pkg.lib.o1_device_error() == 71 and torch.equal(before, c.cache.k)
+
+
+@gpu
+def test_arguments_that_do_not_fit(pkg, dev):
+    E = pkg.O1Error
+    c = pkg.KvCache(4, 16, "uint4", 2, dev)
+    assert c.k.shape == (4, 2, 16, 64) and c.k_scale.shape == (4, 2, 16, 2) and c.k_scale.dtype is torch.bfloat16
+    same = pkg.KvCache.over(c.k, c.v, c.k_scale, c.v_scale)
+    assert same.c.type == 4
+    for args in ((c.k, c.v), (c.k, c.v, c.k_scale[..., 0], c.v_scale), (c.k, c.v, c.k_scale.float(), c.v_scale)):
+        with pytest.raises(E, match="scales"):
+            pkg.KvCache.over(*args)
+    with pytest.raises(E, match="wanted"):
+        pkg.KvCache.over(c.k[..., :32].contiguous(), c.v[..., :32].contiguous(), c.k_scale, c.v_scale)
+    wide = torch.zeros(4, 2, 16, 128, dtype=torch.uint8, device=dev)
+    with pytest.raises(E, match="wanted"):
+        pkg.KvCache.over(wide, wide, c.k_scale, c.v_scale)
+    with pytest.raises(E, match="multiple of 16"):
+        pkg.KvCache(4, 24, "uint4", 2, dev)
+    x, s = normal((3, 2, D), gen(0)).to(dev), torch.arange(3, device=dev)
+    for bad in (x.float(), x[:, :1], x[..., :64], x.cpu()):
+        with pytest.raises(E, match="KvCache.write"):
+            c.write(bad, x, s)
+
+
+def test_entry_points_refuse_before_they_touch_the_gpu(pkg):
+    K, one = pkg.KvCacheC, C.c_void_p(4096)
+    good = dict(k=4096, v=4096, k_scale=4096, v_scale=4096, type=4, pages=4, page_size=16, kv_heads=2, head_dim=128)
+    for want, change in ((6, dict(k=None)), (6, dict(k_scale=None)), (6, dict(v_scale=None)), (9, dict(head_dim=64)), (9, dict(page_size=8)), (9, dict(v_scale=4100)), (9, dict(type=5))):
+        assert pkg.lib.o1_kv_write(C.byref(K(**{**good, **change})), one, 256, one, 256, one, 1) == want, change
+        assert b"kv_write" in pkg.lib.hd_cuda_last_error()
+    pkg.lib.hd_cuda_clear_error()
