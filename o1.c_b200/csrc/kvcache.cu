@@ -440,6 +440,16 @@ __device__ __forceinline__ float lds_f32(uint32_t a) {
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
     return v;
 }
+__device__ __forceinline__ uint32_t lds_u32(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+    return v;
+}
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
@@ -452,13 +462,21 @@ __device__ __forceinline__ void team_sync(int team) { asm volatile("bar.sync %0,
 // Of eight: 0 2 4 6 1 3 5 7's inverse.  Rows kv_perm(2m) and kv_perm(2m + 1) lie four apart, as the swizzle wants them.
 __device__ __forceinline__ int kv_perm(int i) { return (i >> 1) | (i & 1) << 2; }
 
+// Rows of 64 bytes, two to a swizzled line of 128: of eight, 0 3 1 2 4 7 5 6.  Neighbours n = 2m, 2m + 1 (a step of the keys' loads) lie in different halves of their lines, and so do
+// two each of the four rows at even or odd n (a step of the values' loads), in lines whose swizzles differ: no bank is met twice.
+__device__ __forceinline__ int kv4_even(int m) { return (m & 1) | (m & 2) << 1; }            // of n = 2m; n = 2m + 1: the same ^ 3
+__device__ __forceinline__ int kv4_key(int n) { return kv4_even(n >> 1) ^ (n & 1 ? 3 : 0); }
+
 template <int TYPE, int HG>
 struct KvKernel {
-    static constexpr int KEYS = TYPE == KV_BF16 ? 16 : 32, ROWB = TYPE == KV_BF16 ? 256 : 128, TILES = KEYS / 8;
+    static constexpr int KEYS = TYPE == KV_BF16 ? 16 : TYPE == KV_UINT4 ? 64 : 32, TILES = KEYS / 8;
     static constexpr int TEAMS = HG == 1 ? 3 : 2, WARPS = KV_TEAM * TEAMS, STAGES = HG == 1 ? 2 : 3, THREADS = (WARPS + TEAMS) * 32;
     // (HG == 1: 128 registers and 24 slots of 8 KB; HG == 2 holds twice the queries and sums: 168 registers, two teams, again 24 slots)
     // shared memory: the rings, their scales, the teams' join buffers, then Shared
-    static constexpr int SCALES = WARPS * STAGES * KV_STAGE_BYTES, JOIN = SCALES + (TYPE == KV_BF16 ? 0 : WARPS * STAGES * 256), SHARED = JOIN + TEAMS * KV_JOIN_BYTES;
+    static constexpr int SCALE_BYTES = TYPE == KV_BF16 ? 0 : 2 * KEYS * 4, PLACES = KEYS < 32 ? 2 : KEYS / 16;      // of a slot; 16 rows to a place
+    // (four bits have twice the scales, and where there are three teams half the room to join in)
+    static constexpr int JOIN_BYTES = TYPE == KV_UINT4 && HG == 1 ? KV_JOIN_BYTES / 2 : KV_JOIN_BYTES;
+    static constexpr int SCALES = WARPS * STAGES * KV_STAGE_BYTES, JOIN = SCALES + WARPS * STAGES * SCALE_BYTES, SHARED = JOIN + TEAMS * JOIN_BYTES;
     struct Share { int first, here, fan, item, groups, b, head0, heads; };        // a part's group begins at part `first` and has `here` (0: no part), its item at part `item`
     struct Segment { int b, item, first, begin, end, n; };        // first: the item's first chunk; begin ... end - 1: the team's
     struct Shared {
@@ -466,7 +484,7 @@ struct KvKernel {
         Segment seg[TEAMS][2];
         Share share[TEAMS][2];
         int prefix[KV_SEQS + 1], cost[KV_SEQS], len[KV_SEQS], last[TEAMS][2];      // chunks and costs before a sequence
-        int rows[WARPS][STAGES][2];       // where the cache has a chunk's rows, 16 at a time, if new ones may go there, else negative
+        int rows[WARPS][STAGES][PLACES];       // where the cache has a chunk's rows, 16 at a time, if new ones may go there, else negative
         int2 scan[WARPS + TEAMS];
         float m[TEAMS][KV_TEAM][8 * HG], l[TEAMS][KV_TEAM][8 * HG];
     };
@@ -683,7 +701,9 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         const int team = warp - WARPS, id = team * gridDim.x + blockIdx.x;
         // (solo: lane w has the part of warp w)
         const int by = solo ? 1 : KV_TEAM, at_end = begin_of((solo ? (team * KV_TEAM + (lane >> 1 & 3)) * gridDim.x + blockIdx.x : id) + (lane & 1));
-        int f = __shfl_sync(0xffffffffu, at_end, solo ? lane * 2 & 7 : 0), c1 = __shfl_sync(0xffffffffu, at_end, solo ? (lane * 2 & 7) + 1 : 1), place[2] = {-1, -1};
+        int f = __shfl_sync(0xffffffffu, at_end, solo ? lane * 2 & 7 : 0), c1 = __shfl_sync(0xffffffffu, at_end, solo ? (lane * 2 & 7) + 1 : 1), place[K::PLACES];
+#pragma unroll
+        for (int h = 0; h < K::PLACES; ++h) place[h] = -1;
         if (!solo) f += lane;
         if (lane >= KV_TEAM) c1 = 0;
         KvWalk at = {};
@@ -707,21 +727,47 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         for (int round = 0; ok; ++round) {
             unsigned left = __ballot_sync(0xffffffffu, f < c1);
             if (!left) break;
-            const int now[2] = {place[0], place[1]}, slot = round % STAGES;
+            const int slot = round % STAGES;
+            int now[K::PLACES];
+#pragma unroll
+            for (int h = 0; h < K::PLACES; ++h) now[h] = place[h];
             f += by;
             if (f < c1) { at.step(by, sh.prefix, items); look(); }
             for (; left && ok; left &= left - 1) {
-                const int mate = __ffs(left) - 1, w = team * KV_TEAM + mate, p0 = __shfl_sync(0xffffffffu, now[0], mate), p1 = KEYS == 32 ? __shfl_sync(0xffffffffu, now[1], mate) : -1;
+                const int mate = __ffs(left) - 1, w = team * KV_TEAM + mate, p0 = __shfl_sync(0xffffffffu, now[0], mate), p1 = KEYS >= 32 ? __shfl_sync(0xffffffffu, now[1], mate) : -1;
+                int p[K::PLACES];        // (four bits)
+                if (TYPE == KV_UINT4) {
+#pragma unroll
+                    for (int h = 0; h < K::PLACES; ++h) p[h] = __shfl_sync(0xffffffffu, now[h], mate);
+                }
                 uint64_t* const full = &sh.full[w][slot];
                 if (elect_one()) {
                     ok = mbar_wait(&sh.empty[w][slot], ((round / STAGES) & 1) ^ 1);
                     if (!ok) atomicExch(a.err, ERR_KV_WAIT);
                     else {
-                        if (a.kn) { sh.rows[w][slot][0] = failed ? -1 : p0; sh.rows[w][slot][1] = failed ? -1 : p1; }
+                        if (a.kn && TYPE == KV_UINT4) {
+#pragma unroll
+                            for (int h = 0; h < K::PLACES; ++h) sh.rows[w][slot][h] = failed ? -1 : p[h];
+                        } else if (a.kn) { sh.rows[w][slot][0] = failed ? -1 : p0; sh.rows[w][slot][1] = failed ? -1 : p1; }
                         const int r0 = max(p0, 0), r1 = p1 == -2 ? 0 : p1;       // (of a page outside, the cache's first rows are loaded)
                         uint8_t* const dst = smem + (w * STAGES + slot) * KV_STAGE_BYTES;
-                        const uint32_t scales = smem_u32(smem) + K::SCALES + (w * STAGES + slot) * 256;
-                        if (TYPE == KV_BF16) {
+                        const uint32_t scales = smem_u32(smem) + K::SCALES + (w * STAGES + slot) * K::SCALE_BYTES;
+                        if (TYPE == KV_UINT4) {       // (a line of 128 bytes has two rows)
+                            const int step = a.flags & 8 ? 4 : a.flags & 16 ? 2 : 1;        // places to a box
+                            int boxes = 0;
+#pragma unroll
+                            for (int h = 0; h < K::PLACES; ++h) boxes += h % step == 0 && p[h] != -1;
+                            mbar_expect_tx(full, boxes * step * (2048 + 128));
+#pragma unroll
+                            for (int h = 0; h < K::PLACES; ++h) {
+                                if (h % step != 0 || p[h] == -1) continue;
+                                const int r = max(p[h], 0);
+                                tma_load_2d(dst + h * 1024, &k_map, full, 0, r >> 1);
+                                tma_load_2d(dst + 4096 + h * 1024, &v_map, full, 0, r >> 1);
+                                bulk_load(scales + h * 64, a.c.ks + r, step * 64, full);
+                                bulk_load(scales + KEYS * 4 + h * 64, a.c.vs + r, step * 64, full);
+                            }
+                        } else if (TYPE == KV_BF16) {
                             mbar_expect_tx(full, 8192);
                             tma_load_2d(dst, &k_map, full, 0, r0);
                             tma_load_2d(dst + 2048, &k_map, full, 64, r0);
@@ -758,6 +804,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     }
 
     const int team = warp / KV_TEAM, mate = warp % KV_TEAM, g = lane >> 2, t = lane & 3, gp = kv_perm(g), id = team * gridDim.x + blockIdx.x;
+    const int key0 = kv4_even(t);
     // ---- sequences without rows
     for (int b = id; b < a.batch; b += gridDim.x * K::TEAMS) {
         if (sh.len[b] > 0) continue;
@@ -788,6 +835,13 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             const uint16_t* src = a.q + b * a.ldq + (head0 + row) * KV_D;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
+                if (TYPE == KV_UINT4) {       // columns 32 t + 8 i, ...: pairs four apart, as a word's halves have them
+                    const int at = t * 32 + i * 8;
+                    const uint4 v = !on ? make_uint4(0, 0, 0, 0) : (a.flags & 1) ? load8<true>(src + at) : load8<false>(src + at);
+                    qa[h][4 * i] = __byte_perm(v.x, v.z, 0x5410); qa[h][4 * i + 1] = __byte_perm(v.x, v.z, 0x7632);
+                    qa[h][4 * i + 2] = __byte_perm(v.y, v.w, 0x5410); qa[h][4 * i + 3] = __byte_perm(v.y, v.w, 0x7632);
+                    continue;
+                }
                 const int at = TYPE == KV_BF16 ? (4 * i + t) * 8 : (4 * (i >> 1) + t) * 16 + (i & 1) * 8;
                 const uint4 v = !on ? make_uint4(0, 0, 0, 0) : (a.flags & 1) ? load8<true>(src + at) : load8<false>(src + at);
                 qa[h][4 * i] = v.x; qa[h][4 * i + 1] = v.y; qa[h][4 * i + 2] = v.z; qa[h][4 * i + 3] = v.w;
@@ -826,7 +880,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             to = {first, min(fan, count - mine * fan), fan, 2 * from + late, (count + fan - 1) / fan, w.b, head_of(w.item), heads_of(w.item)};
         }
     }
-    float* const buf = reinterpret_cast<float*>(smem + K::JOIN + team * KV_JOIN_BYTES);
+    float* const buf = reinterpret_cast<float*>(smem + K::JOIN + team * K::JOIN_BYTES);
     const int by = solo ? 1 : KV_TEAM;
     int f = solo ? c0 : c0 + mate, slot = 0, parity = 0;
     bool ok = true;
@@ -835,10 +889,34 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         const typename K::Segment seg = segs[k & 1];
         if ((solo || mate == 0) && seg.end < c1) describe(seg.end, segs[(k + 1) & 1]);
         float z_scale[HG], acc[HG][8][4], m[HG], l[HG];
+        float q_sum[HG], offset[HG], most[HG];       // four bits: the queries' sums, sums of the least values, the largest weight
+        int k_up[HG];
 #pragma unroll
         for (int h = 0; h < HG; ++h) {
             z_scale[h] = a.scale * 1.4426950408889634f;
-            if (TYPE != KV_BF16) {
+            if (TYPE == KV_UINT4) {
+                uint32_t top = 0;
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    top = max(top, max(qa[h][i] & 0x7FFFu, (qa[h][i] >> 16) & 0x7FFFu));
+                    sum += bf16lo(qa[h][i]) + bf16hi(qa[h][i]);
+                }
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                // codes are 2^-133 of themselves (below): queries times 2^x, the largest one below 2^127
+                const int x = min(120, 253 - (int)max(top >> 7, 1u));
+                const float up = __uint_as_float((uint32_t)(127 + x) << 23), up16 = up * 0.0625f;
+                z_scale[h] = z_scale[h] * __uint_as_float((uint32_t)(127 + 70) << 23) * __uint_as_float((uint32_t)(127 + 63 - x) << 23);
+                q_sum[h] = sum * __uint_as_float((uint32_t)(127 + x - 70) << 23) * __uint_as_float((uint32_t)(127 - 63) << 23);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) qa[h][i] = pack_bf16x2(bf16lo(qa[h][i]) * (i & 1 ? up16 : up), bf16hi(qa[h][i]) * (i & 1 ? up16 : up));
+                offset[h] = 0.f;
+                most[h] = 0.f;
+                k_up[h] = 101;
+            } else if (TYPE != KV_BF16) {
                 uint32_t top = 0;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = max(top, max(qa[h][i] & 0x7FFFu, (qa[h][i] >> 16) & 0x7FFFu));
@@ -861,7 +939,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         int valid = sh.len[seg.b] - (f - seg.first) * KEYS;       // rows that the sequence has from the warp's chunk on
 #pragma unroll 1
         for (; f < seg.end; f += by, valid -= by * KEYS) {
-            const uint32_t st = smem_u32(smem) + (warp * STAGES + slot) * KV_STAGE_BYTES, scales = smem_u32(smem) + K::SCALES + (warp * STAGES + slot) * 256;
+            const uint32_t st = smem_u32(smem) + (warp * STAGES + slot) * KV_STAGE_BYTES, scales = smem_u32(smem) + K::SCALES + (warp * STAGES + slot) * K::SCALE_BYTES;
             const bool append = a.kn && valid <= KEYS;
             uint4 fresh = make_uint4(0, 0, 0, 0);
             if (append) {
@@ -877,7 +955,17 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 const int64_t at = (int64_t)row + (r & 15);
                 const uint32_t dst = st + (lane < 16 ? 0 : 4096) + r * 128;
                 uint8_t* const base = lane < 16 ? a.c.k : a.c.v;
-                if (TYPE == KV_BF16) {
+                if (TYPE == KV_UINT4) {
+                    uint32_t pair;
+                    const uint32_t codes = quantise8_4(fresh, pair);
+                    const int line = r >> 1;
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(st + (lane < 16 ? 0 : 4096) + line * 128 + ((((r & 1) * 4 + (part >> 2)) ^ (line & 7)) << 4) + (part & 3) * 4), "r"(codes) : "memory");
+                    if (part == 0) asm volatile("st.shared.b32 [%0], %1;" ::"r"(scales + (lane >> 4) * (KEYS * 4) + r * 4), "r"(pair) : "memory");
+                    if (store) {
+                        reinterpret_cast<uint32_t*>(base)[at * 16 + part] = codes;
+                        if (part == 0) reinterpret_cast<uint32_t*>(lane < 16 ? a.c.ks : a.c.vs)[at] = pair;
+                    }
+                } else if (TYPE == KV_BF16) {
                     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (part >> 3) * 2048 + (((part & 7) ^ (r & 7)) << 4)), "r"(fresh.x), "r"(fresh.y), "r"(fresh.z), "r"(fresh.w) : "memory");
                     if (store) reinterpret_cast<uint4*>(base)[at * 16 + part] = fresh;
                 } else {
@@ -896,6 +984,24 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 
             // scores of 8 keys a tile; a tile's column n is its key kv_perm(n), so keys t and t + 4 are this thread's
             float s[TILES][4];
+            if (TYPE == KV_UINT4) {
+                // A tile's column n is its key kv4_key(n): this thread's are key0 and key0 ^ 3.  A word has eight codes; those at bits 0 and 16, and 4 and 20 (and, eight bits on, the other
+                // four), are taken as they lie: as a pair of bf16 they are 2^-133 and 2^-129 times the code, exactly (subnormal, or of the first exponent, which has the same steps), and
+                // the product takes them as such.  Five instructions for eight codes; the queries make up for the powers of two.
+#pragma unroll
+                for (int n = 0; n < TILES; ++n) {
+                    s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+                    const int line = 4 * n + (kv4_key(g) >> 1);
+                    const uint4 k = lds128(st + line * 128 + ((((kv4_key(g) & 1) * 4 + t) ^ (line & 7)) << 4));
+                    const uint32_t w[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t w8 = w[j] >> 8;
+                        mma_bf16(s[n], qa[0][4 * j], HG == 2 ? qa[HG - 1][4 * j] : 0, qa[0][4 * j + 1], HG == 2 ? qa[HG - 1][4 * j + 1] : 0, w[j] & 0x000F000Fu, w[j] & 0x00F000F0u);
+                        mma_bf16(s[n], qa[0][4 * j + 2], HG == 2 ? qa[HG - 1][4 * j + 2] : 0, qa[0][4 * j + 3], HG == 2 ? qa[HG - 1][4 * j + 3] : 0, w8 & 0x000F000Fu, w8 & 0x00F000F0u);
+                    }
+                }
+            } else {
 #pragma unroll
             for (int n = 0; n < TILES; ++n) {
                 s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
@@ -918,8 +1024,26 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                     }
                 }
             }
+            }
             float vs[TILES][2];
-            if (TYPE != KV_BF16) {
+            uint32_t s_top = 0;          // four bits: the largest of the values' scales, as bits
+            if (TYPE == KV_UINT4) {
+#pragma unroll
+                for (int n = 0; n < TILES; ++n) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t pair = lds_u32(scales + (8 * n + (j ? key0 ^ 3 : key0)) * 4);
+#pragma unroll
+                        for (int h = 0; h < HG; ++h) s[n][2 * h + j] = __fmaf_rn(s[n][2 * h + j], bf16lo(pair), bf16hi(pair) * q_sum[h]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < KEYS / 32; ++i) {
+                    const uint32_t pair = lds_u32(scales + KEYS * 4 + (i * 32 + lane) * 4) & 0xFFFFu;
+                    if (i * 32 + lane < valid) s_top = max(s_top, pair);
+                }
+                s_top = __reduce_max_sync(0xffffffffu, s_top) << 16;
+            } else if (TYPE != KV_BF16) {
 #pragma unroll
                 for (int n = 0; n < TILES; ++n) {
 #pragma unroll
@@ -936,7 +1060,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 for (int n = 0; n < TILES; ++n) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        if (8 * n + 4 * j + t < valid) continue;
+                        if (8 * n + (TYPE == KV_UINT4 ? (j ? key0 ^ 3 : key0) : 4 * j + t) < valid) continue;
                         vs[n][j] = 0.f;
 #pragma unroll
                         for (int h = 0; h < HG; ++h) s[n][2 * h + j] = -INFINITY;
@@ -967,7 +1091,30 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                     for (int j = 0; j < 2; ++j) { s[n][2 * h + j] = exp2_fast(__fmaf_rn(s[n][2 * h + j], z_scale[h], -ref)); sum += s[n][2 * h + j]; }
                 }
                 l[h] = l[h] * alpha[h] + sum;
-                if (TYPE != KV_BF16) {
+                if (TYPE == KV_UINT4) {
+                    // Weights times 2^k: with codes of 2^-133 of themselves, the sums are of normal size where the largest weight so far (the product of a chunk's largest
+                    // probability and scale, at most) is between 2^90 and 2^112; weights of 2^-100 of that one are still there.
+                    most[h] = fmaxf(most[h] * alpha[h], exp2_fast(__fmaf_rn(top, z_scale[h], -ref)) * __uint_as_float(s_top));
+                    offset[h] *= alpha[h];
+                    const int e = (int)(__float_as_uint(most[h]) >> 23) - 127;
+                    if (e + k_up[h] < 90 || e + k_up[h] > 111) {
+                        const int k_new = min(min(max(101 - e, -27), 127), k_up[h] + 100);
+                        alpha[h] *= exp2_fast((float)(k_new - k_up[h]));
+                        moved = moved || k_new != k_up[h];
+                        k_up[h] = k_new;
+                    }
+                    const float up = __uint_as_float((uint32_t)(127 + k_up[h]) << 23);
+#pragma unroll
+                    for (int n = 0; n < TILES; ++n) {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            uint32_t pair = lds_u32(scales + KEYS * 4 + (8 * n + (j ? key0 ^ 3 : key0)) * 4);
+                            if (valid < KEYS && 8 * n + (j ? key0 ^ 3 : key0) >= valid) pair = 0;
+                            offset[h] = __fmaf_rn(s[n][2 * h + j], bf16hi(pair), offset[h]);
+                            s[n][2 * h + j] = s[n][2 * h + j] * bf16lo(pair) * up;
+                        }
+                    }
+                } else if (TYPE != KV_BF16) {
 #pragma unroll
                     for (int n = 0; n < TILES; ++n) { s[n][2 * h] *= vs[n][0]; s[n][2 * h + 1] *= vs[n][1]; }
                 }
@@ -991,6 +1138,26 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                         two_parts(s[2 * u + j][2 * h], s[2 * u + j][2 * h + 1], p_hi[h][j], p_lo[h][j]);
                         if (second) p_hi[h][j] = p_lo[h][j];
                     }
+                }
+                if (TYPE == KV_UINT4) {         // columns 16 g ... + 15 of four rows; a tile's rows g are even columns, g + 8 odd ones, which are 16 times as large
+                    uint2 x[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int row = u * 16 + (r >> 1) * 8 + (r & 1 ? key0 ^ 3 : key0), line = row >> 1;
+                        x[r] = lds64(st + 4096 + line * 128 + ((((row & 1) * 4 + (g >> 1)) ^ (line & 7)) << 4) + (g & 1) * 8);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint32_t w[4] = {j < 4 ? x[0].x : x[0].y, j < 4 ? x[1].x : x[1].y, j < 4 ? x[2].x : x[2].y, j < 4 ? x[3].x : x[3].y};
+                        uint32_t a = j & 2 ? prmt<0x7632>(w[0], w[1]) : prmt<0x5410>(w[0], w[1]), b = j & 2 ? prmt<0x7632>(w[2], w[3]) : prmt<0x5410>(w[2], w[3]);
+                        if (j & 1) { a >>= 8; b >>= 8; }
+#pragma unroll
+                        for (int h = 0; h < HG; ++h) {
+                            mma_bf16(acc[h][j], a & 0x000F000Fu, a & 0x00F000F0u, b & 0x000F000Fu, b & 0x00F000F0u, p_hi[h][0], p_hi[h][1]);
+                            if (!twice) mma_bf16(acc[h][j], a & 0x000F000Fu, a & 0x00F000F0u, b & 0x000F000Fu, b & 0x00F000F0u, p_lo[h][0], p_lo[h][1]);
+                        }
+                    }
+                    continue;
                 }
                 constexpr int PIECES = TYPE == KV_BF16 ? 2 : 1;
                 uint4 v[4][PIECES];
@@ -1061,8 +1228,31 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
         }
-        // a thread's accumulators, of heads 2t, 2t + 1 (and 8 + those): columns 64 half + 8 gp + tile of bf16, 16 gp + 8 half + tile of codes
-        auto column = [&](int quarter, int p) { return (TYPE == KV_BF16 ? 64 * (quarter >> 1) + 8 * p : 8 * (quarter >> 1) + 16 * p) + (quarter & 1) * 4; };
+        if (TYPE == KV_UINT4) {        // back to the weights' own size, and what the least values add to every column
+#pragma unroll
+            for (int h = 0; h < HG; ++h) {
+                offset[h] += __shfl_xor_sync(0xffffffffu, offset[h], 1);
+                offset[h] += __shfl_xor_sync(0xffffffffu, offset[h], 2);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float add = __shfl_sync(0xffffffffu, offset[h], 8 * t + 4 * c);
+                    const float down = __uint_as_float((uint32_t)(127 + 100 - __shfl_sync(0xffffffffu, k_up[h], 8 * t + 4 * c)) << 23);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        acc[h][j][c] = __fmaf_rn(acc[h][j][c] * 8589934592.0f, down, add);            // 2^33
+                        acc[h][j][c + 2] = __fmaf_rn(acc[h][j][c + 2] * 536870912.0f, down, add);     // 2^29
+                    }
+                }
+            }
+        }
+        // a thread's accumulators, of heads 2t, 2t + 1 (and 8 + those): columns 64 half + 8 gp + tile of bf16, 16 gp + 8 half + tile of codes of a byte, 16 g + 2 tile (+ 1) of four bits
+        auto four = [&](const float (&d)[8][4], int q, int j) {
+            if (TYPE == KV_UINT4) return make_float4(d[2 * q][j], d[2 * q][j + 2], d[2 * q + 1][j], d[2 * q + 1][j + 2]);
+            const int c = 2 * (q >> 1) + j, at = (q & 1) * 4;
+            return make_float4(d[at][c], d[at + 1][c], d[at + 2][c], d[at + 3][c]);
+        };
+        auto columns_of = [](int i) { return TYPE == KV_UINT4 ? i : kv_perm(i); };
+        auto column = [&](int quarter, int p) { return TYPE == KV_UINT4 ? 16 * p + 4 * quarter : (TYPE == KV_BF16 ? 64 * (quarter >> 1) + 8 * p : 8 * (quarter >> 1) + 16 * p) + (quarter & 1) * 4; };
         if (solo) {
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
@@ -1073,17 +1263,14 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                     const float inv = 1.0f / __shfl_sync(0xffffffffu, l[h], 8 * t + 4 * j);
                     if (head >= heads) continue;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int c = 2 * (q >> 1) + j, four = (q & 1) * 4;
-                        store_row4(a.out + seg.b * a.ldo + (head0 + head) * KV_D + column(q, gp), make_float4(acc[h][four][c], acc[h][four + 1][c], acc[h][four + 2][c], acc[h][four + 3][c]), inv, a.flags & 2);
-                    }
+                    for (int q = 0; q < 4; ++q) store_row4(a.out + seg.b * a.ldo + (head0 + head) * KV_D + column(q, columns_of(g)), four(acc[h], q, j), inv, a.flags & 2);
                 }
             }
             if (seg.end == c1) return;
             continue;
         }
         // ---- the warps' parts together, 32 columns at a time or as many as fit the team's buffer
-        const int log_q = heads <= 4 ? 2 : heads <= 8 ? 1 : 0, quarters = 1 << log_q;
+        const int log_q = (heads <= 4 ? 2 : heads <= 8 ? 1 : 0) - (K::JOIN_BYTES < KV_JOIN_BYTES ? 1 : 0), quarters = 1 << log_q;
 #pragma unroll
         for (int h = 0; h < HG; ++h)
             if (t == 0) { sh.m[team][mate][8 * h + g] = m[h]; sh.l[team][mate][8 * h + g] = l[h]; }
@@ -1097,10 +1284,8 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             for (int h = 0; h < HG; ++h) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const int head = 8 * h + 2 * t + j, c = 2 * (q >> 1) + j, four = (q & 1) * 4;
-                    if (head < heads)
-                        *reinterpret_cast<float4*>(buf + ((mate * heads + head) * quarters + at_q) * 32 + 4 * g) =
-                            make_float4(acc[h][four][c], acc[h][four + 1][c], acc[h][four + 2][c], acc[h][four + 3][c]);
+                    const int head = 8 * h + 2 * t + j;
+                    if (head < heads) *reinterpret_cast<float4*>(buf + ((mate * heads + head) * quarters + at_q) * 32 + 4 * g) = four(acc[h], q, j);
                 }
             }
             if (at_q + 1 < quarters) continue;
@@ -1118,7 +1303,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 o.x += x.x * e; o.y += x.y * e; o.z += x.z * e; o.w += x.w * e;
                 sum += sh.l[team][w][head] * e;
             }
-            const int quarter = q - quarters + 1 + qq, col = column(quarter, kv_perm(at));
+            const int quarter = q - quarters + 1 + qq, col = column(quarter, columns_of(at));
             const bool one = at == 0 && quarter == 0;
             if (whole) {
                 store_row4(a.out + seg.b * a.ldo + (head0 + head) * KV_D + col, o, 1.0f / sum, a.flags & 2);
@@ -1172,44 +1357,6 @@ static cudaError_t launch_attention(const CUtensorMap& k_map, const CUtensorMap&
     // (Chosen on the device instead, by the lengths, it cost all other calls 0.4 us: one kernel with both.)
     if (items > teams && item_chunks <= KV_SOLO && item_chunks * teams <= KV_TEAM * items) return launch_attention<TYPE, HG, true>(k_map, v_map, a, most, st);
     return launch_attention<TYPE, HG, false>(k_map, v_map, a, (int)max((int64_t)1, min((int64_t)most, max((item_chunks * items + KV_TEAM - 1) / KV_TEAM, items))), st);
-}
-
-// Over codes of four bits, a warp to a query head of a sequence, four columns to a lane.
-__global__ void kv_append4_kernel(const KvAttn a) {
-    const int b = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, len = a.lens[b];
-    if (head >= a.c.heads || len <= 0 || len > (int64_t)a.width * a.c.page_size || error_word(a.err)) return;
-    const int page = a.pages[b * a.ldp + (len - 1) / a.c.page_size];
-    if ((unsigned)page >= (unsigned)a.c.pages) return;
-    const int64_t at = ((int64_t)page * a.c.heads + head) * a.c.page_size + (len - 1) % a.c.page_size;
-    uint32_t pair;
-    const uint4 x = load8<false>((lane < 16 ? a.kn + b * a.ldk : a.vn + b * a.ldv) + head * KV_D + (lane & 15) * 8);
-    const uint32_t codes = quantise8_4(x, pair);
-    reinterpret_cast<uint32_t*>(lane < 16 ? a.c.k : a.c.v)[at * 16 + (lane & 15)] = codes;
-    if ((lane & 15) == 0) reinterpret_cast<uint32_t*>(lane < 16 ? a.c.ks : a.c.vs)[at] = pair;
-}
-__global__ void kv_attention4_kernel(const KvAttn a) {
-    const int b = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (head >= a.heads) return;
-    int len = a.lens[b];
-    if (len < 0 || len > (int64_t)a.width * a.c.page_size) { atomicExch(a.bad, ERR_KV_LENGTH); len = 0; }
-    float q[4], o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0.f;
-    for (int i = 0; i < 4; ++i) q[i] = bf16_to_f32(a.q[b * a.ldq + head * KV_D + 4 * lane + i]) * a.scale;
-    for (int t = 0; t < len; ++t) {
-        const int page = a.pages[b * a.ldp + t / a.c.page_size];
-        if ((unsigned)page >= (unsigned)a.c.pages) { atomicExch(a.bad, ERR_KV_PLACE); break; }
-        const int64_t at = ((int64_t)page * a.c.heads + head / a.group) * a.c.page_size + t % a.c.page_size;
-        const uint32_t kp = reinterpret_cast<const uint32_t*>(a.c.ks)[at], vp = reinterpret_cast<const uint32_t*>(a.c.vs)[at];
-        const uint32_t kc = reinterpret_cast<const uint16_t*>(a.c.k)[at * 32 + lane], vc = reinterpret_cast<const uint16_t*>(a.c.v)[at * 32 + lane];
-        float z = 0.f;
-        for (int i = 0; i < 4; ++i) z += q[i] * (bf16hi(kp) + (float)((kc >> (4 * i)) & 15) * bf16lo(kp));
-        for (int s = 16; s > 0; s >>= 1) z += __shfl_xor_sync(0xffffffffu, z, s);
-        const float top = fmaxf(m, z), alpha = m == -INFINITY ? 0.f : expf(m - top), p = expf(z - top);
-        l = l * alpha + p;
-        for (int i = 0; i < 4; ++i) o[i] = o[i] * alpha + p * (bf16hi(vp) + (float)((vc >> (4 * i)) & 15) * bf16lo(vp));
-        m = z != z ? z : top;
-    }
-    for (int i = 0; i < 4; ++i) a.out[b * a.ldo + head * KV_D + 4 * lane + i] = f32_to_bf16(l > 0.f || l != l ? o[i] / l : 0.f);
-    if (a.lse && lane == 0) a.lse[(int64_t)b * a.heads + head] = m + logf(l);
 }
 
 static bool aligned16(const void* p, int64_t ld) { return (((uintptr_t)p) & 15) == 0 && (ld & 7) == 0; }
@@ -1321,7 +1468,7 @@ hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, 
     if (ldq < qrow || ldo < qrow || ldp < width || (k_new && (ldk < krow || ldv < krow))) { set_error("kv_attention: a row pitch is below the row"); return HD_ERR_UNSUPPORTED; }
     if (!(scale > 0.f) || scale > 3.0e38f) { set_error("kv_attention: scale %g", scale); return HD_ERR_UNSUPPORTED; }
     if (workspace_bytes < o1_kv_attention_workspace_bytes(heads, c.heads) || (((uintptr_t)workspace) & 15)) { set_error("kv_attention: workspace too small or unaligned"); return HD_ERR_OOM; }
-    const int group = heads / c.heads, hg = group <= 8 ? 1 : 2, of_heads = (group + 8 * hg - 1) / (8 * hg), keys = cache->type == O1_KV_BF16 ? 16 : 32;
+    const int group = heads / c.heads, hg = group <= 8 ? 1 : 2, of_heads = (group + 8 * hg - 1) / (8 * hg), keys = cache->type == O1_KV_BF16 ? 16 : cache->type == O1_KV_UINT4 ? 64 : 32;
     // the stream's index and costs are ints: fewer sequences a launch where the table allows for more, and a limit of items of a sequence
     const int64_t item_chunks = ((int64_t)width * c.page_size + keys - 1) / keys, each = item_chunks * c.heads * of_heads;
     if ((int64_t)width * c.page_size > INT32_MAX - 64 || each > (1 << 30) || (int64_t)c.heads * of_heads > (1 << 18) || (int64_t)c.pages * c.heads * c.page_size > INT32_MAX) { set_error("kv_attention: a table of %d pages of %d tokens for %d heads, or a cache of %d pages, is too large", width, c.page_size, heads, c.pages); return HD_ERR_UNSUPPORTED; }
@@ -1338,20 +1485,13 @@ hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, 
     a.err = device_error_word();
     a.bad = device_table_word();
     a.flags = (aligned16(q, ldq) ? 1 : 0) | (aligned16(out, ldo) ? 2 : 0) | (aligned16(k_new, ldk) && aligned16(v_new, ldv) ? 4 : 0);
-    if (cache->type == O1_KV_UINT4) {
-        a.batch = batch;
-        a.q = (const uint16_t*)q; a.kn = (const uint16_t*)k_new; a.vn = (const uint16_t*)v_new; a.pages = pages; a.lens = lens; a.out = (uint16_t*)out; a.lse = lse;
-        if (k_new) kv_append4_kernel<<<dim3(batch, (c.heads + 3) / 4), 128, 0, current_stream()>>>(a);
-        kv_attention4_kernel<<<dim3(batch, (heads + 3) / 4), 128, 0, current_stream()>>>(a);
-        o1_launch_count_add(k_new ? 2 : 1);
-        return launch_ok(cudaGetLastError(), "kv_attention") ? HD_OK : HD_ERR_RUNTIME;
-    }
-    // maps of the rows, 128 bytes (64 columns of bf16, all codes) x 16, or 32 where a chunk of codes never crosses a page
-    const bool wide = keys == 32 && c.page_size % 32 == 0;
-    if (wide) a.flags |= 8;
-    const uint64_t rows_all = (uint64_t)c.pages * c.heads * c.page_size, cols = cache->type == O1_KV_BF16 ? 128 : 64;
+    // maps of the rows, 128 bytes (64 columns of bf16, all codes of a byte, two rows of four bits) x 16 rows, or a chunk's where it never crosses a page
+    const bool four_bits = cache->type == O1_KV_UINT4, wide = keys >= 32 && c.page_size % keys == 0, half_wide = four_bits && !wide && c.page_size % 32 == 0;
+    a.flags |= wide ? 8 : half_wide ? 16 : 0;
+    const uint64_t rows_all = (uint64_t)c.pages * c.heads * c.page_size / (four_bits ? 2 : 1), cols = cache->type == O1_KV_BF16 ? 128 : 64;
+    const uint32_t box = four_bits ? (wide ? 32 : half_wide ? 16 : 8) : wide ? 32 : 16;
     CUtensorMap k_map, v_map;
-    if (!make_tmap_bf16(&k_map, c.k, rows_all, cols, cols, wide ? 32 : 16) || !make_tmap_bf16(&v_map, c.v, rows_all, cols, cols, wide ? 32 : 16)) return HD_ERR_RUNTIME;
+    if (!make_tmap_bf16(&k_map, c.k, rows_all, cols, cols, box) || !make_tmap_bf16(&v_map, c.v, rows_all, cols, cols, box)) return HD_ERR_RUNTIME;
     for (int b = 0; b < batch; b += step) {
         a.batch = min(step, batch - b);
         a.q = (const uint16_t*)q + b * ldq;
@@ -1365,6 +1505,7 @@ hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, 
         cudaError_t e;
         if (cache->type == O1_KV_BF16) e = hg == 1 ? launch_attention<KV_BF16, 1>(k_map, v_map, a, item_chunks, items, current_stream()) : launch_attention<KV_BF16, 2>(k_map, v_map, a, item_chunks, items, current_stream());
         else if (cache->type == O1_KV_FP8) e = hg == 1 ? launch_attention<KV_FP8, 1>(k_map, v_map, a, item_chunks, items, current_stream()) : launch_attention<KV_FP8, 2>(k_map, v_map, a, item_chunks, items, current_stream());
+        else if (four_bits) e = hg == 1 ? launch_attention<KV_UINT4, 1>(k_map, v_map, a, item_chunks, items, current_stream()) : launch_attention<KV_UINT4, 2>(k_map, v_map, a, item_chunks, items, current_stream());
         else e = hg == 1 ? launch_attention<KV_INT8, 1>(k_map, v_map, a, item_chunks, items, current_stream()) : launch_attention<KV_INT8, 2>(k_map, v_map, a, item_chunks, items, current_stream());
         if (!launch_ok(e, "kv_attention")) return HD_ERR_RUNTIME;
         o1_launch_count_add(1);
