@@ -382,6 +382,17 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The product alone, nothing added.
+__device__ __forceinline__ void mma_bf16_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// An 8 x 8 matrix of two-byte values, two of a row to a thread, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
 template <int TYPE>
 __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     if (TYPE == KV_BF16) mma_bf16(d, a0, a1, a2, a3, b0, b1);
@@ -625,6 +636,264 @@ __device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, 
     }
 }
 
+// A warp's part of an item over rows of four bits: z_t = s_t (q . c_t) + b_t (sum of q), out = sum p_t s_t c_t + sum p_t b_t, with codes c_t, scales s_t and least values b_t.
+//
+//  * A word has eight codes. Those at bits 0 and 16, or 4 and 20 (or, eight bits on, the other four), are taken as they lie: as a pair of bf16 they are 2^-133 or 2^-129 times
+//    the code, exactly (subnormal, or of the first exponent, whose steps are the same), and the tensor cores multiply them as that. So eight codes of keys take five
+//    instructions, of values six with the pairing of two rows; powers of two in queries and weights make up for them.
+//  * Keys are the rows of the first product's tiles and heads their columns, so a thread has few keys' scales to fetch (8 of 64, for two heads each); movmatrix brings the
+//    probabilities to where the second product wants them.  Up to four heads are there twice: a column and the one four on have the same scores, and each thread does half of the
+//    keys and gives the other its results, one the values and one the rests.
+//  * Weights p_t s_t are held times 2^k: the sums, of codes 2^-133 of themselves, are of normal size where the largest weight so far (a chunk's largest probability times its largest
+//    scale bounds it) is between 2^90 and 2^112, and weights of 2^-80 of that one are still there.  Largest weight and k follow the running maximum, and k moves seldom.
+template <int HG>
+struct KvFour {
+    float zs[HG][2], q_sum[HG][2], m[HG][2], l[HG][2], offset[HG][2], most[HG][2];       // of heads 8 h + 2 t, 2 t + 1
+    int k[HG][2];
+
+    __device__ __forceinline__ void begin(uint32_t (&q)[HG][16], float scale, float (&acc)[HG][8][4]) {
+        const int t = threadIdx.x & 3;
+#pragma unroll
+        for (int h = 0; h < HG; ++h) {
+            uint32_t top = 0;
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                top = max(top, max(q[h][i] & 0x7FFFu, (q[h][i] >> 16) & 0x7FFFu));
+                sum += bf16lo(q[h][i]) + bf16hi(q[h][i]);
+            }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            // queries times 2^x, the largest one below 2^127
+            const int x = min(120, 253 - (int)max(top >> 7, 1u));
+            const float up = __uint_as_float((uint32_t)(127 + x) << 23), up16 = up * 0.0625f;
+            const float z = scale * __uint_as_float((uint32_t)(127 + 70) << 23) * __uint_as_float((uint32_t)(127 + 63 - x) << 23);
+            sum = sum * __uint_as_float((uint32_t)(127 + x - 70) << 23) * __uint_as_float((uint32_t)(127 - 63) << 23);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) q[h][i] = pack_bf16x2(bf16lo(q[h][i]) * (i & 1 ? up16 : up), bf16hi(q[h][i]) * (i & 1 ? up16 : up));
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                zs[h][c] = __shfl_sync(0xffffffffu, z, 8 * t + 4 * c);
+                q_sum[h][c] = __shfl_sync(0xffffffffu, sum, 8 * t + 4 * c);
+                m[h][c] = -INFINITY;
+                l[h][c] = offset[h][c] = most[h][c] = 0.f;
+                k[h][c] = 101;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[h][j][0] = acc[h][j][1] = acc[h][j][2] = acc[h][j][3] = 0.f;
+        }
+    }
+
+    // 64 rows in shared memory at st (keys, then values), of which `valid` are there.  In tiles of 8, row n is the tile's key kv4_key(n).
+    __device__ __forceinline__ void chunk(uint32_t st, uint32_t scales, int valid, bool twice, const uint32_t (&q)[HG][16], float (&acc)[HG][8][4]) {
+        if (HG == 1 && twice) part<true>(st, scales, valid, q, acc);
+        else part<false>(st, scales, valid, q, acc);
+    }
+    template <bool TWICE>
+    __device__ __forceinline__ void part(uint32_t st, uint32_t scales, int valid, const uint32_t (&q)[HG][16], float (&acc)[HG][8][4]) {
+        constexpr int KEYS = 64, MINE = TWICE ? 2 : 4;       // tiles of 16 keys that are this thread's
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, mine = kv4_key(g), key0 = kv4_even(t);
+        const bool upper = t & 2;
+        float s[4][HG][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint4 x[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int line = 8 * i + 4 * r + (mine >> 1);
+                x[r] = lds128(st + line * 128 + ((((mine & 1) * 4 + t) ^ (line & 7)) << 4));
+            }
+            const uint32_t w[4][2] = {{x[0].x, x[1].x}, {x[0].y, x[1].y}, {x[0].z, x[1].z}, {x[0].w, x[1].w}};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                constexpr uint32_t A = 0x000F000Fu, B = 0x00F000F0u;
+                const uint32_t x8 = w[j][0] >> 8, y8 = w[j][1] >> 8;
+#pragma unroll
+                for (int h = 0; h < HG; ++h) {
+                    if (j == 0) mma_bf16_new(s[i][h], w[j][0] & A, w[j][1] & A, w[j][0] & B, w[j][1] & B, q[h][4 * j], q[h][4 * j + 1]);
+                    else mma_bf16(s[i][h], w[j][0] & A, w[j][1] & A, w[j][0] & B, w[j][1] & B, q[h][4 * j], q[h][4 * j + 1]);
+                    mma_bf16(s[i][h], x8 & A, y8 & A, x8 & B, y8 & B, q[h][4 * j + 2], q[h][4 * j + 3]);
+                }
+            }
+        }
+        if (TWICE) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s[i][0][c] = upper ? s[i + 2][0][c] : s[i][0][c];
+            }
+        }
+        const int first = mine + (TWICE && upper ? 32 : 0);        // this thread's keys: first + 8 n
+        const uint32_t pairs = scales + first * 4;
+#pragma unroll
+        for (int n = 0; n < 2 * MINE; ++n) {
+            const uint32_t pair = lds_u32(pairs + n * 32);
+#pragma unroll
+            for (int h = 0; h < HG; ++h) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float& z = s[n >> 1][h][2 * (n & 1) + c];
+                    z = __fmaf_rn(z, bf16lo(pair), bf16hi(pair) * q_sum[h][c]);
+                }
+            }
+        }
+        uint32_t s_top = 0;           // the largest of the values' scales, as bits
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t pair = lds_u32(scales + KEYS * 4 + (i * 32 + lane) * 4) & 0xFFFFu;
+            if (i * 32 + lane < valid) s_top = max(s_top, pair);
+        }
+        s_top = __reduce_max_sync(0xffffffffu, s_top) << 16;
+        if (valid < KEYS) {
+#pragma unroll
+            for (int n = 0; n < 2 * MINE; ++n) {
+                if (first + 8 * n < valid) continue;
+#pragma unroll
+                for (int h = 0; h < HG; ++h) s[n >> 1][h][2 * (n & 1)] = s[n >> 1][h][2 * (n & 1) + 1] = -INFINITY;
+            }
+        }
+        bool moved = false;
+        float alpha[HG][2];
+#pragma unroll
+        for (int h = 0; h < HG; ++h) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < 2 * MINE; ++n) top = fmaxf(top, s[n >> 1][h][2 * (n & 1) + c]);
+#pragma unroll
+                for (int o = TWICE ? 2 : 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const float m_new = fmaxf(m[h][c], top * zs[h][c]), ref = (m_new == -INFINITY ? 0.f : m_new) - KV_LIFT;
+                float a = exp2_fast(m[h][c] - KV_LIFT - ref);
+                m[h][c] = m_new;
+                float sum = 0.f;
+#pragma unroll
+                for (int n = 0; n < 2 * MINE; ++n) {
+                    float& z = s[n >> 1][h][2 * (n & 1) + c];
+                    z = exp2_fast(__fmaf_rn(z, zs[h][c], -ref));
+                    sum += z;
+                }
+                l[h][c] = l[h][c] * a + sum;
+                offset[h][c] *= a;
+                most[h][c] = fmaxf(most[h][c] * a, exp2_fast(__fmaf_rn(top, zs[h][c], -ref)) * __uint_as_float(s_top));
+                const int e = (int)(__float_as_uint(most[h][c]) >> 23) - 127;
+                if ((unsigned)(e + k[h][c] - 90) > 21u) {
+                    const int k_new = min(min(max(101 - e, -27), 127), k[h][c] + 100);
+                    a *= exp2_fast((float)(k_new - k[h][c]));
+                    k[h][c] = k_new;
+                }
+                moved = moved || a != 1.f;
+                alpha[h][c] = a;
+            }
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int h = 0; h < HG; ++h) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { acc[h][j][0] *= alpha[h][0]; acc[h][j][1] *= alpha[h][1]; acc[h][j][2] *= alpha[h][0]; acc[h][j][3] *= alpha[h][1]; }
+            }
+        }
+        // weights, in two parts of bf16; [tile of 16 keys][its upper 8 keys]
+        float up[HG][2];
+#pragma unroll
+        for (int h = 0; h < HG; ++h) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) up[h][c] = __uint_as_float((uint32_t)(127 + k[h][c]) << 23);
+        }
+        uint32_t hi[4][HG][2], lo[4][HG][2];
+#pragma unroll
+        for (int n = 0; n < 2 * MINE; ++n) {
+            uint32_t pair = lds_u32(pairs + KEYS * 4 + n * 32);
+            if (first + 8 * n >= valid) pair = 0;             // what is behind a sequence may be NaN
+#pragma unroll
+            for (int h = 0; h < HG; ++h) {
+                float w[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float p = s[n >> 1][h][2 * (n & 1) + c];
+                    offset[h][c] = __fmaf_rn(p, bf16hi(pair), offset[h][c]);
+                    w[c] = p * bf16lo(pair) * up[h][c];
+                }
+                two_parts(w[0], w[1], hi[n >> 1][h][n & 1], lo[n >> 1][h][n & 1]);
+            }
+        }
+        if (TWICE) {            // heads in the lower columns' threads get the values, the others the rests
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const uint32_t other = __shfl_xor_sync(0xffffffffu, upper ? hi[i][0][r] : lo[i][0][r], 2);
+                    hi[i + 2][0][r] = upper ? lo[i][0][r] : other;
+                    hi[i][0][r] = upper ? other : hi[i][0][r];
+                }
+            }
+        }
+        // out^T += V^T P^T, 16 keys a step: columns 16 g ... + 15 of four rows; a tile's rows g are even columns, g + 8 odd ones, which are 16 times as large
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            uint2 x[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = u * 16 + (r >> 1) * 8 + (r & 1 ? key0 ^ 3 : key0), line = row >> 1;
+                x[r] = lds64(st + 4096 + line * 128 + ((((row & 1) * 4 + (g >> 1)) ^ (line & 7)) << 4) + (g & 1) * 8);
+            }
+#pragma unroll
+            for (int h = 0; h < HG; ++h) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    hi[u][h][r] = transposed(hi[u][h][r]);
+                    if (!TWICE) lo[u][h][r] = transposed(lo[u][h][r]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t w[4] = {j < 4 ? x[0].x : x[0].y, j < 4 ? x[1].x : x[1].y, j < 4 ? x[2].x : x[2].y, j < 4 ? x[3].x : x[3].y};
+                uint32_t a = j & 2 ? prmt<0x7632>(w[0], w[1]) : prmt<0x5410>(w[0], w[1]), b = j & 2 ? prmt<0x7632>(w[2], w[3]) : prmt<0x5410>(w[2], w[3]);
+                if (j & 1) { a >>= 8; b >>= 8; }
+#pragma unroll
+                for (int h = 0; h < HG; ++h) {
+                    mma_bf16(acc[h][j], a & 0x000F000Fu, a & 0x00F000F0u, b & 0x000F000Fu, b & 0x00F000F0u, hi[u][h][0], hi[u][h][1]);
+                    if (!TWICE) mma_bf16(acc[h][j], a & 0x000F000Fu, a & 0x00F000F0u, b & 0x000F000Fu, b & 0x00F000F0u, lo[u][h][0], lo[u][h][1]);
+                }
+            }
+        }
+    }
+
+    // The sums as the other kinds have them (those of `twice` are added by the caller): accumulators of the weights' own size with what the least values add to every
+    // column, maximum and sum of head g (and 8 + g).
+    __device__ __forceinline__ void end(bool twice, float (&acc)[HG][8][4], float (&m_out)[HG], float (&l_out)[HG]) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, from = (twice ? g & 3 : g) >> 1;
+#pragma unroll
+        for (int h = 0; h < HG; ++h) {
+            float m_of[2], l_of[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) {
+                    l[h][c] += __shfl_xor_sync(0xffffffffu, l[h][c], o);
+                    offset[h][c] += __shfl_xor_sync(0xffffffffu, offset[h][c], o);
+                }
+                if (twice) {
+                    l[h][c] += __shfl_xor_sync(0xffffffffu, l[h][c], 2);
+                    offset[h][c] += __shfl_xor_sync(0xffffffffu, offset[h][c], 2);
+                }
+                const float down = __uint_as_float((uint32_t)(127 + 100 - k[h][c]) << 23);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    acc[h][j][c] = __fmaf_rn(acc[h][j][c] * 8589934592.0f, down, offset[h][c]);            // 2^33
+                    acc[h][j][c + 2] = __fmaf_rn(acc[h][j][c + 2] * 536870912.0f, down, offset[h][c]);     // 2^29
+                }
+                m_of[c] = __shfl_sync(0xffffffffu, m[h][c], from);
+                l_of[c] = __shfl_sync(0xffffffffu, l[h][c], from);
+            }
+            m_out[h] = g & 1 ? m_of[1] : m_of[0];
+            l_out[h] = g & 1 ? l_of[1] : l_of[0];
+        }
+    }
+};
+
 // solo: items of at most KV_SOLO chunks, each to one warp; "teams" are then warps.
 template <int TYPE, int HG, bool solo>
 __global__ void __launch_bounds__(KvKernel<TYPE, HG>::THREADS, 1)
@@ -804,7 +1073,6 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     }
 
     const int team = warp / KV_TEAM, mate = warp % KV_TEAM, g = lane >> 2, t = lane & 3, gp = kv_perm(g), id = team * gridDim.x + blockIdx.x;
-    const int key0 = kv4_even(t);
     // ---- sequences without rows
     for (int b = id; b < a.batch; b += gridDim.x * K::TEAMS) {
         if (sh.len[b] > 0) continue;
@@ -889,34 +1157,13 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         const typename K::Segment seg = segs[k & 1];
         if ((solo || mate == 0) && seg.end < c1) describe(seg.end, segs[(k + 1) & 1]);
         float z_scale[HG], acc[HG][8][4], m[HG], l[HG];
-        float q_sum[HG], offset[HG], most[HG];       // four bits: the queries' sums, sums of the least values, the largest weight
-        int k_up[HG];
+        KvFour<HG> four;
+        if (TYPE == KV_UINT4) four.begin(qa, a.scale * 1.4426950408889634f, acc);
+        else
 #pragma unroll
         for (int h = 0; h < HG; ++h) {
             z_scale[h] = a.scale * 1.4426950408889634f;
-            if (TYPE == KV_UINT4) {
-                uint32_t top = 0;
-                float sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    top = max(top, max(qa[h][i] & 0x7FFFu, (qa[h][i] >> 16) & 0x7FFFu));
-                    sum += bf16lo(qa[h][i]) + bf16hi(qa[h][i]);
-                }
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                // codes are 2^-133 of themselves (below): queries times 2^x, the largest one below 2^127
-                const int x = min(120, 253 - (int)max(top >> 7, 1u));
-                const float up = __uint_as_float((uint32_t)(127 + x) << 23), up16 = up * 0.0625f;
-                z_scale[h] = z_scale[h] * __uint_as_float((uint32_t)(127 + 70) << 23) * __uint_as_float((uint32_t)(127 + 63 - x) << 23);
-                q_sum[h] = sum * __uint_as_float((uint32_t)(127 + x - 70) << 23) * __uint_as_float((uint32_t)(127 - 63) << 23);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) qa[h][i] = pack_bf16x2(bf16lo(qa[h][i]) * (i & 1 ? up16 : up), bf16hi(qa[h][i]) * (i & 1 ? up16 : up));
-                offset[h] = 0.f;
-                most[h] = 0.f;
-                k_up[h] = 101;
-            } else if (TYPE != KV_BF16) {
+            if (TYPE != KV_BF16) {
                 uint32_t top = 0;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = max(top, max(qa[h][i] & 0x7FFFu, (qa[h][i] >> 16) & 0x7FFFu));
@@ -982,26 +1229,10 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 __syncwarp();
             }
 
+            if constexpr (TYPE == KV_UINT4) four.chunk(st, scales, valid, twice, qa, acc);
+            else {
             // scores of 8 keys a tile; a tile's column n is its key kv_perm(n), so keys t and t + 4 are this thread's
             float s[TILES][4];
-            if (TYPE == KV_UINT4) {
-                // A tile's column n is its key kv4_key(n): this thread's are key0 and key0 ^ 3.  A word has eight codes; those at bits 0 and 16, and 4 and 20 (and, eight bits on, the other
-                // four), are taken as they lie: as a pair of bf16 they are 2^-133 and 2^-129 times the code, exactly (subnormal, or of the first exponent, which has the same steps), and
-                // the product takes them as such.  Five instructions for eight codes; the queries make up for the powers of two.
-#pragma unroll
-                for (int n = 0; n < TILES; ++n) {
-                    s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-                    const int line = 4 * n + (kv4_key(g) >> 1);
-                    const uint4 k = lds128(st + line * 128 + ((((kv4_key(g) & 1) * 4 + t) ^ (line & 7)) << 4));
-                    const uint32_t w[4] = {k.x, k.y, k.z, k.w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t w8 = w[j] >> 8;
-                        mma_bf16(s[n], qa[0][4 * j], HG == 2 ? qa[HG - 1][4 * j] : 0, qa[0][4 * j + 1], HG == 2 ? qa[HG - 1][4 * j + 1] : 0, w[j] & 0x000F000Fu, w[j] & 0x00F000F0u);
-                        mma_bf16(s[n], qa[0][4 * j + 2], HG == 2 ? qa[HG - 1][4 * j + 2] : 0, qa[0][4 * j + 3], HG == 2 ? qa[HG - 1][4 * j + 3] : 0, w8 & 0x000F000Fu, w8 & 0x00F000F0u);
-                    }
-                }
-            } else {
 #pragma unroll
             for (int n = 0; n < TILES; ++n) {
                 s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
@@ -1024,26 +1255,8 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                     }
                 }
             }
-            }
             float vs[TILES][2];
-            uint32_t s_top = 0;          // four bits: the largest of the values' scales, as bits
-            if (TYPE == KV_UINT4) {
-#pragma unroll
-                for (int n = 0; n < TILES; ++n) {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const uint32_t pair = lds_u32(scales + (8 * n + (j ? key0 ^ 3 : key0)) * 4);
-#pragma unroll
-                        for (int h = 0; h < HG; ++h) s[n][2 * h + j] = __fmaf_rn(s[n][2 * h + j], bf16lo(pair), bf16hi(pair) * q_sum[h]);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < KEYS / 32; ++i) {
-                    const uint32_t pair = lds_u32(scales + KEYS * 4 + (i * 32 + lane) * 4) & 0xFFFFu;
-                    if (i * 32 + lane < valid) s_top = max(s_top, pair);
-                }
-                s_top = __reduce_max_sync(0xffffffffu, s_top) << 16;
-            } else if (TYPE != KV_BF16) {
+            if (TYPE != KV_BF16) {
 #pragma unroll
                 for (int n = 0; n < TILES; ++n) {
 #pragma unroll
@@ -1060,7 +1273,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 for (int n = 0; n < TILES; ++n) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        if (8 * n + (TYPE == KV_UINT4 ? (j ? key0 ^ 3 : key0) : 4 * j + t) < valid) continue;
+                        if (8 * n + 4 * j + t < valid) continue;
                         vs[n][j] = 0.f;
 #pragma unroll
                         for (int h = 0; h < HG; ++h) s[n][2 * h + j] = -INFINITY;
@@ -1091,30 +1304,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                     for (int j = 0; j < 2; ++j) { s[n][2 * h + j] = exp2_fast(__fmaf_rn(s[n][2 * h + j], z_scale[h], -ref)); sum += s[n][2 * h + j]; }
                 }
                 l[h] = l[h] * alpha[h] + sum;
-                if (TYPE == KV_UINT4) {
-                    // Weights times 2^k: with codes of 2^-133 of themselves, the sums are of normal size where the largest weight so far (the product of a chunk's largest
-                    // probability and scale, at most) is between 2^90 and 2^112; weights of 2^-100 of that one are still there.
-                    most[h] = fmaxf(most[h] * alpha[h], exp2_fast(__fmaf_rn(top, z_scale[h], -ref)) * __uint_as_float(s_top));
-                    offset[h] *= alpha[h];
-                    const int e = (int)(__float_as_uint(most[h]) >> 23) - 127;
-                    if (e + k_up[h] < 90 || e + k_up[h] > 111) {
-                        const int k_new = min(min(max(101 - e, -27), 127), k_up[h] + 100);
-                        alpha[h] *= exp2_fast((float)(k_new - k_up[h]));
-                        moved = moved || k_new != k_up[h];
-                        k_up[h] = k_new;
-                    }
-                    const float up = __uint_as_float((uint32_t)(127 + k_up[h]) << 23);
-#pragma unroll
-                    for (int n = 0; n < TILES; ++n) {
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            uint32_t pair = lds_u32(scales + KEYS * 4 + (8 * n + (j ? key0 ^ 3 : key0)) * 4);
-                            if (valid < KEYS && 8 * n + (j ? key0 ^ 3 : key0) >= valid) pair = 0;
-                            offset[h] = __fmaf_rn(s[n][2 * h + j], bf16hi(pair), offset[h]);
-                            s[n][2 * h + j] = s[n][2 * h + j] * bf16lo(pair) * up;
-                        }
-                    }
-                } else if (TYPE != KV_BF16) {
+                if (TYPE != KV_BF16) {
 #pragma unroll
                     for (int n = 0; n < TILES; ++n) { s[n][2 * h] *= vs[n][0]; s[n][2 * h + 1] *= vs[n][1]; }
                 }
@@ -1138,26 +1328,6 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                         two_parts(s[2 * u + j][2 * h], s[2 * u + j][2 * h + 1], p_hi[h][j], p_lo[h][j]);
                         if (second) p_hi[h][j] = p_lo[h][j];
                     }
-                }
-                if (TYPE == KV_UINT4) {         // columns 16 g ... + 15 of four rows; a tile's rows g are even columns, g + 8 odd ones, which are 16 times as large
-                    uint2 x[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int row = u * 16 + (r >> 1) * 8 + (r & 1 ? key0 ^ 3 : key0), line = row >> 1;
-                        x[r] = lds64(st + 4096 + line * 128 + ((((row & 1) * 4 + (g >> 1)) ^ (line & 7)) << 4) + (g & 1) * 8);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const uint32_t w[4] = {j < 4 ? x[0].x : x[0].y, j < 4 ? x[1].x : x[1].y, j < 4 ? x[2].x : x[2].y, j < 4 ? x[3].x : x[3].y};
-                        uint32_t a = j & 2 ? prmt<0x7632>(w[0], w[1]) : prmt<0x5410>(w[0], w[1]), b = j & 2 ? prmt<0x7632>(w[2], w[3]) : prmt<0x5410>(w[2], w[3]);
-                        if (j & 1) { a >>= 8; b >>= 8; }
-#pragma unroll
-                        for (int h = 0; h < HG; ++h) {
-                            mma_bf16(acc[h][j], a & 0x000F000Fu, a & 0x00F000F0u, b & 0x000F000Fu, b & 0x00F000F0u, p_hi[h][0], p_hi[h][1]);
-                            if (!twice) mma_bf16(acc[h][j], a & 0x000F000Fu, a & 0x00F000F0u, b & 0x000F000Fu, b & 0x00F000F0u, p_lo[h][0], p_lo[h][1]);
-                        }
-                    }
-                    continue;
                 }
                 constexpr int PIECES = TYPE == KV_BF16 ? 2 : 1;
                 uint4 v[4][PIECES];
@@ -1208,6 +1378,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                     }
                 }
             }
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.empty[warp][slot]);
             if (++slot == STAGES) { slot = 0; parity ^= 1; }
@@ -1223,30 +1394,15 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 for (int c = 0; c < 4; ++c) acc[0][j][c] += __shfl_xor_sync(0xffffffffu, acc[0][j][c], 2);
             }
         }
-#pragma unroll
-        for (int h = 0; h < HG; ++h) {
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        }
-        if (TYPE == KV_UINT4) {        // back to the weights' own size, and what the least values add to every column
+        if (TYPE == KV_UINT4) four.end(twice, acc, m, l);
+        else
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
-                offset[h] += __shfl_xor_sync(0xffffffffu, offset[h], 1);
-                offset[h] += __shfl_xor_sync(0xffffffffu, offset[h], 2);
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const float add = __shfl_sync(0xffffffffu, offset[h], 8 * t + 4 * c);
-                    const float down = __uint_as_float((uint32_t)(127 + 100 - __shfl_sync(0xffffffffu, k_up[h], 8 * t + 4 * c)) << 23);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        acc[h][j][c] = __fmaf_rn(acc[h][j][c] * 8589934592.0f, down, add);            // 2^33
-                        acc[h][j][c + 2] = __fmaf_rn(acc[h][j][c + 2] * 536870912.0f, down, add);     // 2^29
-                    }
-                }
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
             }
-        }
         // a thread's accumulators, of heads 2t, 2t + 1 (and 8 + those): columns 64 half + 8 gp + tile of bf16, 16 gp + 8 half + tile of codes of a byte, 16 g + 2 tile (+ 1) of four bits
-        auto four = [&](const float (&d)[8][4], int q, int j) {
+        auto four_columns = [&](const float (&d)[8][4], int q, int j) {
             if (TYPE == KV_UINT4) return make_float4(d[2 * q][j], d[2 * q][j + 2], d[2 * q + 1][j], d[2 * q + 1][j + 2]);
             const int c = 2 * (q >> 1) + j, at = (q & 1) * 4;
             return make_float4(d[at][c], d[at + 1][c], d[at + 2][c], d[at + 3][c]);
@@ -1263,7 +1419,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                     const float inv = 1.0f / __shfl_sync(0xffffffffu, l[h], 8 * t + 4 * j);
                     if (head >= heads) continue;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) store_row4(a.out + seg.b * a.ldo + (head0 + head) * KV_D + column(q, columns_of(g)), four(acc[h], q, j), inv, a.flags & 2);
+                    for (int q = 0; q < 4; ++q) store_row4(a.out + seg.b * a.ldo + (head0 + head) * KV_D + column(q, columns_of(g)), four_columns(acc[h], q, j), inv, a.flags & 2);
                 }
             }
             if (seg.end == c1) return;
@@ -1285,7 +1441,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int head = 8 * h + 2 * t + j;
-                    if (head < heads) *reinterpret_cast<float4*>(buf + ((mate * heads + head) * quarters + at_q) * 32 + 4 * g) = four(acc[h], q, j);
+                    if (head < heads) *reinterpret_cast<float4*>(buf + ((mate * heads + head) * quarters + at_q) * 32 + 4 * g) = four_columns(acc[h], q, j);
                 }
             }
             if (at_q + 1 < quarters) continue;
