@@ -655,28 +655,29 @@ struct KvFour {
         const int t = threadIdx.x & 3;
 #pragma unroll
         for (int h = 0; h < HG; ++h) {
+            // (sums: a product with ones, which gives them where this thread wants them)
             uint32_t top = 0;
-            float sum = 0.f;
+            float sum[4];
+            mma_bf16_new(sum, 0x3F803F80u, 0, 0x3F803F80u, 0, q[h][0], q[h][1]);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                top = max(top, max(q[h][i] & 0x7FFFu, (q[h][i] >> 16) & 0x7FFFu));
-                sum += bf16lo(q[h][i]) + bf16hi(q[h][i]);
-            }
+            for (int i = 2; i < 16; i += 2) mma_bf16(sum, 0x3F803F80u, 0, 0x3F803F80u, 0, q[h][i], q[h][i + 1]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = max_u16x2(top, q[h][i] & 0x7FFF7FFFu);
+            top = max(top & 0xFFFFu, top >> 16);
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             // queries times 2^x, the largest one below 2^127
             const int x = min(120, 253 - (int)max(top >> 7, 1u));
-            const float up = __uint_as_float((uint32_t)(127 + x) << 23), up16 = up * 0.0625f;
             const float z = scale * __uint_as_float((uint32_t)(127 + 70) << 23) * __uint_as_float((uint32_t)(127 + 63 - x) << 23);
-            sum = sum * __uint_as_float((uint32_t)(127 + x - 70) << 23) * __uint_as_float((uint32_t)(127 - 63) << 23);
+            const uint32_t up = (uint32_t)(127 + x) * 0x00800080u, up16 = up - 0x02000200u;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) q[h][i] = pack_bf16x2(bf16lo(q[h][i]) * (i & 1 ? up16 : up), bf16hi(q[h][i]) * (i & 1 ? up16 : up));
+            for (int i = 0; i < 16; ++i) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(q[h][i]) : "r"(i & 1 ? up16 : up));
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 zs[h][c] = __shfl_sync(0xffffffffu, z, 8 * t + 4 * c);
-                q_sum[h][c] = __shfl_sync(0xffffffffu, sum, 8 * t + 4 * c);
+                // (the shuffled exponent: x of that head)
+                const int x_of = __shfl_sync(0xffffffffu, x, 8 * t + 4 * c);
+                q_sum[h][c] = sum[c] * __uint_as_float((uint32_t)(127 + x_of - 70) << 23) * __uint_as_float((uint32_t)(127 - 63) << 23);
                 m[h][c] = -INFINITY;
                 l[h][c] = offset[h][c] = most[h][c] = 0.f;
                 k[h][c] = 101;
@@ -697,12 +698,23 @@ struct KvFour {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, mine = kv4_key(g), key0 = kv4_even(t);
         const bool upper = t & 2;
         float s[4][HG][4];
+#ifndef KU
+#define KU 4
+#endif
+#pragma unroll 1
+        for (int i0 = 0; i0 < 4; i0 += KU) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i + KU < 4; ++i)
+#pragma unroll
+            for (int h = 0; h < HG; ++h)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s[i][h][c] = s[i + KU][h][c];
+#pragma unroll
+        for (int i = 4 - KU; i < 4; ++i) {
             uint4 x[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const int line = 8 * i + 4 * r + (mine >> 1);
+                const int line = 8 * (i - 4 + KU + i0) + 4 * r + (mine >> 1);
                 x[r] = lds128(st + line * 128 + ((((mine & 1) * 4 + t) ^ (line & 7)) << 4));
             }
             const uint32_t w[4][2] = {{x[0].x, x[1].x}, {x[0].y, x[1].y}, {x[0].z, x[1].z}, {x[0].w, x[1].w}};
@@ -718,12 +730,18 @@ struct KvFour {
                 }
             }
         }
+        }
         if (TWICE) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) s[i][0][c] = upper ? s[i + 2][0][c] : s[i][0][c];
             }
+        }
+        if (valid < KEYS) {             // what is behind a sequence may be NaN; of its values' scales nothing is left
+            for (int i = lane; i < KEYS; i += 32) if (i >= valid) asm volatile("st.shared.b32 [%0], %1;" ::"r"(scales + KEYS * 4 + i * 4), "r"(0) : "memory");
+            fence_proxy_async_smem();
+            __syncwarp();
         }
         const int first = mine + (TWICE && upper ? 32 : 0);        // this thread's keys: first + 8 n
         const uint32_t pairs = scales + first * 4;
@@ -742,8 +760,7 @@ struct KvFour {
         uint32_t s_top = 0;           // the largest of the values' scales, as bits
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint32_t pair = lds_u32(scales + KEYS * 4 + (i * 32 + lane) * 4) & 0xFFFFu;
-            if (i * 32 + lane < valid) s_top = max(s_top, pair);
+            s_top = max(s_top, lds_u32(scales + KEYS * 4 + (i * 32 + lane) * 4) & 0xFFFFu);
         }
         s_top = __reduce_max_sync(0xffffffffu, s_top) << 16;
         if (valid < KEYS) {
@@ -805,8 +822,7 @@ struct KvFour {
         uint32_t hi[4][HG][2], lo[4][HG][2];
 #pragma unroll
         for (int n = 0; n < 2 * MINE; ++n) {
-            uint32_t pair = lds_u32(pairs + KEYS * 4 + n * 32);
-            if (first + 8 * n >= valid) pair = 0;             // what is behind a sequence may be NaN
+            const uint32_t pair = lds_u32(pairs + KEYS * 4 + n * 32);
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
                 float w[2];
@@ -831,12 +847,17 @@ struct KvFour {
             }
         }
         // out^T += V^T P^T, 16 keys a step: columns 16 g ... + 15 of four rows; a tile's rows g are even columns, g + 8 odd ones, which are 16 times as large
+#ifndef VU
+#define VU 2
+#endif
+#pragma unroll 1
+        for (int u0 = 0; u0 < 4; u0 += VU) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < VU; ++u) {
             uint2 x[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int row = u * 16 + (r >> 1) * 8 + (r & 1 ? key0 ^ 3 : key0), line = row >> 1;
+                const int row = (u0 + u) * 16 + (r >> 1) * 8 + (r & 1 ? key0 ^ 3 : key0), line = row >> 1;
                 x[r] = lds64(st + 4096 + line * 128 + ((((row & 1) * 4 + (g >> 1)) ^ (line & 7)) << 4) + (g & 1) * 8);
             }
 #pragma unroll
@@ -858,6 +879,13 @@ struct KvFour {
                     if (!TWICE) mma_bf16(acc[h][j], a & 0x000F000Fu, a & 0x00F000F0u, b & 0x000F000Fu, b & 0x00F000F0u, lo[u][h][0], lo[u][h][1]);
                 }
             }
+        }
+#pragma unroll
+        for (int u = 0; u + VU < 4; ++u)
+#pragma unroll
+            for (int h = 0; h < HG; ++h)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) { hi[u][h][r] = hi[u + VU][h][r]; if (!TWICE) lo[u][h][r] = lo[u + VU][h][r]; }
         }
     }
 
@@ -980,6 +1008,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             const int tok = at.c * KEYS, len = sh.len[at.b], head = a.chunks_of_heads == 1 ? at.item : at.item / a.chunks_of_heads;
 #pragma unroll
             for (int h = 0; h < KEYS / 16; ++h) {
+                if (TYPE == KV_UINT4 && (a.flags & 8) && h > 0) { place[h] = -1; continue; }        // (of a whole chunk's box only the first one counts)
                 const int token = tok + 16 * h, p = shift >= 0 ? token >> shift : token / ps;
                 place[h] = -1;
                 if (token >= len) continue;
@@ -1007,7 +1036,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 int p[K::PLACES];        // (four bits)
                 if (TYPE == KV_UINT4) {
 #pragma unroll
-                    for (int h = 0; h < K::PLACES; ++h) p[h] = __shfl_sync(0xffffffffu, now[h], mate);
+                    for (int h = 0; h < K::PLACES; ++h) p[h] = h > 0 && (a.flags & 8) ? -1 : __shfl_sync(0xffffffffu, now[h], mate);
                 }
                 uint64_t* const full = &sh.full[w][slot];
                 if (elect_one()) {
@@ -1016,25 +1045,33 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                     else {
                         if (a.kn && TYPE == KV_UINT4) {
 #pragma unroll
-                            for (int h = 0; h < K::PLACES; ++h) sh.rows[w][slot][h] = failed ? -1 : p[h];
+                            for (int h = 0; h < K::PLACES; ++h) sh.rows[w][slot][h] = failed ? -1 : (a.flags & 8) && p[0] >= 0 ? p[0] + 16 * h : p[h];
                         } else if (a.kn) { sh.rows[w][slot][0] = failed ? -1 : p0; sh.rows[w][slot][1] = failed ? -1 : p1; }
                         const int r0 = max(p0, 0), r1 = p1 == -2 ? 0 : p1;       // (of a page outside, the cache's first rows are loaded)
                         uint8_t* const dst = smem + (w * STAGES + slot) * KV_STAGE_BYTES;
                         const uint32_t scales = smem_u32(smem) + K::SCALES + (w * STAGES + slot) * K::SCALE_BYTES;
                         if (TYPE == KV_UINT4) {       // (a line of 128 bytes has two rows)
-                            const int step = a.flags & 8 ? 4 : a.flags & 16 ? 2 : 1;        // places to a box
-                            int boxes = 0;
+                            if (a.flags & 8) {
+                                mbar_expect_tx(full, 8192 + 512);
+                                tma_load_2d(dst, &k_map, full, 0, r0 >> 1);
+                                tma_load_2d(dst + 4096, &v_map, full, 0, r0 >> 1);
+                                bulk_load(scales, a.c.ks + r0, 256, full);
+                                bulk_load(scales + 256, a.c.vs + r0, 256, full);
+                            } else {
+                                const int step = a.flags & 16 ? 2 : 1;        // places to a box
+                                int boxes = 0;
 #pragma unroll
-                            for (int h = 0; h < K::PLACES; ++h) boxes += h % step == 0 && p[h] != -1;
-                            mbar_expect_tx(full, boxes * step * (2048 + 128));
+                                for (int h = 0; h < K::PLACES; ++h) boxes += h % step == 0 && p[h] != -1;
+                                mbar_expect_tx(full, boxes * step * (2048 + 128));
 #pragma unroll
-                            for (int h = 0; h < K::PLACES; ++h) {
-                                if (h % step != 0 || p[h] == -1) continue;
-                                const int r = max(p[h], 0);
-                                tma_load_2d(dst + h * 1024, &k_map, full, 0, r >> 1);
-                                tma_load_2d(dst + 4096 + h * 1024, &v_map, full, 0, r >> 1);
-                                bulk_load(scales + h * 64, a.c.ks + r, step * 64, full);
-                                bulk_load(scales + KEYS * 4 + h * 64, a.c.vs + r, step * 64, full);
+                                for (int h = 0; h < K::PLACES; ++h) {
+                                    if (h % step != 0 || p[h] == -1) continue;
+                                    const int r = max(p[h], 0);
+                                    tma_load_2d(dst + h * 1024, &k_map, full, 0, r >> 1);
+                                    tma_load_2d(dst + 4096 + h * 1024, &v_map, full, 0, r >> 1);
+                                    bulk_load(scales + h * 64, a.c.ks + r, step * 64, full);
+                                    bulk_load(scales + 256 + h * 64, a.c.vs + r, step * 64, full);
+                                }
                             }
                         } else if (TYPE == KV_BF16) {
                             mbar_expect_tx(full, 8192);
