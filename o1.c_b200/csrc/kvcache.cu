@@ -387,6 +387,10 @@ __device__ __forceinline__ void mma_bf16_new(float (&d)[4], uint32_t a0, uint32_
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
+// Four 8 x 8 matrices of two-byte values in shared memory, a row's address from each thread, transposed.
+__device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
 // An 8 x 8 matrix of two-byte values, two of a row to a thread, transposed.
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     uint32_t r;
@@ -454,11 +458,6 @@ __device__ __forceinline__ float lds_f32(uint32_t a) {
 __device__ __forceinline__ uint32_t lds_u32(uint32_t a) {
     uint32_t v;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
-    return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-    uint2 v;
-    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
     return v;
 }
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
@@ -694,48 +693,50 @@ struct KvFour {
     }
     template <bool TWICE>
     __device__ __forceinline__ void part(uint32_t st, uint32_t scales, int valid, const uint32_t (&q)[HG][16], float (&acc)[HG][8][4]) {
-        constexpr int KEYS = 64, MINE = TWICE ? 2 : 4;       // tiles of 16 keys that are this thread's
-        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, mine = kv4_key(g), key0 = kv4_even(t);
+        constexpr int KEYS = 64, MINE = TWICE ? 4 : 8, APART = TWICE ? 16 : 8;       // this thread's keys, and how far apart they are
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, mine = kv4_key(g);
         const bool upper = t & 2;
         float s[4][HG][4];
-#ifndef KU
-#define KU 4
-#endif
-#pragma unroll 1
-        for (int i0 = 0; i0 < 4; i0 += KU) {
+        const int first = mine + (TWICE && upper ? 8 : 0);        // this thread's keys: first + APART n
+        const uint32_t pairs = scales + first * 4;
+        uint32_t kpair[MINE];
 #pragma unroll
-        for (int i = 0; i + KU < 4; ++i)
+        for (int n = 0; n < MINE; ++n) kpair[n] = lds_u32(pairs + n * (APART * 4));
 #pragma unroll
-            for (int h = 0; h < HG; ++h)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) s[i][h][c] = s[i + KU][h][c];
-#pragma unroll
-        for (int i = 4 - KU; i < 4; ++i) {
-            uint4 x[2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int line = 8 * (i - 4 + KU + i0) + 4 * r + (mine >> 1);
-                x[r] = lds128(st + line * 128 + ((((mine & 1) * 4 + t) ^ (line & 7)) << 4));
-            }
-            const uint32_t w[4][2] = {{x[0].x, x[1].x}, {x[0].y, x[1].y}, {x[0].z, x[1].z}, {x[0].w, x[1].w}};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                constexpr uint32_t A = 0x000F000Fu, B = 0x00F000F0u;
-                const uint32_t x8 = w[j][0] >> 8, y8 = w[j][1] >> 8;
-#pragma unroll
-                for (int h = 0; h < HG; ++h) {
-                    if (j == 0) mma_bf16_new(s[i][h], w[j][0] & A, w[j][1] & A, w[j][0] & B, w[j][1] & B, q[h][4 * j], q[h][4 * j + 1]);
-                    else mma_bf16(s[i][h], w[j][0] & A, w[j][1] & A, w[j][0] & B, w[j][1] & B, q[h][4 * j], q[h][4 * j + 1]);
-                    mma_bf16(s[i][h], x8 & A, y8 & A, x8 & B, y8 & B, q[h][4 * j + 2], q[h][4 * j + 3]);
-                }
-            }
-        }
-        }
-        if (TWICE) {
+        for (int i0 = 0; i0 < 4; i0 += 2) {
+            uint4 x[2][2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) s[i][0][c] = upper ? s[i + 2][0][c] : s[i][0][c];
+                for (int r = 0; r < 2; ++r) {
+                    const int line = 8 * (i0 + i) + 4 * r + (mine >> 1);
+                    x[i][r] = lds128(st + line * 128 + ((((mine & 1) * 4 + t) ^ (line & 7)) << 4));
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        constexpr uint32_t A = 0x000F000Fu, B = 0x00F000F0u;
+                        const uint4 &a4 = x[i][0], &b4 = x[i][1];
+                        uint32_t a = j == 0 ? a4.x : j == 1 ? a4.y : j == 2 ? a4.z : a4.w, b = j == 0 ? b4.x : j == 1 ? b4.y : j == 2 ? b4.z : b4.w;
+                        if (half) { a >>= 8; b >>= 8; }
+#pragma unroll
+                        for (int h = 0; h < HG; ++h) {
+                            if (j == 0 && half == 0) mma_bf16_new(s[i0 + i][h], a & A, b & A, a & B, b & B, q[h][0], q[h][1]);
+                            else mma_bf16(s[i0 + i][h], a & A, b & A, a & B, b & B, q[h][4 * j + 2 * half], q[h][4 * j + 2 * half + 1]);
+                        }
+                    }
+                }
+            }
+        }
+        if (TWICE) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) s[i][0][c] = upper ? s[i][0][2 + c] : s[i][0][c];
             }
         }
         if (valid < KEYS) {             // what is behind a sequence may be NaN; of its values' scales nothing is left
@@ -743,16 +744,14 @@ struct KvFour {
             fence_proxy_async_smem();
             __syncwarp();
         }
-        const int first = mine + (TWICE && upper ? 32 : 0);        // this thread's keys: first + 8 n
-        const uint32_t pairs = scales + first * 4;
 #pragma unroll
-        for (int n = 0; n < 2 * MINE; ++n) {
-            const uint32_t pair = lds_u32(pairs + n * 32);
+        for (int n = 0; n < MINE; ++n) {
+            const uint32_t pair = kpair[n];
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    float& z = s[n >> 1][h][2 * (n & 1) + c];
+                    float& z = s[TWICE ? n : n >> 1][h][(TWICE ? 0 : 2 * (n & 1)) + c];
                     z = __fmaf_rn(z, bf16lo(pair), bf16hi(pair) * q_sum[h][c]);
                 }
             }
@@ -765,10 +764,13 @@ struct KvFour {
         s_top = __reduce_max_sync(0xffffffffu, s_top) << 16;
         if (valid < KEYS) {
 #pragma unroll
-            for (int n = 0; n < 2 * MINE; ++n) {
-                if (first + 8 * n < valid) continue;
+            for (int n = 0; n < MINE; ++n) {
+                if (first + APART * n < valid) continue;
 #pragma unroll
-                for (int h = 0; h < HG; ++h) s[n >> 1][h][2 * (n & 1)] = s[n >> 1][h][2 * (n & 1) + 1] = -INFINITY;
+                for (int h = 0; h < HG; ++h) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) s[TWICE ? n : n >> 1][h][(TWICE ? 0 : 2 * (n & 1)) + c] = -INFINITY;
+                }
             }
         }
         bool moved = false;
@@ -779,7 +781,7 @@ struct KvFour {
             for (int c = 0; c < 2; ++c) {
                 float top = -INFINITY;
 #pragma unroll
-                for (int n = 0; n < 2 * MINE; ++n) top = fmaxf(top, s[n >> 1][h][2 * (n & 1) + c]);
+                for (int n = 0; n < MINE; ++n) top = fmaxf(top, s[TWICE ? n : n >> 1][h][(TWICE ? 0 : 2 * (n & 1)) + c]);
 #pragma unroll
                 for (int o = TWICE ? 2 : 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                 const float m_new = fmaxf(m[h][c], top * zs[h][c]), ref = (m_new == -INFINITY ? 0.f : m_new) - KV_LIFT;
@@ -787,8 +789,8 @@ struct KvFour {
                 m[h][c] = m_new;
                 float sum = 0.f;
 #pragma unroll
-                for (int n = 0; n < 2 * MINE; ++n) {
-                    float& z = s[n >> 1][h][2 * (n & 1) + c];
+                for (int n = 0; n < MINE; ++n) {
+                    float& z = s[TWICE ? n : n >> 1][h][(TWICE ? 0 : 2 * (n & 1)) + c];
                     z = exp2_fast(__fmaf_rn(z, zs[h][c], -ref));
                     sum += z;
                 }
@@ -821,45 +823,39 @@ struct KvFour {
         }
         uint32_t hi[4][HG][2], lo[4][HG][2];
 #pragma unroll
-        for (int n = 0; n < 2 * MINE; ++n) {
-            const uint32_t pair = lds_u32(pairs + KEYS * 4 + n * 32);
+        for (int n = 0; n < MINE; ++n) {
+            const uint32_t pair = lds_u32(pairs + KEYS * 4 + n * (APART * 4));
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
                 float w[2];
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    const float p = s[n >> 1][h][2 * (n & 1) + c];
+                    const float p = s[TWICE ? n : n >> 1][h][(TWICE ? 0 : 2 * (n & 1)) + c];
                     offset[h][c] = __fmaf_rn(p, bf16hi(pair), offset[h][c]);
                     w[c] = p * bf16lo(pair) * up[h][c];
                 }
-                two_parts(w[0], w[1], hi[n >> 1][h][n & 1], lo[n >> 1][h][n & 1]);
+                two_parts(w[0], w[1], hi[TWICE ? n : n >> 1][h][TWICE ? 0 : n & 1], lo[TWICE ? n : n >> 1][h][TWICE ? 0 : n & 1]);
             }
         }
         if (TWICE) {            // heads in the lower columns' threads get the values, the others the rests
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const uint32_t other = __shfl_xor_sync(0xffffffffu, upper ? hi[i][0][r] : lo[i][0][r], 2);
-                    hi[i + 2][0][r] = upper ? lo[i][0][r] : other;
-                    hi[i][0][r] = upper ? other : hi[i][0][r];
-                }
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t other = __shfl_xor_sync(0xffffffffu, upper ? hi[i][0][0] : lo[i][0][0], 2);
+                hi[i][0][1] = upper ? lo[i][0][0] : other;
+                hi[i][0][0] = upper ? other : hi[i][0][0];
             }
         }
-        // out^T += V^T P^T, 16 keys a step: columns 16 g ... + 15 of four rows; a tile's rows g are even columns, g + 8 odd ones, which are 16 times as large
-#ifndef VU
-#define VU 2
-#endif
+        // out^T += V^T P^T, 16 keys a step.  A matrix of eight rows and 32 columns, in two-byte pieces of four columns, is loaded transposed: this thread gets columns 4 g ... + 3 of two rows
+        // beside each other, as the product wants them.  A tile's rows g are even columns, g + 8 odd ones, which are 16 times as large.
+        const int row = (lane & 8) + kv4_key(lane & 7);
+        const uint32_t values = st + 4096 + (row >> 1) * 128 + ((((row & 1) * 4 + (lane >> 4)) ^ (row >> 1 & 7)) << 4);
 #pragma unroll 1
-        for (int u0 = 0; u0 < 4; u0 += VU) {
+        for (int u0 = 0; u0 < 4; u0 += 2) {
 #pragma unroll
-        for (int u = 0; u < VU; ++u) {
-            uint2 x[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = (u0 + u) * 16 + (r >> 1) * 8 + (r & 1 ? key0 ^ 3 : key0), line = row >> 1;
-                x[r] = lds64(st + 4096 + line * 128 + ((((row & 1) * 4 + (g >> 1)) ^ (line & 7)) << 4) + (g & 1) * 8);
-            }
+        for (int u = 0; u < 2; ++u) {
+            uint32_t x[2][4];
+            ldmatrix_trans(x[0], values + (u0 + u) * 1024);
+            ldmatrix_trans(x[1], (values ^ 32) + (u0 + u) * 1024);
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
 #pragma unroll
@@ -870,8 +866,7 @@ struct KvFour {
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const uint32_t w[4] = {j < 4 ? x[0].x : x[0].y, j < 4 ? x[1].x : x[1].y, j < 4 ? x[2].x : x[2].y, j < 4 ? x[3].x : x[3].y};
-                uint32_t a = j & 2 ? prmt<0x7632>(w[0], w[1]) : prmt<0x5410>(w[0], w[1]), b = j & 2 ? prmt<0x7632>(w[2], w[3]) : prmt<0x5410>(w[2], w[3]);
+                uint32_t a = x[j >> 2][j & 2], b = x[j >> 2][(j & 2) + 1];
                 if (j & 1) { a >>= 8; b >>= 8; }
 #pragma unroll
                 for (int h = 0; h < HG; ++h) {
@@ -881,11 +876,11 @@ struct KvFour {
             }
         }
 #pragma unroll
-        for (int u = 0; u + VU < 4; ++u)
+        for (int u = 0; u + 2 < 4; ++u)
 #pragma unroll
             for (int h = 0; h < HG; ++h)
 #pragma unroll
-                for (int r = 0; r < 2; ++r) { hi[u][h][r] = hi[u + VU][h][r]; if (!TWICE) lo[u][h][r] = lo[u + VU][h][r]; }
+                for (int r = 0; r < 2; ++r) { hi[u][h][r] = hi[u + 2][h][r]; if (!TWICE) lo[u][h][r] = lo[u + 2][h][r]; }
         }
     }
 
@@ -1438,14 +1433,14 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
                 l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
             }
-        // a thread's accumulators, of heads 2t, 2t + 1 (and 8 + those): columns 64 half + 8 gp + tile of bf16, 16 gp + 8 half + tile of codes of a byte, 16 g + 2 tile (+ 1) of four bits
+        // a thread's accumulators, of heads 2t, 2t + 1 (and 8 + those): columns 64 half + 8 gp + tile of bf16, 16 gp + 8 half + tile of codes of a byte, 32 (tile / 2) + 4 g + 2 (tile % 2) (+ 1) of four bits
         auto four_columns = [&](const float (&d)[8][4], int q, int j) {
             if (TYPE == KV_UINT4) return make_float4(d[2 * q][j], d[2 * q][j + 2], d[2 * q + 1][j], d[2 * q + 1][j + 2]);
             const int c = 2 * (q >> 1) + j, at = (q & 1) * 4;
             return make_float4(d[at][c], d[at + 1][c], d[at + 2][c], d[at + 3][c]);
         };
         auto columns_of = [](int i) { return TYPE == KV_UINT4 ? i : kv_perm(i); };
-        auto column = [&](int quarter, int p) { return TYPE == KV_UINT4 ? 16 * p + 4 * quarter : (TYPE == KV_BF16 ? 64 * (quarter >> 1) + 8 * p : 8 * (quarter >> 1) + 16 * p) + (quarter & 1) * 4; };
+        auto column = [&](int quarter, int p) { return TYPE == KV_UINT4 ? 32 * quarter + 4 * p : (TYPE == KV_BF16 ? 64 * (quarter >> 1) + 8 * p : 8 * (quarter >> 1) + 16 * p) + (quarter & 1) * 4; };
         if (solo) {
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
