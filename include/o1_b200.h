@@ -800,12 +800,13 @@ hd_status o1_kv_attention(const o1_kv_cache *cache, const void *q, int64_t ldq, 
                           const void *v_new, int64_t ldv, const int32_t *pages, int64_t ldp, int width, const int32_t *lens,
                           void *out, int64_t ldo, float *lse, int batch, int heads, float scale, void *workspace,
                           int64_t workspace_bytes);
-/* Pages handed out on the device: the pages and rows of up to max_seqs (at most 8192) sequences and a list of free pages.  table [max_seqs][width]: a sequence's pages in
+/* Pages handed out on the device: the pages and rows of up to max_seqs (at most 8192) sequences and a list of free pages (at most 2^30 of them, and rows of a
+ * sequence or of a call).  table [max_seqs][width]: a sequence's pages in
  * order, -1 behind them; lens [max_seqs]: its rows; free_pages [pages]: a stack, its top at state[0] - 1; state [2]: the number of free pages, and a counter that belongs to
  * these calls (0 between them).  All int32 on the device.  o1_kv_pages_reset makes every page free and every sequence empty.  Calls on the same pages follow one another (one
  * stream, or ordered); like all entry points they can be captured, and a captured call serves what its arguments hold at each replay.
  * o1_kv_pages_grow: counts[b] new rows for sequence seqs[b] (NULL: sequence b).  With the requests' rows behind one another, request b's from starts[b] to starts[b + 1] - 1 (starts
- * [batch + 1]): row r gets slots[r] (for o1_kv_write) and positions[r], its number in the sequence.  slots and positions have room for `rows`; rows behind the last
+ * [batch + 1], at most 2^30): row r gets slots[r] (for o1_kv_write) and positions[r], its number in the sequence.  slots and positions have room for `rows`; rows behind the last
  * request get slot -1 and position 0.  lens[b]: the sequence's rows with the new ones; tables (NULL: not wanted) [batch][ldp]: its row of the table (lens and tables as
  * o1_kv_attention takes them).  Requests are served in order: new pages come from the top of the stack.
  * o1_kv_pages_shrink: sequence seqs[b] keeps its first keep[b] rows (0: it is closed); pages behind them are free again and come back in the order in which they went.

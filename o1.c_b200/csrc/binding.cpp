@@ -24,7 +24,7 @@ decltype(&o1_capture_id) f_capture;
 decltype(&o1_kv_pages_grow) f_grow;
 decltype(&o1_kv_pages_shrink) f_shrink;
 decltype(&o1_rotary) f_rotary;
-PyObject *O1Error, *check;
+PyObject *O1Error, *check, *Grown;
 
 struct Handle {
     const o1_kv_cache* cache;
@@ -65,6 +65,21 @@ struct OnLibrary {
 at::Tensor empty_on(at::IntArrayRef size, at::ScalarType type, int device) {
     return at::Tensor(at::detail::empty_cuda(size, type, c10::Device(c10::kCUDA, (c10::DeviceIndex)device), c10::nullopt));
 }
+// Tensors of several sizes and types in one allocation, which lives as long as any of them (an allocation takes 0.6 us of a call).
+struct Several {
+    at::Tensor all;
+    int64_t used = 0;
+    Several(int64_t bytes, int device) : all(empty_on({bytes}, at::kByte, device)) {}
+    static int64_t room(int64_t values, int64_t size) { return (values * size + 15) & ~(int64_t)15; }
+    at::Tensor next(at::IntArrayRef size, at::ScalarType type) {
+        at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(type));
+        const int64_t each = (int64_t)c10::elementSize(type);
+        t.unsafeGetTensorImpl()->set_storage_offset(used / each);
+        t.unsafeGetTensorImpl()->set_sizes_contiguous(size);
+        used += room(t.numel(), each);
+        return t;
+    }
+};
 bool bf16_on(const at::Tensor& t, int device) { return t.scalar_type() == at::kBFloat16 && t.is_cuda() && t.device().index() == device; }
 
 // bf16 rows [n, heads, 128] whose heads lie side by side; n < 0: any number
@@ -327,7 +342,7 @@ const at::Tensor* ints(PyObject* o, int64_t n, int device, const char* who, cons
     return t;
 }
 
-// pages_grow(address of an o1_kv_pages, device index, its table, counts, rows, seqs or None) -> (slots, positions, starts, lens, pages)
+// pages_grow(address of an o1_kv_pages, device index, its table, counts, rows, seqs or None) -> Grown(slots, positions, starts, lens, pages)
 PyObject* py_grow(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     static const char* who = "KvPages.grow";
@@ -338,17 +353,19 @@ PyObject* py_grow(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!counts) return nullptr;
     const int64_t rows = PyLong_AsLongLong(a[4]), batch = counts->size(0);
     if (PyErr_Occurred()) return nullptr;
-    if (rows < 0 || rows > INT32_MAX) return fail(who, "rows between 0 and 2^31 - 1 wanted");
+    if (rows < 0 || rows > (1 << 30)) return fail(who, "rows between 0 and 2^30 wanted");
     if (batch > pages->max_seqs) return fail(who, "more requests than sequences");
     const at::Tensor* seqs = nullptr;
     if (a[5] != Py_None && !(seqs = ints(a[5], batch, device, who, "seqs"))) return nullptr;
     const OnLibrary on(device);
-    at::Tensor out[5] = {empty_on({rows}, at::kLong, device), empty_on({rows}, at::kInt, device), empty_on({batch + 1}, at::kInt, device), empty_on({batch}, at::kInt, device),
-                         seqs ? empty_on({batch, pages->width}, at::kInt, device) : table->narrow(0, 0, batch)};
+    const int64_t tables = seqs ? batch * pages->width : 0;
+    Several some(Several::room(rows, 8) + Several::room(rows, 4) + Several::room(batch + 1, 4) + Several::room(batch, 4) + Several::room(tables, 4), device);
+    at::Tensor out[5] = {some.next({rows}, at::kLong), some.next({rows}, at::kInt), some.next({batch + 1}, at::kInt), some.next({batch}, at::kInt),
+                         seqs ? some.next({batch, pages->width}, at::kInt) : table->narrow(0, 0, batch)};
     if (!status(f_grow(pages, seqs ? (const int32_t*)seqs->data_ptr() : nullptr, (const int32_t*)counts->data_ptr(), (int)batch, (int64_t*)out[0].data_ptr(), (int32_t*)out[1].data_ptr(),
                        (int)rows, (int32_t*)out[2].data_ptr(), (int32_t*)out[3].data_ptr(), seqs ? (int32_t*)out[4].data_ptr() : nullptr, pages->width), "o1_kv_pages_grow"))
         return nullptr;
-    PyObject* all = PyTuple_New(5);
+    PyObject* all = ((PyTypeObject*)Grown)->tp_alloc((PyTypeObject*)Grown, 5);       // (a named tuple)
     for (int i = 0; all && i < 5; ++i) {
         PyObject* o = THPVariable_Wrap(out[i]);
         if (!o) { Py_DECREF(all); return nullptr; }
@@ -375,13 +392,15 @@ PyObject* py_shrink(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// rotary(address of an o1_rope, device index, positions, inverse, x, y or None[, x, y or None]) -> y or (y, y)
+// rotary(address of an o1_rope, device index, positions, inverse, x, y or None) -> y; x and y may be pairs
 PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     static const char* who = "Rotary";
-    if (n != 6 && n != 8) { PyErr_SetString(PyExc_TypeError, "wrong number of arguments"); return nullptr; }
+    if (!arguments(n, 6)) return nullptr;
+    const bool pair = PyTuple_Check(a[4]), given = a[5] != Py_None;
+    if (pair && (PyTuple_GET_SIZE(a[4]) != 2 || (given && (!PyTuple_Check(a[5]) || PyTuple_GET_SIZE(a[5]) != 2)))) return fail(who, "a tensor or a pair of them, and a pair to fill");
     const auto* rope = (const o1_rope*)PyLong_AsUnsignedLongLong(a[0]);
-    const int device = (int)PyLong_AsLong(a[1]), inverse = PyObject_IsTrue(a[3]), sides = n == 8 ? 2 : 1;
+    const int device = (int)PyLong_AsLong(a[1]), inverse = PyObject_IsTrue(a[3]), sides = pair ? 2 : 1;
     if (PyErr_Occurred()) return nullptr;
     const at::Tensor* positions = tensor(a[2], who);
     if (!positions) return nullptr;
@@ -406,15 +425,16 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor* in[2] = {nullptr, nullptr};
     int64_t ldx[2] = {0, 0}, ldy[2] = {0, 0};
     for (int i = 0; i < sides; ++i) {
-        if (!(in[i] = tensor(a[4 + 2 * i], who))) return nullptr;
+        if (!(in[i] = tensor(pair ? PyTuple_GET_ITEM(a[4], i) : a[4], who))) return nullptr;
         if (i == 0 && in[0]->scalar_type() == at::kFloat) type = at::kFloat;
         if (!rows_of(*in[i], -1, ldx[i])) return nullptr;
+        PyObject* const y = !given ? Py_None : pair ? PyTuple_GET_ITEM(a[5], i) : a[5];
         const int64_t heads = in[i]->size(1);
-        if (a[5 + 2 * i] == Py_None) {
+        if (y == Py_None) {
             out[i] = empty_on({rows, heads, dim}, type, device);
             ldy[i] = heads * dim;
         } else {
-            const at::Tensor* t = tensor(a[5 + 2 * i], who);
+            const at::Tensor* t = tensor(y, who);
             if (!t || !rows_of(*t, heads, ldy[i])) return nullptr;
             out[i] = *t;
         }
@@ -432,9 +452,9 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// setup(addresses of o1_kv_write, o1_kv_read, o1_kv_attention, o1_residual_norm, o1_get_stream, o1_capture_id, o1_kv_pages_grow, o1_kv_pages_shrink, o1_rotary; O1Error; check)
+// setup(addresses of o1_kv_write, o1_kv_read, o1_kv_attention, o1_residual_norm, o1_get_stream, o1_capture_id, o1_kv_pages_grow, o1_kv_pages_shrink, o1_rotary; O1Error; check; Grown)
 PyObject* py_setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    if (!arguments(n, 11)) return nullptr;
+    if (!arguments(n, 12)) return nullptr;
     unsigned long long p[9];
     for (int i = 0; i < 9; ++i) p[i] = PyLong_AsUnsignedLongLong(a[i]);
     if (PyErr_Occurred()) return nullptr;
@@ -448,7 +468,9 @@ PyObject* py_setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
     f_shrink = (decltype(f_shrink))p[7];
     f_rotary = (decltype(f_rotary))p[8];
     O1Error = Py_NewRef(a[9]);
+    if (!PyType_Check(a[11]) || !PyType_IsSubtype((PyTypeObject*)a[11], &PyTuple_Type)) { PyErr_SetString(PyExc_TypeError, "a kind of tuple wanted"); return nullptr; }
     check = Py_NewRef(a[10]);
+    Grown = Py_NewRef(a[11]);
     Py_RETURN_NONE;
 }
 

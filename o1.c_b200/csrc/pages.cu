@@ -14,11 +14,10 @@
 #include "kernels.h"
 #include "../../include/o1_b200.h"
 
-#include <limits.h>
-
 namespace o1 {
 
-static constexpr int PG_THREADS = 512, PG_SEQS = 8192;
+static constexpr int PG_THREADS = 1024, PG_SEQS = 8192;
+static constexpr int PG_FULL = 1 << 30;             // sums end here, and no table or result is larger
 static constexpr int PG_COLS = 128;                // entries of a sequence's table to a warp's step
 static constexpr int ERR_PG_SEQUENCE = 70, ERR_PG_LENGTH = 71, ERR_PG_NONE_LEFT = 73;
 
@@ -33,102 +32,107 @@ struct PgArgs {
     int* bad;
 };
 
-struct PgRequest { int seq, len, pages_before, pages_after; };      // seq < 0: refused (its rows have no slots)
+// seq < 0: refused (its rows have no slots); after: its rows when it is done
+struct PgRequest { int seq, len, after; };
 
-// Sums of v over the block's threads before this one, and over all, of both components.
-__device__ __forceinline__ longlong2 pg_scan(longlong2 v, longlong2& all, longlong2* part) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    longlong2 sum = v;
+// Sums of v over the block's threads before this one, and over all, of both components, which are between 0 and PG_FULL and stay there.
+__device__ __forceinline__ int2 pg_scan(int2 v, int2& all, int2* part) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    int2 sum = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, sum.x, o), y = __shfl_up_sync(0xffffffffu, sum.y, o);
-        if (lane >= o) { sum.x += x; sum.y += y; }
+        const int x = __shfl_up_sync(0xffffffffu, sum.x, o), y = __shfl_up_sync(0xffffffffu, sum.y, o);
+        if (lane >= o) { sum.x = min(sum.x + x, PG_FULL); sum.y = min(sum.y + y, PG_FULL); }
     }
     if (lane == 31) part[warp] = sum;
+    int2 before = make_int2(__shfl_up_sync(0xffffffffu, sum.x, 1), __shfl_up_sync(0xffffffffu, sum.y, 1));
+    if (lane == 0) before = make_int2(0, 0);
     __syncthreads();
-    longlong2 before = make_longlong2(sum.x - v.x, sum.y - v.y);
-    all = make_longlong2(0, 0);
+    int2 p = lane < warps ? part[lane] : make_int2(0, 0);
 #pragma unroll
-    for (int w = 0; w < PG_THREADS / 32; ++w) {
-        const longlong2 p = part[w];
-        if (w < warp) { before.x += p.x; before.y += p.y; }
-        all.x += p.x;
-        all.y += p.y;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, p.x, o), y = __shfl_up_sync(0xffffffffu, p.y, o);
+        if (lane >= o) { p.x = min(p.x + x, PG_FULL); p.y = min(p.y + y, PG_FULL); }
     }
-    __syncthreads();
+    all = make_int2(__shfl_sync(0xffffffffu, p.x, 31), __shfl_sync(0xffffffffu, p.y, 31));
+    const int x = __shfl_sync(0xffffffffu, p.x, max(warp - 1, 0)), y = __shfl_sync(0xffffffffu, p.y, max(warp - 1, 0));
+    if (warp > 0) before = make_int2(min(before.x + x, PG_FULL), min(before.y + y, PG_FULL));
     return before;
 }
 
 template <bool GROW>
-__global__ void __launch_bounds__(PG_THREADS)
+__global__ void __launch_bounds__(PG_THREADS, 1)
 pages_kernel(const PgArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ longlong2 part[PG_THREADS / 32];
+    __shared__ int2 part[32];
     __shared__ int granted, last;
     PgRequest* const req = reinterpret_cast<PgRequest*>(smem);
     int* const start = reinterpret_cast<int*>(req + a.batch);          // [batch + 1] rows before a request
     int* const taken = start + a.batch + 1;                            // [batch] pages before it
     unsigned *const seen = reinterpret_cast<unsigned*>(taken + a.batch), *const twice = seen + ((a.max_seqs + 31) >> 5);
-    const int tid = threadIdx.x, ps = a.page_size, shift = a.page_shift;
+    const int tid = threadIdx.x, threads = blockDim.x, ps = a.page_size, shift = a.page_shift;
     const bool first_block = blockIdx.x == 0;
     grid_dep_launch();
-    if (a.seqs) for (int i = tid; i < ((a.max_seqs + 31) >> 5) * 2; i += PG_THREADS) seen[i] = 0;
+    if (a.seqs) for (int i = tid; i < ((a.max_seqs + 31) >> 5) * 2; i += threads) seen[i] = 0;
     if (tid == 0) granted = 0;
     __syncthreads();
     grid_dep_wait();
     auto whole = [&](int64_t rows) { return (int)(shift >= 0 ? (rows + ps - 1) >> shift : (rows + ps - 1) / ps); };
 
-    // ---- the requests
+    // ---- the requests; a thread's first one is on its way while sequences that the call names twice are found (neither of their requests is served)
     const int have = min(max(a.state[0], 0), a.pages);
-    for (int b = tid; a.seqs && b < a.batch; b += PG_THREADS) {        // a sequence twice: neither request is served
-        const int s = a.seqs[b];
-        if ((unsigned)s < (unsigned)a.max_seqs && (atomicOr(seen + (s >> 5), 1u << (s & 31)) >> (s & 31) & 1)) atomicOr(twice + (s >> 5), 1u << (s & 31));
-    }
-    __syncthreads();
-    longlong2 base = make_longlong2(0, 0);
-    for (int b0 = 0; b0 < a.batch; b0 += PG_THREADS) {
-        const int b = b0 + tid;
-        PgRequest r = {-1, 0, 0, 0};
-        longlong2 mine = make_longlong2(0, 0);
-        int code = 0;
-        if (b < a.batch) {
-            r.seq = a.seqs ? a.seqs[b] : b;
-            const int n = a.asked[b];
-            if ((unsigned)r.seq >= (unsigned)a.max_seqs || (a.seqs && (twice[r.seq >> 5] >> (r.seq & 31) & 1))) { r.seq = -1; code = ERR_PG_SEQUENCE; }
-            else r.len = a.lens[r.seq];
-            const int64_t after = GROW ? (int64_t)r.len + n : n;
-            if (GROW && n > 0) mine.x = n;
-            if (r.seq >= 0 && (n < 0 || r.len < 0 || (GROW ? after : r.len) > (int64_t)a.width * ps || (!GROW && n > r.len))) { r.seq = -1; code = ERR_PG_LENGTH; }
-            if (r.seq >= 0) {
-                r.pages_before = whole(r.len);
-                r.pages_after = whole(after);
-                mine.y = GROW ? r.pages_after - r.pages_before : r.pages_before - r.pages_after;
-            }
+    int seq = -1, asked = 0, len = 0;
+    auto ask = [&](int b) {
+        if (b >= a.batch) return;
+        seq = a.seqs ? a.seqs[b] : b;
+        asked = a.asked[b];
+        len = (unsigned)seq < (unsigned)a.max_seqs ? a.lens[seq] : -1;
+    };
+    ask(tid);
+    if (a.seqs) {
+        for (int b = tid; b < a.batch; b += threads) {
+            const int s = b == tid ? seq : a.seqs[b];
+            if ((unsigned)s < (unsigned)a.max_seqs && (atomicOr(seen + (s >> 5), 1u << (s & 31)) >> (s & 31) & 1)) atomicOr(twice + (s >> 5), 1u << (s & 31));
         }
-        longlong2 all;
-        longlong2 before = pg_scan(mine, all, part);
-        before.x += base.x; before.y += base.y;
-        base.x += all.x; base.y += all.y;
+        __syncthreads();
+    }
+    int2 base = make_int2(0, 0);
+    for (int b0 = 0; b0 < a.batch; b0 += threads) {
+        const int b = b0 + tid;
+        if (b0 > 0) ask(b);
+        int2 mine = make_int2(0, 0);
+        int code = 0;
+        const int64_t after = GROW ? (int64_t)len + asked : asked;
+        if (b < a.batch) {
+            if (GROW) mine.x = min(max(asked, 0), PG_FULL);
+            if ((unsigned)seq >= (unsigned)a.max_seqs || (a.seqs && (twice[seq >> 5] >> (seq & 31) & 1))) { seq = -1; code = ERR_PG_SEQUENCE; }
+            else if (asked < 0 || len < 0 || (GROW ? after : len) > (int64_t)a.width * ps || (!GROW && asked > len)) { seq = -1; code = ERR_PG_LENGTH; }
+            else mine.y = GROW ? whole(after) - whole(len) : whole(len) - whole(after);
+        }
+        int2 all, before = pg_scan(mine, all, part);
+        before = make_int2(min(before.x + base.x, PG_FULL), min(before.y + base.y, PG_FULL));
+        base = make_int2(min(base.x + all.x, PG_FULL), min(base.y + all.y, PG_FULL));
         if (b < a.batch) {
             // Both sums only grow, so what is refused for want of rows or pages has behind it only requests that are too, or that need no page: pages leave the stack from its top.
-            if (GROW && r.seq >= 0 && before.x + mine.x > a.rows && mine.x > 0) { r.seq = -1; code = ERR_PG_LENGTH; }
-            if (r.seq >= 0 && mine.y > 0 && before.y + mine.y > (GROW ? have : a.pages - have)) { r.seq = -1; code = ERR_PG_NONE_LEFT; }
-            req[b] = r;
-            start[b] = (int)min(before.x, (long long)INT_MAX);
-            taken[b] = (int)min(before.y, (long long)INT_MAX);
-            if (r.seq >= 0 && mine.y > 0) atomicMax(&granted, (int)(before.y + mine.y));
+            if (GROW && seq >= 0 && mine.x > a.rows - before.x && mine.x > 0) { seq = -1; code = ERR_PG_LENGTH; }
+            if (seq >= 0 && mine.y > 0 && mine.y > (GROW ? have : a.pages - have) - before.y) { seq = -1; code = ERR_PG_NONE_LEFT; }
+            req[b] = {seq, len, (int)after};
+            start[b] = before.x;
+            taken[b] = before.y;
+            if (seq >= 0 && mine.y > 0) atomicMax(&granted, before.y + mine.y);
             if (first_block) {
                 if (code) atomicExch(a.bad, code);
                 if (GROW) {
                     a.starts[b] = start[b];
-                    a.lens_out[b] = r.seq >= 0 ? r.len + a.asked[b] : 0;
+                    a.lens_out[b] = seq >= 0 ? (int)after : 0;
                 }
             }
         }
+        if (b0 + threads < a.batch) __syncthreads();          // (the scan's sums are read)
     }
     if (tid == 0) {
-        start[a.batch] = (int)min(base.x, (long long)INT_MAX);
-        if (GROW && first_block) a.starts[a.batch] = start[a.batch];
+        start[a.batch] = base.x;
+        if (GROW && first_block) a.starts[a.batch] = base.x;
     }
     __syncthreads();
     const int total = granted, top = (GROW ? have : have + total) - 1;
@@ -136,7 +140,7 @@ pages_kernel(const PgArgs a) {
     // ---- the rows, four to a thread
     if (GROW) {
         const int known = min(start[a.batch], a.rows);
-        for (int64_t r0 = ((int64_t)blockIdx.x * PG_THREADS + tid) * 4; r0 < a.rows; r0 += (int64_t)gridDim.x * PG_THREADS * 4) {
+        for (int64_t r0 = ((int64_t)blockIdx.x * threads + tid) * 4; r0 < a.rows; r0 += (int64_t)gridDim.x * threads * 4) {
             long long slot[4];
             int pos[4], b = 0;
             if (r0 < known) {
@@ -158,7 +162,8 @@ pages_kernel(const PgArgs a) {
                 if (q.seq < 0) continue;
                 const int t = q.len + r - start[b], j = shift >= 0 ? t >> shift : t / ps;
                 if (owner != b || page_of != j) {
-                    page = j < q.pages_before ? a.table[(int64_t)q.seq * a.width + j] : a.free_pages[top - taken[b] - (j - q.pages_before)];
+                    const int known_pages = whole(q.len);
+                    page = j < known_pages ? a.table[(int64_t)q.seq * a.width + j] : a.free_pages[top - taken[b] - (j - known_pages)];
                     owner = b;
                     page_of = j;
                 }
@@ -175,27 +180,33 @@ pages_kernel(const PgArgs a) {
             }
         }
     }
-    // ---- the tables, PG_COLS entries to a warp
-    const int lane = tid & 31, pieces = (a.width + PG_COLS - 1) / PG_COLS;
-    for (int64_t task = (int64_t)blockIdx.x * (PG_THREADS / 32) + (tid >> 5); task < (int64_t)a.batch * pieces; task += (int64_t)gridDim.x * (PG_THREADS / 32)) {
+    // ---- the tables, PG_COLS entries to a warp, from the last warp on (the first ones have rows); a lane's entries all on their way before the first is stored
+    const int lane = tid & 31, pieces = (a.width + PG_COLS - 1) / PG_COLS, warps = threads / 32;
+    for (int64_t task = (int64_t)gridDim.x * warps - 1 - ((int64_t)blockIdx.x * warps + (tid >> 5)); task < (int64_t)a.batch * pieces; task += (int64_t)gridDim.x * warps) {
         const int b = (int)(task / pieces), j0 = (int)(task - (int64_t)b * pieces) * PG_COLS;
         const PgRequest q = req[b];
         int32_t* const row = a.table + (int64_t)max(q.seq, 0) * a.width;
         int32_t* const out = GROW && a.tables_out ? a.tables_out + b * a.ldp : nullptr;
-        const int lo = GROW ? q.pages_before : q.pages_after, hi = GROW ? q.pages_after : q.pages_before;         // pages that come or go
+        const int lo = whole(GROW ? q.len : q.after), hi = whole(GROW ? q.after : q.len);         // pages that come or go
         if (!out && (q.seq < 0 || j0 >= hi || j0 + PG_COLS <= lo)) continue;
+        int page[PG_COLS / 32];
+#pragma unroll
+        for (int i = 0; i < PG_COLS / 32; ++i) {
+            const int j = j0 + i * 32 + lane;
+            const bool moves = q.seq >= 0 && j >= lo && j < hi;
+            page[i] = -1;
+            if (GROW && moves) page[i] = a.free_pages[top - taken[b] - (j - lo)];
+            else if (GROW ? out && q.seq >= 0 && j < lo : moves) page[i] = row[j];
+        }
 #pragma unroll
         for (int i = 0; i < PG_COLS / 32; ++i) {
             const int j = j0 + i * 32 + lane;
             if (j >= a.width) break;
             const bool moves = q.seq >= 0 && j >= lo && j < hi;
-            if (GROW) {
-                int page = -1;
-                if (moves) row[j] = page = a.free_pages[top - taken[b] - (j - lo)];
-                else if (out && q.seq >= 0 && j < lo) page = row[j];
-                if (out) out[j] = page;
-            } else if (moves) {
-                a.free_pages[top - taken[b] - (j - lo)] = row[j];
+            if (GROW && moves) row[j] = page[i];
+            if (out) out[j] = page[i];
+            if (!GROW && moves) {
+                a.free_pages[top - taken[b] - (j - lo)] = page[i];
                 row[j] = -1;
             }
         }
@@ -203,18 +214,14 @@ pages_kernel(const PgArgs a) {
     // ---- lengths and the count of free pages, when all blocks have read them
     __syncthreads();
     if (tid == 0) {
-        bool mine = true;
-        if (gridDim.x > 1) {
-            __threadfence();
-            mine = atomicAdd(a.state + 1, 1) == (int)gridDim.x - 1;
-            __threadfence();
-        }
-        last = mine;
+        int before = gridDim.x - 1;
+        if (gridDim.x > 1) asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(a.state + 1) : "memory");
+        last = before == (int)gridDim.x - 1;
     }
     __syncthreads();
     if (!last) return;
-    for (int b = tid; b < a.batch; b += PG_THREADS)
-        if (req[b].seq >= 0) a.lens[req[b].seq] = GROW ? req[b].len + a.asked[b] : a.asked[b];
+    for (int b = tid; b < a.batch; b += threads)
+        if (req[b].seq >= 0) a.lens[req[b].seq] = req[b].after;
     if (tid == 0) {
         a.state[0] = top + 1 - (GROW ? total : 0);
         if (gridDim.x > 1) a.state[1] = 0;
@@ -237,7 +244,7 @@ static hd_status pages_view(const o1_kv_pages* p, PgArgs* a, const char* what) {
         set_error("%s: pages %d, page_size %d (a multiple of 16), max_seqs %d (at most %d), width %d", what, p->pages, p->page_size, p->max_seqs, PG_SEQS, p->width);
         return HD_ERR_UNSUPPORTED;
     }
-    if ((int64_t)p->width * p->page_size > INT_MAX) { set_error("%s: a table of %d pages of %d tokens is too large", what, p->width, p->page_size); return HD_ERR_UNSUPPORTED; }
+    if ((int64_t)p->width * p->page_size > PG_FULL || p->pages > PG_FULL) { set_error("%s: a table of %d pages of %d tokens, or a list of %d pages, is too large", what, p->width, p->page_size, p->pages); return HD_ERR_UNSUPPORTED; }
     *a = {};
     a->table = p->table; a->lens = p->lens; a->free_pages = p->free_pages; a->state = p->state;
     a->pages = p->pages; a->page_size = p->page_size; a->max_seqs = p->max_seqs; a->width = p->width;
@@ -255,9 +262,11 @@ static hd_status launch_pages(const PgArgs& a, const char* what) {
     static_assert(most <= 232448 - 1024, "more than an SM's block can have");
     if (!func_attr_once(done, (const void*)pages_kernel<GROW>, most, what)) return HD_ERR_RUNTIME;
     const size_t smem = a.batch * (sizeof(PgRequest) + 8) + 4 + (a.seqs ? ((a.max_seqs + 31) / 32) * 8 : 0);
+    // as many threads as there are requests or steps of the rows and tables, one block up to PG_THREADS
     const int64_t work = max((GROW ? (int64_t)a.rows : 0) / 4, (int64_t)a.batch * ((a.width + PG_COLS - 1) / PG_COLS) * 32);
-    const int blocks = (int)max((int64_t)1, min((int64_t)sm_count(), (work + PG_THREADS - 1) / PG_THREADS));
-    if (!launch_ok(launch_chained(pages_kernel<GROW>, dim3(blocks), dim3(PG_THREADS), smem, current_stream(), 1, 1, a), what)) return HD_ERR_RUNTIME;
+    const int threads = (int)min((int64_t)PG_THREADS, max((int64_t)a.batch, work) + 31 & ~(int64_t)31);
+    const int blocks = work <= 2 * PG_THREADS ? 1 : (int)min((int64_t)sm_count(), (work + PG_THREADS - 1) / PG_THREADS);
+    if (!launch_ok(launch_chained(pages_kernel<GROW>, dim3(blocks), dim3(max(threads, 32)), smem, current_stream(), 1, 1, a), what)) return HD_ERR_RUNTIME;
     return HD_OK;
 }
 
@@ -284,7 +293,7 @@ hd_status o1_kv_pages_grow(const o1_kv_pages* pages, const int32_t* seqs, const 
     PgArgs a;
     hd_status st = pages_view(pages, &a, "kv_pages_grow");
     if (st != HD_OK) return st;
-    if (batch < 0 || batch > a.max_seqs || rows < 0) { set_error("kv_pages_grow: batch %d (at most max_seqs %d), rows %d", batch, a.max_seqs, rows); return HD_ERR_UNSUPPORTED; }
+    if (batch < 0 || batch > a.max_seqs || rows < 0 || rows > PG_FULL) { set_error("kv_pages_grow: batch %d (at most max_seqs %d), rows %d (at most 2^30)", batch, a.max_seqs, rows); return HD_ERR_UNSUPPORTED; }
     if ((batch > 0 && (!counts || !lens)) || !starts || (rows > 0 && (!slots || !positions))) { set_error("kv_pages_grow: null argument"); return HD_ERR_MISSING; }
     if (tables && ldp < a.width) { set_error("kv_pages_grow: a row pitch is below the row"); return HD_ERR_UNSUPPORTED; }
     a.seqs = seqs; a.asked = counts; a.batch = batch; a.rows = rows;

@@ -19,13 +19,17 @@
 
 namespace o1 {
 
+// From so many (row, unit, head) triples for an SM on a thread has several heads' units, whose loads are under way while it finds their angles: four of bf16, two of fp32.
+// 16640 rows of 40 heads of bf16: one 66 us, two 63, four 53.8, five 52.9, eight 55.7; 4111 rows of 20 heads of fp32: one 16.8, two 14.2, four 14.7.  With few rows more threads
+// count: 1500 rows of 40 heads 9.5 us with one head to a thread, 5.3 with four; 700 rows 5.6 and 5.0, both the call's own time.
+static constexpr int ROPE_FEW = 1000;
 struct RopeSide { const void* x; void* y; int64_t ldx, ldy; int heads; };
 struct RopeArgs {
     RopeSide side[2];
     const uint64_t* turns;
     const void* positions;
     float factor;
-    int rows, head_dim, rot, heads, slots, units, per_thread, rows_a_block, wide_positions, inverse;      // units: pieces of a head; slots: threads of a row
+    int rows, head_dim, rot, heads, slots, units, rows_a_block, wide_positions, inverse;      // units: pieces of a head; slots: threads of a row
 };
 
 __device__ __forceinline__ void rope_angle(uint64_t turns, int64_t position, float factor, float& c, float& s) {
@@ -82,46 +86,54 @@ struct Piece<float, 1> {
 };
 
 // V values to a piece.  A unit is two pieces whose values pair up: V values and those half a rotation on (HALF), or 2 V neighbours; behind the turned ones, two pieces as they are.
-template <class T, int V, bool HALF>
+// A thread has one unit of N heads.
+template <class T, int V, bool HALF, int N>
 __global__ void __launch_bounds__(256)
 rotary_kernel(const RopeArgs a) {
     grid_dep_launch();
-    grid_dep_wait();
     const int local = threadIdx.x / a.slots;                                   // (slots <= 256: rows side by side in a block; else a row's slots over blockIdx.y)
     const int64_t row = (int64_t)blockIdx.x * a.rows_a_block + (a.rows_a_block > 1 ? local : 0);
     const int slot = a.rows_a_block > 1 ? threadIdx.x - local * a.slots : blockIdx.y * blockDim.x + threadIdx.x;
     if (row >= a.rows || slot >= a.slots || (a.rows_a_block > 1 && local >= a.rows_a_block)) return;
-    const int unit = slot % a.units, group = slot / a.units, turned = a.rot / 2 / V, half = a.rot / 2;
+    const int group = slot / a.units, unit = slot - group * a.units, turned = a.rot / 2 / V;
     const bool turns = unit < turned;
     const int at0 = turns ? (HALF ? unit * V : unit * 2 * V) : a.rot + (unit - turned) * 2 * V;
-    const int at1 = turns && HALF ? at0 + half : at0 + V;
+    const int at1 = turns && HALF ? at0 + a.rot / 2 : at0 + V;
     const bool two = at1 < a.head_dim;              // (behind the turned ones the last unit may have one piece)
-    float c[V], s[V];
-    if (turns) {
+    const int step = a.slots / a.units;             // heads side by side
+    const T* x[N];
+    T* y[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        int head = group + k * step;
+        const RopeSide& side = a.side[head >= a.side[0].heads];
+        if (head >= a.heads) { x[k] = nullptr; continue; }
+        if (head >= a.side[0].heads) head -= a.side[0].heads;
+        x[k] = (const T*)side.x + row * side.ldx + (int64_t)head * a.head_dim;
+        y[k] = (T*)side.y + row * side.ldy + (int64_t)head * a.head_dim;
+    }
+    grid_dep_wait();
+    Piece<T, V> p[N], q[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        if (!x[k]) continue;
+        p[k].load(x[k] + at0);
+        if (two) q[k].load(x[k] + at1);
+    }
+    if (turns) {             // while the values are on their way
         const int64_t position = a.wide_positions ? ((const int64_t*)a.positions)[row] : (int64_t)((const int32_t*)a.positions)[row];
+        float c[V], s[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             rope_angle(a.turns[unit * V + i], position, a.factor, c[i], s[i]);
             if (a.inverse) s[i] = -s[i];
         }
-    }
-    const int step = a.slots / a.units;             // heads side by side
-#pragma unroll 2
-    for (int k = 0; k < a.per_thread; ++k) {
-        int head = group + k * step;
-        if (head >= a.heads) break;
-        const bool second = head >= a.side[0].heads;
-        const RopeSide& side = a.side[second];
-        if (second) head -= a.side[0].heads;
-        const T* const x = (const T*)side.x + row * side.ldx + (int64_t)head * a.head_dim;
-        T* const y = (T*)side.y + row * side.ldy + (int64_t)head * a.head_dim;
-        Piece<T, V> p, q;
-        p.load(x + at0);
-        if (two) q.load(x + at1);
-        if (turns) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if (!x[k]) continue;
             float u[V], w[V], e[V], f[V];
-            p.get(u);
-            q.get(w);
+            p[k].get(u);
+            q[k].get(w);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const int j = 2 * i;
@@ -133,13 +145,25 @@ rotary_kernel(const RopeArgs a) {
                     if (j + 1 < V) e[(j + 1) % V] = x1; else f[(j + 1) % V] = x1;
                 }
             }
-            p.set(e);
-            q.set(f);
+            p[k].set(e);
+            q[k].set(f);
+            p[k].store(y[k] + at0);
+            q[k].store(y[k] + at1);
         }
-        p.store(y + at0);
-        if (two) q.store(y + at1);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if (!x[k]) continue;
+            p[k].store(y[k] + at0);
+            if (two) q[k].store(y[k] + at1);
+        }
     }
 }
+
+template <class T, int V, int N>
+static void (*rotary_of(bool half))(const RopeArgs) { return half ? rotary_kernel<T, V, true, N> : rotary_kernel<T, V, false, N>; }
+template <class T, int V>
+static void (*rotary_of(bool half, int heads))(const RopeArgs) { return heads == 1 ? rotary_of<T, V, 1>(half) : rotary_of<T, V, sizeof(T) == 2 ? 4 : 2>(half); }
 
 }  // namespace o1
 
@@ -222,14 +246,14 @@ hd_status o1_rotary(const o1_rope* rope, const void* positions, int wide_positio
         if (s.heads) vec = vec && (((uintptr_t)s.x | (uintptr_t)s.y) & 15) == 0 && s.ldx % wide == 0 && s.ldy % wide == 0;
     const int v = vec ? wide : 1;
     a.units = a.rot / 2 / v + (a.head_dim - a.rot + 2 * v - 1) / (2 * v);
-    a.per_thread = (int64_t)rows * a.units * a.heads >= (int64_t)sm_count() * 2048 * 4 ? 4 : 1;
-    a.slots = a.units * ((a.heads + a.per_thread - 1) / a.per_thread);
+    const int per_thread = (int64_t)rows * a.units * a.heads >= (int64_t)sm_count() * ROPE_FEW ? (size == 2 ? 4 : 2) : 1;
+    a.slots = a.units * ((a.heads + per_thread - 1) / per_thread);
     a.rows_a_block = a.slots <= 256 ? 256 / a.slots : 1;
     if (a.slots > 256 || a.rows_a_block < 1) a.rows_a_block = 1;
     const dim3 grid((unsigned)(((int64_t)rows + a.rows_a_block - 1) / a.rows_a_block), (unsigned)(a.rows_a_block > 1 ? 1 : (a.slots + 255) / 256));
     if (grid.y > 65535) { set_error("rotary: %d heads of %d are too many", a.heads, a.head_dim); return HD_ERR_UNSUPPORTED; }
-    auto kern = type == O1_ROPE_BF16 ? (vec ? (half ? rotary_kernel<uint16_t, 8, true> : rotary_kernel<uint16_t, 8, false>) : (half ? rotary_kernel<uint16_t, 1, true> : rotary_kernel<uint16_t, 1, false>))
-                                     : (vec ? (half ? rotary_kernel<float, 4, true> : rotary_kernel<float, 4, false>) : (half ? rotary_kernel<float, 1, true> : rotary_kernel<float, 1, false>));
+    auto kern = type == O1_ROPE_BF16 ? (vec ? rotary_of<uint16_t, 8>(half, per_thread) : rotary_of<uint16_t, 1>(half, per_thread))
+                                     : (vec ? rotary_of<float, 4>(half, per_thread) : rotary_of<float, 1>(half, per_thread));
     if (!launch_ok(launch_chained(kern, grid, dim3(256), 0, current_stream(), 1, 1, a), "rotary")) return HD_ERR_RUNTIME;
     o1_launch_count_add(1);
     return HD_OK;

@@ -28,8 +28,11 @@ KINDS = {"bf16": (0, torch.bfloat16), "fp8": (1, torch.float8_e4m3fn), "int8": (
 _BY_DTYPE = {d: n for n, d in KINDS.values()}
 BF16, I32, I64, F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
 _stream = lib.o1_get_stream
+Grown = namedtuple("Grown", "slots positions starts lens pages")
+Grown.__doc__ = """What KvPages.grow gives: slots [rows] int64 and positions [rows] int32 of the new rows, starts [requests + 1] (where each request's rows begin), lens [requests]
+and pages [requests, width] as KvCache.attend takes them."""
 _binding.setup(*(C.cast(f, C.c_void_p).value for f in (lib.o1_kv_write, lib.o1_kv_read, lib.o1_kv_attention, lib.o1_residual_norm, lib.o1_get_stream, lib.o1_capture_id,
-                                                       lib.o1_kv_pages_grow, lib.o1_kv_pages_shrink, lib.o1_rotary)), O1Error, check)
+                                                       lib.o1_kv_pages_grow, lib.o1_kv_pages_shrink, lib.o1_rotary)), O1Error, check, Grown)
 
 
 def _need(ok, what):
@@ -151,11 +154,6 @@ class KvCache:
         return _binding.attend(self._h, self, q, pages, lens, k, v, out, lse, scale)
 
 
-Grown = namedtuple("Grown", "slots positions starts lens pages")
-Grown.__doc__ = """What KvPages.grow gives: slots [rows] int64 and positions [rows] int32 of the new rows, starts [requests + 1] (where each request's rows begin), lens [requests]
-and pages [requests, width] as KvCache.attend takes them."""
-
-
 class KvPages:
     """Which pages of a cache sequences have, handed out on the GPU: table [max_seqs, width] (a sequence's pages in order, -1 behind them), lens [max_seqs] (its rows),
     free [pages] (a stack of free pages) and state [2] (how many are free; the calls' own), all int32.
@@ -181,7 +179,8 @@ class KvPages:
             _need(t.dtype is I32 and t.dim() == dim and t.is_cuda and t.device == table.device and t.is_contiguous() and 0 < t.numel() and max(t.shape) < 2 ** 31,
                   f"KvPages: {name} int32, of {dim} dimensions, contiguous, on one GPU wanted")
         _need(lens.size(0) == table.size(0) <= 8192 and state.size(0) == 2, "KvPages: lens [max_seqs], at most 8192, and state [2] wanted")
-        _need(0 < page_size < 2 ** 31 and page_size % 16 == 0 and table.size(1) * page_size < 2 ** 31, "KvPages: page_size must be a multiple of 16, and a table's rows fewer than 2^31")
+        _need(0 < page_size < 2 ** 31 and page_size % 16 == 0 and table.size(1) * page_size <= 2 ** 30 >= free.numel(),
+              "KvPages: page_size must be a multiple of 16, and a table's rows and the pages at most 2^30")
         self.table, self.lens, self.free, self.state, self.page_size = table, lens, free, state, page_size
         self.pages, self.max_seqs, self.width = free.size(0), *table.shape
         self.device = table.device
@@ -197,7 +196,7 @@ class KvPages:
 
         The requests' rows lie behind one another; rows behind the last one have slot -1.  A request that cannot be served (70: no such sequence, or named twice; 71: too many
         rows; 73: no pages left) has slots of -1 and a length of 0.  pages is the table itself where seqs is None."""
-        return Grown._make(_binding.pages_grow(self._at, self._gpu, self.table, counts, rows, seqs))
+        return _binding.pages_grow(self._at, self._gpu, self.table, counts, rows, seqs)
 
     def shrink(self, keep, seqs=None):
         """Sequences seqs [requests] int32 (None: 0, 1, ...) keep their first keep [requests] int32 rows; the pages behind them are free again."""
@@ -227,9 +226,8 @@ class Rotary:
                          (C.c_double * len(factors))(*factors) if factors else None)
         turns, factor = (C.c_uint64 * (rot_dim // 2))(), C.c_float()
         check(lib.o1_rope_turns(theta, rot_dim, C.byref(c), turns, C.byref(factor)), "o1_rope_turns")
-        signed = [t - 2 ** 64 if t >> 63 else t for t in turns]
         with _on_library(device):
-            self.turns = torch.tensor(signed, dtype=I64).to(device)
+            self.turns = torch.frombuffer(turns, dtype=I64).to(device)
         self.factor, self.head_dim, self.rot_dim, self.layout = factor.value, head_dim, rot_dim, layout
         self.c = RopeC(self.turns.data_ptr(), factor, head_dim, rot_dim, 0 if layout == "half" else 1)
         self._at, self._gpu = C.addressof(self.c), self.turns.get_device()
@@ -238,10 +236,6 @@ class Rotary:
         """Rows x [rows, heads, head_dim] bf16 or fp32 (rows of any pitch), or a pair of them (queries and keys), turned by positions [rows] int32 or int64.
 
         inverse: turned back, which is also the gradient.  out: what to fill, like x (x itself: in place)."""
-        if isinstance(x, tuple):
-            _need(len(x) == 2 and (out is None or len(out) == 2), "Rotary: a tensor or a pair of them")
-            y = (None, None) if out is None else out
-            return _binding.rotary(self._at, self._gpu, positions, inverse, x[0], y[0], x[1], y[1])
         return _binding.rotary(self._at, self._gpu, positions, inverse, x, out)
 
 

@@ -115,7 +115,7 @@ def test_growing_and_shrinking(pkg, dev, pages, page, seqs, width):
         rows = r.choice([total, total + 5, max(0, total - 3), total // 2])
         want = m.grow(counts, rows, names)
         got = p.grow(ints(counts, dev), rows, None if names is None else ints(names, dev))
-        starts = [min(s, 2 ** 31 - 1) for s in want[2]]
+        starts = [min(s, 2 ** 30) for s in want[2]]
         check(got, want[:2] + (starts,) + want[3:5], names is not None)
         if names is None:
             assert got.pages.data_ptr() == p.table.data_ptr()
@@ -234,7 +234,7 @@ def test_arguments_that_do_not_fit(pkg, dev):
         with pytest.raises(E, match="KvPages"):
             pkg.KvPages.over(*bad, 16)
     one = ints([1], dev)
-    for args in ((one.long(), 1), (one.cpu(), 1), (one[None], 1), (ints([1] * 5, dev), 5), (one, -1), (one, 2 ** 31), (ints([1] * 4, dev)[::2], 2), (one, 1, ints([0, 1], dev)),
+    for args in ((one.long(), 1), (one.cpu(), 1), (one[None], 1), (ints([1] * 5, dev), 5), (one, -1), (one, 2 ** 30 + 1), (one, 2 ** 31), (ints([1] * 4, dev)[::2], 2), (one, 1, ints([0, 1], dev)),
                  (one, 1, one.long())):
         with pytest.raises(E, match="KvPages.grow"):
             p.grow(*args)
