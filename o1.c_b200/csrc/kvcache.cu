@@ -342,7 +342,7 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
 static constexpr int KV_STAGE_BYTES = 8192;            // keys and values of a chunk
 static constexpr int KV_SEQS = 256;                    // sequences of a launch
 static constexpr int KV_TEAM = 4;                      // warps
-static constexpr int KV_TEAMS_MAX = 160 * 3;           // what the workspace has room for
+static constexpr int KV_TEAMS_MAX = 160 * 3, KV_UNITS_MAX = KV_TEAMS_MAX * KV_TEAM;      // what the workspace has room for: parts of teams, or of warps
 // Up to so many teams' parts of an item are joined at once (a part to a lane), more in groups of so many: 100003 tokens, 55 parts to an item, in two steps 48.1 us, at once 50.8 (then).
 static constexpr int KV_FLAT = 32, KV_FAN = 16;
 // What an item costs a team beside its chunks (the warps' join, the next queries), in chunks: 4, 7, 10, 12: batch 26.1, 25.5, 24.9, 24.5, shared 22.5, 20.0, 18.1, 17.8,
@@ -352,6 +352,18 @@ static constexpr int KV_ITEM_COST = 10;
 // Nor are those of a quarter of a team's part (half: 582 MB 104), and, where there are no more items than teams, of up to half more cost than a team has on average:
 // 51 sequences of 304 rows of bf16, 8 kv heads, 16.0, cut 20.6; 54 of 1000 of fp8 24.7 and 30.5; 55 of 100 to 700 of bf16 23.0 and 24.3.
 static constexpr int KV_KEEP = 16;
+#ifndef KL
+#define KL 2
+#endif
+#ifndef KK
+#define KK 2
+#endif
+#ifndef KC
+#define KC 2
+#endif
+// Four bits, parts of warps: a warp has at least so many chunks, items of so many are not cut, and an item costs so many beside its own (no barrier, no join within the block): a cost of
+// 1, 2, 4: 96 sequences of 300 to 5400 rows 62.9, 62.9, 64.7, 37 of 0 to 1999 19.8, 19.6, 21.8; kept 1, 2, 6: 62.9, 62.9, 63.4 and 19.6, 19.6, 20.5.
+static constexpr int KV4_LEAST = 2, KV4_KEEP = 2, KV4_ITEM_COST = 2;
 static constexpr int KV_SOLO = 16;                     // chunks of an item that a warp can have for itself (no item of KV_KEEP chunks is cut)
 static_assert(KV_SOLO <= KV_KEEP, "an item of a warp is whole");
 static constexpr int KV_JOIN_BYTES = 8192;             // of a team
@@ -568,12 +580,12 @@ __device__ __forceinline__ bool all_came(unsigned* counter, int wanted) {
     return true;
 }
 
-// The sums of `count` parts of HEADS heads (head, head + KV_TEAM, ... below `heads`), by a warp: the first part is `first`, the others in slot 0 of every `stride`-th
+// The sums of `count` parts of HEADS heads (head, head + APART, ... below `heads`), by a warp: the first part is `first`, the others in slot 0 of every `stride`-th
 // team behind it.  Into the result, or (to_out false) into the first one's place.  A lane has a part's weights; the first parts' rows are under way while the
 // weights are, and all heads' at once.
-template <int HEADS>
+template <int HEADS, int APART>
 __device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, int count, int b, int head, int heads, int head0, bool to_out) {
-    static_assert(KV_FLAT <= 32 && KV_FAN <= 32 && (KV_TEAMS_MAX + KV_FAN - 1) / KV_FAN <= 32, "a part to a lane");
+    static_assert(KV_FLAT <= 32 && KV_FAN <= 32 && (KV_TEAMS_MAX + KV_FAN - 1) / KV_FAN <= 32 && KV_UNITS_MAX <= 32 * 64, "a part to a lane");
     const int lane = threadIdx.x & 31;
     const int64_t step = (int64_t)2 * stride * a.per_item, at0 = (int64_t)first * a.per_item + head, at1 = (int64_t)(first & ~1) * a.per_item + head;
     float4* const mine = reinterpret_cast<float4*>(a.parts) + at0 * (KV_D / 4) + lane;
@@ -583,7 +595,7 @@ __device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, 
 #pragma unroll
     for (int h = 0; h < HEADS; ++h) {
         s[h] = make_float2(-INFINITY, 0.f);
-        if (lane < count && head + h * KV_TEAM < heads) s[h] = __ldcg(stats + h * KV_TEAM);
+        if (lane < count && head + h * APART < heads) s[h] = __ldcg(stats + h * APART);
     }
     float top[HEADS], sum[HEADS], w[HEADS];
     float4 r[HEADS];
@@ -596,7 +608,7 @@ __device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, 
 #pragma unroll
             for (int h = 0; h < HEADS; ++h) {
                 x[i][h] = make_float4(0, 0, 0, 0);
-                if (i0 + i < count && head + h * KV_TEAM < heads) x[i][h] = __ldcg(from + h * (KV_TEAM * KV_D / 4));
+                if (i0 + i < count && head + h * APART < heads) x[i][h] = __ldcg(from + h * (APART * KV_D / 4));
             }
         }
         if (i0 == 0) {
@@ -623,14 +635,14 @@ __device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, 
     }
 #pragma unroll
     for (int h = 0; h < HEADS; ++h) {
-        const int at = head + h * KV_TEAM;
+        const int at = head + h * APART;
         if (at >= heads) break;
         if (to_out) {
             store_row4(a.out + b * a.ldo + (head0 + at) * KV_D + lane * 4, r[h], 1.0f / sum[h], a.flags & 2);
             if (a.lse && lane == 0) a.lse[(int64_t)b * a.heads + head0 + at] = (top[h] - KV_LIFT + log2f(sum[h])) * 0.6931471805599453f;
         } else {
-            mine[h * (KV_TEAM * KV_D / 4)] = r[h];
-            if (lane == 0) a.stats[at0 + h * KV_TEAM] = make_float2(top[h], sum[h]);
+            mine[h * (APART * KV_D / 4)] = r[h];
+            if (lane == 0) a.stats[at0 + h * APART] = make_float2(top[h], sum[h]);
         }
     }
 }
@@ -917,12 +929,26 @@ struct KvFour {
     }
 };
 
-// solo: items of at most KV_SOLO chunks, each to one warp; "teams" are then warps.
+// The sums of any number of parts up to KV_UNITS_MAX by one warp: of more than a lane each, first those of the lanes' first parts, then of the others, then of both.
+template <int HEADS>
+__device__ __forceinline__ void kv_join_many(const KvAttn& a, int first, int stride, int count, int b, int heads, int head0, bool to_out) {
+#pragma unroll 1
+    for (int step = count > 32 ? 0 : 2; step < 3; ++step) {
+        const int from = step == 1 ? (first & ~1) + 64 * stride : first;
+        for (int head = 0; head < heads; head += HEADS)
+            kv_join<HEADS, 1>(a, from, step == 2 && count > 32 ? 32 * stride : stride, step == 0 ? 32 : step == 1 ? count - 32 : min(count, count > 32 ? 2 : 32), b, head, heads, head0, step == 2 && to_out);
+        __syncwarp();
+    }
+}
+
+// solo: items of at most KV_SOLO chunks, each to one warp; "teams" are then warps.  Of four bits: items of any length, and warps' parts that cut them as teams' parts do.
 template <int TYPE, int HG, bool solo>
 __global__ void __launch_bounds__(KvKernel<TYPE, HG>::THREADS, 1)
 kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ KvAttn a) {
     using K = KvKernel<TYPE, HG>;
     constexpr int KEYS = K::KEYS, TILES = K::TILES, WARPS = K::WARPS, STAGES = K::STAGES;
+    constexpr bool cuts = solo && TYPE == KV_UINT4;
+    constexpr int ITEM_COST = cuts ? KV4_ITEM_COST : KV_ITEM_COST;
     extern __shared__ __align__(1024) uint8_t smem[];
     auto& sh = *reinterpret_cast<typename K::Shared*>(smem + K::SHARED);
     const int warp = warp_index(), lane = threadIdx.x & 31, tid = threadIdx.x;
@@ -951,11 +977,11 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         if (len < 0 || len > (int64_t)a.width * ps) { atomicExch(a.bad, ERR_KV_LENGTH); len = 0; }
         const int n = (len + KEYS - 1) / KEYS;
         int2 all;
-        const int2 before = block_scan<WARPS + K::TEAMS>(make_int2(n, n > 0 ? n + KV_ITEM_COST : 0), all, sh.scan);
+        const int2 before = block_scan<WARPS + K::TEAMS>(make_int2(n, n > 0 ? n + ITEM_COST : 0), all, sh.scan);
         if (tid < a.batch) { sh.prefix[tid] = before.x; sh.cost[tid] = before.y; sh.len[tid] = len; }
         if (tid == 0) sh.prefix[a.batch] = all.x;
         all_chunks = all.x;
-        sequences = (all.y - all.x) / KV_ITEM_COST;      // that are not empty
+        sequences = (all.y - all.x) / ITEM_COST;      // that are not empty
         total = all.x * items;
         cost = all.y * items;
         __syncthreads();
@@ -964,9 +990,9 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     // (A team has at least four chunks, one to a warp; eight where sequences are long, which halves the parts to join: one sequence of 2000 rows of bf16 10.3 us, with four
     // 11.7; of 600 rows 9.1 and 8.5.)
     const int least = all_chunks > 48 * sequences ? 2 * KV_TEAM : KV_TEAM, most = gridDim.x * K::TEAMS, wanted = sequences * items;
-    const int teams = solo ? min(KV_TEAM * most, wanted) : min(most, max((total + least - 1) / least, wanted));       // (solo: warps)
+    const int teams = cuts ? min(KV_TEAM * most, max((total + KV4_LEAST - 1) / KV4_LEAST, wanted)) : solo ? min(KV_TEAM * most, wanted) : min(most, max((total + least - 1) / least, wanted));       // (solo: warps)
     const int share = teams > 0 ? total / teams : 0, each = teams > 0 ? cost / teams : 0, over = cost - each * teams;
-    const int keep = max(KV_KEEP, wanted <= most ? each + (each >> 1) - KV_ITEM_COST : share >> 2);
+    const int keep = cuts ? KV4_KEEP : max(KV_KEEP, wanted <= most ? each + (each >> 1) - ITEM_COST : share >> 2);
     auto cost_of = [&](int id) { return each * id + over * id / teams; };         // cost * id / teams, in 32 bits (over and id are below 1921)
     auto begin_of = [&](int id) {
         if (id >= teams) return total;
@@ -976,9 +1002,9 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             const int mid = (lo + hi + 1) >> 1;
             if (sh.cost[mid] * items <= at) lo = mid; else hi = mid - 1;
         }
-        const int n = sh.prefix[lo + 1] - sh.prefix[lo], rel = at - sh.cost[lo] * items, item = rel / (n + KV_ITEM_COST);
-        int c = rel - item * (n + KV_ITEM_COST);
-        if (n <= keep) c = 2 * c < n + KV_ITEM_COST ? 0 : n;      // the nearer end
+        const int n = sh.prefix[lo + 1] - sh.prefix[lo], rel = at - sh.cost[lo] * items, item = rel / (n + ITEM_COST);
+        int c = rel - item * (n + ITEM_COST);
+        if (n <= keep) c = 2 * c < n + ITEM_COST ? 0 : n;      // the nearer end
         else c = min(c, n);
         return sh.prefix[lo] * items + item * n + c;
     };
@@ -1159,16 +1185,18 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     if (solo || mate == 0) describe(c0, segs[0]);
     together();
     ask_queries(segs[0].b, segs[0].item);
-    if (!solo && mate == KV_TEAM - 1 && lane < 2) {
+    typename K::Share* const mine_shared = cuts ? reinterpret_cast<typename K::Share*>(smem + K::JOIN + 1024) + 2 * warp : sh.share[team];
+    const int unit = cuts ? (team * KV_TEAM + mate) * gridDim.x + blockIdx.x : id;
+    if ((cuts || (!solo && mate == KV_TEAM - 1)) && lane < 2) {
         // the items that the team's part begins and ends in, while the first rows are under way: teams from ... to share one, in groups of `fan`; the first
         // one's part is in slot `late`
         KvWalk w;
         w.seek(lane ? c1 - 1 : c0, sh.prefix, a.batch, items);
         const int f0 = (lane ? c1 - 1 : c0) - w.c;
-        typename K::Share& to = sh.share[team][lane];
+        typename K::Share& to = mine_shared[lane];
         if ((c0 <= f0 && f0 + w.n <= c1) || (lane && f0 <= c0)) to.here = 0;         // whole, or slot 0's
         else {
-            const int at = sh.cost[w.b] * items + w.item * (w.n + KV_ITEM_COST);
+            const int at = sh.cost[w.b] * items + w.item * (w.n + ITEM_COST);
             auto owner = [&](int v) {
                 int o = min(teams - 1, (int)((float)v * ((float)teams / (float)cost)));
                 while (cost_of(o) > v) --o;
@@ -1176,7 +1204,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 return o;
             };
             const int from = owner(at), last = owner(at + w.n - 1), late = f0 != begin_of(from), count = last - from + 1;
-            const int fan = count <= KV_FLAT ? count : KV_FAN, mine = (id - from) / fan, first = 2 * (from + mine * fan) + (mine == 0 ? late : 0);
+            const int fan = count <= KV_FLAT ? count : max(KV_FAN, (count + 31) / 32), mine = (unit - from) / fan, first = 2 * (from + mine * fan) + (mine == 0 ? late : 0);
             to = {first, min(fan, count - mine * fan), fan, 2 * from + late, (count + fan - 1) / fan, w.b, head_of(w.item), heads_of(w.item)};
         }
     }
@@ -1441,6 +1469,22 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         };
         auto columns_of = [](int i) { return TYPE == KV_UINT4 ? i : kv_perm(i); };
         auto column = [&](int quarter, int p) { return TYPE == KV_UINT4 ? 32 * quarter + 4 * p : (TYPE == KV_BF16 ? 64 * (quarter >> 1) + 8 * p : 8 * (quarter >> 1) + 16 * p) + (quarter & 1) * 4; };
+        if (cuts && (seg.begin != seg.first || seg.end != seg.first + seg.n)) {         // a part of an item
+            const int64_t at = (int64_t)(2 * unit + (seg.begin == c0 ? 0 : 1)) * a.per_item;
+#pragma unroll
+            for (int h = 0; h < HG; ++h) {
+                if (t == 0 && 8 * h + g < heads) a.stats[at + 8 * h + g] = make_float2(m[h], l[h]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int head = 8 * h + 2 * t + j;
+                    if (head >= heads) continue;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) *reinterpret_cast<float4*>(a.parts + (at + head) * KV_D + column(q, columns_of(g))) = four_columns(acc[h], q, j);
+                }
+            }
+            if (seg.end == c1) break;
+            continue;
+        }
         if (solo) {
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
@@ -1454,6 +1498,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                     for (int q = 0; q < 4; ++q) store_row4(a.out + seg.b * a.ldo + (head0 + head) * KV_D + column(q, columns_of(g)), four_columns(acc[h], q, j), inv, a.flags & 2);
                 }
             }
+            if (cuts && seg.end == c1) break;
             if (seg.end == c1) return;
             continue;
         }
@@ -1503,6 +1548,26 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         }
         if (seg.end == c1) break;
     }
+    if (cuts) {        // ---- items that the warp shares with others
+        __syncwarp();
+        const int here = lane < 2 ? mine_shared[lane].here : 0;
+        if (!__any_sync(0xffffffffu, here > 0)) return;
+        bool last = lane < 2 && here > 0 && all_came(a.arrived + mine_shared[lane].first, here);
+#pragma unroll 1
+        for (int level = 0; level < 2; ++level) {
+            const unsigned now = __ballot_sync(0xffffffffu, last);
+            if (!now) break;
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i) {
+                if (!(now >> i & 1)) continue;
+                const typename K::Share s = mine_shared[i];
+                kv_join_many<4>(a, level ? s.item : s.first, level ? s.fan : 1, level ? s.groups : s.here, s.b, s.heads, s.head0, level || s.groups == 1);
+            }
+            __syncwarp();
+            if (level == 0) last = last && mine_shared[lane].groups > 1 && all_came(a.arrived + 2 * KV_UNITS_MAX + mine_shared[lane].item, mine_shared[lane].groups);
+        }
+        return;
+    }
     // ---- items that the team shares with others: it is known for both at once whether all have come
     team_sync(team);
     const typename K::Share (&shares)[2] = sh.share[team];
@@ -1518,13 +1583,13 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             const typename K::Share s = shares[i];
             again |= level == 0 && s.groups > 1;
             for (int head = (mate - done) & (KV_TEAM - 1); head < s.heads; head += 2 * HG * KV_TEAM)
-                kv_join<2 * HG>(a, level ? s.item : s.first, level ? s.fan : 1, level ? s.groups : s.here, s.b, head, s.heads, s.head0, level || s.groups == 1);
+                kv_join<2 * HG, KV_TEAM>(a, level ? s.item : s.first, level ? s.fan : 1, level ? s.groups : s.here, s.b, head, s.heads, s.head0, level || s.groups == 1);
             done += s.heads;
         }
         if (!again) break;
         team_sync(team);
         if (mate == 0 && lane < 2 && sh.last[team][lane])       // the groups of an item
-            sh.last[team][lane] = shares[lane].groups > 1 && all_came(a.arrived + 2 * KV_TEAMS_MAX + shares[lane].item, shares[lane].groups);
+            sh.last[team][lane] = shares[lane].groups > 1 && all_came(a.arrived + 2 * KV_UNITS_MAX + shares[lane].item, shares[lane].groups);
         team_sync(team);
     }
 }
@@ -1540,6 +1605,14 @@ static cudaError_t launch_attention(const CUtensorMap& k_map, const CUtensorMap&
 template <int TYPE, int HG>
 static cudaError_t launch_attention(const CUtensorMap& k_map, const CUtensorMap& v_map, const KvAttn& a, int64_t item_chunks, int64_t items, cudaStream_t st) {
     const int most = min(sm_count(), KV_TEAMS_MAX / KvKernel<TYPE, HG>::TEAMS), teams = most * KvKernel<TYPE, HG>::TEAMS;
+    // Four bits: parts to warps, which need no barriers but leave more of an item to be joined at the end, where there is much work for each and items are not few, or items are
+    // short and many.  us, to warps and to teams (444 of them): 8 kv heads, 96 sequences of 300 to 5400 rows 62.9 and 65.9, 37 of up to 1999 19.5 and 20.9, 128 of up to 1000
+    // 27.3 and 33.7, 64 of 100 9.4 and 13.5, 128 of 60 8.3 and 19.5; but one of 100003 34.6 and 31.5, 16 of 2000 19.6 and 18.2, 32 of 200 13.2 and 9.3, 60 of up to 400 20.2 and 17.0.
+    if (TYPE == KV_UINT4) {
+        const bool much = 2 * items > teams && item_chunks * items > 16 * teams, many = items > teams && item_chunks * teams <= KV_TEAM * items;
+        if (much || many) return launch_attention<TYPE, HG, true>(k_map, v_map, a, most, st);
+        return launch_attention<TYPE, HG, false>(k_map, v_map, a, (int)max((int64_t)1, min((int64_t)most, max((item_chunks * items + KV_TEAM - 1) / KV_TEAM, items))), st);
+    }
     // A table of few tokens for more items than teams: an item to a warp, where its chunks one after the other take less than a team's items with their joins.
     // us, to warps and to teams: 200 sequences of 30 rows of fp8, 8 kv heads 7.7 and 20; 62 of 54 of bf16, 16 kv heads 9.7 and 12.7; 128 of up to 100 of bf16 11.6 and 13.3.
     // (Chosen on the device instead, by the lengths, it cost all other calls 0.4 us: one kernel with both.)
@@ -1637,7 +1710,7 @@ hd_status o1_kv_read(const o1_kv_cache* cache, void* k, int64_t ldk, void* v, in
 // Two counters and, for every head of an item, 128 values, a maximum and a sum, for each team's two parts.
 int64_t o1_kv_attention_workspace_bytes(int heads, int kv_heads) {
     if (heads <= 0 || kv_heads <= 0 || heads % kv_heads) return -1;
-    return (int64_t)KV_TEAMS_MAX * 2 * (2 * 4 + min(heads / kv_heads, 16) * (KV_D + 2) * 4);
+    return (int64_t)KV_UNITS_MAX * 2 * (2 * 4 + min(heads / kv_heads, 16) * (KV_D + 2) * 4);
 }
 
 hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, const void* k_new, int64_t ldk, const void* v_new, int64_t ldv,
@@ -1666,8 +1739,8 @@ hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, 
     a.c = c;
     a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldp = ldp; a.ldo = ldo;
     a.arrived = (unsigned*)workspace;
-    a.parts = (float*)(a.arrived + 4 * KV_TEAMS_MAX);
-    a.stats = (float2*)(a.parts + (int64_t)2 * KV_TEAMS_MAX * per_item * KV_D);
+    a.parts = (float*)(a.arrived + 4 * KV_UNITS_MAX);
+    a.stats = (float2*)(a.parts + (int64_t)2 * KV_UNITS_MAX * per_item * KV_D);
     a.heads = heads; a.group = group; a.chunks_of_heads = of_heads; a.per_item = per_item; a.width = width;
     a.scale = scale;
     a.err = device_error_word();

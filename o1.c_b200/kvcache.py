@@ -26,6 +26,7 @@ from . import HEAD_DIM, KV_HEADS, ROPE_THETA, KvCacheC, KvPagesC, O1Error, RopeC
 
 KINDS = {"bf16": (0, torch.bfloat16), "fp8": (1, torch.float8_e4m3fn), "int8": (2, torch.int8), "uint4": (4, torch.uint8)}
 _BY_DTYPE = {d: n for n, d in KINDS.values()}
+COUNTERS = 32768         # O1_KV_ATTENTION_COUNTERS: the bytes of a workspace that begin as zeros
 BF16, I32, I64, F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
 _stream = lib.o1_get_stream
 Grown = namedtuple("Grown", "slots positions starts lens pages")
@@ -58,7 +59,9 @@ class _Workspace:
     made, watched = {}, {}
 
     def __init__(self, device, nbytes):
-        self.scratch = _zeros(nbytes, device)
+        with _on_library(device):
+            self.scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            self.scratch[:COUNTERS].zero_()
         self.address = self.scratch.data_ptr()
 
     def data_ptr(self):
