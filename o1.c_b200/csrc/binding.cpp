@@ -80,6 +80,12 @@ struct Several {
         return t;
     }
 };
+// Launches go to the current GPU: from there, memory of another one is out of reach, or a fault.
+bool current(int device, const char* who) {
+    if (c10::cuda::current_device() == device) return true;
+    fail(who, "its memory is on another GPU than the current one");
+    return false;
+}
 bool bf16_on(const at::Tensor& t, int device) { return t.scalar_type() == at::kBFloat16 && t.is_cuda() && t.device().index() == device; }
 
 // bf16 rows [n, heads, 128] whose heads lie side by side; n < 0: any number
@@ -349,6 +355,7 @@ PyObject* py_grow(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!arguments(n, 6)) return nullptr;
     const auto* pages = (const o1_kv_pages*)PyLong_AsUnsignedLongLong(a[0]);
     const int device = (int)PyLong_AsLong(a[1]);
+    if (!current(device, who)) return nullptr;
     const at::Tensor *table = tensor(a[2], who), *counts = table ? ints(a[3], -1, device, who, "counts") : nullptr;
     if (!counts) return nullptr;
     const int64_t rows = PyLong_AsLongLong(a[4]), batch = counts->size(0);
@@ -383,6 +390,7 @@ PyObject* py_shrink(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const auto* pages = (const o1_kv_pages*)PyLong_AsUnsignedLongLong(a[0]);
     const int device = (int)PyLong_AsLong(a[1]);
     if (PyErr_Occurred()) return nullptr;
+    if (!current(device, who)) return nullptr;
     const at::Tensor *keep = ints(a[2], -1, device, who, "keep"), *seqs = nullptr;
     if (!keep) return nullptr;
     if (keep->size(0) > pages->max_seqs) return fail(who, "more requests than sequences");
@@ -403,7 +411,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int device = (int)PyLong_AsLong(a[1]), inverse = PyObject_IsTrue(a[3]), sides = pair ? 2 : 1;
     if (PyErr_Occurred()) return nullptr;
     const at::Tensor* positions = tensor(a[2], who);
-    if (!positions) return nullptr;
+    if (!positions || !current(device, who)) return nullptr;
     const bool wide = positions->scalar_type() == at::kLong;
     if ((!wide && positions->scalar_type() != at::kInt) || positions->dim() != 1 || !positions->is_contiguous() || !positions->is_cuda() || positions->device().index() != device ||
         positions->size(0) > INT32_MAX)

@@ -659,7 +659,7 @@ __device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, 
 //    scale bounds it) is between 2^90 and 2^112, and weights of 2^-80 of that one are still there.  Largest weight and k follow the running maximum, and k moves seldom.
 template <int HG>
 struct KvFour {
-    float zs[HG][2], q_sum[HG][2], m[HG][2], l[HG][2], offset[HG][2], most[HG][2];       // of heads 8 h + 2 t, 2 t + 1
+    float zs[HG][2], q_sum[HG][2], m[HG][2], l[HG][2], offset[HG][2], most[HG][2];       // of heads 8 h + 2 t, 2 t + 1; m in the scores' units, zs of them are one in base 2
     int k[HG][2];
 
     __device__ __forceinline__ void begin(uint32_t (&q)[HG][16], float scale, float (&acc)[HG][8][4]) {
@@ -796,19 +796,20 @@ struct KvFour {
                 for (int n = 0; n < MINE; ++n) top = fmaxf(top, s[TWICE ? n : n >> 1][h][(TWICE ? 0 : 2 * (n & 1)) + c]);
 #pragma unroll
                 for (int o = TWICE ? 2 : 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                const float m_new = fmaxf(m[h][c], top * zs[h][c]), ref = (m_new == -INFINITY ? 0.f : m_new) - KV_LIFT;
-                float a = exp2_fast(m[h][c] - KV_LIFT - ref);
+                // (differences before the factor: of scores of any size, the largest one's exponent is exactly the lift)
+                const float m_new = fmaxf(m[h][c], top), ref = m_new == -INFINITY ? 0.f : m_new;
+                float a = exp2_fast((m[h][c] - ref) * zs[h][c]);
                 m[h][c] = m_new;
                 float sum = 0.f;
 #pragma unroll
                 for (int n = 0; n < MINE; ++n) {
                     float& z = s[TWICE ? n : n >> 1][h][(TWICE ? 0 : 2 * (n & 1)) + c];
-                    z = exp2_fast(__fmaf_rn(z, zs[h][c], -ref));
+                    z = exp2_fast(__fmaf_rn(z - ref, zs[h][c], KV_LIFT));
                     sum += z;
                 }
                 l[h][c] = l[h][c] * a + sum;
                 offset[h][c] *= a;
-                most[h][c] = fmaxf(most[h][c] * a, exp2_fast(__fmaf_rn(top, zs[h][c], -ref)) * __uint_as_float(s_top));
+                most[h][c] = fmaxf(most[h][c] * a, exp2_fast(__fmaf_rn(top - ref, zs[h][c], KV_LIFT)) * __uint_as_float(s_top));
                 const int e = (int)(__float_as_uint(most[h][c]) >> 23) - 127;
                 if ((unsigned)(e + k[h][c] - 90) > 21u) {
                     const int k_new = min(min(max(101 - e, -27), 127), k[h][c] + 100);
@@ -858,41 +859,43 @@ struct KvFour {
             }
         }
         // out^T += V^T P^T, 16 keys a step.  A matrix of eight rows and 32 columns, in two-byte pieces of four columns, is loaded transposed: this thread gets columns 4 g ... + 3 of two rows
-        // beside each other, as the product wants them.  A tile's rows g are even columns, g + 8 odd ones, which are 16 times as large.
+        // beside each other, as the product wants them.  Two steps to a turn of the loop: with all four its instructions outgrow the nearest cache (96 sequences 81 us, then 73).  A tile's rows g are even columns, g + 8 odd ones, which are 16 times as large.
         const int row = (lane & 8) + kv4_key(lane & 7);
         const uint32_t values = st + 4096 + (row >> 1) * 128 + ((((row & 1) * 4 + (lane >> 4)) ^ (row >> 1 & 7)) << 4);
 #pragma unroll 1
         for (int u0 = 0; u0 < 4; u0 += 2) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            uint32_t x[2][4];
-            ldmatrix_trans(x[0], values + (u0 + u) * 1024);
-            ldmatrix_trans(x[1], (values ^ 32) + (u0 + u) * 1024);
-#pragma unroll
-            for (int h = 0; h < HG; ++h) {
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    hi[u][h][r] = transposed(hi[u][h][r]);
-                    if (!TWICE) lo[u][h][r] = transposed(lo[u][h][r]);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                uint32_t a = x[j >> 2][j & 2], b = x[j >> 2][(j & 2) + 1];
-                if (j & 1) { a >>= 8; b >>= 8; }
+            for (int u = 0; u < 2; ++u) {
+                uint32_t x[2][4];
+                ldmatrix_trans(x[0], values + (u0 + u) * 1024);
+                ldmatrix_trans(x[1], (values ^ 32) + (u0 + u) * 1024);
 #pragma unroll
                 for (int h = 0; h < HG; ++h) {
-                    mma_bf16(acc[h][j], a & 0x000F000Fu, a & 0x00F000F0u, b & 0x000F000Fu, b & 0x00F000F0u, hi[u][h][0], hi[u][h][1]);
-                    if (!TWICE) mma_bf16(acc[h][j], a & 0x000F000Fu, a & 0x00F000F0u, b & 0x000F000Fu, b & 0x00F000F0u, lo[u][h][0], lo[u][h][1]);
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        hi[u][h][r] = transposed(hi[u][h][r]);
+                        if (!TWICE) lo[u][h][r] = transposed(lo[u][h][r]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    uint32_t a = x[j >> 2][j & 2], b = x[j >> 2][(j & 2) + 1];
+                    if (j & 1) { a >>= 8; b >>= 8; }
+#pragma unroll
+                    for (int h = 0; h < HG; ++h) {
+                        mma_bf16(acc[h][j], a & 0x000F000Fu, a & 0x00F000F0u, b & 0x000F000Fu, b & 0x00F000F0u, hi[u][h][0], hi[u][h][1]);
+                        if (!TWICE) mma_bf16(acc[h][j], a & 0x000F000Fu, a & 0x00F000F0u, b & 0x000F000Fu, b & 0x00F000F0u, lo[u][h][0], lo[u][h][1]);
+                    }
                 }
             }
-        }
 #pragma unroll
-        for (int u = 0; u + 2 < 4; ++u)
+            for (int u = 0; u < 2; ++u) {
 #pragma unroll
-            for (int h = 0; h < HG; ++h)
+                for (int h = 0; h < HG; ++h) {
 #pragma unroll
-                for (int r = 0; r < 2; ++r) { hi[u][h][r] = hi[u + 2][h][r]; if (!TWICE) lo[u][h][r] = lo[u + 2][h][r]; }
+                    for (int r = 0; r < 2; ++r) { hi[u][h][r] = hi[u + 2][h][r]; if (!TWICE) lo[u][h][r] = lo[u + 2][h][r]; }
+                }
+            }
         }
     }
 
@@ -920,7 +923,7 @@ struct KvFour {
                     acc[h][j][c] = __fmaf_rn(acc[h][j][c] * 8589934592.0f, down, offset[h][c]);            // 2^33
                     acc[h][j][c + 2] = __fmaf_rn(acc[h][j][c + 2] * 536870912.0f, down, offset[h][c]);     // 2^29
                 }
-                m_of[c] = __shfl_sync(0xffffffffu, m[h][c], from);
+                m_of[c] = __shfl_sync(0xffffffffu, m[h][c] * zs[h][c], from);
                 l_of[c] = __shfl_sync(0xffffffffu, l[h][c], from);
             }
             m_out[h] = g & 1 ? m_of[1] : m_of[0];

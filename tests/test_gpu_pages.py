@@ -222,6 +222,29 @@ def test_captured_requests(pkg, dev):
 
 
 @gpu
+def test_calls_on_another_stream_than_torch_s(pkg, dev):
+    """What a call makes is in the order of the library's stream, and lives as long as any part of it."""
+    p, m, s = pkg.KvPages(200, 16, 8, 12, dev), Model(200, 16, 8, 12), torch.cuda.Stream()
+    counts, names = ints([30, 2, 7], dev), ints([1, 2, 3], dev)
+    torch.cuda.synchronize()
+    try:
+        with torch.cuda.stream(s):
+            pkg.use_torch_stream()
+        slots, lens = [], []
+        for _ in range(20):
+            got = p.grow(counts, 39, names)
+            slots.append(got.slots), lens.append(got.lens)
+            p.shrink(ints([0, 0, 0], dev), names)
+            torch.cuda.synchronize()
+        del got
+        junk = [torch.full((4096,), 77, dtype=torch.int32, device=dev) for _ in range(20)]
+    finally:
+        pkg.use_torch_stream()
+    want = m.grow([30, 2, 7], 39, [1, 2, 3])
+    assert all(t.tolist() == want[0] for t in slots) and all(t.tolist() == want[3] for t in lens) and len(junk) == 20
+
+
+@gpu
 def test_arguments_that_do_not_fit(pkg, dev):
     E = pkg.O1Error
     for args in ((0, 16, 1, 1), (4, 24, 2, 2), (4, 16, 9000, 2), (4, 16, 0, 1), (4, 0, 1, 1), (4, 2 ** 24, 1, 2 ** 10)):

@@ -277,6 +277,35 @@ def test_rows_far_from_zero_and_constant_rows(pkg, dev, group):
 
 
 @gpu
+@pytest.mark.parametrize("lens,kv_heads,group", [([70, 700], 1, 4), ([300, 5], 2, 8), ([900, 64], 1, 16), ([100] * 300, 2, 4)])
+def test_queries_that_are_not_finite_or_huge(pkg, dev, lens, kv_heads, group):
+    """A NaN or Inf in a query's head reaches that head's result and no other; queries of 2^-120 and 2^120 among others."""
+    c = Case4(pkg, dev, "uint4", lens, kv_heads, 32, seed=8)
+    c.fill()
+    q = normal((len(lens), kv_heads * group, D), gen(3), 1.5)
+    want, want_l = c.cache.attend(q.to(dev), c.dtable, c.dlens, lse=True)
+    bad = q.clone()
+    bad[0, 1, 5], bad[1, 0, 127], bad[1, 3] = math.nan, math.inf, q[1, 3] * 2.0 ** -120
+    out, lse = c.cache.attend(bad.to(dev), c.dtable, c.dlens, lse=True)
+    for b, h in ((0, 1), (1, 0)):
+        assert not torch.isfinite(out[b, h].float()).any() and not torch.isfinite(lse[b, h])
+    keep = torch.ones(q.shape[:2], dtype=torch.bool)
+    keep[0, 1] = keep[1, 0] = keep[1, 3] = False
+    assert torch.equal(out[keep.to(dev)], want[keep.to(dev)]) and torch.equal(lse[keep.to(dev)], want_l[keep.to(dev)])
+    bad = q.clone()
+    bad[1, 3], bad[0, 2] = q[1, 3] * 2.0 ** -120, 0.0
+    bad[0, 0] = q[0, 0] * 2.0 ** 120          # its largest score takes all
+    out, lse = c.cache.attend(bad.to(dev), c.dtable, c.dlens, lse=True)
+    assert torch.isfinite(out.float()).all()
+    got, ref = out[0, 0].cpu().double(), value(*kept(c.v[0][:, 0]))
+    assert ((got[None] - ref).abs().amax(1) <= 2.0 ** -8 * ref.abs().amax()).any()
+    q[0, 0] = 0.0
+    bad[0, 0] = 0.0
+    out, lse = c.cache.attend(bad.to(dev), c.dtable, c.dlens, lse=True)
+    c.check(bad, out, lse)
+
+
+@gpu
 def test_offsets_past_32_bits(pkg, dev):
     """A cache of more than 2^32 bytes of codes, with rows at its end."""
     heads, page = 8, 128
