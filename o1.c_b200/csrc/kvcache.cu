@@ -189,7 +189,8 @@ __device__ __forceinline__ void store8(uint16_t* p, const uint4& v) {
 // unit's place and scale, and the maxima are found for all units at once: with four exchanges for each and divisions in every lane the write's instructions
 // (135 a unit, now 100) took longer than its bytes, 22.8 us.  Written and read, us: 16640 rows of 8 heads of int8 18.9 + 18.7 (5.5 TB/s), 100000 rows of one head
 // 15.2 + 15.1; a row to a warp 23.5 + 19.5 and 43 + 39, a head to a half warp 34 + 35 for the former.  Few rows have more warps with two units: 1800 rows of
-// 8 heads 3.5 + 3.7, with eight 5.3 + 4.0; 2600 rows 4.5 + 4.7 and 4.3 + 4.3; 4111 rows 6.9 + 7.5 and 5.8 + 6.2.
+// 8 heads 3.5 + 3.7, with eight 5.3 + 4.0; 2600 rows 4.5 + 4.7 and 4.3 + 4.3; 4111 rows 6.9 + 7.5 and 5.8 + 6.2.  Of four bits, 16640 rows of 8 heads: 19 + 16, the write bound by its
+// instructions (110 a unit, 2.9 a clock and SM; the sums of two extremes in place of one), the read by HBM.
 // Launches overlap at any size (the next one is let in once the rows have been asked for: its blocks, placed earlier, leave these unevenly spread, 1000 rows 5.1 us, so
 // 4.1): written and read through a stream, 4111 rows 14.4 us without, 12.4 with; 16640 42.7 and 38.
 static constexpr int KV_EACH = 8, KV_EACH_OF_FEW = 2, KV_FEW_UNITS = 19200;
@@ -338,6 +339,10 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
 //  * Rounding: scores and sums in fp32.  Probabilities (times v's scale) enter the second product as two parts of bf16, value and rest, 16 bits of significand; codes
 //    of a byte are exact in f16 and bf16.  Keys' codes go through f16, which takes fewer instructions, with queries scaled to f16's top by a power of two for each head (those
 //    below 2^-29 of its largest lose bits); values' codes through bf16, whose range a probability needs.  The result is rounded once.
+//  * Rows of four bits (KvFour) are 64 to a chunk and the chunks, for the same bytes, twice the arithmetic: instructions bound them, not memory.  302 MB (96 sequences of 300 to 5400
+//    rows, 8 kv heads, 32 heads) in 63 us, 4.8 TB/s, 73 % of a copy's rate; 109 MB (one of 100003) in 31.5; 39.7 MB (37 of 0 to 1999, 16 heads) in 19.6.  A chunk is 990
+//    instructions (all of a launch's counted), of which an SM issues 2.2 a clock; half of the ALU pipe's time is the codes' masks and shifts.  As the other kinds have it (queries
+//    as rows, codes to pairs of keys by byte permutes) it was 1420 and 99 us.
 // Times below: "batch" 24 sequences of 1 to 2100 rows of bf16, "shared" 32 sequences of 1000 to 3000, 16 query heads on one kv head; us.
 static constexpr int KV_STAGE_BYTES = 8192;            // keys and values of a chunk
 static constexpr int KV_SEQS = 256;                    // sequences of a launch

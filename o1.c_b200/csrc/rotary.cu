@@ -8,8 +8,8 @@
 // position * 2^-65 turns however far out.  Its upper bits are reduced to an eighth of a turn around the nearest quarter (integers), and the Taylor polynomials of sine and
 // cosine to the 9th and 8th power, whose rest is below 2.5e-8 there, do what remains.
 //
-// HBM bound: values in, values out.  A thread has one 16-byte piece of a head (and its partner), finds those angles once and turns that piece of several heads with them, the
-// loads of two heads ahead of their arithmetic.
+// HBM bound: values in, values out; 341 MB (16640 rows of 32 + 8 heads of bf16) in 53.9 us, 6.3 TB/s, 97 % of a copy's rate; 84 MB (4111 rows of 16 + 4 heads of fp32, half of each head
+// turned) in 14.2.  A thread has one 16-byte piece of a head and its partner, of several heads: all its loads are under way while it finds the piece's angles, once for all heads.
 #include "common.cuh"
 #include "kernels.h"
 #include "../../include/o1_b200.h"
