@@ -489,6 +489,24 @@ __device__ __forceinline__ void team_sync(int team) { asm volatile("bar.sync %0,
 // Of eight: 0 2 4 6 1 3 5 7's inverse.  Rows kv_perm(2m) and kv_perm(2m + 1) lie four apart, as the swizzle wants them.
 __device__ __forceinline__ int kv_perm(int i) { return (i >> 1) | (i & 1) << 2; }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 // Rows of 64 bytes, two to a swizzled line of 128: of eight, 0 3 1 2 4 7 5 6.  Neighbours n = 2m, 2m + 1 (a step of the keys' loads) lie in different halves of their lines, and so do
 // two each of the four rows at even or odd n (a step of the values' loads), in lines whose swizzles differ: no bank is met twice.
 __device__ __forceinline__ int kv4_even(int m) { return (m & 1) | (m & 2) << 1; }            // of n = 2m; n = 2m + 1: the same ^ 3
@@ -664,7 +682,8 @@ __device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, 
 //    scale bounds it) is between 2^90 and 2^112, and weights of 2^-80 of that one are still there.  Largest weight and k follow the running maximum, and k moves seldom.
 template <int HG>
 struct KvFour {
-    float zs[HG][2], q_sum[HG][2], m[HG][2], l[HG][2], offset[HG][2], most[HG][2];       // of heads 8 h + 2 t, 2 t + 1; m in the scores' units, zs of them are one in base 2
+    float2 zs[HG], q_sum[HG], l[HG], offset[HG];       // of heads 8 h + 2 t, 2 t + 1
+    float m[HG][2], most[HG][2];       // m in the scores' units, zs of them are one in base 2
     int k[HG][2];
 
     __device__ __forceinline__ void begin(uint32_t (&q)[HG][16], float scale, float (&acc)[HG][8][4]) {
@@ -690,12 +709,13 @@ struct KvFour {
             for (int i = 0; i < 16; ++i) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(q[h][i]) : "r"(i & 1 ? up16 : up));
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                zs[h][c] = __shfl_sync(0xffffffffu, z, 8 * t + 4 * c);
+                (c ? zs[h].y : zs[h].x) = __shfl_sync(0xffffffffu, z, 8 * t + 4 * c);
                 // (the shuffled exponent: x of that head)
                 const int x_of = __shfl_sync(0xffffffffu, x, 8 * t + 4 * c);
-                q_sum[h][c] = sum[c] * __uint_as_float((uint32_t)(127 + x_of - 70) << 23) * __uint_as_float((uint32_t)(127 - 63) << 23);
+                (c ? q_sum[h].y : q_sum[h].x) = sum[c] * __uint_as_float((uint32_t)(127 + x_of - 70) << 23) * __uint_as_float((uint32_t)(127 - 63) << 23);
                 m[h][c] = -INFINITY;
-                l[h][c] = offset[h][c] = most[h][c] = 0.f;
+                l[h] = offset[h] = both(0.f);
+                most[h][c] = 0.f;
                 k[h][c] = 101;
             }
 #pragma unroll
@@ -766,11 +786,10 @@ struct KvFour {
             const uint32_t pair = kpair[n];
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    float& z = s[TWICE ? n : n >> 1][h][(TWICE ? 0 : 2 * (n & 1)) + c];
-                    z = __fmaf_rn(z, bf16lo(pair), bf16hi(pair) * q_sum[h][c]);
-                }
+                float* const z = s[TWICE ? n : n >> 1][h] + (TWICE ? 0 : 2 * (n & 1));
+                const float2 r = fma2(make_float2(z[0], z[1]), both(bf16lo(pair)), mul2(both(bf16hi(pair)), q_sum[h]));
+                z[0] = r.x;
+                z[1] = r.y;
             }
         }
         uint32_t s_top = 0;           // the largest of the values' scales, as bits
@@ -791,68 +810,79 @@ struct KvFour {
             }
         }
         bool moved = false;
-        float alpha[HG][2];
+        float2 alpha[HG];
 #pragma unroll
         for (int h = 0; h < HG; ++h) {
+            float top[2], ref[2], a[2];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float top = -INFINITY;
+                top[c] = -INFINITY;
 #pragma unroll
-                for (int n = 0; n < MINE; ++n) top = fmaxf(top, s[TWICE ? n : n >> 1][h][(TWICE ? 0 : 2 * (n & 1)) + c]);
+                for (int n = 0; n < MINE; ++n) top[c] = fmaxf(top[c], s[TWICE ? n : n >> 1][h][(TWICE ? 0 : 2 * (n & 1)) + c]);
 #pragma unroll
-                for (int o = TWICE ? 2 : 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                for (int o = TWICE ? 2 : 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
                 // (differences before the factor: of scores of any size, the largest one's exponent is exactly the lift)
-                const float m_new = fmaxf(m[h][c], top), ref = m_new == -INFINITY ? 0.f : m_new;
-                float a = exp2_fast((m[h][c] - ref) * zs[h][c]);
+                const float m_new = fmaxf(m[h][c], top[c]);
+                ref[c] = m_new == -INFINITY ? 0.f : m_new;
+                a[c] = exp2_fast((m[h][c] - ref[c]) * (c ? zs[h].y : zs[h].x));
                 m[h][c] = m_new;
-                float sum = 0.f;
+            }
+            const float2 less = make_float2(-ref[0], -ref[1]);
+            float2 sum = both(0.f);
 #pragma unroll
-                for (int n = 0; n < MINE; ++n) {
-                    float& z = s[TWICE ? n : n >> 1][h][(TWICE ? 0 : 2 * (n & 1)) + c];
-                    z = exp2_fast(__fmaf_rn(z - ref, zs[h][c], KV_LIFT));
-                    sum += z;
-                }
-                l[h][c] = l[h][c] * a + sum;
-                offset[h][c] *= a;
-                most[h][c] = fmaxf(most[h][c] * a, exp2_fast(__fmaf_rn(top - ref, zs[h][c], KV_LIFT)) * __uint_as_float(s_top));
+            for (int n = 0; n < MINE; ++n) {
+                float* const z = s[TWICE ? n : n >> 1][h] + (TWICE ? 0 : 2 * (n & 1));
+                const float2 r = fma2(add2(make_float2(z[0], z[1]), less), zs[h], both(KV_LIFT));
+                z[0] = exp2_fast(r.x);
+                z[1] = exp2_fast(r.y);
+                sum = add2(sum, make_float2(z[0], z[1]));
+            }
+            alpha[h] = make_float2(a[0], a[1]);
+            l[h] = fma2(l[h], alpha[h], sum);
+            offset[h] = mul2(offset[h], alpha[h]);
+            const float2 r = fma2(add2(make_float2(top[0], top[1]), less), zs[h], both(KV_LIFT));
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                most[h][c] = fmaxf(most[h][c] * a[c], exp2_fast(c ? r.y : r.x) * __uint_as_float(s_top));
                 const int e = (int)(__float_as_uint(most[h][c]) >> 23) - 127;
                 if ((unsigned)(e + k[h][c] - 90) > 21u) {
                     const int k_new = min(min(max(101 - e, -27), 127), k[h][c] + 100);
-                    a *= exp2_fast((float)(k_new - k[h][c]));
+                    a[c] *= exp2_fast((float)(k_new - k[h][c]));
                     k[h][c] = k_new;
                 }
-                moved = moved || a != 1.f;
-                alpha[h][c] = a;
+                moved = moved || a[c] != 1.f;
             }
+            alpha[h] = make_float2(a[0], a[1]);
         }
         if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) { acc[h][j][0] *= alpha[h][0]; acc[h][j][1] *= alpha[h][1]; acc[h][j][2] *= alpha[h][0]; acc[h][j][3] *= alpha[h][1]; }
+                for (int j = 0; j < 8; ++j) {
+#pragma unroll
+                    for (int c = 0; c < 4; c += 2) {
+                        const float2 r = mul2(make_float2(acc[h][j][c], acc[h][j][c + 1]), alpha[h]);
+                        acc[h][j][c] = r.x;
+                        acc[h][j][c + 1] = r.y;
+                    }
+                }
             }
         }
         // weights, in two parts of bf16; [tile of 16 keys][its upper 8 keys]
-        float up[HG][2];
+        float2 up[HG];
 #pragma unroll
-        for (int h = 0; h < HG; ++h) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) up[h][c] = __uint_as_float((uint32_t)(127 + k[h][c]) << 23);
-        }
+        for (int h = 0; h < HG; ++h) up[h] = make_float2(__uint_as_float((uint32_t)(127 + k[h][0]) << 23), __uint_as_float((uint32_t)(127 + k[h][1]) << 23));
         uint32_t hi[4][HG][2], lo[4][HG][2];
 #pragma unroll
         for (int n = 0; n < MINE; ++n) {
             const uint32_t pair = lds_u32(pairs + KEYS * 4 + n * (APART * 4));
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
-                float w[2];
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const float p = s[TWICE ? n : n >> 1][h][(TWICE ? 0 : 2 * (n & 1)) + c];
-                    offset[h][c] = __fmaf_rn(p, bf16hi(pair), offset[h][c]);
-                    w[c] = p * bf16lo(pair) * up[h][c];
-                }
-                two_parts(w[0], w[1], hi[TWICE ? n : n >> 1][h][TWICE ? 0 : n & 1], lo[TWICE ? n : n >> 1][h][TWICE ? 0 : n & 1]);
+                const float* const z = s[TWICE ? n : n >> 1][h] + (TWICE ? 0 : 2 * (n & 1));
+                const float2 p = make_float2(z[0], z[1]);
+                offset[h] = fma2(p, both(bf16hi(pair)), offset[h]);
+                const float2 w = mul2(mul2(p, both(bf16lo(pair))), up[h]);
+                two_parts(w.x, w.y, hi[TWICE ? n : n >> 1][h][TWICE ? 0 : n & 1], lo[TWICE ? n : n >> 1][h][TWICE ? 0 : n & 1]);
             }
         }
         if (TWICE) {            // heads in the lower columns' threads get the values, the others the rests
@@ -913,23 +943,24 @@ struct KvFour {
             float m_of[2], l_of[2];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
+                float &sum = c ? l[h].y : l[h].x, &add = c ? offset[h].y : offset[h].x;
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) {
-                    l[h][c] += __shfl_xor_sync(0xffffffffu, l[h][c], o);
-                    offset[h][c] += __shfl_xor_sync(0xffffffffu, offset[h][c], o);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    add += __shfl_xor_sync(0xffffffffu, add, o);
                 }
                 if (twice) {
-                    l[h][c] += __shfl_xor_sync(0xffffffffu, l[h][c], 2);
-                    offset[h][c] += __shfl_xor_sync(0xffffffffu, offset[h][c], 2);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                    add += __shfl_xor_sync(0xffffffffu, add, 2);
                 }
                 const float down = __uint_as_float((uint32_t)(127 + 100 - k[h][c]) << 23);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    acc[h][j][c] = __fmaf_rn(acc[h][j][c] * 8589934592.0f, down, offset[h][c]);            // 2^33
-                    acc[h][j][c + 2] = __fmaf_rn(acc[h][j][c + 2] * 536870912.0f, down, offset[h][c]);     // 2^29
+                    acc[h][j][c] = __fmaf_rn(acc[h][j][c] * 8589934592.0f, down, add);            // 2^33
+                    acc[h][j][c + 2] = __fmaf_rn(acc[h][j][c + 2] * 536870912.0f, down, add);     // 2^29
                 }
-                m_of[c] = __shfl_sync(0xffffffffu, m[h][c] * zs[h][c], from);
-                l_of[c] = __shfl_sync(0xffffffffu, l[h][c], from);
+                m_of[c] = __shfl_sync(0xffffffffu, m[h][c] * (c ? zs[h].y : zs[h].x), from);
+                l_of[c] = __shfl_sync(0xffffffffu, sum, from);
             }
             m_out[h] = g & 1 ? m_of[1] : m_of[0];
             l_out[h] = g & 1 ? l_of[1] : l_of[0];
@@ -1222,7 +1253,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     bool ok = true;
 #pragma unroll 1
     for (int k = 0;; ++k) {
-        const typename K::Segment seg = segs[k & 1];
+        typename K::Segment seg = segs[k & 1];
         if ((solo || mate == 0) && seg.end < c1) describe(seg.end, segs[(k + 1) & 1]);
         float z_scale[HG], acc[HG][8][4], m[HG], l[HG];
         KvFour<HG> four;
@@ -1253,11 +1284,12 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 
         int valid = sh.len[seg.b] - (f - seg.first) * KEYS;       // rows that the sequence has from the warp's chunk on
 #pragma unroll 1
-        for (; f < seg.end; f += by, valid -= by * KEYS) {
+        for (const int end = seg.end; f < end; f += by, valid -= by * KEYS) {
             const uint32_t st = smem_u32(smem) + (warp * STAGES + slot) * KV_STAGE_BYTES, scales = smem_u32(smem) + K::SCALES + (warp * STAGES + slot) * K::SCALE_BYTES;
             const bool append = a.kn && valid <= KEYS;
             uint4 fresh = make_uint4(0, 0, 0, 0);
             if (append) {
+                if (TYPE == KV_UINT4) seg = segs[k & 1];        // (not held over the loop: registers are what it is short of)
                 const int kvh = a.chunks_of_heads == 1 ? seg.item : seg.item / a.chunks_of_heads;
                 const uint16_t* src = (lane < 16 ? a.kn + seg.b * a.ldk : a.vn + seg.b * a.ldv) + kvh * KV_D + (lane & 15) * 8;
                 fresh = (a.flags & 4) ? load8<true>(src) : load8<false>(src);
@@ -1266,6 +1298,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             __syncwarp();
             if (append) {     // the sequence's last row is the new one: into the ring, and into the cache
                 const int r = valid - 1, part = lane & 15, row = ok ? sh.rows[warp][slot][r >> 4] : -1;
+                if (TYPE == KV_UINT4) seg = segs[k & 1];
                 const bool store = (a.chunks_of_heads == 1 || seg.item % a.chunks_of_heads == 0) && row >= 0;
                 const int64_t at = (int64_t)row + (r & 15);
                 const uint32_t dst = st + (lane < 16 ? 0 : 4096) + r * 128;
@@ -1452,6 +1485,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             if (++slot == STAGES) { slot = 0; parity ^= 1; }
         }
 
+        if (TYPE == KV_UINT4) seg = segs[k & 1];
         const int head0 = head_of(seg.item), heads = heads_of(seg.item);
         together();
         if (seg.end < c1) ask_queries(segs[(k + 1) & 1].b, segs[(k + 1) & 1].item);
