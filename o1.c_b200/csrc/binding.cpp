@@ -438,15 +438,19 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (!rows_of(*in[i], -1, ldx[i])) return nullptr;
         PyObject* const y = !given ? Py_None : pair ? PyTuple_GET_ITEM(a[5], i) : a[5];
         const int64_t heads = in[i]->size(1);
-        if (y == Py_None) {
-            out[i] = empty_on({rows, heads, dim}, type, device);
-            ldy[i] = heads * dim;
-        } else {
-            const at::Tensor* t = tensor(y, who);
-            if (!t || !rows_of(*t, heads, ldy[i])) return nullptr;
-            out[i] = *t;
-        }
+        ldy[i] = heads * dim;
+        if (y == Py_None) continue;
+        const at::Tensor* t = tensor(y, who);
+        if (!t || !rows_of(*t, heads, ldy[i])) return nullptr;
+        out[i] = *t;
     }
+    if (sides == 2 && !out[0].defined() && !out[1].defined()) {
+        const int64_t size = (int64_t)c10::elementSize(type);
+        Several some(Several::room(rows * ldy[0], size) + Several::room(rows * ldy[1], size), device);
+        for (int i = 0; i < 2; ++i) out[i] = some.next({rows, in[i]->size(1), dim}, type);
+    }
+    for (int i = 0; i < sides; ++i)
+        if (!out[i].defined()) out[i] = empty_on({rows, in[i]->size(1), dim}, type, device);
     if (!status(f_rotary(rope, positions->data_ptr(), wide, in[0]->data_ptr(), ldx[0], out[0].data_ptr(), ldy[0], (int)in[0]->size(1), sides == 2 ? in[1]->data_ptr() : nullptr, ldx[1],
                          sides == 2 ? out[1].data_ptr() : nullptr, ldy[1], sides == 2 ? (int)in[1]->size(1) : 0, (int)rows, type == at::kFloat ? O1_ROPE_FP32 : O1_ROPE_BF16, inverse),
                 "o1_rotary"))
