@@ -189,8 +189,8 @@ __device__ __forceinline__ void store8(uint16_t* p, const uint4& v) {
 // unit's place and scale, and the maxima are found for all units at once: with four exchanges for each and divisions in every lane the write's instructions
 // (135 a unit, now 100) took longer than its bytes, 22.8 us.  Written and read, us: 16640 rows of 8 heads of int8 18.9 + 18.7 (5.5 TB/s), 100000 rows of one head
 // 15.2 + 15.1; a row to a warp 23.5 + 19.5 and 43 + 39, a head to a half warp 34 + 35 for the former.  Few rows have more warps with two units: 1800 rows of
-// 8 heads 3.5 + 3.7, with eight 5.3 + 4.0; 2600 rows 4.5 + 4.7 and 4.3 + 4.3; 4111 rows 6.9 + 7.5 and 5.8 + 6.2.  Of four bits, 16640 rows of 8 heads: 19 + 16, the write bound by its
-// instructions (110 a unit, 2.9 a clock and SM; the sums of two extremes in place of one), the read by HBM.
+// 8 heads 3.5 + 3.7, with eight 5.3 + 4.0; 2600 rows 4.5 + 4.7 and 4.3 + 4.3; 4111 rows 6.9 + 7.5 and 5.8 + 6.2.  Of four bits (kv_write4_kernel), 16640 rows
+// of 8 heads: 18 + 16.
 // Launches overlap at any size (the next one is let in once the rows have been asked for: its blocks, placed earlier, leave these unevenly spread, 1000 rows 5.1 us, so
 // 4.1): written and read through a stream, 4111 rows 14.4 us without, 12.4 with; 16640 42.7 and 38.
 static constexpr int KV_EACH = 8, KV_EACH_OF_FEW = 2, KV_FEW_UNITS = 19200;
@@ -201,7 +201,7 @@ __device__ __forceinline__ int64_t place(int64_t slot, int head, const KvView& c
     const int64_t page = c.page_shift >= 0 ? slot >> c.page_shift : slot / c.page_size;
     return (page * c.heads + head) * c.page_size + slot - page * c.page_size;
 }
-template <bool VEC, int EACH, bool FOUR>
+template <bool VEC, int EACH>
 __global__ void __launch_bounds__(128, EACH == 8 ? 9 : 12)
 kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk, const uint16_t* __restrict__ v, int64_t ldv,
                 const int64_t* __restrict__ slots, unsigned units, const int* err, int* bad) {
@@ -227,23 +227,8 @@ kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk,
     }
     const int64_t places = place(failed ? -1 : slot, from + mine - my_row * c.heads, c, bad);
     grid_dep_launch();
-    float inv = 0.f, least = 0.f;
-    if (FOUR) {          // as below, the largest and the least value together
-        uint32_t top[EACH];
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) top[i] = extremes(x[i]);
-#pragma unroll
-        for (int o = 8, n = EACH / 2; o > 0; o >>= 1, n >>= 1) {
-            if (n == 0) top[0] = max_nan_bf16x2(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
-#pragma unroll
-            for (int i = 0; i < n; ++i) {
-                const uint32_t keep = lane & o ? top[n + i] : top[i], give = lane & o ? top[i] : top[n + i];
-                top[i] = max_nan_bf16x2(keep, __shfl_xor_sync(0xffffffffu, give, o));
-            }
-        }
-        const uint32_t pair = scale4_of(top[0], inv, least);
-        if (places >= 0 && lane % (16 / EACH) == 0) reinterpret_cast<uint32_t*>(scales)[places] = pair;
-    } else if (type != KV_BF16) {
+    float inv = 0.f;
+    if (type != KV_BF16) {
         // maxima: a step halves the lanes that a unit is spread over, and, until a lane has one, its units
         uint32_t top[EACH];
 #pragma unroll
@@ -263,11 +248,67 @@ kv_write_kernel(KvView c, int type, const uint16_t* __restrict__ k, int64_t ldk,
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
         const int64_t at = __shfl_sync(0xffffffffu, places, i * (16 / EACH), 16);
-        const float f = __shfl_sync(0xffffffffu, inv, i * (16 / EACH), 16), from_least = FOUR ? __shfl_sync(0xffffffffu, least, i * (16 / EACH), 16) : 0.f;
+        const float f = __shfl_sync(0xffffffffu, inv, i * (16 / EACH), 16);
         if (at < 0) continue;
-        if (FOUR) reinterpret_cast<uint32_t*>(base)[at * 16 + lane] = codes4_of(x[i], f, from_least);
-        else if (type == KV_BF16) reinterpret_cast<uint4*>(base)[at * 16 + lane] = x[i];
+        if (type == KV_BF16) reinterpret_cast<uint4*>(base)[at * 16 + lane] = x[i];
         else reinterpret_cast<uint2*>(base)[at * 16 + lane] = codes_of(x[i], type, f);
+    }
+}
+
+// Codes of four bits: the same with a unit to eight lanes, two pieces of eight columns to each, since the instructions of a unit (its place, scale and least value from the lane that has
+// them, its addresses) come once for sixteen values: written and read, 8000 rows of 8
+// heads 17.1 us, with sixteen lanes to a unit 18.1, 16640 rows 34.1 and 34.8.
+template <bool VEC, int EACH>
+__global__ void __launch_bounds__(128, EACH == 8 ? 9 : 12)
+kv_write4_kernel(KvView c, const uint16_t* __restrict__ k, int64_t ldk, const uint16_t* __restrict__ v, int64_t ldv, const int64_t* __restrict__ slots, unsigned units, const int* err,
+                 int* bad) {
+    constexpr int MINE = EACH / 2;             // of a group of eight lanes, every other one of the warp's
+    grid_dep_wait();
+    const unsigned from = (blockIdx.x * 4 + (threadIdx.x >> 5)) * EACH;
+    if (from >= units) return;
+    const int lane = threadIdx.x & 7, group = (threadIdx.x >> 3) & 1, count = min((unsigned)EACH, units - from);
+    const bool is_v = threadIdx.x & 16;
+    const int mine = 2 * (lane / (8 / MINE)) + group;       // the unit whose place and scale are this lane's
+    const unsigned row = (from + group) / (unsigned)c.heads, my_row = (from + mine) / (unsigned)c.heads;
+    const int64_t slot = mine < count ? slots[my_row] : -1, ld = is_v ? ldv : ldk;
+    const int failed = error_word(err);        // rows that a failed kernel should have made stay out of the cache
+    int head = from + group - row * c.heads;
+    const uint16_t* src = (is_v ? v : k) + row * ld + lane * 8;
+    uint32_t* const base = reinterpret_cast<uint32_t*>(is_v ? c.v : c.k);
+    uint32_t* const scales = reinterpret_cast<uint32_t*>(is_v ? c.vs : c.ks);
+    uint4 x[MINE][2];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+        x[i][0] = x[i][1] = make_uint4(0, 0, 0, 0);
+        if (2 * i + group < count) { x[i][0] = load8<VEC>(src + head * KV_D); x[i][1] = load8<VEC>(src + head * KV_D + 64); }
+        head += 2;
+        while (head >= c.heads) { head -= c.heads; src += ld; }
+    }
+    const int64_t places = place(failed ? -1 : slot, from + mine - my_row * c.heads, c, bad);
+    grid_dep_launch();
+    // the largest and the least value together: a step halves the lanes that a unit is spread over, and, until a lane has one, its units
+    uint32_t top[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) top[i] = max_nan_bf16x2(extremes(x[i][0]), extremes(x[i][1]));
+#pragma unroll
+    for (int o = 4, n = MINE / 2; o > 0; o >>= 1, n >>= 1) {
+        if (n == 0) top[0] = max_nan_bf16x2(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const uint32_t keep = lane & o ? top[n + i] : top[i], give = lane & o ? top[i] : top[n + i];
+            top[i] = max_nan_bf16x2(keep, __shfl_xor_sync(0xffffffffu, give, o));
+        }
+    }
+    float inv, least;
+    const uint32_t pair = scale4_of(top[0], inv, least);
+    if (places >= 0 && lane % (8 / MINE) == 0) scales[places] = pair;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+        const int64_t at = __shfl_sync(0xffffffffu, places, i * (8 / MINE), 8);
+        const float f = __shfl_sync(0xffffffffu, inv, i * (8 / MINE), 8), b = __shfl_sync(0xffffffffu, least, i * (8 / MINE), 8);
+        if (at < 0) continue;
+        base[at * 16 + lane] = codes4_of(x[i][0], f, b);
+        base[at * 16 + 8 + lane] = codes4_of(x[i][1], f, b);
     }
 }
 
@@ -340,7 +381,7 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
 //    of a byte are exact in f16 and bf16.  Keys' codes go through f16, which takes fewer instructions, with queries scaled to f16's top by a power of two for each head (those
 //    below 2^-29 of its largest lose bits); values' codes through bf16, whose range a probability needs.  The result is rounded once.
 //  * Rows of four bits (KvFour) are 64 to a chunk and the chunks, for the same bytes, twice the arithmetic: instructions bound them, not memory.  302 MB (96 sequences of 300 to 5400
-//    rows, 8 kv heads, 32 heads) in 63 us, 4.8 TB/s, 73 % of a copy's rate; 109 MB (one of 100003) in 31.5; 39.7 MB (37 of 0 to 1999, 16 heads) in 19.6.  A chunk is 990
+//    rows, 8 kv heads, 32 heads) in 62.5 us, 4.8 TB/s, 74 % of a copy's rate; 109 MB (one of 100003) in 31.1; 39.7 MB (37 of 0 to 1999, 16 heads) in 19.5.  A chunk is some 960
 //    instructions (all of a launch's counted), of which an SM issues 2.2 a clock; half of the ALU pipe's time is the codes' masks and shifts.  As the other kinds have it (queries
 //    as rows, codes to pairs of keys by byte permutes) it was 1420 and 99 us.
 // Times below: "batch" 24 sequences of 1 to 2100 rows of bf16, "shared" 32 sequences of 1000 to 3000, 16 query heads on one kv head; us.
@@ -1708,12 +1749,14 @@ hd_status o1_kv_write(const o1_kv_cache* cache, const void* k, int64_t ldk, cons
         const unsigned units = (unsigned)min(most, rows - first) * c.heads;
         const bool few = units < KV_FEW_UNITS;
         const unsigned block = 4 * (few ? KV_EACH_OF_FEW : KV_EACH);
-        auto kern = cache->type == O1_KV_UINT4 ? (few ? (vec ? kv_write_kernel<true, KV_EACH_OF_FEW, true> : kv_write_kernel<false, KV_EACH_OF_FEW, true>)
-                                                        : (vec ? kv_write_kernel<true, KV_EACH, true> : kv_write_kernel<false, KV_EACH, true>))
-                    : few ? (vec ? kv_write_kernel<true, KV_EACH_OF_FEW, false> : kv_write_kernel<false, KV_EACH_OF_FEW, false>)
-                          : (vec ? kv_write_kernel<true, KV_EACH, false> : kv_write_kernel<false, KV_EACH, false>);
-        if (!launch_ok(launch_chained(kern, dim3((units + block - 1) / block), dim3(128), 0, current_stream(), 1, 1, c, cache->type, (const uint16_t*)k + first * ldk, ldk,
-                                      (const uint16_t*)v + first * ldv, ldv, slots + first, units, (const int*)device_error_word(), device_table_word()), "kv_write"))
+        auto kern = few ? (vec ? kv_write_kernel<true, KV_EACH_OF_FEW> : kv_write_kernel<false, KV_EACH_OF_FEW>) : vec ? kv_write_kernel<true, KV_EACH> : kv_write_kernel<false, KV_EACH>;
+        auto kern4 = few ? (vec ? kv_write4_kernel<true, KV_EACH_OF_FEW> : kv_write4_kernel<false, KV_EACH_OF_FEW>) : vec ? kv_write4_kernel<true, KV_EACH> : kv_write4_kernel<false, KV_EACH>;
+        const uint16_t *const k_at = (const uint16_t*)k + first * ldk, *const v_at = (const uint16_t*)v + first * ldv;
+        const dim3 grid((units + block - 1) / block);
+        const int* const err = device_error_word();
+        if (!launch_ok(cache->type == O1_KV_UINT4 ? launch_chained(kern4, grid, dim3(128), 0, current_stream(), 1, 1, c, k_at, ldk, v_at, ldv, slots + first, units, err, device_table_word())
+                                                  : launch_chained(kern, grid, dim3(128), 0, current_stream(), 1, 1, c, cache->type, k_at, ldk, v_at, ldv, slots + first, units, err, device_table_word()),
+                       "kv_write"))
             return HD_ERR_RUNTIME;
         o1_launch_count_add(1);
         if (rows - first <= most) break;
