@@ -381,7 +381,7 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
 //    of a byte are exact in f16 and bf16.  Keys' codes go through f16, which takes fewer instructions, with queries scaled to f16's top by a power of two for each head (those
 //    below 2^-29 of its largest lose bits); values' codes through bf16, whose range a probability needs.  The result is rounded once.
 //  * Rows of four bits (KvFour) are 64 to a chunk and the chunks, for the same bytes, twice the arithmetic: instructions bound them, not memory.  302 MB (96 sequences of 300 to 5400
-//    rows, 8 kv heads, 32 heads) in 62.5 us, 4.8 TB/s, 74 % of a copy's rate; 109 MB (one of 100003) in 31.1; 39.7 MB (37 of 0 to 1999, 16 heads) in 19.5.  A chunk is some 960
+//    rows, 8 kv heads, 32 heads) in 62.5 us, 4.8 TB/s, 74 % of a copy's rate; 109 MB (one of 100003) in 30.4; 39.7 MB (37 of 0 to 1999, 16 heads) in 19.5.  A chunk is some 960
 //    instructions (all of a launch's counted), of which an SM issues 2.2 a clock; half of the ALU pipe's time is the codes' masks and shifts.  As the other kinds have it (queries
 //    as rows, codes to pairs of keys by byte permutes) it was 1420 and 99 us.
 // Times below: "batch" 24 sequences of 1 to 2100 rows of bf16, "shared" 32 sequences of 1000 to 3000, 16 query heads on one kv head; us.
@@ -417,6 +417,7 @@ static constexpr int KV_JOIN_STEP = 4;                 // parts that a join has 
 static constexpr int ERR_KV_WAIT = 72;                 // a wait of the attention kernel ran out
 static constexpr float KV_LIFT = 20.0f;                // probabilities are relative to 2^-20 of the largest: those that fp32 has no value for are 2^-146 and less of it
 
+static constexpr int KV4_JOIN_STEP = 8;                // of four bits and up to four heads: one head to a warp (one of 100003 rows 31.1 us, with a step of 4 30.45, 8 30.4, 16 31)
 struct KvAttn {
     KvView c;
     const uint16_t *q, *kn, *vn;
@@ -647,7 +648,7 @@ __device__ __forceinline__ bool all_came(unsigned* counter, int wanted) {
 // The sums of `count` parts of HEADS heads (head, head + APART, ... below `heads`), by a warp: the first part is `first`, the others in slot 0 of every `stride`-th
 // team behind it.  Into the result, or (to_out false) into the first one's place.  A lane has a part's weights; the first parts' rows are under way while the
 // weights are, and all heads' at once.
-template <int HEADS, int APART>
+template <int HEADS, int APART, int STEP = KV_JOIN_STEP>
 __device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, int count, int b, int head, int heads, int head0, bool to_out) {
     static_assert(KV_FLAT <= 32 && KV_FAN <= 32 && (KV_TEAMS_MAX + KV_FAN - 1) / KV_FAN <= 32 && KV_UNITS_MAX <= 32 * 64, "a part to a lane");
     const int lane = threadIdx.x & 31;
@@ -664,10 +665,10 @@ __device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, 
     float top[HEADS], sum[HEADS], w[HEADS];
     float4 r[HEADS];
 #pragma unroll 1
-    for (int i0 = 0; i0 < count; i0 += KV_JOIN_STEP, src += KV_JOIN_STEP * step * (KV_D / 4)) {
-        float4 x[KV_JOIN_STEP][HEADS];
+    for (int i0 = 0; i0 < count; i0 += STEP, src += STEP * step * (KV_D / 4)) {
+        float4 x[STEP][HEADS];
 #pragma unroll
-        for (int i = 0; i < KV_JOIN_STEP; ++i) {
+        for (int i = 0; i < STEP; ++i) {
             const float4* const from = i0 + i == 0 ? mine : src + i * step * (KV_D / 4);
 #pragma unroll
             for (int h = 0; h < HEADS; ++h) {
@@ -689,7 +690,7 @@ __device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, 
             }
         }
 #pragma unroll
-        for (int i = 0; i < KV_JOIN_STEP; ++i) {
+        for (int i = 0; i < STEP; ++i) {
 #pragma unroll
             for (int h = 0; h < HEADS; ++h) {
                 const float f = __shfl_sync(0xffffffffu, w[h], i0 + i);
@@ -1665,8 +1666,13 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             if (!sh.last[team][i]) continue;
             const typename K::Share s = shares[i];
             again |= level == 0 && s.groups > 1;
-            for (int head = (mate - done) & (KV_TEAM - 1); head < s.heads; head += 2 * HG * KV_TEAM)
-                kv_join<2 * HG, KV_TEAM>(a, level ? s.item : s.first, level ? s.fan : 1, level ? s.groups : s.here, s.b, head, s.heads, s.head0, level || s.groups == 1);
+            if (TYPE == KV_UINT4 && s.heads <= KV_TEAM) {
+                const int head = (mate - done) & (KV_TEAM - 1);
+                if (head < s.heads) kv_join<1, KV_TEAM, KV4_JOIN_STEP>(a, level ? s.item : s.first, level ? s.fan : 1, level ? s.groups : s.here, s.b, head, s.heads, s.head0, level || s.groups == 1);
+            } else {
+                for (int head = (mate - done) & (KV_TEAM - 1); head < s.heads; head += 2 * HG * KV_TEAM)
+                    kv_join<2 * HG, KV_TEAM>(a, level ? s.item : s.first, level ? s.fan : 1, level ? s.groups : s.here, s.b, head, s.heads, s.head0, level || s.groups == 1);
+            }
             done += s.heads;
         }
         if (!again) break;
