@@ -561,8 +561,8 @@ struct KvKernel {
     // (HG == 1: 128 registers and 24 slots of 8 KB; HG == 2 holds twice the queries and sums: 168 registers, two teams, again 24 slots)
     // shared memory: the rings, their scales, the teams' join buffers, then Shared
     static constexpr int SCALE_BYTES = TYPE == KV_BF16 ? 0 : 2 * KEYS * 4, PLACES = KEYS < 32 ? 2 : KEYS / 16;      // of a slot; 16 rows to a place
-    // (four bits have twice the scales, and where there are three teams half the room to join in)
-    static constexpr int JOIN_BYTES = TYPE == KV_UINT4 && HG == 1 ? KV_JOIN_BYTES / 2 : KV_JOIN_BYTES;
+    // (four bits have twice the scales, and half the room to join in)
+    static constexpr int JOIN_BYTES = TYPE == KV_UINT4 ? KV_JOIN_BYTES / 2 : KV_JOIN_BYTES;
     static constexpr int SCALES = WARPS * STAGES * KV_STAGE_BYTES, JOIN = SCALES + WARPS * STAGES * SCALE_BYTES, SHARED = JOIN + TEAMS * JOIN_BYTES;
     struct Share { int first, here, fan, item, groups, b, head0, heads; };        // a part's group begins at part `first` and has `here` (0: no part), its item at part `item`
     struct Segment { int b, item, first, begin, end, n; };        // first: the item's first chunk; begin ... end - 1: the team's
@@ -722,60 +722,58 @@ __device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, 
 //    keys and gives the other its results, one the values and one the rests.
 //  * Weights p_t s_t are held times 2^k: the sums, of codes 2^-133 of themselves, are of normal size where the largest weight so far (a chunk's largest probability times its largest
 //    scale bounds it) is between 2^90 and 2^112, and weights of 2^-80 of that one are still there.  Largest weight and k follow the running maximum, and k moves seldom.
-template <int HG>
+//  * At most eight heads: more on a kv head are items of their own, which read its rows again (from L2 as a rule).  With sixteen to an item, as the other kinds have it, registers
+//    spill and two teams are left: 128 sequences of up to 4000 rows, 2 kv heads of 16: 56.6 us, now 44.5; 50000 rows of one 22.2, now 18.4.
 struct KvFour {
-    float2 zs[HG], q_sum[HG], l[HG], offset[HG];       // of heads 8 h + 2 t, 2 t + 1
-    float m[HG][2], most[HG][2];       // m in the scores' units, zs of them are one in base 2
-    int k[HG][2];
+    float2 zs, q_sum, l, offset;       // of heads 2 t, 2 t + 1
+    float m[2], most[2];       // m in the scores' units, zs of them are one in base 2
+    int k[2];
 
-    __device__ __forceinline__ void begin(uint32_t (&q)[HG][16], float scale, float (&acc)[HG][8][4]) {
+    __device__ __forceinline__ void begin(uint32_t (&q)[16], float scale, float (&acc)[8][4]) {
         const int t = threadIdx.x & 3;
+        // (sums: a product with ones, which gives them where this thread wants them)
+        uint32_t top = 0;
+        float sum[4];
+        mma_bf16_new(sum, 0x3F803F80u, 0, 0x3F803F80u, 0, q[0], q[1]);
 #pragma unroll
-        for (int h = 0; h < HG; ++h) {
-            // (sums: a product with ones, which gives them where this thread wants them)
-            uint32_t top = 0;
-            float sum[4];
-            mma_bf16_new(sum, 0x3F803F80u, 0, 0x3F803F80u, 0, q[h][0], q[h][1]);
+        for (int i = 2; i < 16; i += 2) mma_bf16(sum, 0x3F803F80u, 0, 0x3F803F80u, 0, q[i], q[i + 1]);
 #pragma unroll
-            for (int i = 2; i < 16; i += 2) mma_bf16(sum, 0x3F803F80u, 0, 0x3F803F80u, 0, q[h][i], q[h][i + 1]);
+        for (int i = 0; i < 16; ++i) top = max_u16x2(top, q[i] & 0x7FFF7FFFu);
+        top = max(top & 0xFFFFu, top >> 16);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // queries times 2^x, the largest one below 2^127
+        const int x = min(120, 253 - (int)max(top >> 7, 1u));
+        const float z = scale * __uint_as_float((uint32_t)(127 + 70) << 23) * __uint_as_float((uint32_t)(127 + 63 - x) << 23);
+        const uint32_t up = (uint32_t)(127 + x) * 0x00800080u, up16 = up - 0x02000200u;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top = max_u16x2(top, q[h][i] & 0x7FFF7FFFu);
-            top = max(top & 0xFFFFu, top >> 16);
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // queries times 2^x, the largest one below 2^127
-            const int x = min(120, 253 - (int)max(top >> 7, 1u));
-            const float z = scale * __uint_as_float((uint32_t)(127 + 70) << 23) * __uint_as_float((uint32_t)(127 + 63 - x) << 23);
-            const uint32_t up = (uint32_t)(127 + x) * 0x00800080u, up16 = up - 0x02000200u;
+        for (int i = 0; i < 16; ++i) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(q[i]) : "r"(i & 1 ? up16 : up));
 #pragma unroll
-            for (int i = 0; i < 16; ++i) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(q[h][i]) : "r"(i & 1 ? up16 : up));
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                (c ? zs[h].y : zs[h].x) = __shfl_sync(0xffffffffu, z, 8 * t + 4 * c);
-                // (the shuffled exponent: x of that head)
-                const int x_of = __shfl_sync(0xffffffffu, x, 8 * t + 4 * c);
-                (c ? q_sum[h].y : q_sum[h].x) = sum[c] * __uint_as_float((uint32_t)(127 + x_of - 70) << 23) * __uint_as_float((uint32_t)(127 - 63) << 23);
-                m[h][c] = -INFINITY;
-                l[h] = offset[h] = both(0.f);
-                most[h][c] = 0.f;
-                k[h][c] = 101;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) acc[h][j][0] = acc[h][j][1] = acc[h][j][2] = acc[h][j][3] = 0.f;
+        for (int c = 0; c < 2; ++c) {
+            (c ? zs.y : zs.x) = __shfl_sync(0xffffffffu, z, 8 * t + 4 * c);
+            // (the shuffled exponent: x of that head)
+            const int x_of = __shfl_sync(0xffffffffu, x, 8 * t + 4 * c);
+            (c ? q_sum.y : q_sum.x) = sum[c] * __uint_as_float((uint32_t)(127 + x_of - 70) << 23) * __uint_as_float((uint32_t)(127 - 63) << 23);
+            m[c] = -INFINITY;
+            l = offset = both(0.f);
+            most[c] = 0.f;
+            k[c] = 101;
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
     }
 
     // 64 rows in shared memory at st (keys, then values), of which `valid` are there.  In tiles of 8, row n is the tile's key kv4_key(n).
-    __device__ __forceinline__ void chunk(uint32_t st, uint32_t scales, int valid, bool twice, const uint32_t (&q)[HG][16], float (&acc)[HG][8][4]) {
-        if (HG == 1 && twice) part<true>(st, scales, valid, q, acc);
+    __device__ __forceinline__ void chunk(uint32_t st, uint32_t scales, int valid, bool twice, const uint32_t (&q)[16], float (&acc)[8][4]) {
+        if (twice) part<true>(st, scales, valid, q, acc);
         else part<false>(st, scales, valid, q, acc);
     }
     template <bool TWICE>
-    __device__ __forceinline__ void part(uint32_t st, uint32_t scales, int valid, const uint32_t (&q)[HG][16], float (&acc)[HG][8][4]) {
+    __device__ __forceinline__ void part(uint32_t st, uint32_t scales, int valid, const uint32_t (&q)[16], float (&acc)[8][4]) {
         constexpr int KEYS = 64, MINE = TWICE ? 4 : 8, APART = TWICE ? 16 : 8;       // this thread's keys, and how far apart they are
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, mine = kv4_key(g);
         const bool upper = t & 2;
-        float s[4][HG][4];
+        float s[4][4];
         const int first = mine + (TWICE && upper ? 8 : 0);        // this thread's keys: first + APART n
         const uint32_t pairs = scales + first * 4;
         uint32_t kpair[MINE];
@@ -802,11 +800,8 @@ struct KvFour {
                         const uint4 &a4 = x[i][0], &b4 = x[i][1];
                         uint32_t a = j == 0 ? a4.x : j == 1 ? a4.y : j == 2 ? a4.z : a4.w, b = j == 0 ? b4.x : j == 1 ? b4.y : j == 2 ? b4.z : b4.w;
                         if (half) { a >>= 8; b >>= 8; }
-#pragma unroll
-                        for (int h = 0; h < HG; ++h) {
-                            if (j == 0 && half == 0) mma_bf16_new(s[i0 + i][h], a & A, b & A, a & B, b & B, q[h][0], q[h][1]);
-                            else mma_bf16(s[i0 + i][h], a & A, b & A, a & B, b & B, q[h][4 * j + 2 * half], q[h][4 * j + 2 * half + 1]);
-                        }
+                        if (j == 0 && half == 0) mma_bf16_new(s[i0 + i], a & A, b & A, a & B, b & B, q[0], q[1]);
+                        else mma_bf16(s[i0 + i], a & A, b & A, a & B, b & B, q[4 * j + 2 * half], q[4 * j + 2 * half + 1]);
                     }
                 }
             }
@@ -815,7 +810,7 @@ struct KvFour {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) s[i][0][c] = upper ? s[i][0][2 + c] : s[i][0][c];
+                for (int c = 0; c < 2; ++c) s[i][c] = upper ? s[i][2 + c] : s[i][c];
             }
         }
         if (valid < KEYS) {             // what is behind a sequence may be NaN; of its values' scales nothing is left
@@ -826,117 +821,97 @@ struct KvFour {
 #pragma unroll
         for (int n = 0; n < MINE; ++n) {
             const uint32_t pair = kpair[n];
-#pragma unroll
-            for (int h = 0; h < HG; ++h) {
-                float* const z = s[TWICE ? n : n >> 1][h] + (TWICE ? 0 : 2 * (n & 1));
-                const float2 r = fma2(make_float2(z[0], z[1]), both(bf16lo(pair)), mul2(both(bf16hi(pair)), q_sum[h]));
-                z[0] = r.x;
-                z[1] = r.y;
-            }
+            float* const z = s[TWICE ? n : n >> 1] + (TWICE ? 0 : 2 * (n & 1));
+            const float2 r = fma2(make_float2(z[0], z[1]), both(bf16lo(pair)), mul2(both(bf16hi(pair)), q_sum));
+            z[0] = r.x;
+            z[1] = r.y;
         }
         uint32_t s_top = 0;           // the largest of the values' scales, as bits
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            s_top = max(s_top, lds_u32(scales + KEYS * 4 + (i * 32 + lane) * 4) & 0xFFFFu);
-        }
+        for (int i = 0; i < 2; ++i) s_top = max(s_top, lds_u32(scales + KEYS * 4 + (i * 32 + lane) * 4) & 0xFFFFu);
         s_top = __reduce_max_sync(0xffffffffu, s_top) << 16;
         if (valid < KEYS) {
 #pragma unroll
             for (int n = 0; n < MINE; ++n) {
                 if (first + APART * n < valid) continue;
 #pragma unroll
-                for (int h = 0; h < HG; ++h) {
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) s[TWICE ? n : n >> 1][h][(TWICE ? 0 : 2 * (n & 1)) + c] = -INFINITY;
-                }
+                for (int c = 0; c < 2; ++c) s[TWICE ? n : n >> 1][(TWICE ? 0 : 2 * (n & 1)) + c] = -INFINITY;
             }
         }
         bool moved = false;
-        float2 alpha[HG];
+        float top[2], ref[2], a[2];
 #pragma unroll
-        for (int h = 0; h < HG; ++h) {
-            float top[2], ref[2], a[2];
+        for (int c = 0; c < 2; ++c) {
+            top[c] = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                top[c] = -INFINITY;
+            for (int n = 0; n < MINE; ++n) top[c] = fmaxf(top[c], s[TWICE ? n : n >> 1][(TWICE ? 0 : 2 * (n & 1)) + c]);
 #pragma unroll
-                for (int n = 0; n < MINE; ++n) top[c] = fmaxf(top[c], s[TWICE ? n : n >> 1][h][(TWICE ? 0 : 2 * (n & 1)) + c]);
+            for (int o = TWICE ? 2 : 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
+            // (differences before the factor: of scores of any size, the largest one's exponent is exactly the lift)
+            const float m_new = fmaxf(m[c], top[c]);
+            ref[c] = m_new == -INFINITY ? 0.f : m_new;
+            a[c] = exp2_fast((m[c] - ref[c]) * (c ? zs.y : zs.x));
+            m[c] = m_new;
+        }
+        const float2 less = make_float2(-ref[0], -ref[1]);
+        float2 sum = both(0.f);
 #pragma unroll
-                for (int o = TWICE ? 2 : 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
-                // (differences before the factor: of scores of any size, the largest one's exponent is exactly the lift)
-                const float m_new = fmaxf(m[h][c], top[c]);
-                ref[c] = m_new == -INFINITY ? 0.f : m_new;
-                a[c] = exp2_fast((m[h][c] - ref[c]) * (c ? zs[h].y : zs[h].x));
-                m[h][c] = m_new;
+        for (int n = 0; n < MINE; ++n) {
+            float* const z = s[TWICE ? n : n >> 1] + (TWICE ? 0 : 2 * (n & 1));
+            const float2 r = fma2(add2(make_float2(z[0], z[1]), less), zs, both(KV_LIFT));
+            z[0] = exp2_fast(r.x);
+            z[1] = exp2_fast(r.y);
+            sum = add2(sum, make_float2(z[0], z[1]));
+        }
+        l = fma2(l, make_float2(a[0], a[1]), sum);
+        offset = mul2(offset, make_float2(a[0], a[1]));
+        const float2 r = fma2(add2(make_float2(top[0], top[1]), less), zs, both(KV_LIFT));
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            most[c] = fmaxf(most[c] * a[c], exp2_fast(c ? r.y : r.x) * __uint_as_float(s_top));
+            const int e = (int)(__float_as_uint(most[c]) >> 23) - 127;
+            if ((unsigned)(e + k[c] - 90) > 21u) {
+                const int k_new = min(min(max(101 - e, -27), 127), k[c] + 100);
+                a[c] *= exp2_fast((float)(k_new - k[c]));
+                k[c] = k_new;
             }
-            const float2 less = make_float2(-ref[0], -ref[1]);
-            float2 sum = both(0.f);
-#pragma unroll
-            for (int n = 0; n < MINE; ++n) {
-                float* const z = s[TWICE ? n : n >> 1][h] + (TWICE ? 0 : 2 * (n & 1));
-                const float2 r = fma2(add2(make_float2(z[0], z[1]), less), zs[h], both(KV_LIFT));
-                z[0] = exp2_fast(r.x);
-                z[1] = exp2_fast(r.y);
-                sum = add2(sum, make_float2(z[0], z[1]));
-            }
-            alpha[h] = make_float2(a[0], a[1]);
-            l[h] = fma2(l[h], alpha[h], sum);
-            offset[h] = mul2(offset[h], alpha[h]);
-            const float2 r = fma2(add2(make_float2(top[0], top[1]), less), zs[h], both(KV_LIFT));
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                most[h][c] = fmaxf(most[h][c] * a[c], exp2_fast(c ? r.y : r.x) * __uint_as_float(s_top));
-                const int e = (int)(__float_as_uint(most[h][c]) >> 23) - 127;
-                if ((unsigned)(e + k[h][c] - 90) > 21u) {
-                    const int k_new = min(min(max(101 - e, -27), 127), k[h][c] + 100);
-                    a[c] *= exp2_fast((float)(k_new - k[h][c]));
-                    k[h][c] = k_new;
-                }
-                moved = moved || a[c] != 1.f;
-            }
-            alpha[h] = make_float2(a[0], a[1]);
+            moved = moved || a[c] != 1.f;
         }
         if (__any_sync(0xffffffffu, moved)) {
+            const float2 alpha = make_float2(a[0], a[1]);
 #pragma unroll
-            for (int h = 0; h < HG; ++h) {
+            for (int j = 0; j < 8; ++j) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-#pragma unroll
-                    for (int c = 0; c < 4; c += 2) {
-                        const float2 r = mul2(make_float2(acc[h][j][c], acc[h][j][c + 1]), alpha[h]);
-                        acc[h][j][c] = r.x;
-                        acc[h][j][c + 1] = r.y;
-                    }
+                for (int c = 0; c < 4; c += 2) {
+                    const float2 r = mul2(make_float2(acc[j][c], acc[j][c + 1]), alpha);
+                    acc[j][c] = r.x;
+                    acc[j][c + 1] = r.y;
                 }
             }
         }
         // weights, in two parts of bf16; [tile of 16 keys][its upper 8 keys]
-        float2 up[HG];
-#pragma unroll
-        for (int h = 0; h < HG; ++h) up[h] = make_float2(__uint_as_float((uint32_t)(127 + k[h][0]) << 23), __uint_as_float((uint32_t)(127 + k[h][1]) << 23));
-        uint32_t hi[4][HG][2], lo[4][HG][2];
+        const float2 up = make_float2(__uint_as_float((uint32_t)(127 + k[0]) << 23), __uint_as_float((uint32_t)(127 + k[1]) << 23));
+        uint32_t hi[4][2], lo[4][2];
 #pragma unroll
         for (int n = 0; n < MINE; ++n) {
             const uint32_t pair = lds_u32(pairs + KEYS * 4 + n * (APART * 4));
-#pragma unroll
-            for (int h = 0; h < HG; ++h) {
-                const float* const z = s[TWICE ? n : n >> 1][h] + (TWICE ? 0 : 2 * (n & 1));
-                const float2 p = make_float2(z[0], z[1]);
-                offset[h] = fma2(p, both(bf16hi(pair)), offset[h]);
-                const float2 w = mul2(mul2(p, both(bf16lo(pair))), up[h]);
-                two_parts(w.x, w.y, hi[TWICE ? n : n >> 1][h][TWICE ? 0 : n & 1], lo[TWICE ? n : n >> 1][h][TWICE ? 0 : n & 1]);
-            }
+            const float* const z = s[TWICE ? n : n >> 1] + (TWICE ? 0 : 2 * (n & 1));
+            const float2 p = make_float2(z[0], z[1]);
+            offset = fma2(p, both(bf16hi(pair)), offset);
+            const float2 w = mul2(mul2(p, both(bf16lo(pair))), up);
+            two_parts(w.x, w.y, hi[TWICE ? n : n >> 1][TWICE ? 0 : n & 1], lo[TWICE ? n : n >> 1][TWICE ? 0 : n & 1]);
         }
         if (TWICE) {            // heads in the lower columns' threads get the values, the others the rests
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t other = __shfl_xor_sync(0xffffffffu, upper ? hi[i][0][0] : lo[i][0][0], 2);
-                hi[i][0][1] = upper ? lo[i][0][0] : other;
-                hi[i][0][0] = upper ? other : hi[i][0][0];
+                const uint32_t other = __shfl_xor_sync(0xffffffffu, upper ? hi[i][0] : lo[i][0], 2);
+                hi[i][1] = upper ? lo[i][0] : other;
+                hi[i][0] = upper ? other : hi[i][0];
             }
         }
         // out^T += V^T P^T, 16 keys a step.  A matrix of eight rows and 32 columns, in two-byte pieces of four columns, is loaded transposed: this thread gets columns 4 g ... + 3 of two rows
-        // beside each other, as the product wants them.  Two steps to a turn of the loop: with all four its instructions outgrow the nearest cache (96 sequences 81 us, then 73).  A tile's rows g are even columns, g + 8 odd ones, which are 16 times as large.
+        // beside each other, as the product wants them.  A tile's rows g are even columns, g + 8 odd ones, which are 16 times as large.  Two steps to a turn of the loop: with all four its
+        // instructions outgrow the nearest cache (96 sequences 81 us, then 73).
         const int row = (lane & 8) + kv4_key(lane & 7);
         const uint32_t values = st + 4096 + (row >> 1) * 128 + ((((row & 1) * 4 + (lane >> 4)) ^ (row >> 1 & 7)) << 4);
 #pragma unroll 1
@@ -947,66 +922,54 @@ struct KvFour {
                 ldmatrix_trans(x[0], values + (u0 + u) * 1024);
                 ldmatrix_trans(x[1], (values ^ 32) + (u0 + u) * 1024);
 #pragma unroll
-                for (int h = 0; h < HG; ++h) {
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        hi[u][h][r] = transposed(hi[u][h][r]);
-                        if (!TWICE) lo[u][h][r] = transposed(lo[u][h][r]);
-                    }
+                for (int r = 0; r < 2; ++r) {
+                    hi[u][r] = transposed(hi[u][r]);
+                    if (!TWICE) lo[u][r] = transposed(lo[u][r]);
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     uint32_t a = x[j >> 2][j & 2], b = x[j >> 2][(j & 2) + 1];
                     if (j & 1) { a >>= 8; b >>= 8; }
-#pragma unroll
-                    for (int h = 0; h < HG; ++h) {
-                        mma_bf16(acc[h][j], a & 0x000F000Fu, a & 0x00F000F0u, b & 0x000F000Fu, b & 0x00F000F0u, hi[u][h][0], hi[u][h][1]);
-                        if (!TWICE) mma_bf16(acc[h][j], a & 0x000F000Fu, a & 0x00F000F0u, b & 0x000F000Fu, b & 0x00F000F0u, lo[u][h][0], lo[u][h][1]);
-                    }
+                    mma_bf16(acc[j], a & 0x000F000Fu, a & 0x00F000F0u, b & 0x000F000Fu, b & 0x00F000F0u, hi[u][0], hi[u][1]);
+                    if (!TWICE) mma_bf16(acc[j], a & 0x000F000Fu, a & 0x00F000F0u, b & 0x000F000Fu, b & 0x00F000F0u, lo[u][0], lo[u][1]);
                 }
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
 #pragma unroll
-                for (int h = 0; h < HG; ++h) {
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) { hi[u][h][r] = hi[u + 2][h][r]; if (!TWICE) lo[u][h][r] = lo[u + 2][h][r]; }
-                }
+                for (int r = 0; r < 2; ++r) { hi[u][r] = hi[u + 2][r]; if (!TWICE) lo[u][r] = lo[u + 2][r]; }
             }
         }
     }
 
     // The sums as the other kinds have them (those of `twice` are added by the caller): accumulators of the weights' own size with what the least values add to every
-    // column, maximum and sum of head g (and 8 + g).
-    __device__ __forceinline__ void end(bool twice, float (&acc)[HG][8][4], float (&m_out)[HG], float (&l_out)[HG]) {
+    // column, maximum and sum of head g.
+    __device__ __forceinline__ void end(bool twice, float (&acc)[8][4], float& m_out, float& l_out) {
         const int lane = threadIdx.x & 31, g = lane >> 2, from = (twice ? g & 3 : g) >> 1;
+        float m_of[2], l_of[2];
 #pragma unroll
-        for (int h = 0; h < HG; ++h) {
-            float m_of[2], l_of[2];
+        for (int c = 0; c < 2; ++c) {
+            float &sum = c ? l.y : l.x, &add = c ? offset.y : offset.x;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float &sum = c ? l[h].y : l[h].x, &add = c ? offset[h].y : offset[h].x;
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1) {
-                    sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                    add += __shfl_xor_sync(0xffffffffu, add, o);
-                }
-                if (twice) {
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                    add += __shfl_xor_sync(0xffffffffu, add, 2);
-                }
-                const float down = __uint_as_float((uint32_t)(127 + 100 - k[h][c]) << 23);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    acc[h][j][c] = __fmaf_rn(acc[h][j][c] * 8589934592.0f, down, add);            // 2^33
-                    acc[h][j][c + 2] = __fmaf_rn(acc[h][j][c + 2] * 536870912.0f, down, add);     // 2^29
-                }
-                m_of[c] = __shfl_sync(0xffffffffu, m[h][c] * (c ? zs[h].y : zs[h].x), from);
-                l_of[c] = __shfl_sync(0xffffffffu, sum, from);
+            for (int o = 4; o < 32; o <<= 1) {
+                sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                add += __shfl_xor_sync(0xffffffffu, add, o);
             }
-            m_out[h] = g & 1 ? m_of[1] : m_of[0];
-            l_out[h] = g & 1 ? l_of[1] : l_of[0];
+            if (twice) {
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                add += __shfl_xor_sync(0xffffffffu, add, 2);
+            }
+            const float down = __uint_as_float((uint32_t)(127 + 100 - k[c]) << 23);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                acc[j][c] = __fmaf_rn(acc[j][c] * 8589934592.0f, down, add);            // 2^33
+                acc[j][c + 2] = __fmaf_rn(acc[j][c + 2] * 536870912.0f, down, add);     // 2^29
+            }
+            m_of[c] = __shfl_sync(0xffffffffu, m[c] * (c ? zs.y : zs.x), from);
+            l_of[c] = __shfl_sync(0xffffffffu, sum, from);
         }
+        m_out = g & 1 ? m_of[1] : m_of[0];
+        l_out = g & 1 ? l_of[1] : l_of[0];
     }
 };
 
@@ -1298,8 +1261,8 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         typename K::Segment seg = segs[k & 1];
         if ((solo || mate == 0) && seg.end < c1) describe(seg.end, segs[(k + 1) & 1]);
         float z_scale[HG], acc[HG][8][4], m[HG], l[HG];
-        KvFour<HG> four;
-        if (TYPE == KV_UINT4) four.begin(qa, a.scale * 1.4426950408889634f, acc);
+        KvFour four;
+        if (TYPE == KV_UINT4) four.begin(qa[0], a.scale * 1.4426950408889634f, acc[0]);
         else
 #pragma unroll
         for (int h = 0; h < HG; ++h) {
@@ -1372,7 +1335,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 __syncwarp();
             }
 
-            if constexpr (TYPE == KV_UINT4) four.chunk(st, scales, valid, twice, qa, acc);
+            if constexpr (TYPE == KV_UINT4) four.chunk(st, scales, valid, twice, qa[0], acc[0]);
             else {
             // scores of 8 keys a tile; a tile's column n is its key kv_perm(n), so keys t and t + 4 are this thread's
             float s[TILES][4];
@@ -1538,7 +1501,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
                 for (int c = 0; c < 4; ++c) acc[0][j][c] += __shfl_xor_sync(0xffffffffu, acc[0][j][c], 2);
             }
         }
-        if (TYPE == KV_UINT4) four.end(twice, acc, m, l);
+        if (TYPE == KV_UINT4) four.end(twice, acc[0], m[0], l[0]);
         else
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
@@ -1820,7 +1783,7 @@ hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, 
     if (ldq < qrow || ldo < qrow || ldp < width || (k_new && (ldk < krow || ldv < krow))) { set_error("kv_attention: a row pitch is below the row"); return HD_ERR_UNSUPPORTED; }
     if (!(scale > 0.f) || scale > 3.0e38f) { set_error("kv_attention: scale %g", scale); return HD_ERR_UNSUPPORTED; }
     if (workspace_bytes < o1_kv_attention_workspace_bytes(heads, c.heads) || (((uintptr_t)workspace) & 15)) { set_error("kv_attention: workspace too small or unaligned"); return HD_ERR_OOM; }
-    const int group = heads / c.heads, hg = group <= 8 ? 1 : 2, of_heads = (group + 8 * hg - 1) / (8 * hg), keys = cache->type == O1_KV_BF16 ? 16 : cache->type == O1_KV_UINT4 ? 64 : 32;
+    const int group = heads / c.heads, hg = group <= 8 || cache->type == O1_KV_UINT4 ? 1 : 2, of_heads = (group + 8 * hg - 1) / (8 * hg), keys = cache->type == O1_KV_BF16 ? 16 : cache->type == O1_KV_UINT4 ? 64 : 32;
     // the stream's index and costs are ints: fewer sequences a launch where the table allows for more, and a limit of items of a sequence
     const int64_t item_chunks = ((int64_t)width * c.page_size + keys - 1) / keys, each = item_chunks * c.heads * of_heads;
     if ((int64_t)width * c.page_size > INT32_MAX - 64 || each > (1 << 30) || (int64_t)c.heads * of_heads > (1 << 18) || (int64_t)c.pages * c.heads * c.page_size > INT32_MAX) { set_error("kv_attention: a table of %d pages of %d tokens for %d heads, or a cache of %d pages, is too large", width, c.page_size, heads, c.pages); return HD_ERR_UNSUPPORTED; }
@@ -1857,7 +1820,7 @@ hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, 
         cudaError_t e;
         if (cache->type == O1_KV_BF16) e = hg == 1 ? launch_attention<KV_BF16, 1>(k_map, v_map, a, item_chunks, items, current_stream()) : launch_attention<KV_BF16, 2>(k_map, v_map, a, item_chunks, items, current_stream());
         else if (cache->type == O1_KV_FP8) e = hg == 1 ? launch_attention<KV_FP8, 1>(k_map, v_map, a, item_chunks, items, current_stream()) : launch_attention<KV_FP8, 2>(k_map, v_map, a, item_chunks, items, current_stream());
-        else if (four_bits) e = hg == 1 ? launch_attention<KV_UINT4, 1>(k_map, v_map, a, item_chunks, items, current_stream()) : launch_attention<KV_UINT4, 2>(k_map, v_map, a, item_chunks, items, current_stream());
+        else if (four_bits) e = launch_attention<KV_UINT4, 1>(k_map, v_map, a, item_chunks, items, current_stream());
         else e = hg == 1 ? launch_attention<KV_INT8, 1>(k_map, v_map, a, item_chunks, items, current_stream()) : launch_attention<KV_INT8, 2>(k_map, v_map, a, item_chunks, items, current_stream());
         if (!launch_ok(e, "kv_attention")) return HD_ERR_RUNTIME;
         o1_launch_count_add(1);
