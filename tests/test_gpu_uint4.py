@@ -244,6 +244,54 @@ def test_a_sequence_alone_and_among_others(pkg, dev, lens):
 
 
 # ------------------------------------------------------------------ what four bits add
+# More items than half of the teams, and much work: parts to warps, an item joined from as many as have some of it (of the longest one from more than a thousand, in groups).
+AMONG = [([1] * 120 + [100000] + [3] * 120, 1, 2, 32), ([2] * 130 + [20000, 0, 9000] + [70] * 110, 1, 8, 64), ([64 + 61 * (i % 40) for i in range(120)], 2, 4, 48),
+         ([500 + i for i in range(150)], 2, 12, 16)]
+
+
+@gpu
+@pytest.mark.parametrize("lens,kv_heads,group,page", AMONG)
+def test_long_sequences_among_many(pkg, dev, lens, kv_heads, group, page):
+    c = Case4(pkg, dev, "uint4", lens, kv_heads, page, seed=len(lens))
+    c.fill()
+    q = normal((len(lens), kv_heads * group, D), gen(13), 1.5)
+    out, lse = c.cache.attend(q.to(dev), c.dtable, c.dlens, lse=True)
+    c.check(q, out, lse)
+    for _ in range(3):
+        again, lse2 = c.cache.attend(q.to(dev), c.dtable, c.dlens, lse=True)
+        assert torch.equal(out, again) and torch.equal(lse, lse2)
+    assert torch.equal(out, c.cache.attend(q.to(dev), c.dtable, c.dlens))
+
+
+@gpu
+@pytest.mark.parametrize("lens,kv_heads,group,page", [AMONG[0], AMONG[2]])
+def test_new_rows_of_long_sequences_among_many(pkg, dev, lens, kv_heads, group, page):
+    base.test_new_rows_appended_by_the_same_call(pkg, dev, "uint4", [n for n in lens], kv_heads, group, page)
+
+
+@gpu
+def test_many_sequences_with_wrong_tables(pkg, dev):
+    for lens, page in (([1 + b % 40 for b in range(260)], 16), ([300 + b for b in range(150)], 32)):
+        c = Case4(pkg, dev, "uint4", lens, 2, page)
+        c.fill()
+        n = len(lens)
+        q = normal((n, 8, D), gen(1)).to(dev)
+        good = c.cache.attend(q, c.dtable, c.dlens)
+        assert pkg.lib.o1_device_error() == 0
+        t, ln = c.dtable.clone(), c.dlens.clone()
+        t[100, 0], t[7, 0] = c.cache.pages, -1
+        out = c.cache.attend(q, t, c.dlens)
+        rest = [b for b in range(n) if b not in (7, 100)]
+        assert pkg.lib.o1_device_error() == 70 and torch.equal(out[rest], good[rest])
+        ln[100], ln[7] = -1, page * c.table.shape[1] + 1
+        out = c.cache.attend(q, c.dtable, ln)
+        # (lengths decide how rows are shared out: the others within their bounds, not the same bits)
+        assert pkg.lib.o1_device_error() == 71 and (out[[7, 100]] == 0).all()
+        c.lens = [0 if b in (7, 100) else x for b, x in enumerate(lens)]
+        c.k, c.v = ([x[:k] for x, k in zip(rows, c.lens)] for rows in (c.k, c.v))
+        c.check(q.cpu(), out)
+
+
 @gpu
 @pytest.mark.parametrize("group", [1, 4, 5, 8, 16])
 def test_values_of_very_different_sizes(pkg, dev, group):
