@@ -31,7 +31,7 @@ BF16, I32, I64, F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
 _stream = lib.o1_get_stream
 Grown = namedtuple("Grown", "slots positions starts lens pages")
 Grown.__doc__ = """What KvPages.grow gives: slots [rows] int64 and positions [rows] int32 of the new rows, starts [requests + 1] (where each request's rows begin), lens [requests]
-and pages [requests, width] as KvCache.attend takes them."""
+and pages [requests, width] as KvCache.attend takes them.  (One allocation, which lives as long as any of them.)"""
 _binding.setup(*(C.cast(f, C.c_void_p).value for f in (lib.o1_kv_write, lib.o1_kv_read, lib.o1_kv_attention, lib.o1_residual_norm, lib.o1_get_stream, lib.o1_capture_id,
                                                        lib.o1_kv_pages_grow, lib.o1_kv_pages_shrink, lib.o1_rotary)), O1Error, check, Grown)
 
@@ -238,7 +238,7 @@ class Rotary:
     def __call__(self, x, positions, inverse=False, out=None):
         """Rows x [rows, heads, head_dim] bf16 or fp32 (rows of any pitch), or a pair of them (queries and keys), turned by positions [rows] int32 or int64.
 
-        inverse: turned back, which is also the gradient.  out: what to fill, like x (x itself: in place)."""
+        inverse: turned back, which is also the gradient.  out: what to fill, like x (x itself: in place).  (A pair's results share an allocation.)"""
         return _binding.rotary(self._at, self._gpu, positions, inverse, x, out)
 
 
