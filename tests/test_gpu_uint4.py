@@ -264,6 +264,27 @@ def test_long_sequences_among_many(pkg, dev, lens, kv_heads, group, page):
 
 
 @gpu
+@pytest.mark.parametrize("rows,batch,group", [(100000, 450, 1), (30000, 450, 4), (30000, 300, 7), (100000, 1, 4)])
+def test_long_sums_keep_their_bits(pkg, dev, rows, batch, group):
+    """Hundreds of chunks a warp with scores that hardly differ: codes are not negative, so that their sums grow all the way, and the tensor cores cut what they add; the error stays
+    that of a short sequence.  (All sequences have the same rows.)"""
+    c = Case4(pkg, dev, "uint4", [rows], 1, 64, seed=9, width_extra=0)
+    c.fill()
+    q = normal((batch, group, D), gen(3), 0.05)
+    out, lse = c.cache.attend(q.to(dev), c.dtable.expand(batch, -1).contiguous(), c.dlens.expand(batch).contiguous(), lse=True)
+    held = [kept(x[0][:, 0]) for x in (c.k, c.v)]
+    (k, v), (ka, va) = ([f(*h) for h in held] for f in (value, magnitude))
+    some = slice(0, 450, 29)
+    qd = q[some].double()
+    z = qd @ k.T * D ** -0.5
+    ref = torch.logsumexp(z, -1)
+    p = torch.exp(z - ref[..., None])
+    size = (qd.abs() @ ka.T * D ** -0.5).amax(-1)
+    between(out[some], p @ v, (p @ va) * (2.0 * 2.0 ** -19 * size + 2.0 ** -17 + 2.0 ** -18)[..., None], "out")
+    assert ((lse[some].cpu().double() - ref).abs() <= 2.0 ** -19 * size + 2.0 ** -21 * (1 + ref.abs())).all()
+
+
+@gpu
 @pytest.mark.parametrize("lens,kv_heads,group,page", [AMONG[0], AMONG[2]])
 def test_new_rows_of_long_sequences_among_many(pkg, dev, lens, kv_heads, group, page):
     base.test_new_rows_appended_by_the_same_call(pkg, dev, "uint4", [n for n in lens], kv_heads, group, page)
