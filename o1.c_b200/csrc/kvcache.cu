@@ -381,7 +381,7 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
 //    of a byte are exact in f16 and bf16.  Keys' codes go through f16, which takes fewer instructions, with queries scaled to f16's top by a power of two for each head (those
 //    below 2^-29 of its largest lose bits); values' codes through bf16, whose range a probability needs.  The result is rounded once.
 //  * Rows of four bits (KvFour) are 64 to a chunk and the chunks, for the same bytes, twice the arithmetic: instructions bound them, not memory.  302 MB (96 sequences of 300 to 5400
-//    rows, 8 kv heads, 32 heads) in 62.5 us, 4.8 TB/s, 74 % of a copy's rate; 109 MB (one of 100003) in 30.4; 39.7 MB (37 of 0 to 1999, 16 heads) in 19.5.  A chunk is some 960
+//    rows, 8 kv heads, 32 heads) in 63.4 us, 4.75 TB/s, 73 % of a copy's rate; 109 MB (one of 100003) in 30.6; 39.7 MB (37 of 0 to 1999, 16 heads) in 20.2.  A chunk is some 980
 //    instructions (all of a launch's counted), of which an SM issues 2.2 a clock; half of the ALU pipe's time is the codes' masks and shifts.  As the other kinds have it (queries
 //    as rows, codes to pairs of keys by byte permutes) it was 1420 and 99 us.
 // Times below: "batch" 24 sequences of 1 to 2100 rows of bf16, "shared" 32 sequences of 1000 to 3000, 16 query heads on one kv head; us.
@@ -722,6 +722,10 @@ __device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, 
 //    keys and gives the other its results, one the values and one the rests.
 //  * Weights p_t s_t are held times 2^k: the sums, of codes 2^-133 of themselves, are of normal size where the largest weight so far (a chunk's largest probability times its largest
 //    scale bounds it) is between 2^90 and 2^112, and weights of 2^-80 of that one are still there.  Largest weight and k follow the running maximum, and k moves seldom.
+//  * Codes are not negative, so a column's sum grows with every row, and what the tensor cores cut off from each product's sum is always to one side: 400 chunks on end (450 sequences of
+//    100000 rows that weigh the same) put a result 1.2e-5 off, 0.4 % of it. So one column's sum, which the others are near, is taken off all of them where sums are rescaled, and every
+//    64 chunks, and counts as the least values do: 0.02 of that is left. It costs 302 MB 1.1 of 63.4 us, by its registers; as a step of its own behind the products, or between
+//    two loops, no less.
 //  * At most eight heads: more on a kv head are items of their own, which read its rows again (from L2 as a rule).  With sixteen to an item, as the other kinds have it, registers
 //    spill and two teams are left: 128 sequences of up to 4000 rows, 2 kv heads of 16: 56.6 us, now 44.5; 50000 rows of one 22.2, now 18.4.
 struct KvFour {
@@ -838,7 +842,7 @@ struct KvFour {
                 for (int c = 0; c < 2; ++c) s[TWICE ? n : n >> 1][(TWICE ? 0 : 2 * (n & 1)) + c] = -INFINITY;
             }
         }
-        bool moved = false;
+        bool moved = (valid & KEYS * 60) == KEYS * 60;          // (four chunks of each 64, one to a warp of a team)
         float top[2], ref[2], a[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -879,15 +883,14 @@ struct KvFour {
         }
         if (__any_sync(0xffffffffu, moved)) {
             const float2 alpha = make_float2(a[0], a[1]);
+            const float2 off = mul2(make_float2(__shfl_sync(0xffffffffu, acc[0][0], lane & 3), __shfl_sync(0xffffffffu, acc[0][1], lane & 3)), alpha);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-#pragma unroll
-                for (int c = 0; c < 4; c += 2) {
-                    const float2 r = mul2(make_float2(acc[j][c], acc[j][c + 1]), alpha);
-                    acc[j][c] = r.x;
-                    acc[j][c + 1] = r.y;
-                }
+                const float2 even = fma2(make_float2(acc[j][0], acc[j][1]), alpha, mul2(off, both(-1.f))), odd = fma2(make_float2(acc[j][2], acc[j][3]), alpha, mul2(off, both(-16.f)));
+                acc[j][0] = even.x; acc[j][1] = even.y; acc[j][2] = odd.x; acc[j][3] = odd.y;
             }
+            const float2 down = make_float2(__uint_as_float((uint32_t)(127 + 100 - k[0]) << 23), __uint_as_float((uint32_t)(127 + 100 - k[1]) << 23));
+            if (lane < 4) offset = fma2(mul2(off, both(8589934592.0f)), down, offset);        // 2^33
         }
         // weights, in two parts of bf16; [tile of 16 keys][its upper 8 keys]
         const float2 up = make_float2(__uint_as_float((uint32_t)(127 + k[0]) << 23), __uint_as_float((uint32_t)(127 + k[1]) << 23));

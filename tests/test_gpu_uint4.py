@@ -285,6 +285,21 @@ def test_long_sums_keep_their_bits(pkg, dev, rows, batch, group):
 
 
 @gpu
+def test_long_sums_lean_to_no_side(pkg, dev):
+    """400 chunks a warp.  What is left of the error is the result's rounding: at most half a step, 2^-8 of the value, to either side alike, so that its square is (2^-8 x)^2 / 3 at most on
+    average and the mean over the 128 columns (the sequences' results are close to one another and count as one) within 6 deviations of 0.  Cut sums lean to one side by three times that."""
+    c = Case4(pkg, dev, "uint4", [100000], 1, 64, seed=9, width_extra=0)
+    c.fill()
+    q = normal((450, 1, D), gen(3), 0.05)
+    out = c.cache.attend(q.to(dev), c.dtable.expand(450, -1).contiguous(), c.dlens.expand(450).contiguous())
+    k, v = (value(*kept(x[0][:, 0])) for x in (c.k, c.v))
+    qd = q[:20].double()
+    ref = torch.softmax(qd @ k.T * D ** -0.5, -1) @ v
+    error = out[:20].cpu().double() - ref
+    assert abs(error.mean().item()) <= 6 * 2.0 ** -8 * (ref.square().mean().item() / 3 / D) ** 0.5
+
+
+@gpu
 @pytest.mark.parametrize("lens,kv_heads,group,page", [AMONG[0], AMONG[2]])
 def test_new_rows_of_long_sequences_among_many(pkg, dev, lens, kv_heads, group, page):
     base.test_new_rows_appended_by_the_same_call(pkg, dev, "uint4", [n for n in lens], kv_heads, group, page)
