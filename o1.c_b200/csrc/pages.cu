@@ -37,6 +37,9 @@ struct PgArgs {
 // seq < 0: refused (its rows have no slots); after: its rows when it is done
 struct PgRequest { int seq, len, after; };
 
+// (twice PG_FULL is beyond int)
+__device__ __forceinline__ int pg_add(int a, int b) { return (int)min((unsigned)a + (unsigned)b, (unsigned)PG_FULL); }
+
 // Sums of v over the block's threads before this one, and over all, of both components, which are between 0 and PG_FULL and stay there.
 __device__ __forceinline__ int2 pg_scan(int2 v, int2& all, int2* part) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -44,7 +47,7 @@ __device__ __forceinline__ int2 pg_scan(int2 v, int2& all, int2* part) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int x = __shfl_up_sync(0xffffffffu, sum.x, o), y = __shfl_up_sync(0xffffffffu, sum.y, o);
-        if (lane >= o) { sum.x = min(sum.x + x, PG_FULL); sum.y = min(sum.y + y, PG_FULL); }
+        if (lane >= o) { sum.x = pg_add(sum.x, x); sum.y = pg_add(sum.y, y); }
     }
     if (lane == 31) part[warp] = sum;
     int2 before = make_int2(__shfl_up_sync(0xffffffffu, sum.x, 1), __shfl_up_sync(0xffffffffu, sum.y, 1));
@@ -54,11 +57,11 @@ __device__ __forceinline__ int2 pg_scan(int2 v, int2& all, int2* part) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int x = __shfl_up_sync(0xffffffffu, p.x, o), y = __shfl_up_sync(0xffffffffu, p.y, o);
-        if (lane >= o) { p.x = min(p.x + x, PG_FULL); p.y = min(p.y + y, PG_FULL); }
+        if (lane >= o) { p.x = pg_add(p.x, x); p.y = pg_add(p.y, y); }
     }
     all = make_int2(__shfl_sync(0xffffffffu, p.x, 31), __shfl_sync(0xffffffffu, p.y, 31));
     const int x = __shfl_sync(0xffffffffu, p.x, max(warp - 1, 0)), y = __shfl_sync(0xffffffffu, p.y, max(warp - 1, 0));
-    if (warp > 0) before = make_int2(min(before.x + x, PG_FULL), min(before.y + y, PG_FULL));
+    if (warp > 0) before = make_int2(pg_add(before.x, x), pg_add(before.y, y));
     return before;
 }
 
@@ -112,8 +115,8 @@ pages_kernel(const PgArgs a) {
             else mine.y = GROW ? whole(after) - whole(len) : whole(len) - whole(after);
         }
         int2 all, before = pg_scan(mine, all, part);
-        before = make_int2(min(before.x + base.x, PG_FULL), min(before.y + base.y, PG_FULL));
-        base = make_int2(min(base.x + all.x, PG_FULL), min(base.y + all.y, PG_FULL));
+        before = make_int2(pg_add(before.x, base.x), pg_add(before.y, base.y));
+        base = make_int2(pg_add(base.x, all.x), pg_add(base.y, all.y));
         if (b < a.batch) {
             // Both sums only grow, so what is refused for want of rows or pages has behind it only requests that are too, or that need no page: pages leave the stack from its top.
             if (GROW && seq >= 0 && mine.x > a.rows - before.x && mine.x > 0) { seq = -1; code = ERR_PG_LENGTH; }

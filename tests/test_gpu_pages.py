@@ -137,6 +137,21 @@ def test_growing_and_shrinking(pkg, dev, pages, page, seqs, width):
 
 
 @gpu
+@pytest.mark.parametrize("many", [2, 3, 4, 5, 8, 33, 1100])
+def test_many_counts_beyond_every_limit(pkg, dev, many):
+    """Counts whose sum passes 2^31, and 2^32: none of them is served, nor what is behind them, and what is before them is; sums end at 2^30."""
+    seqs = many + 4
+    p, m = pkg.KvPages(64, 16, seqs, 8, dev), Model(64, 16, seqs, 8)
+    for names in (None, list(range(seqs - 1, -1, -1))):
+        counts = [3, 0] + [2 ** 31 - 1] * many + [0, 5]
+        got = p.grow(ints(counts, dev), 40, names and ints(names, dev))
+        want = m.grow(counts, 40, names)
+        check(got, want[:2] + ([min(s, 2 ** 30) for s in want[2]],) + want[3:5], names is not None)
+        m.same(p)
+        code(pkg, want[5])
+
+
+@gpu
 def test_what_goes_comes_back_in_its_order(pkg, dev):
     p = pkg.KvPages(100, 16, 10, 30, dev)
     p.grow(ints([5, 100, 0, 33], dev), 138, ints([3, 1, 9, 0], dev))
