@@ -192,6 +192,7 @@ class KvPages:
 
     def reset(self):
         """Every page free, every sequence empty."""
+        _need(torch.cuda.current_device() == self._gpu, "KvPages.reset: its memory is on another GPU than the current one")
         check(lib.o1_kv_pages_reset(C.byref(self.c)), "o1_kv_pages_reset")
 
     def grow(self, counts, rows, seqs=None):

@@ -287,6 +287,20 @@ def test_arguments_that_do_not_fit(pkg, dev):
     pkg.check_cuda_errbuf("after refusals")
 
 
+@gpu
+def test_pages_of_another_gpu_are_refused(pkg, dev):
+    p = pkg.KvPages(8, 16, 4, 4, dev)
+    p._gpu += 1           # (as if its memory were there)
+    one = ints([1], dev)
+    for call in (p.reset, lambda: p.grow(one, 1), lambda: p.shrink(one)):
+        with pytest.raises(pkg.O1Error, match="another GPU than the current one"):
+            call()
+    p._gpu -= 1
+    p.reset()
+    check(p.grow(one, 1), ([0], [0], [0, 1], [1], [[0, -1, -1, -1]]))
+    code(pkg, set())
+
+
 def test_entry_points_refuse_before_they_touch_the_gpu(pkg):
     lib, one = pkg.lib, C.c_void_p(4096)
     good = dict(table=4096, lens=4096, free_pages=4096, state=4096, pages=4, page_size=16, max_seqs=3, width=5)
