@@ -476,6 +476,13 @@ __device__ __forceinline__ void two_parts(float a, float b, uint32_t& hi, uint32
     hi = pack_bf16x2(a, b);
     lo = pack_bf16x2(a - bf16lo(hi), b - bf16hi(hi));
 }
+// The same, and what neither holds.
+__device__ __forceinline__ float2 two_parts_lost(float2 x, uint32_t& hi, uint32_t& lo) {
+    hi = pack_bf16x2(x.x, x.y);
+    const float2 rest = make_float2(x.x - bf16lo(hi), x.y - bf16hi(hi));
+    lo = pack_bf16x2(rest.x, rest.y);
+    return make_float2(rest.x - bf16lo(lo), rest.y - bf16hi(lo));
+}
 template <int SEL>
 __device__ __forceinline__ uint32_t prmt(uint32_t x, uint32_t y) {      // (a selector's top bit: the byte's sign, eight times)
     uint32_t r;
@@ -726,6 +733,8 @@ __device__ __forceinline__ void kv_join(const KvAttn& a, int first, int stride, 
 //    100000 rows that weigh the same) put a result 1.2e-5 off, 0.4 % of it. So one column's sum, which the others are near, is taken off all of them where sums are rescaled, and every
 //    64 chunks, and counts as the least values do: 0.02 of that is left. It costs 302 MB 1.1 of 63.4 us, by its registers; as a step of its own behind the products, or between
 //    two loops, no less.
+//  * What a weight loses to its two parts of bf16 (2^-17 of it at most) is lost to the codes alone, while the least value counts with all of p: 7.5 times that, the codes' middle, goes to
+//    the least values' sum, so that the loss is one of s (c - 7.5), not of s c.  Results of normal rows are half as far from 64 bits before their rounding; 302 MB 60.6 -> 60.9 us.
 //  * At most eight heads: more on a kv head are items of their own, which read its rows again (from L2 as a rule).  With sixteen to an item, as the other kinds have it, registers
 //    spill and two teams are left: 128 sequences of up to 4000 rows, 2 kv heads of 16: 56.6 us, now 44.5; 50000 rows of one 22.2, now 18.4.
 struct KvFour {
@@ -895,6 +904,7 @@ struct KvFour {
         // weights, in two parts of bf16; [tile of 16 keys][its upper 8 keys]
         const float2 up = make_float2(__uint_as_float((uint32_t)(127 + k[0]) << 23), __uint_as_float((uint32_t)(127 + k[1]) << 23));
         uint32_t hi[4][2], lo[4][2];
+        float2 lost = both(0.f);
 #pragma unroll
         for (int n = 0; n < MINE; ++n) {
             const uint32_t pair = lds_u32(pairs + KEYS * 4 + n * (APART * 4));
@@ -902,8 +912,10 @@ struct KvFour {
             const float2 p = make_float2(z[0], z[1]);
             offset = fma2(p, both(bf16hi(pair)), offset);
             const float2 w = mul2(mul2(p, both(bf16lo(pair))), up);
-            two_parts(w.x, w.y, hi[TWICE ? n : n >> 1][TWICE ? 0 : n & 1], lo[TWICE ? n : n >> 1][TWICE ? 0 : n & 1]);
+            lost = add2(lost, two_parts_lost(w, hi[TWICE ? n : n >> 1][TWICE ? 0 : n & 1], lo[TWICE ? n : n >> 1][TWICE ? 0 : n & 1]));
         }
+        offset = fma2(mul2(lost, both(7.5f * 7.888609052210118e-31f)), make_float2(__uint_as_float((uint32_t)(127 + 100 - k[0]) << 23), __uint_as_float((uint32_t)(127 + 100 - k[1]) << 23)),
+                      offset);            // (2^-100)
         if (TWICE) {            // heads in the lower columns' threads get the values, the others the rests
 #pragma unroll
             for (int i = 0; i < 4; ++i) {

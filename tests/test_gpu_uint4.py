@@ -482,3 +482,23 @@ def test_entry_points_refuse_before_they_touch_the_gpu(pkg):
         assert pkg.lib.o1_kv_write(C.byref(K(**{**good, **change})), one, 256, one, 256, one, 1) == want, change
         assert b"kv_write" in pkg.lib.hd_cuda_last_error()
     pkg.lib.hd_cuda_clear_error()
+
+
+# ------------------------------------------------------------------ bits of the sums
+@gpu
+@pytest.mark.parametrize("kv_heads,group,batch", [(1, 1, 40), (2, 4, 40), (1, 8, 40), (8, 1, 60), (8, 4, 60), (8, 8, 60)])
+def test_values_in_the_middle_of_their_rows(pkg, dev, kv_heads, group, batch):
+    """Rows of -7.5, 7.5 and half ones (a scale of 1, codes 7 and 8), each key twice with the halves' signs turned: exactly zero in all but two columns.  What a probability loses to 16 bits takes
+    the codes' middle with it, so that only sums in fp32 are left: 2^-19 of the codes' (as for scores) and 2^-20 of the least values' (16 additions), 7.5 each.  (62 of 64 rows weigh the same, and
+    16 bits of a weight are off by up to 2^-17: 5.7e-5 where the bound is 2.1e-5.)"""
+    c = Case4(pkg, dev, "uint4", [64] * batch, kv_heads, 64, seed=3, width_extra=0)
+    sign = torch.where((torch.arange(64)[:, None] + torch.arange(D)) % 2 > 0, 0.5, -0.5).bfloat16()
+    sign[:, 0], sign[:, 1] = -7.5, 7.5
+    for b in range(batch):
+        c.k[b][:2], c.k[b][2:] = c.k[b][:1], c.k[b][2:3]
+        c.v[b][:] = sign[:, None]
+    c.fill()
+    q = normal((batch, kv_heads * group, D), gen(3), 0.4)
+    out, lse = c.cache.attend(q.to(dev), c.dtable, c.dlens, lse=True)
+    c.check(q, out, lse)
+    assert float(out[..., 2:].float().abs().max()) <= 7.5 * (2.0 ** -19 + 2.0 ** -20)
