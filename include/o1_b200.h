@@ -794,7 +794,7 @@ hd_status o1_kv_read(const o1_kv_cache *cache, void *k, int64_t ldk, void *v, in
  * attended to by the same call; no other sequence of the call has that slot among its rows.  workspace: o1_kv_attention_workspace_bytes(heads, kv_heads) bytes, 16-byte aligned, its first
  * O1_KV_ATTENTION_COUNTERS bytes zero-filled once before its first use and all of it left to these calls from then on; calls that may overlap on the GPU each need their own.  The result is the same
  * bits from call to call with the same lengths and width; beside other sequences a sequence's differs by the order of its fp32 sums.  Values of v up to 2^90 in magnitude (the sums are 2^20 times larger and in fp32);
- * with O1_KV_UINT4 queries up to 2^124; at most 2^31 - 1 rows (pages *
+ * with O1_KV_UINT4 scale at most 2^114 and scale times the largest |q| of a head at most 2^121; at most 2^31 - 1 rows (pages *
  * kv_heads * page_size) in the cache. */
 #define O1_KV_ATTENTION_COUNTERS 32768
 int64_t o1_kv_attention_workspace_bytes(int heads, int kv_heads);

@@ -417,6 +417,7 @@ static constexpr int KV_JOIN_STEP = 4;                 // parts that a join has 
 static constexpr int ERR_KV_WAIT = 72;                 // a wait of the attention kernel ran out
 static constexpr float KV_LIFT = 20.0f;                // probabilities are relative to 2^-20 of the largest: those that fp32 has no value for are 2^-146 and less of it
 
+static constexpr float KV4_SCALE_MAX = 0x1p114f;       // of four bits (see KvFour::begin)
 static constexpr int KV4_JOIN_STEP = 8;                // of four bits and up to four heads: one head to a warp (one of 100003 rows 31.1 us, with a step of 4 30.45, 8 30.4, 16 31)
 struct KvAttn {
     KvView c;
@@ -755,9 +756,10 @@ struct KvFour {
         top = max(top & 0xFFFFu, top >> 16);
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // queries times 2^x, the largest one below 2^127
-        const int x = min(120, 253 - (int)max(top >> 7, 1u));
-        const float z = scale * __uint_as_float((uint32_t)(127 + 70) << 23) * __uint_as_float((uint32_t)(127 + 63 - x) << 23);
+        // queries times 2^x, the largest one below 2^128; the factor 2^(133 - x) that makes up for it in two steps, each at least 1: nothing on the way is larger than z, which is finite
+        // where scale times the largest query, or times 2^7, is at most 2^121
+        const int x = min(120, 254 - (int)max(top >> 7, 1u)), h = (133 - x) >> 1;
+        const float z = scale * __uint_as_float((uint32_t)(127 + h) << 23) * __uint_as_float((uint32_t)(127 + 133 - x - h) << 23);
         const uint32_t up = (uint32_t)(127 + x) * 0x00800080u, up16 = up - 0x02000200u;
 #pragma unroll
         for (int i = 0; i < 16; ++i) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(q[i]) : "r"(i & 1 ? up16 : up));
@@ -1796,7 +1798,7 @@ hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, 
     if (!q || (!pages && width > 0) || !lens || !out || !workspace || (!k_new != !v_new)) { set_error("kv_attention: null argument"); return HD_ERR_MISSING; }
     const int64_t qrow = (int64_t)heads * KV_D, krow = (int64_t)c.heads * KV_D;
     if (ldq < qrow || ldo < qrow || ldp < width || (k_new && (ldk < krow || ldv < krow))) { set_error("kv_attention: a row pitch is below the row"); return HD_ERR_UNSUPPORTED; }
-    if (!(scale > 0.f) || scale > 3.0e38f) { set_error("kv_attention: scale %g", scale); return HD_ERR_UNSUPPORTED; }
+    if (!(scale > 0.f) || scale > (cache->type == O1_KV_UINT4 ? KV4_SCALE_MAX : 3.0e38f)) { set_error("kv_attention: scale %g", scale); return HD_ERR_UNSUPPORTED; }
     if (workspace_bytes < o1_kv_attention_workspace_bytes(heads, c.heads) || (((uintptr_t)workspace) & 15)) { set_error("kv_attention: workspace too small or unaligned"); return HD_ERR_OOM; }
     const int group = heads / c.heads, hg = group <= 8 || cache->type == O1_KV_UINT4 ? 1 : 2, of_heads = (group + 8 * hg - 1) / (8 * hg), keys = cache->type == O1_KV_BF16 ? 16 : cache->type == O1_KV_UINT4 ? 64 : 32;
     // the stream's index and costs are ints: fewer sequences a launch where the table allows for more, and a limit of items of a sequence

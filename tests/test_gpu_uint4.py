@@ -502,3 +502,47 @@ def test_values_in_the_middle_of_their_rows(pkg, dev, kv_heads, group, batch):
     out, lse = c.cache.attend(q.to(dev), c.dtable, c.dlens, lse=True)
     c.check(q, out, lse)
     assert float(out[..., 2:].float().abs().max()) <= 7.5 * (2.0 ** -19 + 2.0 ** -20)
+
+
+# ------------------------------------------------------------------ the range of queries
+def one_row_takes_all(c, q, out, lse, scale):
+    """A score's error is 2^-19 of the sum of its terms' magnitudes: where the largest one is ahead by four times that, its row is the result and its score the log-sum-exp."""
+    ref, ref_l, _, tol_l = c.reference(q, scale)
+    n = c.lens[0]
+    (k, ka), (v, va) = ([f(*kept(x[0])).repeat_interleave(q.size(1) // c.hk, 1) for f in (value, magnitude)] for x in (c.k, c.v))
+    z = torch.einsum("hd,thd->ht", q[0].double(), k)
+    size = torch.einsum("hd,thd->ht", q[0].double().abs(), ka).amax(-1)
+    top = z.topk(2).values
+    sure = top[:, 0] - top[:, 1] > 4 * 2.0 ** -19 * size
+    assert sure.sum() > len(sure) // 2 and n > 1
+    heads, rows = torch.arange(len(sure))[sure], z.argmax(-1)[sure]
+    between(out[0, heads], v[rows, heads], 2.0 ** -17 * va[rows, heads], "out")
+    assert ((lse.cpu().double() - ref_l).abs() <= tol_l)[0].all()
+
+
+@gpu
+@pytest.mark.parametrize("scale,top", [(None, 121), (None, 123), (None, 124), (1.0, 120), (1.0, 121), (2.0 ** 40, 81), (2.0 ** 70, 51), (2.0 ** 114, 7), (2.0 ** -60, 120), (2.0 ** -100, 100)])
+@pytest.mark.parametrize("lens,kv_heads,group", [([300], 2, 4), ([300], 1, 8), ([300] * 60, 8, 2)])
+def test_queries_up_to_the_limit(pkg, dev, lens, kv_heads, group, scale, top):
+    """scale times the largest query up to 2^121: one row takes all (with the smaller scales some do), and nothing on the way leaves fp32."""
+    c = Case4(pkg, dev, "uint4", lens, kv_heads, 32, seed=11)
+    if scale is not None and scale > 2.0 ** 100:
+        c.k = [(x.float() * 2.0 ** -20).to(torch.bfloat16) for x in c.k]         # (scores of fp32's range)
+    c.fill()
+    q = normal((len(lens), kv_heads * group, D), gen(3))
+    q = (q.float() / q.float().abs().amax(-1, keepdim=True) * 2.0 ** top).to(torch.bfloat16)
+    assert float(q.float().abs().max()) == 2.0 ** top
+    out, lse = c.cache.attend(q.to(dev), c.dtable, c.dlens, lse=True, scale=scale)
+    c.check(q, out, lse, scale=scale)
+    if (scale or D ** -0.5) * 2.0 ** top > 2.0 ** 30:
+        one_row_takes_all(c, q, out, lse, scale)
+
+
+def test_scales_beyond_the_limit_are_refused(pkg):
+    one = C.c_void_p(4096)
+    good = dict(k=4096, v=4096, k_scale=4096, v_scale=4096, type=4, pages=4, page_size=16, kv_heads=2, head_dim=128)
+    for scale in (2.0 ** 114.5, 3.0e38, math.inf, math.nan, 0.0, -1.0):
+        k = pkg.KvCacheC(**good)
+        assert pkg.lib.o1_kv_attention(C.byref(k), one, 256, None, 0, None, 0, one, 4, 4, one, one, 256, None, 1, 2, scale, one, 1 << 30) == 9, scale
+        assert b"scale" in pkg.lib.hd_cuda_last_error()
+    pkg.lib.hd_cuda_clear_error()
