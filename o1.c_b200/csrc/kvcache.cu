@@ -745,12 +745,12 @@ struct KvFour {
 
     __device__ __forceinline__ void begin(uint32_t (&q)[16], float scale, float (&acc)[8][4]) {
         const int t = threadIdx.x & 3;
-        // (sums: a product with ones, which gives them where this thread wants them)
+        // (sums: a product with 2^-8, which gives them where this thread wants them; 128 of the largest queries are 2^135, with this 2^127)
         uint32_t top = 0;
         float sum[4];
-        mma_bf16_new(sum, 0x3F803F80u, 0, 0x3F803F80u, 0, q[0], q[1]);
+        mma_bf16_new(sum, 0x3B803B80u, 0, 0x3B803B80u, 0, q[0], q[1]);
 #pragma unroll
-        for (int i = 2; i < 16; i += 2) mma_bf16(sum, 0x3F803F80u, 0, 0x3F803F80u, 0, q[i], q[i + 1]);
+        for (int i = 2; i < 16; i += 2) mma_bf16(sum, 0x3B803B80u, 0, 0x3B803B80u, 0, q[i], q[i + 1]);
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = max_u16x2(top, q[i] & 0x7FFF7FFFu);
         top = max(top & 0xFFFFu, top >> 16);
@@ -768,7 +768,7 @@ struct KvFour {
             (c ? zs.y : zs.x) = __shfl_sync(0xffffffffu, z, 8 * t + 4 * c);
             // (the shuffled exponent: x of that head)
             const int x_of = __shfl_sync(0xffffffffu, x, 8 * t + 4 * c);
-            (c ? q_sum.y : q_sum.x) = sum[c] * __uint_as_float((uint32_t)(127 + x_of - 70) << 23) * __uint_as_float((uint32_t)(127 - 63) << 23);
+            (c ? q_sum.y : q_sum.x) = sum[c] * __uint_as_float((uint32_t)(127 + x_of - 62) << 23) * __uint_as_float((uint32_t)(127 - 63) << 23);
             m[c] = -INFINITY;
             l = offset = both(0.f);
             most[c] = 0.f;

@@ -546,3 +546,25 @@ def test_scales_beyond_the_limit_are_refused(pkg):
         assert pkg.lib.o1_kv_attention(C.byref(k), one, 256, None, 0, None, 0, one, 4, 4, one, one, 256, None, 1, 2, scale, one, 1 << 30) == 9, scale
         assert b"scale" in pkg.lib.hd_cuda_last_error()
     pkg.lib.hd_cuda_clear_error()
+
+
+@gpu
+@pytest.mark.parametrize("spread", [False, True])
+@pytest.mark.parametrize("top,scale", [(124, None), (121, 1.0), (123, 2.0 ** -20), (127, 2.0 ** -6), (127, 2.0 ** -30), (60, None), (-60, None), (-110, None)])
+@pytest.mark.parametrize("lens,kv_heads,group", [([300, 41], 2, 4), ([300, 64], 1, 8), ([100] * 60, 8, 2)])
+def test_queries_of_one_sign(pkg, dev, lens, kv_heads, group, scale, top, spread):
+    """A head's queries of one sign, whose sum is up to 128 times the largest of them, and keys as small (or as large) as they are large, so that scores are ordinary: rows of one value, of which the
+    sum alone makes the scores, and with a value of another size in one column."""
+    c = Case4(pkg, dev, "uint4", lens, kv_heads, 32, seed=12)
+    for b, x in enumerate(c.k):
+        one = x.float()[..., :1].expand(x.shape).clone()
+        if spread:
+            one[..., 5] = one[..., 5] * 3 + 40
+        c.k[b] = (one * 2.0 ** -top * 0.05 / (scale or D ** -0.5)).to(torch.bfloat16)
+    c.fill()
+    q = normal((len(lens), kv_heads * group, D), gen(3)).float().abs().clamp(0.5, 2.0) * 2.0 ** (top - 1)
+    q[:, ::2] *= -1
+    q = q.to(torch.bfloat16)
+    assert torch.isfinite(q.float()).all() and float(q.float().abs().max()) == 2.0 ** top
+    out, lse = c.cache.attend(q.to(dev), c.dtable, c.dlens, lse=True, scale=scale)
+    c.check(q, out, lse, scale=scale)
