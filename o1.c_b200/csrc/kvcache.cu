@@ -1619,6 +1619,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         bool last = lane < 2 && here > 0 && all_came(a.arrived + mine_shared[lane].first, here);
 #pragma unroll 1
         for (int level = 0; level < 2; ++level) {
+            __syncwarp();          // what these two lanes have seen come, the others read (a vote alone orders no memory)
             const unsigned now = __ballot_sync(0xffffffffu, last);
             if (!now) break;
 #pragma unroll 1

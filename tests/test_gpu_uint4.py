@@ -568,3 +568,20 @@ def test_queries_of_one_sign(pkg, dev, lens, kv_heads, group, scale, top, spread
     assert torch.isfinite(q.float()).all() and float(q.float().abs().max()) == 2.0 ** top
     out, lse = c.cache.attend(q.to(dev), c.dtable, c.dlens, lse=True, scale=scale)
     c.check(q, out, lse, scale=scale)
+
+
+@gpu
+def test_parts_of_warps_are_joined_when_all_have_come(pkg, dev):
+    """One item in more than a thousand warps' parts (two levels of joins) among others of two and more, many times over and launch upon launch: the same bits each time, with nothing left of the
+    launch before, whose queries are others."""
+    lens = [1] * 120 + [100000] + [700 + 3 * i for i in range(120)]
+    c = Case4(pkg, dev, "uint4", lens, 2, 32, seed=14)
+    c.fill()
+    qs = [normal((len(lens), 8, D), gen(i), 1.5) for i in (1, 2)]
+    on_gpu = [q.to(dev) for q in qs]
+    first = [c.cache.attend(q, c.dtable, c.dlens, lse=True) for q in on_gpu]
+    c.check(qs[0], *first[0])
+    again = [[c.cache.attend(q, c.dtable, c.dlens, lse=True) for q in on_gpu] for _ in range(60)]
+    for pair in again:
+        for got, want in zip(pair, first):
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
