@@ -136,7 +136,7 @@ PyObject* py_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!arguments(n, 4)) return nullptr;
     Handle* h = handle(a[0]);
     const at::Tensor *k = tensor(a[1], who), *v = k ? tensor(a[2], who) : nullptr, *slots = v ? tensor(a[3], who) : nullptr;
-    if (!h || !slots || (h->cache->type == O1_KV_UINT4 && !current(h->device, who))) return nullptr;
+    if (!h || !slots || !current(h->device, who)) return nullptr;
     int64_t ldk, ldv;
     const int64_t rows = slots_of(*slots, h, who);
     if (rows < 0 || !rows_ok(*k, rows, h->heads, h->device, ldk, "KvCache.write: k") || !rows_ok(*v, rows, h->heads, h->device, ldv, "KvCache.write: v")) return nullptr;
@@ -152,7 +152,7 @@ PyObject* py_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!arguments(n, 4)) return nullptr;
     Handle* h = handle(a[0]);
     const at::Tensor* slots = tensor(a[1], who);
-    if (!h || !slots || (h->cache->type == O1_KV_UINT4 && !current(h->device, who))) return nullptr;
+    if (!h || !slots || !current(h->device, who)) return nullptr;
     const int64_t rows = slots_of(*slots, h, who);
     if (rows < 0) return nullptr;
     const OnLibrary on(h->device);
@@ -182,7 +182,7 @@ PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!arguments(n, 10)) return nullptr;
     Handle* h = handle(a[0]);
     const at::Tensor *q = tensor(a[2], who), *pages = q ? tensor(a[3], who) : nullptr, *lens = pages ? tensor(a[4], who) : nullptr;
-    if (!h || !lens || (h->cache->type == O1_KV_UINT4 && !current(h->device, who))) return nullptr;
+    if (!h || !lens || !current(h->device, who)) return nullptr;
     if (q->dim() != 3) return fail(who, "q [batch, heads, 128] wanted");
     const int64_t batch = q->size(0), heads = q->size(1);
     int64_t ldq, ldk = 0, ldv = 0, ldo;
@@ -277,6 +277,7 @@ PyObject* py_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!branch) return nullptr;
     if (x->dim() != 2 || branch->dim() != 2 || !x->is_cuda()) return fail(who, "x and branch bf16 [rows, cols] on the GPU wanted");
     const int device = x->device().index();
+    if (!current(device, who)) return nullptr;
     const int64_t rows = x->size(0), cols = x->size(1);
     if (rows > INT32_MAX || cols > INT32_MAX) return fail(who, "too many rows or columns");
     auto like_x = [&](const at::Tensor& t) { return t.dim() == 2 && bf16_on(t, device) && t.size(0) == rows && t.size(1) == cols; };

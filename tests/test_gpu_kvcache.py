@@ -799,3 +799,35 @@ def test_probabilities_keep_sixteen_bits(pkg, dev, kind, lens, kv_heads, group):
     c.k, c.v = ([value(*quantised(x, kind)) for x in rows] for rows in (c.k, c.v))
     c.kind = "bf16"
     c.check(q, out, lse, what=kind)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "int8", "uint4"])
+def test_memory_of_another_gpu_is_refused(pkg, dev, kind):
+    c = pkg.KvCache(4, 16, kind, 2, dev)
+    x, s = normal((3, 2, D), gen(0)).to(dev), torch.arange(3, device=dev)
+    c.write(x, x, s)
+    want = c.read(s)
+    table, lens = torch.zeros(3, 1, dtype=torch.int32, device=dev), torch.tensor([1, 2, 3], dtype=torch.int32, device=dev)
+    real, c._h = c._h, pkg.kvcache._binding.handle(C.addressof(c.c), 2, dev.index + 1)           # (as if its memory were there)
+    for call in (lambda: c.write(x, x, s), lambda: c.read(s), lambda: c.attend(x, table, lens)):
+        with pytest.raises(pkg.O1Error, match="another GPU than the current one"):
+            call()
+    c._h = real
+    assert all(torch.equal(a, b) for a, b in zip(c.read(s), want))
+    pkg.check_cuda_errbuf("after refusals")
+
+
+@gpu
+def test_memory_of_another_gpu_among_two_is_refused(pkg, dev):
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one GPU")
+    c, x, s = pkg.KvCache(4, 16, "bf16", 2, dev), normal((3, 2, D), gen(0)).to(dev), torch.arange(3, device=dev)
+    rows = x.flatten(1)
+    try:
+        torch.cuda.set_device(1)
+        for call in (lambda: c.write(x, x, s), lambda: c.read(s), lambda: pkg.residual_norm(rows, rows, None)):
+            with pytest.raises(pkg.O1Error, match="another GPU than the current one"):
+                call()
+    finally:
+        torch.cuda.set_device(dev)
