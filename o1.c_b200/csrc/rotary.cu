@@ -5,11 +5,11 @@
 // fp32 products, which at position 10^6 are 0.03 radians off.
 //
 // Angles: a frequency is kept in turns a position, as the 64-bit fraction of a turn.  position * frequency mod 1 is then one 64-bit product whose overflow is the whole turns: exact to
-// position * 2^-65 turns however far out.  Its upper bits are reduced to an eighth of a turn around the nearest quarter (integers), and the Taylor polynomials of sine and
-// cosine to the 9th and 8th power, whose rest is below 2.5e-8 there, do what remains.
+// position * 2^-65 turns however far out.  It is reduced to an eighth of a turn around the nearest quarter with all its bits (integers; cut to 32 of them first, the sine of a slow pair's
+// first positions was 3 % off), rounded to fp32 once, and the Taylor polynomials of sine and cosine to the 9th and 8th power, whose rest is below 2.5e-8 there, do what remains.
 //
-// HBM bound: values in, values out; 341 MB (16640 rows of 32 + 8 heads of bf16) in 53.9 us, 6.3 TB/s, 97 % of a copy's rate; 84 MB (4111 rows of 16 + 4 heads of fp32, half of each head
-// turned) in 14.2.  A thread has one 16-byte piece of a head and its partner, of several heads: all its loads are under way while it finds the piece's angles, once for all heads.
+// HBM bound: values in, values out; 341 MB (16640 rows of 32 + 8 heads of bf16) in 52.8 us, 6.45 TB/s, 99 % of a copy's rate (neighbours as pairs 54.4); 84 MB (4111 rows of 16 + 4 heads of
+// fp32, half of each head turned) in 14.7.  A thread has one 16-byte piece of a head and its partner, of several heads: all its loads are under way while it finds the piece's angles, once for all heads.
 #include "common.cuh"
 #include "kernels.h"
 #include "../../include/o1_b200.h"
@@ -21,7 +21,7 @@ namespace o1 {
 
 // From so many (row, unit, head) triples for an SM on a thread has several heads' units, whose loads are under way while it finds their angles: four of bf16, two of fp32.
 // 16640 rows of 40 heads of bf16: one 66 us, two 63, four 53.8, five 52.9, eight 55.7; 4111 rows of 20 heads of fp32: one 16.8, two 14.2, four 14.7.  With few rows more threads
-// count: 1500 rows of 40 heads 9.5 us with one head to a thread, 5.3 with four; 700 rows 5.6 and 5.0, both the call's own time.
+// count: 1500 rows of 40 heads 9.5 us with one head to a thread, 5.3 with four; 700 rows 5.6 and 5.0, both the call's own time.  (With angles of 32 bits and without the bound on registers.)
 static constexpr int ROPE_FEW = 1000;
 struct RopeSide { const void* x; void* y; int64_t ldx, ldy; int heads; };
 struct RopeArgs {
@@ -32,17 +32,19 @@ struct RopeArgs {
     int rows, head_dim, rot, heads, slots, units, rows_a_block, wide_positions, inverse;      // units: pieces of a head; slots: threads of a row
 };
 
-__device__ __forceinline__ void rope_angle(uint64_t turns, int64_t position, float factor, float& c, float& s) {
-    const int t = (int)(uint32_t)((turns * (uint64_t)position) >> 32);
-    const unsigned quarter = ((unsigned)t + 0x20000000u) >> 30;
-    const float a = (float)(int)((unsigned)t - (quarter << 30)) * 1.4629180792671596e-9f;       // 2 pi / 2^32
+// Cosine and sine times their factors, of which the sine's has the sign of the direction.
+__device__ __forceinline__ void rope_angle(uint64_t turns, int64_t position, float factor, float factor_s, float& c, float& s) {
+    const uint64_t t = turns * (uint64_t)position;
+    const unsigned hi = (unsigned)(t >> 32), quarter = (hi + 0x20000000u) >> 30;
+    // 2 pi / 2^64 and / 2^32 (two conversions of 32 bits; one of 64 takes as long, and more registers)
+    const float a = __fmaf_rn((float)(uint32_t)t, 3.4061215800865545e-19f, (float)(int)(hi - (quarter << 30)) * 1.4629180792671596e-9f);
     const float a2 = a * a;
-    float sn = a * __fmaf_rn(a2, __fmaf_rn(a2, __fmaf_rn(a2, __fmaf_rn(a2, 2.7557319e-6f, -1.9841270e-4f), 8.3333333e-3f), -0.16666667f), 1.0f);
-    float cs = __fmaf_rn(a2, __fmaf_rn(a2, __fmaf_rn(a2, __fmaf_rn(a2, 2.4801587e-5f, -1.3888889e-3f), 4.1666668e-2f), -0.5f), 1.0f);
-    if (quarter & 1) { const float x = sn; sn = cs; cs = -x; }
-    if (quarter & 2) { sn = -sn; cs = -cs; }
-    c = cs * factor;
-    s = sn * factor;
+    const float sn = a * __fmaf_rn(a2, __fmaf_rn(a2, __fmaf_rn(a2, __fmaf_rn(a2, 2.7557319e-6f, -1.9841270e-4f), 8.3333333e-3f), -0.16666667f), 1.0f);
+    const float cs = __fmaf_rn(a2, __fmaf_rn(a2, __fmaf_rn(a2, __fmaf_rn(a2, 2.4801587e-5f, -1.3888889e-3f), 4.1666668e-2f), -0.5f), 1.0f);
+    const unsigned half = (quarter << 30) & 0x80000000u;         // half a turn on: both signs
+    const bool odd = quarter & 1;
+    c = (odd ? -sn : cs) * __uint_as_float(__float_as_uint(factor) ^ half);
+    s = (odd ? cs : sn) * __uint_as_float(__float_as_uint(factor_s) ^ half);
 }
 
 // The piece p of V values of T at an address.
@@ -86,9 +88,10 @@ struct Piece<float, 1> {
 };
 
 // V values to a piece.  A unit is two pieces whose values pair up: V values and those half a rotation on (HALF), or 2 V neighbours; behind the turned ones, two pieces as they are.
-// A thread has one unit of N heads.
+// A thread has one unit of N heads.  Registers are bounded so that four blocks (fp32: six) share an SM, where values are under way for long: 16640 rows of 40 heads of bf16 54.5 us without,
+// 52.8 with, 4111 of 20 of fp32 15.3 and 14.7.
 template <class T, int V, bool HALF, int N>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, V * sizeof(T) == 16 && N > 1 ? (sizeof(T) == 2 ? 4 : 6) : 0)
 rotary_kernel(const RopeArgs a) {
     grid_dep_launch();
     const int local = threadIdx.x / a.slots;                                   // (slots <= 256: rows side by side in a block; else a row's slots over blockIdx.y)
@@ -125,8 +128,7 @@ rotary_kernel(const RopeArgs a) {
         float c[V], s[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            rope_angle(a.turns[unit * V + i], position, a.factor, c[i], s[i]);
-            if (a.inverse) s[i] = -s[i];
+            rope_angle(a.turns[unit * V + i], position, a.factor, a.inverse ? -a.factor : a.factor, c[i], s[i]);
         }
 #pragma unroll
         for (int k = 0; k < N; ++k) {

@@ -209,7 +209,7 @@ class KvPages:
 
 class Rotary:
     """Rotary positions: the first rot_dim values of each head turned in pairs, "half" (i, i + rot_dim / 2) or "interleaved" (2i, 2i + 1), by position *
-    theta^(-2i / rot_dim).  Angles are exact at any position (turns as 64-bit fractions).
+    theta^(-2i / rot_dim).  Angles are exact to position * 2^-65 turns (64-bit fractions of a turn), then rounded to fp32 once reduced.
 
     scaling, for contexts longer than the model was made for: {"kind": "linear", "factor": f}, {"kind": "ntk", "factor": f}, {"kind": "yarn", "factor": f, "original":
     rows, "fast": 32, "slow": 1}, or {"kind": "factors", "factors": [rot_dim / 2 divisors]}; with "attention": what results are multiplied by."""

@@ -274,3 +274,29 @@ def test_arguments_that_do_not_fit(pkg, dev):
         rope(x, pos, out=x[:, :1])
     assert rope(x[:0], pos[:0]).shape == (0, 2, 128) and rope(x[:, :0], pos).shape == (3, 0, 128)
     pkg.check_cuda_errbuf("after refusals")
+
+
+@gpu
+@pytest.mark.parametrize("theta,scaling", [(THETA, {"kind": "linear", "factor": 8.0}), (THETA, {"kind": "yarn", "factor": 32.0, "original": 16640.0}), (1.0e9, None), (10000.0, None)])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_sines_keep_their_bits(pkg, dev, theta, scaling, layout):
+    """Pairs (1, 0) and (0, 1) in fp32 give sines and cosines themselves, small ones too: within 2^-21 of their own size (an angle's rounding to fp32, a constant's, a product's, a sum's, two of the
+    polynomial's, one with the factor: seven of 2^-24, and the polynomials' rest, 2.5e-8)."""
+    rot = 128
+    rope = pkg.Rotary(rot, rot, theta, layout, scaling, dev)
+    positions = [0, 1, 2, 3, 5, 17, 100, 1000, 16640, 999983, -1, -3, 2 ** 31 - 1, -2 ** 31, 2 ** 45 + 1, -2 ** 62 + 3]
+    first = torch.arange(rot // 2) * (1 if layout == "half" else 2)
+    second = first + (rot // 2 if layout == "half" else 1)
+    x = torch.zeros(len(positions), 2, rot)
+    x[:, 0, first], x[:, 1, second] = 1.0, 1.0
+    got = rope(x.to(dev), torch.tensor(positions, device=dev)).cpu().double()
+    sin, cos = (torch.zeros(len(positions), rot // 2, dtype=torch.float64) for _ in range(2))
+    for i, p in enumerate(positions):
+        for j, t in enumerate(rope.turns.tolist()):
+            t = p * (t % 2 ** 64) % 2 ** 64
+            quarter = (t + 2 ** 61) // 2 ** 62
+            a = (t - quarter * 2 ** 62) * (math.pi / 2 ** 63)
+            s, c = ((math.sin(a), math.cos(a)), (math.cos(a), -math.sin(a)), (-math.sin(a), -math.cos(a)), (-math.cos(a), math.sin(a)))[quarter % 4]
+            sin[i, j], cos[i, j] = s * rope.factor, c * rope.factor
+    for g, want in ((got[:, 0, first], cos), (got[:, 0, second], sin), (got[:, 1, first], -sin), (got[:, 1, second], cos)):
+        assert ((g - want).abs() <= 2.0 ** -21 * want.abs()).all(), ((g - want).abs() / want.abs().clamp_min(1e-300)).max()
