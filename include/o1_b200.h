@@ -791,13 +791,15 @@ hd_status o1_kv_read(const o1_kv_cache *cache, void *k, int64_t ldk, void *v, in
  * columns, heads a multiple of kv_heads (query head j reads kv head j / (heads / kv_heads)); lse (may be NULL) [batch, heads] fp32:
  * log of the sum of exponentials, to join the result with that of other keys.  lens[b] == 0: out row 0, lse -inf.
  * k_new / v_new (both or neither): each sequence's row at position lens[b] - 1, stored into the cache (as by o1_kv_write) and
- * attended to by the same call; no other sequence of the call has that slot among its rows.  workspace: o1_kv_attention_workspace_bytes(heads, kv_heads) bytes, 16-byte aligned, its first
+ * attended to by the same call; no other sequence of the call has that slot among its rows.  workspace: o1_kv_attention_workspace_bytes(heads, kv_heads) bytes for any kind of cache, or
+ * o1_kv_attention_workspace_bytes_of(cache->type, heads, kv_heads), which is more with O1_KV_UINT4 and makes calls of many sequences faster there; 16-byte aligned, its first
  * O1_KV_ATTENTION_COUNTERS bytes zero-filled once before its first use and all of it left to these calls from then on; calls that may overlap on the GPU each need their own.  The result is the same
- * bits from call to call with the same lengths and width; beside other sequences a sequence's differs by the order of its fp32 sums.  Values of v up to 2^90 in magnitude (the sums are 2^20 times larger and in fp32);
+ * bits from call to call with the same lengths, width and (O1_KV_UINT4) room in the workspace; beside other sequences a sequence's differs by the order of its fp32 sums.  Values of v up to 2^90 in magnitude (the sums are 2^20 times larger and in fp32);
  * with O1_KV_UINT4 scale at most 2^114 and scale times the largest |q| of a head at most 2^121; at most 2^31 - 1 rows (pages *
  * kv_heads * page_size) in the cache. */
 #define O1_KV_ATTENTION_COUNTERS 32768
 int64_t o1_kv_attention_workspace_bytes(int heads, int kv_heads);
+int64_t o1_kv_attention_workspace_bytes_of(int type, int heads, int kv_heads);
 hd_status o1_kv_attention(const o1_kv_cache *cache, const void *q, int64_t ldq, const void *k_new, int64_t ldk,
                           const void *v_new, int64_t ldv, const int32_t *pages, int64_t ldp, int width, const int32_t *lens,
                           void *out, int64_t ldo, float *lse, int batch, int heads, float scale, void *workspace,
@@ -860,11 +862,13 @@ hd_status o1_residual_norm(const void *x, int64_t ldx, const void *branch, int64
 /* The decoder blocks on cached rows: caches [n_layers] (one of each block, with the same pages and page_size, so that one page table serves
  * all), ids int64 on the device, pos_f32 [3, rows] as hd_forward's, out [rows, hidden] bf16: the rows behind the final norm.
  * o1_prompt_rows: all rows of one sequence, causal, their keys and values into slots[r] of each cache.  o1_decode_step: one new row of each of `batch` sequences, which
- * becomes row lens[b] - 1 of sequence b.  scratch: o1_decode_scratch_bytes(rows, ...) bytes, zero-filled once; one for each
+ * becomes row lens[b] - 1 of sequence b.  scratch: o1_decode_scratch_bytes(rows, ...) bytes for any kind of caches, or o1_decode_scratch_bytes_of(type, rows, ...), which is more with
+ * O1_KV_UINT4 and makes steps of many sequences faster there; zero-filled once, one for each
  * stream.  The residual stream's norms are of its unrounded sums (o1_residual_norm), so the rows agree with hd_decoder_block's within rounding.  A row is a
  * function of its own sequence within rounding too: the same step gives the same bits, but how a sequence's cached rows are shared out, and with it the order of fp32
  * sums, follows from the lengths of all sequences of the step. */
 int64_t o1_decode_scratch_bytes(int64_t rows, int heads, int kv_heads, int hidden, int ff_hidden, int head_dim);
+int64_t o1_decode_scratch_bytes_of(int type, int64_t rows, int heads, int kv_heads, int hidden, int ff_hidden, int head_dim);
 hd_status o1_prompt_rows(const hd_forward_binding *bw, const o1_kv_cache *caches, const int64_t *ids, const float *pos_f32,
                          const int64_t *slots, void *scratch, int64_t scratch_bytes, void *out, int rows, int heads,
                          int kv_heads, int hidden, int ff_hidden, int head_dim, int vocab);

@@ -306,6 +306,7 @@ _sig("o1_denoise_step_cfg_host", c_int, C.POINTER(ForwardBinding), C.POINTER(For
 
 _sig("o1_kv_write", c_int, C.POINTER(KvCacheC), _P, c_int64, _P, c_int64, _P, c_int)
 _sig("o1_kv_read", c_int, C.POINTER(KvCacheC), _P, c_int64, _P, c_int64, _P, c_int)
+_sig("o1_kv_attention_workspace_bytes_of", c_int64, c_int, c_int, c_int)
 _sig("o1_kv_attention_workspace_bytes", c_int64, c_int, c_int)
 _sig("o1_kv_attention", c_int, C.POINTER(KvCacheC), _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, c_int, _P, _P,
      c_int64, _P, c_int, c_int, c_float, _P, c_int64)
@@ -318,6 +319,7 @@ _sig("o1_kv_pages_shrink", c_int, C.POINTER(KvPagesC), _P, _P, c_int)
 _sig("o1_rope_turns", c_int, C.c_double, c_int, C.POINTER(RopeScalingC), C.POINTER(c_uint64), C.POINTER(c_float))
 _sig("o1_rotary", c_int, C.POINTER(RopeC), _P, c_int, _P, c_int64, _P, c_int64, c_int, _P, c_int64, _P, c_int64, c_int, c_int, c_int, c_int)
 
+_sig("o1_decode_scratch_bytes_of", c_int64, c_int, c_int64, c_int, c_int, c_int, c_int, c_int)
 _sig("o1_decode_scratch_bytes", c_int64, c_int64, c_int, c_int, c_int, c_int, c_int)
 _sig("o1_prompt_rows", c_int, C.POINTER(ForwardBinding), C.POINTER(KvCacheC), _P, _P, _P, _P, c_int64, _P, c_int, c_int, c_int,
      c_int, c_int, c_int, c_int)

@@ -25,12 +25,12 @@ struct Scratch {
     void* attention;
     int64_t attention_bytes, bytes;
 };
-Scratch carve(void* base, int64_t rows, int heads, int kv_heads, int hidden, int ff, int hd) {
+Scratch carve(void* base, int type, int64_t rows, int heads, int kv_heads, int hidden, int ff, int hd) {
     Scratch s = {};
     uint8_t* p = (uint8_t*)base;
     auto take = [&](int64_t n) { uint8_t* at = p; p += (n + 255) & ~(int64_t)255; return at; };
     rows = rows < MIN_ROWS ? MIN_ROWS : rows;
-    s.attention_bytes = o1_kv_attention_workspace_bytes(heads, kv_heads);
+    s.attention_bytes = o1_kv_attention_workspace_bytes_of(type, heads, kv_heads);
     s.attention = take(s.attention_bytes);       // first: the part that stays between calls
     s.x = (uint16_t*)take(rows * hidden * 2);
     s.ln = (uint16_t*)take(rows * hidden * 2);
@@ -93,9 +93,12 @@ hd_status run(const hd_forward_binding* bw, const Scratch& s, const int64_t* ids
 
 extern "C" {
 
+int64_t o1_decode_scratch_bytes_of(int type, int64_t rows, int heads, int kv_heads, int hidden, int ff_hidden, int head_dim) {
+    if (rows < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || hidden <= 0 || ff_hidden <= 0 || head_dim <= 0 || o1_kv_attention_workspace_bytes_of(type, heads, kv_heads) < 0) return -1;
+    return carve(nullptr, type, rows, heads, kv_heads, hidden, ff_hidden, head_dim).bytes + 256;
+}
 int64_t o1_decode_scratch_bytes(int64_t rows, int heads, int kv_heads, int hidden, int ff_hidden, int head_dim) {
-    if (rows < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || hidden <= 0 || ff_hidden <= 0 || head_dim <= 0) return -1;
-    return carve(nullptr, rows, heads, kv_heads, hidden, ff_hidden, head_dim).bytes + 256;
+    return o1_decode_scratch_bytes_of(O1_KV_BF16, rows, heads, kv_heads, hidden, ff_hidden, head_dim);
 }
 
 hd_status o1_prompt_rows(const hd_forward_binding* bw, const o1_kv_cache* caches, const int64_t* ids, const float* pos_f32, const int64_t* slots, void* scratch,
@@ -104,7 +107,7 @@ hd_status o1_prompt_rows(const hd_forward_binding* bw, const o1_kv_cache* caches
     if (st != HD_OK || rows == 0) return st;
     if (!ids || !pos_f32 || !slots || !scratch || !out) { hd_set_error("decode: null argument"); return HD_ERR_MISSING; }
     if (scratch_bytes < o1_decode_scratch_bytes(rows, heads, kv_heads, hidden, ff_hidden, head_dim)) { hd_set_error("decode: scratch too small"); return HD_ERR_OOM; }
-    const Scratch s = carve((void*)(((uintptr_t)scratch + 255) & ~(uintptr_t)255), rows, heads, kv_heads, hidden, ff_hidden, head_dim);
+    const Scratch s = carve((void*)(((uintptr_t)scratch + 255) & ~(uintptr_t)255), O1_KV_BF16, rows, heads, kv_heads, hidden, ff_hidden, head_dim);
     DEC_TRY(mrope_table64_rows(pos_f32, rows, 0, rows, 5000000.0f, s.cs, current_stream()), "rotary table");
     const int qc = heads * head_dim, kc = kv_heads * head_dim, ld = qc + 2 * kc;
     const float scale = (float)(1.0 / sqrt((double)head_dim));
@@ -126,7 +129,8 @@ hd_status o1_decode_step(const hd_forward_binding* bw, const o1_kv_cache* caches
     if (st != HD_OK || batch == 0) return st;
     if (!ids || !pos_f32 || !pages || !lens || !scratch || !out) { hd_set_error("decode: null argument"); return HD_ERR_MISSING; }
     if (scratch_bytes < o1_decode_scratch_bytes(batch, heads, kv_heads, hidden, ff_hidden, head_dim)) { hd_set_error("decode: scratch too small"); return HD_ERR_OOM; }
-    const Scratch s = carve((void*)(((uintptr_t)scratch + 255) & ~(uintptr_t)255), batch, heads, kv_heads, hidden, ff_hidden, head_dim);
+    const int room = scratch_bytes < o1_decode_scratch_bytes_of(O1_KV_UINT4, batch, heads, kv_heads, hidden, ff_hidden, head_dim) ? O1_KV_BF16 : O1_KV_UINT4;
+    const Scratch s = carve((void*)(((uintptr_t)scratch + 255) & ~(uintptr_t)255), room, batch, heads, kv_heads, hidden, ff_hidden, head_dim);
     DEC_TRY(mrope_table64_rows(pos_f32, batch, 0, batch, 5000000.0f, s.cs, current_stream()), "rotary table");
     const int qc = heads * head_dim, kc = kv_heads * head_dim, ld = qc + 2 * kc;
     const float scale = (float)(1.0 / sqrt((double)head_dim));

@@ -1673,14 +1673,14 @@ static cudaError_t launch_attention(const CUtensorMap& k_map, const CUtensorMap&
     return launch_chained(kv_attention_kernel<TYPE, HG, SOLO>, dim3((unsigned)blocks), dim3(K::THREADS), K::SMEM, st, 1, 1, k_map, v_map, a);
 }
 template <int TYPE, int HG>
-static cudaError_t launch_attention(const CUtensorMap& k_map, const CUtensorMap& v_map, const KvAttn& a, int64_t item_chunks, int64_t items, cudaStream_t st) {
+static cudaError_t launch_attention(const CUtensorMap& k_map, const CUtensorMap& v_map, const KvAttn& a, int64_t item_chunks, int64_t items, cudaStream_t st, bool warps = true) {
     const int most = min(sm_count(), KV_TEAMS_MAX / KvKernel<TYPE, HG>::TEAMS), teams = most * KvKernel<TYPE, HG>::TEAMS;
-    // Four bits: parts to warps, which need no barriers but leave more of an item to be joined at the end, where there is much work for each and items are not few, or items are
+    // Four bits: parts to warps (where the workspace has room for them), which need no barriers but leave more of an item to be joined at the end, where there is much work for each and items are not few, or items are
     // short and many.  us, to warps and to teams (444 of them): 8 kv heads, 96 sequences of 300 to 5400 rows 62.9 and 65.9, 37 of up to 1999 19.5 and 20.9, 128 of up to 1000
     // 27.3 and 33.7, 64 of 100 9.4 and 13.5, 128 of 60 8.3 and 19.5; but one of 100003 34.6 and 31.5, 16 of 2000 19.6 and 18.2, 32 of 200 13.2 and 9.3, 60 of up to 400 20.2 and 17.0.
     if (TYPE == KV_UINT4) {
         const bool much = 2 * items > teams && item_chunks * items > 16 * teams, many = items > teams && item_chunks * teams <= KV_TEAM * items;
-        if (much || many) return launch_attention<TYPE, HG, true>(k_map, v_map, a, most, st);
+        if ((much || many) && warps) return launch_attention<TYPE, HG, true>(k_map, v_map, a, most, st);
         return launch_attention<TYPE, HG, false>(k_map, v_map, a, (int)max((int64_t)1, min((int64_t)most, max((item_chunks * items + KV_TEAM - 1) / KV_TEAM, items))), st);
     }
     // A table of few tokens for more items than teams: an item to a warp, where its chunks one after the other take less than a team's items with their joins.
@@ -1779,10 +1779,17 @@ hd_status o1_kv_read(const o1_kv_cache* cache, void* k, int64_t ldk, void* v, in
     return HD_OK;
 }
 
-// Two counters and, for every head of an item, 128 values, a maximum and a sum, for each team's two parts.
+// Two counters (of as many as there are with any kind, so that kinds can share a workspace) and, for every head of an item, 128 values, a maximum and a sum, for the two parts of each team, or
+// of each warp.
+static int64_t attention_bytes(int units, int per_item) { return (int64_t)KV_UNITS_MAX * 2 * 2 * 4 + (int64_t)units * 2 * per_item * (KV_D + 2) * 4; }
 int64_t o1_kv_attention_workspace_bytes(int heads, int kv_heads) {
     if (heads <= 0 || kv_heads <= 0 || heads % kv_heads) return -1;
-    return (int64_t)KV_UNITS_MAX * 2 * (2 * 4 + min(heads / kv_heads, 16) * (KV_D + 2) * 4);
+    return attention_bytes(KV_TEAMS_MAX, min(heads / kv_heads, 16));
+}
+int64_t o1_kv_attention_workspace_bytes_of(int type, int heads, int kv_heads) {
+    const int64_t any = o1_kv_attention_workspace_bytes(heads, kv_heads);
+    if (any < 0 || (type != O1_KV_BF16 && type != O1_KV_FP8 && type != O1_KV_INT8 && type != O1_KV_UINT4)) return -1;
+    return type == O1_KV_UINT4 ? max(any, attention_bytes(KV_UNITS_MAX, min(heads / kv_heads, 8))) : any;
 }
 
 hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, const void* k_new, int64_t ldk, const void* v_new, int64_t ldv,
@@ -1812,7 +1819,8 @@ hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, 
     a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldp = ldp; a.ldo = ldo;
     a.arrived = (unsigned*)workspace;
     a.parts = (float*)(a.arrived + 4 * KV_UNITS_MAX);
-    a.stats = (float2*)(a.parts + (int64_t)2 * KV_UNITS_MAX * per_item * KV_D);
+    const bool warps = cache->type == O1_KV_UINT4 && workspace_bytes >= o1_kv_attention_workspace_bytes_of(O1_KV_UINT4, heads, c.heads);         // room for parts of warps
+    a.stats = (float2*)(a.parts + (int64_t)2 * (warps ? KV_UNITS_MAX : KV_TEAMS_MAX) * per_item * KV_D);
     a.heads = heads; a.group = group; a.chunks_of_heads = of_heads; a.per_item = per_item; a.width = width;
     a.scale = scale;
     a.err = device_error_word();
@@ -1838,7 +1846,7 @@ hd_status o1_kv_attention(const o1_kv_cache* cache, const void* q, int64_t ldq, 
         cudaError_t e;
         if (cache->type == O1_KV_BF16) e = hg == 1 ? launch_attention<KV_BF16, 1>(k_map, v_map, a, item_chunks, items, current_stream()) : launch_attention<KV_BF16, 2>(k_map, v_map, a, item_chunks, items, current_stream());
         else if (cache->type == O1_KV_FP8) e = hg == 1 ? launch_attention<KV_FP8, 1>(k_map, v_map, a, item_chunks, items, current_stream()) : launch_attention<KV_FP8, 2>(k_map, v_map, a, item_chunks, items, current_stream());
-        else if (four_bits) e = launch_attention<KV_UINT4, 1>(k_map, v_map, a, item_chunks, items, current_stream());
+        else if (four_bits) e = launch_attention<KV_UINT4, 1>(k_map, v_map, a, item_chunks, items, current_stream(), warps);
         else e = hg == 1 ? launch_attention<KV_INT8, 1>(k_map, v_map, a, item_chunks, items, current_stream()) : launch_attention<KV_INT8, 2>(k_map, v_map, a, item_chunks, items, current_stream());
         if (!launch_ok(e, "kv_attention")) return HD_ERR_RUNTIME;
         o1_launch_count_add(1);

@@ -139,7 +139,7 @@ class KvCache:
 
     def _workspace(self, heads):
         """Address and bytes of attend()'s scratch for the library's current stream."""
-        need = lib.o1_kv_attention_workspace_bytes(heads, self.kv_heads)
+        need = lib.o1_kv_attention_workspace_bytes_of(self.c.type, heads, self.kv_heads)
         _need(need >= 0, f"KvCache.attend: heads {heads} (a multiple of kv_heads {self.kv_heads})")
         capture = lib.o1_capture_id()
         w = _Workspace.get(self.device, capture, need)
@@ -275,7 +275,7 @@ class Decoder:
         """Scratch for so many rows on the current stream."""
         key = _stream()
         s = self._scratch.get(key)
-        need = lib.o1_decode_scratch_bytes(rows, *self.dims[:5])
+        need = lib.o1_decode_scratch_bytes_of(self._c[0].type, rows, *self.dims[:5])
         if s is None or s.numel() < need:
             s = self._scratch[key] = _zeros(need, self.device)
         return s

@@ -88,3 +88,32 @@ def test_a_captured_step_with_pages_of_the_gpu(pkg, dev, models, kind):  # noqa:
         assert kept[0].lens.tolist() == [plain._len[names[s]] for s in seqs]
         assert torch.equal(out, want)
     assert pkg.lib.o1_device_error() == 0
+
+
+@gpu
+def test_a_step_in_either_scratch(pkg, dev, models):  # noqa: F811
+    """o1_decode_step over rows of four bits of many sequences, in the scratch that any kind needs and in that of four bits: the rows that Decoder.step gives, within a block's tolerance of them."""
+    w, n, page, layers = models[3], 80, 16, 3
+    lens = [1 + (37 * i) % 150 for i in range(n)]
+    dec = pkg.Decoder(w, n, 160, "uint4", page)
+    names = [dec.prompt(ids_of(k, k).to(dev))[0] for k in lens]
+    for s, k in zip(names, lens):
+        dec._grow(s, k + 1)             # the new row's page
+    ids = ids_of(n, 5).to(dev)
+    tables = torch.stack([dec._table[s] for s in names])
+    at = torch.tensor(lens, dtype=torch.int32, device=dev) + 1
+    pos = (at - 1).float().expand(3, n).contiguous()
+    outs = []
+    for kind in (0, 4):
+        size = pkg.lib.o1_decode_scratch_bytes_of(kind, n, *dec.dims[:5])
+        scratch = torch.full((size + 4096,), 0xA5, dtype=torch.uint8, device=dev)
+        scratch[:32768 + 256] = 0
+        out = torch.empty(n, DIMS["hidden"], dtype=torch.bfloat16, device=dev)
+        for _ in range(2):          # (the row is written again)
+            pkg.check(pkg.lib.o1_decode_step(C.byref(w.binding), dec._c, pkg.ptr(ids), pkg.ptr(pos), pkg.ptr(tables), dec.width, dec.width, pkg.ptr(at), pkg.ptr(scratch), size, pkg.ptr(out), n,
+                                             *dec.dims), "o1_decode_step")
+        assert (scratch[size:] == 0xA5).all()
+        outs.append(out)
+    want = dec.step(names, ids)
+    assert torch.equal(outs[1], want)
+    within(outs[0], want.cpu(), 0.8 * math.sqrt(1e-2 * layers))

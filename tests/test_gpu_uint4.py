@@ -585,3 +585,50 @@ def test_parts_of_warps_are_joined_when_all_have_come(pkg, dev):
     for pair in again:
         for got, want in zip(pair, first):
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ------------------------------------------------------------------ workspaces
+def test_workspaces_by_kind(pkg):
+    """Two counters of four bytes for the two parts of 1920 warps, then 130 values for each head of the two parts of 480 teams, whatever the kind, or (four bits, at most eight heads) of the warps."""
+    lib = pkg.lib
+    for heads, kv_heads in ((1, 1), (32, 8), (16, 2), (16, 1), (32, 1), (128, 2)):
+        group = heads // kv_heads
+        plain = lib.o1_kv_attention_workspace_bytes(heads, kv_heads)
+        assert plain == 1920 * 2 * 8 + 480 * 2 * min(group, 16) * 130 * 4
+        assert [lib.o1_kv_attention_workspace_bytes_of(t, heads, kv_heads) for t in (0, 1, 2)] == [plain] * 3
+        assert lib.o1_kv_attention_workspace_bytes_of(4, heads, kv_heads) == 1920 * 2 * 8 + 1920 * 2 * min(group, 8) * 130 * 4 > plain
+    for args in ((3, 4, 2), (5, 4, 2), (-1, 4, 2), (0, 4, 3), (4, 0, 1), (4, 4, 0)):
+        assert lib.o1_kv_attention_workspace_bytes_of(*args) == -1
+    dims = (9, 32, 8, 4096, 12288, 128)
+    plain = lib.o1_decode_scratch_bytes(*dims)
+    assert plain == lib.o1_decode_scratch_bytes_of(0, *dims) == lib.o1_decode_scratch_bytes_of(2, *dims) and lib.o1_decode_scratch_bytes_of(3, *dims) == -1
+    assert lib.o1_decode_scratch_bytes_of(4, *dims) - plain == lib.o1_kv_attention_workspace_bytes_of(4, 32, 8) - lib.o1_kv_attention_workspace_bytes(32, 8)
+
+
+def attend_in(pkg, c, q, room):
+    """o1_kv_attention in a workspace that the caller has; a guard behind it."""
+    at, n = room
+    out = torch.empty_like(q)
+    pkg.check(pkg.lib.o1_kv_attention(C.byref(c.cache.c), pkg.ptr(q), q.size(1) * D, None, 0, None, 0, pkg.ptr(c.dtable), c.dtable.size(1), c.dtable.size(1), pkg.ptr(c.dlens), pkg.ptr(out),
+                                      q.size(1) * D, None, len(c.lens), q.size(1), D ** -0.5, pkg.ptr(at), n), "o1_kv_attention")
+    return out
+
+
+@gpu
+@pytest.mark.parametrize("lens,kv_heads,group,page", AMONG + [([60] * 128, 8, 4, 64), ([100000], 2, 4, 64)])
+def test_workspaces_of_either_size(pkg, dev, lens, kv_heads, group, page):
+    """With the room that any kind needs, and with that of four bits; the larger one also between calls over rows of a byte, which use the same counters.  Nothing behind them is written."""
+    c, other = Case4(pkg, dev, "uint4", lens, kv_heads, page, seed=15), Case4(pkg, dev, "int8", [900, 3, 5000], kv_heads, page, seed=16)
+    c.fill(), other.fill()
+    q, q2 = normal((len(lens), kv_heads * group, D), gen(13), 1.5), normal((3, kv_heads * group, D), gen(14))
+    want2 = other.cache.attend(q2.to(dev), other.dtable, other.dlens)
+    for size in (pkg.lib.o1_kv_attention_workspace_bytes(kv_heads * group, kv_heads), pkg.lib.o1_kv_attention_workspace_bytes_of(4, kv_heads * group, kv_heads)):
+        space = torch.full((size + 4096,), 0xA5, dtype=torch.uint8, device=dev)
+        space[:32768] = 0
+        outs = []
+        for _ in range(2):
+            outs.append(attend_in(pkg, c, q.to(dev), (space, size)))
+            assert torch.equal(attend_in(pkg, other, q2.to(dev), (space, size)), want2)
+        c.check(q, outs[0])
+        assert torch.equal(outs[0], outs[1]) and (space[size:] == 0xA5).all() and (space[:30720] == 0).all()
+    assert torch.equal(outs[0], c.cache.attend(q.to(dev), c.dtable, c.dlens))
