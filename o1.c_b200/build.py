@@ -73,7 +73,7 @@ def build(verbose=False, force=False):
             procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     binding, how = _binding()
     if binding is None:
-        sys.stderr.write(f"{os.path.basename(BINDING)} is not built ({how}): KvCache, Decoder and residual_norm are not to be had from Python\n")
+        sys.stderr.write(f"{os.path.basename(BINDING)} is not built ({how}): KvCache, KvPages, Rotary, Decoder and residual_norm are not to be had from Python\n")
     elif force or _stale(binding, [BINDING_SRC, headers[-1]]):
         for old in glob.glob(os.path.join(CSRC, "binding.*.o")):       # of another torch
             os.remove(old)

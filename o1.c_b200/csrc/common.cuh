@@ -124,10 +124,4 @@ int* device_error_word();   // per-device int set by kernels whose bounded waits
 int* device_table_word();   // per-device int beside it: what a kernel found wrong in a caller's table (slots, pages, lengths); it stops no other kernel
 int sm_count();
 
-#define O1_CUDA_OK(call, what)                                                     \
-    do {                                                                           \
-        cudaError_t e__ = (call);                                                  \
-        if (e__ != cudaSuccess) o1::set_error("%s: %s", what, cudaGetErrorString(e__)); \
-    } while (0)
-
 }  // namespace o1

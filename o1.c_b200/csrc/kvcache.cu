@@ -398,15 +398,6 @@ static constexpr int KV_ITEM_COST = 10;
 // Nor are those of a quarter of a team's part (half: 582 MB 104), and, where there are no more items than teams, of up to half more cost than a team has on average:
 // 51 sequences of 304 rows of bf16, 8 kv heads, 16.0, cut 20.6; 54 of 1000 of fp8 24.7 and 30.5; 55 of 100 to 700 of bf16 23.0 and 24.3.
 static constexpr int KV_KEEP = 16;
-#ifndef KL
-#define KL 2
-#endif
-#ifndef KK
-#define KK 2
-#endif
-#ifndef KC
-#define KC 2
-#endif
 // Four bits, parts of warps: a warp has at least so many chunks, items of so many are not cut, and an item costs so many beside its own (no barrier, no join within the block): a cost of
 // 1, 2, 4: 96 sequences of 300 to 5400 rows 62.9, 62.9, 64.7, 37 of 0 to 1999 19.8, 19.6, 21.8; kept 1, 2, 6: 62.9, 62.9, 63.4 and 19.6, 19.6, 20.5.
 static constexpr int KV4_LEAST = 2, KV4_KEEP = 2, KV4_ITEM_COST = 2;

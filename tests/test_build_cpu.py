@@ -71,3 +71,14 @@ def test_a_binding_of_another_torch_is_refused():
         else:
             raise SystemExit("imported")
         """)
+
+
+def test_every_macro_of_the_sources_is_read():
+    """A macro that a build flag could set and nothing reads would measure the same kernel under another name."""
+    import re
+    csrc = os.path.join(PKG, "csrc")
+    sources = {f: open(os.path.join(csrc, f)).read() for f in os.listdir(csrc) if f.endswith((".cu", ".cuh", ".h", ".cpp"))}
+    for f, text in sources.items():
+        for name in set(re.findall(r"^[ \t]*#[ \t]*define[ \t]+(\w+)", text, re.M)):
+            used = "\n".join(re.sub(rf"^[ \t]*#[ \t]*(define|ifndef|ifdef|undef)[ \t]+{name}\b", "", t, flags=re.M) for t in sources.values())
+            assert re.search(rf"\b{name}\b", used), f"{f}: {name}"
