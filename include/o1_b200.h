@@ -831,7 +831,7 @@ hd_status o1_kv_pages_shrink(const o1_kv_pages *pages, const int32_t *seqs, cons
  * o1_rope_turns fills them on the host, theta^(-2i / rot_dim), and gives the factor: O1_ROPE_LINEAR divides all by `factor`; O1_ROPE_NTK takes theta * factor^(rot_dim /
  * (rot_dim - 2)); O1_ROPE_YARN (the YaRN method) divides pairs that turn at most `slow` times within `original` positions, leaves those that turn `fast` times or more, with a
  * linear ramp between, and multiplies results by 0.1 ln(factor) + 1; O1_ROPE_FACTORS divides pair i by factors[i].  attention > 0: the factor of results instead.
- * o1_rotary: x [rows, ldx] with `heads` heads of head_dim side by side into y (which may be x), and x2 into y2 likewise in the same launch (heads2 0: not there; queries and
+ * o1_rotary: x [rows, ldx] with `heads` heads of head_dim side by side into y (which may be x, and shares no memory with it or x2 otherwise), and x2 into y2 likewise in the same launch (heads2 0: not there; queries and
  * keys as a rule); type O1_ROPE_BF16 or O1_ROPE_FP32; positions [rows] int32, or int64 where wide_positions, negative ones too.  inverse: turned back (also the gradient). */
 enum { O1_ROPE_HALF = 0, O1_ROPE_INTERLEAVED = 1 };
 enum { O1_ROPE_BF16 = 0, O1_ROPE_FP32 = 1 };

@@ -167,6 +167,22 @@ static void (*rotary_of(bool half))(const RopeArgs) { return half ? rotary_kerne
 template <class T, int V>
 static void (*rotary_of(bool half, int heads))(const RopeArgs) { return heads == 1 ? rotary_of<T, V, 1>(half) : rotary_of<T, V, sizeof(T) == 2 ? 4 : 2>(half); }
 
+// Whether any row of one set of rows and any of another share an address: `rows` of each, wa and wb bytes wide, lda and ldb bytes apart (at least as far as they are wide).
+static bool rows_meet(const void* a, int64_t lda, int64_t wa, const void* b, int64_t ldb, int64_t wb, int64_t rows) {
+    const int64_t d = (int64_t)((uintptr_t)b - (uintptr_t)a);
+    if (wa == 0 || wb == 0 || d >= (rows - 1) * lda + wa || -d >= (rows - 1) * ldb + wb) return false;
+    auto below = [](int64_t n, int64_t by) { return n / by - (n % by < 0); };             // the quotient, rounded down
+    if (lda == ldb) {        // slices of wider rows, as a rule: b's row i + m is d + m * ld behind a's row i, and only the two nearest can be in its reach
+        const int64_t m = -below(d, lda), r = d + m * lda;
+        return (r < wa && m < rows && -m < rows) || (r - lda > -wb && m - 1 < rows && 1 - m < rows);
+    }
+    for (int64_t i = 0; i < rows; ++i) {      // of b's rows those from the first one that ends behind a's row's beginning to the last one that begins before its end
+        const int64_t at = i * lda - d, first = below(at - wb, ldb) + 1, last = below(at + wa - 1, ldb);
+        if (max(first, (int64_t)0) <= min(last, rows - 1)) return true;
+    }
+    return false;
+}
+
 }  // namespace o1
 
 using namespace o1;
@@ -233,6 +249,14 @@ hd_status o1_rotary(const o1_rope* rope, const void* positions, int wide_positio
     const int size = type == O1_ROPE_BF16 ? 2 : 4, wide = 16 / size;
     if ((((uintptr_t)x | (uintptr_t)y | (uintptr_t)(heads2 ? x2 : nullptr) | (uintptr_t)(heads2 ? y2 : nullptr)) & (size - 1)) || ((uintptr_t)positions & (wide_positions ? 7 : 3))) {
         set_error("rotary: an address is not a multiple of its type's size");
+        return HD_ERR_UNSUPPORTED;
+    }
+    // Threads read and write in no order: a result may take the place of its own rows, and no other's.
+    auto meet = [&](const void* p, int64_t ldp, int64_t wp, const void* q, int64_t ldq, int64_t wq) { return rows_meet(p, ldp * size, wp * size, q, ldq * size, wq * size, rows); };
+    auto same = [&](const void* p, int64_t ldp, const void* q, int64_t ldq) { return p == q && (ldp == ldq || rows == 1); };
+    if ((!same(x, ldx, y, ldy) && meet(x, ldx, w, y, ldy, w)) ||
+        (heads2 && ((!same(x2, ldx2, y2, ldy2) && meet(x2, ldx2, w2, y2, ldy2, w2)) || meet(x, ldx, w, y2, ldy2, w2) || meet(x2, ldx2, w2, y, ldy, w) || meet(y, ldy, w, y2, ldy2, w2)))) {
+        set_error("rotary: results share memory with rows other than their own (which they may take the place of, row for row), or with one another");
         return HD_ERR_UNSUPPORTED;
     }
     RopeArgs a = {};

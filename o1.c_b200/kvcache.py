@@ -239,7 +239,8 @@ class Rotary:
     def __call__(self, x, positions, inverse=False, out=None):
         """Rows x [rows, heads, head_dim] bf16 or fp32 (rows of any pitch), or a pair of them (queries and keys), turned by positions [rows] int32 or int64.
 
-        inverse: turned back, which is also the gradient.  out: what to fill, like x (x itself: in place).  (A pair's results share an allocation.)"""
+        inverse: turned back, which is also the gradient.  out: what to fill, like x (x itself: in place; no other
+        memory of x's, nor one another's).  (A pair's results share an allocation.)"""
         return _binding.rotary(self._at, self._gpu, positions, inverse, x, out)
 
 

@@ -300,3 +300,72 @@ def test_sines_keep_their_bits(pkg, dev, theta, scaling, layout):
             sin[i, j], cos[i, j] = s * rope.factor, c * rope.factor
     for g, want in ((got[:, 0, first], cos), (got[:, 0, second], sin), (got[:, 1, first], -sin), (got[:, 1, second], cos)):
         assert ((g - want).abs() <= 2.0 ** -21 * want.abs()).all(), ((g - want).abs() / want.abs().clamp_min(1e-300)).max()
+
+
+# (columns of a buffer of 1024-value rows: from, heads, first row) of x, y, x2, y2, heads of 128; rows 4
+MEMORY = [(False, [(0, 2, 0), (128, 2, 0)]), (False, [(0, 2, 0), (0, 2, 1)]), (False, [(0, 2, 1), (0, 2, 0)]), (False, [(0, 2, 0), (1024 - 128, 2, 0)]), (False, [(1024 - 128, 2, 0), (0, 2, 1)]),
+          (False, [(0, 2, 0), (0, 2, 3)]), (False, [(0, 2, 0), (0, 2, 0), (128, 1, 0), (512, 1, 0)]), (False, [(0, 2, 0), (512, 2, 0), (256, 1, 0), (0, 1, 0)]),
+          (False, [(0, 2, 0), (512, 2, 0), (256, 1, 0), (640, 1, 0)]), (False, [(0, 2, 0), (0, 2, 0), (0, 2, 0), (0, 2, 0)]), (False, [(0, 2, 0), (512, 2, 0), (512, 2, 0), (0, 2, 0)]),
+          (True, [(0, 2, 0), (0, 2, 0)]), (True, [(0, 2, 0), (256, 2, 0)]), (True, [(256, 2, 0), (0, 2, 0)]), (True, [(0, 2, 0), (0, 2, 4)]), (True, [(0, 2, 4), (0, 2, 0)]),
+          (True, [(0, 2, 0), (0, 2, 0), (256, 1, 0), (256, 1, 0)]), (True, [(0, 2, 0), (256, 2, 0), (0, 2, 0), (512, 2, 0)]), (True, [(0, 2, 0), (256, 2, 2), (512, 1, 1), (640, 1, 3)]),
+          (True, [(768, 2, 0), (0, 2, 1)])]
+
+
+@pytest.mark.parametrize("case", [c for ok, c in MEMORY if not ok])
+def test_results_over_other_rows_are_refused(pkg, case):
+    at = [C.c_void_p(4096 + 2 * (row * 1024 + column)) for column, _, row in case] + [None] * (4 - len(case))
+    heads = [h for _, h, _ in case] + [0, 0]
+    r = pkg.RopeC(turns=4096, factor=1.0, head_dim=128, rot_dim=128, layout=0)
+    assert pkg.lib.o1_rotary(C.byref(r), C.c_void_p(4096), 0, at[0], 1024, at[1], 1024, heads[0], at[2], 1024, at[3], 1024, heads[2], 4, 0, 0) == 9
+    assert b"share memory" in pkg.lib.hd_cuda_last_error()
+    pkg.lib.hd_cuda_clear_error()
+
+
+def test_results_over_other_rows_of_another_pitch_are_refused(pkg):
+    """Rows 1024 apart into rows of other pitches, against every address of both."""
+    r = pkg.RopeC(turns=4096, factor=1.0, head_dim=16, rot_dim=16, layout=0)
+    refused = 0
+    for ldy in (16, 24, 40, 56, 64, 200):
+        for off in range(-200, 200, 8):
+            x = {(i * 48 + j) for i in range(4) for j in range(16)}
+            y = {(off + i * ldy + j) for i in range(4) for j in range(16)}
+            if not x & y:
+                continue           # (nothing that would be launched)
+            refused += 1
+            assert pkg.lib.o1_rotary(C.byref(r), C.c_void_p(4096), 0, C.c_void_p(8192), 48, C.c_void_p(8192 + 2 * off), ldy, 1, None, 0, None, 0, 0, 4, 0, 0) == 9, (ldy, off)
+    assert refused > 60
+    pkg.lib.hd_cuda_clear_error()
+
+
+@gpu
+@pytest.mark.parametrize("case", [c for ok, c in MEMORY if ok])
+def test_results_beside_other_rows(pkg, dev, case):
+    rope = pkg.Rotary(128, device=dev)
+    wide = torch.randn(9, 1024, generator=gen(1)).bfloat16().to(dev)
+    pos = torch.arange(4, dtype=torch.int32, device=dev) + 5
+    views = [wide[row:row + 4, column:column + h * 128].unflatten(1, (h, 128)) if column + h * 128 <= 1024 else None for column, h, row in case]
+    want = [rope(x.clone(), pos) for x in views[::2]]
+    if len(case) == 2:
+        rope(views[0], pos, out=views[1])
+    else:
+        rope((views[0], views[2]), pos, out=(views[1], views[3]))
+    for y, w in zip(views[1::2], want):
+        assert torch.equal(y, w)
+
+
+@gpu
+def test_results_between_rows_of_another_pitch(pkg, dev):
+    """Every pitch and offset that shares nothing with the rows, in one buffer."""
+    rope = pkg.Rotary(16, device=dev)
+    pos = torch.arange(4, dtype=torch.int32, device=dev) + 5
+    done = 0
+    for ldy in (16, 24, 40, 48, 56, 64, 200):
+        for off in range(-200, 200, 8):
+            if {(i * 48 + j) for i in range(4) for j in range(16)} & {(off + i * ldy + j) for i in range(4) for j in range(16)}:
+                continue
+            done += 1
+            buf = torch.randn(1200, generator=gen(done)).bfloat16().to(dev)
+            x, y = buf[200:].as_strided((4, 1, 16), (48, 16, 1), 200), buf.as_strided((4, 1, 16), (ldy, 16, 1), 200 + off)
+            want = rope(x.clone(), pos)
+            assert torch.equal(rope(x, pos, out=y), want)
+    assert done > 100
