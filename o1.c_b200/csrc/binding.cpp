@@ -2,6 +2,7 @@
 // For a few rows such a call is bound by the host: one new row of one sequence took 10.2 us through ctypes, of which the library and the launch are 3.9.
 // The entry points come as addresses from the loaded library (setup); nothing of it is linked here, and the library knows nothing of torch.
 #include <ATen/core/Tensor.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Exceptions.h>
@@ -401,7 +402,7 @@ PyObject* py_shrink(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// rotary(address of an o1_rope, device index, positions, inverse, x, y or None) -> y; x and y may be pairs
+// rotary(address of an o1_rope, device index, positions, inverse, x, y or None) -> y; x and y may be pairs.  NotImplemented: x needs a gradient
 PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     static const char* who = "Rotary";
@@ -444,6 +445,15 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor* t = tensor(y, who);
         if (!t || !rows_of(*t, heads, ldy[i])) return nullptr;
         out[i] = *t;
+    }
+    if (at::GradMode::is_enabled()) {
+        bool needed = false, filled = false;
+        for (int i = 0; i < sides; ++i) {
+            needed = needed || in[i]->requires_grad();
+            filled = filled || (out[i].defined() && out[i].requires_grad());
+        }
+        if (filled || (needed && given)) return fail(who, "out has no gradient: torch.no_grad(), or no out, where rows or out need one");
+        if (needed) return Py_NewRef(Py_NotImplemented);          // (the caller's: an autograd function around this call)
     }
     if (sides == 2 && !out[0].defined() && !out[1].defined()) {
         const int64_t size = (int64_t)c10::elementSize(type);

@@ -207,6 +207,31 @@ class KvPages:
         _binding.pages_shrink(self._at, self._gpu, keep, seqs)
 
 
+class _Turned(torch.autograd.Function):
+    """Rotary's call on rows that need a gradient, which is the results' turned back."""
+
+    @staticmethod
+    def forward(ctx, rope, positions, inverse, *x):
+        ctx.rope, ctx.inverse = rope, inverse
+        ctx.save_for_backward(positions)
+        return rope(x if len(x) > 1 else x[0], positions, inverse)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        positions, = ctx.saved_tensors
+        wanted = [i for i, needed in enumerate(ctx.needs_input_grad[3:]) if needed]
+        rows = tuple(grads[i].contiguous() for i in wanted)
+        # on the stream that autograd has for it, where the gradients are made
+        stream = _stream()
+        lib.o1_set_stream(C.c_void_p(torch.cuda.current_stream(positions.device).cuda_stream))
+        try:
+            turned = ctx.rope(rows if len(rows) > 1 else rows[0], positions, not ctx.inverse)
+        finally:
+            lib.o1_set_stream(C.c_void_p(stream))
+        back = dict(zip(wanted, turned if len(rows) > 1 else (turned,)))
+        return (None, None, None, *(back.get(i) for i in range(len(grads))))
+
+
 class Rotary:
     """Rotary positions: the first rot_dim values of each head turned in pairs, "half" (i, i + rot_dim / 2) or "interleaved" (2i, 2i + 1), by position *
     theta^(-2i / rot_dim).  Angles are exact to position * 2^-65 turns (64-bit fractions of a turn), then rounded to fp32 once reduced.
@@ -239,9 +264,10 @@ class Rotary:
     def __call__(self, x, positions, inverse=False, out=None):
         """Rows x [rows, heads, head_dim] bf16 or fp32 (rows of any pitch), or a pair of them (queries and keys), turned by positions [rows] int32 or int64.
 
-        inverse: turned back, which is also the gradient.  out: what to fill, like x (x itself: in place; no other
-        memory of x's, nor one another's).  (A pair's results share an allocation.)"""
-        return _binding.rotary(self._at, self._gpu, positions, inverse, x, out)
+        inverse: turned back.  out: what to fill, like x (x itself: in place; no other memory of x's, nor one another's).  (A pair's results share an allocation.)
+        Rows that need a gradient get results with one (not into out)."""
+        y = _binding.rotary(self._at, self._gpu, positions, inverse, x, out)
+        return _Turned.apply(self, positions, bool(inverse), *(x if isinstance(x, tuple) else (x,))) if y is NotImplemented else y
 
 
 def residual_norm(x, branch, pre_w, post_w=None, gate=None, scale=None, shift=None, alpha=1.0, eps=1e-6, y=None, h=None):

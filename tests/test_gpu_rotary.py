@@ -369,3 +369,118 @@ def test_results_between_rows_of_another_pitch(pkg, dev):
             want = rope(x.clone(), pos)
             assert torch.equal(rope(x, pos, out=y), want)
     assert done > 100
+
+
+# ------------------------------------------------------------------ gradients
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("inverse", [False, True])
+def test_rows_that_need_a_gradient(pkg, dev, dtype, layout, inverse):
+    """Results' gradients turned back, by the formula in 64 bits: of one tensor, of both of a pair, of one of a pair, of slices of wider rows, with gradients of any layout."""
+    rope = pkg.Rotary(96, 64, 10000.0, layout, {"kind": "yarn", "factor": 4.0, "original": 128.0}, dev)
+    pos = torch.arange(13, dtype=torch.int32) * 91
+    at = pos.to(dev)
+    q, k, gq, gk = (normal((13, h, 96), gen(i), dtype).to(dev) for i, h in enumerate((4, 2, 4, 2)))
+    plain = rope((q, k), at, inverse)
+    q.requires_grad_(), k.requires_grad_()
+    y = rope(q, at, inverse)
+    assert torch.equal(y, plain[0]) and y.requires_grad
+    y.backward(gq)
+    check(rope, gq, q.grad, pos, inverse=not inverse)
+    for need in ((True, True), (True, False), (False, True)):
+        x = [t.detach().clone().requires_grad_(n) for t, n in zip((q, k), need)]
+        ys = rope(tuple(x), at, inverse)
+        assert all(torch.equal(a, b) for a, b in zip(ys, plain))
+        (ys[0].float() * gq.float()).sum().add((ys[1].float() * gk.float()).sum()).backward()
+        for t, g, n in zip(x, (gq, gk), need):
+            assert (t.grad is not None) == n
+            if n:
+                check(rope, g, t.grad, pos, inverse=not inverse)
+    wide = normal((13, 6 * 96), gen(9), dtype).to(dev).requires_grad_()
+    a, b = rope((wide[:, :4 * 96].unflatten(1, (4, 96)), wide[:, 4 * 96:].unflatten(1, (2, 96))), at, inverse)
+    torch.autograd.backward((a, b), (gq.transpose(0, 1).contiguous().transpose(0, 1), gk))
+    check(rope, torch.cat([gq, gk], 1), wide.grad.unflatten(1, (6, 96)), pos, inverse=not inverse)
+    one = q.detach().clone().requires_grad_()
+    rope(one, at, inverse).sum().backward()            # (a gradient of one value for all)
+    check(rope, torch.ones_like(one), one.grad, pos, inverse=not inverse)
+    used = [t.detach().clone().requires_grad_() for t in (q, k)]
+    rope(tuple(used), at, inverse)[1].backward(gk)      # (the other one's result is not used)
+    check(rope, gk, used[1].grad, pos, inverse=not inverse)
+    assert used[0].grad is None or not used[0].grad.any()
+
+
+@gpu
+def test_a_gradient_against_differences(pkg, dev):
+    """Of a function that is not linear: sum of g * y^2 / 2, whose second derivatives are known too (the gradient of a gradient)."""
+    rope = pkg.Rotary(32, 24, 10000.0, "interleaved", device=dev)
+    at = torch.arange(7, dtype=torch.int32, device=dev) * 5
+    x, g, d = (normal((7, 2, 32), gen(i), torch.float32).to(dev) for i in (1, 2, 3))
+    x.requires_grad_()
+
+    def f(t):
+        return (g.double() * rope(t, at).double().square()).sum() / 2
+
+    grad, = torch.autograd.grad(f(x), x, create_graph=True)
+    step = 2.0 ** -4
+    with torch.no_grad():
+        along = (f(x + step * d) - f(x - step * d)) / (2 * step)
+    # quadratic: the difference is exact but for roundings, 2^-20 of some 450 terms of about 4 each, in y and in the gradient
+    assert abs(float((grad.detach().double() * d.double()).sum() - along)) < 2.0 ** -20 / step * 4 * x.numel()
+    second, = torch.autograd.grad((grad * d).sum(), x)
+    with torch.no_grad():
+        want = rope(g * rope(d, at), at, inverse=True)
+    assert (second - want).abs().max() < 2.0 ** -18 * float(want.abs().max())
+
+
+@gpu
+def test_no_gradient_where_none_is_wanted(pkg, dev):
+    rope = pkg.Rotary(64, device=dev)
+    at = torch.arange(3, dtype=torch.int32, device=dev)
+    x = normal((3, 2, 64), gen(1), torch.float32).to(dev).requires_grad_()
+    want = rope(x.detach(), at)
+    with torch.no_grad():
+        assert not rope(x, at).requires_grad and torch.equal(rope(x, at, out=torch.empty_like(want)), want)
+    with torch.inference_mode():
+        assert torch.equal(rope((x, x), at)[1], want)
+    for call in (lambda: rope(x, at, out=torch.empty_like(want)), lambda: rope(x * 1.0, at, out=x), lambda: rope(want, at, out=torch.empty_like(want).requires_grad_()),
+                 lambda: rope((want, x), at, out=(torch.empty_like(want), torch.empty_like(want)))):
+        with pytest.raises(pkg.O1Error, match="gradient"):
+            call()
+
+
+@gpu
+def test_gradients_on_streams_and_in_graphs(pkg, dev):
+    """Backward on the stream that autograd takes, wherever the library's is by then; forward and backward as one graph, replayed with other rows, gradients and positions."""
+    rope = pkg.Rotary(64, device=dev)
+    pos = torch.arange(300, dtype=torch.int32, device=dev)
+    x, g = (normal((300, 8, 64), gen(i), torch.float32).to(dev) for i in (1, 2))
+    want, s = rope(g, pos, inverse=True), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    try:
+        leaf = x.clone().requires_grad_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            pkg.use_torch_stream()
+            y = rope(leaf, pos)
+        pkg.use_torch_stream()
+        torch.cuda.synchronize()
+        back, = torch.autograd.grad(y, leaf, g)
+        torch.cuda.synchronize()
+        assert torch.equal(back, want) and pkg.lib.o1_get_stream() in (None, torch.cuda.current_stream().cuda_stream)
+        del y, leaf
+        static = x.clone().requires_grad_()
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=s):
+            pkg.use_torch_stream()
+            y = rope(static, pos)
+            back, = torch.autograd.grad(y, static, g)
+    finally:
+        pkg.use_torch_stream()
+    for i in range(3):
+        with torch.no_grad():
+            static.copy_(x * (i + 1)), g.mul_(-2.0), pos.add_(11)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, rope(static.detach(), pos)) and torch.equal(back, rope(g, pos, inverse=True))
