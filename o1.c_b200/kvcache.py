@@ -8,6 +8,7 @@ Where torch's current stream is another one, what these calls make (caches, resu
 ordering that, and their inputs, with torch's own work is the caller's.
 """
 import ctypes as C
+import math
 import os
 from collections import namedtuple
 
@@ -249,6 +250,8 @@ class Rotary:
         _need(kind in kinds, f"Rotary: scaling of kind {kind!r} (one of {', '.join(kinds)})")
         unknown = set(scaling) - {"factor", "original", "fast", "slow", "attention", "factors"}
         _need(not unknown, f"Rotary: scaling has no {', '.join(sorted(unknown))}")
+        _need(kind in ("none", "factors") or "factor" in scaling, f"Rotary: scaling of kind {kind} has a factor")
+        _need("attention" not in scaling or 0.0 < scaling["attention"] < math.inf, "Rotary: attention, what results are multiplied by, is positive and finite")
         factors = [float(f) for f in scaling.get("factors", ())]
         _need(len(factors) == (rot_dim // 2 if kind == "factors" else 0), "Rotary: factors, one for each pair, belong to scaling of that kind")
         c = RopeScalingC(kinds[kind], scaling.get("factor", 1.0), scaling.get("original", 0.0), scaling.get("fast", 32.0), scaling.get("slow", 1.0), scaling.get("attention", 0.0),

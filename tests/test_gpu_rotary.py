@@ -484,3 +484,14 @@ def test_gradients_on_streams_and_in_graphs(pkg, dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, rope(static.detach(), pos)) and torch.equal(back, rope(g, pos, inverse=True))
+
+
+@gpu
+def test_scalings_that_would_be_passed_over_are_refused(pkg, dev):
+    """A factor left out was 1, and a factor of results that is not positive was the method's own; an infinite one gave infinities."""
+    for s in ({"kind": "linear"}, {"kind": "ntk"}, {"kind": "yarn", "original": 4096.0}, *({"kind": "yarn", "factor": 4.0, "original": 4096.0, "attention": a} for a in (0.0, -1.0, math.nan, math.inf)),
+              {"kind": "none", "attention": 0}):
+        with pytest.raises(pkg.O1Error, match="Rotary"):
+            pkg.Rotary(64, scaling=s, device=dev)
+    assert pkg.Rotary(64, scaling={"kind": "none", "attention": 1.5}, device=dev).factor == 1.5
+    assert pkg.Rotary(64, scaling={"kind": "factors", "factors": [2.0] * 32}, device=dev).factor == 1.0
