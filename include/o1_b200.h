@@ -812,7 +812,7 @@ hd_status o1_kv_attention(const o1_kv_cache *cache, const void *q, int64_t ldq, 
  * o1_kv_pages_grow: counts[b] new rows for sequence seqs[b] (NULL: sequence b).  With the requests' rows behind one another, request b's from starts[b] to starts[b + 1] - 1 (starts
  * [batch + 1], at most 2^30): row r gets slots[r] (for o1_kv_write) and positions[r], its number in the sequence.  slots and positions have room for `rows`; rows behind the last
  * request get slot -1 and position 0.  lens[b]: the sequence's rows with the new ones; tables (NULL: not wanted) [batch][ldp]: its row of the table (lens and tables as
- * o1_kv_attention takes them).  Requests are served in order: new pages come from the top of the stack.
+ * o1_kv_attention takes them).  Results share no memory with one another, the requests or the pages.  Requests are served in order: new pages come from the top of the stack.
  * o1_kv_pages_shrink: sequence seqs[b] keeps its first keep[b] rows (0: it is closed); pages behind them are free again and come back in the order in which they went.
  * A request that cannot be served changes nothing of its sequence, its rows get slot -1 and its lens[b] is 0; others are as without it, but for the places of their rows.
  * o1_device_error() then gives 70 (no such sequence, or one that the call names twice: neither request is served), 71 (a negative count, more rows than width pages

@@ -301,6 +301,19 @@ hd_status o1_kv_pages_grow(const o1_kv_pages* pages, const int32_t* seqs, const 
     if (batch < 0 || batch > a.max_seqs || rows < 0 || rows > PG_FULL) { set_error("kv_pages_grow: batch %d (at most max_seqs %d), rows %d (at most 2^30)", batch, a.max_seqs, rows); return HD_ERR_UNSUPPORTED; }
     if ((batch > 0 && (!counts || !lens)) || !starts || (rows > 0 && (!slots || !positions))) { set_error("kv_pages_grow: null argument"); return HD_ERR_MISSING; }
     if (tables && ldp < a.width) { set_error("kv_pages_grow: a row pitch is below the row"); return HD_ERR_UNSUPPORTED; }
+    // Blocks read requests and state while others write results.
+    struct Range { const void* at; int64_t bytes; };
+    const int64_t n = batch, max_seqs = a.max_seqs;
+    const Range ranges[] = {{slots, rows * 8ll}, {positions, rows * 4ll}, {starts, (n + 1) * 4}, {lens, n * 4}, {tables, n > 0 && tables ? ((n - 1) * ldp + a.width) * 4 : 0},
+                            {counts, n * 4}, {seqs, seqs ? n * 4 : 0}, {a.table, max_seqs * a.width * 4}, {a.lens, max_seqs * 4}, {a.free_pages, a.pages * 4ll}, {a.state, 8}};
+    for (int i = 0; i < 5; ++i) {
+        for (int j = i + 1; j < 11; ++j) {
+            const Range &r = ranges[i], &q = ranges[j];
+            if (r.bytes == 0 || q.bytes == 0 || (uintptr_t)r.at + r.bytes <= (uintptr_t)q.at || (uintptr_t)q.at + q.bytes <= (uintptr_t)r.at) continue;
+            set_error("kv_pages_grow: a result shares memory with another one, the requests or the pages themselves");
+            return HD_ERR_UNSUPPORTED;
+        }
+    }
     a.seqs = seqs; a.asked = counts; a.batch = batch; a.rows = rows;
     a.slots = slots; a.positions = positions; a.starts = starts; a.lens_out = lens; a.tables_out = tables; a.ldp = ldp;
     st = launch_pages<true>(a, "kv_pages_grow");

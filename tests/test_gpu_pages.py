@@ -406,3 +406,36 @@ def test_a_server(pkg, dev, kind, layout, page, captured):
         torch.cuda.synchronize()
         check_step(which, q, k, out)
     assert pkg.lib.o1_device_error() == 0
+
+
+def test_results_over_what_is_read_are_refused(pkg):
+    """Results that share a byte with one another, with the requests or with the pages' own arrays: other blocks still read those.  (All of these are refused before anything is launched.)"""
+    base = dict(table=0x100000, lens=0x200000, free_pages=0x300000, state=0x400000)
+    k = pkg.KvPagesC(**base, pages=50, page_size=16, max_seqs=8, width=5)
+    good = dict(seqs=0x500000, counts=0x600000, slots=0x700000, positions=0x800000, starts=0x900000, lens=0xA00000, tables=0xB00000)
+    size = dict(seqs=5 * 4, counts=5 * 4, slots=11 * 8, positions=11 * 4, starts=6 * 4, lens=5 * 4, tables=(4 * 7 + 5) * 4)
+    own = dict(table=8 * 5 * 4, lens=8 * 4, free_pages=50 * 4, state=8)
+    for name in ("slots", "positions", "starts", "lens", "tables"):
+        others = [(good[o], size[o]) for o in good if o != name] + [(base[o], own[o]) for o in own]
+        for at, n in others:
+            for where in (at, at + n - 4, at - size[name] + 4):
+                p = {o: C.c_void_p(v) for o, v in {**good, name: where}.items()}
+                assert pkg.lib.o1_kv_pages_grow(C.byref(k), p["seqs"], p["counts"], 5, p["slots"], p["positions"], 11, p["starts"], p["lens"], p["tables"], 7) == 9, (name, hex(where))
+                assert b"shares memory" in pkg.lib.hd_cuda_last_error()
+    pkg.lib.hd_cuda_clear_error()
+
+
+@gpu
+def test_results_right_behind_one_another(pkg, dev):
+    """One buffer for all results and the requests, not a byte between them."""
+    p, m = pkg.KvPages(60, 16, 6, 9, dev), Model(60, 16, 6, 9)
+    counts, names, rows = [70, 1, 0, 33], [4, 0, 2, 5], 104
+    want = m.grow(counts, rows, names)
+    sizes = [rows * 2, rows, 5, 4, 4 * 9, 4, 4]
+    buf = torch.full((sum(sizes),), 77, dtype=torch.int32, device=dev)
+    slots, positions, starts, lens, tables, c, n = buf.split(sizes)
+    c.copy_(ints(counts, dev)), n.copy_(ints(names, dev))
+    pkg.check(pkg.lib.o1_kv_pages_grow(C.byref(p.c), pkg.ptr(n), pkg.ptr(c), 4, pkg.ptr(slots), pkg.ptr(positions), rows, pkg.ptr(starts), pkg.ptr(lens), pkg.ptr(tables), 9), "grow")
+    check(pkg.kvcache.Grown(slots.view(torch.int64), positions, starts, lens, tables.view(4, 9)), want[:5])
+    assert c.tolist() == counts and n.tolist() == names
+    m.same(p)
