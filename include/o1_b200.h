@@ -795,7 +795,7 @@ hd_status o1_kv_read(const o1_kv_cache *cache, void *k, int64_t ldk, void *v, in
  * o1_kv_attention_workspace_bytes_of(cache->type, heads, kv_heads), which is more with O1_KV_UINT4 and makes calls of many sequences faster there; 16-byte aligned, its first
  * O1_KV_ATTENTION_COUNTERS bytes zero-filled once before its first use and all of it left to these calls from then on; calls that may overlap on the GPU each need their own.  The result is the same
  * bits from call to call with the same lengths, width and (O1_KV_UINT4) room in the workspace; beside other sequences a sequence's differs by the order of its fp32 sums.  Values of v up to 2^90 in magnitude (the sums are 2^20 times larger and in fp32);
- * with O1_KV_UINT4 scale at most 2^114 and scale times the largest |q| of a head at most 2^121; at most 2^31 - 1 rows (pages *
+ * with O1_KV_UINT4 scale at most 2^114 and scale times the largest |q| of a head at most 2^121, with the other kinds scores (scale * q . k) up to 2^29 in magnitude; at most 2^31 - 1 rows (pages *
  * kv_heads * page_size) in the cache. */
 #define O1_KV_ATTENTION_COUNTERS 32768
 int64_t o1_kv_attention_workspace_bytes(int heads, int kv_heads);

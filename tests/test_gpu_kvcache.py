@@ -831,3 +831,25 @@ def test_memory_of_another_gpu_among_two_is_refused(pkg, dev):
                 call()
     finally:
         torch.cuda.set_device(dev)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "int8"])
+@pytest.mark.parametrize("lens,kv_heads,group", [([300], 2, 4), ([300], 1, 16), ([100] * 70, 8, 2)])
+def test_scores_up_to_the_limit(pkg, dev, kind, lens, kv_heads, group):
+    """Scores of up to 2^29: the largest one's row is the result where it is ahead by more than four times a score's error, 2^-19 of its terms' magnitudes.  (A probability has no place for a rounding of
+    its maximum by more than 2^7, which is 2^31 of them.)"""
+    c = Case(pkg, dev, kind, lens, kv_heads, 32, seed=11)
+    c.fill()
+    q = normal((len(lens), kv_heads * group, D), gen(3), 2.0 ** 26)
+    k, v = (value(*quantised(x[0], kind)).repeat_interleave(group, 1) for x in (c.k, c.v))
+    z = torch.einsum("hd,thd->ht", q[0].double(), k) * D ** -0.5
+    size = (torch.einsum("hd,thd->ht", q[0].double().abs(), k.abs()) * D ** -0.5).amax(-1)
+    assert 2.0 ** 27 < float(z.abs().max()) < 2.0 ** 29
+    out, lse = c.cache.attend(q.to(dev), c.dtable, c.dlens, lse=True)
+    c.check(q, out, lse, what=kind)
+    top = z.topk(2).values
+    sure = top[:, 0] - top[:, 1] > 4 * 2.0 ** -19 * size
+    assert sure.sum() > len(sure) // 2
+    rows, heads = z.argmax(-1)[sure], torch.arange(len(sure))[sure]
+    between(out[0, heads], v[rows, heads], v[rows, heads].abs() * 2.0 ** -12, kind)
