@@ -380,10 +380,11 @@ kv_read_kernel(KvView c, int type, uint16_t* __restrict__ k, int64_t ldk, uint16
 //  * Rounding: scores and sums in fp32.  Probabilities (times v's scale) enter the second product as two parts of bf16, value and rest, 16 bits of significand; codes
 //    of a byte are exact in f16 and bf16.  Keys' codes go through f16, which takes fewer instructions, with queries scaled to f16's top by a power of two for each head (those
 //    below 2^-29 of its largest lose bits); values' codes through bf16, whose range a probability needs.  The result is rounded once.
-//  * Rows of four bits (KvFour) are 64 to a chunk and the chunks, for the same bytes, twice the arithmetic: instructions bound them, not memory.  302 MB (96 sequences of 300 to 5400
-//    rows, 8 kv heads, 32 heads) in 63.4 us, 4.75 TB/s, 73 % of a copy's rate; 109 MB (one of 100003) in 30.6; 39.7 MB (37 of 0 to 1999, 16 heads) in 20.2.  A chunk is some 980
-//    instructions (all of a launch's counted), of which an SM issues 2.2 a clock; half of the ALU pipe's time is the codes' masks and shifts.  As the other kinds have it (queries
-//    as rows, codes to pairs of keys by byte permutes) it was 1420 and 99 us.
+//  * Rows of four bits (KvFour) are 64 to a chunk and the chunks, for the same bytes, twice the arithmetic.  302 MB (96 sequences of 300 to 5400 rows, 8 kv heads, 32 heads) in 61.4 us,
+//    4.9 TB/s, 75 % of a copy's rate; 109 MB (one of 100003) in 30.7; 39.7 MB (37 of 0 to 1999, 16 heads) in 20.8.  A chunk is some 1000 instructions (all of a launch's counted) in chains
+//    that depend on one another, and those bound it, with 15 warps on an SM at 128 registers (parts of warps: 28 bytes of them spilled): neither memory nor any pipe is at its limit, 2.2
+//    instructions a clock and SM (1.9 for one sequence), the ALU pipe busy 54 %, half of that the codes' masks and shifts, the tensor pipe 28 %.  As the other kinds have it
+//    (queries as rows, codes to pairs of keys by byte permutes) it was 1420 instructions and 99 us.
 // Times below: "batch" 24 sequences of 1 to 2100 rows of bf16, "shared" 32 sequences of 1000 to 3000, 16 query heads on one kv head; us.
 static constexpr int KV_STAGE_BYTES = 8192;            // keys and values of a chunk
 static constexpr int KV_SEQS = 256;                    // sequences of a launch
@@ -1666,9 +1667,11 @@ static cudaError_t launch_attention(const CUtensorMap& k_map, const CUtensorMap&
 template <int TYPE, int HG>
 static cudaError_t launch_attention(const CUtensorMap& k_map, const CUtensorMap& v_map, const KvAttn& a, int64_t item_chunks, int64_t items, cudaStream_t st, bool warps = true) {
     const int most = min(sm_count(), KV_TEAMS_MAX / KvKernel<TYPE, HG>::TEAMS), teams = most * KvKernel<TYPE, HG>::TEAMS;
-    // Four bits: parts to warps (where the workspace has room for them), which need no barriers but leave more of an item to be joined at the end, where there is much work for each and items are not few, or items are
-    // short and many.  us, to warps and to teams (444 of them): 8 kv heads, 96 sequences of 300 to 5400 rows 62.9 and 65.9, 37 of up to 1999 19.5 and 20.9, 128 of up to 1000
+    // Four bits: parts to warps (where the workspace has room for them), which need no barriers but leave more of an item to be joined at the end, where there is much work for each and
+    // items are not few, or items are short and many.  us, to warps and to teams (444 of them): 8 kv heads, 96 sequences of 300 to 5400 rows 62.9 and 65.9, 37 of up to 1999 19.5 and 20.9, 128 of up to 1000
     // 27.3 and 33.7, 64 of 100 9.4 and 13.5, 128 of 60 8.3 and 19.5; but one of 100003 34.6 and 31.5, 16 of 2000 19.6 and 18.2, 32 of 200 13.2 and 9.3, 60 of up to 400 20.2 and 17.0.
+    // (These had tables as wide as their longest sequence.  The rule sees the table, not the lengths: with room for 4096 or 16384 rows, 32 of 200 go to warps and take 13.5 us instead of
+    // 8.4, 60 of up to 400 16.1 instead of 13.9; 37 of up to 1999, 128 of up to 1000 and 96 of up to 5400 take what they take under a tight table.)
     if (TYPE == KV_UINT4) {
         const bool much = 2 * items > teams && item_chunks * items > 16 * teams, many = items > teams && item_chunks * teams <= KV_TEAM * items;
         if ((much || many) && warps) return launch_attention<TYPE, HG, true>(k_map, v_map, a, most, st);
